@@ -272,6 +272,51 @@ int lowbit_greedy_start_cuda(const void* d_logits, int dtype, int64_t row_stride
                              int64_t* d_suppress_ids, int length, int suppress_below, int n_suppress,
                              const int64_t* suppress_ids, void* stream);
 
+/* ---- A paged key/value cache: many requests that come and go.  The reference's serving engine keeps such a cache; its XPU kernels are
+ * closed.  A cache is [n_pages][page_size][Hkv][D], D contiguous, strides {page, row, head} in elements (host arrays): fp16 or bf16 as the
+ * activations, or one e5m2 byte per element as in the cache above (cache_dtype B200_QT_FP8_E5M2).  Row r of the block table
+ * (int32 [R][width]) names the pages of request r in the order of its tokens, -1 where it has none; a slot is page * page_size + row.
+ * Packed tokens: those of request r are rows cu_seqlens[r] .. cu_seqlens[r + 1] - 1 (int32 [R + 1] on the device).
+ *
+ * lowbit_paged_step_cuda: what a step needs, from d_held (tokens that each request holds) and d_new (tokens that it brings).  Pages that the
+ * new tokens need beyond ceil(held / page_size) come off the top of the stack d_free_pages[0 .. *d_free_count) and are entered into the
+ * table; *d_free_left (may be d_free_count) = pages left.  d_cu_seqlens [R + 1], d_seq_lens [R] = held + new, and for each of n_tokens
+ * rows d_positions and d_slots (int64): the position and the slot, 0 and -1 behind the last token.  Where the stack or the table's
+ * width runs out, entries and slots are -1 and *d_missing counts the pages that were not to be had; later requests go without first.
+ * lowbit_paged_release_cuda: rows with d_done[r] != 0 give back every page of their row (in its order) and become -1. */
+int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_held, int R, int32_t* d_table, int64_t table_stride, int width,
+                           const int32_t* d_free_pages, int n_pages, const int32_t* d_free_count, int32_t* d_free_left, int page_size,
+                           int64_t n_tokens, int32_t* d_cu_seqlens, int32_t* d_seq_lens, int64_t* d_positions, int64_t* d_slots,
+                           int32_t* d_missing, void* stream);
+int lowbit_paged_release_cuda(const uint8_t* d_done, int R, int32_t* d_table, int64_t table_stride, int width, int32_t* d_free_pages,
+                              int n_pages, int32_t* d_free_count, void* stream);
+/* Rotary embedding (rotate_half pairing over the first rotary_dim elements of a head, tables [n_positions][>= rotary_dim / 2] indexed by
+ * position; rotary_dim 0: none, tables and positions NULL) of the q and k heads of the merged projection's output d_qkv
+ * [T][(Hq + 2 Hkv) * D], in place, and the write of keys and values into their slots; a slot outside the cache is not written.
+ * fp32 arithmetic, one rounding to the activations' type; e5m2 keeps those, rounded to nearest even, saturating. */
+int lowbit_paged_rope_append_cuda(void* d_qkv, int dtype, int64_t token_stride, int64_t T, int Hq, int Hkv, int D, int rotary_dim,
+                                  const void* d_cos, const void* d_sin, int cs_dtype, int64_t cs_row_stride, int64_t n_positions,
+                                  const int64_t* d_positions, const int64_t* d_slots, void* d_k_cache, const int64_t* k_strides,
+                                  void* d_v_cache, const int64_t* v_strides, int cache_dtype, int n_pages, int page_size, void* stream);
+/* Attention of every request's new tokens (one, or a chunk of its prompt; already in the cache) over its pages: token i of n sees keys
+ * 0 .. seq_len - n + i; one that sees none gives zeros, rows of d_out behind the last request stay as they are.  q, out [T][Hq][D],
+ * strides {token, head}; fp16 / bf16, D a multiple of 16 up to 256, Hq a multiple of Hkv; pointers and strides 16-byte aligned.  A key
+ * in a page outside the cache makes its request's rows NaN.  max_query: no request brings more new tokens than that (T is always
+ * right).  Softmax and sums in fp32.  workspace: lowbit_sdp_paged_workspace_size() bytes, one per call in flight, not initialised. */
+size_t lowbit_sdp_paged_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_query);
+int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t* q_strides, int64_t T, const void* d_k, const int64_t* k_strides,
+                          const void* d_v, const int64_t* v_strides, int cache_dtype, int n_pages, int page_size, const int32_t* d_table,
+                          int64_t table_stride, int width, const int32_t* d_seq_lens, const int32_t* d_cu_seqlens, int R, int Hq, int Hkv,
+                          int D, float scale, int64_t max_query, void* d_out, const int64_t* out_strides, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* Attention of whole prompts that lie behind one another (no cache): q, out [T][Hq][D], k, v [T][Hkv][D], strides {token, head}; causal
+ * within each prompt, or without (causal 0).  max_seqlen: no prompt is longer (T is always right).  Otherwise as above. */
+size_t lowbit_sdp_packed_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_seqlen);
+int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t* q_strides, int64_t T, const void* d_k, const int64_t* k_strides,
+                           const void* d_v, const int64_t* v_strides, const int32_t* d_cu_seqlens, int R, int Hq, int Hkv, int D, float scale,
+                           int causal, int64_t max_seqlen, void* d_out, const int64_t* out_strides, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 /* canonical <-> device layout on device buffers (same byte size, src != dst).
  * to_device != 0: canonical -> tiled ; 0: tiled -> canonical. */
 int lowbit_relayout_cuda(const void* d_src, void* d_dst, int64_t rows, int64_t k, int qtype,

@@ -657,3 +657,84 @@ def lowbit_sdp_fp8_prefill(q, k, v, mask, causal, scale, out, stream):
                                                     _strides3(mask) if mask is not None else None, int(bool(causal)), float(scale),
                                                     B, Hq, Hkv, S, L, D, out.data_ptr(), _DT_OF[out.dtype], _strides3(out), stream),
            "lowbit_sdp_fp8_prefill_cuda")
+
+
+# ---------------------------------------------------------------- the paged key/value cache
+QT_FP8_E5M2 = 19
+_lib.lowbit_paged_step_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                        ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64] + [ctypes.c_void_p] * 6
+_lib.lowbit_paged_step_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_release_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+                                           ctypes.c_void_p, ctypes.c_void_p]
+_lib.lowbit_paged_release_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_rope_append_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4 + \
+    [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _I64P,
+     ctypes.c_void_p, _I64P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+_lib.lowbit_paged_rope_append_cuda.restype = ctypes.c_int
+_lib.lowbit_sdp_paged_workspace_size.argtypes = [ctypes.c_int64] + [ctypes.c_int] * 4 + [ctypes.c_int64]
+_lib.lowbit_sdp_paged_workspace_size.restype = ctypes.c_size_t
+_lib.lowbit_sdp_paged_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, _I64P, ctypes.c_int64, ctypes.c_void_p, _I64P, ctypes.c_void_p, _I64P, ctypes.c_int,
+                                       ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p] + \
+    [ctypes.c_int] * 4 + [ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, _I64P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+_lib.lowbit_sdp_paged_cuda.restype = ctypes.c_int
+_lib.lowbit_sdp_packed_workspace_size.argtypes = _lib.lowbit_sdp_paged_workspace_size.argtypes
+_lib.lowbit_sdp_packed_workspace_size.restype = ctypes.c_size_t
+_lib.lowbit_sdp_packed_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, _I64P, ctypes.c_int64, ctypes.c_void_p, _I64P, ctypes.c_void_p, _I64P, ctypes.c_void_p] + \
+    [ctypes.c_int] * 4 + [ctypes.c_float, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, _I64P, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+_lib.lowbit_sdp_packed_cuda.restype = ctypes.c_int
+
+
+def _strides(t, n):
+    return (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def lowbit_paged_step(new, held, table, free_pages, free_count, free_left, page_size, cu_seqlens, seq_lens, positions, slots, missing, stream):
+    _check(_lib.lowbit_paged_step_cuda(new.data_ptr(), held.data_ptr(), new.shape[0], table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
+                                       free_pages.shape[0], free_count.data_ptr(), free_left.data_ptr(), int(page_size), positions.shape[0],
+                                       cu_seqlens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), missing.data_ptr(), stream),
+           "lowbit_paged_step_cuda")
+
+
+def lowbit_paged_release(done, table, free_pages, free_count, stream):
+    _check(_lib.lowbit_paged_release_cuda(done.data_ptr(), table.shape[0], table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
+                                          free_pages.shape[0], free_count.data_ptr(), stream), "lowbit_paged_release_cuda")
+
+
+def _cache_dtype(cache):
+    return QT_FP8_E5M2 if cache.element_size() == 1 else _DT_OF[cache.dtype]
+
+
+def lowbit_paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary_dim, cos, sin, positions, slots, k_cache, v_cache, stream):
+    """qkv [T, (Hq + 2 Hkv) * D]; cos / sin [positions, rotary_dim] or None; caches [pages, page_size, Hkv, D]"""
+    _check(_lib.lowbit_paged_rope_append_cuda(qkv.data_ptr(), _DT_OF[qkv.dtype], qkv.stride(0), qkv.shape[0], n_heads, n_kv_heads, head_dim, rotary_dim,
+                                              cos.data_ptr() if rotary_dim else None, sin.data_ptr() if rotary_dim else None,
+                                              _DT_OF[cos.dtype] if rotary_dim else 0, cos.stride(0) if rotary_dim else 0, cos.shape[0] if rotary_dim else 0,
+                                              positions.data_ptr() if rotary_dim else None, slots.data_ptr(), k_cache.data_ptr(), _strides(k_cache, 3),
+                                              v_cache.data_ptr(), _strides(v_cache, 3), _cache_dtype(k_cache), k_cache.shape[0], k_cache.shape[1], stream),
+           "lowbit_paged_rope_append_cuda")
+
+
+def lowbit_sdp_paged_workspace_size(t, r, hq, hkv, d, max_query):
+    return _lib.lowbit_sdp_paged_workspace_size(t, r, hq, hkv, d, max_query)
+
+
+def lowbit_sdp_paged(q, k_cache, v_cache, table, seq_lens, cu_seqlens, scale, max_query, out, workspace, stream):
+    """q, out [T, Hq, D]; caches [pages, page_size, Hkv, D]"""
+    T, Hq, D = q.shape
+    _check(_lib.lowbit_sdp_paged_cuda(q.data_ptr(), _DT_OF[q.dtype], _strides(q, 2), T, k_cache.data_ptr(), _strides(k_cache, 3), v_cache.data_ptr(),
+                                      _strides(v_cache, 3), _cache_dtype(k_cache), k_cache.shape[0], k_cache.shape[1], table.data_ptr(), table.stride(0),
+                                      table.shape[1], seq_lens.data_ptr(), cu_seqlens.data_ptr(), table.shape[0], Hq, k_cache.shape[2], D, float(scale),
+                                      int(max_query), out.data_ptr(), _strides(out, 2), workspace.data_ptr(), workspace.numel(), stream),
+           "lowbit_sdp_paged_cuda")
+
+
+def lowbit_sdp_packed_workspace_size(t, r, hq, hkv, d, max_seqlen):
+    return _lib.lowbit_sdp_packed_workspace_size(t, r, hq, hkv, d, max_seqlen)
+
+
+def lowbit_sdp_packed(q, k, v, cu_seqlens, scale, causal, max_seqlen, out, workspace, stream):
+    """q, out [T, Hq, D]; k, v [T, Hkv, D]"""
+    T, Hq, D = q.shape
+    _check(_lib.lowbit_sdp_packed_cuda(q.data_ptr(), _DT_OF[q.dtype], _strides(q, 2), T, k.data_ptr(), _strides(k, 2), v.data_ptr(), _strides(v, 2),
+                                       cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, float(scale), int(bool(causal)), int(max_seqlen),
+                                       out.data_ptr(), _strides(out, 2), workspace.data_ptr(), workspace.numel(), stream), "lowbit_sdp_packed_cuda")

@@ -1,0 +1,639 @@
+"""The paged key/value cache (transformers/paged_kv.py): bookkeeping against whole numbers computed here, the cache write and the two
+attentions against 64-bit statements.
+
+Bounds.  A rounding is off by half a step, h(t) = finfo(t).eps / 2 of the value.  An attention's output is rounded once, h(out) |o|; its
+probabilities may be rounded to the type t of the values in the product (the activations', fp16 over e5m2), each h(t) of itself, which moves
+the output by up to h(t) (a + |o|) with a = sum p |v| / sum p.  The sums: a score's D products drop up to 2^-23 of their absolute sum in
+each of D / 8 steps, and that much of its probability; exp2 2^-22; the products with the values up to 2^-23 of a in each of L / 8 steps."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def paged(native_lib):
+    from ipex_llm_b200.transformers import paged_kv
+    yield paged_kv
+    if torch.cuda.is_available():
+        assert not native_lib.lowbit_gemm_wait_expired()
+
+
+# ------------------------------------------------------------------ pages, slots, positions
+def step_statement(new, held, table, stack, page, n_tokens):
+    """the same in whole numbers: (table, cu, seq_lens, positions, slots, left, missing); the table's rows as lists"""
+    table, stack, missing = [list(row) for row in table], list(stack), 0
+    cu, lens, positions, slots = [0], [], [], []
+    for r, (n, h) in enumerate(zip(new, held)):
+        for c in range(-(-h // page), -(-(h + n) // page)):
+            if c >= len(table[r]):
+                missing += 1
+            elif stack:
+                table[r][c] = stack.pop()
+            else:
+                table[r][c] = -1
+                missing += 1
+        for p in range(h, h + n):
+            c = p // page
+            pg = table[r][c] if c < len(table[r]) else -1
+            positions.append(p)
+            slots.append(pg * page + p % page if pg >= 0 else -1)
+        cu.append(cu[-1] + n)
+        lens.append(h + n)
+    pad = n_tokens - len(slots)
+    return table, cu, lens, (positions + [0] * pad)[:n_tokens], (slots + [-1] * pad)[:n_tokens], len(stack), missing
+
+
+def start(held, page, width, pages, g, spare=None):
+    """a table that holds what the requests hold, and the stack of free pages (``spare`` of them)"""
+    order = torch.randperm(pages, generator=g).tolist()
+    table = []
+    for h in held:
+        row = [order.pop() for _ in range(min(-(-h // page), width))]
+        table.append(row + [-1] * (width - len(row)))
+    return table, order if spare is None else order[:spare]
+
+
+STEPS = [([1], [0], 16, 4), ([1], [15], 16, 4), ([1], [16], 16, 4), ([1, 1, 1], [0, 31, 32], 16, 8), ([0, 5, 0, 40, 1], [3, 0, 0, 7, 64], 8, 16),
+         ([100, 1, 300], [0, 0, 1], 1, 400), ([33, 17], [20, 6], 7, 20), ([0, 0], [9, 0], 4, 4), ([700], [3], 128, 9)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad", [0, 3, 200])
+@pytest.mark.parametrize("new,held,page,width", STEPS)
+def test_step(paged, cuda_device, new, held, page, width, pad):
+    check_step(paged, cuda_device, new, held, page, width, sum(new) + pad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,page", [(31, 16), (33, 64), (1000, 16), (1024, 8), (1025, 32), (2500, 16)])
+def test_step_of_many_requests(paged, cuda_device, R, page):
+    g = torch.Generator().manual_seed(R)
+    held = torch.randint(0, 500, (R,), generator=g).tolist()
+    new = [n if i % 5 == 0 else 1 for i, n in enumerate(torch.randint(0, 90, (R,), generator=g).tolist())]
+    check_step(paged, cuda_device, new, held, page, -(-600 // page), sum(new) + 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spare", [0, 1, 3])
+@pytest.mark.parametrize("new,held,page,width", [([40, 5, 20], [0, 3, 1], 8, 8), ([1, 1, 1, 1], [8, 16, 7, 24], 8, 8), ([30, 90], [2, 1], 8, 4)])
+def test_step_without_enough_pages(paged, cuda_device, new, held, page, width, spare):
+    """earlier requests are served first; what is left gets -1, and the count of it; the same where the table is too narrow"""
+    check_step(paged, cuda_device, new, held, page, width, sum(new), spare)
+
+
+def check_step(paged, dev, new, held, page, width, n_tokens, spare=None):
+    g = torch.Generator().manual_seed(sum(new) + page)
+    pages = sum(-(-h // page) for h in held) + sum(-(-n // page) + 1 for n in new) + 2
+    table, stack = start(held, page, width, pages, g, spare)
+    want = step_statement(new, held, table, stack, page, n_tokens)
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)                                 # noqa: E731
+    wide = torch.full((len(new), width + 3), 77, dtype=torch.int32, device=dev)                   # rows of a wider table
+    wide[:, :width] = on(table)
+    free = torch.full((pages,), -5, dtype=torch.int32, device=dev)
+    free[:len(stack)] = on(stack)
+    count = on([len(stack)])
+    for in_place in (False, True):
+        t = wide.clone()
+        st = paged.paged_step(on(new), on(held), t[:, :width], free, count, page, n_tokens, free_left=count if in_place else None)
+        assert t[:, :width].tolist() == want[0] and bool((t[:, width:] == 77).all())
+        assert (st.cu_seqlens.tolist(), st.seq_lens.tolist(), st.positions.tolist(), st.slots.tolist()) == want[1:5]
+        assert (st.free_count.item(), st.missing.item()) == want[5:]
+        assert count.item() == (want[5] if in_place else len(stack))
+
+
+@pytest.mark.gpu
+def test_fewer_rows_than_tokens(paged, cuda_device):
+    """rows of the step beyond those asked for are not written anywhere"""
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)                         # noqa: E731
+    st = paged.paged_step(on([3, 9]), on([0, 0]), torch.full((2, 4), -1, dtype=torch.int32, device=cuda_device), on([4, 5, 6, 7]), on([4]), 4, 5)
+    assert st.positions.tolist() == [0, 1, 2, 0, 1] and st.slots.tolist() == [28, 29, 30, 24, 25] and st.cu_seqlens.tolist() == [0, 3, 12]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [1, 5, 40, 1500])
+def test_release_returns_every_page_once(paged, cuda_device, width):
+    g = torch.Generator().manual_seed(width)
+    R, pages = 9, 9 * width + 4
+    held = torch.randint(0, width * 4 + 1, (R,), generator=g).tolist()
+    table, stack = start(held, 4, width, pages, g)
+    done = [True, False, True, True, False, False, True, False, True]
+    free = torch.full((pages,), -5, dtype=torch.int32, device=cuda_device)
+    free[:len(stack)] = torch.tensor(stack, dtype=torch.int32, device=cuda_device)
+    count = torch.tensor([len(stack)], dtype=torch.int32, device=cuda_device)
+    t = torch.tensor(table, dtype=torch.int32, device=cuda_device)
+    for _ in range(2):                                                                            # the second time there is nothing to return
+        paged.paged_release(torch.tensor(done, device=cuda_device), t, free, count)
+        want = stack + [p for row, d in zip(table, done) if d for p in row if p >= 0]
+        assert count.item() == len(want) and free[:len(want)].tolist() == want and bool((free[len(want):] == -5).all())
+        assert t.tolist() == [[-1] * width if d else row for row, d in zip(table, done)]
+
+
+# ------------------------------------------------------------------ the write into the cache
+def rotated(x, cos, sin):
+    """64 bits: x [T, H, D], tables [T, rotary width]"""
+    R = cos.shape[-1]
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    a = x[..., :R]
+    return torch.cat([a * c + torch.cat([-a[..., R // 2:], a[..., :R // 2]], -1) * s, x[..., R:]], -1)
+
+
+def tables(dim, n, dev, dtype=torch.float32):
+    a = torch.arange(n, device=dev, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, dim, 2, device=dev, dtype=torch.float64) / dim)
+    return torch.cat([a.cos()] * 2, -1).to(dtype), torch.cat([a.sin()] * 2, -1).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("eight", [True, False])
+@pytest.mark.parametrize("T,heads,kv_heads,dim,rotary,table_type", [(1, 32, 32, 128, 128, "f32"), (7, 4, 2, 64, 64, "same"), (300, 14, 2, 96, 32, "f32"), (33, 8, 1, 256, 256, "same"),
+                                                                    (65, 3, 3, 80, 80, "f32"), (20, 2, 1, 48, 6, "same"), (40, 0, 2, 64, 64, "f32"), (130, 8, 4, 128, 0, "f32")])
+def test_append(paged, cuda_device, dtype, eight, T, heads, kv_heads, dim, rotary, table_type):
+    g = torch.Generator(device=cuda_device).manual_seed(T)
+    page, width = 8, (heads + 2 * kv_heads) * dim
+    pages = T // page + 3
+    whole = torch.randn(T, width + 16, generator=g, device=cuda_device).to(dtype)                 # rows with something between them
+    qkv = whole[:, :width]
+    qkv[0, -1] = 60000.0                                                                          # saturates in e5m2 (57344)
+    before = whole.clone()
+    # the layout of a cache whose heads come before its rows
+    caches = [torch.randn(pages, kv_heads, page, dim, generator=g, device=cuda_device).to(dtype).transpose(1, 2) for _ in range(2)]
+    if eight:
+        caches = [c.to(torch.float8_e5m2).view(torch.uint8) for c in caches]
+    held = [c.clone() for c in caches]
+    slots = torch.randperm(pages * page, generator=g, device=cuda_device)[:T]
+    slots[T // 2] = -1 if T > 1 else slots[0]
+    if T > 30:
+        slots[5] = pages * page                                                                   # no slot of the cache
+    positions = torch.randint(0, 500, (T,), generator=g, device=cuda_device)
+    positions[-1] = 10 ** 10                                                                      # beyond the tables: the last row
+    cos, sin = tables(max(rotary, 2), 500, cuda_device, torch.float32 if table_type == "f32" else dtype)
+    paged.paged_rope_append(qkv, heads, kv_heads, dim, *((cos, sin) if rotary else (None, None)), positions if rotary else None, slots, *caches)
+    x = before[:, :width].double().view(T, heads + 2 * kv_heads, dim)
+    n = heads + kv_heads
+    if rotary:
+        at = positions.clamp(max=499)
+        want = rotated(x[:, :n], cos[at], sin[at])
+        # two products, one sum, one rounding
+        scale = rotated(x[:, :n].abs(), cos[at].abs(), -sin[at].abs())
+        got = qkv.double().view(T, -1, dim)[:, :n]
+        assert bool(((got - want).abs() <= HALF[dtype] * want.abs() + 2.0 ** -22 * (scale.abs() + want.abs() + x[:, :n].abs().amax()) + 1e-7).all())
+    else:
+        assert torch.equal(qkv, before[:, :width])
+    assert torch.equal(whole[:, width:], before[:, width:])
+    assert torch.equal(qkv[:, n * dim:], before[:, n * dim:width])                                # the values stay
+    now = qkv.reshape(T, -1, dim)
+    for cache, old, rows in zip(caches, held, (now[:, heads:n], now[:, n:])):
+        flat, was = cache.reshape(pages * page, kv_heads, dim), old.reshape(pages * page, kv_heads, dim).clone()
+        ok = (slots >= 0) & (slots < pages * page)
+        # the bytes are those of the rounded activations, and everything else stays
+        was[slots[ok]] = rows[ok].float().clamp(-57344, 57344).to(torch.float8_e5m2).view(torch.uint8) if eight else rows[ok]
+        assert torch.equal(flat.view(torch.uint8), was.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ attention
+def statement(q, k, v, cu, lens, scale, causal=True):
+    """64 bits.  q [T, H, D]; k, v: lists of [len_r, G, D]; returns the outputs, the same with |v|, and the largest absolute sum of a score"""
+    out, absolute, largest = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device), 0.0
+    group = q.shape[1] // k[0].shape[1]
+    for r in range(len(lens)):
+        a, b, n = cu[r], cu[r + 1], lens[r]
+        if a == b or n == 0:
+            continue
+        kr, vr = (t.double().repeat_interleave(group, 1) for t in (k[r], v[r]))
+        s = torch.einsum("ihd,jhd->hij", q[a:b].double(), kr) * scale
+        largest = max(largest, float(torch.einsum("ihd,jhd->hij", q[a:b].double().abs(), kr.abs()).max()) * scale)
+        if causal:
+            unseen = torch.arange(n, device=q.device)[None] > n - (b - a) + torch.arange(b - a, device=q.device)[:, None]
+            s = s.masked_fill(unseen, -math.inf)
+        p = torch.softmax(s, -1)
+        p = torch.where(torch.isnan(p), torch.zeros_like(p), p)
+        out[a:b] = torch.einsum("hij,jhd->ihd", p, vr)
+        absolute[a:b] = torch.einsum("hij,jhd->ihd", p, vr.abs())
+    return out, absolute, largest
+
+
+def bound(want, absolute, largest, dtype, p_dtype, dim, keys):
+    score = dim / 8 * largest * 2.0 ** -23 + 2.0 ** -22
+    return HALF[dtype] * want.abs() + HALF[p_dtype] * (absolute + want.abs()) + (2 * score + (keys / 8 + 8) * 2.0 ** -23) * absolute + 1e-7
+
+
+def requests(dev, new, held, heads, kv_heads, dim, dtype, eight, page, seed=0, q_scale=1.5, stale=math.nan):
+    """(q, caches, table, lens, cu, the keys and values of every request): rows and pages that nobody holds are ``stale``"""
+    g = torch.Generator(device=dev).manual_seed(seed + sum(new) + 7 * len(new))
+    lens = [h + n for h, n in zip(held, new)]
+    counts = [-(-n // page) for n in lens]
+    pages, width = sum(counts) + 2, max(counts + [1]) + 1
+    caches = [torch.full((pages, page, kv_heads, dim), stale, device=dev).to(torch.float8_e5m2 if eight else dtype) for _ in range(2)]
+    order = torch.randperm(pages, generator=g, device=dev)
+    table = torch.full((len(new), width), -1, dtype=torch.int32, device=dev)
+    rows, first = [[], []], 0
+    for r, (c, n) in enumerate(zip(counts, lens)):
+        mine = order[first:first + c]
+        first += c
+        table[r, :c] = mine.int()
+        for cache, keep in zip(caches, rows):
+            x = torch.randn(n, kv_heads, dim, generator=g, device=dev).to(cache.dtype)
+            keep.append(x)
+            at = mine[torch.arange(n, device=dev) // page] * page + torch.arange(n, device=dev) % page
+            cache.view(torch.uint8 if eight else torch.int16).view(-1, kv_heads, dim)[at] = x.view(torch.uint8 if eight else torch.int16)
+    q = (q_scale * torch.randn(sum(new), heads, dim, generator=g, device=dev)).to(dtype)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)                                 # noqa: E731
+    if eight:
+        caches = [c.view(torch.uint8) for c in caches]
+    return q, caches, table, on(lens), on(cu), rows, cu, lens
+
+
+def check_paged(paged, dev, new, held, heads, kv_heads, dim, dtype, eight, page, scale=None, hint=None, **kw):
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(dev, new, held, heads, kv_heads, dim, dtype, eight, page, **kw)
+    scale = dim ** -0.5 if scale is None else scale
+    got = paged.sdp_paged(q, *caches, table, lens, cu, scale, max_query_len=hint)
+    if eight:
+        rows = [[x.half() for x in part] for part in rows]
+    want, absolute, largest = statement(q, *rows, cu_list, len_list, scale)
+    limit = bound(want, absolute, largest, dtype, torch.float16 if eight else dtype, dim, max(len_list))
+    far = (got.double() - want).abs()
+    assert bool((far <= limit).all()), f"{float((far / limit).max()):.2f} of the bound"
+    return got
+
+
+KINDS = [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 2, 128), (8, 1, 64), (2, 2, 96), (7, 1, 80), (16, 1, 128), (6, 2, 256), (5, 5, 16), (3, 1, 192)])
+@pytest.mark.parametrize("held,page", [([0], 16), ([1, 15, 16, 17, 0], 16), ([127, 128, 129, 5, 1000], 8), ([255, 300, 31, 32, 33], 1), ([3000, 2, 700], 24)])
+def test_single_tokens(paged, cuda_device, dtype, eight, heads, kv_heads, dim, held, page):
+    check_paged(paged, cuda_device, [1] * len(held), held, heads, kv_heads, dim, dtype, eight, page, hint=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 2, 128), (8, 1, 64), (2, 2, 96), (7, 1, 80), (6, 2, 256), (3, 1, 192), (5, 1, 32)])
+@pytest.mark.parametrize("new,held,page", [([2], [0], 16), ([5, 1, 3], [100, 0, 16], 16), ([128], [0], 32), ([129, 1, 17], [3, 500, 0], 24), ([300, 2, 0, 64], [1000, 30, 40, 64], 64),
+                                           ([33, 257], [127, 1], 8)])
+def test_chunks(paged, cuda_device, dtype, eight, heads, kv_heads, dim, new, held, page):
+    check_paged(paged, cuda_device, new, held, heads, kv_heads, dim, dtype, eight, page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("R,heads,kv_heads", [(3, 32, 8), (70, 8, 2), (300, 4, 4), (1100, 2, 1)])
+def test_many_requests_of_different_lengths(paged, cuda_device, dtype, eight, R, heads, kv_heads):
+    g = torch.Generator().manual_seed(R)
+    held = [int(2 ** float(x)) for x in torch.rand(R, generator=g) * (11 if R < 100 else 8)]
+    for most in (1, 40):
+        new = [1 if i % 4 else 1 + int(x) for i, x in enumerate(torch.randint(0, most, (R,), generator=g))]
+        check_paged(paged, cuda_device, new, held, heads, kv_heads, 128, dtype, eight, 16, hint=most)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("new,held", [([1], [9000]), ([700], [2500]), ([1, 300, 1], [6000, 1500, 3])])
+@pytest.mark.parametrize("q_scale", [0.05, 4.0, 40.0])
+def test_flat_and_steep_softmax(paged, cuda_device, dtype, eight, new, held, q_scale):
+    """nearly equal probabilities over many keys, and scores of hundreds that pick single ones"""
+    check_paged(paged, cuda_device, new, held, 8, 2, 128, dtype, eight, 16, q_scale=q_scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+def test_requests_without_keys_and_rows_behind_the_last(paged, cuda_device, dtype, eight):
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, [3, 0, 1, 150], [20, 9, 4, 7], 8, 2, 64, dtype, eight, 16)
+    lens[0], lens[3] = 0, 140                                   # a request without keys; one whose first ten tokens see none
+    out = torch.full((q.shape[0] + 9, 8, 64), 5.0, dtype=dtype, device=cuda_device)
+    wide = torch.cat([q, torch.full((9, 8, 64), math.nan, dtype=dtype, device=cuda_device)])
+    got = paged.sdp_paged(wide, *caches, table, lens, cu, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert bool((out[:3] == 0).all()) and bool((out[4:14] == 0).all()) and bool((out[q.shape[0]:] == 5).all())
+    if eight:
+        rows = [[x.half() for x in part] for part in rows]
+    rows = [[x[:n] for x, n in zip(part, lens.tolist())] for part in rows]
+    want, absolute, largest = statement(q, *rows, cu_list, lens.tolist(), 64 ** -0.5)
+    want[4:14], absolute[4:14] = 0, 0
+    limit = bound(want, absolute, largest, dtype, torch.float16 if eight else dtype, 64, 157)
+    assert bool(((out[:q.shape[0]].double() - want).abs() <= limit).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("new", [[1, 1, 1], [200, 150, 90]])
+def test_values_that_are_not_numbers_stay_with_their_request(paged, cuda_device, dtype, eight, new):
+    """another request's infinities and NaN, and a page that does not exist, reach no row of the others"""
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, new, [300, 31, 77], 4, 2, 128, dtype, eight, 16)
+    want = paged.sdp_paged(q, *caches, table, lens, cu)
+    bad = {torch.float16: 0x7e00, torch.bfloat16: 0x7fc0}[dtype]
+    for cache in caches:
+        cache.view(torch.uint8 if eight else torch.int16)[table[1, 1].long(), 3] = 0x7f if eight else bad
+    got = paged.sdp_paged(q, *caches, table, lens, cu)
+    a, b = cu_list[1], cu_list[2]
+    assert torch.equal(got[:a], want[:a]) and torch.equal(got[b:], want[b:]) and bool(torch.isnan(got[b - 1]).all())
+    table[1, 0] = -1
+    table[2, 2] = 10 ** 6
+    got = paged.sdp_paged(q, *caches, table, lens, cu)
+    assert torch.equal(got[:a], want[:a]) and bool(torch.isnan(got[b - 1]).all()) and bool(torch.isnan(got[-1]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", [KINDS[1], KINDS[3]])
+def test_a_cache_beyond_32_bits(paged, cuda_device, dtype, eight):
+    """offsets of more than 2^32 elements, and a layout with the heads in front of the rows"""
+    page, kv_heads, dim, pages = 16, 2, 128, (1 << 32) // (16 * 2 * 128) + 40
+    kind = torch.uint8 if eight else dtype
+    caches = [torch.zeros(pages, kv_heads, page, dim, dtype=kind, device=cuda_device).transpose(1, 2) for _ in range(2)]
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    table = torch.tensor([[pages - 1, 3, pages - 7], [2, pages - 2, -1]], dtype=torch.int32, device=cuda_device)
+    lens, cu = torch.tensor([40, 19], dtype=torch.int32, device=cuda_device), torch.tensor([0, 20, 21], dtype=torch.int32, device=cuda_device)
+    rows = [[], []]
+    for r, n in enumerate((40, 19)):
+        for cache, keep in zip(caches, rows):
+            x = torch.randn(n, kv_heads, dim, generator=g, device=cuda_device).to(torch.float8_e5m2 if eight else dtype)
+            keep.append(x.half() if eight else x)
+            for j in range(n):
+                cache[int(table[r, j // page]), j % page] = x[j].view(torch.uint8) if eight else x[j]
+    q = torch.randn(21, 4, dim, generator=g, device=cuda_device).to(dtype)
+    got = paged.sdp_paged(q, *caches, table, lens, cu)
+    want, absolute, largest = statement(q, *rows, [0, 20, 21], [40, 19], dim ** -0.5)
+    assert bool(((got.double() - want).abs() <= bound(want, absolute, largest, dtype, torch.float16 if eight else dtype, dim, 40)).all())
+
+
+@pytest.mark.gpu
+def test_views_and_layouts(paged, cuda_device):
+    """queries inside the merged projection's output, outputs with room between the heads, heads before rows, a misaligned query"""
+    dev, dtype = cuda_device, torch.bfloat16
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(dev, [1, 70, 4], [90, 33, 8], 8, 2, 64, dtype, False, 16)
+    want = paged.sdp_paged(q, *caches, table, lens, cu)
+    flat = torch.randn(q.shape[0], 12 * 64, device=dev).to(dtype)
+    flat[:, :8 * 64] = q.flatten(1)
+    view = flat.view(q.shape[0], 12, 64)[:, :8]
+    turned = [c.transpose(1, 2).contiguous().transpose(1, 2) for c in caches]
+    out = torch.full((q.shape[0], 8, 96), 3.0, device=dev).to(dtype)
+    paged.sdp_paged(view, *turned, table, lens, cu, out=out[..., :64])
+    assert torch.equal(out[..., :64], want) and bool((out[..., 64:] == 3).all())
+    odd = torch.empty(q.numel() + 1, dtype=dtype, device=dev)[1:].view(q.shape)
+    odd.copy_(q)
+    assert odd.data_ptr() % 16 and torch.equal(paged.sdp_paged(odd, *caches, table, lens, cu), want)
+
+
+# ------------------------------------------------------------------ packed prompts
+def check_packed(paged, dev, lens, heads, kv_heads, dim, dtype, causal=True, q_scale=1.5, hint=True, pad=0):
+    g = torch.Generator(device=dev).manual_seed(sum(lens) + heads)
+    T = sum(lens)
+    x = torch.randn(T + pad, heads + 2 * kv_heads, dim, generator=g, device=dev)
+    x[:, :heads] *= q_scale
+    x = x.to(dtype)
+    x[T:] = math.nan                                            # padding behind the last prompt
+    q, k, v = x.split([heads, kv_heads, kv_heads], 1)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    out = torch.full((T + pad, heads, dim), 7.0, dtype=dtype, device=dev)
+    got = paged.sdp_packed(q, k, v, torch.tensor(cu, dtype=torch.int32, device=dev), is_causal=causal, max_seqlen=max(lens) if hint else None, out=out)
+    assert bool((got[T:] == 7).all())
+    parts = [[t[a:b] for a, b in zip(cu, cu[1:])] for t in (k, v)]
+    want, absolute, largest = statement(q[:T], *parts, cu, lens, dim ** -0.5, causal)
+    limit = bound(want, absolute, largest, dtype, dtype, dim, max(lens))
+    far = (got[:T].double() - want).abs()
+    assert bool((far <= limit).all()), f"{float((far / limit).max()):.2f} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 2, 128), (8, 1, 64), (2, 2, 96), (7, 1, 80), (6, 2, 256), (3, 1, 192), (12, 4, 64), (5, 1, 16)])
+@pytest.mark.parametrize("lens", [[1], [1, 1, 2], [64, 63, 65], [128, 1, 127, 129], [0, 300, 0, 5], [517, 256]])
+def test_packed(paged, cuda_device, dtype, heads, kv_heads, dim, lens):
+    check_packed(paged, cuda_device, lens, heads, kv_heads, dim, dtype, hint=sum(lens) % 2 == 0, pad=sum(lens) % 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim,lens", [(4, 2, 128, [1, 130, 700]), (2, 2, 64, [90, 257]), (2, 1, 256, [300])])
+def test_packed_without_a_causal_mask(paged, cuda_device, dtype, heads, kv_heads, dim, lens):
+    check_packed(paged, cuda_device, lens, heads, kv_heads, dim, dtype, causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([2100, 900, 33], 32, 8), ([3000], 8, 8), ([40] * 90, 8, 2), ([1 + i % 7 for i in range(700)], 4, 2)])
+@pytest.mark.parametrize("q_scale", [0.05, 1.5, 20.0])
+def test_packed_long_and_many(paged, cuda_device, dtype, lens, heads, kv_heads, q_scale):
+    check_packed(paged, cuda_device, lens, heads, kv_heads, 128, dtype, q_scale=q_scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_packed_neighbours_do_not_meet(paged, cuda_device, dtype):
+    """infinities and NaN of one prompt reach no row of another"""
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    lens, cu = [70, 30, 200, 5], [0, 70, 100, 300, 305]
+    q, k, v = (torch.randn(305, h, 128, generator=g, device=cuda_device).to(dtype) for h in (4, 2, 2))
+    on = torch.tensor(cu, dtype=torch.int32, device=cuda_device)
+    want = paged.sdp_packed(q, k, v, on)
+    k[80], v[81], v[299] = math.nan, math.inf, -math.inf
+    got = paged.sdp_packed(q, k, v, on)
+    for r, bad in enumerate((False, True, True, False)):
+        if not bad:
+            assert torch.equal(got[cu[r]:cu[r + 1]], want[cu[r]:cu[r + 1]])
+    assert bool(torch.isnan(got[99]).any()) and not bool(torch.isfinite(got[299]).any())
+
+
+# ------------------------------------------------------------------ together, recorded, on other streams
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", [(torch.float16, True), (torch.bfloat16, False)])
+def test_a_server(paged, cuda_device, dtype, eight):
+    """requests come, run and go: pages are handed out and come back, and every step's attention is that over all of a request's own tokens"""
+    dev, heads, kv_heads, dim, page, pages, rows = cuda_device, 8, 2, 64, 8, 60, 5
+    g = torch.Generator(device=dev).manual_seed(1)
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)                                 # noqa: E731
+    kind = torch.uint8 if eight else dtype
+    caches = [torch.full((pages, page, kv_heads, dim), 0x7f, dtype=torch.uint8, device=dev) if eight else torch.full((pages, page, kv_heads, dim), math.nan, dtype=kind, device=dev)
+              for _ in range(2)]
+    cos, sin = tables(dim, 300, dev)
+    table, stack, count = torch.full((rows, 20), -1, dtype=torch.int32, device=dev), torch.arange(pages, dtype=torch.int32, device=dev), on([pages])
+    held, past = [0] * rows, [[[], []] for _ in range(rows)]
+    plan = [[9, 0, 30, 1, 0], [1, 17, 1, 1, 0], [1, 1, 1, 0, 5], "0", [40, 1, 1, 0, 1], [1, 1, 1, 8, 1], "24", [1, 1, 12, 1, 3], [1, 1, 1, 1, 1]]
+    for step in plan:
+        if isinstance(step, str):
+            done = torch.zeros(rows, dtype=torch.bool, device=dev)
+            for r in map(int, step):
+                done[r], held[r], past[r] = True, 0, [[], []]
+            paged.paged_release(done, table, stack, count)
+            continue
+        T = sum(step)
+        st = paged.paged_step(on(step), on(held), table, stack, count, page, T, free_left=count)
+        qkv = torch.randn(T, (heads + 2 * kv_heads) * dim, generator=g, device=dev).to(dtype)
+        paged.paged_rope_append(qkv, heads, kv_heads, dim, cos, sin, st.positions, st.slots, *caches)
+        x = qkv.view(T, -1, dim)
+        got = paged.sdp_paged(x[:, :heads], *caches, table, st.seq_lens, st.cu_seqlens)
+        cu = st.cu_seqlens.tolist()
+        for r in range(rows):
+            for part, first in zip(past[r], (heads, heads + kv_heads)):
+                new = x[cu[r]:cu[r + 1], first:first + kv_heads]
+                part.append(new.to(torch.float8_e5m2).half() if eight else new)
+            held[r] += step[r]
+        k, v = ([torch.cat(past[r][i]) for r in range(rows)] for i in (0, 1))
+        want, absolute, largest = statement(x[:, :heads], k, v, cu, held, dim ** -0.5)
+        assert bool(((got.double() - want).abs() <= bound(want, absolute, largest, dtype, torch.float16 if eight else dtype, dim, 300)).all())
+        if held == step and not eight:                          # nobody held anything before: the prompts' own attention says the same
+            packed = paged.sdp_packed(x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:], st.cu_seqlens)
+            assert bool(((packed.double() - want).abs() <= bound(want, absolute, largest, dtype, dtype, dim, 300)).all())
+        assert st.missing.item() == 0 and count.item() == pages - sum(-(-h // page) for h in held)
+    paged.paged_release(torch.ones(rows, dtype=torch.bool, device=dev), table, stack, count)
+    assert sorted(stack.tolist()) == list(range(pages)) and count.item() == pages
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+def test_a_recorded_step_serves_other_lengths(paged, cuda_device, dtype, eight):
+    """one graph of step, write and attention, replayed while the lengths on the device move; two graphs of it do not meet in a workspace"""
+    dev, heads, kv_heads, dim, page, R, width = cuda_device, 8, 2, 128, 16, 6, 80
+    g = torch.Generator(device=dev).manual_seed(2)
+    pages = R * width
+    kind = torch.uint8 if eight else dtype
+    caches = [torch.randn(pages, page, kv_heads, dim, generator=g, device=dev).to(torch.float8_e5m2).view(torch.uint8) if eight
+              else torch.randn(pages, page, kv_heads, dim, generator=g, device=dev).to(kind) for _ in range(2)]
+    table = torch.randperm(pages, generator=g, device=dev).to(torch.int32).view(R, width)          # every page handed out: nothing to take
+    keep = table.clone()
+    stack, count = torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    new, held = torch.ones(R, dtype=torch.int32, device=dev), torch.zeros(R, dtype=torch.int32, device=dev)
+    qkv = torch.randn(16, (heads + 2 * kv_heads) * dim, generator=g, device=dev).to(dtype)
+    cos, sin = tables(dim, 2000, dev)
+
+    def call(x):
+        st = paged.paged_step(new, held, table, stack, count, page, 16)
+        paged.paged_rope_append(x, heads, kv_heads, dim, cos, sin, st.positions, st.slots, *caches)
+        out = torch.zeros(16, heads, dim, dtype=dtype, device=dev)
+        return paged.sdp_paged(x.view(16, -1, dim)[:, :heads], *caches, table, st.seq_lens, st.cu_seqlens, out=out, max_query_len=4)
+
+    side, recorded = torch.cuda.Stream(), []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(qkv.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(2):
+        graph, x = torch.cuda.CUDAGraph(), qkv.clone()
+        with torch.cuda.graph(graph):
+            y = call(x)
+        recorded.append((graph, x, y))
+    for counts, lens in (([1] * 6, [5, 100, 31, 0, 700, 64]), ([4, 1, 0, 3, 2, 4], [1201, 2, 9, 1, 641, 4]), ([1, 0, 0, 0, 0, 0], [1000, 0, 0, 0, 0, 0])):
+        new.copy_(torch.tensor(counts, dtype=torch.int32))
+        held.copy_(torch.tensor(lens, dtype=torch.int32))
+        # a new token that opens a page gets none here (the stack is empty): its entry becomes -1
+        before = [c.clone() for c in caches]
+        opens = bool((((held + new + page - 1) // page) > ((held + page - 1) // page)).any())
+        for graph, x, y in recorded:
+            for c, b in zip(caches, before):
+                c.copy_(b)
+            table.copy_(keep)
+            x.copy_(qkv)
+            graph.replay()
+        results = [y.clone() for _, _, y in recorded]
+        assert torch.equal(*[torch.nan_to_num(r) for r in results])
+        for c, b in zip(caches, before):
+            c.copy_(b)
+        table.copy_(keep)
+        want = call(qkv.clone())
+        assert torch.equal(torch.nan_to_num(want), torch.nan_to_num(results[0])) and (opens or not bool(torch.isnan(want[:sum(counts)]).any()))
+
+
+@pytest.mark.gpu
+def test_on_other_streams_at_once(paged, cuda_device):
+    """two streams, other lengths on each, many calls in flight: every result is that of the call alone"""
+    sets = [requests(cuda_device, new, held, 8, 2, 128, torch.bfloat16, eight, 16, seed=i)
+            for i, (new, held, eight) in enumerate([([1] * 5, [3000, 20, 700, 1, 90], False), ([300, 1], [20, 900], False), ([1, 1], [5000, 6], True)])]
+    call = lambda s: paged.sdp_paged(s[0], *s[1], s[2], s[3], s[4])                               # noqa: E731
+    want = [call(s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[] for _ in sets]
+    for _ in range(20):
+        for stream, s, keep in zip(streams, sets, got):
+            with torch.cuda.stream(stream):
+                keep.append(call(s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for keep, w in zip(got, want) for x in keep)
+
+
+# ------------------------------------------------------------------ what is refused
+def test_refusals_without_a_device(native_lib):
+    """bad arguments are refused before anything touches a device"""
+    lib, p = native_lib._lib, ctypes.cast(ctypes.create_string_buffer(4096 + 16), ctypes.c_void_p)
+    p = ctypes.c_void_p(p.value + 15 & ~15)
+    s2, s3, odd = (ctypes.c_int64 * 2)(256, 64), (ctypes.c_int64 * 3)(1024, 64, 64), (ctypes.c_int64 * 2)(256, 65)
+
+    def refused(rc, needle):
+        msg = lib.b200_lowbit_last_error_string().decode()
+        lib.b200_lowbit_clear_error()
+        return rc != 0 and needle in msg
+
+    step = lambda R=2, width=4, stride=4, pages=8, page=16, n=3, table=p: lib.lowbit_paged_step_cuda(               # noqa: E731
+        p, p, R, table, stride, width, p, pages, p, p, page, n, p, p, p, p, p, None)
+    for bad in (dict(R=0), dict(width=0), dict(stride=3), dict(pages=0), dict(page=0), dict(n=-1), dict(table=None)):
+        assert refused(step(**bad), "lowbit_paged_step_cuda"), bad
+    assert refused(lib.lowbit_paged_release_cuda(p, 0, p, 4, 4, p, 8, p, None), "lowbit_paged_release_cuda")
+    append = lambda dtype=1, cache=1, T=3, heads=2, kv=1, dim=64, rotary=64, cos=p, stride=256, pages=4: lib.lowbit_paged_rope_append_cuda(   # noqa: E731
+        p, dtype, stride, T, heads, kv, dim, rotary, cos, p, 0, 64, 10, p, p, p, s3, p, s3, cache, pages, 16, None)
+    for bad in (dict(dtype=0, cache=0), dict(cache=2), dict(kv=0), dict(rotary=66), dict(rotary=31), dict(cos=None), dict(stride=255), dict(pages=0), dict(T=-1)):
+        assert refused(append(**bad), "lowbit_paged_rope_append_cuda"), bad
+
+    def attend(q=p, dtype=1, q_strides=s2, T=4, cache=1, pages=4, page=16, table=p, width=2, R=2, heads=4, kv=2, dim=64, scale=0.1):
+        return lib.lowbit_sdp_paged_cuda(q, dtype, q_strides, T, p, s3, p, s3, cache, pages, page, table, width, width, p, p, R, heads, kv, dim, scale, T, p, s2, p, 0, None)
+    for bad in (dict(q=None), dict(dtype=0, cache=0), dict(cache=2), dict(cache=0), dict(q_strides=odd), dict(T=-1), dict(pages=0), dict(page=0), dict(table=None), dict(width=0),
+                dict(R=0), dict(kv=3), dict(dim=72), dict(dim=272), dict(scale=0.0), dict(scale=math.nan), dict(page=1 << 30), dict(q=ctypes.c_void_p(p.value + 2))):
+        assert refused(attend(**bad), "lowbit_sdp_paged_cuda"), bad
+
+    def packed(q=p, dtype=1, strides=s2, T=4, R=2, heads=4, kv=2, dim=64, scale=0.1):
+        return lib.lowbit_sdp_packed_cuda(q, dtype, strides, T, p, strides, p, strides, p, R, heads, kv, dim, scale, 1, T, p, s2, p, 0, None)
+    for bad in (dict(q=None), dict(dtype=0), dict(dtype=19), dict(strides=odd), dict(T=-1), dict(T=1 << 31), dict(R=0), dict(heads=5), dict(dim=24), dict(scale=-1.0)):
+        assert refused(packed(**bad), "lowbit_sdp_packed_cuda"), bad
+
+
+def test_refusals_on_the_cpu(paged):
+    i = lambda *n: torch.zeros(n, dtype=torch.int32)                                              # noqa: E731
+    x = torch.zeros(2, 4, 64, dtype=torch.float16)
+    c = torch.zeros(3, 16, 4, 64, dtype=torch.float16)
+    for call in (lambda: paged.paged_step(i(2), i(2), i(2, 4), i(5), i(1), 16, 2), lambda: paged.paged_release(torch.zeros(2, dtype=torch.bool), i(2, 4), i(5), i(1)),
+                 lambda: paged.paged_rope_append(x.view(2, 256), 2, 1, 64, None, None, None, torch.zeros(2, dtype=torch.int64), c[:, :, :1], c[:, :, :1]),
+                 lambda: paged.sdp_paged(x, c, c, i(2, 4), i(2), i(3)), lambda: paged.sdp_packed(x, x, x, i(3))):
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            call()
+    for t in (x.float().requires_grad_(), x.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="backward"):
+            paged.sdp_packed(t, x, x, i(3))
+
+
+@pytest.mark.gpu
+def test_refusals(paged, cuda_device):
+    dev = cuda_device
+    i = lambda *n: torch.zeros(n, dtype=torch.int32, device=dev)                                  # noqa: E731
+    h = lambda *n: torch.zeros(n, dtype=torch.float16, device=dev)                                # noqa: E731
+    q, c, table, lens, cu = h(6, 4, 64), h(3, 16, 2, 64), i(2, 4), i(2), i(3)
+    bad = [lambda: paged.paged_step(i(2), i(3), table, i(5), i(1), 16, 2), lambda: paged.paged_step(i(2), i(2).long(), table, i(5), i(1), 16, 2),
+           lambda: paged.paged_step(i(2), i(2), table.t(), i(5), i(1), 16, 2), lambda: paged.paged_step(i(2), i(2), i(3, 4), i(5), i(1), 16, 2),
+           lambda: paged.paged_step(i(2), i(2), table, i(5), i(1), 0, 2), lambda: paged.paged_step(i(2), i(2), table, i(5), i(1).cpu(), 16, 2),
+           lambda: paged.paged_step(i(0), i(0), i(0, 4), i(5), i(1), 16, 2), lambda: paged.paged_step(i(2), i(2), table, i(5), i(1), 16, -1),
+           lambda: paged.paged_release(i(2), table, i(5), i(1)), lambda: paged.paged_release(torch.zeros(3, dtype=torch.bool, device=dev), table, i(5), i(1)),
+           lambda: paged.sdp_paged(q.float(), c.float(), c.float(), table, lens, cu), lambda: paged.sdp_paged(q, c.bfloat16(), c.bfloat16(), table, lens, cu),
+           lambda: paged.sdp_paged(q, c, c[:, :, :1], table, lens, cu), lambda: paged.sdp_paged(q, c[..., :32], c[..., :32], table, lens, cu),
+           lambda: paged.sdp_paged(h(6, 3, 64), c, c, table, lens, cu), lambda: paged.sdp_paged(h(6, 4, 72), h(3, 16, 2, 72), h(3, 16, 2, 72), table, lens, cu),
+           lambda: paged.sdp_paged(h(6, 4, 272), h(3, 16, 2, 272), h(3, 16, 2, 272), table, lens, cu), lambda: paged.sdp_paged(q, c, c, table, i(3), cu),
+           lambda: paged.sdp_paged(q, c, c, table, lens, i(4)), lambda: paged.sdp_paged(q, c, c, table, lens, cu.long()), lambda: paged.sdp_paged(q, c, c, table, lens, cu, scale=0.0),
+           lambda: paged.sdp_paged(q, c, c, table, lens, cu, out=h(6, 4, 32)), lambda: paged.sdp_paged(q, c, c, table, lens, cu, max_query_len=-1),
+           lambda: paged.sdp_paged(q, c, c, table.long(), lens, cu), lambda: paged.sdp_paged(q, c, c, table, lens.cpu(), cu),
+           lambda: paged.sdp_paged(q, h(3, 16, 2, 68)[..., :64], c, table, lens, cu),
+           lambda: paged.sdp_packed(q, h(5, 2, 64), h(5, 2, 64), cu), lambda: paged.sdp_packed(q, h(6, 3, 64), h(6, 3, 64), cu), lambda: paged.sdp_packed(q, h(6, 2, 64), h(6, 2, 64).bfloat16(), cu),
+           lambda: paged.paged_rope_append(h(6, 512), 4, 2, 64, None, None, None, torch.zeros(5, dtype=torch.int64, device=dev), c, c),
+           lambda: paged.paged_rope_append(h(6, 500), 4, 2, 64, None, None, None, torch.zeros(6, dtype=torch.int64, device=dev), c, c),
+           lambda: paged.paged_rope_append(h(1, 512).expand(6, 512), 4, 2, 64, None, None, None, torch.zeros(6, dtype=torch.int64, device=dev), c, c),
+           lambda: paged.paged_rope_append(h(6, 512), 4, 2, 64, h(9, 66), h(9, 66), torch.zeros(6, dtype=torch.int64, device=dev), torch.zeros(6, dtype=torch.int64, device=dev), c, c)]
+    for n, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {n} was taken")
+    assert paged.sdp_paged(q[:0], c, c, table, lens, cu).shape == (0, 4, 64) and paged.sdp_packed(q[:0], q[:0], q[:0], cu).shape == (0, 4, 64)
