@@ -37,4 +37,61 @@ __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& A, int r) {
     return q;
 }
 
+// ---- work in equal shares.  The tiles of all units (a request's kv head; or a block of its rows on one) lie behind one another, n of them
+// in all, and block c of C takes tiles c n / C .. (c + 1) n / C: whatever the lengths, every block reads as many.  A unit whose tiles
+// lie in several blocks leaves its sums there, each block's slot 1 for a unit that began in it and slot 0 for one that did not, and the
+// merge adds them up in the order of the keys.
+__host__ __device__ inline int64_t share_begin(int64_t n, int c, int C) { return n * c / C; }
+__host__ __device__ inline int share_of(int64_t tile, int64_t n, int C) { return (int)(((tile + 1) * C - 1) / n); }      // the block that takes a tile
+
+// sum over the block before this thread, and of all of it
+__device__ __forceinline__ int64_t block_before(int64_t x, int64_t* warps, int64_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (blockDim.x + 31) >> 5;
+    int64_t s = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d) s += y;
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = s;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+    for (int w = 0; w < n; w++) {
+        if (w < warp) before += warps[w];
+        total += warps[w];
+    }
+    return before + s - x;
+}
+// the whole block: tiles of all requests (count(r) of request r), and the request that holds tile `pick(total)` with the tiles before it.
+// Two walks over the requests when they are more than the threads
+template <typename Count, typename Pick>
+__device__ __forceinline__ int64_t find_tile(int R, Count count, Pick pick, int64_t* warps, int* r_out, int64_t* before_out) {
+    int64_t all = 0, mine = 0, first = 0;
+    for (int r0 = 0; r0 < R; r0 += blockDim.x) {
+        const int r = r0 + threadIdx.x;
+        int64_t total;
+        mine = r < R ? count(r) : 0;
+        first = all + block_before(mine, warps, total);
+        all += total;
+    }
+    const int64_t want = all > 0 ? pick(all) : -1;
+    if (R <= (int)blockDim.x) {
+        if (mine > 0 && first <= want && want < first + mine) { *r_out = threadIdx.x; *before_out = first; }
+    } else {
+        int64_t sum = 0;
+        for (int r0 = 0; r0 < R; r0 += blockDim.x) {
+            const int r = r0 + threadIdx.x;
+            int64_t total;
+            mine = r < R ? count(r) : 0;
+            first = sum + block_before(mine, warps, total);
+            sum += total;
+            if (mine > 0 && first <= want && want < first + mine) { *r_out = r; *before_out = first; }
+        }
+    }
+    __syncthreads();
+    return all;
+}
+
 }  // namespace lowbit

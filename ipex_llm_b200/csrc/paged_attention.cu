@@ -11,7 +11,7 @@ namespace {
 
 // a warp per (token, query head): one pass over the keys with the running maximum and sum
 template <typename T, bool E5M2>
-__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const PagedAttnArgs A) {
+__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const PagedAttnArgs A, int above) {
     const int lane = threadIdx.x & 31;
     const int64_t w = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
     const int64_t t = w / A.Hq;
@@ -24,6 +24,7 @@ __global__ void __launch_bounds__(128) paged_attention_simple_kernel(const Paged
         q = paged_req(A, r);
         if (t >= q.q0 && t < q.q0 + q.n) break;
     }
+    if ((int64_t)q.n * (A.Hq / A.Hkv) <= above) return;
     auto load = [&](const void* p, int64_t i) -> float {
         if (sizeof(T) == 2 && E5M2) return decode_e5m2(((const uint8_t*)p)[i]);
         if constexpr (std::is_same<T, __half>::value) return __half2float(((const __half*)p)[i]);
@@ -72,6 +73,462 @@ __global__ void __launch_bounds__(128) paged_attention_simple_kernel(const Paged
     }
 }
 
+// ------------------------------------------------------------------ few rows (decoding): at most 16 rows = new tokens x heads of a group
+constexpr int FEW_ROWS = 16;
+
+template <int DP, bool E5M2> struct Few {
+    static constexpr int kWarps = DP == 256 ? 4 : 8, kStages = DP == 64 ? 6 : 3;
+    static constexpr int kKeys = E5M2 ? 32 : 16;                      // a warp's keys of a tile
+    static constexpr int kTile = kWarps * kKeys;
+    static constexpr int kRow = DP * (E5M2 ? 1 : 2);                  // bytes
+    static constexpr int kHalf = kKeys * kRow, kStage = 2 * kHalf;    // keys, values
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kSums = kWarps * 8 * DP * 4, kSmem = kRing + kSums + kWarps * FEW_ROWS * 8;
+    static constexpr int kPart = FEW_ROWS * DP + 2 * FEW_ROWS;        // floats of a slot
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(x) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+    return r;
+}
+template <bool TRANS> __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    if (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+    else asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF) asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// two values rounded to 16 bits, and what that left
+template <bool BF> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if (BF) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
+        hi = *reinterpret_cast<const uint32_t*>(&h);
+        lo = *reinterpret_cast<const uint32_t*>(&l);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+        hi = *reinterpret_cast<const uint32_t*>(&h);
+        lo = *reinterpret_cast<const uint32_t*>(&l);
+    }
+}
+template <bool BF> __device__ __forceinline__ float unpack16(uint32_t w, int hi) {
+    if (BF) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return hi ? __high2float(h) : __low2float(h);
+}
+__device__ __forceinline__ uint32_t pack_half(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool BF> __device__ __forceinline__ void store4(uint16_t* p, const float4& x, float by) {
+    uint2 w;
+    if (BF) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x * by, x.y * by), b = __floats2bfloat162_rn(x.z * by, x.w * by);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else w = make_uint2(pack_half(x.x * by, x.y * by), pack_half(x.z * by, x.w * by));
+    *reinterpret_cast<uint2*>(p) = w;
+}
+
+// a request's tiles on one kv head: none where its rows are another kernel's, one where it has no keys (its rows become zeros)
+__device__ __forceinline__ int64_t few_tiles(const PagedReq& q, int group, int tile) {
+    if (q.n <= 0 || (int64_t)q.n * group > FEW_ROWS) return 0;
+    return q.len > 0 ? (q.len + tile - 1) / tile : 1;
+}
+
+// where a block is in its share: request, kv head, tile of that head
+struct FewAt {
+    PagedReq q; int r, hk; int64_t tile, tiles;
+    __device__ __forceinline__ void next(const PagedAttnArgs& A, int group, int tile_keys) {
+        if (++tile < tiles) return;
+        tile = 0;
+        if (++hk < A.Hkv) return;
+        hk = 0;
+        do {
+            if (++r >= A.R) { tiles = 0; return; }
+            q = paged_req(A, r);
+            tiles = few_tiles(q, group, tile_keys);
+        } while (tiles == 0);
+    }
+};
+
+template <int DP, bool BF, bool E5M2>
+__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
+    using F = Few<DP, E5M2>;
+    constexpr bool MBF = BF && !E5M2;                                 // type in the products: fp16 over e5m2
+    constexpr int NW = F::kWarps, ST = F::kStages, KW = F::kKeys, ROW = F::kRow, CH = ROW / 16, NT = KW / 8;
+    extern __shared__ __align__(128) uint8_t few_smem[];
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = A.Hq / A.Hkv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int C = gridDim.x, c = blockIdx.x;
+    const int64_t all = find_tile(A.R, [&](int r) { return few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
+                                  [&](int64_t n) { return share_begin(n, c, C); }, scan, &found_r, &found_before);
+    if (all == 0) return;
+    const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
+    if (first == last) return;
+    FewAt at;                                                          // of the products
+    at.r = found_r;
+    at.q = paged_req(A, at.r);
+    at.tiles = few_tiles(at.q, group, F::kTile);
+    at.hk = (int)((first - found_before) / at.tiles);
+    at.tile = (first - found_before) % at.tiles;
+    FewAt in = at;                                                     // of the copies
+
+    const uint32_t ring = smem_addr(few_smem) + warp * ST * F::kStage;
+    float* const sums = reinterpret_cast<float*>(few_smem + F::kRing);                       // [warp][8][DP]
+    float2* const stats = reinterpret_cast<float2*>(few_smem + F::kRing + F::kSums);         // [warp][16]
+    // columns behind D stay zero: they are never copied to
+    if (A.D < DP) {
+        for (int i = lane; i < ST * F::kStage / 16; i += 32) sts16(ring + 16 * i, 0u);
+        __syncwarp();
+    }
+    const int live = A.D * (E5M2 ? 1 : 2) / 16;                        // 16-byte pieces of a row
+    // which piece of a row lies where: keys are read 8 rows x 16 bytes (ldmatrix), or a lane 16 bytes of row g; values a lane of rows 2 t
+    auto k_at = [&](int row, int piece) { return (uint32_t)(row * ROW + ((E5M2 ? (CH >= 8 ? piece ^ ((row & 1) << 2) : piece) : piece ^ (row & 7)) << 4)); };
+    auto v_at = [&](int row, int piece) {
+        const int turn = !E5M2 ? row & 7 : CH == 4 ? (row >> 1) & 3 : CH == 8 ? row & 6 : ((row >> 1) & 1) | (row & 4);
+        return (uint32_t)(row * ROW + ((piece ^ turn) << 4));
+    };
+    // the page of this lane's key in the copies' tile, one tile ahead of its copies
+    int page = 0;
+    auto key_of = [&](const FewAt& w) { return w.tile * F::kTile + warp * KW + (KW == 32 ? lane : lane & 15); };
+    auto ask = [&]() {
+        const int64_t key = key_of(in);
+        if (in.tiles > 0 && key < in.q.len) page = A.table[in.r * A.table_stride + (int)key / A.page_size];
+    };
+    auto copy = [&](int stage) {
+        const uint32_t dst = ring + stage * F::kStage;
+        const int64_t key = key_of(in);
+        const bool here = key < in.q.len, bad = here && (page < 0 || page >= A.n_pages);
+        if (__any_sync(0xffffffffu, here)) {
+            const int row = (int)key % A.page_size;
+            const int64_t ko = here && !bad ? page * A.k_sp + row * A.k_ss + in.hk * A.k_sh : 0, vo = here && !bad ? page * A.v_sp + row * A.v_ss + in.hk * A.v_sh : 0;
+            const uint32_t state = here ? bad ? 2u : 1u : 0u;
+#pragma unroll
+            for (int i = 0; i < KW * CH / 32; i++) {
+                const int r = (i * 32 + lane) / CH, piece = lane % CH;
+                const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                const uint32_t s = __shfl_sync(0xffffffffu, state, r);
+                if (piece < live) {
+                    const uint32_t bytes = s == 1 ? 16u : 0u;
+                    cp16(dst + k_at(r, piece), (const uint8_t*)A.k + kr * (E5M2 ? 1 : 2) + piece * 16, bytes);
+                    if (s == 2) sts16(dst + F::kHalf + v_at(r, piece), E5M2 ? 0x7f7f7f7fu : 0x7fff7fffu);      // no such page: not a number
+                    else cp16(dst + F::kHalf + v_at(r, piece), (const uint8_t*)A.v + vr * (E5M2 ? 1 : 2) + piece * 16, bytes);
+                }
+            }
+        }
+        in.next(A, group, F::kTile);
+        ask();
+    };
+    const int n = (int)(last - first);
+    ask();
+    for (int s = 0; s < ST - 1; s++) {
+        if (s < n) copy(s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // the unit's queries as A fragments; factor = scale x log2 e (x what a row was divided by) of rows g and g + 8
+    uint32_t qf[DP / 16][4];
+    float factor[2], m[2], sum[2], o[DP / 8][4];
+    int64_t see[2];
+    int rows = 0;
+    bool begun = false, from_start = false;
+    for (int i = 0; i < n; i++) {
+        const int stage = i % ST;
+        if (i + ST - 1 < n) copy((i + ST - 1) % ST);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!begun) {
+            begun = true;
+            from_start = at.tile == 0;
+            rows = at.q.n * group;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = g + 8 * h, token = row / group;
+                see[h] = row < rows ? (int64_t)at.q.len - at.q.n + token + 1 : 0;
+                const uint16_t* p = (const uint16_t*)A.q + (at.q.q0 + token) * A.q_st + (int64_t)(at.hk * group + row % group) * A.q_sh;
+                factor[h] = A.scale_log2e;
+                if (E5M2) {
+                    // k-step (c, s) of lane t holds elements 64 c + 16 t + 4 s .. + 3, the order in which a lane reads a key's bytes
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int cc = 0; cc < DP / 64; cc++) {
+                        const int d = 64 * cc + 16 * t;
+                        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+                        if (row < rows && d < A.D) { x = *reinterpret_cast<const uint4*>(p + d); y = *reinterpret_cast<const uint4*>(p + d + 8); }
+                        const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            qf[4 * cc + e / 2][h + 2 * (e & 1)] = w[e];
+                            big = max(big, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+                        }
+                    }
+                    if (BF) {
+                        // bf16 enters as fp16, divided by a power of two that brings the row's largest value to 2^14: exact but for what
+                        // lies 2^-28 below it (fp16's last bit, 2^-24), where a 32-bit sum with that value ends too
+                        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                        const int ex = (int)(big >> 7) - 127 - 14, e = big >= 0x7f80u || big == 0u ? 0 : ex < -100 ? -100 : ex;
+                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                        factor[h] *= __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                        for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+                            for (int z = 0; z < 2; z++) {
+                                const uint32_t w = qf[k][h + 2 * z];
+                                qf[k][h + 2 * z] = pack_half(unpack16<true>(w, 0) * down, unpack16<true>(w, 1) * down);
+                            }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+                        for (int z = 0; z < 2; z++) {
+                            const int d = 16 * k + 8 * z + 2 * t;
+                            qf[k][h + 2 * z] = row < rows && d < A.D ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+                        }
+                }
+                m[h] = -INFINITY; sum[h] = 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < DP / 8; u++) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.0f;
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        __syncwarp();
+        const int64_t key0 = at.tile * F::kTile + warp * KW;
+        const uint32_t ks = ring + stage * F::kStage, vs = ks + F::kHalf;
+        if (key0 < at.q.len) {
+            const bool few = rows <= 8;
+            float s[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+            if (E5M2) {
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int cc = 0; cc < DP / 64; cc++) {
+                        const uint4 w = lds16(ks + k_at(8 * j + g, 4 * cc + t));
+                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++)                    // e5m2 is the upper byte of fp16
+                            mma<false>(s[j], qf[4 * cc + k][0], qf[4 * cc + k][1], qf[4 * cc + k][2], qf[4 * cc + k][3], __byte_perm(x[k], 0u, 0x1404u), __byte_perm(x[k], 0u, 0x3424u));
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++) {
+                    uint32_t b[4];
+                    ldsm4<false>(b, ks + k_at((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                    mma<MBF>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                    mma<MBF>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                }
+            }
+            float corr[2], mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int h = e >> 1;
+                    s[j][e] = key0 + 8 * j + 2 * t + (e & 1) < see[h] ? s[j][e] * factor[h] : -INFINITY;
+                    mx[h] = fmaxf(mx[h], s[j][e]);
+                }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                const float to = fmaxf(m[h], mx[h]);
+                corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
+                m[h] = to;
+                sum[h] *= corr[h];
+            }
+            if (few) corr[1] = corr[0];                                // rows 8 .. 15 of the sums are the low parts of 0 .. 7
+            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+                for (int u = 0; u < DP / 8; u++) { o[u][0] *= corr[0]; o[u][1] *= corr[0]; o[u][2] *= corr[1]; o[u][3] *= corr[1]; }
+            }
+            const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+            uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float x = ex2(s[j][2 * h] - ref[h]), y = ex2(s[j][2 * h + 1] - ref[h]);
+                    sum[h] += x + y;
+                    split2<MBF>(x, y, hi[j][h], lo[j][h]);
+                }
+            // probabilities as two 16-bit values each; up to 8 rows the low parts are the products' other 8 rows, at no cost
+            auto values = [&](int j, float (&acc)[4], uint32_t b0, uint32_t b1) {
+                if (few) mma<MBF>(acc, hi[2 * j][0], lo[2 * j][0], hi[2 * j + 1][0], lo[2 * j + 1][0], b0, b1);
+                else {
+                    mma<MBF>(acc, lo[2 * j][0], lo[2 * j][1], lo[2 * j + 1][0], lo[2 * j + 1][1], b0, b1);
+                    mma<MBF>(acc, hi[2 * j][0], hi[2 * j][1], hi[2 * j + 1][0], hi[2 * j + 1][1], b0, b1);
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < NT / 2; j++) {                         // 16 keys
+                if (E5M2) {
+                    // column tile u holds elements (DP / 8) n + u, n = 0 .. 7: a lane's bytes of a row lie together
+                    constexpr int B = DP / 8, W = B / 4;
+                    uint32_t x[4][W];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
+                        if (B == 8) {
+                            const uint2 w = lds8(vs + v_at(row, g >> 1) + 8 * (g & 1));
+                            x[k][0] = w.x; x[k][1] = w.y;
+                        } else {
+#pragma unroll
+                            for (int z = 0; z < B / 16; z++) {
+                                const uint4 w = lds16(vs + v_at(row, g * (B / 16) + z));
+                                x[k][(4 * z) % W] = w.x; x[k][(4 * z + 1) % W] = w.y; x[k][(4 * z + 2) % W] = w.z; x[k][(4 * z + 3) % W] = w.w;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < DP / 8; u += 2) {
+                        const uint32_t sel = u & 2 ? 0x7362u : 0x5140u;
+                        const uint32_t p = __byte_perm(x[0][u / 4], x[1][u / 4], sel), q = __byte_perm(x[2][u / 4], x[3][u / 4], sel);
+                        values(j, o[u], __byte_perm(p, 0u, 0x1404u), __byte_perm(q, 0u, 0x1404u));
+                        values(j, o[u + 1], __byte_perm(p, 0u, 0x3424u), __byte_perm(q, 0u, 0x3424u));
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < DP / 8; u += 2) {
+                        uint32_t b[4];
+                        ldsm4<true>(b, vs + v_at(16 * j + (lane & 15), u + (lane >> 4)));
+                        values(j, o[u], b[0], b[1]);
+                        values(j, o[u + 1], b[2], b[3]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
+        // ---- the unit's last tile here: the warps' sums to one, divided and stored, or left for the merge
+        const bool whole = from_start && at.tile + 1 == at.tiles;
+        float* const part = A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+            if (t == 0) stats[warp * FEW_ROWS + g + 8 * h] = make_float2(m[h], sum[h]);
+        }
+        for (int h = 0; h < (rows > 8 ? 2 : 1); h++) {
+            float* const mine = sums + (warp * 8 + g) * DP;
+#pragma unroll
+            for (int u = 0; u < DP / 8; u++) {
+                const float x = rows > 8 ? (h ? o[u][2] : o[u][0]) : o[u][0] + o[u][2], y = rows > 8 ? (h ? o[u][3] : o[u][1]) : o[u][1] + o[u][3];
+                if (E5M2) { mine[2 * t * (DP / 8) + u] = x; mine[(2 * t + 1) * (DP / 8) + u] = y; }
+                else *reinterpret_cast<float2*>(mine + 8 * u + 2 * t) = make_float2(x, y);
+            }
+            __syncthreads();
+            for (int row = 8 * h + warp; row < rows && row < 8 * h + 8; row += NW) {
+                float top = -INFINITY, total = 0.0f, weight[NW];
+#pragma unroll
+                for (int w = 0; w < NW; w++) top = fmaxf(top, stats[w * FEW_ROWS + row].x);
+#pragma unroll
+                for (int w = 0; w < NW; w++) {
+                    const float2 st = stats[w * FEW_ROWS + row];
+                    weight[w] = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
+                    total += weight[w] * st.y;
+                }
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                const int token = row / group;
+                uint16_t* const dst = (uint16_t*)A.out + (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh;
+                for (int d = 4 * lane; d < DP; d += 128) {
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < NW; w++) {
+                        const float4 y = *reinterpret_cast<const float4*>(sums + (w * 8 + row - 8 * h) * DP + d);
+                        x.x = fmaf(weight[w], y.x, x.x); x.y = fmaf(weight[w], y.y, x.y); x.z = fmaf(weight[w], y.z, x.z); x.w = fmaf(weight[w], y.w, x.w);
+                    }
+                    if (whole) {
+                        if (d < A.D) store4<BF>(dst + d, x, inv);
+                    } else *reinterpret_cast<float4*>(part + row * DP + d) = x;
+                }
+                if (!whole && lane == 0) *reinterpret_cast<float2*>(part + FEW_ROWS * DP + 2 * row) = make_float2(top, total);
+            }
+            __syncthreads();
+        }
+        begun = false;
+        at.next(A, group, F::kTile);
+    }
+}
+
+// the units that began in block c and went on in others: their parts in the order of the keys
+template <int DP, bool BF, bool E5M2>
+__global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArgs A, int C) {
+    using F = Few<DP, E5M2>;
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    const int group = A.Hq / A.Hkv, c = blockIdx.x;
+    // written by what ran before the kernel in front, which has waited for it
+    const int64_t all = find_tile(A.R, [&](int r) { return few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
+                                  [&](int64_t n) { return share_begin(n, c + 1, C) - 1; }, scan, &found_r, &found_before);
+    if (all == 0) return;
+    const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
+    if (first == last) return;
+    const PagedReq q = paged_req(A, found_r);
+    const int64_t tiles = few_tiles(q, group, F::kTile);
+    const int hk = (int)((last - 1 - found_before) / tiles);
+    const int64_t from = found_before + hk * tiles, to = from + tiles;
+    if (from < first || to <= last) return;                            // began earlier, or ends here
+    const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int row = warp; row < rows; row += 8) {
+        auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
+        auto none = [&](int b) { return share_begin(all, b, C) == share_begin(all, b + 1, C); };
+        float top = -INFINITY;
+        for (int b = c; b <= end; b++)
+            if (!none(b)) top = fmaxf(top, slot(b)[FEW_ROWS * DP + 2 * row]);
+        float total = 0.0f;
+        float4 x[DP > 128 ? 2 : 1];
+#pragma unroll
+        for (int z = 0; z < (DP > 128 ? 2 : 1); z++) x[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int b = c; b <= end; b++) {
+            if (none(b)) continue;
+            const float* const p = slot(b);
+            const float2 st = *reinterpret_cast<const float2*>(p + FEW_ROWS * DP + 2 * row);
+            const float w = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
+            total = fmaf(w, st.y, total);
+#pragma unroll
+            for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
+                const int d = 4 * lane + 128 * z;
+                if (d >= DP) continue;
+                const float4 y = *reinterpret_cast<const float4*>(p + row * DP + d);
+                x[z].x = fmaf(w, y.x, x[z].x); x[z].y = fmaf(w, y.y, x[z].y); x[z].z = fmaf(w, y.z, x[z].z); x[z].w = fmaf(w, y.w, x[z].w);
+            }
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        uint16_t* const dst = (uint16_t*)A.out + (q.q0 + row / group) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
+#pragma unroll
+        for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
+            const int d = 4 * lane + 128 * z;
+            if (d < A.D) store4<BF>(dst + d, x[z], inv);
+        }
+    }
+}
+
 bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int unit) { return !((uintptr_t)p & 15) && !((a | b | c) & (unit - 1)); }
 
 // what both entry points refuse
@@ -92,15 +549,40 @@ int check(const PagedAttnArgs& A, const char* name) {
     return LB_OK;
 }
 
-int launch(const PagedAttnArgs& A, cudaStream_t st) {
+template <int DP, bool BF, bool E5M2> int few_launch(const PagedAttnArgs& A, cudaStream_t st) {
+    using F = Few<DP, E5M2>;
+    static bool configured[64] = {};                                   // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        cudaFuncSetAttribute(paged_few_kernel<DP, BF, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        configured[dev & 63] = true;
+    }
+    const int C = sm_count();
+    launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
+    note_launch();
+    launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C), 256, 0, st, true, A, C);
+    note_launch();
+    return check_launch();
+}
+template <int DP> int few_launch_types(const PagedAttnArgs& A, cudaStream_t st) {
+    if (A.cache_dtype == CACHE_E5M2) return A.dtype == DT_BF16 ? few_launch<DP, true, true>(A, st) : few_launch<DP, false, true>(A, st);
+    return A.dtype == DT_BF16 ? few_launch<DP, true, false>(A, st) : few_launch<DP, false, false>(A, st);
+}
+size_t few_part_bytes(int D) {
+    const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    return (size_t)sm_count() * 2 * (FEW_ROWS * dp + 2 * FEW_ROWS) * sizeof(float);
+}
+
+int simple_launch(const PagedAttnArgs& A, int above, cudaStream_t st) {
     const int64_t warps = A.T * A.Hq;
     const dim3 grid((unsigned)((warps + 3) / 4));
     if (A.dtype == DT_F16) {
-        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__half, true><<<grid, 128, 0, st>>>(A);
-        else paged_attention_simple_kernel<__half, false><<<grid, 128, 0, st>>>(A);
+        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__half, true><<<grid, 128, 0, st>>>(A, above);
+        else paged_attention_simple_kernel<__half, false><<<grid, 128, 0, st>>>(A, above);
     } else {
-        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__nv_bfloat16, true><<<grid, 128, 0, st>>>(A);
-        else paged_attention_simple_kernel<__nv_bfloat16, false><<<grid, 128, 0, st>>>(A);
+        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__nv_bfloat16, true><<<grid, 128, 0, st>>>(A, above);
+        else paged_attention_simple_kernel<__nv_bfloat16, false><<<grid, 128, 0, st>>>(A, above);
     }
     note_launch();
     return check_launch();
@@ -110,8 +592,8 @@ int launch(const PagedAttnArgs& A, cudaStream_t st) {
 }  // namespace lowbit
 
 extern "C" size_t lowbit_sdp_paged_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_query) {
-    (void)T; (void)R; (void)Hq; (void)Hkv; (void)D; (void)max_query;
-    return 0;
+    (void)T; (void)R; (void)Hq; (void)Hkv; (void)max_query;
+    return D > 0 && D <= 256 ? few_part_bytes(D) : 0;
 }
 
 extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t* q_strides, int64_t T, const void* d_k, const int64_t* k_strides,
@@ -120,7 +602,6 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
                                      int D, float scale, int64_t max_query, void* d_out, const int64_t* out_strides, void* workspace,
                                      size_t workspace_bytes, void* stream) {
     reset_launch_count();
-    (void)max_query; (void)workspace; (void)workspace_bytes;
     if (!d_table || !d_seq_lens || !q_strides || !k_strides || !v_strides || !out_strides || n_pages <= 0 || page_size <= 0 || width <= 0 || table_stride < width ||
         (int64_t)width * page_size > 0x7fffffffll) {
         set_error(LB_ERR_ARG, "lowbit_sdp_paged_cuda: bad argument (pages %d, page_size %d, width %d)", n_pages, page_size, width);
@@ -137,7 +618,15 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
     A.scale_log2e = scale * 1.4426950408889634f;
     if (const int rc = check(A, "lowbit_sdp_paged_cuda")) return rc;
     if (T == 0) return LB_OK;
-    return launch(A, (cudaStream_t)stream);
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_sdp_paged_workspace_size(T, R, Hq, Hkv, D, max_query)) {
+        set_error(LB_ERR_WORKSPACE, "lowbit_sdp_paged_cuda: a 16-byte aligned workspace of lowbit_sdp_paged_workspace_size() bytes is needed");
+        return LB_ERR_WORKSPACE;
+    }
+    A.part = (float*)workspace;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (const int rc = D <= 64 ? few_launch_types<64>(A, st) : D <= 128 ? few_launch_types<128>(A, st) : few_launch_types<256>(A, st)) return rc;
+    if (max_query * (Hq / Hkv) <= FEW_ROWS) return LB_OK;
+    return simple_launch(A, FEW_ROWS, st);
 }
 
 extern "C" size_t lowbit_sdp_packed_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_seqlen) {
@@ -166,5 +655,5 @@ extern "C" int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t*
     A.scale_log2e = scale * 1.4426950408889634f;
     if (const int rc = check(A, "lowbit_sdp_packed_cuda")) return rc;
     if (T == 0) return LB_OK;
-    return launch(A, (cudaStream_t)stream);
+    return simple_launch(A, 0, (cudaStream_t)stream);
 }
