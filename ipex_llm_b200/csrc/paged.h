@@ -37,6 +37,11 @@ __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& A, int r) {
     return q;
 }
 
+// paged_prompt.cu: requests with more than `above` rows (new tokens x heads of a group) a kv head
+int paged_prompt_max_group(int D);
+size_t paged_prompt_part_bytes(int D);
+int paged_prompt_launch(PagedAttnArgs A, int above, cudaStream_t st);
+
 // ---- work in equal shares.  The tiles of all units (a request's kv head; or a block of its rows on one) lie behind one another, n of them
 // in all, and block c of C takes tiles c n / C .. (c + 1) n / C: whatever the lengths, every block reads as many.  A unit whose tiles
 // lie in several blocks leaves its sums there, each block's slot 1 for a unit that began in it and slot 0 for one that did not, and the

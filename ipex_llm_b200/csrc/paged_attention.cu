@@ -1,77 +1,12 @@
 // paged_attention.cu -- attention of the new tokens of many requests over a paged cache, and of packed prompts over themselves:
 //   out[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - max),   j = the keys that token t of its request sees.
 // Token i of a request's n new ones, which holds len, sees keys 0 .. len - n + i; a token that sees none gives zeros.
-#include <type_traits>
 #include "paged.h"
 
 using namespace lowbit;
 
 namespace lowbit {
 namespace {
-
-// a warp per (token, query head): one pass over the keys with the running maximum and sum
-template <typename T, bool E5M2>
-__global__ void __launch_bounds__(128) paged_attention_simple_kernel(const PagedAttnArgs A, int above) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x * (int64_t)(blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t t = w / A.Hq;
-    const int h = (int)(w % A.Hq), hk = h / (A.Hq / A.Hkv);
-    if (t >= A.T) return;
-    int r = 0;
-    PagedReq q;
-    for (;; r++) {
-        if (r == A.R) return;                                   // behind the last request
-        q = paged_req(A, r);
-        if (t >= q.q0 && t < q.q0 + q.n) break;
-    }
-    if ((int64_t)q.n * (A.Hq / A.Hkv) <= above) return;
-    auto load = [&](const void* p, int64_t i) -> float {
-        if (sizeof(T) == 2 && E5M2) return decode_e5m2(((const uint8_t*)p)[i]);
-        if constexpr (std::is_same<T, __half>::value) return __half2float(((const __half*)p)[i]);
-        else return __bfloat162float(((const __nv_bfloat16*)p)[i]);
-    };
-    float x[8], o[8], m = -INFINITY, sum = 0.0f;
-    const int E = (A.D + 31) / 32;
-    for (int e = 0; e < 8; e++) {
-        const int d = lane + 32 * e;
-        x[e] = 0.0f; o[e] = 0.0f;
-        if (d < A.D) {
-            const int64_t at = t * A.q_st + h * A.q_sh + d;
-            if constexpr (std::is_same<T, __half>::value) x[e] = __half2float(((const __half*)A.q)[at]);
-            else x[e] = __bfloat162float(((const __nv_bfloat16*)A.q)[at]);
-        }
-    }
-    const int64_t i = t - q.q0, see = A.causal ? min((int64_t)q.len, q.len - q.n + i + 1) : q.len;
-    for (int64_t j = 0; j < see; j++) {
-        int64_t kb, vb;
-        bool bad = false;
-        if (A.table) {
-            const int pg = A.table[r * A.table_stride + j / A.page_size], in = (int)(j % A.page_size);
-            bad = pg < 0 || pg >= A.n_pages;
-            kb = bad ? 0 : pg * A.k_sp + in * A.k_ss + hk * A.k_sh;
-            vb = bad ? 0 : pg * A.v_sp + in * A.v_ss + hk * A.v_sh;
-        } else {
-            kb = (q.q0 + j) * A.k_ss + hk * A.k_sh;
-            vb = (q.q0 + j) * A.v_ss + hk * A.v_sh;
-        }
-        float s = 0.0f;
-        for (int e = 0; e < E; e++) { const int d = lane + 32 * e; if (d < A.D) s = fmaf(x[e], load(A.k, kb + d), s); }
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= A.scale_log2e;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : exp2f(m - mn), p = s == -INFINITY ? 0.0f : exp2f(s - mn);
-        sum = fmaf(sum, c, p);
-        for (int e = 0; e < E; e++) { const int d = lane + 32 * e; if (d < A.D) o[e] = fmaf(p, bad ? NAN : load(A.v, vb + d), o[e] * c); }
-        m = mn;
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    for (int e = 0; e < E; e++) {
-        const int d = lane + 32 * e;
-        if (d >= A.D) break;
-        const int64_t at = t * A.o_st + h * A.o_sh + d;
-        if constexpr (std::is_same<T, __half>::value) ((__half*)A.out)[at] = __float2half_rn(o[e] * inv);
-        else ((__nv_bfloat16*)A.out)[at] = __float2bfloat16_rn(o[e] * inv);
-    }
-}
 
 // ------------------------------------------------------------------ few rows (decoding): at most 16 rows = new tokens x heads of a group
 constexpr int FEW_ROWS = 16;
@@ -533,7 +468,7 @@ bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int unit) { return 
 
 // what both entry points refuse
 int check(const PagedAttnArgs& A, const char* name) {
-    if (!A.q || !A.k || !A.v || !A.cu || !A.out || A.R <= 0 || A.T < 0 || A.Hq <= 0 || A.Hkv <= 0 || A.Hq % A.Hkv || A.D <= 0 || A.D % 16 || A.D > 256 ||
+    if (!A.q || !A.k || !A.v || !A.cu || !A.out || A.R <= 0 || A.T < 0 || A.Hq <= 0 || A.Hkv <= 0 || A.Hq % A.Hkv || A.Hq / A.Hkv > paged_prompt_max_group(A.D) || A.D <= 0 || A.D % 16 || A.D > 256 ||
         (A.dtype != DT_F16 && A.dtype != DT_BF16) || (A.cache_dtype != A.dtype && !(A.table && A.cache_dtype == CACHE_E5M2)) || !(A.scale_log2e > 0.0f) ||
         A.T * A.Hq > 0x7fffffffll) {
         set_error(LB_ERR_ARG, "%s: bad argument (R %d, T %lld, Hq %d, Hkv %d, D %d, dtype %d, cache dtype %d)", name, A.R, (long long)A.T, A.Hq, A.Hkv, A.D, A.dtype,
@@ -574,26 +509,14 @@ size_t few_part_bytes(int D) {
     return (size_t)sm_count() * 2 * (FEW_ROWS * dp + 2 * FEW_ROWS) * sizeof(float);
 }
 
-int simple_launch(const PagedAttnArgs& A, int above, cudaStream_t st) {
-    const int64_t warps = A.T * A.Hq;
-    const dim3 grid((unsigned)((warps + 3) / 4));
-    if (A.dtype == DT_F16) {
-        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__half, true><<<grid, 128, 0, st>>>(A, above);
-        else paged_attention_simple_kernel<__half, false><<<grid, 128, 0, st>>>(A, above);
-    } else {
-        if (A.cache_dtype == CACHE_E5M2) paged_attention_simple_kernel<__nv_bfloat16, true><<<grid, 128, 0, st>>>(A, above);
-        else paged_attention_simple_kernel<__nv_bfloat16, false><<<grid, 128, 0, st>>>(A, above);
-    }
-    note_launch();
-    return check_launch();
-}
-
 }  // namespace
 }  // namespace lowbit
 
 extern "C" size_t lowbit_sdp_paged_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_query) {
-    (void)T; (void)R; (void)Hq; (void)Hkv; (void)max_query;
-    return D > 0 && D <= 256 ? few_part_bytes(D) : 0;
+    (void)T; (void)R;
+    if (D <= 0 || D > 256) return 0;
+    const size_t few = few_part_bytes(D);
+    return Hkv > 0 && max_query * (Hq / Hkv) <= FEW_ROWS ? few : few + paged_prompt_part_bytes(D);
 }
 
 extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t* q_strides, int64_t T, const void* d_k, const int64_t* k_strides,
@@ -626,12 +549,13 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
     cudaStream_t st = (cudaStream_t)stream;
     if (const int rc = D <= 64 ? few_launch_types<64>(A, st) : D <= 128 ? few_launch_types<128>(A, st) : few_launch_types<256>(A, st)) return rc;
     if (max_query * (Hq / Hkv) <= FEW_ROWS) return LB_OK;
-    return simple_launch(A, FEW_ROWS, st);
+    A.part = (float*)((uint8_t*)workspace + few_part_bytes(D));
+    return paged_prompt_launch(A, FEW_ROWS, st);
 }
 
 extern "C" size_t lowbit_sdp_packed_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_seqlen) {
-    (void)T; (void)R; (void)Hq; (void)Hkv; (void)D; (void)max_seqlen;
-    return 0;
+    (void)T; (void)R; (void)Hq; (void)Hkv; (void)max_seqlen;
+    return D > 0 && D <= 256 ? paged_prompt_part_bytes(D) : 0;
 }
 
 extern "C" int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t* q_strides, int64_t T, const void* d_k, const int64_t* k_strides,
@@ -639,7 +563,6 @@ extern "C" int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t*
                                       int causal, int64_t max_seqlen, void* d_out, const int64_t* out_strides, void* workspace, size_t workspace_bytes,
                                       void* stream) {
     reset_launch_count();
-    (void)max_seqlen; (void)workspace; (void)workspace_bytes;
     if (!q_strides || !k_strides || !v_strides || !out_strides || T > 0x7fffffffll) {
         set_error(LB_ERR_ARG, "lowbit_sdp_packed_cuda: bad argument (T %lld)", (long long)T);
         return LB_ERR_ARG;
@@ -655,5 +578,10 @@ extern "C" int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t*
     A.scale_log2e = scale * 1.4426950408889634f;
     if (const int rc = check(A, "lowbit_sdp_packed_cuda")) return rc;
     if (T == 0) return LB_OK;
-    return simple_launch(A, 0, (cudaStream_t)stream);
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_sdp_packed_workspace_size(T, R, Hq, Hkv, D, max_seqlen)) {
+        set_error(LB_ERR_WORKSPACE, "lowbit_sdp_packed_cuda: a 16-byte aligned workspace of lowbit_sdp_packed_workspace_size() bytes is needed");
+        return LB_ERR_WORKSPACE;
+    }
+    A.part = (float*)workspace;
+    return paged_prompt_launch(A, 0, (cudaStream_t)stream);
 }

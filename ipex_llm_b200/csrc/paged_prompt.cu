@@ -1,0 +1,699 @@
+// paged_prompt.cu -- attention of many rows: chunks of prompts over a paged cache, and packed prompts over themselves.
+//
+// A unit is NT tiles of 128 rows of one kv head; a request's rows there are (new token, head of the group), tokens first, so that all heads
+// that share a kv head share every key that is read.  Keys come in tiles of 128:
+//   S_t = Q_t . K^T   tcgen05.mma M = 128, N = 128, both operands in shared memory, S in tensor memory (lane = row);
+//   softmax           four warps a tile, a thread per row: the row's 128 scores in registers, P back into tensor memory over S;
+//   O_t += P_t . V    A operand = P in tensor memory, B operand = V as it lies in the cache (rows = keys: the MN-major descriptor).
+// Warps 0 .. 4 NT - 1: softmax; the next four copy keys and values into a ring of 128-byte swizzled tiles (cp.async, or e5m2 bytes expanded
+// to fp16 on the way), rows that a request does not hold as zeros; the next one issues the MMAs and owns the tensor memory.
+// Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
+#include "paged.h"
+#include "tc_common.cuh"
+
+using namespace lowbit;
+using namespace lowbit::gemmtc;
+
+namespace lowbit {
+namespace {
+
+constexpr int PR_KEYS = 128;
+
+template <int DP, bool E5M2> struct Prompt {
+    static constexpr int NT = DP == 256 ? 1 : 2, kRows = 128 * NT;
+    static constexpr int kTile = 128 * DP * 2, kSlots = DP == 256 ? 2 : DP == 128 ? 4 : 8;
+    static constexpr int kWarps = 4 * NT + 8;
+    static constexpr int kSmem = 1024 + (NT + kSlots) * kTile + 512;
+    // registers a thread: softmax, copies, MMAs (the launch's are 128 or 168)
+    static constexpr int kSoftRegs = NT == 2 ? 184 : 232, kCopyRegs = NT == 2 ? 80 : 144, kMmaRegs = NT == 2 ? 64 : 128;
+    static constexpr int64_t kPart = (int64_t)NT * 128 * (DP + 2);     // floats of a slot: [t][DP / 4][128] float4, [t][128] float2
+};
+
+__device__ __forceinline__ void tmem_ld32x(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32x(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16x(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16x(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// A operand in tensor memory
+__device__ __forceinline__ void umma_ts_w(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ------------------------------------------------------------------ the units and their key tiles
+// sum of floor((a i + b) / m) over i = 0 .. n - 1 (a, b >= 0), by the Euclidean exchange of a and m
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+    int64_t s = 0;
+    while (n > 0) {
+        if (a >= m) { s += (n - 1) * n / 2 * (a / m); a %= m; }
+        if (b >= m) { s += n * (b / m); b %= m; }
+        const int64_t y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const int64_t h = m; m = a; a = h;
+    }
+    return s;
+}
+struct Units {
+    int n, units, tpu, causal, off, len;                      // new tokens, units, tokens of a unit; keys before the first new token
+    __device__ __forceinline__ Units(const PagedReq& q, int group, int rows, int causal_, int above) {
+        tpu = rows / group;
+        causal = causal_;
+        n = (int64_t)q.n * group > above ? q.n : 0;
+        units = (n + tpu - 1) / tpu;
+        len = q.len;
+        off = q.len - q.n;
+    }
+    // key tiles of unit u: one at least, so that rows without keys are written too
+    __device__ __forceinline__ int tiles(int u) const {
+        const int end = causal ? off + min((u + 1) * tpu, n) : len;
+        return end <= PR_KEYS ? 1 : (end - 1) / PR_KEYS + 1;
+    }
+    // ... of the first u units
+    __device__ __forceinline__ int64_t before(int u) const {
+        if (u <= 0) return 0;
+        if (!causal) return (int64_t)u * tiles(0);
+        if (u >= units) return before(units - 1) + tiles(units - 1);
+        // those whose last token has at most PR_KEYS keys count one each: (i + 1) tpu + off <= PR_KEYS
+        const int room = PR_KEYS - off, ones = room < tpu ? 0 : min(u, room / tpu);
+        return ones + floor_sum(u - ones, PR_KEYS, tpu, off + (int64_t)(ones + 1) * tpu + PR_KEYS - 1);
+    }
+};
+// a block's way through its share: pieces of units, key tiles a .. b - 1 of unit (r, hk, u)
+struct PromptAt {
+    PagedReq q; int r, hk, u, units, tpu, a, b, tiles, left;
+    __device__ __forceinline__ void piece(const PagedAttnArgs& A, int group, int rows, int above) {
+        const Units w(q, group, rows, A.causal, above);
+        tiles = w.tiles(u);
+        b = min(tiles, a + left);
+        left -= b - a;
+    }
+    __device__ __forceinline__ bool next(const PagedAttnArgs& A, int group, int rows, int above) {
+        if (left <= 0) return false;
+        a = 0;
+        if (++u >= units) {
+            u = 0;
+            if (++hk >= A.Hkv) {
+                hk = 0;
+                do {
+                    if (++r >= A.R) return false;
+                    q = paged_req(A, r);
+                    units = Units(q, group, rows, A.causal, above).units;
+                } while (units == 0);
+            }
+        }
+        piece(A, group, rows, above);
+        return true;
+    }
+    // key tiles that the rows of tile t need, and whether the piece has any of them
+    __device__ __forceinline__ int tiles_of(const PagedAttnArgs& A, int group, int t) const {
+        const int first = u * tpu, end = min(first + tpu, q.n);
+        if (128 * t / group >= end - first) return 0;
+        const int last = min(first + (128 * t + 127) / group + 1, end);
+        const int keys = A.causal ? q.len - q.n + last : q.len;
+        return keys <= 0 ? 0 : (keys - 1) / PR_KEYS + 1;
+    }
+};
+// blocks that share n tiles: none takes less than a few, the price of a piece
+__device__ __forceinline__ int sharers(int64_t n, int C) { return (int)min((int64_t)C, (n + 1) / 2); }
+
+// the whole block: where tile `pick` of all lies; `all` = tiles of all units
+template <typename Pick>
+__device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group, int rows, int above, Pick pick, int64_t* scan, int* found_r, int64_t* found_before, PromptAt& at) {
+    int64_t want = 0;
+    const int64_t all = find_tile(A.R, [&](int r) { const Units w(paged_req(A, r), group, rows, A.causal, above); return w.before(w.units) * A.Hkv; },
+                                  [&](int64_t n) { return want = pick(n); }, scan, found_r, found_before);
+    if (all == 0 || want < 0) return all;
+    at.r = *found_r;
+    at.q = paged_req(A, at.r);
+    const Units w(at.q, group, rows, A.causal, above);
+    at.units = w.units;
+    at.tpu = w.tpu;
+    const int64_t per = w.before(w.units), x = want - *found_before;
+    at.hk = (int)(x / per);
+    const int64_t y = x % per;
+    // the last unit that begins at y or before: a warp's lanes look at 32 places at a time
+    int lo = 0, hi = w.units;                                          // before(lo) <= y < before(hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, u = lo + step * (int)(threadIdx.x & 31);
+        const uint32_t yes = __ballot_sync(0xffffffffu, u < hi && w.before(u) <= y);
+        lo += step * (31 - __clz(yes));
+        hi = min(hi, lo + step);
+    }
+    at.u = lo;
+    at.a = (int)(y - w.before(lo));
+    return all;
+}
+
+template <int DP, bool BF, bool E5M2, bool PAGED>
+__global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prompt_kernel(const PagedAttnArgs A, int above) {
+    using P = Prompt<DP, E5M2>;
+    constexpr int NT = P::NT, SLOTS = P::kSlots, TILE = P::kTile, HALF = 128 * 128;        // a tile is halves of 64 columns
+    constexpr bool MBF = BF && !E5M2;                                 // type in the products: fp16 over e5m2
+    extern __shared__ uint8_t pr_raw[];
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    const uint32_t base = (smem_u32(pr_raw) + 1023u) & ~1023u;
+    const uint32_t qs = base, ring = base + NT * TILE, bars = ring + SLOTS * TILE;
+    auto kv_full = [&](int s) { return bars + s * 8; };
+    auto kv_empty = [&](int s) { return bars + 64 + s * 8; };
+    auto s_full = [&](int t) { return bars + 128 + t * 8; };
+    auto p_full = [&](int t, int c) { return bars + 144 + (2 * t + c) * 8; };              // P of 64 keys
+    auto pv_done = [&](int t) { return bars + 176 + t * 8; };
+    auto q_full = [&](int t) { return bars + 192 + t * 8; };
+    auto o_free = [&](int t) { return bars + 208 + t * 8; };
+    const uint32_t drained = bars + 224, tmem_slot = bars + 232;
+    constexpr uint32_t TMEM_COLS = 512;                                // S_t at 128 t, O_t at 128 NT + DP t
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int group = A.Hq / A.Hkv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SLOTS; s++) { mbar_init(kv_full(s), 4); mbar_init(kv_empty(s), 1); }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(s_full(t), 1); mbar_init(p_full(t, 0), 4); mbar_init(p_full(t, 1), 4); mbar_init(pv_done(t), 1);
+            mbar_init(q_full(t), 4); mbar_init(o_free(t), 4);
+        }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4 * NT + 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (A.D < DP) {                                                    // columns behind D are never copied to
+        for (uint32_t i = threadIdx.x * 16; i < (uint32_t)((NT + SLOTS) * TILE); i += blockDim.x * 16) sts4(base + i, 0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    PromptAt at;
+    int C = gridDim.x;
+    const int c = blockIdx.x;
+    const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, gridDim.x); return c < C ? share_begin(n, c, C) : -1; }, scan, &found_r,
+                                   &found_before, at);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    // not before every block holds its columns: a dependent that allocates in front of its wait must find nobody who still wants some
+    asm volatile("griddepcontrol.launch_dependents;");
+    at.left = all > 0 && c < C ? (int)(share_begin(all, c + 1, C) - share_begin(all, c, C)) : 0;
+    const bool any = at.left > 0;
+    if (any) at.piece(A, group, P::kRows, above);
+
+    if (warp < 4 * NT) {
+        // ================= softmax: thread = row =================
+        regs_inc<P::kSoftRegs>();
+        const int t = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        const uint32_t st = tmem + lanes + t * 128, ot = tmem + lanes + NT * 128 + t * DP;
+        uint32_t steps = 0;                                            // key tiles so far
+        float mul = A.scale_log2e;
+        // the unit's queries into tile t: the products that read the last ones are done
+        auto queries = [&](const PromptAt& w) {
+            if (min(w.b, w.tiles_of(A, group, t)) <= w.a) return;      // no key of the piece for this tile: nobody waits for it
+            const int row = 128 * t + r, first = w.u * w.tpu, token = first + row / group;
+            const bool live = row < w.tpu * group && token < w.q.n;
+            const int64_t from = live ? (w.q.q0 + token) * A.q_st + (int64_t)(w.hk * group + row % group) * A.q_sh : -1;
+            const uint32_t dst = qs + t * TILE;
+            if (BF && E5M2) {
+                // bf16 enters as fp16, divided by a power of two that brings the row's largest value to 2^14: exact but for what lies 2^-28
+                // below it (fp16's last bit, 2^-24), where a 32-bit sum with that value ends too
+                const uint4* p = reinterpret_cast<const uint4*>((const uint16_t*)A.q + (live ? from : 0));
+                uint32_t big = 0;
+                for (int i = 0; i < A.D / 8; i++) {
+                    const uint4 w4 = live ? p[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t v[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) big = max(big, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
+                }
+                const int ex = (int)(big >> 7) - 127 - 14, e2 = big >= 0x7f80u || big == 0u ? 0 : ex < -100 ? -100 : ex;
+                const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+                mul = A.scale_log2e * __uint_as_float((uint32_t)(127 + e2) << 23);
+                for (int i = 0; i < A.D / 8; i++) {
+                    const uint4 w4 = live ? p[i] : make_uint4(0, 0, 0, 0);
+                    uint32_t v[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = h2u(__floats2half2_rn(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down));
+                    sts4(dst + (i >> 3) * HALF + r * 128 + (((i & 7) ^ (r & 7)) << 4), v[0], v[1], v[2], v[3]);
+                }
+            } else {
+                constexpr int CH = DP / 8, RP = 32 / CH;               // 16-byte pieces of a row, rows a pass
+#pragma unroll 4
+                for (int i = 0; i < 32 / RP; i++) {
+                    const int l = i * RP + lane / CH, piece = lane % CH, rr = 32 * quarter + l;
+                    const int64_t o = __shfl_sync(0xffffffffu, from, l);
+                    if (piece * 8 < A.D) cp16(dst + (piece >> 3) * HALF + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4), (const uint16_t*)A.q + (o < 0 ? 0 : o) + piece * 8, o < 0 ? 0u : 16u);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full(t));
+        };
+        if (any) {
+            queries(at);
+            for (bool more = true; more;) {
+                const int row = 128 * t + r, first = at.u * at.tpu, token = first + row / group;
+                const bool live = row < at.tpu * group && token < at.q.n;
+                const int off = at.q.len - at.q.n;
+                const int n_vis = !live ? 0 : A.causal ? off + token + 1 : at.q.len;       // keys the row sees
+                // keys below: every row of the warp sees them (rows behind the unit's are nobody's)
+                const int plain_end = A.causal ? off + first + (128 * t + 32 * quarter) / group + 1 : at.q.len;
+                const int end = min(at.b, at.tiles_of(A, group, t));
+                float m_ref = -INFINITY, sum = 0.0f;
+                for (int j = at.a; j < end; j++, steps++) {
+                    if (!mbar_wait_lim(s_full(t), steps & 1, A.waits)) goto done;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    float x[128];
+#pragma unroll
+                    for (int i = 0; i < 128; i += 32) tmem_ld32x(st + i, x + i);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (j >= plain_end / PR_KEYS) {
+                        const int left = n_vis - j * PR_KEYS;
+#pragma unroll
+                        for (int i = 0; i < 128; i++) x[i] = i < left ? x[i] : -INFINITY;
+                    }
+                    float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+#pragma unroll
+                    for (int i = 4; i < 128; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
+                    const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * mul;
+                    const bool grow = mx > m_ref + 6.0f;                           // -inf: any visible key
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float m_new = grow ? mx : m_ref;
+                        if (j > at.a) {
+                            // the P . V before this Q . K is done: O is at rest
+                            const float corr = grow ? ex2(m_ref - m_new) : 1.0f;
+                            sum *= corr;
+#pragma unroll 1
+                            for (int i = 0; i < DP; i += 16) {
+                                float o[16];
+                                tmem_ld16x(ot + i, o);
+                                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                                for (int e = 0; e < 16; e++) o[e] *= corr;
+                                tmem_st16x(ot + i, reinterpret_cast<const uint32_t*>(o));
+                            }
+                        }
+                        m_ref = m_new;
+                    }
+                    // fp16: 2^8 above the reference's place, so that values from 2^-24 to 2^14 of it are normal numbers or close
+                    const float shift = (MBF ? 0.0f : 8.0f) - (m_ref == -INFINITY ? 0.0f : m_ref);
+                    float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const int k = 64 * h + 2 * i;
+                            const float p0 = ex2(fmaf(x[k], mul, shift)), p1 = ex2(fmaf(x[k + 1], mul, shift));
+                            const float p2 = ex2(fmaf(x[k + 2], mul, shift)), p3 = ex2(fmaf(x[k + 3], mul, shift));
+                            a0 += p0; a1 += p1; a2 += p2; a3 += p3;
+                            p[i] = pack2<MBF>(p0, p1);
+                            p[i + 1] = pack2<MBF>(p2, p3);
+                        }
+                        tmem_st32x(st + 32 * h, p);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_full(t, h));
+                    }
+                    sum += (a0 + a1) + (a2 + a3);
+                }
+                // the next unit's queries, while this one's last product runs
+                const PromptAt was = at;
+                more = at.next(A, group, P::kRows, above);
+                if (more) queries(at);
+                const bool some = end > was.a, whole = was.a == 0 && was.b == was.tiles;
+                if (some) {
+                    if (!mbar_wait_lim(pv_done(t), (steps - 1) & 1, A.waits)) goto done;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;                 // a row without a key gives zeros
+                const int64_t oi = (was.q.q0 + token) * A.o_st + (int64_t)(was.hk * group + row % group) * A.o_sh;
+                float* const part = A.part + ((int64_t)c * 2 + (was.a == 0 ? 1 : 0)) * P::kPart;
+#pragma unroll 1
+                for (int i = 0; i < DP; i += 32) {
+                    float o[32];
+                    if (some) {
+                        tmem_ld32x(ot + i, o);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.0f;
+                    }
+                    if (whole) {
+                        if (live) {
+                            uint4* p = reinterpret_cast<uint4*>((uint16_t*)A.out + oi + i);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (i + 8 * e < A.D)
+                                    p[e] = make_uint4(pack2<BF>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<BF>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                                      pack2<BF>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<BF>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                        }
+                    } else if (some) {
+                        float4* p = reinterpret_cast<float4*>(part) + (int64_t)(t * (DP / 4) + i / 4) * 128 + r;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) p[e * 128] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (!whole) reinterpret_cast<float2*>(part + (int64_t)NT * 128 * DP)[t * 128 + r] = make_float2(m_ref, sum);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (some && lane == 0) mbar_arrive(o_free(t));
+            }
+        }
+    } else if (warp < 4 * NT + 4) {
+        // ================= keys and values into the ring =================
+        regs_dec<P::kCopyRegs>();
+        const int w0 = 32 * (warp - 4 * NT);                           // this warp's rows of a tile: lane = row
+        constexpr int CH = E5M2 ? DP / 16 : DP / 8, RP = 32 / CH, PASSES = 32 / RP;
+        const int live = A.D * (E5M2 ? 1 : 2) / 16, piece = lane % CH;
+        int j = at.a;
+        int64_t ko = 0, vo = 0;
+        uint32_t state = 0;                                            // of this lane's key: none, there, in no page
+        int page = 0;
+        bool more = any;
+        auto ask = [&]() {
+            const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
+            if (PAGED && more && key < at.q.len) page = A.table[at.r * A.table_stride + (int)key / A.page_size];
+        };
+        auto place = [&]() {                                           // of this lane's key, and on to the next tile
+            const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
+            const bool here = key < at.q.len;
+            if (PAGED) {
+                const bool bad = here && (page < 0 || page >= A.n_pages);
+                const int row = (int)key % A.page_size;
+                state = here ? bad ? 2u : 1u : 0u;
+                ko = state == 1 ? page * A.k_sp + row * A.k_ss + at.hk * A.k_sh : 0;
+                vo = state == 1 ? page * A.v_sp + row * A.v_ss + at.hk * A.v_sh : 0;
+            } else {
+                state = here ? 1u : 0u;
+                ko = here ? (at.q.q0 + key) * A.k_ss + at.hk * A.k_sh : 0;
+                vo = here ? (at.q.q0 + key) * A.v_ss + at.hk * A.v_sh : 0;
+            }
+            if (++j >= at.b) {
+                more = at.next(A, group, P::kRows, above);
+                j = at.a;
+            }
+            ask();
+        };
+        const uint32_t total = any ? (uint32_t)(share_begin(all, c + 1, C) - share_begin(all, c, C)) : 0u, items = A.waits.limit < 0 ? total : 2 * total;
+        ask();
+        if (E5M2) {
+            uint4 w[PASSES];
+            auto fetch = [&](uint32_t item) {
+                if (!(item & 1)) place();
+                const uint8_t* const src = (const uint8_t*)((item & 1) ? A.v : A.k);
+                const uint32_t none = (item & 1) ? 0x7f7f7f7fu : 0u;
+#pragma unroll
+                for (int i = 0; i < PASSES; i++) {
+                    const int l = i * RP + lane / CH;
+                    const int64_t o = __shfl_sync(0xffffffffu, (item & 1) ? vo : ko, l);
+                    const uint32_t s = __shfl_sync(0xffffffffu, state, l);
+                    const uint32_t z = s == 2 ? none : 0u;
+                    w[i] = make_uint4(z, z, z, z);
+                    if (s == 1 && piece < live) w[i] = *reinterpret_cast<const uint4*>(src + o + piece * 16);
+                }
+            };
+            if (items > 0) fetch(0);
+            for (uint32_t item = 0; item < items; item++) {
+                const int s = item % SLOTS;
+                const uint32_t round = item / SLOTS;
+                if (!mbar_wait_lim(kv_empty(s), (round & 1) ^ 1, A.waits)) goto done;
+                const uint32_t dst = ring + s * TILE + (piece >> 2) * HALF;
+                const int c0 = 2 * (piece & 3);
+#pragma unroll
+                for (int i = 0; i < PASSES; i++) {
+                    const int rr = w0 + i * RP + lane / CH;
+                    const uint32_t a = dst + rr * 128 + ((c0 ^ (rr & 7)) << 4), b = dst + rr * 128 + (((c0 + 1) ^ (rr & 7)) << 4);
+                    if (piece < live) {                                // e5m2 is the upper byte of fp16
+                        sts4(a, __byte_perm(w[i].x, 0u, 0x1404u), __byte_perm(w[i].x, 0u, 0x3424u), __byte_perm(w[i].y, 0u, 0x1404u), __byte_perm(w[i].y, 0u, 0x3424u));
+                        sts4(b, __byte_perm(w[i].z, 0u, 0x1404u), __byte_perm(w[i].z, 0u, 0x3424u), __byte_perm(w[i].w, 0u, 0x1404u), __byte_perm(w[i].w, 0u, 0x3424u));
+                    }
+                }
+                if (item + 1 < items) fetch(item + 1);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kv_full(s));
+            }
+        } else {
+            constexpr int AHEAD = SLOTS > 2 ? 2 : 1;                   // items under way behind the one that is waited for
+            auto copy = [&](uint32_t item) {
+                if (!(item & 1)) place();
+                const uint32_t dst = ring + item % SLOTS * TILE + (piece >> 3) * HALF;
+                const uint16_t* const src = (const uint16_t*)((item & 1) ? A.v : A.k);
+#pragma unroll 8
+                for (int i = 0; i < PASSES; i++) {
+                    const int l = i * RP + lane / CH, rr = w0 + l;
+                    const int64_t o = __shfl_sync(0xffffffffu, (item & 1) ? vo : ko, l);
+                    const uint32_t s = __shfl_sync(0xffffffffu, state, l), a = dst + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
+                    if (piece < live) {
+                        if (PAGED && s == 2 && (item & 1)) sts4(a, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);     // no such page: not a number
+                        else cp16(a, src + o + piece * 8, s == 1 ? 16u : 0u);
+                    }
+                }
+            };
+            uint32_t told = 0;                                         // items that have been handed over
+            auto hand_over = [&](uint32_t upto) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                for (; told < upto; told++)
+                    if (lane == 0) mbar_arrive(kv_full(told % SLOTS));
+            };
+            for (uint32_t item = 0; item < items; item++) {
+                const uint32_t empty = kv_empty(item % SLOTS), parity = ((item / SLOTS) & 1) ^ 1;
+                if (!__all_sync(0xffffffffu, mbar_test(empty, parity))) {          // who holds the slot may wait for what is under way
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    hand_over(item);
+                    if (!mbar_wait_lim(empty, parity, A.waits)) goto done;
+                }
+                copy(item);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+                if (item >= AHEAD && told < item + 1 - AHEAD) hand_over(item + 1 - AHEAD);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            hand_over(items);
+        }
+    } else {
+        regs_dec<P::kMmaRegs>();
+        if (warp == 4 * NT + 4 && any) {
+            // ================= MMA issuer: the whole warp runs the loop, one elected lane issues =================
+            const uint32_t leader = elect_leader();
+            // c F32, a / b fp16 or bf16, M = 128; S: N = 128, both operands K-major; O: N = DP, A in TMEM, B (values) MN-major (bit 16)
+            const uint32_t id = (1u << 4) | (MBF ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 4) << 24);
+            const uint32_t id_s = id | ((128u >> 3) << 17), id_o = id | (((uint32_t)DP >> 3) << 17) | (1u << 16);
+            uint32_t steps[2] = {0, 0}, turns[2] = {0, 0};              // key tiles, and pieces with any, of a tile so far
+            uint32_t item = 0;                                         // of the piece's first keys
+            auto slot = [&](uint32_t i) { return ring + i % SLOTS * TILE; };
+            auto arrived = [&](uint32_t i) { return mbar_wait_lim(kv_full(i % SLOTS), (i / SLOTS) & 1, A.waits); };
+            auto scores = [&](int t, uint32_t i) {
+                const uint64_t qd = make_desc(qs + t * TILE), kd = make_desc(slot(i));
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++) {
+                    const uint64_t step = (uint64_t)(((k >> 2) * HALF + (k & 3) * 32) >> 4);
+                    umma_f16_w(tmem + t * 128, qd + step, kd + step, id_s, k > 0 ? 1u : 0u, leader);
+                }
+                umma_commit_w(s_full(t), leader);
+            };
+            auto values = [&](int t, uint32_t i, int h, bool fresh) {   // 64 keys
+                // V tile: element (d, key) at half(d / 64), row key: LBO = the next 64 d, SBO = the next 8 keys; 16 keys a step
+                const uint64_t vd = (make_desc(slot(i)) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(HALF >> 4) << 16);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 32 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 0 && k == 0 ? 0u : 1u, leader);
+            };
+            for (;;) {
+                const int a = at.a, b = at.b;
+                const int end[2] = {min(b, at.tiles_of(A, group, 0)), NT == 2 ? min(b, at.tiles_of(A, group, 1)) : 0};
+                if (!arrived(item)) goto done;
+                for (int t = 0; t < NT; t++) {
+                    if (end[t] <= a) continue;
+                    if (!mbar_wait_lim(q_full(t), turns[t] & 1, A.waits)) goto done;
+                    if (steps[t] > 0 && !mbar_wait_lim(pv_done(t), (steps[t] - 1) & 1, A.waits)) goto done;      // S and P share their columns
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    scores(t, item);
+                }
+                umma_commit_w(kv_empty(item % SLOTS), leader);
+                for (int j = a; j < b; j++, item += 2) {
+                    if (!arrived(item + 1)) goto done;
+                    for (int t = 0; t < NT; t++) {
+                        if (j >= end[t]) continue;
+                        if (j == a && turns[t]++ > 0 && !mbar_wait_lim(o_free(t), turns[t] & 1, A.waits)) goto done;
+                        for (int h = 0; h < 2; h++) {
+                            if (!mbar_wait_lim(p_full(t, h), steps[t] & 1, A.waits)) goto done;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            values(t, item + 1, h, j == a);
+                        }
+                        umma_commit_w(pv_done(t), leader);
+                        steps[t]++;
+                        if (j + 1 < end[t]) {
+                            if (!arrived(item + 2) || !mbar_wait_lim(pv_done(t), (steps[t] - 1) & 1, A.waits)) goto done;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            scores(t, item + 2);
+                        }
+                    }
+                    umma_commit_w(kv_empty((item + 1) % SLOTS), leader);
+                    if (j + 1 < b) {
+                        if (!arrived(item + 2)) goto done;
+                        umma_commit_w(kv_empty((item + 2) % SLOTS), leader);
+                    }
+                }
+                if (!at.next(A, group, P::kRows, above)) break;
+            }
+        }
+    }
+done:
+    asm volatile("cp.async.wait_all;" ::: "memory");                   // behind a wait that ran out copies may still be under way
+    __syncwarp();
+    if (warp == 4 * NT + 4) {
+        // ... and MMAs: nobody leaves their memory
+        const uint32_t leader = elect_leader();
+        umma_commit_w(drained, leader);
+        mbar_wait_lim(drained, 0u, Waits{A.waits.word, kWaitCycles});
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 4 * NT + 4) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// the units that began in block c and went on in others: their parts in the order of the keys.  A thread per row, a quarter of the columns a block
+template <int DP, bool BF, bool E5M2>
+__global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_kernel(const PagedAttnArgs A, int above, int blocks) {
+    using P = Prompt<DP, E5M2>;
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    const int group = A.Hq / A.Hkv, c = blockIdx.x;
+    int C = blocks;
+    PromptAt at;
+    // written by what ran before the kernel in front, which has waited for it
+    const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, blocks); return c < C ? share_begin(n, c + 1, C) - 1 : -1; }, scan, &found_r,
+                                   &found_before, at);
+    if (all == 0 || c >= C) return;
+    const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
+    if (first == last) return;
+    const int64_t tiles = Units(at.q, group, P::kRows, A.causal, above).tiles(at.u), from = last - 1 - at.a, to = from + tiles;
+    if (from < first || to <= last) return;                            // began earlier, or ends here
+    const int end = share_of(to - 1, all, C), t = threadIdx.x >> 7, r = threadIdx.x & 127, row = threadIdx.x, token = at.u * at.tpu + row / group;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (row >= at.tpu * group || token >= at.q.n) return;
+    auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * P::kPart; };
+    auto stat = [&](int b) { return reinterpret_cast<const float2*>(slot(b) + (int64_t)P::NT * 128 * DP)[t * 128 + r]; };
+    float top = -INFINITY, total = 0.0f;
+    for (int b = c; b <= end; b++) top = fmaxf(top, stat(b).x);
+    for (int b = c; b <= end; b++) {
+        const float2 s = stat(b);
+        if (s.y != 0.0f) total = fmaf(s.x == -INFINITY ? s.y : ex2(s.x - top), s.y, total);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* const dst = (uint16_t*)A.out + (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh;
+    const int per = DP / gridDim.y, d0 = blockIdx.y * per;
+    for (int d = d0; d < d0 + per && d < A.D; d += 8) {
+        float x[8] = {};
+        for (int b = c; b <= end; b++) {
+            const float2 s = stat(b);
+            if (s.y == 0.0f) continue;                                 // no key for this row: nothing was stored
+            const float w = s.x == -INFINITY ? s.y : ex2(s.x - top);
+            const float4* p = reinterpret_cast<const float4*>(slot(b)) + (int64_t)(t * (DP / 4) + d / 4) * 128 + r;
+            const float4 y = p[0], z = p[128];
+            x[0] = fmaf(w, y.x, x[0]); x[1] = fmaf(w, y.y, x[1]); x[2] = fmaf(w, y.z, x[2]); x[3] = fmaf(w, y.w, x[3]);
+            x[4] = fmaf(w, z.x, x[4]); x[5] = fmaf(w, z.y, x[5]); x[6] = fmaf(w, z.z, x[6]); x[7] = fmaf(w, z.w, x[7]);
+        }
+        *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack2<BF>(x[0] * inv, x[1] * inv), pack2<BF>(x[2] * inv, x[3] * inv), pack2<BF>(x[4] * inv, x[5] * inv),
+                                                        pack2<BF>(x[6] * inv, x[7] * inv));
+    }
+}
+
+template <int DP, bool BF, bool E5M2, bool PAGED> int launch(const PagedAttnArgs& A, int above, cudaStream_t st) {
+    using P = Prompt<DP, E5M2>;
+    static bool configured[64] = {};                                   // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        cudaFuncSetAttribute(paged_prompt_kernel<DP, BF, E5M2, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
+        configured[dev & 63] = true;
+    }
+    const int C = sm_count();
+    launch_behind(paged_prompt_kernel<DP, BF, E5M2, PAGED>, dim3((unsigned)C), P::kWarps * 32, P::kSmem, st, launch_overlaps(st), A, above);
+    note_launch();
+    launch_behind(paged_prompt_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, 4), P::kRows, 0, st, true, A, above, C);
+    note_launch();
+    return check_launch();
+}
+template <int DP> int launch_types(const PagedAttnArgs& A, int above, cudaStream_t st) {
+    if (!A.table) return A.dtype == DT_BF16 ? launch<DP, true, false, false>(A, above, st) : launch<DP, false, false, false>(A, above, st);
+    if (A.cache_dtype == CACHE_E5M2) return A.dtype == DT_BF16 ? launch<DP, true, true, true>(A, above, st) : launch<DP, false, true, true>(A, above, st);
+    return A.dtype == DT_BF16 ? launch<DP, true, false, true>(A, above, st) : launch<DP, false, false, true>(A, above, st);
+}
+
+}  // namespace
+
+int paged_prompt_max_group(int D) { return D <= 128 ? 256 : 128; }
+size_t paged_prompt_part_bytes(int D) {
+    const int64_t floats = D <= 64 ? Prompt<64, false>::kPart : D <= 128 ? Prompt<128, false>::kPart : Prompt<256, false>::kPart;
+    return (size_t)sm_count() * 2 * floats * sizeof(float);
+}
+int paged_prompt_launch(PagedAttnArgs A, int above, cudaStream_t st) {
+    if (const int rc = make_waits(&A.waits, kWaitCycles)) return rc;
+    return A.D <= 64 ? launch_types<64>(A, above, st) : A.D <= 128 ? launch_types<128>(A, above, st) : launch_types<256>(A, above, st);
+}
+
+}  // namespace lowbit
