@@ -46,8 +46,38 @@ int paged_prompt_launch(PagedAttnArgs A, int above, cudaStream_t st);
 // in all, and block c of C takes tiles c n / C .. (c + 1) n / C: whatever the lengths, every block reads as many.  A unit whose tiles
 // lie in several blocks leaves its sums there, each block's slot 1 for a unit that began in it and slot 0 for one that did not, and the
 // merge adds them up in the order of the keys.
-__host__ __device__ inline int64_t share_begin(int64_t n, int c, int C) { return n * c / C; }
-__host__ __device__ inline int share_of(int64_t tile, int64_t n, int C) { return (int)(((tile + 1) * C - 1) / n); }      // the block that takes a tile
+// Divisions are written out in 32 bits: a 64-bit one is a call, and a kernel that calls anything keeps the registers of its launch
+// (setmaxnreg is ignored).
+__device__ __forceinline__ uint64_t div_small(uint64_t n, uint32_t d, uint32_t& rem) {      // d < 2^16, 16 bits at a time
+    uint64_t q = 0;
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 48; i >= 0; i -= 16) {
+        const uint32_t x = r << 16 | ((uint32_t)(n >> i) & 0xffffu);
+        q = q << 16 | x / d;
+        r = x % d;
+    }
+    rem = r;
+    return q;
+}
+__device__ __forceinline__ int64_t share_begin(int64_t n, int c, int C) {
+    uint32_t rem;
+    const uint64_t q = div_small((uint64_t)n, (uint32_t)C, rem);
+    return (int64_t)q * c + rem * (uint32_t)c / (uint32_t)C;
+}
+__device__ __forceinline__ int share_of(int64_t tile, int64_t n, int C) {                   // the block that takes a tile
+    int c = min(C - 1, (int)(__fdividef((float)tile, (float)n) * (float)C));
+    while (c > 0 && share_begin(n, c, C) > tile) c--;
+    while (c + 1 < C && share_begin(n, c + 1, C) <= tile) c++;
+    return c;
+}
+__device__ __forceinline__ int div_few(int64_t x, int64_t y, int64_t& rem) {                // a quotient of a few thousand at most
+    int q = (int)__fdividef((float)x, (float)y);
+    while (q > 0 && q * y > x) q--;
+    while ((q + 1) * y <= x) q++;
+    rem = x - q * y;
+    return q;
+}
 
 // sum over the block before this thread, and of all of it
 __device__ __forceinline__ int64_t block_before(int64_t x, int64_t* warps, int64_t& total) {

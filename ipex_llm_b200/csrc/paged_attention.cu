@@ -127,8 +127,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     at.r = found_r;
     at.q = paged_req(A, at.r);
     at.tiles = few_tiles(at.q, group, F::kTile);
-    at.hk = (int)((first - found_before) / at.tiles);
-    at.tile = (first - found_before) % at.tiles;
+    at.hk = div_few(first - found_before, at.tiles, at.tile);
     FewAt in = at;                                                     // of the copies
 
     const uint32_t ring = smem_addr(few_smem) + warp * ST * F::kStage;
@@ -425,7 +424,8 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
     if (first == last) return;
     const PagedReq q = paged_req(A, found_r);
     const int64_t tiles = few_tiles(q, group, F::kTile);
-    const int hk = (int)((last - 1 - found_before) / tiles);
+    int64_t within;
+    const int hk = div_few(last - 1 - found_before, tiles, within);
     const int64_t from = found_before + hk * tiles, to = from + tiles;
     if (from < first || to <= last) return;                            // began earlier, or ends here
     const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -8,6 +8,7 @@
 // Warps 0 .. 4 NT - 1: softmax; the next four copy keys and values into a ring of 128-byte swizzled tiles (cp.async, or e5m2 bytes expanded
 // to fp16 on the way), rows that a request does not hold as zeros; the next one issues the MMAs and owns the tensor memory.
 // Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
+#include <string.h>
 #include "paged.h"
 #include "tc_common.cuh"
 
@@ -25,7 +26,7 @@ template <int DP, bool E5M2> struct Prompt {
     static constexpr int kWarps = 4 * NT + 8;
     static constexpr int kSmem = 1024 + (NT + kSlots) * kTile + 512;
     // registers a thread: softmax, copies, MMAs (the launch's are 128 or 168)
-    static constexpr int kSoftRegs = NT == 2 ? 184 : 232, kCopyRegs = NT == 2 ? 80 : 144, kMmaRegs = NT == 2 ? 64 : 128;
+    static constexpr int kSoftRegs = NT == 2 ? 152 : 232, kCopyRegs = NT == 2 ? 104 : 144, kMmaRegs = NT == 2 ? 104 : 128;
     static constexpr int64_t kPart = (int64_t)NT * 128 * (DP + 2);     // floats of a slot: [t][DP / 4][128] float4, [t][128] float2
 };
 
@@ -92,16 +93,16 @@ template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setm
 
 // ------------------------------------------------------------------ the units and their key tiles
 // sum of floor((a i + b) / m) over i = 0 .. n - 1 (a, b >= 0), by the Euclidean exchange of a and m
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+__device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     int64_t s = 0;
     while (n > 0) {
-        if (a >= m) { s += (n - 1) * n / 2 * (a / m); a %= m; }
-        if (b >= m) { s += n * (b / m); b %= m; }
-        const int64_t y = a * n + b;
+        if (a >= m) { s += (int64_t)n * (n - 1) / 2 * (a / m); a %= m; }
+        if (b >= m) { s += (int64_t)n * (b / m); b %= m; }
+        const uint32_t y = a * n + b;                                  // at most the tokens of a request
         if (y < m) break;
         n = y / m;
         b = y % m;
-        const int64_t h = m; m = a; a = h;
+        const uint32_t h = m; m = a; a = h;
     }
     return s;
 }
@@ -124,10 +125,11 @@ struct Units {
     __device__ __forceinline__ int64_t before(int u) const {
         if (u <= 0) return 0;
         if (!causal) return (int64_t)u * tiles(0);
-        if (u >= units) return before(units - 1) + tiles(units - 1);
+        const int last = u >= units ? tiles(units - 1) : 0;            // which may have fewer tokens
+        if (u >= units) u = units - 1;
         // those whose last token has at most PR_KEYS keys count one each: (i + 1) tpu + off <= PR_KEYS
         const int room = PR_KEYS - off, ones = room < tpu ? 0 : min(u, room / tpu);
-        return ones + floor_sum(u - ones, PR_KEYS, tpu, off + (int64_t)(ones + 1) * tpu + PR_KEYS - 1);
+        return last + ones + floor_sum(u - ones, PR_KEYS, tpu, (uint32_t)off + (uint32_t)(ones + 1) * tpu + PR_KEYS - 1);
     }
 };
 // a block's way through its share: pieces of units, key tiles a .. b - 1 of unit (r, hk, u)
@@ -166,7 +168,7 @@ struct PromptAt {
     }
 };
 // blocks that share n tiles: none takes less than a few, the price of a piece
-__device__ __forceinline__ int sharers(int64_t n, int C) { return (int)min((int64_t)C, (n + 1) / 2); }
+__device__ __forceinline__ int sharers(int64_t n, int C) { return (int)min((int64_t)C, (n + 1) >> 1); }
 
 // the whole block: where tile `pick` of all lies; `all` = tiles of all units
 template <typename Pick>
@@ -181,8 +183,8 @@ __device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group,
     at.units = w.units;
     at.tpu = w.tpu;
     const int64_t per = w.before(w.units), x = want - *found_before;
-    at.hk = (int)(x / per);
-    const int64_t y = x % per;
+    int64_t y;
+    at.hk = div_few(x, per, y);
     // the last unit that begins at y or before: a warp's lanes look at 32 places at a time
     int lo = 0, hi = w.units;                                          // before(lo) <= y < before(hi)
     while (hi - lo > 1) {
@@ -196,8 +198,11 @@ __device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group,
     return all;
 }
 
+// keys and values in the order of their tensor maps: [D][rows of a page][heads][pages], or [D][heads][tokens]
+struct PromptMaps { CUtensorMap k, v; };
+
 template <int DP, bool BF, bool E5M2, bool PAGED>
-__global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prompt_kernel(const PagedAttnArgs A, int above) {
+__global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prompt_kernel(const PagedAttnArgs A, const __grid_constant__ PromptMaps M, int box, int above) {
     using P = Prompt<DP, E5M2>;
     constexpr int NT = P::NT, SLOTS = P::kSlots, TILE = P::kTile, HALF = 128 * 128;        // a tile is halves of 64 columns
     constexpr bool MBF = BF && !E5M2;                                 // type in the products: fp16 over e5m2
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     PromptAt at;
-    int C = gridDim.x;
+    int C = gridDim.x, issued = 0;
     const int c = blockIdx.x;
     const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, gridDim.x); return c < C ? share_begin(n, c, C) : -1; }, scan, &found_r,
                                    &found_before, at);
@@ -317,18 +322,27 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 for (int j = at.a; j < end; j++, steps++) {
                     if (!mbar_wait_lim(s_full(t), steps & 1, A.waits)) goto done;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    float x[128];
+                    // 64 scores in registers at a time (128 spilled): the maximum of the first half, of the second, whose exponentials
+                    // follow at once, then those of the first, read again
+                    const bool plain = j < plain_end / PR_KEYS;
+                    const int left = n_vis - j * PR_KEYS;
+                    float x[64], m0, m1, m2, m3;
+                    auto load = [&](int h) {
+                        tmem_ld32x(st + 64 * h, x);
+                        tmem_ld32x(st + 64 * h + 32, x + 32);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (!plain) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += 32) tmem_ld32x(st + i, x + i);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (j >= plain_end / PR_KEYS) {
-                        const int left = n_vis - j * PR_KEYS;
+                            for (int i = 0; i < 64; i++) x[i] = 64 * h + i < left ? x[i] : -INFINITY;
+                        }
+                    };
+                    load(0);
+                    m0 = x[0]; m1 = x[1]; m2 = x[2]; m3 = x[3];
 #pragma unroll
-                        for (int i = 0; i < 128; i++) x[i] = i < left ? x[i] : -INFINITY;
-                    }
-                    float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
+                    for (int i = 4; i < 64; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
+                    load(1);
 #pragma unroll
-                    for (int i = 4; i < 128; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
+                    for (int i = 0; i < 64; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
                     const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * mul;
                     const bool grow = mx > m_ref + 6.0f;                           // -inf: any visible key
                     if (__any_sync(0xffffffffu, grow)) {
@@ -352,24 +366,26 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                     // fp16: 2^8 above the reference's place, so that values from 2^-24 to 2^14 of it are normal numbers or close
                     const float shift = (MBF ? 0.0f : 8.0f) - (m_ref == -INFINITY ? 0.0f : m_ref);
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    // P of a half goes where its scores were
+                    auto exponentials = [&](int h) {
                         uint32_t p[32];
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const int k = 64 * h + 2 * i;
-                            const float p0 = ex2(fmaf(x[k], mul, shift)), p1 = ex2(fmaf(x[k + 1], mul, shift));
-                            const float p2 = ex2(fmaf(x[k + 2], mul, shift)), p3 = ex2(fmaf(x[k + 3], mul, shift));
+                            const float p0 = ex2(fmaf(x[2 * i], mul, shift)), p1 = ex2(fmaf(x[2 * i + 1], mul, shift));
+                            const float p2 = ex2(fmaf(x[2 * i + 2], mul, shift)), p3 = ex2(fmaf(x[2 * i + 3], mul, shift));
                             a0 += p0; a1 += p1; a2 += p2; a3 += p3;
                             p[i] = pack2<MBF>(p0, p1);
                             p[i + 1] = pack2<MBF>(p2, p3);
                         }
-                        tmem_st32x(st + 32 * h, p);
+                        tmem_st32x(st + 64 * h, p);
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) mbar_arrive(p_full(t, h));
-                    }
+                    };
+                    exponentials(1);
+                    load(0);
+                    exponentials(0);
                     sum += (a0 + a1) + (a2 + a3);
                 }
                 // the next unit's queries, while this one's last product runs
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         int j = at.a;
         int64_t ko = 0, vo = 0;
         uint32_t state = 0;                                            // of this lane's key: none, there, in no page
-        int page = 0;
+        int page = 0, at_page = 0, at_row = 0, at_head = 0;
         bool more = any;
         auto ask = [&]() {
             const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
@@ -438,10 +454,12 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 const bool bad = here && (page < 0 || page >= A.n_pages);
                 const int row = (int)key % A.page_size;
                 state = here ? bad ? 2u : 1u : 0u;
+                at_page = page; at_row = row; at_head = at.hk;
                 ko = state == 1 ? page * A.k_sp + row * A.k_ss + at.hk * A.k_sh : 0;
                 vo = state == 1 ? page * A.v_sp + row * A.v_ss + at.hk * A.v_sh : 0;
             } else {
                 state = here ? 1u : 0u;
+                at_row = (int)(at.q.q0 + key); at_head = at.hk;
                 ko = here ? (at.q.q0 + key) * A.k_ss + at.hk * A.k_sh : 0;
                 vo = here ? (at.q.q0 + key) * A.v_ss + at.hk * A.v_sh : 0;
             }
@@ -491,43 +509,53 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 if (lane == 0) mbar_arrive(kv_full(s));
             }
         } else {
-            constexpr int AHEAD = SLOTS > 2 ? 2 : 1;                   // items under way behind the one that is waited for
-            auto copy = [&](uint32_t item) {
-                if (!(item & 1)) place();
-                const uint32_t dst = ring + item % SLOTS * TILE + (piece >> 3) * HALF;
-                const uint16_t* const src = (const uint16_t*)((item & 1) ? A.v : A.k);
+            // a warp's 32 rows: boxes of rows that lie in one page by TMA (box: 8, 16 or 32 rows; 0: the layout allows none), in the order of
+            // the ring.  What may not reach a product, values behind the last key, is written as zeros: such rows are copied one by one
+            for (uint32_t item = 0; item < items; item++) {
+                const int s = item % SLOTS;
+                const bool is_v = item & 1;
+                issued = item;
+                if (!is_v) place();
+                if (!mbar_wait_lim(kv_empty(s), ((item / SLOTS) & 1) ^ 1, A.waits)) goto done;
+                const uint32_t dst = ring + s * TILE;
+                if (box && (!is_v || __all_sync(0xffffffffu, state == 1))) {
+                    const bool first = lane % box == 0 && state == 1;  // keys: whatever else lies in the box is masked
+                    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, first)) * box * (DP * 2);
+                    if (lane == 0) {
+                        if (bytes) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_full(s)), "r"(bytes) : "memory");
+                        else mbar_arrive(kv_full(s));
+                    }
+                    __syncwarp();
+                    if (first) {
+#pragma unroll
+                        for (int h = 0; h < DP / 64; h++) {
+                            const uint32_t to = dst + h * HALF + (w0 + lane) * 128;
+                            if (PAGED) asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                                    ::"r"(to), "l"(is_v ? &M.v : &M.k), "r"(64 * h), "r"(at_row), "r"(at_head), "r"(at_page), "r"(kv_full(s)) : "memory");
+                            else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                              ::"r"(to), "l"(is_v ? &M.v : &M.k), "r"(64 * h), "r"(at_head), "r"(at_row), "r"(kv_full(s)) : "memory");
+                        }
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                const uint16_t* const src = (const uint16_t*)(is_v ? A.v : A.k);
 #pragma unroll 8
                 for (int i = 0; i < PASSES; i++) {
                     const int l = i * RP + lane / CH, rr = w0 + l;
-                    const int64_t o = __shfl_sync(0xffffffffu, (item & 1) ? vo : ko, l);
-                    const uint32_t s = __shfl_sync(0xffffffffu, state, l), a = dst + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
+                    const int64_t o = __shfl_sync(0xffffffffu, is_v ? vo : ko, l);
+                    const uint32_t of = __shfl_sync(0xffffffffu, state, l), a = dst + (piece >> 3) * HALF + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
                     if (piece < live) {
-                        if (PAGED && s == 2 && (item & 1)) sts4(a, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);     // no such page: not a number
-                        else cp16(a, src + o + piece * 8, s == 1 ? 16u : 0u);
+                        if (PAGED && of == 2 && is_v) sts4(a, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);     // no such page: not a number
+                        else cp16(a, src + o + piece * 8, of == 1 ? 16u : 0u);
                     }
                 }
-            };
-            uint32_t told = 0;                                         // items that have been handed over
-            auto hand_over = [&](uint32_t upto) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                for (; told < upto; told++)
-                    if (lane == 0) mbar_arrive(kv_full(told % SLOTS));
-            };
-            for (uint32_t item = 0; item < items; item++) {
-                const uint32_t empty = kv_empty(item % SLOTS), parity = ((item / SLOTS) & 1) ^ 1;
-                if (!__all_sync(0xffffffffu, mbar_test(empty, parity))) {          // who holds the slot may wait for what is under way
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    hand_over(item);
-                    if (!mbar_wait_lim(empty, parity, A.waits)) goto done;
-                }
-                copy(item);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
-                if (item >= AHEAD && told < item + 1 - AHEAD) hand_over(item + 1 - AHEAD);
+                if (lane == 0) mbar_arrive(kv_full(s));
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            hand_over(items);
+            issued = items;
         }
     } else {
         regs_dec<P::kMmaRegs>();
@@ -555,12 +583,15 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 const uint64_t vd = (make_desc(slot(i)) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(HALF >> 4) << 16);
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 32 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 0 && k == 0 ? 0u : 1u, leader);
+                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 64 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 1 && k == 0 ? 0u : 1u, leader);
             };
             for (;;) {
-                const int a = at.a, b = at.b;
-                const int end[2] = {min(b, at.tiles_of(A, group, 0)), NT == 2 ? min(b, at.tiles_of(A, group, 1)) : 0};
+                // lane 0's, so that the compiler knows them to be the warp's: operands that it takes for a lane's own cost a move per MMA
+                auto warps_own = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+                const int a = warps_own(at.a), b = warps_own(at.b);
+                const int end[2] = {warps_own(min(b, at.tiles_of(A, group, 0))), NT == 2 ? warps_own(min(b, at.tiles_of(A, group, 1))) : 0};
                 if (!arrived(item)) goto done;
+#pragma unroll
                 for (int t = 0; t < NT; t++) {
                     if (end[t] <= a) continue;
                     if (!mbar_wait_lim(q_full(t), turns[t] & 1, A.waits)) goto done;
@@ -571,10 +602,12 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 umma_commit_w(kv_empty(item % SLOTS), leader);
                 for (int j = a; j < b; j++, item += 2) {
                     if (!arrived(item + 1)) goto done;
+#pragma unroll
                     for (int t = 0; t < NT; t++) {
                         if (j >= end[t]) continue;
                         if (j == a && turns[t]++ > 0 && !mbar_wait_lim(o_free(t), turns[t] & 1, A.waits)) goto done;
-                        for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int h = 1; h >= 0; h--) {
                             if (!mbar_wait_lim(p_full(t, h), steps[t] & 1, A.waits)) goto done;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                             values(t, item + 1, h, j == a);
@@ -600,6 +633,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
 done:
     asm volatile("cp.async.wait_all;" ::: "memory");                   // behind a wait that ran out copies may still be under way
     __syncwarp();
+    if (!E5M2 && warp >= 4 * NT && warp < 4 * NT + 4) drain_ring(issued, SLOTS, kv_full, A.waits);
     if (warp == 4 * NT + 4) {
         // ... and MMAs: nobody leaves their memory
         const uint32_t leader = elect_leader();
@@ -662,6 +696,40 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_
     }
 }
 
+// boxes of 64 elements x `box` rows: rows that are a multiple of it apart never share one with another page; 0 rows where the strides of a
+// tensor map cannot say it (a broadcast dimension) or a page's rows are no multiple of 8
+int prompt_maps(const PagedAttnArgs& A, PromptMaps* M, int* box) {
+    *box = 0;
+    memset(M, 0, sizeof(*M));
+    const int rows = A.table ? (A.page_size & -A.page_size) : 32;
+    if (rows < 8) return LB_OK;
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) { set_error(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver"); return LB_ERR_CUDA; }
+    const int b = rows < 32 ? rows : 32;
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t ss = (cuuint64_t)(i ? A.v_ss : A.k_ss) * 2, sh = (cuuint64_t)(i ? A.v_sh : A.k_sh) * 2, sp = (cuuint64_t)(i ? A.v_sp : A.k_sp) * 2;
+        const cuuint64_t dims[4] = {(cuuint64_t)A.D, (cuuint64_t)(A.table ? A.page_size : A.Hkv), (cuuint64_t)(A.table ? A.Hkv : A.T), (cuuint64_t)A.n_pages};
+        const cuuint64_t strides[3] = {A.table ? ss : sh, A.table ? sh : ss, sp};
+        const cuuint32_t boxes[4] = {64, A.table ? (cuuint32_t)b : 1u, A.table ? 1u : (cuuint32_t)b, 1}, unit[4] = {1, 1, 1, 1};
+        const int rank = A.table ? 4 : 3;
+        for (int d = 1; d < rank; d++)
+            if (strides[d - 1] == 0 || strides[d - 1] >= ((cuuint64_t)1 << 40)) return LB_OK;
+        auto encode = [&] { return enc(i ? &M->v : &M->k, A.dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                                       const_cast<void*>(i ? A.v : A.k), dims, strides, boxes, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
+        CUresult r = encode();
+        if (r == CUDA_ERROR_INVALID_CONTEXT) {                         // a thread before its first runtime call: bind its device's context
+            int dev = 0;
+            cudaGetDevice(&dev);
+            cudaSetDevice(dev);
+            r = encode();
+        }
+        if (r != CUDA_SUCCESS) { set_error(LB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r); return LB_ERR_CUDA; }
+    }
+    *box = b;
+    return LB_OK;
+}
+
 template <int DP, bool BF, bool E5M2, bool PAGED> int launch(const PagedAttnArgs& A, int above, cudaStream_t st) {
     using P = Prompt<DP, E5M2>;
     static bool configured[64] = {};                                   // the attribute is per device
@@ -672,7 +740,12 @@ template <int DP, bool BF, bool E5M2, bool PAGED> int launch(const PagedAttnArgs
         configured[dev & 63] = true;
     }
     const int C = sm_count();
-    launch_behind(paged_prompt_kernel<DP, BF, E5M2, PAGED>, dim3((unsigned)C), P::kWarps * 32, P::kSmem, st, launch_overlaps(st), A, above);
+    PromptMaps M;
+    int box = 0;
+    if (!E5M2) {
+        if (const int rc = prompt_maps(A, &M, &box)) return rc;
+    }
+    launch_behind(paged_prompt_kernel<DP, BF, E5M2, PAGED>, dim3((unsigned)C), P::kWarps * 32, P::kSmem, st, launch_overlaps(st), A, M, box, above);
     note_launch();
     launch_behind(paged_prompt_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, 4), P::kRows, 0, st, true, A, above, C);
     note_launch();
