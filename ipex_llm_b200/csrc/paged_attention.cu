@@ -1,9 +1,12 @@
 // paged_attention.cu -- attention of the new tokens of many requests over a paged cache, and of packed prompts over themselves:
 //   out[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j - max),   j = the keys that token t of its request sees.
 // Token i of a request's n new ones, which holds len, sees keys 0 .. len - n + i; a token that sees none gives zeros.
+#include <string.h>
 #include "paged.h"
+#include "tc_common.cuh"
 
 using namespace lowbit;
+using namespace lowbit::gemmtc;
 
 namespace lowbit {
 namespace {
@@ -83,14 +86,14 @@ template <bool BF> __device__ __forceinline__ void store4(uint16_t* p, const flo
 }
 
 // a request's tiles on one kv head: none where its rows are another kernel's, one where it has no keys (its rows become zeros)
-__device__ __forceinline__ int64_t few_tiles(const PagedReq& q, int group, int tile) {
+__device__ __forceinline__ int few_tiles(const PagedReq& q, int group, int tile) {
     if (q.n <= 0 || (int64_t)q.n * group > FEW_ROWS) return 0;
-    return q.len > 0 ? (q.len + tile - 1) / tile : 1;
+    return q.len > 0 ? (q.len - 1) / tile + 1 : 1;
 }
 
 // where a block is in its share: request, kv head, tile of that head
 struct FewAt {
-    PagedReq q; int r, hk; int64_t tile, tiles;
+    PagedReq q; int r, hk, tile, tiles;
     __device__ __forceinline__ void next(const PagedAttnArgs& A, int group, int tile_keys) {
         if (++tile < tiles) return;
         tile = 0;
@@ -104,262 +107,233 @@ struct FewAt {
     }
 };
 
-template <int DP, bool BF, bool E5M2>
-__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
-    using F = Few<DP, E5M2>;
-    constexpr bool MBF = BF && !E5M2;                                 // type in the products: fp16 over e5m2
-    constexpr int NW = F::kWarps, ST = F::kStages, KW = F::kKeys, ROW = F::kRow, CH = ROW / 16, NT = KW / 8;
-    extern __shared__ __align__(128) uint8_t few_smem[];
-    __shared__ int64_t scan[32];
-    __shared__ int found_r;
-    __shared__ int64_t found_before;
-    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = A.Hq / A.Hkv;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
-    const int C = gridDim.x, c = blockIdx.x;
-    const int64_t all = find_tile(A.R, [&](int r) { return few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
-                                  [&](int64_t n) { return share_begin(n, c, C); }, scan, &found_r, &found_before);
-    if (all == 0) return;
+// the whole block: where its share begins; returns the tiles of it
+__device__ __forceinline__ int few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at) {
+    const int64_t all = find_tile(A.R, [&](int r) { return (int64_t)few_tiles(paged_req(A, r), group, tile) * A.Hkv; }, [&](int64_t n) { return share_begin(n, c, C); }, scan,
+                                  found_r, found_before);
+    if (all == 0) return 0;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return;
-    FewAt at;                                                          // of the products
-    at.r = found_r;
+    if (first == last) return 0;
+    at.r = *found_r;
     at.q = paged_req(A, at.r);
-    at.tiles = few_tiles(at.q, group, F::kTile);
-    at.hk = div_few(first - found_before, at.tiles, at.tile);
-    FewAt in = at;                                                     // of the copies
+    at.tiles = few_tiles(at.q, group, tile);
+    int64_t within;
+    at.hk = div_few(first - *found_before, at.tiles, within);
+    at.tile = (int)within;
+    return (int)(last - first);
+}
 
-    const uint32_t ring = smem_addr(few_smem) + warp * ST * F::kStage;
-    float* const sums = reinterpret_cast<float*>(few_smem + F::kRing);                       // [warp][8][DP]
-    float2* const stats = reinterpret_cast<float2*>(few_smem + F::kRing + F::kSums);         // [warp][16]
-    // columns behind D stay zero: they are never copied to
-    if (A.D < DP) {
-        for (int i = lane; i < ST * F::kStage / 16; i += 32) sts16(ring + 16 * i, 0u);
-        __syncwarp();
+// Where a 16-byte piece of a row lies, in bytes.  Copied by TMA (rows of a page in one box): halves of 128 bytes a row, swizzled 128 bytes
+// wide (64-byte rows: 64).  Copied by cp.async, in a warp's own 16 or 32 rows: keys so that 8 rows x 16 bytes (ldmatrix) or rows g and pieces t
+// (e5m2) meet every bank once, values so that rows 2 t do.
+template <int DP, bool E5M2, bool TMA> struct FewAtSmem {
+    using F = Few<DP, E5M2>;
+    static constexpr int CH = F::kRow / 16;
+    __device__ static __forceinline__ uint32_t tma(int row, int piece) {
+        if (CH == 4) return (uint32_t)(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+        return (uint32_t)((piece >> 3) * (F::kTile * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
     }
-    const int live = A.D * (E5M2 ? 1 : 2) / 16;                        // 16-byte pieces of a row
-    // which piece of a row lies where: keys are read 8 rows x 16 bytes (ldmatrix), or a lane 16 bytes of row g; values a lane of rows 2 t
-    auto k_at = [&](int row, int piece) { return (uint32_t)(row * ROW + ((E5M2 ? (CH >= 8 ? piece ^ ((row & 1) << 2) : piece) : piece ^ (row & 7)) << 4)); };
-    auto v_at = [&](int row, int piece) {
+    __device__ static __forceinline__ uint32_t key(int row, int piece) {
+        if (TMA) return tma(row, piece);
+        return (uint32_t)(row * F::kRow + ((E5M2 ? (CH >= 8 ? piece ^ ((row & 1) << 2) : piece) : piece ^ (row & 7)) << 4));
+    }
+    __device__ static __forceinline__ uint32_t value(int row, int piece) {
+        if (TMA) return tma(row, piece);
         const int turn = !E5M2 ? row & 7 : CH == 4 ? (row >> 1) & 3 : CH == 8 ? row & 6 : ((row >> 1) & 1) | (row & 4);
-        return (uint32_t)(row * ROW + ((piece ^ turn) << 4));
-    };
-    // the page of this lane's key in the copies' tile, one tile ahead of its copies
-    int page = 0;
-    auto key_of = [&](const FewAt& w) { return w.tile * F::kTile + warp * KW + (KW == 32 ? lane : lane & 15); };
-    auto ask = [&]() {
-        const int64_t key = key_of(in);
-        if (in.tiles > 0 && key < in.q.len) page = A.table[in.r * A.table_stride + (int)key / A.page_size];
-    };
-    auto copy = [&](int stage) {
-        const uint32_t dst = ring + stage * F::kStage;
-        const int64_t key = key_of(in);
-        const bool here = key < in.q.len, bad = here && (page < 0 || page >= A.n_pages);
-        if (__any_sync(0xffffffffu, here)) {
-            const int row = (int)key % A.page_size;
-            const int64_t ko = here && !bad ? page * A.k_sp + row * A.k_ss + in.hk * A.k_sh : 0, vo = here && !bad ? page * A.v_sp + row * A.v_ss + in.hk * A.v_sh : 0;
-            const uint32_t state = here ? bad ? 2u : 1u : 0u;
-#pragma unroll
-            for (int i = 0; i < KW * CH / 32; i++) {
-                const int r = (i * 32 + lane) / CH, piece = lane % CH;
-                const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-                const uint32_t s = __shfl_sync(0xffffffffu, state, r);
-                if (piece < live) {
-                    const uint32_t bytes = s == 1 ? 16u : 0u;
-                    cp16(dst + k_at(r, piece), (const uint8_t*)A.k + kr * (E5M2 ? 1 : 2) + piece * 16, bytes);
-                    if (s == 2) sts16(dst + F::kHalf + v_at(r, piece), E5M2 ? 0x7f7f7f7fu : 0x7fff7fffu);      // no such page: not a number
-                    else cp16(dst + F::kHalf + v_at(r, piece), (const uint8_t*)A.v + vr * (E5M2 ? 1 : 2) + piece * 16, bytes);
-                }
-            }
-        }
-        in.next(A, group, F::kTile);
-        ask();
-    };
-    const int n = (int)(last - first);
-    ask();
-    for (int s = 0; s < ST - 1; s++) {
-        if (s < n) copy(s);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        return (uint32_t)(row * F::kRow + ((piece ^ turn) << 4));
     }
-    // the unit's queries as A fragments; factor = scale x log2 e (x what a row was divided by) of rows g and g + 8
+};
+
+// a warp's part of a unit: its queries as A fragments, the running maxima and sums of rows g and g + 8, the weighted values
+template <int DP, bool BF, bool E5M2, bool TMA> struct FewWarp {
+    using F = Few<DP, E5M2>;
+    using At = FewAtSmem<DP, E5M2, TMA>;
+    static constexpr bool MBF = BF && !E5M2;                          // type in the products: fp16 over e5m2
+    static constexpr int NT = F::kKeys / 8;
     uint32_t qf[DP / 16][4];
-    float factor[2], m[2], sum[2], o[DP / 8][4];
-    int64_t see[2];
-    int rows = 0;
-    bool begun = false, from_start = false;
-    for (int i = 0; i < n; i++) {
-        const int stage = i % ST;
-        if (i + ST - 1 < n) copy((i + ST - 1) % ST);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (!begun) {
-            begun = true;
-            from_start = at.tile == 0;
-            rows = at.q.n * group;
+    float factor[2], m[2], sum[2], o[DP / 8][4];                       // factor: scale x log2 e (x what a row was divided by)
+    int see[2], rows;
+
+    __device__ __forceinline__ void begin(const PagedAttnArgs& A, const PagedReq& q, int hk, int group, int g, int t) {
+        rows = q.n * group;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int row = g + 8 * h, token = row / group;
-                see[h] = row < rows ? (int64_t)at.q.len - at.q.n + token + 1 : 0;
-                const uint16_t* p = (const uint16_t*)A.q + (at.q.q0 + token) * A.q_st + (int64_t)(at.hk * group + row % group) * A.q_sh;
-                factor[h] = A.scale_log2e;
-                if (E5M2) {
-                    // k-step (c, s) of lane t holds elements 64 c + 16 t + 4 s .. + 3, the order in which a lane reads a key's bytes
-                    uint32_t big = 0;
+        for (int h = 0; h < 2; h++) {
+            const int row = g + 8 * h, token = row / group;
+            see[h] = row < rows ? q.len - q.n + token + 1 : 0;
+            const uint16_t* p = (const uint16_t*)A.q + (q.q0 + token) * A.q_st + (int64_t)(hk * group + row % group) * A.q_sh;
+            factor[h] = A.scale_log2e;
+            if (E5M2) {
+                // k-step (c, s) of lane t holds elements 64 c + 16 t + 4 s .. + 3, the order in which a lane reads a key's bytes
+                uint32_t big = 0;
 #pragma unroll
-                    for (int cc = 0; cc < DP / 64; cc++) {
-                        const int d = 64 * cc + 16 * t;
-                        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-                        if (row < rows && d < A.D) { x = *reinterpret_cast<const uint4*>(p + d); y = *reinterpret_cast<const uint4*>(p + d + 8); }
-                        const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                for (int cc = 0; cc < DP / 64; cc++) {
+                    const int d = 64 * cc + 16 * t;
+                    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+                    if (row < rows && d < A.D) { x = *reinterpret_cast<const uint4*>(p + d); y = *reinterpret_cast<const uint4*>(p + d + 8); }
+                    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            qf[4 * cc + e / 2][h + 2 * (e & 1)] = w[e];
-                            big = max(big, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
-                        }
+                    for (int e = 0; e < 8; e++) {
+                        qf[4 * cc + e / 2][h + 2 * (e & 1)] = w[e];
+                        big = max(big, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
                     }
-                    if (BF) {
-                        // bf16 enters as fp16, divided by a power of two that brings the row's largest value to 2^14: exact but for what
-                        // lies 2^-28 below it (fp16's last bit, 2^-24), where a 32-bit sum with that value ends too
-                        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                        const int ex = (int)(big >> 7) - 127 - 14, e = big >= 0x7f80u || big == 0u ? 0 : ex < -100 ? -100 : ex;
-                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                        factor[h] *= __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                        for (int k = 0; k < DP / 16; k++)
-#pragma unroll
-                            for (int z = 0; z < 2; z++) {
-                                const uint32_t w = qf[k][h + 2 * z];
-                                qf[k][h + 2 * z] = pack_half(unpack16<true>(w, 0) * down, unpack16<true>(w, 1) * down);
-                            }
-                    }
-                } else {
+                }
+                if (BF) {
+                    // bf16 enters as fp16, divided by a power of two that brings the row's largest value to 2^14: exact but for what lies 2^-28
+                    // below it (fp16's last bit, 2^-24), where a 32-bit sum with that value ends too
+                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                    const int ex = (int)(big >> 7) - 127 - 14, e = big >= 0x7f80u || big == 0u ? 0 : ex < -100 ? -100 : ex;
+                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                    factor[h] *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
                     for (int k = 0; k < DP / 16; k++)
 #pragma unroll
                         for (int z = 0; z < 2; z++) {
-                            const int d = 16 * k + 8 * z + 2 * t;
-                            qf[k][h + 2 * z] = row < rows && d < A.D ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+                            const uint32_t w = qf[k][h + 2 * z];
+                            qf[k][h + 2 * z] = pack_half(unpack16<true>(w, 0) * down, unpack16<true>(w, 1) * down);
                         }
                 }
-                m[h] = -INFINITY; sum[h] = 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < DP / 8; u++) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.0f;
-        }
-        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-        __syncwarp();
-        const int64_t key0 = at.tile * F::kTile + warp * KW;
-        const uint32_t ks = ring + stage * F::kStage, vs = ks + F::kHalf;
-        if (key0 < at.q.len) {
-            const bool few = rows <= 8;
-            float s[NT][4];
-#pragma unroll
-            for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-            if (E5M2) {
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int cc = 0; cc < DP / 64; cc++) {
-                        const uint4 w = lds16(ks + k_at(8 * j + g, 4 * cc + t));
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++)                    // e5m2 is the upper byte of fp16
-                            mma<false>(s[j], qf[4 * cc + k][0], qf[4 * cc + k][1], qf[4 * cc + k][2], qf[4 * cc + k][3], __byte_perm(x[k], 0u, 0x1404u), __byte_perm(x[k], 0u, 0x3424u));
-                    }
             } else {
 #pragma unroll
-                for (int k = 0; k < DP / 16; k++) {
-                    uint32_t b[4];
-                    ldsm4<false>(b, ks + k_at((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-                    mma<MBF>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
-                    mma<MBF>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
-                }
+                for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+                    for (int z = 0; z < 2; z++) {
+                        const int d = 16 * k + 8 * z + 2 * t;
+                        qf[k][h + 2 * z] = row < rows && d < A.D ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+                    }
             }
-            float corr[2], mx[2] = {-INFINITY, -INFINITY};
+            m[h] = -INFINITY; sum[h] = 0.0f;
+        }
 #pragma unroll
-            for (int j = 0; j < NT; j++)
+        for (int u = 0; u < DP / 8; u++) o[u][0] = o[u][1] = o[u][2] = o[u][3] = 0.0f;
+    }
+
+    // 16 or 32 keys from key0 on, in rows row0 .. of the tiles at ks and vs; `len`: values behind it are whatever was there (TMA)
+    __device__ __forceinline__ void keys(uint32_t ks, uint32_t vs, int row0, int key0, int len, int g, int t, int lane) {
+        const bool few = rows <= 8;
+        float s[NT][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int h = e >> 1;
-                    s[j][e] = key0 + 8 * j + 2 * t + (e & 1) < see[h] ? s[j][e] * factor[h] : -INFINITY;
-                    mx[h] = fmaxf(mx[h], s[j][e]);
+        for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+        if (E5M2) {
+#pragma unroll
+            for (int cc = 0; cc < DP / 64; cc++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const uint4 w = lds16(ks + At::key(row0 + 8 * j + g, 4 * cc + t));
+                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++)                        // e5m2 is the upper byte of fp16
+                        mma<false>(s[j], qf[4 * cc + k][0], qf[4 * cc + k][1], qf[4 * cc + k][2], qf[4 * cc + k][3], __byte_perm(x[k], 0u, 0x1404u), __byte_perm(x[k], 0u, 0x3424u));
                 }
+        } else {
+#pragma unroll
+            for (int k = 0; k < DP / 16; k++) {
+                uint32_t b[4];
+                ldsm4<false>(b, ks + At::key(row0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                mma<MBF>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+                mma<MBF>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+            }
+        }
+        // a row of nobody (see = 0) has no scores; every other row of the warp sees keys up to its own
+        float corr[2], mx[2] = {-INFINITY, -INFINITY};
+        const int first = key0 + 2 * t;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int h = e >> 1;
+                s[j][e] = first + 8 * j + (e & 1) < see[h] ? s[j][e] * factor[h] : -INFINITY;
+                mx[h] = fmaxf(mx[h], s[j][e]);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+            const float to = fmaxf(m[h], mx[h]);
+            corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
+            m[h] = to;
+            sum[h] *= corr[h];
+        }
+        if (few) corr[1] = corr[0];                                    // rows 8 .. 15 of the sums are the low parts of 0 .. 7
+        if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+            for (int u = 0; u < DP / 8; u++) { o[u][0] *= corr[0]; o[u][1] *= corr[0]; o[u][2] *= corr[1]; o[u][3] *= corr[1]; }
+        }
+        const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                const float to = fmaxf(m[h], mx[h]);
-                corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
-                m[h] = to;
-                sum[h] *= corr[h];
+                const float x = ex2(s[j][2 * h] - ref[h]), y = ex2(s[j][2 * h + 1] - ref[h]);
+                sum[h] += x + y;
+                split2<MBF>(x, y, hi[j][h], lo[j][h]);
             }
-            if (few) corr[1] = corr[0];                                // rows 8 .. 15 of the sums are the low parts of 0 .. 7
-            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
-#pragma unroll
-                for (int u = 0; u < DP / 8; u++) { o[u][0] *= corr[0]; o[u][1] *= corr[0]; o[u][2] *= corr[1]; o[u][3] *= corr[1]; }
+        // probabilities as two 16-bit values each; up to 8 rows the low parts are the products' other 8 rows, at no cost
+        auto values = [&](int j, float (&acc)[4], uint32_t b0, uint32_t b1) {
+            if (few) mma<MBF>(acc, hi[2 * j][0], lo[2 * j][0], hi[2 * j + 1][0], lo[2 * j + 1][0], b0, b1);
+            else {
+                mma<MBF>(acc, lo[2 * j][0], lo[2 * j][1], lo[2 * j + 1][0], lo[2 * j + 1][1], b0, b1);
+                mma<MBF>(acc, hi[2 * j][0], hi[2 * j][1], hi[2 * j + 1][0], hi[2 * j + 1][1], b0, b1);
             }
-            const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-            uint32_t hi[NT][2], lo[NT][2];
+        };
+        const bool cut = TMA && key0 + F::kKeys > len;                 // values behind the last key do not reach a product
 #pragma unroll
-            for (int j = 0; j < NT; j++)
+        for (int j = 0; j < NT / 2; j++) {                             // 16 keys
+            if (E5M2) {
+                // column tile u holds elements (DP / 8) n + u, n = 0 .. 7: a lane's bytes of a row lie together
+                constexpr int B = DP / 8, W = B / 4;
+                uint32_t x[4][W];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float x = ex2(s[j][2 * h] - ref[h]), y = ex2(s[j][2 * h + 1] - ref[h]);
-                    sum[h] += x + y;
-                    split2<MBF>(x, y, hi[j][h], lo[j][h]);
-                }
-            // probabilities as two 16-bit values each; up to 8 rows the low parts are the products' other 8 rows, at no cost
-            auto values = [&](int j, float (&acc)[4], uint32_t b0, uint32_t b1) {
-                if (few) mma<MBF>(acc, hi[2 * j][0], lo[2 * j][0], hi[2 * j + 1][0], lo[2 * j + 1][0], b0, b1);
-                else {
-                    mma<MBF>(acc, lo[2 * j][0], lo[2 * j][1], lo[2 * j + 1][0], lo[2 * j + 1][1], b0, b1);
-                    mma<MBF>(acc, hi[2 * j][0], hi[2 * j][1], hi[2 * j + 1][0], hi[2 * j + 1][1], b0, b1);
-                }
-            };
+                for (int k = 0; k < 4; k++) {
+                    const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
+                    if (B == 8) {
+                        const uint2 w = lds8(vs + At::value(row0 + row, g >> 1) + 8 * (g & 1));
+                        x[k][0] = w.x; x[k][1] = w.y;
+                    } else {
 #pragma unroll
-            for (int j = 0; j < NT / 2; j++) {                         // 16 keys
-                if (E5M2) {
-                    // column tile u holds elements (DP / 8) n + u, n = 0 .. 7: a lane's bytes of a row lie together
-                    constexpr int B = DP / 8, W = B / 4;
-                    uint32_t x[4][W];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int row = 16 * j + 2 * t + (k & 1) + 8 * (k >> 1);
-                        if (B == 8) {
-                            const uint2 w = lds8(vs + v_at(row, g >> 1) + 8 * (g & 1));
-                            x[k][0] = w.x; x[k][1] = w.y;
-                        } else {
-#pragma unroll
-                            for (int z = 0; z < B / 16; z++) {
-                                const uint4 w = lds16(vs + v_at(row, g * (B / 16) + z));
-                                x[k][(4 * z) % W] = w.x; x[k][(4 * z + 1) % W] = w.y; x[k][(4 * z + 2) % W] = w.z; x[k][(4 * z + 3) % W] = w.w;
-                            }
+                        for (int z = 0; z < B / 16; z++) {
+                            const uint4 w = lds16(vs + At::value(row0 + row, g * (B / 16) + z));
+                            x[k][(4 * z) % W] = w.x; x[k][(4 * z + 1) % W] = w.y; x[k][(4 * z + 2) % W] = w.z; x[k][(4 * z + 3) % W] = w.w;
                         }
                     }
+                    if (cut && key0 + row >= len) {
 #pragma unroll
-                    for (int u = 0; u < DP / 8; u += 2) {
-                        const uint32_t sel = u & 2 ? 0x7362u : 0x5140u;
-                        const uint32_t p = __byte_perm(x[0][u / 4], x[1][u / 4], sel), q = __byte_perm(x[2][u / 4], x[3][u / 4], sel);
-                        values(j, o[u], __byte_perm(p, 0u, 0x1404u), __byte_perm(q, 0u, 0x1404u));
-                        values(j, o[u + 1], __byte_perm(p, 0u, 0x3424u), __byte_perm(q, 0u, 0x3424u));
+                        for (int z = 0; z < W; z++) x[k][z] = 0u;
                     }
-                } else {
+                }
 #pragma unroll
-                    for (int u = 0; u < DP / 8; u += 2) {
-                        uint32_t b[4];
-                        ldsm4<true>(b, vs + v_at(16 * j + (lane & 15), u + (lane >> 4)));
-                        values(j, o[u], b[0], b[1]);
-                        values(j, o[u + 1], b[2], b[3]);
-                    }
+                for (int u = 0; u < DP / 8; u += 2) {
+                    const uint32_t sel = u & 2 ? 0x7362u : 0x5140u;
+                    const uint32_t p = __byte_perm(x[0][u / 4], x[1][u / 4], sel), q = __byte_perm(x[2][u / 4], x[3][u / 4], sel);
+                    values(j, o[u], __byte_perm(p, 0u, 0x1404u), __byte_perm(q, 0u, 0x1404u));
+                    values(j, o[u + 1], __byte_perm(p, 0u, 0x3424u), __byte_perm(q, 0u, 0x3424u));
+                }
+            } else {
+                uint32_t keep[2];                                      // of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const int left = len - key0 - 2 * t - 8 * z;
+                    keep[z] = left >= 2 ? 0xffffffffu : left == 1 ? 0x0000ffffu : 0u;
+                }
+#pragma unroll
+                for (int u = 0; u < DP / 8; u += 2) {
+                    uint32_t b[4];
+                    ldsm4<true>(b, vs + At::value(row0 + 16 * j + (lane & 15), u + (lane >> 4)));
+                    if (cut) { b[0] &= keep[0]; b[1] &= keep[1]; b[2] &= keep[0]; b[3] &= keep[1]; }
+                    values(j, o[u], b[0], b[1]);
+                    values(j, o[u + 1], b[2], b[3]);
                 }
             }
         }
-        __syncwarp();
-        if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
-        // ---- the unit's last tile here: the warps' sums to one, divided and stored, or left for the merge
-        const bool whole = from_start && at.tile + 1 == at.tiles;
-        float* const part = A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart;
+    }
+
+    // the unit's last tile here: the warps' sums to one, divided and stored, or left for the merge.  All NW warps; sync: a barrier of theirs
+    template <typename Sync>
+    __device__ __forceinline__ void finish(const PagedAttnArgs& A, const PagedReq& q, int hk, int group, bool whole, float* part, float* sums, float2* stats, int warp, int lane,
+                                           Sync sync) {
+        constexpr int NW = F::kWarps;
+        const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
@@ -374,7 +348,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
                 if (E5M2) { mine[2 * t * (DP / 8) + u] = x; mine[(2 * t + 1) * (DP / 8) + u] = y; }
                 else *reinterpret_cast<float2*>(mine + 8 * u + 2 * t) = make_float2(x, y);
             }
-            __syncthreads();
+            sync();
             for (int row = 8 * h + warp; row < rows && row < 8 * h + 8; row += NW) {
                 float top = -INFINITY, total = 0.0f, weight[NW];
 #pragma unroll
@@ -387,7 +361,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
                 }
                 const float inv = total == 0.0f ? 0.0f : 1.0f / total;
                 const int token = row / group;
-                uint16_t* const dst = (uint16_t*)A.out + (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh;
+                uint16_t* const dst = (uint16_t*)A.out + (q.q0 + token) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
                 for (int d = 4 * lane; d < DP; d += 128) {
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -401,11 +375,199 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
                 }
                 if (!whole && lane == 0) *reinterpret_cast<float2*>(part + FEW_ROWS * DP + 2 * row) = make_float2(top, total);
             }
-            __syncthreads();
+            sync();
         }
+    }
+};
+
+// every warp copies its own keys: page sizes that TMA has no box for
+template <int DP, bool BF, bool E5M2>
+__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
+    using F = Few<DP, E5M2>;
+    using W = FewWarp<DP, BF, E5M2, false>;
+    constexpr int ST = F::kStages, KW = F::kKeys, CH = F::kRow / 16;
+    extern __shared__ __align__(128) uint8_t few_smem[];
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = A.Hq / A.Hkv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int C = gridDim.x, c = blockIdx.x;
+    FewAt at;                                                          // of the products
+    const int n = few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at);
+    if (n == 0) return;
+    FewAt in = at;                                                     // of the copies
+
+    const uint32_t ring = smem_addr(few_smem) + warp * ST * F::kStage;
+    float* const sums = reinterpret_cast<float*>(few_smem + F::kRing);                       // [warp][8][DP]
+    float2* const stats = reinterpret_cast<float2*>(few_smem + F::kRing + F::kSums);         // [warp][16]
+    // columns behind D stay zero: they are never copied to
+    if (A.D < DP) {
+        for (int i = lane; i < ST * F::kStage / 16; i += 32) sts16(ring + 16 * i, 0u);
+        __syncwarp();
+    }
+    const int live = A.D * (E5M2 ? 1 : 2) / 16;                        // 16-byte pieces of a row
+    // the page of this lane's key in the copies' tile, one tile ahead of its copies
+    int page = 0;
+    auto key_of = [&](const FewAt& w) { return w.tile * F::kTile + warp * KW + (KW == 32 ? lane : lane & 15); };
+    auto ask = [&]() {
+        const int key = key_of(in);
+        if (in.tiles > 0 && key < in.q.len) page = A.table[in.r * A.table_stride + key / A.page_size];
+    };
+    auto copy = [&](int stage) {
+        const uint32_t dst = ring + stage * F::kStage;
+        const int key = key_of(in);
+        const bool here = key < in.q.len, bad = here && (page < 0 || page >= A.n_pages);
+        if (__any_sync(0xffffffffu, here)) {
+            const int row = key % A.page_size;
+            const int64_t ko = here && !bad ? page * A.k_sp + row * A.k_ss + in.hk * A.k_sh : 0, vo = here && !bad ? page * A.v_sp + row * A.v_ss + in.hk * A.v_sh : 0;
+            const uint32_t state = here ? bad ? 2u : 1u : 0u;
+#pragma unroll
+            for (int i = 0; i < KW * CH / 32; i++) {
+                const int r = (i * 32 + lane) / CH, piece = lane % CH;
+                const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                const uint32_t s = __shfl_sync(0xffffffffu, state, r);
+                if (piece < live) {
+                    const uint32_t bytes = s == 1 ? 16u : 0u;
+                    cp16(dst + W::At::key(r, piece), (const uint8_t*)A.k + kr * (E5M2 ? 1 : 2) + piece * 16, bytes);
+                    if (s == 2) sts16(dst + F::kHalf + W::At::value(r, piece), E5M2 ? 0x7f7f7f7fu : 0x7fff7fffu);      // no such page: not a number
+                    else cp16(dst + F::kHalf + W::At::value(r, piece), (const uint8_t*)A.v + vr * (E5M2 ? 1 : 2) + piece * 16, bytes);
+                }
+            }
+        }
+        in.next(A, group, F::kTile);
+        ask();
+    };
+    ask();
+    for (int s = 0; s < ST - 1; s++) {
+        if (s < n) copy(s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    W w;
+    bool begun = false, from_start = false;
+    for (int i = 0; i < n; i++) {
+        if (i + ST - 1 < n) copy((i + ST - 1) % ST);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!begun) {
+            begun = true;
+            from_start = at.tile == 0;
+            w.begin(A, at.q, at.hk, group, g, t);
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        __syncwarp();
+        const int key0 = at.tile * F::kTile + warp * KW;
+        const uint32_t ks = ring + i % ST * F::kStage;
+        if (key0 < at.q.len) w.keys(ks, ks + F::kHalf, 0, key0, at.q.len, g, t, lane);
+        __syncwarp();
+        if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
+        w.finish(A, at.q, at.hk, group, from_start && at.tile + 1 == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
+                 [] { __syncthreads(); });
         begun = false;
         at.next(A, group, F::kTile);
     }
+}
+
+// keys and values: [D][rows of a page][heads][pages]
+struct FewMaps { CUtensorMap k, v; };
+
+// one warp more fetches whole tiles by TMA, a box of 8 or 16 rows of a page a lane
+template <int DP, bool BF, bool E5M2>
+__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_few_tma_kernel(const PagedAttnArgs A, const __grid_constant__ FewMaps M, int box) {
+    using F = Few<DP, E5M2>;
+    constexpr int NW = F::kWarps, ST = F::kRing / (F::kStage * NW), KW = F::kKeys, HALVES = F::kRow <= 128 ? 1 : F::kRow / 128, WIDE = F::kRow < 128 ? F::kRow : 128;
+    constexpr int TILE = F::kTile * F::kRow;                           // bytes of a tile's keys
+    extern __shared__ uint8_t few_raw[];
+    __shared__ int64_t scan[32];
+    __shared__ int found_r;
+    __shared__ int64_t found_before;
+    __shared__ __align__(8) uint64_t bars[2 * ST];
+    __shared__ uint32_t bad_boxes[ST];
+    __shared__ volatile int gave_up;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = A.Hq / A.Hkv;
+    const uint32_t ring = (smem_addr(few_raw) + 1023u) & ~1023u;
+    auto full = [&](int s) { return smem_addr(bars + s); };
+    auto empty = [&](int s) { return smem_addr(bars + ST + s); };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int s = 0; s < ST; s++) { mbar_init(full(s), 1); mbar_init(empty(s), NW); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const int C = gridDim.x, c = blockIdx.x;
+    FewAt at;
+    const int n = few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at);
+    if (n == 0) return;
+    if (warp == NW) {
+        // ================= the copies =================
+        const int boxes = F::kTile / box, total = A.waits.limit < 0 ? n / 2 : n;
+        int page = 0, issued = 0;
+        auto ask = [&]() {
+            const int key = at.tile * F::kTile + lane * box;
+            if (at.tiles > 0 && lane < boxes && key < at.q.len) page = A.table[at.r * A.table_stride + key / A.page_size];
+        };
+        ask();
+        for (; issued < total; issued++) {
+            const int s = issued % ST;
+            if (!mbar_wait_lim(empty(s), ((issued / ST) & 1) ^ 1, A.waits)) break;
+            const int key = at.tile * F::kTile + lane * box;
+            const bool here = lane < boxes && key < at.q.len, good = here && page >= 0 && page < A.n_pages;
+            const uint32_t bad = __ballot_sync(0xffffffffu, here && !good), bytes = __popc(__ballot_sync(0xffffffffu, good)) * box * (HALVES * WIDE * 2);
+            if (lane == 0) {
+                bad_boxes[s] = bad;
+                if (bytes) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(s)), "r"(bytes) : "memory");
+                else mbar_arrive(full(s));
+            }
+            __syncwarp();
+            if (good) {
+                const int row = key % A.page_size;
+                const uint32_t dst = ring + s * (2 * TILE) + lane * box * WIDE;
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++)
+                        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                     ::"r"(dst + v * TILE + h * (F::kTile * 128)), "l"(v ? &M.v : &M.k), "r"(h * (E5M2 ? 128 : 64)), "r"(row), "r"(at.hk), "r"(page), "r"(full(s)) : "memory");
+            }
+            __syncwarp();
+            at.next(A, group, F::kTile);
+            ask();
+        }
+        // nobody leaves while copies are under way
+        drain_ring(issued, ST, full, A.waits);
+    } else {
+        float* const sums = reinterpret_cast<float*>(few_raw + (ring - smem_addr(few_raw)) + F::kRing);
+        float2* const stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(sums) + F::kSums);
+        FewWarp<DP, BF, E5M2, true> w;
+        bool begun = false, from_start = false;
+        for (int i = 0; i < n; i++) {
+            const int s = i % ST;
+            if (!begun) {
+                begun = true;
+                from_start = at.tile == 0;
+                w.begin(A, at.q, at.hk, group, g, t);
+            }
+            // a wait that ran out in one warp ends them all; they go through the motions, because they meet at barriers
+            if (!gave_up && !mbar_wait_lim(full(s), (i / ST) & 1, A.waits)) gave_up = 1;
+            const int key0 = at.tile * F::kTile + warp * KW;
+            const uint32_t ks = ring + s * (2 * TILE);
+            if (key0 < at.q.len) {
+                w.keys(ks, ks + TILE, warp * KW, key0, at.q.len, g, t, lane);
+                if (bad_boxes[s] >> (warp * KW / box) & ((1u << ((KW + box - 1) / box)) - 1)) w.sum[0] = w.sum[1] = NAN;       // no such page
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+            if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
+            w.finish(A, at.q, at.hk, group, from_start && at.tile + 1 == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
+                     [] { asm volatile("barrier.sync 1, %0;" ::"n"(NW * 32) : "memory"); });
+            begun = false;
+            at.next(A, group, F::kTile);
+        }
+    }
+    __syncthreads();
 }
 
 // the units that began in block c and went on in others: their parts in the order of the keys
@@ -417,7 +579,7 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
     __shared__ int64_t found_before;
     const int group = A.Hq / A.Hkv, c = blockIdx.x;
     // written by what ran before the kernel in front, which has waited for it
-    const int64_t all = find_tile(A.R, [&](int r) { return few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
+    const int64_t all = find_tile(A.R, [&](int r) { return (int64_t)few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
                                   [&](int64_t n) { return share_begin(n, c + 1, C) - 1; }, scan, &found_r, &found_before);
     if (all == 0) return;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
@@ -484,17 +646,56 @@ int check(const PagedAttnArgs& A, const char* name) {
     return LB_OK;
 }
 
-template <int DP, bool BF, bool E5M2> int few_launch(const PagedAttnArgs& A, cudaStream_t st) {
+// boxes of up to 16 rows; 0 rows where a page's rows are no multiple of 8 or a stride is none of a tensor map's
+template <int DP, bool E5M2> int few_maps(const PagedAttnArgs& A, FewMaps* M, int* box) {
+    using F = Few<DP, E5M2>;
+    *box = 0;
+    memset(M, 0, sizeof(*M));
+    const int rows = A.page_size & -A.page_size, b = rows < 16 ? rows : 16;
+    if (b < 8) return LB_OK;
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) { set_error(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver"); return LB_ERR_CUDA; }
+    const cuuint64_t size = E5M2 ? 1 : 2;
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t strides[3] = {(cuuint64_t)(i ? A.v_ss : A.k_ss) * size, (cuuint64_t)(i ? A.v_sh : A.k_sh) * size, (cuuint64_t)(i ? A.v_sp : A.k_sp) * size};
+        const cuuint64_t dims[4] = {(cuuint64_t)A.D, (cuuint64_t)A.page_size, (cuuint64_t)A.Hkv, (cuuint64_t)A.n_pages};
+        const cuuint32_t boxes[4] = {(cuuint32_t)((F::kRow < 128 ? F::kRow : 128) / size), (cuuint32_t)b, 1, 1}, unit[4] = {1, 1, 1, 1};
+        for (const cuuint64_t st : strides)
+            if (st == 0 || st >= ((cuuint64_t)1 << 40)) return LB_OK;
+        auto encode = [&] { return enc(i ? &M->v : &M->k, E5M2 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : A.dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(i ? A.v : A.k), dims, strides, boxes, unit,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, F::kRow < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
+        CUresult r = encode();
+        if (r == CUDA_ERROR_INVALID_CONTEXT) {                         // a thread before its first runtime call: bind its device's context
+            int dev = 0;
+            cudaGetDevice(&dev);
+            cudaSetDevice(dev);
+            r = encode();
+        }
+        if (r != CUDA_SUCCESS) { set_error(LB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r); return LB_ERR_CUDA; }
+    }
+    *box = b;
+    return LB_OK;
+}
+
+template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, cudaStream_t st) {
     using F = Few<DP, E5M2>;
     static bool configured[64] = {};                                   // the attribute is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
         cudaFuncSetAttribute(paged_few_kernel<DP, BF, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        cudaFuncSetAttribute(paged_few_tma_kernel<DP, BF, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem + 1024);
         configured[dev & 63] = true;
     }
     const int C = sm_count();
-    launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
+    FewMaps M;
+    int box = 0;
+    if (const int rc = few_maps<DP, E5M2>(A, &M, &box)) return rc;
+    if (box) {
+        if (const int rc = make_waits(&A.waits, kWaitCycles)) return rc;
+        launch_behind(paged_few_tma_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32 + 32, F::kSmem + 1024, st, launch_overlaps(st), A, M, box);
+    } else launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
     note_launch();
     launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C), 256, 0, st, true, A, C);
     note_launch();
