@@ -61,6 +61,7 @@ __device__ __forceinline__ uint64_t div_small(uint64_t n, uint32_t d, uint32_t& 
     return q;
 }
 __device__ __forceinline__ int64_t share_begin(int64_t n, int c, int C) {
+    if (n < 1 << 20) return (uint32_t)n * (uint32_t)c / (uint32_t)C;                        // C is at most some thousands
     uint32_t rem;
     const uint64_t q = div_small((uint64_t)n, (uint32_t)C, rem);
     return (int64_t)q * c + rem * (uint32_t)c / (uint32_t)C;

@@ -91,36 +91,54 @@ __device__ __forceinline__ int few_tiles(const PagedReq& q, int group, int tile)
     return q.len > 0 ? (q.len - 1) / tile + 1 : 1;
 }
 
-// where a block is in its share: request, kv head, tile of that head
+// What a unit costs beside its keys (queries, the warps' sums, the result), in tiles: shares are taken of places, FEW_EXTRA of them in front of
+// a unit's tiles, so that blocks with many short requests are not the last
+constexpr int FEW_EXTRA = 1;
+// where a block is in its share: request, kv head, tile of that head, and the end of the piece that it takes of them
 struct FewAt {
-    PagedReq q; int r, hk, tile, tiles;
-    __device__ __forceinline__ void next(const PagedAttnArgs& A, int group, int tile_keys) {
-        if (++tile < tiles) return;
-        tile = 0;
-        if (++hk < A.Hkv) return;
-        hk = 0;
-        do {
-            if (++r >= A.R) { tiles = 0; return; }
-            q = paged_req(A, r);
-            tiles = few_tiles(q, group, tile_keys);
-        } while (tiles == 0);
+    PagedReq q; int r, hk, tile, end, tiles, left;
+    __device__ __forceinline__ bool piece(int place) {
+        const int take = min(tiles + FEW_EXTRA - place, left);
+        left -= take;
+        tile = max(place - FEW_EXTRA, 0);
+        end = max(place + take - FEW_EXTRA, 0);
+        return tile < end;
     }
+    __device__ __forceinline__ bool next(const PagedAttnArgs& A, int group, int tile_keys) {
+        if (++tile < end) return true;
+        while (left > 0) {
+            if (++hk >= A.Hkv) {
+                hk = 0;
+                do {
+                    if (++r >= A.R) return false;
+                    q = paged_req(A, r);
+                    tiles = few_tiles(q, group, tile_keys);
+                } while (tiles == 0);
+            }
+            if (piece(0)) return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool last() const { return tile + 1 == end; }
 };
-
-// the whole block: where its share begins; returns the tiles of it
-__device__ __forceinline__ int few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at) {
-    const int64_t all = find_tile(A.R, [&](int r) { return (int64_t)few_tiles(paged_req(A, r), group, tile) * A.Hkv; }, [&](int64_t n) { return share_begin(n, c, C); }, scan,
-                                  found_r, found_before);
-    if (all == 0) return 0;
+__device__ __forceinline__ int64_t few_places(const PagedReq& q, const PagedAttnArgs& A, int group, int tile) {
+    const int tiles = few_tiles(q, group, tile);
+    return tiles ? (int64_t)(tiles + FEW_EXTRA) * A.Hkv : 0;
+}
+// the whole block: where its share begins; false: it has none
+__device__ __forceinline__ bool few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at) {
+    const int64_t all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, tile); }, [&](int64_t n) { return share_begin(n, c, C); }, scan, found_r,
+                                  found_before);
+    if (all == 0) return false;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return 0;
+    if (first == last) return false;
     at.r = *found_r;
     at.q = paged_req(A, at.r);
     at.tiles = few_tiles(at.q, group, tile);
-    int64_t within;
-    at.hk = div_few(first - *found_before, at.tiles, within);
-    at.tile = (int)within;
-    return (int)(last - first);
+    at.left = (int)(last - first);
+    int64_t place;
+    at.hk = div_few(first - *found_before, at.tiles + FEW_EXTRA, place);
+    return at.piece((int)place) || at.next(A, group, tile);
 }
 
 // Where a 16-byte piece of a row lies, in bytes.  Copied by TMA (rows of a page in one box): halves of 128 bytes a row, swizzled 128 bytes
@@ -144,20 +162,25 @@ template <int DP, bool E5M2, bool TMA> struct FewAtSmem {
     }
 };
 
-// a warp's part of a unit: its queries as A fragments, the running maxima and sums of rows g and g + 8, the weighted values
-template <int DP, bool BF, bool E5M2, bool TMA> struct FewWarp {
+// a warp's part of a unit: its queries as A fragments, the running maxima and sums of rows g and g + 8 (EIGHT: no unit has more than 8, and rows
+// 8 .. 15 of the products hold the probabilities' low parts), the weighted values
+template <int DP, bool BF, bool E5M2, bool TMA, bool EIGHT> struct FewWarp {
     using F = Few<DP, E5M2>;
     using At = FewAtSmem<DP, E5M2, TMA>;
     static constexpr bool MBF = BF && !E5M2;                          // type in the products: fp16 over e5m2
-    static constexpr int NT = F::kKeys / 8;
+    static constexpr int NT = F::kKeys / 8, H = EIGHT ? 1 : 2;
     uint32_t qf[DP / 16][4];
     float factor[2], m[2], sum[2], o[DP / 8][4];                       // factor: scale x log2 e (x what a row was divided by)
     int see[2], rows;
 
     __device__ __forceinline__ void begin(const PagedAttnArgs& A, const PagedReq& q, int hk, int group, int g, int t) {
         rows = q.n * group;
+        if (EIGHT) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+            for (int k = 0; k < DP / 16; k++) qf[k][1] = qf[k][3] = 0u;
+        }
+#pragma unroll
+        for (int h = 0; h < H; h++) {
             const int row = g + 8 * h, token = row / group;
             see[h] = row < rows ? q.len - q.n + token + 1 : 0;
             const uint16_t* p = (const uint16_t*)A.q + (q.q0 + token) * A.q_st + (int64_t)(hk * group + row % group) * A.q_sh;
@@ -210,68 +233,92 @@ template <int DP, bool BF, bool E5M2, bool TMA> struct FewWarp {
 
     // 16 or 32 keys from key0 on, in rows row0 .. of the tiles at ks and vs; `len`: values behind it are whatever was there (TMA)
     __device__ __forceinline__ void keys(uint32_t ks, uint32_t vs, int row0, int key0, int len, int g, int t, int lane) {
-        const bool few = rows <= 8;
         float s[NT][4];
 #pragma unroll
         for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
         if (E5M2) {
 #pragma unroll
-            for (int cc = 0; cc < DP / 64; cc++)
+            for (int cc = 0; cc < DP / 64; cc++) {
+                uint32_t x[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
                     const uint4 w = lds16(ks + At::key(row0 + 8 * j + g, 4 * cc + t));
-                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++)                        // e5m2 is the upper byte of fp16
-                        mma<false>(s[j], qf[4 * cc + k][0], qf[4 * cc + k][1], qf[4 * cc + k][2], qf[4 * cc + k][3], __byte_perm(x[k], 0u, 0x1404u), __byte_perm(x[k], 0u, 0x3424u));
+                    x[j][0] = w.x; x[j][1] = w.y; x[j][2] = w.z; x[j][3] = w.w;
                 }
-        } else {
 #pragma unroll
-            for (int k = 0; k < DP / 16; k++) {
-                uint32_t b[4];
+                for (int k = 0; k < 4; k++)                            // e5m2 is the upper byte of fp16
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+                        mma<false>(s[j], qf[4 * cc + k][0], qf[4 * cc + k][1], qf[4 * cc + k][2], qf[4 * cc + k][3], __byte_perm(x[j][k], 0u, 0x1404u),
+                                   __byte_perm(x[j][k], 0u, 0x3424u));
+            }
+        } else {
+            // even and odd steps on sums of their own: an accumulator is free again only after some 20 clocks
+            float s1[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; j++) s1[j][0] = s1[j][1] = s1[j][2] = s1[j][3] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < DP / 16; k += 2) {
+                uint32_t b[4], d[4];
                 ldsm4<false>(b, ks + At::key(row0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                ldsm4<false>(d, ks + At::key(row0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + 2 + ((lane >> 3) & 1)));
                 mma<MBF>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
                 mma<MBF>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+                mma<MBF>(s1[0], qf[k + 1][0], qf[k + 1][1], qf[k + 1][2], qf[k + 1][3], d[0], d[1]);
+                mma<MBF>(s1[1], qf[k + 1][0], qf[k + 1][1], qf[k + 1][2], qf[k + 1][3], d[2], d[3]);
             }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[j][e] += s1[j][e];
         }
-        // a row of nobody (see = 0) has no scores; every other row of the warp sees keys up to its own
-        float corr[2], mx[2] = {-INFINITY, -INFINITY};
+        // a row of nobody (see = 0) has no scores; rows of a request see keys up to their own, the first one the fewest
         const int first = key0 + 2 * t;
+        float mx[H];
+        bool grow = false;
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+        for (int h = 0; h < H; h++) {
+            mx[h] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int h = e >> 1;
-                s[j][e] = first + 8 * j + (e & 1) < see[h] ? s[j][e] * factor[h] : -INFINITY;
-                mx[h] = fmaxf(mx[h], s[j][e]);
-            }
+            for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+                for (int e = 0; e < 2; e++) {
+                    float& x = s[j][2 * h + e];
+                    x = first + 8 * j + e < see[h] ? x * factor[h] : -INFINITY;
+                    mx[h] = fmaxf(mx[h], x);
+                }
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            const float to = fmaxf(m[h], mx[h]);
-            corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
-            m[h] = to;
-            sum[h] *= corr[h];
+            grow |= mx[h] > m[h] + 4.0f;                               // -inf: any key
         }
-        if (few) corr[1] = corr[0];                                    // rows 8 .. 15 of the sums are the low parts of 0 .. 7
-        if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+        // the reference follows the maximum when that grew by more than 2^4: probabilities up to 16 are as exact as those up to 1
+        if (__any_sync(0xffffffffu, grow)) {
+            float corr[2];
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                const float to = mx[h] > m[h] + 4.0f ? mx[h] : m[h];
+                corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
+                m[h] = to;
+                sum[h] *= corr[h];
+            }
+            if (EIGHT) corr[1] = corr[0];
 #pragma unroll
             for (int u = 0; u < DP / 8; u++) { o[u][0] *= corr[0]; o[u][1] *= corr[0]; o[u][2] *= corr[1]; o[u][3] *= corr[1]; }
         }
-        const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-        uint32_t hi[NT][2], lo[NT][2];
+        uint32_t hi[NT][H], lo[NT][H];
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+        for (int h = 0; h < H; h++) {
+            const float ref = m[h] == -INFINITY ? 0.0f : m[h];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float x = ex2(s[j][2 * h] - ref[h]), y = ex2(s[j][2 * h + 1] - ref[h]);
+            for (int j = 0; j < NT; j++) {
+                const float x = ex2(s[j][2 * h] - ref), y = ex2(s[j][2 * h + 1] - ref);
                 sum[h] += x + y;
                 split2<MBF>(x, y, hi[j][h], lo[j][h]);
             }
+        }
         // probabilities as two 16-bit values each; up to 8 rows the low parts are the products' other 8 rows, at no cost
         auto values = [&](int j, float (&acc)[4], uint32_t b0, uint32_t b1) {
-            if (few) mma<MBF>(acc, hi[2 * j][0], lo[2 * j][0], hi[2 * j + 1][0], lo[2 * j + 1][0], b0, b1);
+            if constexpr (EIGHT) mma<MBF>(acc, hi[2 * j][0], lo[2 * j][0], hi[2 * j + 1][0], lo[2 * j + 1][0], b0, b1);
             else {
                 mma<MBF>(acc, lo[2 * j][0], lo[2 * j][1], lo[2 * j + 1][0], lo[2 * j + 1][1], b0, b1);
                 mma<MBF>(acc, hi[2 * j][0], hi[2 * j][1], hi[2 * j + 1][0], hi[2 * j + 1][1], b0, b1);
@@ -335,16 +382,16 @@ template <int DP, bool BF, bool E5M2, bool TMA> struct FewWarp {
         constexpr int NW = F::kWarps;
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < H; h++) {
             sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
             sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
             if (t == 0) stats[warp * FEW_ROWS + g + 8 * h] = make_float2(m[h], sum[h]);
         }
-        for (int h = 0; h < (rows > 8 ? 2 : 1); h++) {
+        for (int h = 0; h < (EIGHT || rows <= 8 ? 1 : 2); h++) {
             float* const mine = sums + (warp * 8 + g) * DP;
 #pragma unroll
             for (int u = 0; u < DP / 8; u++) {
-                const float x = rows > 8 ? (h ? o[u][2] : o[u][0]) : o[u][0] + o[u][2], y = rows > 8 ? (h ? o[u][3] : o[u][1]) : o[u][1] + o[u][3];
+                const float x = EIGHT ? o[u][0] + o[u][2] : h ? o[u][2] : o[u][0], y = EIGHT ? o[u][1] + o[u][3] : h ? o[u][3] : o[u][1];
                 if (E5M2) { mine[2 * t * (DP / 8) + u] = x; mine[(2 * t + 1) * (DP / 8) + u] = y; }
                 else *reinterpret_cast<float2*>(mine + 8 * u + 2 * t) = make_float2(x, y);
             }
@@ -384,7 +431,7 @@ template <int DP, bool BF, bool E5M2, bool TMA> struct FewWarp {
 template <int DP, bool BF, bool E5M2>
 __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
     using F = Few<DP, E5M2>;
-    using W = FewWarp<DP, BF, E5M2, false>;
+    using W = FewWarp<DP, BF, E5M2, false, false>;
     constexpr int ST = F::kStages, KW = F::kKeys, CH = F::kRow / 16;
     extern __shared__ __align__(128) uint8_t few_smem[];
     __shared__ int64_t scan[32];
@@ -396,9 +443,9 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     asm volatile("griddepcontrol.launch_dependents;");
     const int C = gridDim.x, c = blockIdx.x;
     FewAt at;                                                          // of the products
-    const int n = few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at);
-    if (n == 0) return;
+    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at)) return;
     FewAt in = at;                                                     // of the copies
+    bool to_copy = true;
 
     const uint32_t ring = smem_addr(few_smem) + warp * ST * F::kStage;
     float* const sums = reinterpret_cast<float*>(few_smem + F::kRing);                       // [warp][8][DP]
@@ -414,9 +461,10 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     auto key_of = [&](const FewAt& w) { return w.tile * F::kTile + warp * KW + (KW == 32 ? lane : lane & 15); };
     auto ask = [&]() {
         const int key = key_of(in);
-        if (in.tiles > 0 && key < in.q.len) page = A.table[in.r * A.table_stride + key / A.page_size];
+        if (to_copy && key < in.q.len) page = A.table[in.r * A.table_stride + key / A.page_size];
     };
     auto copy = [&](int stage) {
+        if (!to_copy) return;
         const uint32_t dst = ring + stage * F::kStage;
         const int key = key_of(in);
         const bool here = key < in.q.len, bad = here && (page < 0 || page >= A.n_pages);
@@ -437,18 +485,18 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
                 }
             }
         }
-        in.next(A, group, F::kTile);
+        to_copy = in.next(A, group, F::kTile);
         ask();
     };
     ask();
     for (int s = 0; s < ST - 1; s++) {
-        if (s < n) copy(s);
+        copy(s);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     W w;
-    bool begun = false, from_start = false;
-    for (int i = 0; i < n; i++) {
-        if (i + ST - 1 < n) copy((i + ST - 1) % ST);
+    bool begun = false, from_start = false, more = true;
+    for (int i = 0; more; i++) {
+        copy((i + ST - 1) % ST);
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (!begun) {
             begun = true;
@@ -461,20 +509,21 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
         const uint32_t ks = ring + i % ST * F::kStage;
         if (key0 < at.q.len) w.keys(ks, ks + F::kHalf, 0, key0, at.q.len, g, t, lane);
         __syncwarp();
-        if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
-        w.finish(A, at.q, at.hk, group, from_start && at.tile + 1 == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
+        if (!at.last()) { at.tile++; continue; }
+        w.finish(A, at.q, at.hk, group, from_start && at.end == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
                  [] { __syncthreads(); });
         begun = false;
-        at.next(A, group, F::kTile);
+        more = at.next(A, group, F::kTile);
     }
 }
 
 // keys and values: [D][rows of a page][heads][pages]
 struct FewMaps { CUtensorMap k, v; };
 
-// one warp more fetches whole tiles by TMA, a box of 8 or 16 rows of a page a lane
-template <int DP, bool BF, bool E5M2>
-__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_few_tma_kernel(const PagedAttnArgs A, const __grid_constant__ FewMaps M, int box) {
+// Four warps more fetch whole tiles by TMA, a box of 8 to 32 rows of a page a lane: a warp issues one in 80 to 95 clocks, and a tile of pages of 16
+// rows takes 32 of them (one warp for all: 3100 clocks a tile, 2360 for the products)
+template <int DP, bool BF, bool E5M2, bool EIGHT>
+__global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_few_tma_kernel(const PagedAttnArgs A, const __grid_constant__ FewMaps M, int box) {
     using F = Few<DP, E5M2>;
     constexpr int NW = F::kWarps, ST = F::kRing / (F::kStage * NW), KW = F::kKeys, HALVES = F::kRow <= 128 ? 1 : F::kRow / 128, WIDE = F::kRow < 128 ? F::kRow : 128;
     constexpr int TILE = F::kTile * F::kRow;                           // bytes of a tile's keys
@@ -483,7 +532,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_fe
     __shared__ int found_r;
     __shared__ int64_t found_before;
     __shared__ __align__(8) uint64_t bars[2 * ST];
-    __shared__ uint32_t bad_boxes[ST];
+    __shared__ __align__(16) uint32_t bad_boxes[ST][4];
     __shared__ volatile int gave_up;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = A.Hq / A.Hkv;
@@ -494,37 +543,38 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_fe
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) {
         gave_up = 0;
-        for (int s = 0; s < ST; s++) { mbar_init(full(s), 1); mbar_init(empty(s), NW); }
+        for (int s = 0; s < ST; s++) { mbar_init(full(s), 4); mbar_init(empty(s), NW); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const int C = gridDim.x, c = blockIdx.x;
     FewAt at;
-    const int n = few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at);
-    if (n == 0) return;
-    if (warp == NW) {
-        // ================= the copies =================
-        const int boxes = F::kTile / box, total = A.waits.limit < 0 ? n / 2 : n;
+    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at)) return;
+    if (warp >= NW) {
+        // ================= the copies: this warp's boxes of a tile =================
+        const int boxes = F::kTile / box, own = max(boxes / 4, 1), mine = own * (warp - NW) + lane, most = A.waits.limit < 0 ? at.left / 2 : 0x7fffffff;
+        const bool some = lane < own && mine < boxes;
         int page = 0, issued = 0;
+        bool more = true;
         auto ask = [&]() {
-            const int key = at.tile * F::kTile + lane * box;
-            if (at.tiles > 0 && lane < boxes && key < at.q.len) page = A.table[at.r * A.table_stride + key / A.page_size];
+            const int key = at.tile * F::kTile + mine * box;
+            if (more && some && key < at.q.len) page = A.table[at.r * A.table_stride + key / A.page_size];
         };
         ask();
-        for (; issued < total; issued++) {
+        for (; more && issued < most; issued++) {
             const int s = issued % ST;
             if (!mbar_wait_lim(empty(s), ((issued / ST) & 1) ^ 1, A.waits)) break;
-            const int key = at.tile * F::kTile + lane * box;
-            const bool here = lane < boxes && key < at.q.len, good = here && page >= 0 && page < A.n_pages;
+            const int key = at.tile * F::kTile + mine * box;
+            const bool here = some && key < at.q.len, good = here && page >= 0 && page < A.n_pages;
             const uint32_t bad = __ballot_sync(0xffffffffu, here && !good), bytes = __popc(__ballot_sync(0xffffffffu, good)) * box * (HALVES * WIDE * 2);
             if (lane == 0) {
-                bad_boxes[s] = bad;
+                bad_boxes[s][warp - NW] = bad << own * (warp - NW);
                 if (bytes) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(s)), "r"(bytes) : "memory");
                 else mbar_arrive(full(s));
             }
             __syncwarp();
             if (good) {
                 const int row = key % A.page_size;
-                const uint32_t dst = ring + s * (2 * TILE) + lane * box * WIDE;
+                const uint32_t dst = ring + s * (2 * TILE) + mine * box * WIDE;
 #pragma unroll
                 for (int v = 0; v < 2; v++)
 #pragma unroll
@@ -533,7 +583,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_fe
                                      ::"r"(dst + v * TILE + h * (F::kTile * 128)), "l"(v ? &M.v : &M.k), "r"(h * (E5M2 ? 128 : 64)), "r"(row), "r"(at.hk), "r"(page), "r"(full(s)) : "memory");
             }
             __syncwarp();
-            at.next(A, group, F::kTile);
+            more = at.next(A, group, F::kTile);
             ask();
         }
         // nobody leaves while copies are under way
@@ -541,9 +591,9 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_fe
     } else {
         float* const sums = reinterpret_cast<float*>(few_raw + (ring - smem_addr(few_raw)) + F::kRing);
         float2* const stats = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(sums) + F::kSums);
-        FewWarp<DP, BF, E5M2, true> w;
-        bool begun = false, from_start = false;
-        for (int i = 0; i < n; i++) {
+        FewWarp<DP, BF, E5M2, true, EIGHT> w;
+        bool begun = false, from_start = false, more = true;
+        for (int i = 0; more; i++) {
             const int s = i % ST;
             if (!begun) {
                 begun = true;
@@ -556,15 +606,16 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 32), 1) paged_fe
             const uint32_t ks = ring + s * (2 * TILE);
             if (key0 < at.q.len) {
                 w.keys(ks, ks + TILE, warp * KW, key0, at.q.len, g, t, lane);
-                if (bad_boxes[s] >> (warp * KW / box) & ((1u << ((KW + box - 1) / box)) - 1)) w.sum[0] = w.sum[1] = NAN;       // no such page
+                const uint4 bad = *reinterpret_cast<const uint4*>(bad_boxes[s]);
+                if ((bad.x | bad.y | bad.z | bad.w) >> (warp * KW / box) & ((1u << ((KW + box - 1) / box)) - 1)) w.sum[0] = w.sum[EIGHT ? 0 : 1] = NAN;       // no such page
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(s));
-            if (at.tile + 1 < at.tiles && i + 1 < n) { at.next(A, group, F::kTile); continue; }
-            w.finish(A, at.q, at.hk, group, from_start && at.tile + 1 == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
+            if (!at.last()) { at.tile++; continue; }
+            w.finish(A, at.q, at.hk, group, from_start && at.end == at.tiles, A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * F::kPart, sums, stats, warp, lane,
                      [] { asm volatile("barrier.sync 1, %0;" ::"n"(NW * 32) : "memory"); });
             begun = false;
-            at.next(A, group, F::kTile);
+            more = at.next(A, group, F::kTile);
         }
     }
     __syncthreads();
@@ -579,17 +630,17 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
     __shared__ int64_t found_before;
     const int group = A.Hq / A.Hkv, c = blockIdx.x;
     // written by what ran before the kernel in front, which has waited for it
-    const int64_t all = find_tile(A.R, [&](int r) { return (int64_t)few_tiles(paged_req(A, r), group, F::kTile) * A.Hkv; },
+    const int64_t all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, F::kTile); },
                                   [&](int64_t n) { return share_begin(n, c + 1, C) - 1; }, scan, &found_r, &found_before);
     if (all == 0) return;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
     if (first == last) return;
     const PagedReq q = paged_req(A, found_r);
-    const int64_t tiles = few_tiles(q, group, F::kTile);
+    const int places = few_tiles(q, group, F::kTile) + FEW_EXTRA;
     int64_t within;
-    const int hk = div_few(last - 1 - found_before, tiles, within);
-    const int64_t from = found_before + hk * tiles, to = from + tiles;
-    if (from < first || to <= last) return;                            // began earlier, or ends here
+    const int hk = div_few(last - 1 - found_before, places, within);
+    const int64_t from = found_before + (int64_t)hk * places, to = from + places;
+    if (first - from > FEW_EXTRA || last - from <= FEW_EXTRA || to <= last) return;        // its first tile is another block's, or it ends here
     const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int row = warp; row < rows; row += 8) {
@@ -646,12 +697,12 @@ int check(const PagedAttnArgs& A, const char* name) {
     return LB_OK;
 }
 
-// boxes of up to 16 rows; 0 rows where a page's rows are no multiple of 8 or a stride is none of a tensor map's
+// boxes of up to 32 rows; 0 rows where a page's rows are no multiple of 8 or a stride is none of a tensor map's
 template <int DP, bool E5M2> int few_maps(const PagedAttnArgs& A, FewMaps* M, int* box) {
     using F = Few<DP, E5M2>;
     *box = 0;
     memset(M, 0, sizeof(*M));
-    const int rows = A.page_size & -A.page_size, b = rows < 16 ? rows : 16;
+    const int rows = A.page_size & -A.page_size, b = rows < 32 ? rows : 32;
     if (b < 8) return LB_OK;
     EncodeTiledFn enc = encode_fn();
     if (!enc) { set_error(LB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver"); return LB_ERR_CUDA; }
@@ -663,7 +714,7 @@ template <int DP, bool E5M2> int few_maps(const PagedAttnArgs& A, FewMaps* M, in
         for (const cuuint64_t st : strides)
             if (st == 0 || st >= ((cuuint64_t)1 << 40)) return LB_OK;
         auto encode = [&] { return enc(i ? &M->v : &M->k, E5M2 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : A.dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(i ? A.v : A.k), dims, strides, boxes, unit,
-                                       CU_TENSOR_MAP_INTERLEAVE_NONE, F::kRow < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, F::kRow < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, F::kRow >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : F::kRow == 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B,
                                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
         CUresult r = encode();
         if (r == CUDA_ERROR_INVALID_CONTEXT) {                         // a thread before its first runtime call: bind its device's context
@@ -678,14 +729,15 @@ template <int DP, bool E5M2> int few_maps(const PagedAttnArgs& A, FewMaps* M, in
     return LB_OK;
 }
 
-template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, cudaStream_t st) {
+template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, bool eight, cudaStream_t st) {
     using F = Few<DP, E5M2>;
     static bool configured[64] = {};                                   // the attribute is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
         cudaFuncSetAttribute(paged_few_kernel<DP, BF, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-        cudaFuncSetAttribute(paged_few_tma_kernel<DP, BF, E5M2>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem + 1024);
+        cudaFuncSetAttribute(paged_few_tma_kernel<DP, BF, E5M2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem + 1024);
+        cudaFuncSetAttribute(paged_few_tma_kernel<DP, BF, E5M2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem + 1024);
         configured[dev & 63] = true;
     }
     const int C = sm_count();
@@ -694,16 +746,17 @@ template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, cudaStream
     if (const int rc = few_maps<DP, E5M2>(A, &M, &box)) return rc;
     if (box) {
         if (const int rc = make_waits(&A.waits, kWaitCycles)) return rc;
-        launch_behind(paged_few_tma_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32 + 32, F::kSmem + 1024, st, launch_overlaps(st), A, M, box);
+        launch_behind(eight ? paged_few_tma_kernel<DP, BF, E5M2, true> : paged_few_tma_kernel<DP, BF, E5M2, false>, dim3((unsigned)C), F::kWarps * 32 + 128, F::kSmem + 1024, st,
+                      launch_overlaps(st), A, M, box);
     } else launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
     note_launch();
     launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C), 256, 0, st, true, A, C);
     note_launch();
     return check_launch();
 }
-template <int DP> int few_launch_types(const PagedAttnArgs& A, cudaStream_t st) {
-    if (A.cache_dtype == CACHE_E5M2) return A.dtype == DT_BF16 ? few_launch<DP, true, true>(A, st) : few_launch<DP, false, true>(A, st);
-    return A.dtype == DT_BF16 ? few_launch<DP, true, false>(A, st) : few_launch<DP, false, false>(A, st);
+template <int DP> int few_launch_types(const PagedAttnArgs& A, bool eight, cudaStream_t st) {
+    if (A.cache_dtype == CACHE_E5M2) return A.dtype == DT_BF16 ? few_launch<DP, true, true>(A, eight, st) : few_launch<DP, false, true>(A, eight, st);
+    return A.dtype == DT_BF16 ? few_launch<DP, true, false>(A, eight, st) : few_launch<DP, false, false>(A, eight, st);
 }
 size_t few_part_bytes(int D) {
     const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
@@ -748,7 +801,8 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
     }
     A.part = (float*)workspace;
     cudaStream_t st = (cudaStream_t)stream;
-    if (const int rc = D <= 64 ? few_launch_types<64>(A, st) : D <= 128 ? few_launch_types<128>(A, st) : few_launch_types<256>(A, st)) return rc;
+    const bool eight = max_query * (Hq / Hkv) <= 8;                    // no unit has more rows, whoever else comes along
+    if (const int rc = D <= 64 ? few_launch_types<64>(A, eight, st) : D <= 128 ? few_launch_types<128>(A, eight, st) : few_launch_types<256>(A, eight, st)) return rc;
     if (max_query * (Hq / Hkv) <= FEW_ROWS) return LB_OK;
     A.part = (float*)((uint8_t*)workspace + few_part_bytes(D));
     return paged_prompt_launch(A, FEW_ROWS, st);
