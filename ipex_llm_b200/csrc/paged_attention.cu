@@ -642,29 +642,42 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
     const int64_t from = found_before + (int64_t)hk * places, to = from + places;
     if (first - from > FEW_EXTRA || last - from <= FEW_EXTRA || to <= last) return;        // its first tile is another block's, or it ends here
     const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // with fewer places than blocks some have none
+    auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
+    auto none = [&](int b) { return all < C && share_begin(all, b, C) == share_begin(all, b + 1, C); };
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int row = warp; row < rows; row += 8) {
-        auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
-        auto none = [&](int b) { return share_begin(all, b, C) == share_begin(all, b + 1, C); };
-        float top = -INFINITY;
-        for (int b = c; b <= end; b++)
+        float top = -INFINITY, total = 0.0f;
+        for (int b = c + lane; b <= end; b += 32)
             if (!none(b)) top = fmaxf(top, slot(b)[FEW_ROWS * DP + 2 * row]);
-        float total = 0.0f;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         float4 x[DP > 128 ? 2 : 1];
 #pragma unroll
         for (int z = 0; z < (DP > 128 ? 2 : 1); z++) x[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int b = c; b <= end; b++) {
-            if (none(b)) continue;
-            const float* const p = slot(b);
-            const float2 st = *reinterpret_cast<const float2*>(p + FEW_ROWS * DP + 2 * row);
-            const float w = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
-            total = fmaf(w, st.y, total);
+        for (int b0 = c; b0 <= end; b0 += 32) {
+            // a lane finds a part's weight, and all add up its values
+            float mine = 0.0f, part_sum = 0.0f;
+            const bool here = b0 + lane <= end && !none(b0 + lane);
+            if (here) {
+                const float2 st = *reinterpret_cast<const float2*>(slot(b0 + lane) + FEW_ROWS * DP + 2 * row);
+                mine = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
+                part_sum = st.y;
+            }
+            const uint32_t parts = __ballot_sync(0xffffffffu, here);
+#pragma unroll 4
+            for (int k = 0; k < 32 && b0 + k <= end; k++) {
+                const float w = __shfl_sync(0xffffffffu, mine, k);
+                total = fmaf(w, __shfl_sync(0xffffffffu, part_sum, k), total);
+                if (!(parts >> k & 1)) continue;
+                const float* const p = slot(b0 + k);
 #pragma unroll
-            for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
-                const int d = 4 * lane + 128 * z;
-                if (d >= DP) continue;
-                const float4 y = *reinterpret_cast<const float4*>(p + row * DP + d);
-                x[z].x = fmaf(w, y.x, x[z].x); x[z].y = fmaf(w, y.y, x[z].y); x[z].z = fmaf(w, y.z, x[z].z); x[z].w = fmaf(w, y.w, x[z].w);
+                for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
+                    const int d = 4 * lane + 128 * z;
+                    if (d >= DP) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(p + row * DP + d);
+                    x[z].x = fmaf(w, y.x, x[z].x); x[z].y = fmaf(w, y.y, x[z].y); x[z].z = fmaf(w, y.z, x[z].z); x[z].w = fmaf(w, y.w, x[z].w);
+                }
             }
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
