@@ -135,6 +135,7 @@ def build(force=False, verbose=False, ptxas_info=False):
 
 
 HOST_SRC = os.path.join(CSRC, "host", "linear_host.cpp")
+HOST_SRCS = [HOST_SRC, os.path.join(CSRC, "host", "paged_host.cpp")]
 
 
 def host_lib():
@@ -148,7 +149,8 @@ def build_host(force=False, verbose=False):
     """the CPython module behind LowBitLinear.forward (csrc/host).  Safe to call from several processes at once."""
     import sysconfig
     path = host_lib()
-    if not force and os.path.exists(path) and os.path.getmtime(path) >= os.path.getmtime(HOST_SRC):
+    deps = HOST_SRCS + [os.path.join(CSRC, "host", "paged_host.h")]
+    if not force and os.path.exists(path) and os.path.getmtime(path) >= max(map(os.path.getmtime, deps)):
         return path
     import torch
     from torch.utils import cpp_extension
@@ -159,12 +161,12 @@ def build_host(force=False, verbose=False):
     tmp = f"{path}.{os.getpid()}"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f for d in includes for f in ("-isystem", d)]
-    cmd += [HOST_SRC, "-o", tmp, "-L", lib_dir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib_dir}"]
+    cmd += HOST_SRCS + ["-o", tmp, "-L", lib_dir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib_dir}"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"g++ failed on {HOST_SRCS}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, path)
     return path
 

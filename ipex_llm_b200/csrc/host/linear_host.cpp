@@ -3,13 +3,14 @@
 // same took 20 us around a 4 us kernel.  A CPython module (b200_host); the kernels are reached through the addresses of
 // libb200lowbit.so's entry points, which the package hands over once.  Beside it, attention over the 8-bit cache (attention: the Python
 // statements took 24 us around kernels of 5 to 17 us) and the look at a mixture's experts that every call of theirs begins with
-// (expert_addresses).
+// (expert_addresses).  The paged cache's operators: paged_host.cpp.
 #include <vector>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include "paged_host.h"
 
 namespace {
 
@@ -238,6 +239,11 @@ PyMethodDef methods[] = {{"attach", attach, METH_VARARGS, nullptr},
                          {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
                          {"expert_addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(expert_addresses)), METH_FASTCALL, nullptr},
                          {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear)), METH_FASTCALL, nullptr},
+                         {"attach_paged", attach_paged, METH_VARARGS, nullptr},
+                         {"paged_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_step)), METH_FASTCALL, nullptr},
+                         {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_append)), METH_FASTCALL, nullptr},
+                         {"sdp_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sdp_paged)), METH_FASTCALL, nullptr},
+                         {"sdp_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sdp_packed)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

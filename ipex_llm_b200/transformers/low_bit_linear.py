@@ -60,6 +60,9 @@ def _load_host():
                                 for f in ("lowbit_matmul_cuda", "lowbit_matmul_workspace_size", "lowbit_hint_next_weights", "lowbit_sdp_fp8_cuda",
                                           "lowbit_sdp_fp8_supported", "lowbit_sdp_fp8_workspace_size", "lowbit_sdp_fp8_prefill_strided_cuda",
                                           "lowbit_sdp_fp8_prefill_supported")))
+                module.attach_paged(*(ctypes.cast(getattr(ggml._lib, f), ctypes.c_void_p).value
+                                      for f in ("lowbit_paged_step_cuda", "lowbit_paged_rope_append_cuda", "lowbit_sdp_paged_workspace_size", "lowbit_sdp_paged_cuda",
+                                                "lowbit_sdp_packed_workspace_size", "lowbit_sdp_packed_cuda")))
                 _host = module
             except Exception as e:
                 warnings.warn(f"the native host side of LowBitLinear and attention is not available, its Python statements run instead: {e}")

@@ -18,6 +18,7 @@ import torch
 from ipex_llm_b200.utils.common import invalidInputError, LazyModule
 
 ggml = LazyModule("ipex_llm_b200.ggml.model.llama.llama_cpp")      # loaded by the first call of one of its kernels
+linears = LazyModule("ipex_llm_b200.transformers.low_bit_linear")   # their native host side has these operators' too
 
 _HALF = (torch.float16, torch.bfloat16)
 
@@ -30,6 +31,15 @@ class PagedStep(NamedTuple):
     slots: torch.Tensor               # int64 [n_tokens]: its slot, -1 behind the last and where no page was to be had
     free_count: torch.Tensor          # int32 [1]: free pages left
     missing: torch.Tensor             # int32 [1]: pages that were not to be had
+
+
+def _native(name, *args):
+    """the plain call in one native call (csrc/host/paged_host.cpp); None where the statements here serve or refuse it"""
+    host = linears._host if linears._host is not None else linears._load_host()
+    out = getattr(host, name)(*args) if host else None
+    if type(out) is int:
+        ggml._check(out, "lowbit_" + name)
+    return out
 
 
 def _stream(device):
@@ -74,6 +84,9 @@ def paged_step(query_lens, context_lens, block_table, free_pages, free_count, pa
     int32 [1]: the stack that they come off, the last first; ``n_tokens``: rows of the step's activations (at least the sum of
     ``query_lens``: what is behind it is padding).  ``free_left``: where the number of pages left goes, a new tensor by default;
     ``free_count`` itself for a server's loop.  Returns a ``PagedStep``."""
+    out = _native("paged_step", query_lens, context_lens, block_table, free_pages, free_count, page_size, n_tokens, free_left)
+    if out is not None:
+        return PagedStep._make(out)
     R = query_lens.shape[0]
     dev = _device(query_lens, context_lens, block_table, free_pages, free_count)
     _ints(query_lens, R, "query_lens")
@@ -116,6 +129,8 @@ def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, s
     place, and the write of keys and values into their ``slots`` (int64 [T]; -1: not written).  ``cos`` / ``sin`` [positions, rotary width]
     in the rotate_half layout, indexed by ``positions`` (int64 [T]; beyond the tables: their last row); a rotary width below head_dim
     leaves the other elements; None: no rotation.  e5m2 caches keep the rounded activations' nearest value, saturating."""
+    if _native("paged_append", qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache) is not None:
+        return
     _no_grad(qkv)
     invalidInputError(qkv.dim() == 2 and qkv.dtype in _HALF and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and (qkv.stride(1) == 1 or qkv.numel() == 0),
                       f"qkv must be a half-precision [T, {(n_heads + 2 * n_kv_heads) * head_dim}] with contiguous rows")
@@ -170,6 +185,10 @@ def sdp_paged(query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=
     ``scaled_dot_product_attention``.  ``max_query_len``: no request brings more new tokens (1 for a decode step); never knowing is
     right, knowing saves launches.  A token that sees no key gives zeros; rows behind the last request are left as they are in
     ``out``, a new tensor by default.  Pages outside the cache (-1) make their request's rows NaN."""
+    if out is None:
+        result = _native("sdp_paged", query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_query_len)
+        if result is not None:
+            return result
     _no_grad(query, k_cache, v_cache)
     dev = _device(query, k_cache, v_cache, block_table, seq_lens, cu_seqlens)
     _table(block_table)
@@ -195,6 +214,10 @@ def sdp_packed(query, key, value, cu_seqlens, scale=None, is_causal=True, max_se
     """Attention of whole prompts that lie behind one another, each over itself: ``query`` [T, heads, head_dim], ``key`` / ``value``
     [T, kv_heads, head_dim] (views of the merged projection's output serve), prompt r = rows cu_seqlens[r] .. cu_seqlens[r + 1].
     ``max_seqlen``: no prompt is longer.  Rows behind the last prompt are left as they are in ``out``."""
+    if out is None:
+        result = _native("sdp_packed", query, key, value, cu_seqlens, scale, is_causal, max_seqlen)
+        if result is not None:
+            return result
     _no_grad(query, key, value)
     dev = _device(query, key, value, cu_seqlens)
     invalidInputError(key.dim() == 3 and key.shape == value.shape and key.shape[0] == query.shape[0] and key.shape[2] == query.shape[-1] and key.shape[1] > 0
