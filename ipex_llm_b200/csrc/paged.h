@@ -101,30 +101,27 @@ __device__ __forceinline__ int64_t block_before(int64_t x, int64_t* warps, int64
     return before + s - x;
 }
 // the whole block: tiles of all requests (count(r) of request r), and the request that holds tile `pick(total)` with the tiles before it.
-// Two walks over the requests when they are more than the threads
+// Two walks over the requests when they are more than the threads; one loop for both, since a block waits for this code to be fetched
+// before its first copy
 template <typename Count, typename Pick>
 __device__ __forceinline__ int64_t find_tile(int R, Count count, Pick pick, int64_t* warps, int* r_out, int64_t* before_out) {
-    int64_t all = 0, mine = 0, first = 0;
-    for (int r0 = 0; r0 < R; r0 += blockDim.x) {
-        const int r = r0 + threadIdx.x;
-        int64_t total;
-        mine = r < R ? count(r) : 0;
-        first = all + block_before(mine, warps, total);
-        all += total;
-    }
-    const int64_t want = all > 0 ? pick(all) : -1;
-    if (R <= (int)blockDim.x) {
-        if (mine > 0 && first <= want && want < first + mine) { *r_out = threadIdx.x; *before_out = first; }
-    } else {
-        int64_t sum = 0;
+    int64_t all = 0, sum = 0, want = -1;
+    const bool twice = R > (int)blockDim.x;
+#pragma unroll 1
+    for (int walk = twice ? 0 : 1; walk < 2; walk++) {
+        sum = 0;
+#pragma unroll 1
         for (int r0 = 0; r0 < R; r0 += blockDim.x) {
             const int r = r0 + threadIdx.x;
             int64_t total;
-            mine = r < R ? count(r) : 0;
-            first = sum + block_before(mine, warps, total);
+            const int64_t mine = r < R ? count(r) : 0;
+            const int64_t first = sum + block_before(mine, warps, total);
             sum += total;
+            if (!twice && sum > 0) want = pick(sum);
             if (mine > 0 && first <= want && want < first + mine) { *r_out = r; *before_out = first; }
         }
+        all = sum;
+        if (walk == 0 && all > 0) want = pick(all);
     }
     __syncthreads();
     return all;

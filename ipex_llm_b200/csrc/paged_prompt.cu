@@ -24,7 +24,8 @@ template <int DP, bool E5M2> struct Prompt {
     static constexpr int NT = DP == 256 ? 1 : 2, kRows = 128 * NT;
     static constexpr int kTile = 128 * DP * 2, kSlots = DP == 256 ? 2 : DP == 128 ? 4 : 8;
     static constexpr int kWarps = 4 * NT + 8;
-    static constexpr int kSmem = 1024 + (NT + kSlots) * kTile + 512;
+    static constexpr int kStageAt = (NT + kSlots) * kTile + 512;
+    static constexpr int kSmem = 1024 + kStageAt + 4 * NT * 4096;          // 4 KB a softmax warp for results on their way out
     // registers a thread: softmax, copies, MMAs (the launch's are 128 or 168)
     static constexpr int kSoftRegs = NT == 2 ? 152 : 232, kCopyRegs = NT == 2 ? 104 : 144, kMmaRegs = NT == 2 ? 104 : 128;
     static constexpr int64_t kPart = (int64_t)NT * 128 * (DP + 2);     // floats of a slot: [t][DP / 4][128] float4, [t][128] float2
@@ -88,31 +89,46 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // ------------------------------------------------------------------ the units and their key tiles
-// sum of floor((a i + b) / m) over i = 0 .. n - 1 (a, b >= 0), by the Euclidean exchange of a and m
-__device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-    int64_t s = 0;
-    while (n > 0) {
-        if (a >= m) { s += (int64_t)n * (n - 1) / 2 * (a / m); a %= m; }
-        if (b >= m) { s += (int64_t)n * (b / m); b %= m; }
-        const uint32_t y = a * n + b;                                  // at most the tokens of a request
-        if (y < m) break;
+// sum of floor((a i + b) / 128) over i = 0 .. n - 1, by the Euclidean exchange of a and the divisor; the first step, by 128, needs no division
+__device__ __forceinline__ int64_t floor_sum128(uint32_t n, uint32_t a, uint32_t b) {
+    if (n == 0) return 0;
+    int64_t s = (int64_t)n * (n - 1) / 2 * (a >> 7) + (int64_t)n * (b >> 7);
+    a &= 127u; b &= 127u;
+    uint32_t y = a * n + b, m = 128;                                   // at most the tokens of a request
+    while (y >= m) {
         n = y / m;
-        b = y % m;
+        b = y - n * m;
         const uint32_t h = m; m = a; a = h;
+        const uint32_t qa = a / m, qb = b / m;
+        s += (int64_t)n * (n - 1) / 2 * qa + (int64_t)n * qb;
+        a -= qa * m;
+        b -= qb * m;
+        y = a * n + b;
     }
     return s;
 }
+// What a unit costs beside its key tiles (queries, result, a pipeline that drains), in tiles: shares are taken of places, PR_EXTRA of them in
+// front of a unit's tiles, so that blocks with many short prompts are not the last
+constexpr int PR_EXTRA = 2;
+// A unit of up to so many key tiles is never split: it is the block's in whose share it begins.  A part costs a store and a load of its 32-bit
+// sums (128 KB a unit) and its merge, more than such a unit is worth
+constexpr int PR_WHOLE = 4;
 struct Units {
     int n, units, tpu, causal, off, len;                      // new tokens, units, tokens of a unit; keys before the first new token
     __device__ __forceinline__ Units(const PagedReq& q, int group, int rows, int causal_, int above) {
         tpu = rows / group;
         causal = causal_;
         n = (int64_t)q.n * group > above ? q.n : 0;
-        units = (n + tpu - 1) / tpu;
+        units = n > 0 ? (n - 1) / tpu + 1 : 0;
         len = q.len;
         off = q.len - q.n;
     }
@@ -121,42 +137,46 @@ struct Units {
         const int end = causal ? off + min((u + 1) * tpu, n) : len;
         return end <= PR_KEYS ? 1 : (end - 1) / PR_KEYS + 1;
     }
-    // ... of the first u units
-    __device__ __forceinline__ int64_t before(int u) const {
+    // places of the first u units
+    __device__ __forceinline__ int64_t before(int u) const { return tiles_before(u) + (int64_t)min(u, units) * PR_EXTRA; }
+    __device__ __forceinline__ int64_t tiles_before(int u) const {
         if (u <= 0) return 0;
         if (!causal) return (int64_t)u * tiles(0);
         const int last = u >= units ? tiles(units - 1) : 0;            // which may have fewer tokens
         if (u >= units) u = units - 1;
         // those whose last token has at most PR_KEYS keys count one each: (i + 1) tpu + off <= PR_KEYS
         const int room = PR_KEYS - off, ones = room < tpu ? 0 : min(u, room / tpu);
-        return last + ones + floor_sum(u - ones, PR_KEYS, tpu, (uint32_t)off + (uint32_t)(ones + 1) * tpu + PR_KEYS - 1);
+        return last + ones + floor_sum128(u - ones, tpu, (uint32_t)off + (uint32_t)(ones + 1) * tpu + PR_KEYS - 1);
     }
 };
 // a block's way through its share: pieces of units, key tiles a .. b - 1 of unit (r, hk, u)
 struct PromptAt {
     PagedReq q; int r, hk, u, units, tpu, a, b, tiles, left;
-    __device__ __forceinline__ void piece(const PagedAttnArgs& A, int group, int rows, int above) {
+    __device__ __forceinline__ bool piece(const PagedAttnArgs& A, int group, int rows, int above, int place) {
         const Units w(q, group, rows, A.causal, above);
         tiles = w.tiles(u);
-        b = min(tiles, a + left);
-        left -= b - a;
+        const int rest = tiles + PR_EXTRA - place, take = tiles <= PR_WHOLE ? rest : min(rest, left);
+        left -= take;
+        a = max(place - PR_EXTRA, 0);
+        b = max(place + take - PR_EXTRA, 0);
+        return a < b && (place == 0 || tiles > PR_WHOLE);
     }
     __device__ __forceinline__ bool next(const PagedAttnArgs& A, int group, int rows, int above) {
-        if (left <= 0) return false;
-        a = 0;
-        if (++u >= units) {
-            u = 0;
-            if (++hk >= A.Hkv) {
-                hk = 0;
-                do {
-                    if (++r >= A.R) return false;
-                    q = paged_req(A, r);
-                    units = Units(q, group, rows, A.causal, above).units;
-                } while (units == 0);
+        while (left > 0) {
+            if (++u >= units) {
+                u = 0;
+                if (++hk >= A.Hkv) {
+                    hk = 0;
+                    do {
+                        if (++r >= A.R) return false;
+                        q = paged_req(A, r);
+                        units = Units(q, group, rows, A.causal, above).units;
+                    } while (units == 0);
+                }
             }
+            if (piece(A, group, rows, above, 0)) return true;
         }
-        piece(A, group, rows, above);
-        return true;
+        return false;
     }
     // key tiles that the rows of tile t need, and whether the piece has any of them
     __device__ __forceinline__ int tiles_of(const PagedAttnArgs& A, int group, int t) const {
@@ -167,12 +187,12 @@ struct PromptAt {
         return keys <= 0 ? 0 : (keys - 1) / PR_KEYS + 1;
     }
 };
-// blocks that share n tiles: none takes less than a few, the price of a piece
-__device__ __forceinline__ int sharers(int64_t n, int C) { return (int)min((int64_t)C, (n + 1) >> 1); }
+// blocks that share n places: none takes fewer than three, which cost about what a part of a unit adds
+__device__ __forceinline__ int sharers(int64_t n, int C) { return n < 3 * (int64_t)C ? max((int)n / 3, 1) : C; }
 
-// the whole block: where tile `pick` of all lies; `all` = tiles of all units
+// the whole block: where place `pick` of all lies (`place` of its unit); `all` = places of all units
 template <typename Pick>
-__device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group, int rows, int above, Pick pick, int64_t* scan, int* found_r, int64_t* found_before, PromptAt& at) {
+__device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group, int rows, int above, Pick pick, int64_t* scan, int* found_r, int64_t* found_before, PromptAt& at, int& place) {
     int64_t want = 0;
     const int64_t all = find_tile(A.R, [&](int r) { const Units w(paged_req(A, r), group, rows, A.causal, above); return w.before(w.units) * A.Hkv; },
                                   [&](int64_t n) { return want = pick(n); }, scan, found_r, found_before);
@@ -185,16 +205,31 @@ __device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group,
     const int64_t per = w.before(w.units), x = want - *found_before;
     int64_t y;
     at.hk = div_few(x, per, y);
-    // the last unit that begins at y or before: a warp's lanes look at 32 places at a time
-    int lo = 0, hi = w.units;                                          // before(lo) <= y < before(hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, u = lo + step * (int)(threadIdx.x & 31);
-        const uint32_t yes = __ballot_sync(0xffffffffu, u < hi && w.before(u) <= y);
-        lo += step * (31 - __clz(yes));
-        hi = min(hi, lo + step);
+    // the last unit that begins at y or before.  Places up to unit u grow with u^2: the 32 units around the root of that are looked at first,
+    // one a lane, and 32 places of what is left at a time if it is none of them
+    int lo = 0, hi = w.units, from = 0, step = 1;                      // before(lo) <= y < before(hi)
+    int64_t reached = 0;                                               // before(lo)
+    if (hi > 32) {
+        const float q = A.causal ? w.tpu / 256.0f : 0.0f, l = PR_EXTRA + 0.5f + (A.causal ? (w.off + 0.5f * w.tpu) / PR_KEYS : (float)w.tiles(0) - 0.5f);
+        const float root = q > 0.0f ? (sqrtf(fmaxf(l * l + 4.0f * q * (float)y, 0.0f)) - l) / (2.0f * q) : (float)y / l;
+        from = max(0, min(hi - 32, (int)root - 16));
     }
+#pragma unroll 1
+    do {
+        const int u = from + step * (int)(threadIdx.x & 31);
+        const int64_t mine = w.before(u);
+        const uint32_t yes = __ballot_sync(0xffffffffu, u < hi && mine <= y);
+        if (yes) {
+            const int l = 31 - __clz(yes);
+            lo = from + step * l;
+            reached = __shfl_sync(0xffffffffu, mine, l);
+            if (l < 31) hi = min(hi, lo + step);
+        } else hi = from;
+        from = lo;
+        step = (hi - lo + 31) / 32;
+    } while (hi - lo > 1);
     at.u = lo;
-    at.a = (int)(y - w.before(lo));
+    place = (int)(y - reached);
     return all;
 }
 
@@ -243,10 +278,10 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     PromptAt at;
-    int C = gridDim.x, issued = 0;
+    int C = gridDim.x, issued = 0, place = 0;
     const int c = blockIdx.x;
     const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, gridDim.x); return c < C ? share_begin(n, c, C) : -1; }, scan, &found_r,
-                                   &found_before, at);
+                                   &found_before, at, place);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -255,8 +290,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
     // not before every block holds its columns: a dependent that allocates in front of its wait must find nobody who still wants some
     asm volatile("griddepcontrol.launch_dependents;");
     at.left = all > 0 && c < C ? (int)(share_begin(all, c + 1, C) - share_begin(all, c, C)) : 0;
-    const bool any = at.left > 0;
-    if (any) at.piece(A, group, P::kRows, above);
+    const bool any = at.left > 0 && (at.piece(A, group, P::kRows, above, place) || at.next(A, group, P::kRows, above));
 
     if (warp < 4 * NT) {
         // ================= softmax: thread = row =================
@@ -264,11 +298,11 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         const int t = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
         const uint32_t st = tmem + lanes + t * 128, ot = tmem + lanes + NT * 128 + t * DP;
+        const uint32_t stage = base + P::kStageAt + warp * 4096;
         uint32_t steps = 0;                                            // key tiles so far
         float mul = A.scale_log2e;
         // the unit's queries into tile t: the products that read the last ones are done
         auto queries = [&](const PromptAt& w) {
-            if (min(w.b, w.tiles_of(A, group, t)) <= w.a) return;      // no key of the piece for this tile: nobody waits for it
             const int row = 128 * t + r, first = w.u * w.tpu, token = first + row / group;
             const bool live = row < w.tpu * group && token < w.q.n;
             const int64_t from = live ? (w.q.q0 + token) * A.q_st + (int64_t)(w.hk * group + row % group) * A.q_sh : -1;
@@ -302,14 +336,18 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                     const int64_t o = __shfl_sync(0xffffffffu, from, l);
                     if (piece * 8 < A.D) cp16(dst + (piece >> 3) * HALF + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4), (const uint16_t*)A.q + (o < 0 ? 0 : o) + piece * 8, o < 0 ? 0u : 16u);
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
             }
+        };
+        auto hand_over = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full(t));
         };
+        // whether the piece has keys for this tile: else nobody waits for its queries
+        auto needed = [&](const PromptAt& w) { return min(w.b, w.tiles_of(A, group, t)) > w.a; };
         if (any) {
-            queries(at);
+            if (needed(at)) { queries(at); hand_over(); }
             for (bool more = true; more;) {
                 const int row = 128 * t + r, first = at.u * at.tpu, token = first + row / group;
                 const bool live = row < at.tpu * group && token < at.q.n;
@@ -318,12 +356,17 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 // keys below: every row of the warp sees them (rows behind the unit's are nobody's)
                 const int plain_end = A.causal ? off + first + (128 * t + 32 * quarter) / group + 1 : at.q.len;
                 const int end = min(at.b, at.tiles_of(A, group, t));
+                const bool some = end > at.a, from_start = at.a == 0, whole = from_start && at.b == at.tiles;
+                const int64_t oi = live ? (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh : -1;
                 float m_ref = -INFINITY, sum = 0.0f;
-                for (int j = at.a; j < end; j++, steps++) {
+                const int start = at.a;
+                more = at.next(A, group, P::kRows, above);             // in the time that the first scores take
+                const bool coming = more && needed(at);                // the next piece's queries
+                for (int j = start; j < end; j++, steps++) {
                     if (!mbar_wait_lim(s_full(t), steps & 1, A.waits)) goto done;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    // 64 scores in registers at a time (128 spilled): the maximum of the first half, of the second, whose exponentials
-                    // follow at once, then those of the first, read again
+                    // 64 scores in registers at a time, by loops that are not unrolled: the roles share an instruction cache, and this one in a
+                    // row, three loads instead of four, took 640 us where this takes 553 (8000 tokens, 32 heads)
                     const bool plain = j < plain_end / PR_KEYS;
                     const int left = n_vis - j * PR_KEYS;
                     float x[64], m0, m1, m2, m3;
@@ -336,18 +379,18 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                             for (int i = 0; i < 64; i++) x[i] = 64 * h + i < left ? x[i] : -INFINITY;
                         }
                     };
-                    load(0);
-                    m0 = x[0]; m1 = x[1]; m2 = x[2]; m3 = x[3];
+                    m0 = m1 = m2 = m3 = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
+                        load(h);
 #pragma unroll
-                    for (int i = 4; i < 64; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
-                    load(1);
-#pragma unroll
-                    for (int i = 0; i < 64; i += 4) { m0 = fmaxf(m0, x[i]); m1 = fmaxf(m1, x[i + 1]); m2 = fmaxf(m2, x[i + 2]); m3 = fmaxf(m3, x[i + 3]); }
+                        for (int i = 0; i < 64; i += 8) { m0 = max3(m0, x[i], x[i + 1]); m1 = max3(m1, x[i + 2], x[i + 3]); m2 = max3(m2, x[i + 4], x[i + 5]); m3 = max3(m3, x[i + 6], x[i + 7]); }
+                    }
                     const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * mul;
                     const bool grow = mx > m_ref + 6.0f;                           // -inf: any visible key
                     if (__any_sync(0xffffffffu, grow)) {
                         const float m_new = grow ? mx : m_ref;
-                        if (j > at.a) {
+                        if (j > start) {
                             // the P . V before this Q . K is done: O is at rest
                             const float corr = grow ? ex2(m_ref - m_new) : 1.0f;
                             sum *= corr;
@@ -383,46 +426,49 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                         __syncwarp();
                         if (lane == 0) mbar_arrive(p_full(t, h));
                     };
-                    exponentials(1);
-                    load(0);
-                    exponentials(0);
+#pragma unroll 1
+                    for (int h = 0; h < 2; h++) {
+                        load(h);
+                        exponentials(h);
+                    }
                     sum += (a0 + a1) + (a2 + a3);
                 }
-                // the next unit's queries, while this one's last product runs
-                const PromptAt was = at;
-                more = at.next(A, group, P::kRows, above);
-                if (more) queries(at);
-                const bool some = end > was.a, whole = was.a == 0 && was.b == was.tiles;
+                if (coming) queries(at);                               // the last product with the old ones is done
                 if (some) {
                     if (!mbar_wait_lim(pv_done(t), (steps - 1) & 1, A.waits)) goto done;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
+                if (coming) hand_over();
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;                 // a row without a key gives zeros
-                const int64_t oi = (was.q.q0 + token) * A.o_st + (int64_t)(was.hk * group + row % group) * A.o_sh;
-                float* const part = A.part + ((int64_t)c * 2 + (was.a == 0 ? 1 : 0)) * P::kPart;
+                float* const part = A.part + ((int64_t)c * 2 + (from_start ? 1 : 0)) * P::kPart;
 #pragma unroll 1
-                for (int i = 0; i < DP; i += 32) {
-                    float o[32];
+                for (int i = 0; i < DP; i += 64) {
+                    float o[64];
                     if (some) {
                         tmem_ld32x(ot + i, o);
+                        tmem_ld32x(ot + i + 32, o + 32);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = 0.0f;
+                        for (int e = 0; e < 64; e++) o[e] = 0.0f;
                     }
                     if (whole) {
-                        if (live) {
-                            uint4* p = reinterpret_cast<uint4*>((uint16_t*)A.out + oi + i);
+                        // through shared memory, so that a store writes four rows of 128 bytes and not 32 of 16
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (i + 8 * e < A.D)
-                                    p[e] = make_uint4(pack2<BF>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<BF>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                                      pack2<BF>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<BF>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                        for (int e = 0; e < 8; e++)
+                            sts4(stage + lane * 128 + ((e ^ (lane & 7)) << 4), pack2<BF>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<BF>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                 pack2<BF>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<BF>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int l = 4 * e + (lane >> 3), piece = lane & 7;
+                            const int64_t to = __shfl_sync(0xffffffffu, oi, l);
+                            if (to >= 0 && i + 8 * piece < A.D) *reinterpret_cast<uint4*>((uint16_t*)A.out + to + i + 8 * piece) = lds128(stage + l * 128 + ((piece ^ (l & 7)) << 4));
                         }
                     } else if (some) {
                         float4* p = reinterpret_cast<float4*>(part) + (int64_t)(t * (DP / 4) + i / 4) * 128 + r;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) p[e * 128] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int e = 0; e < 16; e++) p[e * 128] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                     __syncwarp();
                 }
@@ -447,7 +493,8 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
             const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
             if (PAGED && more && key < at.q.len) page = A.table[at.r * A.table_stride + (int)key / A.page_size];
         };
-        auto place = [&]() {                                           // of this lane's key, and on to the next tile
+        bool more_keys = any, over = false;                            // tiles behind the one that was placed; behind the last item
+        auto where = [&]() {                                           // this lane's key lies, and on to the next tile
             const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
             const bool here = key < at.q.len;
             if (PAGED) {
@@ -467,14 +514,16 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 more = at.next(A, group, P::kRows, above);
                 j = at.a;
             }
+            more_keys = more;
             ask();
         };
-        const uint32_t total = any ? (uint32_t)(share_begin(all, c + 1, C) - share_begin(all, c, C)) : 0u, items = A.waits.limit < 0 ? total : 2 * total;
+        uint32_t left = any ? A.waits.limit < 0 ? (uint32_t)(share_begin(all, c + 1, C) - share_begin(all, c, C)) : 0xffffffffu : 0u;      // items, two a tile
+        uint32_t item = 0;
         ask();
         if (E5M2) {
             uint4 w[PASSES];
             auto fetch = [&](uint32_t item) {
-                if (!(item & 1)) place();
+                if (!(item & 1)) where();
                 const uint8_t* const src = (const uint8_t*)((item & 1) ? A.v : A.k);
                 const uint32_t none = (item & 1) ? 0x7f7f7f7fu : 0u;
 #pragma unroll
@@ -487,8 +536,8 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                     if (s == 1 && piece < live) w[i] = *reinterpret_cast<const uint4*>(src + o + piece * 16);
                 }
             };
-            if (items > 0) fetch(0);
-            for (uint32_t item = 0; item < items; item++) {
+            if (any) fetch(0);
+            for (; !over && left > 0; item++, left--) {
                 const int s = item % SLOTS;
                 const uint32_t round = item / SLOTS;
                 if (!mbar_wait_lim(kv_empty(s), (round & 1) ^ 1, A.waits)) goto done;
@@ -503,7 +552,8 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                         sts4(b, __byte_perm(w[i].z, 0u, 0x1404u), __byte_perm(w[i].z, 0u, 0x3424u), __byte_perm(w[i].w, 0u, 0x1404u), __byte_perm(w[i].w, 0u, 0x3424u));
                     }
                 }
-                if (item + 1 < items) fetch(item + 1);
+                if ((item & 1) && !more_keys) over = true;
+                else fetch(item + 1);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kv_full(s));
@@ -511,11 +561,12 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         } else {
             // a warp's 32 rows: boxes of rows that lie in one page by TMA (box: 8, 16 or 32 rows; 0: the layout allows none), in the order of
             // the ring.  What may not reach a product, values behind the last key, is written as zeros: such rows are copied one by one
-            for (uint32_t item = 0; item < items; item++) {
+            for (; !over && left > 0; item++, left--) {
                 const int s = item % SLOTS;
                 const bool is_v = item & 1;
                 issued = item;
-                if (!is_v) place();
+                if (!is_v) where();
+                else over = !more_keys;
                 if (!mbar_wait_lim(kv_empty(s), ((item / SLOTS) & 1) ^ 1, A.waits)) goto done;
                 const uint32_t dst = ring + s * TILE;
                 if (box && (!is_v || __all_sync(0xffffffffu, state == 1))) {
@@ -555,7 +606,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kv_full(s));
             }
-            issued = items;
+            issued = item;
         }
     } else {
         regs_dec<P::kMmaRegs>();
@@ -583,7 +634,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 const uint64_t vd = (make_desc(slot(i)) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(HALF >> 4) << 16);
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 64 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 1 && k == 0 ? 0u : 1u, leader);
+                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 64 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 0 && k == 0 ? 0u : 1u, leader);
             };
             for (;;) {
                 // lane 0's, so that the compiler knows them to be the warp's: operands that it takes for a lane's own cost a move per MMA
@@ -607,7 +658,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                         if (j >= end[t]) continue;
                         if (j == a && turns[t]++ > 0 && !mbar_wait_lim(o_free(t), turns[t] & 1, A.waits)) goto done;
 #pragma unroll
-                        for (int h = 1; h >= 0; h--) {
+                        for (int h = 0; h < 2; h++) {
                             if (!mbar_wait_lim(p_full(t, h), steps[t] & 1, A.waits)) goto done;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                             values(t, item + 1, h, j == a);
@@ -658,14 +709,17 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_
     const int group = A.Hq / A.Hkv, c = blockIdx.x;
     int C = blocks;
     PromptAt at;
+    int place = 0;
     // written by what ran before the kernel in front, which has waited for it
     const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, blocks); return c < C ? share_begin(n, c + 1, C) - 1 : -1; }, scan, &found_r,
-                                   &found_before, at);
+                                   &found_before, at, place);
     if (all == 0 || c >= C) return;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
     if (first == last) return;
-    const int64_t tiles = Units(at.q, group, P::kRows, A.causal, above).tiles(at.u), from = last - 1 - at.a, to = from + tiles;
-    if (from < first || to <= last) return;                            // began earlier, or ends here
+    const int tiles = Units(at.q, group, P::kRows, A.causal, above).tiles(at.u);
+    if (tiles <= PR_WHOLE) return;
+    const int64_t from = last - 1 - place, to = from + PR_EXTRA + tiles;
+    if (first - from > PR_EXTRA || last - from <= PR_EXTRA || to <= last) return;          // its first tile is another block's, or it ends here
     const int end = share_of(to - 1, all, C), t = threadIdx.x >> 7, r = threadIdx.x & 127, row = threadIdx.x, token = at.u * at.tpu + row / group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= at.tpu * group || token >= at.q.n) return;
@@ -679,21 +733,25 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     uint16_t* const dst = (uint16_t*)A.out + (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh;
-    const int per = DP / gridDim.y, d0 = blockIdx.y * per;
-    for (int d = d0; d < d0 + per && d < A.D; d += 8) {
-        float x[8] = {};
-        for (int b = c; b <= end; b++) {
-            const float2 s = stat(b);
-            if (s.y == 0.0f) continue;                                 // no key for this row: nothing was stored
-            const float w = s.x == -INFINITY ? s.y : ex2(s.x - top);
-            const float4* p = reinterpret_cast<const float4*>(slot(b)) + (int64_t)(t * (DP / 4) + d / 4) * 128 + r;
-            const float4 y = p[0], z = p[128];
-            x[0] = fmaf(w, y.x, x[0]); x[1] = fmaf(w, y.y, x[1]); x[2] = fmaf(w, y.z, x[2]); x[3] = fmaf(w, y.w, x[3]);
-            x[4] = fmaf(w, z.x, x[4]); x[5] = fmaf(w, z.y, x[5]); x[6] = fmaf(w, z.z, x[6]); x[7] = fmaf(w, z.w, x[7]);
+    constexpr int PER = DP / 4;                                        // columns of this block
+    const int d0 = blockIdx.y * PER;
+    float x[PER] = {};
+    for (int b = c; b <= end; b++) {
+        const float2 s = stat(b);
+        if (s.y == 0.0f) continue;                                     // no key for this row: nothing was stored
+        const float w = s.x == -INFINITY ? s.y : ex2(s.x - top);
+        const float4* p = reinterpret_cast<const float4*>(slot(b)) + (int64_t)(t * (DP / 4) + d0 / 4) * 128 + r;
+#pragma unroll
+        for (int i = 0; i < PER / 4; i++) {
+            const float4 y = p[i * 128];
+            x[4 * i] = fmaf(w, y.x, x[4 * i]); x[4 * i + 1] = fmaf(w, y.y, x[4 * i + 1]); x[4 * i + 2] = fmaf(w, y.z, x[4 * i + 2]); x[4 * i + 3] = fmaf(w, y.w, x[4 * i + 3]);
         }
-        *reinterpret_cast<uint4*>(dst + d) = make_uint4(pack2<BF>(x[0] * inv, x[1] * inv), pack2<BF>(x[2] * inv, x[3] * inv), pack2<BF>(x[4] * inv, x[5] * inv),
-                                                        pack2<BF>(x[6] * inv, x[7] * inv));
     }
+#pragma unroll
+    for (int i = 0; i < PER; i += 8)
+        if (d0 + i < A.D)
+            *reinterpret_cast<uint4*>(dst + d0 + i) = make_uint4(pack2<BF>(x[i] * inv, x[i + 1] * inv), pack2<BF>(x[i + 2] * inv, x[i + 3] * inv),
+                                                                 pack2<BF>(x[i + 4] * inv, x[i + 5] * inv), pack2<BF>(x[i + 6] * inv, x[i + 7] * inv));
 }
 
 // boxes of 64 elements x `box` rows: rows that are a multiple of it apart never share one with another page; 0 rows where the strides of a
