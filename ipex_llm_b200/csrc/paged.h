@@ -31,7 +31,8 @@ __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& A, int r) {
     const int64_t e = b < q.q0 ? q.q0 : b > A.T ? A.T : b;
     q.n = (int)(e - q.q0);
     if (A.table) {
-        const int64_t held = A.seq_lens[r], most = (int64_t)A.width * A.page_size;
+        // tokens behind row T are not there, and the others see what they would with them
+        const int64_t held = A.seq_lens[r] - (b > A.T ? b - (a > A.T ? a : A.T) : 0), most = (int64_t)A.width * A.page_size;
         q.len = (int)(held < 0 ? 0 : held > most ? most : held);
     } else q.len = q.n;
     return q;

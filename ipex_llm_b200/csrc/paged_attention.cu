@@ -601,7 +601,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
                 w.begin(A, at.q, at.hk, group, g, t);
             }
             // a wait that ran out in one warp ends them all; they go through the motions, because they meet at barriers
-            if (!gave_up && !mbar_wait_lim(full(s), (i / ST) & 1, A.waits)) gave_up = 1;
+            if (!__any_sync(0xffffffffu, gave_up) && !mbar_wait_lim(full(s), (i / ST) & 1, A.waits)) gave_up = 1;
             const int key0 = at.tile * F::kTile + warp * KW;
             const uint32_t ks = ring + s * (2 * TILE);
             if (key0 < at.q.len) {
@@ -629,18 +629,20 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
     __shared__ int found_r;
     __shared__ int64_t found_before;
     const int group = A.Hq / A.Hkv, c = blockIdx.x;
-    // written by what ran before the kernel in front, which has waited for it
+    // a block waits before it leaves too: what comes behind in the stream may wait for this kernel alone
+    auto leave = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    // the lists were written by what ran before the kernel in front, which has waited for it
     const int64_t all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, F::kTile); },
                                   [&](int64_t n) { return share_begin(n, c + 1, C) - 1; }, scan, &found_r, &found_before);
-    if (all == 0) return;
+    if (all == 0) return leave();
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return;
+    if (first == last) return leave();
     const PagedReq q = paged_req(A, found_r);
     const int places = few_tiles(q, group, F::kTile) + FEW_EXTRA;
     int64_t within;
     const int hk = div_few(last - 1 - found_before, places, within);
     const int64_t from = found_before + (int64_t)hk * places, to = from + places;
-    if (first - from > FEW_EXTRA || last - from <= FEW_EXTRA || to <= last) return;        // its first tile is another block's, or it ends here
+    if (first - from > FEW_EXTRA || last - from <= FEW_EXTRA || to <= last) return leave();        // its first tile is another block's, or it ends here
     const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // with fewer places than blocks some have none
     auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };

@@ -710,16 +710,18 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_
     int C = blocks;
     PromptAt at;
     int place = 0;
-    // written by what ran before the kernel in front, which has waited for it
+    // a block waits before it leaves too: what comes behind in the stream may wait for this kernel alone
+    auto leave = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    // the lists were written by what ran before the kernel in front, which has waited for it
     const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, blocks); return c < C ? share_begin(n, c + 1, C) - 1 : -1; }, scan, &found_r,
                                    &found_before, at, place);
-    if (all == 0 || c >= C) return;
+    if (all == 0 || c >= C) return leave();
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return;
+    if (first == last) return leave();
     const int tiles = Units(at.q, group, P::kRows, A.causal, above).tiles(at.u);
-    if (tiles <= PR_WHOLE) return;
+    if (tiles <= PR_WHOLE) return leave();
     const int64_t from = last - 1 - place, to = from + PR_EXTRA + tiles;
-    if (first - from > PR_EXTRA || last - from <= PR_EXTRA || to <= last) return;          // its first tile is another block's, or it ends here
+    if (first - from > PR_EXTRA || last - from <= PR_EXTRA || to <= last) return leave();          // its first tile is another block's, or it ends here
     const int end = share_of(to - 1, all, C), t = threadIdx.x >> 7, r = threadIdx.x & 127, row = threadIdx.x, token = at.u * at.tpu + row / group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (row >= at.tpu * group || token >= at.q.n) return;

@@ -560,6 +560,76 @@ def test_on_other_streams_at_once(paged, cuda_device):
     assert all(torch.equal(x, w) for keep, w in zip(got, want) for x in keep)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("new,rows", [([3, 9], 5), ([40, 300, 7], 200), ([1, 1, 1], 2)])
+def test_tokens_behind_the_last_row(paged, cuda_device, dtype, eight, new, rows):
+    """a list that names more rows than there are: those that are there see the keys that they would see with the others"""
+    q, caches, table, lens, cu = requests(cuda_device, new, [100 + 30 * i for i in range(len(new))], 4, 2, 64, dtype, eight, 16)[:5]
+    there = cu.clamp(max=rows)
+    fewer = lens - (cu - there).diff()
+    want = paged.sdp_paged(q[:rows], *caches, table, fewer, there)
+    assert torch.equal(paged.sdp_paged(q[:rows], *caches, table, lens, cu), want) and not bool(torch.isnan(want).any())
+
+
+# ------------------------------------------------------------------ waits
+def waiting_calls(paged, dev):
+    t, b = torch.float16, torch.bfloat16
+    sets = {"tokens": requests(dev, [1] * 40, [2500] * 40, 8, 2, 128, b, False, 16), "tokens, e5m2": requests(dev, [1] * 40, [2500] * 40, 8, 2, 128, t, True, 16),
+            "chunk": requests(dev, [600], [3000], 8, 2, 128, b, False, 16), "chunk, e5m2": requests(dev, [600], [3000], 8, 2, 128, b, True, 16),
+            "chunk without boxes": requests(dev, [600], [3000], 8, 2, 64, t, False, 4)}
+    calls = {name: lambda s=s: paged.sdp_paged(s[0], *s[1], s[2], s[3], s[4]) for name, s in sets.items()}
+    q = torch.randn(3000, 12, 64, generator=torch.Generator(device=dev).manual_seed(4), device=dev).to(t)
+    cu = torch.tensor([0, 900, 3000], dtype=torch.int32, device=dev)
+    return {**calls, "prompts": lambda: paged.sdp_packed(q[:, :4], q[:, 4:8], q[:, 8:], cu)}
+
+
+WAITING = ["tokens", "tokens, e5m2", "chunk", "chunk, e5m2", "chunk without boxes", "prompts"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clocks", [20, 100000])
+@pytest.mark.parametrize("name", WAITING)
+def test_a_wait_that_runs_out_is_reported_once(paged, native_lib, cuda_device, name, clocks):
+    """below zero half of a launch's copies never come, and the waits for them run out after that many clocks; the next call says so, and
+    the one after is right"""
+    call = waiting_calls(paged, cuda_device)[name]
+    want = call()
+    assert not native_lib.lowbit_gemm_wait_expired()
+    native_lib._lib.lowbit_debug_set_wait_limit(-clocks)
+    try:
+        call()
+    finally:
+        native_lib._lib.lowbit_debug_set_wait_limit(0)
+    assert native_lib.lowbit_gemm_wait_expired()
+    with pytest.raises(native_lib.LowBitNativeError, match="ran out"):
+        call()
+    assert not native_lib.lowbit_gemm_wait_expired()
+    assert torch.equal(call(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clocks", [1, 300, 1500, 6000, 30000])
+@pytest.mark.parametrize("name", WAITING)
+def test_wherever_a_wait_runs_out_the_next_call_is_right(paged, native_lib, cuda_device, name, clocks):
+    """limits of the order of the kernels' own waits: they run out in the middle of the work, or not at all"""
+    call = waiting_calls(paged, cuda_device)[name]
+    want = call()
+    for _ in range(2):
+        native_lib._lib.lowbit_debug_set_wait_limit(clocks)
+        try:
+            call()
+        except native_lib.LowBitNativeError as e:
+            assert "ran out" in str(e)
+        finally:
+            native_lib._lib.lowbit_debug_set_wait_limit(0)
+        if native_lib.lowbit_gemm_wait_expired():
+            with pytest.raises(native_lib.LowBitNativeError, match="ran out"):
+                call()
+            torch.cuda.synchronize()
+        assert torch.equal(call(), want)
+
+
 # ------------------------------------------------------------------ what is refused
 def test_refusals_without_a_device(native_lib):
     """bad arguments are refused before anything touches a device"""
