@@ -45,8 +45,8 @@ int paged_prompt_launch(PagedAttnArgs A, int above, cudaStream_t st);
 
 // ---- work in equal shares.  The tiles of all units (a request's kv head; or a block of its rows on one) lie behind one another, n of them
 // in all, and block c of C takes tiles c n / C .. (c + 1) n / C: whatever the lengths, every block reads as many.  A unit whose tiles
-// lie in several blocks leaves its sums there, each block's slot 1 for a unit that began in it and slot 0 for one that did not, and the
-// merge adds them up in the order of the keys.
+// lie in several blocks leaves its sums there, each block's slot 1 for a unit that began in it and slot 0 for one that did not, and a note
+// in the block that it began in; the merge adds them up in the order of the keys.
 // Divisions are written out in 32 bits: a 64-bit one is a call, and a kernel that calls anything keeps the registers of its launch
 // (setmaxnreg is ignored).
 __device__ __forceinline__ uint64_t div_small(uint64_t n, uint32_t d, uint32_t& rem) {      // d < 2^16, 16 bits at a time
@@ -79,6 +79,14 @@ __device__ __forceinline__ int div_few(int64_t x, int64_t y, int64_t& rem) {    
     while ((q + 1) * y <= x) q++;
     rem = x - q * y;
     return q;
+}
+
+// Of block c: the unit that began in it and goes on in others, to block `end`.  Rows are (token, head of the group).  The merge could find all
+// this out from the lists, but starts when the block's registers are free, and then every clock counts
+struct __align__(16) SplitNote { int rows, hk, end, few; int64_t q0, unused; };         // rows 0: there is none; few: places of all, where blocks have none
+// b of the unit's tiles were in block c
+__device__ __forceinline__ SplitNote split_note(int rows, int hk, int64_t q0, int b, int tiles, int64_t all, int c, int C) {
+    return {rows, hk, share_of(share_begin(all, c + 1, C) - b + tiles - 1, all, C), all < C ? (int)all : 0, q0, 0};
 }
 
 // sum over the block before this thread, and of all of it

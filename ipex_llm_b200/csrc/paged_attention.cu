@@ -125,9 +125,10 @@ __device__ __forceinline__ int64_t few_places(const PagedReq& q, const PagedAttn
     const int tiles = few_tiles(q, group, tile);
     return tiles ? (int64_t)(tiles + FEW_EXTRA) * A.Hkv : 0;
 }
+template <int DP, bool E5M2> __device__ __forceinline__ SplitNote* few_notes(const PagedAttnArgs& A, int C) { return reinterpret_cast<SplitNote*>(A.part + (int64_t)C * 2 * Few<DP, E5M2>::kPart); }
 // the whole block: where its share begins; false: it has none
-__device__ __forceinline__ bool few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at) {
-    const int64_t all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, tile); }, [&](int64_t n) { return share_begin(n, c, C); }, scan, found_r,
+__device__ __forceinline__ bool few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at, int64_t& all) {
+    all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, tile); }, [&](int64_t n) { return share_begin(n, c, C); }, scan, found_r,
                                   found_before);
     if (all == 0) return false;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
@@ -443,7 +444,9 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     asm volatile("griddepcontrol.launch_dependents;");
     const int C = gridDim.x, c = blockIdx.x;
     FewAt at;                                                          // of the products
-    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at)) return;
+    int64_t all;
+    if (threadIdx.x == 0) few_notes<DP, E5M2>(A, C)[c].rows = 0;
+    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at, all)) return;
     FewAt in = at;                                                     // of the copies
     bool to_copy = true;
 
@@ -501,6 +504,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
         if (!begun) {
             begun = true;
             from_start = at.tile == 0;
+            if (from_start && at.end < at.tiles && threadIdx.x == 0) few_notes<DP, E5M2>(A, C)[c] = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
             w.begin(A, at.q, at.hk, group, g, t);
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
@@ -548,7 +552,10 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
     }
     const int C = gridDim.x, c = blockIdx.x;
     FewAt at;
-    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at)) return;
+    int64_t all;
+    const bool notes = threadIdx.x == NW * 32;
+    if (notes) few_notes<DP, E5M2>(A, C)[c].rows = 0;
+    if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at, all)) return;
     if (warp >= NW) {
         // ================= the copies: this warp's boxes of a tile =================
         const int boxes = F::kTile / box, own = max(boxes / 4, 1), mine = own * (warp - NW) + lane, most = A.waits.limit < 0 ? at.left / 2 : 0x7fffffff;
@@ -582,6 +589,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
                         asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                                      ::"r"(dst + v * TILE + h * (F::kTile * 128)), "l"(v ? &M.v : &M.k), "r"(h * (E5M2 ? 128 : 64)), "r"(row), "r"(at.hk), "r"(page), "r"(full(s)) : "memory");
             }
+            if (notes && at.tile == 0 && at.end < at.tiles) few_notes<DP, E5M2>(A, C)[c] = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
             __syncwarp();
             more = at.next(A, group, F::kTile);
             ask();
@@ -625,29 +633,13 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
 template <int DP, bool BF, bool E5M2>
 __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArgs A, int C) {
     using F = Few<DP, E5M2>;
-    __shared__ int64_t scan[32];
-    __shared__ int found_r;
-    __shared__ int64_t found_before;
-    const int group = A.Hq / A.Hkv, c = blockIdx.x;
-    // a block waits before it leaves too: what comes behind in the stream may wait for this kernel alone
-    auto leave = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
-    // the lists were written by what ran before the kernel in front, which has waited for it
-    const int64_t all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, F::kTile); },
-                                  [&](int64_t n) { return share_begin(n, c + 1, C) - 1; }, scan, &found_r, &found_before);
-    if (all == 0) return leave();
-    const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return leave();
-    const PagedReq q = paged_req(A, found_r);
-    const int places = few_tiles(q, group, F::kTile) + FEW_EXTRA;
-    int64_t within;
-    const int hk = div_few(last - 1 - found_before, places, within);
-    const int64_t from = found_before + (int64_t)hk * places, to = from + places;
-    if (first - from > FEW_EXTRA || last - from <= FEW_EXTRA || to <= last) return leave();        // its first tile is another block's, or it ends here
-    const int end = share_of(to - 1, all, C), rows = q.n * group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // with fewer places than blocks some have none
-    auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
-    auto none = [&](int b) { return all < C && share_begin(all, b, C) == share_begin(all, b + 1, C); };
+    const int group = A.Hq / A.Hkv, c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const SplitNote note = few_notes<DP, E5M2>(A, C)[c];
+    const int rows = note.rows, end = note.end, hk = note.hk;
+    auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
+    // with fewer places than blocks some have none
+    auto none = [&](int b) { return note.few && share_begin(note.few, b, C) == share_begin(note.few, b + 1, C); };
     for (int row = warp; row < rows; row += 8) {
         float top = -INFINITY, total = 0.0f;
         for (int b = c + lane; b <= end; b += 32)
@@ -683,7 +675,7 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArg
             }
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        uint16_t* const dst = (uint16_t*)A.out + (q.q0 + row / group) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
+        uint16_t* const dst = (uint16_t*)A.out + (note.q0 + row / group) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
 #pragma unroll
         for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
             const int d = 4 * lane + 128 * z;
@@ -775,15 +767,16 @@ template <int DP> int few_launch_types(const PagedAttnArgs& A, bool eight, cudaS
 }
 size_t few_part_bytes(int D) {
     const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-    return (size_t)sm_count() * 2 * (FEW_ROWS * dp + 2 * FEW_ROWS) * sizeof(float);
+    return (size_t)sm_count() * (2 * (FEW_ROWS * dp + 2 * FEW_ROWS) * sizeof(float) + sizeof(SplitNote));
 }
 
 }  // namespace
 }  // namespace lowbit
 
 extern "C" size_t lowbit_sdp_paged_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_query) {
-    (void)T; (void)R;
+    (void)R;
     if (D <= 0 || D > 256) return 0;
+    if (max_query > T) max_query = T;
     const size_t few = few_part_bytes(D);
     return Hkv > 0 && max_query * (Hq / Hkv) <= FEW_ROWS ? few : few + paged_prompt_part_bytes(D);
 }
@@ -815,6 +808,7 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
         return LB_ERR_WORKSPACE;
     }
     A.part = (float*)workspace;
+    if (max_query > T) max_query = T;
     cudaStream_t st = (cudaStream_t)stream;
     const bool eight = max_query * (Hq / Hkv) <= 8;                    // no unit has more rows, whoever else comes along
     if (const int rc = D <= 64 ? few_launch_types<64>(A, eight, st) : D <= 128 ? few_launch_types<128>(A, eight, st) : few_launch_types<256>(A, eight, st)) return rc;

@@ -233,6 +233,8 @@ __device__ __forceinline__ int64_t open_share(const PagedAttnArgs& A, int group,
     return all;
 }
 
+template <int DP, bool E5M2> __device__ __forceinline__ SplitNote* prompt_notes(const PagedAttnArgs& A, int C) { return reinterpret_cast<SplitNote*>(A.part + C * 2 * Prompt<DP, E5M2>::kPart); }
+
 // keys and values in the order of their tensor maps: [D][rows of a page][heads][pages], or [D][heads][tokens]
 struct PromptMaps { CUtensorMap k, v; };
 
@@ -484,6 +486,8 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         const int w0 = 32 * (warp - 4 * NT);                           // this warp's rows of a tile: lane = row
         constexpr int CH = E5M2 ? DP / 16 : DP / 8, RP = 32 / CH, PASSES = 32 / RP;
         const int live = A.D * (E5M2 ? 1 : 2) / 16, piece = lane % CH;
+        const bool notes = threadIdx.x == 4 * NT * 32;
+        if (notes) prompt_notes<DP, E5M2>(A, gridDim.x)[c].rows = 0;
         int j = at.a;
         int64_t ko = 0, vo = 0;
         uint32_t state = 0;                                            // of this lane's key: none, there, in no page
@@ -510,6 +514,8 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 ko = here ? (at.q.q0 + key) * A.k_ss + at.hk * A.k_sh : 0;
                 vo = here ? (at.q.q0 + key) * A.v_ss + at.hk * A.v_sh : 0;
             }
+            if (notes && j == 0 && at.b < at.tiles)
+                prompt_notes<DP, E5M2>(A, gridDim.x)[c] = split_note(min(at.tpu, at.q.n - at.u * at.tpu) * group, at.hk, at.q.q0 + at.u * at.tpu, at.b, at.tiles, all, c, C);
             if (++j >= at.b) {
                 more = at.next(A, group, P::kRows, above);
                 j = at.a;
@@ -701,30 +707,13 @@ done:
 
 // the units that began in block c and went on in others: their parts in the order of the keys.  A thread per row, a quarter of the columns a block
 template <int DP, bool BF, bool E5M2>
-__global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_kernel(const PagedAttnArgs A, int above, int blocks) {
+__global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_kernel(const PagedAttnArgs A, int blocks) {
     using P = Prompt<DP, E5M2>;
-    __shared__ int64_t scan[32];
-    __shared__ int found_r;
-    __shared__ int64_t found_before;
-    const int group = A.Hq / A.Hkv, c = blockIdx.x;
-    int C = blocks;
-    PromptAt at;
-    int place = 0;
-    // a block waits before it leaves too: what comes behind in the stream may wait for this kernel alone
-    auto leave = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
-    // the lists were written by what ran before the kernel in front, which has waited for it
-    const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, blocks); return c < C ? share_begin(n, c + 1, C) - 1 : -1; }, scan, &found_r,
-                                   &found_before, at, place);
-    if (all == 0 || c >= C) return leave();
-    const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
-    if (first == last) return leave();
-    const int tiles = Units(at.q, group, P::kRows, A.causal, above).tiles(at.u);
-    if (tiles <= PR_WHOLE) return leave();
-    const int64_t from = last - 1 - place, to = from + PR_EXTRA + tiles;
-    if (first - from > PR_EXTRA || last - from <= PR_EXTRA || to <= last) return leave();          // its first tile is another block's, or it ends here
-    const int end = share_of(to - 1, all, C), t = threadIdx.x >> 7, r = threadIdx.x & 127, row = threadIdx.x, token = at.u * at.tpu + row / group;
+    const int group = A.Hq / A.Hkv, c = blockIdx.x, t = threadIdx.x >> 7, r = threadIdx.x & 127, row = threadIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (row >= at.tpu * group || token >= at.q.n) return;
+    const SplitNote note = prompt_notes<DP, E5M2>(A, blocks)[c];
+    if (row >= note.rows) return;
+    const int end = note.end;
     auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * P::kPart; };
     auto stat = [&](int b) { return reinterpret_cast<const float2*>(slot(b) + (int64_t)P::NT * 128 * DP)[t * 128 + r]; };
     float top = -INFINITY, total = 0.0f;
@@ -734,7 +723,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kRows)) paged_prompt_merge_
         if (s.y != 0.0f) total = fmaf(s.x == -INFINITY ? s.y : ex2(s.x - top), s.y, total);
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t* const dst = (uint16_t*)A.out + (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh;
+    uint16_t* const dst = (uint16_t*)A.out + (note.q0 + row / group) * A.o_st + (int64_t)(note.hk * group + row % group) * A.o_sh;
     constexpr int PER = DP / 4;                                        // columns of this block
     const int d0 = blockIdx.y * PER;
     float x[PER] = {};
@@ -807,7 +796,7 @@ template <int DP, bool BF, bool E5M2, bool PAGED> int launch(const PagedAttnArgs
     }
     launch_behind(paged_prompt_kernel<DP, BF, E5M2, PAGED>, dim3((unsigned)C), P::kWarps * 32, P::kSmem, st, launch_overlaps(st), A, M, box, above);
     note_launch();
-    launch_behind(paged_prompt_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, 4), P::kRows, 0, st, true, A, above, C);
+    launch_behind(paged_prompt_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, 4), P::kRows, 0, st, true, A, C);
     note_launch();
     return check_launch();
 }
@@ -822,7 +811,7 @@ template <int DP> int launch_types(const PagedAttnArgs& A, int above, cudaStream
 int paged_prompt_max_group(int D) { return D <= 128 ? 256 : 128; }
 size_t paged_prompt_part_bytes(int D) {
     const int64_t floats = D <= 64 ? Prompt<64, false>::kPart : D <= 128 ? Prompt<128, false>::kPart : Prompt<256, false>::kPart;
-    return (size_t)sm_count() * 2 * floats * sizeof(float);
+    return (size_t)sm_count() * (2 * floats * sizeof(float) + sizeof(SplitNote));
 }
 int paged_prompt_launch(PagedAttnArgs A, int above, cudaStream_t st) {
     if (const int rc = make_waits(&A.waits, kWaitCycles)) return rc;
