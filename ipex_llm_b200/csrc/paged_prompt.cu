@@ -527,39 +527,58 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         uint32_t item = 0;
         ask();
         if (E5M2) {
-            uint4 w[PASSES];
-            auto fetch = [&](uint32_t item) {
-                if (!(item & 1)) where();
-                const uint8_t* const src = (const uint8_t*)((item & 1) ? A.v : A.k);
-                const uint32_t none = (item & 1) ? 0x7f7f7f7fu : 0u;
+            // Bytes come by cp.async into the slot that their halves will fill, AHEAD items early, and a warp spreads its 32 rows in place.  (Loads
+            // into registers an item ahead: the shuffles of addresses waited for them, 2700 clocks an item.)  A slot becomes free once the
+            // item behind its own is there, so two of the ring are never ahead.
+            constexpr int AHEAD = SLOTS - 2;
+            const uint32_t raw = w0 * 128 + lane * 16;                 // pieces of the warp's rows in a line, 4 KB a half
+            auto issue = [&]() {
+                if (!over && left > 0) {
+                    const int s = issued % SLOTS;
+                    const bool is_v = issued & 1;
+                    if (!is_v) where();
+                    else over = !more_keys;
+                    if (!mbar_wait_lim(kv_empty(s), ((issued / SLOTS) & 1) ^ 1, A.waits)) return false;
+                    const uint8_t* const src = (const uint8_t*)(is_v ? A.v : A.k);
 #pragma unroll
-                for (int i = 0; i < PASSES; i++) {
-                    const int l = i * RP + lane / CH;
-                    const int64_t o = __shfl_sync(0xffffffffu, (item & 1) ? vo : ko, l);
-                    const uint32_t s = __shfl_sync(0xffffffffu, state, l);
-                    const uint32_t z = s == 2 ? none : 0u;
-                    w[i] = make_uint4(z, z, z, z);
-                    if (s == 1 && piece < live) w[i] = *reinterpret_cast<const uint4*>(src + o + piece * 16);
+                    for (int i = 0; i < PASSES; i++) {
+                        const int l = i * RP + lane / CH;
+                        const int64_t o = __shfl_sync(0xffffffffu, is_v ? vo : ko, l);
+                        const uint32_t of = __shfl_sync(0xffffffffu, state, l), to = ring + s * TILE + (i >> 3) * HALF + (i & 7) * 512 + raw;
+                        if (of == 2 && is_v) sts4(to, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);       // no such page: not a number
+                        else if (piece < live) cp16(to, src + o + piece * 16, of == 1 ? 16u : 0u);
+                    }
+                    issued++;
+                    left--;
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                return true;
             };
-            if (any) fetch(0);
-            for (; !over && left > 0; item++, left--) {
+#pragma unroll 1
+            for (int i = 0; i < AHEAD; i++)
+                if (!issue()) goto done;
+            for (;; item++) {
+                if (!issue()) goto done;
+                if ((int)item == issued) break;
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+                __syncwarp();
                 const int s = item % SLOTS;
-                const uint32_t round = item / SLOTS;
-                if (!mbar_wait_lim(kv_empty(s), (round & 1) ^ 1, A.waits)) goto done;
-                const uint32_t dst = ring + s * TILE + (piece >> 2) * HALF;
+                const uint32_t slot = ring + s * TILE, dst = slot + (piece >> 2) * HALF;
                 const int c0 = 2 * (piece & 3);
+                uint4 x[PASSES];
 #pragma unroll
                 for (int i = 0; i < PASSES; i++) {
+                    x[i] = lds128(slot + (i >> 3) * HALF + (i & 7) * 512 + raw);
+                    if (piece >= live) x[i] = make_uint4(0, 0, 0, 0);  // columns behind D
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < PASSES; i++) {                     // e5m2 is the upper byte of fp16
                     const int rr = w0 + i * RP + lane / CH;
                     const uint32_t a = dst + rr * 128 + ((c0 ^ (rr & 7)) << 4), b = dst + rr * 128 + (((c0 + 1) ^ (rr & 7)) << 4);
-                    if (piece < live) {                                // e5m2 is the upper byte of fp16
-                        sts4(a, __byte_perm(w[i].x, 0u, 0x1404u), __byte_perm(w[i].x, 0u, 0x3424u), __byte_perm(w[i].y, 0u, 0x1404u), __byte_perm(w[i].y, 0u, 0x3424u));
-                        sts4(b, __byte_perm(w[i].z, 0u, 0x1404u), __byte_perm(w[i].z, 0u, 0x3424u), __byte_perm(w[i].w, 0u, 0x1404u), __byte_perm(w[i].w, 0u, 0x3424u));
-                    }
+                    sts4(a, __byte_perm(x[i].x, 0u, 0x1404u), __byte_perm(x[i].x, 0u, 0x3424u), __byte_perm(x[i].y, 0u, 0x1404u), __byte_perm(x[i].y, 0u, 0x3424u));
+                    sts4(b, __byte_perm(x[i].z, 0u, 0x1404u), __byte_perm(x[i].z, 0u, 0x3424u), __byte_perm(x[i].w, 0u, 0x1404u), __byte_perm(x[i].w, 0u, 0x3424u));
                 }
-                if ((item & 1) && !more_keys) over = true;
-                else fetch(item + 1);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kv_full(s));
