@@ -81,12 +81,15 @@ __device__ __forceinline__ int div_few(int64_t x, int64_t y, int64_t& rem) {    
     return q;
 }
 
+// blocks that share n places: none takes fewer than `least`
+__device__ __forceinline__ int sharers(int64_t n, int least, int C) { return n < (int64_t)least * C ? max((int)n / least, 1) : C; }
+
 // Of block c: the unit that began in it and goes on in others, to block `end`.  Rows are (token, head of the group).  The merge could find all
 // this out from the lists, but starts when the block's registers are free, and then every clock counts
-struct __align__(16) SplitNote { int rows, hk, end, few; int64_t q0, unused; };         // rows 0: there is none; few: places of all, where blocks have none
+struct __align__(16) SplitNote { int rows, hk, end, unused; int64_t q0, unused2; };     // rows 0: there is none
 // b of the unit's tiles were in block c
 __device__ __forceinline__ SplitNote split_note(int rows, int hk, int64_t q0, int b, int tiles, int64_t all, int c, int C) {
-    return {rows, hk, share_of(share_begin(all, c + 1, C) - b + tiles - 1, all, C), all < C ? (int)all : 0, q0, 0};
+    return {rows, hk, share_of(share_begin(all, c + 1, C) - b + tiles - 1, all, C), 0, q0, 0};
 }
 
 // sum over the block before this thread, and of all of it

@@ -12,6 +12,13 @@ namespace lowbit {
 namespace {
 
 // ------------------------------------------------------------------ few rows (decoding): at most 16 rows = new tokens x heads of a group
+// One pass over the keys: a warp takes 16 or 32 of a tile, S = Q . K^T and O += P . V by mma.sync m16n8k16 with the running maximum and sum of its
+// keys in registers; the warps' sums meet once a unit.  16 rows do not fill a tcgen05 tile (128), and what bounds the kernel is what it reads:
+// 100 requests of 200 to 8000 bf16 keys, 64 heads on 8, in 124 us (6.1 TB/s), 64 requests of 100 to 16000 e5m2 keys, 32 on 8, in 84.5 us (4.8 TB/s;
+// there the spreading of bytes to halves and the exponentials keep the warps as busy as the reads).
+// P enters the product as a 16-bit value and what its rounding left, two rows of one MMA or two MMAs, so that only the result is rounded.
+// At most 16 rows, the MMA's; beside the kernel of many rows (paged_prompt.cu), both with 16 rows: 64 requests of 1000 keys, 32 heads on 8, 62 / 91 us (e5m2
+// 60 / 132), 8 of 4000, 32 on 2, 21 / 33, 64 of 316, 8 on 8, 36 / 53.
 constexpr int FEW_ROWS = 16;
 
 template <int DP, bool E5M2> struct Few {
@@ -92,8 +99,12 @@ __device__ __forceinline__ int few_tiles(const PagedReq& q, int group, int tile)
 }
 
 // What a unit costs beside its keys (queries, the warps' sums, the result), in tiles: shares are taken of places, FEW_EXTRA of them in front of
-// a unit's tiles, so that blocks with many short requests are not the last
-constexpr int FEW_EXTRA = 1;
+// a unit's tiles, so that blocks with many short requests are not the last.  0 / 1 / 2 / 3: the 64 e5m2 requests above 124 / 100 / 84 / 88 us, the 100 of bf16
+// 148 / 129 / 124 / 126, one token over 4000 e5m2 keys 18.6 / 17.3 / 17.3 / 18.1
+constexpr int FEW_EXTRA = 2;
+// Places that a block takes at least.  1 / 2 / 3: one request of 8000 bf16 keys, 16 heads on one, 25 / 18 / 16 us, of e5m2 20 / 16 / 18, of 500 e5m2 keys, 32 heads,
+// 10.4 / 10.6 / 11.7
+constexpr int FEW_LEAST = 2;
 // where a block is in its share: request, kv head, tile of that head, and the end of the piece that it takes of them
 struct FewAt {
     PagedReq q; int r, hk, tile, end, tiles, left;
@@ -127,10 +138,10 @@ __device__ __forceinline__ int64_t few_places(const PagedReq& q, const PagedAttn
 }
 template <int DP, bool E5M2> __device__ __forceinline__ SplitNote* few_notes(const PagedAttnArgs& A, int C) { return reinterpret_cast<SplitNote*>(A.part + (int64_t)C * 2 * Few<DP, E5M2>::kPart); }
 // the whole block: where its share begins; false: it has none
-__device__ __forceinline__ bool few_open(const PagedAttnArgs& A, int group, int tile, int c, int C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at, int64_t& all) {
-    all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, tile); }, [&](int64_t n) { return share_begin(n, c, C); }, scan, found_r,
-                                  found_before);
-    if (all == 0) return false;
+__device__ __forceinline__ bool few_open(const PagedAttnArgs& A, int group, int tile, int c, int& C, int64_t* scan, int* found_r, int64_t* found_before, FewAt& at, int64_t& all) {
+    all = find_tile(A.R, [&](int r) { return few_places(paged_req(A, r), A, group, tile); },
+                    [&](int64_t n) { C = sharers(n, FEW_LEAST, C); return c < C ? share_begin(n, c, C) : -1; }, scan, found_r, found_before);
+    if (all == 0 || c >= C) return false;
     const int64_t first = share_begin(all, c, C), last = share_begin(all, c + 1, C);
     if (first == last) return false;
     at.r = *found_r;
@@ -428,7 +439,8 @@ template <int DP, bool BF, bool E5M2, bool TMA, bool EIGHT> struct FewWarp {
     }
 };
 
-// every warp copies its own keys: page sizes that TMA has no box for
+// Every warp copies its own keys: page sizes that TMA has no box for (no multiple of 8 rows, or a stride of 0).  Where both serve: one token over 4000 e5m2
+// keys 20.5 us for 17.3, the 64 requests 130 for 100, the 100 requests 173 for 129
 template <int DP, bool BF, bool E5M2>
 __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
     using F = Few<DP, E5M2>;
@@ -442,10 +454,12 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     const int group = A.Hq / A.Hkv;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int C = gridDim.x, c = blockIdx.x;
+    const int c = blockIdx.x;
+    int C = gridDim.x;
     FewAt at;                                                          // of the products
     int64_t all;
-    if (threadIdx.x == 0) few_notes<DP, E5M2>(A, C)[c].rows = 0;
+    SplitNote* const note = few_notes<DP, E5M2>(A, gridDim.x) + c;
+    if (threadIdx.x == 0) note->rows = 0;
     if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at, all)) return;
     FewAt in = at;                                                     // of the copies
     bool to_copy = true;
@@ -504,7 +518,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
         if (!begun) {
             begun = true;
             from_start = at.tile == 0;
-            if (from_start && at.end < at.tiles && threadIdx.x == 0) few_notes<DP, E5M2>(A, C)[c] = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
+            if (from_start && at.end < at.tiles && threadIdx.x == 0) *note = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
             w.begin(A, at.q, at.hk, group, g, t);
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
@@ -550,11 +564,13 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
         for (int s = 0; s < ST; s++) { mbar_init(full(s), 4); mbar_init(empty(s), NW); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const int C = gridDim.x, c = blockIdx.x;
+    const int c = blockIdx.x;
+    int C = gridDim.x;
     FewAt at;
     int64_t all;
     const bool notes = threadIdx.x == NW * 32;
-    if (notes) few_notes<DP, E5M2>(A, C)[c].rows = 0;
+    SplitNote* const note = few_notes<DP, E5M2>(A, gridDim.x) + c;
+    if (notes) note->rows = 0;
     if (!few_open(A, group, F::kTile, c, C, scan, &found_r, &found_before, at, all)) return;
     if (warp >= NW) {
         // ================= the copies: this warp's boxes of a tile =================
@@ -589,7 +605,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
                         asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                                      ::"r"(dst + v * TILE + h * (F::kTile * 128)), "l"(v ? &M.v : &M.k), "r"(h * (E5M2 ? 128 : 64)), "r"(row), "r"(at.hk), "r"(page), "r"(full(s)) : "memory");
             }
-            if (notes && at.tile == 0 && at.end < at.tiles) few_notes<DP, E5M2>(A, C)[c] = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
+            if (notes && at.tile == 0 && at.end < at.tiles) *note = split_note(at.q.n * group, at.hk, at.q.q0, at.end, at.tiles, all, c, C);
             __syncwarp();
             more = at.next(A, group, F::kTile);
             ask();
@@ -629,58 +645,52 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
     __syncthreads();
 }
 
-// the units that began in block c and went on in others: their parts in the order of the keys
+// the units that began in block c and went on in others: their parts in the order of the keys, a row a warp
 template <int DP, bool BF, bool E5M2>
-__global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttnArgs A, int C) {
+__global__ void __launch_bounds__(128) paged_few_merge_kernel(const PagedAttnArgs A) {
     using F = Few<DP, E5M2>;
-    const int group = A.Hq / A.Hkv, c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = A.Hq / A.Hkv, c = blockIdx.x, row = 4 * blockIdx.y + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const SplitNote note = few_notes<DP, E5M2>(A, C)[c];
-    const int rows = note.rows, end = note.end, hk = note.hk;
+    const SplitNote note = few_notes<DP, E5M2>(A, gridDim.x)[c];
+    if (row >= note.rows) return;
+    const int end = note.end, hk = note.hk;
     auto slot = [&](int b) { return A.part + ((int64_t)b * 2 + (b == c ? 1 : 0)) * F::kPart; };
-    // with fewer places than blocks some have none
-    auto none = [&](int b) { return note.few && share_begin(note.few, b, C) == share_begin(note.few, b + 1, C); };
-    for (int row = warp; row < rows; row += 8) {
-        float top = -INFINITY, total = 0.0f;
-        for (int b = c + lane; b <= end; b += 32)
-            if (!none(b)) top = fmaxf(top, slot(b)[FEW_ROWS * DP + 2 * row]);
+    float top = -INFINITY, total = 0.0f;
+    for (int b = c + lane; b <= end; b += 32)
+        top = fmaxf(top, slot(b)[FEW_ROWS * DP + 2 * row]);
 #pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        float4 x[DP > 128 ? 2 : 1];
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float4 x[DP > 128 ? 2 : 1];
 #pragma unroll
-        for (int z = 0; z < (DP > 128 ? 2 : 1); z++) x[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int b0 = c; b0 <= end; b0 += 32) {
-            // a lane finds a part's weight, and all add up its values
-            float mine = 0.0f, part_sum = 0.0f;
-            const bool here = b0 + lane <= end && !none(b0 + lane);
-            if (here) {
-                const float2 st = *reinterpret_cast<const float2*>(slot(b0 + lane) + FEW_ROWS * DP + 2 * row);
-                mine = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
-                part_sum = st.y;
-            }
-            const uint32_t parts = __ballot_sync(0xffffffffu, here);
-#pragma unroll 4
-            for (int k = 0; k < 32 && b0 + k <= end; k++) {
-                const float w = __shfl_sync(0xffffffffu, mine, k);
-                total = fmaf(w, __shfl_sync(0xffffffffu, part_sum, k), total);
-                if (!(parts >> k & 1)) continue;
-                const float* const p = slot(b0 + k);
+    for (int z = 0; z < (DP > 128 ? 2 : 1); z++) x[z] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int b0 = c; b0 <= end; b0 += 32) {
+        // a lane finds a part's weight, and all add up its values
+        float mine = 0.0f, part_sum = 0.0f;
+        if (b0 + lane <= end) {
+            const float2 st = *reinterpret_cast<const float2*>(slot(b0 + lane) + FEW_ROWS * DP + 2 * row);
+            mine = st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : st.y) : ex2(st.x - top);
+            part_sum = st.y;
+        }
+#pragma unroll 8
+        for (int k = 0; k < 32 && b0 + k <= end; k++) {
+            const float w = __shfl_sync(0xffffffffu, mine, k);
+            total = fmaf(w, __shfl_sync(0xffffffffu, part_sum, k), total);
+            const float* const p = slot(b0 + k);
 #pragma unroll
-                for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
-                    const int d = 4 * lane + 128 * z;
-                    if (d >= DP) continue;
-                    const float4 y = *reinterpret_cast<const float4*>(p + row * DP + d);
-                    x[z].x = fmaf(w, y.x, x[z].x); x[z].y = fmaf(w, y.y, x[z].y); x[z].z = fmaf(w, y.z, x[z].z); x[z].w = fmaf(w, y.w, x[z].w);
-                }
+            for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
+                const int d = 4 * lane + 128 * z;
+                if (d >= DP) continue;
+                const float4 y = *reinterpret_cast<const float4*>(p + row * DP + d);
+                x[z].x = fmaf(w, y.x, x[z].x); x[z].y = fmaf(w, y.y, x[z].y); x[z].z = fmaf(w, y.z, x[z].z); x[z].w = fmaf(w, y.w, x[z].w);
             }
         }
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        uint16_t* const dst = (uint16_t*)A.out + (note.q0 + row / group) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* const dst = (uint16_t*)A.out + (note.q0 + row / group) * A.o_st + (int64_t)(hk * group + row % group) * A.o_sh;
 #pragma unroll
-        for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
-            const int d = 4 * lane + 128 * z;
-            if (d < A.D) store4<BF>(dst + d, x[z], inv);
-        }
+    for (int z = 0; z < (DP > 128 ? 2 : 1); z++) {
+        const int d = 4 * lane + 128 * z;
+        if (d < A.D) store4<BF>(dst + d, x[z], inv);
     }
 }
 
@@ -757,7 +767,7 @@ template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, bool eight
                       launch_overlaps(st), A, M, box);
     } else launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
     note_launch();
-    launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C), 256, 0, st, true, A, C);
+    launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, FEW_ROWS / 4), 128, 0, st, true, A);
     note_launch();
     return check_launch();
 }
@@ -810,7 +820,9 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
     A.part = (float*)workspace;
     if (max_query > T) max_query = T;
     cudaStream_t st = (cudaStream_t)stream;
-    const bool eight = max_query * (Hq / Hkv) <= 8;                    // no unit has more rows, whoever else comes along
+    // no unit has more than 8 rows: the other 8 of the MMA carry what rounding P left.  Else / so: one token over 4000 e5m2 keys 19.3 / 17.3 us, the 64
+    // requests 114 / 100, the 100 requests 138 / 129
+    const bool eight = max_query * (Hq / Hkv) <= 8;
     if (const int rc = D <= 64 ? few_launch_types<64>(A, eight, st) : D <= 128 ? few_launch_types<128>(A, eight, st) : few_launch_types<256>(A, eight, st)) return rc;
     if (max_query * (Hq / Hkv) <= FEW_ROWS) return LB_OK;
     A.part = (float*)((uint8_t*)workspace + few_part_bytes(D));

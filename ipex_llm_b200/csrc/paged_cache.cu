@@ -77,8 +77,8 @@ __device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
 // and new pages are then dealt to the cluster's threads, who find their request in the sums.  What a token's slot needs of pages that
 // the step itself hands out comes from the stack, so nobody waits for the table.  The count of free pages is read by all before the first
 // block writes it (it may be written in place): that is what the cluster is for.
-// What bounds it: launch and two passes of dependent loads.  32 requests with a token each: 2.9 us; 500 requests, 19000 tokens: 5.4 us
-// (one block 54 us).
+// What bounds it: the launch and two passes of dependent loads.  32 requests with a token each 3.1 us; 500 requests, 19000 tokens 8.0 us, most of it
+// the search of every token for its request.
 __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const StepArgs A) {
     __shared__ Three sums[32];
     __shared__ int64_t first[STEP_THREADS];
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs A) {
 }
 
 // The same for rows on 16 bytes: 16 elements a thread, two runs of 8 that are each other's partners (rotated heads), or of one piece.  A head's
-// tables are read once a head, from L1.  What bounds it: DRAM, 8000 tokens of 32 / 8 heads (217 MB) in 45 us, 4.8 TB/s (a pair a
-// thread: 209 us).
+// tables are read once a head, from L1.  What bounds it: DRAM, 8000 tokens of 32 / 8 heads (217 MB) in 35.6 us, 6.1 TB/s.  The kernel of a pair a
+// thread, half precision into e5m2: 32 tokens 2.8 us for 2.2, 256 tokens 7.7 for 2.7, 8000 tokens 202 for 35.
 template <typename T, bool E5M2, typename C>
 __global__ void __launch_bounds__(256) paged_append_vec_kernel(const AppendArgs A) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -304,13 +304,15 @@ extern "C" int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_hel
     }
     const StepArgs A = {d_new, d_held, R, d_table, table_stride, width, d_free_pages, n_pages, d_free_count, d_free_left, page_size, n_tokens,
                         d_cu_seqlens, d_seq_lens, d_positions, d_slots, d_missing};
-    // a block for a decode step, a cluster of eight (the most that any device takes) where it has thousands of tokens to write.  32 / 500
-    // requests with a token each: 2.9 / 3.9 us with one block, 3.4 / 4.3 with eight; 19000 tokens 11.9 and 5.4 us
-    const bool many = n_tokens > 4 * STEP_THREADS;
+    // A block for a decode step, a cluster of eight (the most that any device takes) for more tokens; blocks of 1024 threads where requests or
+    // tokens are many.  One block / eight, of 256 threads: 32 requests with a token each 3.1 / 3.5 us, 4 with 800 tokens in all 4.5 / 3.6, 16
+    // with 5000 14 / 4.8; of 1024: 500 requests with a token each 4.5 / 4.7, 19000 tokens 27 / 8.4.  256 / 1024 threads, eight blocks: 5000 tokens 4.8 /
+    // 5.1, 8000 tokens 6.1 / 5.4; one block: 256 requests 3.3 / 4.3, 500 requests 4.9 / 4.5.
+    const bool many = n_tokens > 512, wide = R > 256 || n_tokens > 6000;
     cudaStream_t st = (cudaStream_t)stream;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(many ? 8 : 1);
-    cfg.blockDim = dim3(many || R > 256 || n_tokens > 1024 ? STEP_THREADS : 256);
+    cfg.blockDim = dim3(wide ? STEP_THREADS : 256);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -358,7 +360,8 @@ extern "C" int lowbit_paged_rope_append_cuda(void* d_qkv, int dtype, int64_t tok
         !(((uintptr_t)d_k_cache | (uintptr_t)d_v_cache) & (cache_dtype == CACHE_E5M2 ? 7 : 15)) &&
         !((k_strides[0] | k_strides[1] | k_strides[2] | v_strides[0] | v_strides[1] | v_strides[2]) & 7) &&
         (rotary_dim == 0 || (!(((uintptr_t)d_cos | (uintptr_t)d_sin) & 15) && !(cs_row_stride & table)))) {
-        const int64_t want = (chunks + 255) / 256, most = (int64_t)sm_count() * 8;
+        // five blocks an SM, as many as are resident; eight: 41 us where this takes 35.6 (8000 tokens, 32 / 8 heads)
+        const int64_t want = (chunks + 255) / 256, most = (int64_t)sm_count() * 5;
         const unsigned grid = (unsigned)(want < most ? want : most);
         if (dtype == DT_F16) cache_dtype == CACHE_E5M2 ? append_vec<__half, true>(A, grid, st) : append_vec<__half, false>(A, grid, st);
         else cache_dtype == CACHE_E5M2 ? append_vec<__nv_bfloat16, true>(A, grid, st) : append_vec<__nv_bfloat16, false>(A, grid, st);

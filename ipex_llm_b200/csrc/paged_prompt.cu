@@ -3,11 +3,19 @@
 // A unit is NT tiles of 128 rows of one kv head; a request's rows there are (new token, head of the group), tokens first, so that all heads
 // that share a kv head share every key that is read.  Keys come in tiles of 128:
 //   S_t = Q_t . K^T   tcgen05.mma M = 128, N = 128, both operands in shared memory, S in tensor memory (lane = row);
-//   softmax           four warps a tile, a thread per row: the row's 128 scores in registers, P back into tensor memory over S;
+//   softmax           four warps a tile, a thread per row: the maximum in one reading of the row's 128 scores, exp2 in another, 64 in registers at
+//                     a time, P back into tensor memory over S;
 //   O_t += P_t . V    A operand = P in tensor memory, B operand = V as it lies in the cache (rows = keys: the MN-major descriptor).
-// Warps 0 .. 4 NT - 1: softmax; the next four copy keys and values into a ring of 128-byte swizzled tiles (cp.async, or e5m2 bytes expanded
-// to fp16 on the way), rows that a request does not hold as zeros; the next one issues the MMAs and owns the tensor memory.
+// Warps 0 .. 4 NT - 1: softmax; the next four copy keys and values into a ring of 128-byte swizzled tiles (TMA, a box per run of rows in a page;
+// rows behind the last key and pages without boxes by cp.async; e5m2 bytes spread to fp16 in their slot); the next one issues the MMAs and owns the
+// tensor memory.
 // Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
+// P is rounded once, to the type of the values, so that P . V is one product; the row's sum is of the unrounded ones.  In an output that adds up
+// to sqrt(2) of the error that rounding the output alone leaves.
+// What bounds it: the softmax, 2050 of 4050 clocks a step of 256 rows and 128 keys (two loads of S, 128 exponentials a thread, P's store) with the
+// products between two steps of a tile (QK 660, PV 460) and the waits of the roles for one another.  8 prompts of 200 to 4000 tokens, 32 heads on 8,
+// bf16: 223 us, 677 TFLOP/s; one of 8000, 32 heads: 546 us, 960 TFLOP/s; 512 tokens behind 16000 keys, 32 on 8: 155 us, 876 TFLOP/s.
+// With TMA / without: 223 / 234, 546 / 630, 155 / 246 us.
 #include <string.h>
 #include "paged.h"
 #include "tc_common.cuh"
@@ -117,10 +125,11 @@ __device__ __forceinline__ int64_t floor_sum128(uint32_t n, uint32_t a, uint32_t
     return s;
 }
 // What a unit costs beside its key tiles (queries, result, a pipeline that drains), in tiles: shares are taken of places, PR_EXTRA of them in
-// front of a unit's tiles, so that blocks with many short prompts are not the last
+// front of a unit's tiles, so that blocks with many short prompts are not the last.  0 / 1 / 2 / 3: the 8 prompts 351 / 294 / 274 / 274 us (before the softmax
+// had its loops; then 268 with 1 and 230 with 2)
 constexpr int PR_EXTRA = 2;
 // A unit of up to so many key tiles is never split: it is the block's in whose share it begins.  A part costs a store and a load of its 32-bit
-// sums (128 KB a unit) and its merge, more than such a unit is worth
+// sums (128 KB a unit) and its merge, more than such a unit is worth: 7 prompts of 17 to 300 tokens 21.5 us with 0, 19.4 with 2 and with 4
 constexpr int PR_WHOLE = 4;
 struct Units {
     int n, units, tpu, causal, off, len;                      // new tokens, units, tokens of a unit; keys before the first new token
@@ -187,8 +196,8 @@ struct PromptAt {
         return keys <= 0 ? 0 : (keys - 1) / PR_KEYS + 1;
     }
 };
-// blocks that share n places: none takes fewer than three, which cost about what a part of a unit adds
-__device__ __forceinline__ int sharers(int64_t n, int C) { return n < 3 * (int64_t)C ? max((int)n / 3, 1) : C; }
+// places that a block takes at least.  1 / 3 / 6: a prompt of 2000 tokens, 4 heads on one 31.0 / 28.8 / - us, seven of 17 to 300 tokens 17.6 / 17.5 / 24
+constexpr int PR_LEAST = 3;
 
 // the whole block: where place `pick` of all lies (`place` of its unit); `all` = places of all units
 template <typename Pick>
@@ -282,7 +291,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
     PromptAt at;
     int C = gridDim.x, issued = 0, place = 0;
     const int c = blockIdx.x;
-    const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, gridDim.x); return c < C ? share_begin(n, c, C) : -1; }, scan, &found_r,
+    const int64_t all = open_share(A, group, P::kRows, above, [&](int64_t n) { C = sharers(n, PR_LEAST, gridDim.x); return c < C ? share_begin(n, c, C) : -1; }, scan, &found_r,
                                    &found_before, at, place);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
