@@ -192,7 +192,7 @@ PyObject* sdp_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *table = plain(a[3]), *lens = plain(a[4]), *cu = plain(a[5]);
     float scale;
     int64_t most;
-    if (!q || q->dim() != 3 || !caches_ok(k, v, *q, q->size(2)) || !aligned(*k) || !aligned(*v) || !queries_ok(q, k->size(2), a[6], a[7], &scale, &most) || !table_ok(table, *q))
+    if (!q || q->dim() != 3 || !caches_ok(k, v, *q, q->size(2)) || wants_grad(*k) || wants_grad(*v) || !aligned(*k) || !aligned(*v) || !queries_ok(q, k->size(2), a[6], a[7], &scale, &most) || !table_ok(table, *q))
         Py_RETURN_NONE;
     const int64_t R = table->size(0), T = q->size(0), H = q->size(1), D = q->size(2);
     if (!ints(lens, R, at::kInt, *q) || !ints(cu, R + 1, at::kInt, *q) || table->size(1) * k->size(1) >= (int64_t)1 << 31) Py_RETURN_NONE;

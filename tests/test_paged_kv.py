@@ -562,6 +562,15 @@ def test_on_other_streams_at_once(paged, cuda_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("new,held", [([1, 1], [20, 7000]), ([2, 300], [700, 5000])])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 1, 64), (64, 1, 128), (256, 1, 128), (128, 1, 256)])
+def test_many_heads_on_one(paged, cuda_device, dtype, eight, new, held, heads, kv_heads, dim):
+    """a kv head's keys in the parts of many blocks, for 16 rows and more, up to the most heads that there may be; a hint beyond all rows is no hint"""
+    check_paged(paged, cuda_device, new, held, heads, kv_heads, dim, dtype, eight, 16, hint=1 << 62)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
 @pytest.mark.parametrize("new,rows", [([3, 9], 5), ([40, 300, 7], 200), ([1, 1, 1], 2)])
 def test_tokens_behind_the_last_row(paged, cuda_device, dtype, eight, new, rows):
     """a list that names more rows than there are: those that are there see the keys that they would see with the others"""
@@ -706,4 +715,12 @@ def test_refusals(paged, cuda_device):
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {n} was taken")
+    wants = c.clone().requires_grad_()
+    for call in (lambda: paged.sdp_paged(q, wants, c, table, lens, cu), lambda: paged.sdp_paged(q, c, wants, table, lens, cu)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
+    wide = h(6, 514, 64)                                                                          # more heads on one than a unit has rows
+    for call in (lambda: paged.sdp_paged(wide, h(3, 16, 2, 64), h(3, 16, 2, 64), table, lens, cu), lambda: paged.sdp_packed(wide, q[:, :2], q[:, :2], cu)):
+        with pytest.raises(RuntimeError, match="bad argument"):
+            call()
     assert paged.sdp_paged(q[:0], c, c, table, lens, cu).shape == (0, 4, 64) and paged.sdp_packed(q[:0], q[:0], q[:0], cu).shape == (0, 4, 64)
