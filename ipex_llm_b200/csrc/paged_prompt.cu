@@ -126,7 +126,7 @@ __device__ __forceinline__ int64_t floor_sum128(uint32_t n, uint32_t a, uint32_t
 }
 // What a unit costs beside its key tiles (queries, result, a pipeline that drains), in tiles: shares are taken of places, PR_EXTRA of them in
 // front of a unit's tiles, so that blocks with many short prompts are not the last.  0 / 1 / 2 / 3: the 8 prompts 351 / 294 / 274 / 274 us (before the softmax
-// had its loops; then 268 with 1 and 230 with 2)
+// had its loops; since then 268 with 1, and 2 / 3 / 4: 226 / 218 / 222), 40 requests with chunks to 300 and tokens over e5m2 pages 103 / 107 / 109
 constexpr int PR_EXTRA = 2;
 // A unit of up to so many key tiles is never split: it is the block's in whose share it begins.  A part costs a store and a load of its 32-bit
 // sums (128 KB a unit) and its merge, more than such a unit is worth: 7 prompts of 17 to 300 tokens 21.5 us with 0, 19.4 with 2 and with 4
