@@ -57,20 +57,6 @@ template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a
     else asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two values rounded to 16 bits, and what that left
-template <bool BF> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    if (BF) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        const __nv_bfloat162 l = __floats2bfloat162_rn(x - __low2float(h), y - __high2float(h));
-        hi = *reinterpret_cast<const uint32_t*>(&h);
-        lo = *reinterpret_cast<const uint32_t*>(&l);
-    } else {
-        const __half2 h = __floats2half2_rn(x, y);
-        const __half2 l = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
-        hi = *reinterpret_cast<const uint32_t*>(&h);
-        lo = *reinterpret_cast<const uint32_t*>(&l);
-    }
-}
 template <bool BF> __device__ __forceinline__ float unpack16(uint32_t w, int hi) {
     if (BF) return __uint_as_float(hi ? w & 0xffff0000u : w << 16);
     const __half2 h = *reinterpret_cast<const __half2*>(&w);

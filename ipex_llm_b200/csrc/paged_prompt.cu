@@ -10,12 +10,13 @@
 // rows behind the last key and pages without boxes by cp.async; e5m2 bytes spread to fp16 in their slot); the next one issues the MMAs and owns the
 // tensor memory.
 // Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
-// P is rounded once, to the type of the values, so that P . V is one product; the row's sum is of the unrounded ones.  In an output that adds up
-// to sqrt(2) of the error that rounding the output alone leaves.
-// What bounds it: the softmax, 2050 of 4050 clocks a step of 256 rows and 128 keys (two loads of S, 128 exponentials a thread, P's store) with the
-// products between two steps of a tile (QK 660, PV 460) and the waits of the roles for one another.  8 prompts of 200 to 4000 tokens, 32 heads on 8,
-// bf16: 223 us, 677 TFLOP/s; one of 8000, 32 heads: 546 us, 960 TFLOP/s; 512 tokens behind 16000 keys, 32 on 8: 155 us, 876 TFLOP/s.
-// With TMA / without: 223 / 234, 546 / 630, 155 / 246 us.
+// P enters P . V as two 16-bit values, the second with what the rounding of the first left, and both multiply V: only the result is rounded.  With one
+// value (182 / 155 us a chunk, 687 / 545 the long prompt below) an output added up to sqrt(2) of the error that rounding the output alone leaves.
+// What bounds it: the softmax (two loads of S, 128 exponentials a thread, both parts' stores) with the products between two steps of a tile (3072 clocks of
+// MMAs a step of 256 rows and 128 keys, of which one tile's run beside the other's softmax) and the waits of the roles for one another.  8 prompts of 200
+// to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one of 8000, 32 heads, fp16: 687 us, 763 TFLOP/s; 512 tokens behind
+// 16000 keys, 32 on 8, bf16: 182 us, 748 TFLOP/s.
+// Before P had two parts, with TMA / without: 223 / 234, 546 / 630, 155 / 246 us.
 #include <string.h>
 #include "paged.h"
 #include "tc_common.cuh"
@@ -420,18 +421,22 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                     // fp16: 2^8 above the reference's place, so that values from 2^-24 to 2^14 of it are normal numbers or close
                     const float shift = (MBF ? 0.0f : 8.0f) - (m_ref == -INFINITY ? 0.0f : m_ref);
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
-                    // P of a half goes where its scores were
+                    // P of 32 keys goes where their scores were: the high parts to the first 16 columns, what their rounding left to the others
                     auto exponentials = [&](int h) {
-                        uint32_t p[32];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float p0 = ex2(fmaf(x[2 * i], mul, shift)), p1 = ex2(fmaf(x[2 * i + 1], mul, shift));
-                            const float p2 = ex2(fmaf(x[2 * i + 2], mul, shift)), p3 = ex2(fmaf(x[2 * i + 3], mul, shift));
-                            a0 += p0; a1 += p1; a2 += p2; a3 += p3;
-                            p[i] = pack2<MBF>(p0, p1);
-                            p[i + 1] = pack2<MBF>(p2, p3);
+                        for (int c = 0; c < 2; c++) {
+                            uint32_t hi[16], lo[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float* const s = x + 32 * c + 2 * i;
+                                const float p0 = ex2(fmaf(s[0], mul, shift)), p1 = ex2(fmaf(s[1], mul, shift)), p2 = ex2(fmaf(s[2], mul, shift)), p3 = ex2(fmaf(s[3], mul, shift));
+                                a0 += p0; a1 += p1; a2 += p2; a3 += p3;
+                                split2<MBF>(p0, p1, hi[i], lo[i]);
+                                split2<MBF>(p2, p3, hi[i + 1], lo[i + 1]);
+                            }
+                            tmem_st16x(st + 64 * h + 32 * c, hi);
+                            tmem_st16x(st + 64 * h + 32 * c + 16, lo);
                         }
-                        tmem_st32x(st + 64 * h, p);
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
@@ -668,7 +673,9 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 const uint64_t vd = (make_desc(slot(i)) & ~((uint64_t)0x3fff << 16)) | ((uint64_t)(HALF >> 4) << 16);
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 64 + k * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 0 && k == 0 ? 0u : 1u, leader);
+#pragma unroll
+                    for (int l = 0; l < 2; l++)                        // P's high and low parts
+                        umma_ts_w(tmem + NT * 128 + t * DP, tmem + t * 128 + h * 64 + (k >> 1) * 32 + l * 16 + (k & 1) * 8, vd + (uint64_t)(((4 * h + k) * 2048) >> 4), id_o, fresh && h == 0 && k == 0 && l == 0 ? 0u : 1u, leader);
             };
             for (;;) {
                 // lane 0's, so that the compiler knows them to be the warp's: operands that it takes for a lane's own cost a move per MMA

@@ -581,6 +581,82 @@ def test_tokens_behind_the_last_row(paged, cuda_device, dtype, eight, new, rows)
     assert torch.equal(paged.sdp_paged(q[:rows], *caches, table, lens, cu), want) and not bool(torch.isnan(want).any())
 
 
+# ------------------------------------------------------------------ what is rounded, and what is not
+# P enters its product as two values of type t, the second with what the rounding of the first left: h(t)^2 of itself is lost, and nothing else but
+# the result is rounded.  In fp16 neither part has bits below 2^-24, half of which a stored value may be off by; a row's largest key is stored as
+# at least 2^LIFT, so that moves the output by up to 2^(-25 - LIFT) sum |v|.
+# Queries and keys are small whole numbers here: the scores' sums are exact in 32 bits, and what is left is the exponent e = score log2(e), whose
+# factor is off by 2^-23 of itself and which is rounded (with up to 16 beside it) once in the exponential and once whenever the row's reference moves:
+# by more than 2^4 each time, and where the parts of warps and blocks meet (2).
+LIFT = 8
+
+
+def bound_once(want, absolute, steepest, v_sum, dtype, p_dtype, keys):
+    e = 1.4427 * steepest
+    score = 2.0 ** -22 + 0.7 * (e * 2.0 ** -23 + (2 * e + 16) * 2.0 ** -24 * (3 + 2 * e / 4))
+    lost = HALF[p_dtype] ** 2 * absolute + (2.0 ** (-25 - LIFT) * v_sum if p_dtype == torch.float16 else 0)
+    # an output of fp16 has no bits below 2^-24 either
+    return HALF[dtype] * want.abs() + 2.0 ** -25 + (1 + HALF[dtype]) * (lost + (2 * score + (keys / 8 + 8) * 2.0 ** -23) * absolute)
+
+
+def check_once(got, q, k, v, cu, lens, scale, dtype, p_dtype, causal=True):
+    heads = q.shape[1]
+    want, absolute, _ = statement(q, k, v, cu, lens, scale, causal)
+    steepest = max(float(torch.einsum("ihd,jhd->hij", q[a:b].double(), x.double().repeat_interleave(heads // x.shape[1], 1)).abs().max()) * scale
+                   for x, a, b in zip(k, cu, cu[1:]))
+    v_sum = torch.cat([x.double().abs().sum(0).repeat_interleave(heads // x.shape[1], 0)[None].expand(b - a, -1, -1) for x, a, b in zip(v, cu, cu[1:])])
+    limit = bound_once(want, absolute, steepest, v_sum, dtype, p_dtype, max(lens))
+    return float(((got.double() - want).abs() / limit).max())
+
+
+def whole(x):
+    return x.float().round().clamp(-4, 4).to(x.dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 1, 64), (6, 2, 256)])
+@pytest.mark.parametrize("new,held,page", [([130], [0], 16), ([70, 200], [30, 20], 24), ([40], [100], 4), ([150], [800], 32)])
+def test_chunks_round_the_result_alone(paged, cuda_device, dtype, eight, heads, kv_heads, dim, new, held, page):
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, new, held, heads, kv_heads, dim, dtype, eight, page)
+    q, keys = whole(q), caches[0].view(torch.float8_e5m2) if eight else caches[0]
+    caches[0] = whole(keys).view(torch.uint8) if eight else whole(keys)
+    k, v = ([x.half() if eight else x for x in part] for part in (map(whole, rows[0]), rows[1]))
+    scale = 0.25 * dim ** -0.5
+    got = paged.sdp_paged(q, *caches, table, lens, cu, scale)
+    assert check_once(got, q, k, v, cu_list, len_list, scale, dtype, torch.float16 if eight else dtype) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,dim,lens", [(8, 2, 128, [500, 33, 157]), (4, 4, 64, [200]), (3, 1, 256, [90, 140])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_round_the_result_alone(paged, cuda_device, dtype, heads, kv_heads, dim, lens, causal):
+    g = torch.Generator(device=cuda_device).manual_seed(dim)
+    q, k, v = (1.5 * torch.randn(sum(lens), heads + 2 * kv_heads, dim, generator=g, device=cuda_device)).to(dtype).split([heads, kv_heads, kv_heads], 1)
+    q, k, cu, scale = whole(q), whole(k), [0], 0.25 * dim ** -0.5
+    for n in lens:
+        cu.append(cu[-1] + n)
+    got = paged.sdp_packed(q, k, v, torch.tensor(cu, dtype=torch.int32, device=cuda_device), scale, is_causal=causal)
+    k, v = ([t[a:b] for a, b in zip(cu, cu[1:])] for t in (k, v))
+    assert check_once(got, q, k, v, cu, lens, scale, dtype, dtype, causal) <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("keys", [30, 150])
+def test_the_bound_tells_probabilities_of_one_value(dtype, keys):
+    """an oracle that rounds its probabilities once is outside it, one that keeps what that left is inside"""
+    g = torch.Generator().manual_seed(keys)
+    q, k, v = ((1.5 * torch.randn(n, 2, 128, generator=g)).to(dtype) for n in (40, keys, keys))
+    q, k, scale = whole(q), whole(k), 0.25 * 128 ** -0.5
+    s = torch.einsum("ihd,jhd->hij", q.float(), k.float()) * scale
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    high = p.to(dtype).float()
+    for parts, inside in ((high, False), (high + (p - high).to(dtype).float(), True)):
+        o = (torch.einsum("hij,jhd->ihd", parts, v.float()) / p.sum(-1).t()[..., None]).to(dtype)
+        assert (check_once(o, q, [k], [v], [0, 40], [keys], scale, dtype, dtype, False) <= 1) == inside
+
+
 # ------------------------------------------------------------------ waits
 def waiting_calls(paged, dev):
     t, b = torch.float16, torch.bfloat16
