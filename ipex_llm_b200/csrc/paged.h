@@ -22,6 +22,12 @@ struct PagedAttnArgs {
     float* part; Waits waits;
 };
 
+// Probabilities are kept relative to a reference that follows a row's maximum when that grew by more than 2^P_GROW, and in fp16 2^P_LIFT above their
+// place (the division by their sum, which has it too, takes it out): a ratio to the reference from 2^-25 to 2^4 is a normal number, below that the
+// two parts that enter the product share fp16's last bit, 2^-24, so that a key is off by at most 2^-36 of the reference.  Without, a key 2^-14 below the
+// largest lost bits and one 2^-25 below all of them, while the sum counted both.  bf16 has the range of 32 bits.
+constexpr float P_GROW = 4.0f, P_LIFT = 11.0f;                // 2^(4 + 11) < 65504
+
 // two values rounded to 16 bits, and what that left.  bf16 by the multiply-add that takes a 16-bit factor, without unpacking (a chunk of 512 behind 16000
 // keys 182 us, 188 without); fp16's conversions cost nothing more as they are
 template <bool BF> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {

@@ -16,7 +16,8 @@ namespace {
 // keys in registers; the warps' sums meet once a unit.  16 rows do not fill a tcgen05 tile (128), and what bounds the kernel is what it reads:
 // 100 requests of 200 to 8000 bf16 keys, 64 heads on 8, in 124 us (6.1 TB/s), 64 requests of 100 to 16000 e5m2 keys, 32 on 8, in 84.5 us (4.8 TB/s;
 // there the spreading of bytes to halves and the exponentials keep the warps as busy as the reads).
-// P enters the product as a 16-bit value and what its rounding left, two rows of one MMA or two MMAs, so that only the result is rounded.
+// P enters the product as a 16-bit value and what its rounding left, two rows of one MMA or two MMAs, so that only the result is rounded
+// (fp16's range: P_LIFT in paged.h).
 // At most 16 rows, the MMA's; beside the kernel of many rows (paged_prompt.cu), both with 16 rows: 64 requests of 1000 keys, 32 heads on 8, 62 / 91 us (e5m2
 // 60 / 132), 8 of 4000, 32 on 2, 21 / 33, 64 of 316, 8 on 8, 36 / 53.
 constexpr int FEW_ROWS = 16;
@@ -287,14 +288,14 @@ template <int DP, bool BF, bool E5M2, bool TMA, bool EIGHT> struct FewWarp {
                 }
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            grow |= mx[h] > m[h] + 4.0f;                               // -inf: any key
+            grow |= mx[h] > m[h] + P_GROW;                             // -inf: any key
         }
-        // the reference follows the maximum when that grew by more than 2^4: probabilities up to 16 are as exact as those up to 1
+        // the reference follows the maximum when that grew by more than 2^P_GROW: probabilities up to that are as exact as those up to 1
         if (__any_sync(0xffffffffu, grow)) {
             float corr[2];
 #pragma unroll
             for (int h = 0; h < H; h++) {
-                const float to = mx[h] > m[h] + 4.0f ? mx[h] : m[h];
+                const float to = mx[h] > m[h] + P_GROW ? mx[h] : m[h];
                 corr[h] = m[h] == to ? 1.0f : ex2(m[h] - to);
                 m[h] = to;
                 sum[h] *= corr[h];
@@ -306,10 +307,10 @@ template <int DP, bool BF, bool E5M2, bool TMA, bool EIGHT> struct FewWarp {
         uint32_t hi[NT][H], lo[NT][H];
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+            const float shift = (MBF ? 0.0f : P_LIFT) - (m[h] == -INFINITY ? 0.0f : m[h]);
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                const float x = ex2(s[j][2 * h] - ref), y = ex2(s[j][2 * h + 1] - ref);
+                const float x = ex2(s[j][2 * h] + shift), y = ex2(s[j][2 * h + 1] + shift);
                 sum[h] += x + y;
                 split2<MBF>(x, y, hi[j][h], lo[j][h]);
             }

@@ -10,8 +10,8 @@
 // rows behind the last key and pages without boxes by cp.async; e5m2 bytes spread to fp16 in their slot); the next one issues the MMAs and owns the
 // tensor memory.
 // Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
-// P enters P . V as two 16-bit values, the second with what the rounding of the first left, and both multiply V: only the result is rounded.  With one
-// value (182 / 155 us a chunk, 687 / 545 the long prompt below) an output added up to sqrt(2) of the error that rounding the output alone leaves.
+// P enters P . V as two 16-bit values, the second with what the rounding of the first left, and both multiply V: only the result is rounded
+// (fp16's range: P_LIFT in paged.h).  With one value (182 / 155 us a chunk, 687 / 545 the long prompt below) an output added up to sqrt(2) of the error that rounding the output alone leaves.
 // What bounds it: the softmax (two loads of S, 128 exponentials a thread, both parts' stores) with the products between two steps of a tile (3072 clocks of
 // MMAs a step of 256 rows and 128 keys, of which one tile's run beside the other's softmax) and the waits of the roles for one another.  8 prompts of 200
 // to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one of 8000, 32 heads, fp16: 687 us, 763 TFLOP/s; 512 tokens behind
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                         for (int i = 0; i < 64; i += 8) { m0 = max3(m0, x[i], x[i + 1]); m1 = max3(m1, x[i + 2], x[i + 3]); m2 = max3(m2, x[i + 4], x[i + 5]); m3 = max3(m3, x[i + 6], x[i + 7]); }
                     }
                     const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * mul;
-                    const bool grow = mx > m_ref + 6.0f;                           // -inf: any visible key
+                    const bool grow = mx > m_ref + (MBF ? 6.0f : P_GROW);          // -inf: any visible key; bf16 has room for more
                     if (__any_sync(0xffffffffu, grow)) {
                         const float m_new = grow ? mx : m_ref;
                         if (j > start) {
@@ -418,8 +418,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                         }
                         m_ref = m_new;
                     }
-                    // fp16: 2^8 above the reference's place, so that values from 2^-24 to 2^14 of it are normal numbers or close
-                    const float shift = (MBF ? 0.0f : 8.0f) - (m_ref == -INFINITY ? 0.0f : m_ref);
+                    const float shift = (MBF ? 0.0f : P_LIFT) - (m_ref == -INFINITY ? 0.0f : m_ref);
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
                     // P of 32 keys goes where their scores were: the high parts to the first 16 columns, what their rounding left to the others
                     auto exponentials = [&](int h) {
