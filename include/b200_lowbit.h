@@ -283,13 +283,19 @@ int lowbit_greedy_start_cuda(const void* d_logits, int dtype, int64_t row_stride
  * table; *d_free_left (may be d_free_count) = pages left.  d_cu_seqlens [R + 1], d_seq_lens [R] = held + new, and for each of n_tokens
  * rows d_positions and d_slots (int64): the position and the slot, 0 and -1 behind the last token.  Where the stack or the table's
  * width runs out, entries and slots are -1 and *d_missing counts the pages that were not to be had; later requests go without first.
- * lowbit_paged_release_cuda: rows with d_done[r] != 0 give back every page of their row (in its order) and become -1. */
+ * What the table names behind d_held is written over: a step that ran short is taken back before it is repeated (the pages that it did hand
+ * out would be nobody's), by lowbit_paged_release_behind_cuda for all rows with its d_held, and so are tokens that a request drops.  The count that
+ * a later call gets is the one that this call left.
+ * lowbit_paged_release_cuda: rows with d_done[r] != 0 give back every page of their row (in its order) and become -1.
+ * lowbit_paged_release_behind_cuda: those rows give back the pages behind their first ceil(d_held[r] / page_size). */
 int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_held, int R, int32_t* d_table, int64_t table_stride, int width,
                            const int32_t* d_free_pages, int n_pages, const int32_t* d_free_count, int32_t* d_free_left, int page_size,
                            int64_t n_tokens, int32_t* d_cu_seqlens, int32_t* d_seq_lens, int64_t* d_positions, int64_t* d_slots,
                            int32_t* d_missing, void* stream);
 int lowbit_paged_release_cuda(const uint8_t* d_done, int R, int32_t* d_table, int64_t table_stride, int width, int32_t* d_free_pages,
                               int n_pages, int32_t* d_free_count, void* stream);
+int lowbit_paged_release_behind_cuda(const uint8_t* d_done, const int32_t* d_held, int R, int32_t* d_table, int64_t table_stride, int width,
+                                     int page_size, int32_t* d_free_pages, int n_pages, int32_t* d_free_count, void* stream);
 /* Rotary embedding (rotate_half pairing over the first rotary_dim elements of a head, tables [n_positions][>= rotary_dim / 2] indexed by
  * position; rotary_dim 0: none, tables and positions NULL) of the q and k heads of the merged projection's output d_qkv
  * [T][(Hq + 2 Hkv) * D], in place, and the write of keys and values into their slots; a slot outside the cache is not written.

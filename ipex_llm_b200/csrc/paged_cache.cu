@@ -4,7 +4,8 @@
 // off a stack of free ones; its row of the block table; and for every new token its position and its slot (page * page_size + row).  With
 //   need_r = ceil((held_r + new_r) / page_size) - ceil(held_r / page_size)      and      before_r = sum of need over the requests in front,
 // request r's i-th new page is free[count - 1 - (before_r + i)], so a token's slot follows from two prefix sums and nobody waits for a
-// neighbour's page.
+// neighbour's page.  What the table names behind held_r is written over, not looked at: such pages (a step that ran short and is repeated, tokens that a
+// request drops) go back first (lowbit_paged_release_behind_cuda).
 #include "paged.h"
 
 using namespace lowbit;
@@ -138,9 +139,9 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const StepArgs
     }
 }
 
-// rows that are done give back every page that they hold, in the order of the table, and forget them
-__global__ void __launch_bounds__(STEP_THREADS) paged_release_kernel(const uint8_t* done, int R, int32_t* table, int64_t table_stride, int width,
-                                                                     int32_t* pages, int n_pages, int32_t* count) {
+// rows that are done give back every page that they hold, in the order of the table, and forget them; with `held` those behind its tokens
+__global__ void __launch_bounds__(STEP_THREADS) paged_release_kernel(const uint8_t* done, const int32_t* held, int page_size, int R, int32_t* table, int64_t table_stride,
+                                                                     int width, int32_t* pages, int n_pages, int32_t* count) {
     __shared__ Three sums[32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_release_kernel(const uint8
     for (int r = 0; r < R; r++) {
         if (!done[r]) continue;
         int32_t* row = table + r * table_stride;
-        for (int c0 = 0; c0 < width; c0 += blockDim.x) {
+        for (int c0 = held ? min(pages_of(max(held[r], 0), page_size), width) : 0; c0 < width; c0 += blockDim.x) {
             const int c = c0 + threadIdx.x;
             const int page = c < width ? row[c] : -1;
             Three total;
@@ -324,17 +325,28 @@ extern "C" int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_hel
     return check_launch();
 }
 
-extern "C" int lowbit_paged_release_cuda(const uint8_t* d_done, int R, int32_t* d_table, int64_t table_stride, int width, int32_t* d_free_pages,
-                                         int n_pages, int32_t* d_free_count, void* stream) {
+static int release(const char* name, const uint8_t* d_done, const int32_t* d_held, int page_size, int R, int32_t* d_table, int64_t table_stride, int width, int32_t* d_free_pages,
+                   int n_pages, int32_t* d_free_count, void* stream) {
     reset_launch_count();
-    if (!d_done || !d_table || !d_free_pages || !d_free_count || R <= 0 || width <= 0 || table_stride < width || n_pages <= 0) {
-        set_error(LB_ERR_ARG, "lowbit_paged_release_cuda: bad argument (R %d, width %d, pages %d)", R, width, n_pages);
+    if (!d_done || !d_table || !d_free_pages || !d_free_count || R <= 0 || width <= 0 || table_stride < width || n_pages <= 0 || page_size <= 0) {
+        set_error(LB_ERR_ARG, "%s: bad argument (R %d, width %d, pages %d, page_size %d)", name, R, width, n_pages, page_size);
         return LB_ERR_ARG;
     }
-    launch_behind(paged_release_kernel, dim3(1), STEP_THREADS, 0, (cudaStream_t)stream, launch_overlaps((cudaStream_t)stream), d_done, R, d_table, table_stride, width, d_free_pages,
-                  n_pages, d_free_count);
+    launch_behind(paged_release_kernel, dim3(1), STEP_THREADS, 0, (cudaStream_t)stream, launch_overlaps((cudaStream_t)stream), d_done, d_held, page_size, R, d_table, table_stride,
+                  width, d_free_pages, n_pages, d_free_count);
     note_launch();
     return check_launch();
+}
+
+extern "C" int lowbit_paged_release_cuda(const uint8_t* d_done, int R, int32_t* d_table, int64_t table_stride, int width, int32_t* d_free_pages,
+                                         int n_pages, int32_t* d_free_count, void* stream) {
+    return release("lowbit_paged_release_cuda", d_done, nullptr, 1, R, d_table, table_stride, width, d_free_pages, n_pages, d_free_count, stream);
+}
+
+extern "C" int lowbit_paged_release_behind_cuda(const uint8_t* d_done, const int32_t* d_held, int R, int32_t* d_table, int64_t table_stride, int width,
+                                                int page_size, int32_t* d_free_pages, int n_pages, int32_t* d_free_count, void* stream) {
+    if (!d_held) page_size = 0;                                        // refused
+    return release("lowbit_paged_release_behind_cuda", d_done, d_held, page_size, R, d_table, table_stride, width, d_free_pages, n_pages, d_free_count, stream);
 }
 
 extern "C" int lowbit_paged_rope_append_cuda(void* d_qkv, int dtype, int64_t token_stride, int64_t T, int Hq, int Hkv, int D, int rotary_dim,

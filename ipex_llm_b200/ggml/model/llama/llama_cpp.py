@@ -667,6 +667,9 @@ _lib.lowbit_paged_step_cuda.restype = ctypes.c_int
 _lib.lowbit_paged_release_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                            ctypes.c_void_p, ctypes.c_void_p]
 _lib.lowbit_paged_release_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_release_behind_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+                                                  ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]
+_lib.lowbit_paged_release_behind_cuda.restype = ctypes.c_int
 _lib.lowbit_paged_rope_append_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4 + \
     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _I64P,
      ctypes.c_void_p, _I64P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
@@ -698,6 +701,11 @@ def lowbit_paged_step(new, held, table, free_pages, free_count, free_left, page_
 def lowbit_paged_release(done, table, free_pages, free_count, stream):
     _check(_lib.lowbit_paged_release_cuda(done.data_ptr(), table.shape[0], table.data_ptr(), table.stride(0), table.shape[1], free_pages.data_ptr(),
                                           free_pages.shape[0], free_count.data_ptr(), stream), "lowbit_paged_release_cuda")
+
+
+def lowbit_paged_release_behind(done, held, table, page_size, free_pages, free_count, stream):
+    _check(_lib.lowbit_paged_release_behind_cuda(done.data_ptr(), held.data_ptr(), table.shape[0], table.data_ptr(), table.stride(0), table.shape[1], int(page_size),
+                                                 free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), stream), "lowbit_paged_release_behind_cuda")
 
 
 def _cache_dtype(cache):

@@ -83,7 +83,12 @@ def paged_step(query_lens, context_lens, block_table, free_pages, free_count, pa
     -1 where a request has no page: the pages that the new tokens need are entered (in place); ``free_pages`` int32 [N] with ``free_count``
     int32 [1]: the stack that they come off, the last first; ``n_tokens``: rows of the step's activations (at least the sum of
     ``query_lens``: what is behind it is padding).  ``free_left``: where the number of pages left goes, a new tensor by default;
-    ``free_count`` itself for a server's loop.  Returns a ``PagedStep``."""
+    ``free_count`` itself for a server's loop.  Returns a ``PagedStep``.
+
+    Where ``missing`` is not 0 the pages that there were have been handed out, to earlier requests first.  The step is repeated after it has been
+    taken back, ``paged_release(every row, block_table, free_pages, the count that it left, context_lens, page_size)``, and somebody has gone: what the
+    table names behind ``context_lens`` is written over, and pages that only it named would be nobody's.  The same holds for tokens that a request
+    drops.  The count that the next call gets is the one that this call left: an older one hands pages out twice."""
     out = _native("paged_step", query_lens, context_lens, block_table, free_pages, free_count, page_size, n_tokens, free_left)
     if out is not None:
         return PagedStep._make(out)
@@ -111,17 +116,26 @@ def paged_step(query_lens, context_lens, block_table, free_pages, free_count, pa
     return out
 
 
-def paged_release(done, block_table, free_pages, free_count):
+def paged_release(done, block_table, free_pages, free_count, held=None, page_size=None):
     """Requests that are done give their pages back: rows of ``block_table`` with ``done`` (bool or uint8 [R]) set go onto the stack
-    ``free_pages`` / ``free_count`` and become -1, in place."""
+    ``free_pages`` / ``free_count`` and become -1, in place.  With ``held`` (int32 [R]: tokens that they keep) and the ``page_size`` they give back
+    only what lies behind those: a step that found too few pages is taken back so, and tokens that a request drops."""
     dev = _device(done, block_table, free_pages, free_count)
     invalidInputError(done.dtype in (torch.bool, torch.uint8) and done.dim() == 1 and done.is_contiguous() and done.shape[0] > 0, "done must be a contiguous bool [R]")
     _table(block_table)
     invalidInputError(block_table.shape[0] == done.shape[0], f"{done.shape[0]} requests, {block_table.shape[0]} rows of the block table")
     _ints(free_pages, free_pages.shape[0], "free_pages")
     _ints(free_count, 1, "free_count")
+    invalidInputError((held is None) == (page_size is None), "held and page_size come together")
+    if held is not None:
+        _device(done, held)
+        _ints(held, done.shape[0], "held")
+        invalidInputError(int(page_size) > 0, "page_size must be positive")
     with torch.cuda.device(dev):
-        ggml.lowbit_paged_release(done, block_table, free_pages, free_count, _stream(dev))
+        if held is None:
+            ggml.lowbit_paged_release(done, block_table, free_pages, free_count, _stream(dev))
+        else:
+            ggml.lowbit_paged_release_behind(done, held, block_table, page_size, free_pages, free_count, _stream(dev))
 
 
 def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache):

@@ -132,6 +132,58 @@ def test_release_returns_every_page_once(paged, cuda_device, width):
         assert t.tolist() == [[-1] * width if d else row for row, d in zip(table, done)]
 
 
+def owned_once(table, stack, count, pages):
+    """every page is named by one row or lies on the stack, once"""
+    return sorted([x for row in table.tolist() for x in row if x >= 0] + stack[:int(count)].tolist()) == list(range(pages))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("new,held,page,width,spare,victim", [([40, 5, 20], [3, 9, 17], 8, 9, 3, 1), ([1, 1, 1, 1], [8, 16, 7, 24], 8, 8, 1, 3), ([30, 2, 90], [2, 60, 1], 8, 4, 5, 1),
+                                                              ([700, 1, 2000], [5, 900, 16], 1, 2100, 800, 1)])
+def test_a_step_that_ran_short_is_taken_back_and_repeated(paged, cuda_device, new, held, page, width, spare, victim, in_place):
+    """pages that it handed out go back, a request goes, and the step is repeated: every page stays somebody's, once"""
+    g = torch.Generator().manual_seed(page + sum(new))
+    pages = sum(min(-(-h // page), width) for h in held) + spare
+    table, stack = start(held, page, width, pages, g)
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)                         # noqa: E731
+    t, free, count = on(table), torch.full((pages,), -5, dtype=torch.int32, device=cuda_device), on([len(stack)])
+    free[:len(stack)] = on(stack)
+    st = paged.paged_step(on(new), on(held), t, free, count, page, sum(new), free_left=count if in_place else None)
+    assert st.missing.item() > 0 and owned_once(t, free, st.free_count, pages)
+    everyone = torch.ones(len(new), dtype=torch.bool, device=cuda_device)
+    paged.paged_release(everyone, t, free, st.free_count, on(held), page)
+    assert t.tolist() == table and st.free_count.item() == len(stack) and owned_once(t, free, st.free_count, pages)
+    paged.paged_release(torch.arange(len(new), device=cuda_device) == victim, t, free, st.free_count)
+    new[victim:victim + 1], held[victim:victim + 1] = [0], [0]
+    again = paged.paged_step(on(new), on(held), t, free, st.free_count, page, sum(new))
+    assert owned_once(t, free, again.free_count, pages)
+    want = [min(-(-(h + n) // page), width) for h, n in zip(held, new)]
+    wanted = sum(want) - sum(min(-(-h // page), width) for h in held)
+    assert again.free_count.item() == max(st.free_count.item() - wanted, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [3, 40, 1500])
+def test_tokens_that_a_request_drops_give_their_pages_back(paged, cuda_device, width):
+    g = torch.Generator().manual_seed(width)
+    R, page, pages = 7, 4, 7 * width + 4
+    held = torch.randint(0, width * page + 1, (R,), generator=g).tolist()
+    keep = [min(int(x * (h + 9)), h + 3) for x, h in zip(torch.rand(R, generator=g).tolist(), held)]   # a few more than they hold: nothing goes
+    keep[0], keep[1] = -2, 0
+    done = [True, True, False, True, True, False, True]
+    table, stack = start(held, page, width, pages, g)
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)                         # noqa: E731
+    wide, free, count = torch.full((R, width + 3), 77, dtype=torch.int32, device=cuda_device), torch.full((pages,), -5, dtype=torch.int32, device=cuda_device), on([len(stack)])
+    wide[:, :width], free[:len(stack)] = on(table), on(stack)
+    first = [min(-(-max(k, 0) // page), width) for k in keep]
+    for _ in range(2):                                                                            # the second time there is nothing to return
+        paged.paged_release(torch.tensor(done, device=cuda_device), wide[:, :width], free, count, on(keep), page)
+        want = stack + [p for row, d, f in zip(table, done, first) if d for p in row[f:] if p >= 0]
+        assert count.item() == len(want) and free[:len(want)].tolist() == want and bool((free[len(want):] == -5).all())
+        assert wide[:, :width].tolist() == [row[:f] + [-1] * (width - f) if d else row for row, d, f in zip(table, done, first)] and bool((wide[:, width:] == 77).all())
+
+
 # ------------------------------------------------------------------ the write into the cache
 def rotated(x, cos, sin):
     """64 bits: x [T, H, D], tables [T, rotary width]"""
@@ -811,6 +863,24 @@ def test_refusals_on_the_cpu(paged):
     for t in (x.float().requires_grad_(), x.clone().requires_grad_()):
         with pytest.raises(RuntimeError, match="backward"):
             paged.sdp_packed(t, x, x, i(3))
+
+
+def test_what_a_row_keeps_is_refused_without_a_device(native_lib, paged):
+    lib, p = native_lib._lib, ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p)
+    behind = lambda done=p, held=p, R=2, stride=4, width=4, page=16, pages=8, table=p: lib.lowbit_paged_release_behind_cuda(   # noqa: E731
+        done, held, R, table, stride, width, page, p, pages, p, None)
+    for bad in (dict(done=None), dict(held=None), dict(R=0), dict(stride=3), dict(width=0), dict(page=0), dict(pages=0), dict(table=None)):
+        assert behind(**bad) != 0 and "lowbit_paged_release_behind_cuda" in lib.b200_lowbit_last_error_string().decode(), bad
+        lib.b200_lowbit_clear_error()
+
+
+@pytest.mark.gpu
+def test_what_a_row_keeps_is_refused(paged, cuda_device):
+    i = lambda *n: torch.zeros(n, dtype=torch.int32, device=cuda_device)                          # noqa: E731
+    done = torch.zeros(2, dtype=torch.bool, device=cuda_device)
+    for held, page in ((i(2), None), (None, 16), (i(3), 16), (i(2).long(), 16), (i(2), 0), (i(2).cpu(), 16)):
+        with pytest.raises(RuntimeError):
+            paged.paged_release(done, i(2, 4), i(5), i(1), held, page)
 
 
 @pytest.mark.gpu
