@@ -55,7 +55,8 @@ bool aligned(const at::Tensor& t) {
         if (t.stride(d) % unit) return false;
     return true;
 }
-bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// a gradient, or a tangent of forward mode (which no_grad does not end)
+bool wants_grad(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 bool caches_ok(const at::Tensor* k, const at::Tensor* v, const at::Tensor& like, int64_t dim) {
     return k && v && k->dim() == 4 && v->sizes() == k->sizes() && k->numel() > 0 && k->scalar_type() == v->scalar_type() && k->stride(3) == 1 && v->stride(3) == 1 &&
            k->size(3) == dim && k->device() == like.device() && v->device() == like.device() && (k->scalar_type() == at::kByte || k->scalar_type() == like.scalar_type()) &&
@@ -140,7 +141,7 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         Py_RETURN_NONE;
     const int64_t T = x->size(0);
     if (T <= 0 || x->size(1) != (Hq + 2 * Hkv) * D || x->stride(1) != 1 || (T > 1 && x->stride(0) < x->size(1)) || !ints(slots, T, at::kLong, *x) || !caches_ok(k, v, *x, D) ||
-        k->size(2) != Hkv)
+        k->size(2) != Hkv || wants_grad(*k) || wants_grad(*v))
         Py_RETURN_NONE;
     const at::Tensor *cos = nullptr, *sin = nullptr, *pos = nullptr;
     int64_t R = 0;
@@ -148,7 +149,8 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (a[4] != Py_None) {
         cos = plain(a[4]), sin = plain(a[5]), pos = plain(a[6]);
         if (!cos || !sin || !ints(pos, T, at::kLong, *x) || cos->dim() != 2 || sin->sizes() != cos->sizes() || sin->strides() != cos->strides() || cos->stride(1) != 1 ||
-            cos->size(0) <= 0 || cos->scalar_type() != sin->scalar_type() || cos->device() != x->device() || sin->device() != x->device())
+            cos->size(0) <= 0 || cos->scalar_type() != sin->scalar_type() || cos->device() != x->device() || sin->device() != x->device() || wants_grad(*cos) ||
+            wants_grad(*sin))
             Py_RETURN_NONE;
         table = cos->scalar_type() == at::kFloat ? 0 : half_code(*cos);
         R = cos->size(1);

@@ -8,7 +8,8 @@ of every activation.
 
 A step of a server is ``paged_step`` once (pages, slots, positions: one launch, nothing comes back to the host, so a step can be recorded),
 then per layer ``paged_rope_append`` on the projection's output and ``sdp_paged`` -- or ``sdp_packed`` where every request starts with its
-whole prompt -- and ``paged_release`` for requests that are done.  None of them has a backward pass.
+whole prompt -- and ``paged_release`` for requests that are done.  None of them has a backward pass: tensors that want a
+gradient, or carry a tangent of forward mode, are refused.
 """
 import math
 from typing import NamedTuple
@@ -65,7 +66,10 @@ def _table(block_table):
 
 
 def _no_grad(*tensors):
+    """none of them (None: not given) wants a gradient or carries a tangent"""
+    tensors = [t for t in tensors if t is not None]
     invalidInputError(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), "the paged cache's operators have no backward pass")
+    invalidInputError(all(torch.autograd.forward_ad.unpack_dual(t).tangent is None for t in tensors), "the paged cache's operators have no forward-mode derivative (a tensor carries a tangent)")
 
 
 def _caches(k_cache, v_cache, dtype, head_dim):
@@ -145,7 +149,7 @@ def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, s
     leaves the other elements; None: no rotation.  e5m2 caches keep the rounded activations' nearest value, saturating."""
     if _native("paged_append", qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache) is not None:
         return
-    _no_grad(qkv)
+    _no_grad(qkv, cos, sin, k_cache, v_cache)
     invalidInputError(qkv.dim() == 2 and qkv.dtype in _HALF and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and (qkv.stride(1) == 1 or qkv.numel() == 0),
                       f"qkv must be a half-precision [T, {(n_heads + 2 * n_kv_heads) * head_dim}] with contiguous rows")
     invalidInputError(qkv.shape[0] <= 1 or qkv.stride(0) >= qkv.shape[1], "the rows of qkv overlap")
@@ -204,7 +208,7 @@ def sdp_paged(query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=
         result = _native("sdp_paged", query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_query_len)
         if result is not None:
             return result
-    _no_grad(query, k_cache, v_cache)
+    _no_grad(query, k_cache, v_cache, out)
     dev = _device(query, k_cache, v_cache, block_table, seq_lens, cu_seqlens)
     _table(block_table)
     _caches(k_cache, v_cache, query.dtype, query.shape[-1])
@@ -233,7 +237,7 @@ def sdp_packed(query, key, value, cu_seqlens, scale=None, is_causal=True, max_se
         result = _native("sdp_packed", query, key, value, cu_seqlens, scale, is_causal, max_seqlen)
         if result is not None:
             return result
-    _no_grad(query, key, value)
+    _no_grad(query, key, value, out)
     dev = _device(query, key, value, cu_seqlens)
     invalidInputError(key.dim() == 3 and key.shape == value.shape and key.shape[0] == query.shape[0] and key.shape[2] == query.shape[-1] and key.shape[1] > 0
                       and key.dtype == query.dtype and value.dtype == query.dtype, "keys and values must be [T, kv_heads, head_dim] of the queries' type")

@@ -865,6 +865,47 @@ def test_refusals_on_the_cpu(paged):
             paged.sdp_packed(t, x, x, i(3))
 
 
+def derivatives(paged, dev):
+    """(name, call): every operator with each of its tensors in turn wanting a gradient (``wants``) or carrying a tangent"""
+    fw = torch.autograd.forward_ad
+    i = lambda *n: torch.zeros(n, dtype=torch.int32, device=dev)                                  # noqa: E731
+    h = lambda *n: torch.zeros(n, dtype=torch.float16, device=dev)                                # noqa: E731
+    at = torch.zeros(6, dtype=torch.int64, device=dev)
+    append = lambda qkv, k, v, cos, sin: paged.paged_rope_append(qkv, 4, 2, 64, cos, sin, at, at, k, v)              # noqa: E731
+    attend = lambda q, k, v, out: paged.sdp_paged(q, k, v, i(2, 4), i(2), i(3), out=out)                               # noqa: E731
+    packed = lambda q, k, v, out: paged.sdp_packed(q, k, v, i(3), out=out)                                            # noqa: E731
+    q, c, p = h(6, 4, 64), h(3, 16, 2, 64), h(6, 2, 64)
+    for name, call, tensors in (("append", append, (h(6, 512), c, c, h(9, 64), h(9, 64))), ("paged", attend, (q, c, c, h(6, 4, 64))), ("packed", packed, (q, p, p, h(6, 4, 64))),
+                                ("paged, plain", lambda *t: attend(*t, None), (q, c, c)), ("packed, plain", lambda *t: packed(*t, None), (q, p, p))):
+        for n in range(len(tensors)):
+            def run(change, call=call, tensors=tensors, n=n):
+                return call(*(change(t) if j == n else t.clone() for j, t in enumerate(tensors)))
+            yield f"{name} {n}", lambda run=run: run(lambda t: t.clone().requires_grad_()), lambda run=run: run(lambda t: fw.make_dual(t.clone(), torch.ones_like(t)))
+
+
+def check_derivatives(paged, dev):
+    for name, wants, carries in derivatives(paged, dev):
+        with pytest.raises(RuntimeError, match="backward"):
+            wants()
+            pytest.fail(name)
+        for mode in (torch.enable_grad, torch.no_grad):                                           # no_grad does not end forward mode
+            with mode(), torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+                carries()
+                pytest.fail(name)
+
+
+def test_what_would_need_a_derivative_is_refused_on_the_cpu(paged):
+    check_derivatives(paged, "cpu")
+
+
+@pytest.mark.gpu
+def test_what_would_need_a_derivative_is_refused(paged, cuda_device):
+    check_derivatives(paged, cuda_device)
+    for _, wants, _ in derivatives(paged, cuda_device):
+        with torch.no_grad():
+            wants()
+
+
 def test_what_a_row_keeps_is_refused_without_a_device(native_lib, paged):
     lib, p = native_lib._lib, ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p)
     behind = lambda done=p, held=p, R=2, stride=4, width=4, page=16, pages=8, table=p: lib.lowbit_paged_release_behind_cuda(   # noqa: E731
