@@ -667,6 +667,26 @@ def whole(x):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 128), (8, 1, 64), (16, 1, 128), (6, 2, 256), (5, 5, 16), (12, 1, 96)])
+@pytest.mark.parametrize("new,held,page", [([1, 1, 1], [30, 150, 7], 16), ([1], [150], 1), ([1], [900], 32), ([1, 3, 1], [100, 90, 33], 24)])
+def test_tokens_round_the_result_alone(paged, cuda_device, dtype, eight, heads, kv_heads, dim, new, held, page):
+    """values that nearly cancel, so that the weights' own error is not behind the result's rounding; up to 8 rows a request, and up to 16"""
+    new = [min(n, 16 * kv_heads // heads) for n in new]
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, new, held, heads, kv_heads, dim, dtype, eight, page)
+    q, kind = whole(q), torch.float8_e5m2 if eight else dtype
+    turned = [[whole(x) for x in rows[0]], [(x.float() + 8 - 16 * (torch.arange(len(x), device=cuda_device) % 2)[:, None, None]).to(kind) for x in rows[1]]]
+    for cache, part in zip(caches, turned):
+        for r, x in enumerate(part):
+            j = torch.arange(len(x), device=cuda_device)
+            cache[table[r, j // page].long(), j % page] = x.view(torch.uint8) if eight else x
+    k, v = ([x.half() if eight else x for x in part] for part in turned)
+    scale = 0.25 * dim ** -0.5
+    got = paged.sdp_paged(q, *caches, table, lens, cu, scale, max_query_len=max(new))
+    assert check_once(got, q, k, v, cu_list, len_list, scale, dtype, torch.float16 if eight else dtype) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (8, 1, 64), (6, 2, 256)])
 @pytest.mark.parametrize("new,held,page", [([130], [0], 16), ([70, 200], [30, 20], 24), ([40], [100], 4), ([150], [800], 32)])
 def test_chunks_round_the_result_alone(paged, cuda_device, dtype, eight, heads, kv_heads, dim, new, held, page):
@@ -696,11 +716,13 @@ def test_prompts_round_the_result_alone(paged, cuda_device, dtype, heads, kv_hea
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("keys", [30, 150])
-def test_the_bound_tells_probabilities_of_one_value(dtype, keys):
+@pytest.mark.parametrize("cancel", [0, 8])
+def test_the_bound_tells_probabilities_of_one_value(dtype, keys, cancel):
     """an oracle that rounds its probabilities once is outside it, one that keeps what that left is inside"""
     g = torch.Generator().manual_seed(keys)
     q, k, v = ((1.5 * torch.randn(n, 2, 128, generator=g)).to(dtype) for n in (40, keys, keys))
     q, k, scale = whole(q), whole(k), 0.25 * 128 ** -0.5
+    v = (v.float() + cancel - 2 * cancel * (torch.arange(keys) % 2)[:, None, None]).to(dtype)
     s = torch.einsum("ihd,jhd->hij", q.float(), k.float()) * scale
     p = torch.exp(s - s.amax(-1, keepdim=True))
     high = p.to(dtype).float()
