@@ -48,6 +48,10 @@ int gemv_get_pdl();
 // Who releases early has his TMEM by then (a dependent may allocate in front of its wait), and no parameter is const __restrict__.
 // In a recorded step (the switch on) the launches of these kernels stay ordinary: kernels there read inputs ahead of their wait because an
 // ordinary launch lies in front of them; and in a stream that is being captured the graph's edges are left as they were.
+// Two launches overlap there too: the merges of the paged attentions, behind the kernel of the same call (paged_attention.cu, paged_prompt.cu).  That
+// kernel is ordinary, and its merge waits for all of it before it reads anything, in every block, and releases nobody before it ends; so whatever lies
+// behind the merge has the kernel and all in front of it done, as behind an ordinary launch.  A merge that read ahead of its wait, left before it or
+// released early could not be launched so.
 inline bool launch_overlaps(cudaStream_t st) {
     if (gemv_get_pdl()) return false;
     cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;

@@ -754,6 +754,7 @@ template <int DP, bool BF, bool E5M2> int few_launch(PagedAttnArgs A, bool eight
                       launch_overlaps(st), A, M, box);
     } else launch_behind(paged_few_kernel<DP, BF, E5M2>, dim3((unsigned)C), F::kWarps * 32, F::kSmem, st, launch_overlaps(st), A);
     note_launch();
+    // overlaps in a recorded step too: every block waits first, and none releases before it ends (lowbit_internal.h)
     launch_behind(paged_few_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, FEW_ROWS / 4), 128, 0, st, true, A);
     note_launch();
     return check_launch();

@@ -830,6 +830,7 @@ template <int DP, bool BF, bool E5M2, bool PAGED> int launch(const PagedAttnArgs
     }
     launch_behind(paged_prompt_kernel<DP, BF, E5M2, PAGED>, dim3((unsigned)C), P::kWarps * 32, P::kSmem, st, launch_overlaps(st), A, M, box, above);
     note_launch();
+    // overlaps in a recorded step too: every block waits first, and none releases before it ends (lowbit_internal.h)
     launch_behind(paged_prompt_merge_kernel<DP, BF, E5M2>, dim3((unsigned)C, 4), P::kRows, 0, st, true, A, C);
     note_launch();
     return check_launch();
