@@ -308,7 +308,7 @@ int lowbit_paged_rope_append_cuda(void* d_qkv, int dtype, int64_t token_stride, 
  * 0 .. seq_len - n + i; one that sees none gives zeros, rows of d_out behind the last request stay as they are.  q, out [T][Hq][D],
  * strides {token, head}; fp16 / bf16, D a multiple of 16 up to 256, Hq a multiple of Hkv, at most 256 heads on one (128 where D > 128); pointers and
  * strides 16-byte aligned.  A key in a page outside the cache makes its request's rows NaN, and so may one that is not finite, of keys
- * that a row does not see too.  max_query: no request brings more new tokens than that (T is always right); rows of one that does are
+ * that a row does not see too; a request that holds more tokens than its row of the table can name gives NaN.  max_query: no request brings more new tokens than that (T is always right); rows of one that does are
  * undefined.  Tokens that cu_seqlens names behind row T are not there: the others see what they would with them.
  * Softmax and sums in fp32.  workspace: lowbit_sdp_paged_workspace_size() bytes, one per call in flight, not initialised. */
 size_t lowbit_sdp_paged_workspace_size(int64_t T, int R, int Hq, int Hkv, int D, int64_t max_query);

@@ -57,9 +57,17 @@ __device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& A, int r) {
     if (A.table) {
         // tokens behind row T are not there, and the others see what they would with them
         const int64_t held = A.seq_lens[r] - (b > A.T ? b - (a > A.T ? a : A.T) : 0), most = (int64_t)A.width * A.page_size;
-        q.len = (int)(held < 0 ? 0 : held > most ? most : held);
+        // more than its row of the table can name: every token sees the first key without a page
+        const int64_t len = held > most ? most + q.n : held;
+        q.len = (int)(len < 0 ? 0 : len > 0x7fffffff ? 0x7fffffff : len);
     } else q.len = q.n;
     return q;
+}
+
+// the page of a request's key, -1 behind the table's width
+__device__ __forceinline__ int paged_page(const PagedAttnArgs& A, int r, int key) {
+    const int c = key / A.page_size;
+    return c < A.width ? A.table[r * A.table_stride + c] : -1;
 }
 
 // paged_prompt.cu: requests with more than `above` rows (new tokens x heads of a group) a kv head

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_ker
     auto key_of = [&](const FewAt& w) { return w.tile * F::kTile + warp * KW + (KW == 32 ? lane : lane & 15); };
     auto ask = [&]() {
         const int key = key_of(in);
-        if (to_copy && key < in.q.len) page = A.table[in.r * A.table_stride + key / A.page_size];
+        if (to_copy && key < in.q.len) page = paged_page(A, in.r, key);
     };
     auto copy = [&](int stage) {
         if (!to_copy) return;
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32 + 128), 1) paged_f
         bool more = true;
         auto ask = [&]() {
             const int key = at.tile * F::kTile + mine * box;
-            if (more && some && key < at.q.len) page = A.table[at.r * A.table_stride + key / A.page_size];
+            if (more && some && key < at.q.len) page = paged_page(A, at.r, key);
         };
         ask();
         for (; more && issued < most; issued++) {

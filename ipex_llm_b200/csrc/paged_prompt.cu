@@ -508,7 +508,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
         bool more = any;
         auto ask = [&]() {
             const int64_t key = (int64_t)j * PR_KEYS + w0 + lane;
-            if (PAGED && more && key < at.q.len) page = A.table[at.r * A.table_stride + (int)key / A.page_size];
+            if (PAGED && more && key < at.q.len) page = paged_page(A, at.r, (int)key);
         };
         bool more_keys = any, over = false;                            // tiles behind the one that was placed; behind the last item
         auto where = [&]() {                                           // this lane's key lies, and on to the next tile

@@ -203,7 +203,7 @@ def sdp_paged(query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=
     ``scaled_dot_product_attention``, at most 256 on one kv head (128 where head_dim is above 128).  ``max_query_len``: no request brings more
     new tokens (1 for a decode step; the rows of one that does are undefined); never knowing is right, knowing saves launches.  A token that
     sees no key gives zeros; rows behind the last request are left as they are in ``out``, a new tensor by default.  Pages outside the
-    cache (-1) make their request's rows NaN; keys or values that are not finite may do so to all rows of their request."""
+    cache (-1) make their request's rows NaN, and so do more tokens than its row of the table can name; keys or values that are not finite may do so to all rows of their request."""
     if out is None:
         result = _native("sdp_paged", query, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale, max_query_len)
         if result is not None:

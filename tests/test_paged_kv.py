@@ -394,6 +394,28 @@ def test_values_that_are_not_numbers_stay_with_their_request(paged, cuda_device,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight", KINDS)
+@pytest.mark.parametrize("new,held", [([1, 1, 1, 1], [31, 300, 2000, 48]), ([3, 1, 2, 16], [29, 300, 64, 32]), ([32, 10, 200, 300], [0, 60, 900, 20]), ([1, 20, 1, 40], [31, 45, 65, 30])])
+@pytest.mark.parametrize("page", [16, 4])
+def test_a_request_that_holds_more_than_its_row_can_name(paged, cuda_device, dtype, eight, new, held, page):
+    """its rows are NaN, as for a page that is not there, and not the attention of other positions; one that fills its row is not touched by it"""
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, new, held, 4, 2, 64, dtype, eight, page)
+    width = 32 // page
+    got = paged.sdp_paged(q, *caches, table[:, :width], lens, cu)
+    if eight:
+        rows = [[x.half() for x in part] for part in rows]
+    want, absolute, largest = statement(q, *rows, cu_list, len_list, 64 ** -0.5)
+    limit = bound(want, absolute, largest, dtype, torch.float16 if eight else dtype, 64, 32)
+    assert len_list[0] == 32
+    for r, n in enumerate(len_list):
+        a, b = cu_list[r], cu_list[r + 1]
+        if n > 32:
+            assert bool(torch.isnan(got[a:b]).all()), r
+        else:
+            assert bool(((got[a:b].double() - want[a:b]).abs() <= limit[a:b]).all()), r
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,eight", [KINDS[1], KINDS[3]])
 def test_a_cache_beyond_32_bits(paged, cuda_device, dtype, eight):
     """offsets of more than 2^32 elements, and a layout with the heads in front of the rows"""
