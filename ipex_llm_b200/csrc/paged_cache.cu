@@ -19,12 +19,15 @@ struct StepArgs {
     const int32_t* pages; int n_pages; const int32_t* count; int32_t* left;
     int page_size; int64_t n_tokens;
     int32_t *cu, *seq_lens; int64_t *positions, *slots; int32_t* missing;
+    int lost_most;                                            // pages behind the table's width that a request counts at most: the sum stays in 32 bits
 };
 
 constexpr int STEP_THREADS = 1024;
 
+constexpr int64_t MOST = 0x7fffffff;
+
 __device__ __forceinline__ int pages_of(int64_t tokens, int page) {
-    return tokens < 1ll << 31 ? (int)(((uint32_t)tokens + (uint32_t)page - 1u) / (uint32_t)page) : (int)((tokens + page - 1) / page);
+    return tokens <= MOST ? (int)(((uint32_t)tokens + (uint32_t)page - 1u) / (uint32_t)page) : (int)min((tokens + page - 1) / page, MOST);
 }
 
 // inclusive sums of three values over the block; t*: those of the whole block
@@ -99,7 +102,8 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const StepArgs
         const int r = r0 + threadIdx.x, in_round = min((int)blockDim.x, A.R - r0);
         const int held = r < A.R ? max(A.held[r], 0) : 0, fresh = r < A.R ? max(A.fresh[r], 0) : 0;
         const int had = min(pages_of(held, A.page_size), A.width), all_pages = pages_of((int64_t)held + fresh, A.page_size);
-        const int need = max(min(all_pages, A.width) - had, 0), lost = r < A.R ? max(all_pages - A.width, 0) - max(pages_of(held, A.page_size) - A.width, 0) : 0;
+        const int need = max(min(all_pages, A.width) - had, 0);
+        const int lost = r < A.R ? min(max(all_pages - A.width, 0) - max(pages_of(held, A.page_size) - A.width, 0), A.lost_most) : 0;
         Three total;
         const Three x = block_scan3({fresh, need, lost}, sums, total);
         first[threadIdx.x] = tokens + x.a - fresh;
@@ -107,8 +111,8 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const StepArgs
         holds[threadIdx.x] = held;
         has[threadIdx.x] = had;
         if (r < A.R && rank == 0) {
-            A.cu[r + 1] = (int32_t)(tokens + x.a);
-            A.seq_lens[r] = held + fresh;
+            A.cu[r + 1] = (int32_t)min(tokens + x.a, MOST);             // what 32 bits cannot say is their largest, and behind every row
+            A.seq_lens[r] = (int32_t)min((int64_t)held + fresh, MOST);
         }
         __syncthreads();
         // page i of the round's new ones
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(STEP_THREADS) paged_step_kernel(const StepArgs
     if (blocks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     else __syncthreads();
     if (me == 0) {
-        *A.missing = max(taken - count, 0) + over;
+        *A.missing = (int32_t)min((int64_t)max(taken - count, 0) + over, MOST);
         *A.left = max(count - taken, 0);
     }
 }
@@ -298,13 +302,14 @@ extern "C" int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_hel
                                       int32_t* d_missing, void* stream) {
     reset_launch_count();
     if (!d_new || !d_held || !d_table || !d_free_pages || !d_free_count || !d_free_left || !d_cu_seqlens || !d_seq_lens || !d_missing ||
-        (n_tokens > 0 && (!d_positions || !d_slots)) || R <= 0 || width <= 0 || table_stride < width || n_pages <= 0 || page_size <= 0 || n_tokens < 0) {
+        (n_tokens > 0 && (!d_positions || !d_slots)) || R <= 0 || width <= 0 || table_stride < width || n_pages <= 0 || page_size <= 0 || n_tokens < 0 ||
+        (int64_t)R * width > 0x7fffffffll) {                            // pages are counted in 32 bits
         set_error(LB_ERR_ARG, "lowbit_paged_step_cuda: bad argument (R %d, width %d, pages %d, page_size %d, tokens %lld)", R, width, n_pages, page_size,
                   (long long)n_tokens);
         return LB_ERR_ARG;
     }
     const StepArgs A = {d_new, d_held, R, d_table, table_stride, width, d_free_pages, n_pages, d_free_count, d_free_left, page_size, n_tokens,
-                        d_cu_seqlens, d_seq_lens, d_positions, d_slots, d_missing};
+                        d_cu_seqlens, d_seq_lens, d_positions, d_slots, d_missing, 0x7fffffff / R};
     // A block for a decode step, a cluster of eight (the most that any device takes) for more tokens; blocks of 1024 threads where requests or
     // tokens are many.  One block / eight, of 256 threads: 32 requests with a token each 3.1 / 3.5 us, 4 with 800 tokens in all 4.5 / 3.6, 16
     // with 5000 14 / 4.8; of 1024: 500 requests with a token each 4.5 / 4.7, 19000 tokens 27 / 8.4.  256 / 1024 threads, eight blocks: 5000 tokens 4.8 /

@@ -132,6 +132,42 @@ def test_release_returns_every_page_once(paged, cuda_device, width):
         assert t.tolist() == [[-1] * width if d else row for row, d in zip(table, done)]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 2])
+def test_lengths_that_32_bits_cannot_add(paged, cuda_device, page):
+    """a request that would bring its end beyond 2^31: what its row can name is handed out once, and the counts are the largest that there are"""
+    most = (1 << 31) - 1
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)                         # noqa: E731
+    for new, held in (([most], [1]), ([2, most, most], [1, 3, 2]), ([most, most], [most, 0])):
+        R, width = len(new), 4
+        had = [min(-(-h // page), width) for h in held]
+        table = [[10 * r + c if c < had[r] else -1 for c in range(width)] for r in range(R)]
+        stack = list(range(100, 130))
+        want, left = [list(row) for row in table], list(stack)
+        for r in range(R):
+            for c in range(had[r], min(-(-(held[r] + new[r]) // page), width)):
+                want[r][c] = left.pop()
+        t, count = on(table), on([len(stack)])
+        st = paged.paged_step(on(new), on(held), t, on(stack), count, page, 6)
+        assert t.tolist() == want and st.free_count.item() == len(left)
+        ends = [0]
+        for n in new:
+            ends.append(ends[-1] + n)
+        assert st.cu_seqlens.tolist() == [min(e, most) for e in ends] and st.seq_lens.tolist() == [min(h + n, most) for h, n in zip(held, new)]
+        for i, (p, s) in enumerate(zip(st.positions.tolist(), st.slots.tolist())):
+            r = next(r for r in range(R) if ends[r + 1] > i)
+            at = held[r] + i - ends[r]
+            assert p == at and s == (want[r][at // page] * page + at % page if at // page < width else -1)
+        assert st.missing.item() > most // 8
+
+
+def test_a_table_of_more_entries_than_32_bits_is_refused(native_lib):
+    lib, p = native_lib._lib, ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p)
+    assert lib.lowbit_paged_step_cuda(p, p, 1 << 16, p, 1 << 15, 1 << 15, p, 8, p, p, 16, 3, p, p, p, p, p, None) != 0
+    assert "lowbit_paged_step_cuda" in lib.b200_lowbit_last_error_string().decode()
+    lib.b200_lowbit_clear_error()
+
+
 def owned_once(table, stack, count, pages):
     """every page is named by one row or lies on the stack, once"""
     return sorted([x for row in table.tolist() for x in row if x >= 0] + stack[:int(count)].tolist()) == list(range(pages))
