@@ -714,7 +714,7 @@ def _cache_dtype(cache):
 
 def lowbit_paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary_dim, cos, sin, positions, slots, k_cache, v_cache, stream):
     """qkv [T, (Hq + 2 Hkv) * D]; cos / sin [positions, rotary_dim] or None; caches [pages, page_size, Hkv, D]"""
-    _check(_lib.lowbit_paged_rope_append_cuda(qkv.data_ptr(), _DT_OF[qkv.dtype], qkv.stride(0), qkv.shape[0], n_heads, n_kv_heads, head_dim, rotary_dim,
+    _check(_lib.lowbit_paged_rope_append_cuda(qkv.data_ptr(), _DT_OF[qkv.dtype], qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1], qkv.shape[0], n_heads, n_kv_heads, head_dim, rotary_dim,
                                               cos.data_ptr() if rotary_dim else None, sin.data_ptr() if rotary_dim else None,
                                               _DT_OF[cos.dtype] if rotary_dim else 0, cos.stride(0) if rotary_dim else 0, cos.shape[0] if rotary_dim else 0,
                                               positions.data_ptr() if rotary_dim else None, slots.data_ptr(), k_cache.data_ptr(), _strides(k_cache, 3),

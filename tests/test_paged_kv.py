@@ -654,6 +654,32 @@ def test_a_recorded_step_serves_other_lengths(paged, cuda_device, dtype, eight):
 
 
 @pytest.mark.gpu
+def test_the_python_statements_say_the_same(paged, cuda_device, monkeypatch):
+    """what serves where the native host side is not to be had, a lone token with any stride among it"""
+    dev = cuda_device
+    on = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)                                 # noqa: E731
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(paged, "_native", lambda *args: None)
+        g = torch.Generator(device=dev).manual_seed(8)
+        for T in (1, 5):
+            table, free, count = torch.full((1, 4), -1, dtype=torch.int32, device=dev), on([3, 1, 0, 2]), on([4])
+            st = paged.paged_step(on([T]), on([0]), table, free, count, 2, T)
+            cos, sin = tables(64, 50, dev)
+            caches = [torch.zeros(4, 2, 2, 64, dtype=torch.float16, device=dev) for _ in range(2)]
+            qkv = torch.randn(T, 8 * 64, generator=g, device=dev).half()
+            if T == 1:
+                qkv = qkv.as_strided((1, 512), (1, 1))
+            paged.paged_rope_append(qkv, 4, 2, 64, cos, sin, st.positions, st.slots, *caches)
+            x = qkv.view(T, 8, 64)
+            results.append((*st, table, qkv.clone(), *caches, paged.sdp_paged(x[:, :4], *caches, table, st.seq_lens, st.cu_seqlens, max_query_len=T),
+                            paged.sdp_packed(x[:, :4], x[:, 4:6], x[:, 6:], st.cu_seqlens)))
+    for a, b in ((results[0], results[2]), (results[1], results[3])):
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and len(a) == len(b)
+
+
+@pytest.mark.gpu
 def test_on_other_streams_at_once(paged, cuda_device):
     """two streams, other lengths on each, many calls in flight: every result is that of the call alone"""
     sets = [requests(cuda_device, new, held, 8, 2, 128, torch.bfloat16, eight, 16, seed=i)
