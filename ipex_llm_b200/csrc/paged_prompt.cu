@@ -370,7 +370,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                 const int end = min(at.b, at.tiles_of(A, group, t));
                 const bool some = end > at.a, from_start = at.a == 0, whole = from_start && at.b == at.tiles;
                 const int64_t oi = live ? (at.q.q0 + token) * A.o_st + (int64_t)(at.hk * group + row % group) * A.o_sh : -1;
-                float m_ref = -INFINITY, sum = 0.0f;
+                float top = -INFINITY, sum = 0.0f;              // the reference, as a score
                 const int start = at.a;
                 more = at.next(A, group, P::kRows, above);             // in the time that the first scores take
                 const bool coming = more && needed(at);                // the next piece's queries
@@ -398,13 +398,13 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
 #pragma unroll
                         for (int i = 0; i < 64; i += 8) { m0 = max3(m0, x[i], x[i + 1]); m1 = max3(m1, x[i + 2], x[i + 3]); m2 = max3(m2, x[i + 4], x[i + 5]); m3 = max3(m3, x[i + 6], x[i + 7]); }
                     }
-                    const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * mul;
-                    const bool grow = mx > m_ref + (MBF ? 6.0f : P_GROW);          // -inf: any visible key; bf16 has room for more
+                    const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+                    const bool grow = (mx - top) * mul > (MBF ? 6.0f : P_GROW);    // -inf: any visible key; bf16 has room for more
                     if (__any_sync(0xffffffffu, grow)) {
-                        const float m_new = grow ? mx : m_ref;
+                        const float top_new = grow ? mx : top;
                         if (j > start) {
                             // the P . V before this Q . K is done: O is at rest
-                            const float corr = grow ? ex2(m_ref - m_new) : 1.0f;
+                            const float corr = grow ? ex2((top - top_new) * mul) : 1.0f;
                             sum *= corr;
 #pragma unroll 1
                             for (int i = 0; i < DP; i += 16) {
@@ -416,9 +416,12 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                                 tmem_st16x(ot + i, reinterpret_cast<const uint32_t*>(o));
                             }
                         }
-                        m_ref = m_new;
+                        top = top_new;
                     }
-                    const float shift = (MBF ? 0.0f : P_LIFT) - (m_ref == -INFINITY ? 0.0f : m_ref);
+                    // the multiply-add's two terms are each rounded once: 2^-8 apart up to 2^16.  Beyond, scores lose the reference first, exactly or nearly
+                    const float m_ref = top == -INFINITY ? 0.0f : top * mul;
+                    const bool steep = fabsf(m_ref) > 65536.0f, any_steep = __any_sync(0xffffffffu, steep);
+                    const float shift = (MBF ? 0.0f : P_LIFT) - (steep ? 0.0f : m_ref);
                     float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
                     // P of 32 keys goes where their scores were: the high parts to the first 16 columns, what their rounding left to the others
                     auto exponentials = [&](int h) {
@@ -444,10 +447,15 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
 #pragma unroll 1
                     for (int h = 0; h < 2; h++) {
                         load(h);
+                        if (any_steep) {
+#pragma unroll
+                            for (int i = 0; i < 64; i++) x[i] -= steep ? top : 0.0f;
+                        }
                         exponentials(h);
                     }
                     sum += (a0 + a1) + (a2 + a3);
                 }
+                const float m_ref = top * mul;
                 if (coming) queries(at);                               // the last product with the old ones is done
                 if (some) {
                     if (!mbar_wait_lim(pv_done(t), (steps - 1) & 1, A.waits)) goto done;

@@ -392,6 +392,31 @@ def test_flat_and_steep_softmax(paged, cuda_device, dtype, eight, new, held, q_s
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,eight,big", [(torch.float16, False, 2.0 ** 12), (torch.float16, False, 1.0), (torch.bfloat16, False, 2.0 ** 90), (torch.bfloat16, False, 2.0 ** 12),
+                                             (torch.float16, True, 2.0 ** 12), (torch.bfloat16, True, 2.0 ** 90), (torch.bfloat16, True, 2.0 ** 12)])
+@pytest.mark.parametrize("new,held", [([1], [700]), ([3, 1], [20, 300]), ([40], [200]), ([300, 70], [0, 900])])
+def test_scores_beyond_what_32_bits_tell_apart(paged, cuda_device, dtype, eight, big, new, held):
+    """scores of 10^4 to 10^31, whose neighbours in 32 bits lie up to 10^24 apart: a row takes the value of its largest, far ahead of the others"""
+    heads, kv_heads, dim = 4, 2, 64
+    q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, new, held, heads, kv_heads, dim, dtype, eight, 16)
+    q, kind = (whole(q).double() * big).to(dtype), torch.float8_e5m2 if eight else dtype
+    k = [(whole(x).float() * 4096).to(kind) for x in rows[0]]
+    for r, x in enumerate(k):
+        j = torch.arange(len(x), device=cuda_device)
+        caches[0][table[r, j // 16].long(), j % 16] = x.view(torch.uint8) if eight else x
+    got = paged.sdp_paged(q, *caches, table, lens, cu)
+    assert bool(torch.isfinite(got).all())
+    for r, (a, b, n) in enumerate(zip(cu_list, cu_list[1:], len_list)):
+        s = torch.einsum("ihd,jhd->hij", q[a:b].double(), k[r].double().repeat_interleave(2, 1)) * dim ** -0.5          # exact: whole numbers of few bits
+        s = s.masked_fill(torch.arange(n, device=cuda_device)[None] > n - (b - a) + torch.arange(b - a, device=cuda_device)[:, None], -math.inf)
+        top = s.topk(min(2, n), -1).values
+        # the second is behind by more than the scores' rounding and than any weight that counts
+        clear = (top[..., 0] - top[..., -1] > 64 + top[..., 0].abs() * 2.0 ** -20) | (torch.arange(b - a, device=cuda_device)[None] + n - (b - a) == 0)
+        want = rows[1][r].to(dtype).repeat_interleave(2, 1).permute(1, 0, 2).gather(1, s.argmax(-1)[..., None].expand(-1, -1, dim)).transpose(0, 1)
+        assert bool((clear.float().mean() > 0.5)) and torch.equal(got[a:b][clear.t()], want[clear.t()])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,eight", KINDS)
 def test_requests_without_keys_and_rows_behind_the_last(paged, cuda_device, dtype, eight):
     q, caches, table, lens, cu, rows, cu_list, len_list = requests(cuda_device, [3, 0, 1, 150], [20, 9, 4, 7], 8, 2, 64, dtype, eight, 16)
