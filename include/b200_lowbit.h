@@ -281,7 +281,7 @@ int lowbit_greedy_start_cuda(const void* d_logits, int dtype, int64_t row_stride
  * lowbit_paged_step_cuda: what a step needs, from d_held (tokens that each request holds) and d_new (tokens that it brings).  Pages that the
  * new tokens need beyond ceil(held / page_size) come off the top of the stack d_free_pages[0 .. *d_free_count) and are entered into the
  * table; *d_free_left (may be d_free_count) = pages left.  d_cu_seqlens [R + 1], d_seq_lens [R] = held + new, and for each of n_tokens
- * rows d_positions and d_slots (int64): the position and the slot, 0 and -1 behind the last token.  Where the stack or the table's
+ * rows d_positions and d_slots (int64): the position and the slot, 0 and -1 behind the last token.  R * width < 2^31.  Where the stack or the table's
  * width runs out, entries and slots are -1 and *d_missing counts the pages that were not to be had; later requests go without first.
  * What the table names behind d_held is written over: a step that ran short is taken back before it is repeated (the pages that it did hand
  * out would be nobody's), by lowbit_paged_release_behind_cuda for all rows with its d_held, and so are tokens that a request drops.  The count that

@@ -29,7 +29,7 @@ struct PagedAttnArgs {
 constexpr float P_GROW = 4.0f, P_LIFT = 11.0f;                // 2^(4 + 11) < 65504
 
 // two values rounded to 16 bits, and what that left.  bf16 by the multiply-add that takes a 16-bit factor, without unpacking (a chunk of 512 behind 16000
-// keys 182 us, 188 without); fp16's conversions cost nothing more as they are
+// keys 181 us, 188 without); fp16's conversions cost nothing more as they are
 template <bool BF> __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     if (BF) asm("{\n\t.reg .b16 p, q, m;\n\t.reg .f32 a, b;\n\t"
                 "cvt.rn.bf16x2.f32 %0, %3, %2;\n\t"

@@ -14,12 +14,13 @@ namespace {
 // ------------------------------------------------------------------ few rows (decoding): at most 16 rows = new tokens x heads of a group
 // One pass over the keys: a warp takes 16 or 32 of a tile, S = Q . K^T and O += P . V by mma.sync m16n8k16 with the running maximum and sum of its
 // keys in registers; the warps' sums meet once a unit.  16 rows do not fill a tcgen05 tile (128), and what bounds the kernel is what it reads:
-// 100 requests of 200 to 8000 bf16 keys, 64 heads on 8, in 124 us (6.1 TB/s), 64 requests of 100 to 16000 e5m2 keys, 32 on 8, in 84.5 us (4.8 TB/s;
-// there the spreading of bytes to halves and the exponentials keep the warps as busy as the reads).
+// 100 requests of 200 to 8000 bf16 keys, 64 heads on 8, in 124 us (6.1 TB/s), 64 requests of 100 to 16000 e5m2 keys, 32 on 8, in 84.7 us (4.8 TB/s;
+// there the two computing warps of a scheduler wait for the fixed latencies of their chains: issue slots 44 % busy, tensor pipe 31 %, DRAM 72 %).
 // P enters the product as a 16-bit value and what its rounding left, two rows of one MMA or two MMAs, so that only the result is rounded
 // (fp16's range: P_LIFT in paged.h).
-// At most 16 rows, the MMA's; beside the kernel of many rows (paged_prompt.cu), both with 16 rows: 64 requests of 1000 keys, 32 heads on 8, 62 / 91 us (e5m2
-// 60 / 132), 8 of 4000, 32 on 2, 21 / 33, 64 of 316, 8 on 8, 36 / 53.
+// At most 16 rows, the MMA's.  This kernel / that of many rows (paged_prompt.cu), 64 requests of 1000 keys on 8 heads, with 4, 8, 12 and 16 rows: bf16 52, 53,
+// 58, 59 / 97 us, e5m2 43, 44, 57, 58 / 134 to 137; one of 8000 with 16 rows 19 / 39, e5m2 19 / 43.  From 17 rows on there is the other alone: 64 requests with
+// 20 to 48 rows 105 to 107, e5m2 146 to 148, so that one row more than 16 costs as much as 30.
 constexpr int FEW_ROWS = 16;
 
 template <int DP, bool E5M2> struct Few {
@@ -86,11 +87,11 @@ __device__ __forceinline__ int few_tiles(const PagedReq& q, int group, int tile)
 }
 
 // What a unit costs beside its keys (queries, the warps' sums, the result), in tiles: shares are taken of places, FEW_EXTRA of them in front of
-// a unit's tiles, so that blocks with many short requests are not the last.  0 / 1 / 2 / 3: the 64 e5m2 requests above 124 / 100 / 84 / 88 us, the 100 of bf16
-// 148 / 129 / 124 / 126, one token over 4000 e5m2 keys 18.6 / 17.3 / 17.3 / 18.1
+// a unit's tiles, so that blocks with many short requests are not the last.  0 / 1 / 2 / 3: the 64 e5m2 requests above 124 / 102 / 85 / 88 us, the 100 of bf16
+// 148 / 129 / 124 / 126, one token over 4000 e5m2 keys 18.3 / 17.1 / 16.9 / 17.8
 constexpr int FEW_EXTRA = 2;
-// Places that a block takes at least.  1 / 2 / 3: one request of 8000 bf16 keys, 16 heads on one, 25 / 18 / 16 us, of e5m2 20 / 16 / 18, of 500 e5m2 keys, 32 heads,
-// 10.4 / 10.6 / 11.7
+// Places that a block takes at least.  1 / 2 / 3: one request of 8000 bf16 keys, 16 heads on one, 25.5 / 17.3 / 16.3 us, of e5m2 20.4 / 16.2 / 17.9, of 500 e5m2 keys,
+// 32 heads, 10.4 / 10.6 / 11.7
 constexpr int FEW_LEAST = 2;
 // where a block is in its share: request, kv head, tile of that head, and the end of the piece that it takes of them
 struct FewAt {
@@ -427,7 +428,7 @@ template <int DP, bool BF, bool E5M2, bool TMA, bool EIGHT> struct FewWarp {
 };
 
 // Every warp copies its own keys: page sizes that TMA has no box for (no multiple of 8 rows, or a stride of 0).  Where both serve: one token over 4000 e5m2
-// keys 20.5 us for 17.3, the 64 requests 130 for 100, the 100 requests 173 for 129
+// keys 20.4 us for 16.9, the 64 requests 125 for 85, the 100 requests 173 for 124
 template <int DP, bool BF, bool E5M2>
 __global__ void __launch_bounds__((Few<DP, E5M2>::kWarps * 32), 1) paged_few_kernel(const PagedAttnArgs A) {
     using F = Few<DP, E5M2>;
@@ -808,8 +809,8 @@ extern "C" int lowbit_sdp_paged_cuda(const void* d_q, int q_dtype, const int64_t
     A.part = (float*)workspace;
     if (max_query > T) max_query = T;
     cudaStream_t st = (cudaStream_t)stream;
-    // no unit has more than 8 rows: the other 8 of the MMA carry what rounding P left.  Else / so: one token over 4000 e5m2 keys 19.3 / 17.3 us, the 64
-    // requests 114 / 100, the 100 requests 138 / 129
+    // no unit has more than 8 rows: the other 8 of the MMA carry what rounding P left.  Else / so: one token over 4000 e5m2 keys 19.1 / 16.9 us, the 64
+    // requests 104 / 85, the 100 requests 126 / 124
     const bool eight = max_query * (Hq / Hkv) <= 8;
     if (const int rc = D <= 64 ? few_launch_types<64>(A, eight, st) : D <= 128 ? few_launch_types<128>(A, eight, st) : few_launch_types<256>(A, eight, st)) return rc;
     if (max_query * (Hq / Hkv) <= FEW_ROWS) return LB_OK;

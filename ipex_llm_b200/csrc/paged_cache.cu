@@ -313,7 +313,8 @@ extern "C" int lowbit_paged_step_cuda(const int32_t* d_new, const int32_t* d_hel
     // A block for a decode step, a cluster of eight (the most that any device takes) for more tokens; blocks of 1024 threads where requests or
     // tokens are many.  One block / eight, of 256 threads: 32 requests with a token each 3.1 / 3.5 us, 4 with 800 tokens in all 4.5 / 3.6, 16
     // with 5000 14 / 4.8; of 1024: 500 requests with a token each 4.5 / 4.7, 19000 tokens 27 / 8.4.  256 / 1024 threads, eight blocks: 5000 tokens 4.8 /
-    // 5.1, 8000 tokens 6.1 / 5.4; one block: 256 requests 3.3 / 4.3, 500 requests 4.9 / 4.5.
+    // 5.0, 7000 5.5 / 5.0, 8000 6.1 / 5.2; one block: 256 requests 3.3 / 4.2, 257 4.6 / 4.2, 500 5.0 / 4.4.  Near the borders, one block / eight: 400 tokens of one or 4
+    // requests 3.5 / 3.6, of 100 4.0 / 3.4, 600 of 4 4.0 / 3.5, of 100 4.7 / 3.4.
     const bool many = n_tokens > 512, wide = R > 256 || n_tokens > 6000;
     cudaStream_t st = (cudaStream_t)stream;
     cudaLaunchConfig_t cfg = {};

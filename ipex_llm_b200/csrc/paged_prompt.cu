@@ -11,12 +11,13 @@
 // tensor memory.
 // Two tiles alternate: one's products run while the other is in its softmax.  The blocks share the key tiles of all units equally (paged.h).
 // P enters P . V as two 16-bit values, the second with what the rounding of the first left, and both multiply V: only the result is rounded
-// (fp16's range: P_LIFT in paged.h).  With one value (182 / 155 us a chunk, 687 / 545 the long prompt below) an output added up to sqrt(2) of the error that rounding the output alone leaves.
-// What bounds it: the softmax (two loads of S, 128 exponentials a thread, both parts' stores) with the products between two steps of a tile (3072 clocks of
-// MMAs a step of 256 rows and 128 keys, of which one tile's run beside the other's softmax) and the waits of the roles for one another.  8 prompts of 200
-// to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one of 8000, 32 heads, fp16: 687 us, 763 TFLOP/s; 512 tokens behind
-// 16000 keys, 32 on 8, bf16: 182 us, 748 TFLOP/s.
-// Before P had two parts, with TMA / without: 223 / 234, 546 / 630, 155 / 246 us.
+// (fp16's range: P_LIFT in paged.h).  With one value an output added up to sqrt(2) of the error that rounding the output alone leaves; one value / two: the 8
+// prompts below 223 / 268 us, the long one 545 / 690, the chunk 155 / 181.
+// What bounds it: a tile's chain in a step of 256 rows and 128 keys, 5200 clocks: its softmax 3400 (maximum 570, exponentials and both parts of P 2800, while the
+// other tile's warps are in theirs), P V of the last 64 keys 790, Q K of the next ones 790; 32768 exponentials need 2048 clocks of a step, the MMAs of both
+// tiles 3072 (tensor pipe 48 %, issue slots 46 %).  8 prompts of 200 to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one
+// of 8000, 32 heads, fp16: 690 us, 760 TFLOP/s (820 us in a long loop, under the power cap); 512 tokens behind 16000 keys, 32 on 8, bf16: 181 us, 752 TFLOP/s,
+// over e5m2 pages 272 us.  With TMA / without: 269 / 291, 698 / 746, 181 / 261 us.
 #include <string.h>
 #include "paged.h"
 #include "tc_common.cuh"
@@ -51,16 +52,6 @@ __device__ __forceinline__ void tmem_ld32x(uint32_t taddr, float* v) {
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32x(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 __device__ __forceinline__ void tmem_ld16x(uint32_t taddr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -126,11 +117,12 @@ __device__ __forceinline__ int64_t floor_sum128(uint32_t n, uint32_t a, uint32_t
     return s;
 }
 // What a unit costs beside its key tiles (queries, result, a pipeline that drains), in tiles: shares are taken of places, PR_EXTRA of them in
-// front of a unit's tiles, so that blocks with many short prompts are not the last.  0 / 1 / 2 / 3: the 8 prompts 351 / 294 / 274 / 274 us (before the softmax
-// had its loops; since then 268 with 1, and 2 / 3 / 4: 226 / 218 / 222), 40 requests with chunks to 300 and tokens over e5m2 pages 103 / 107 / 109
+// front of a unit's tiles, so that blocks with many short prompts are not the last.  0 / 1 / 2 / 3: the 8 prompts above 377 / 291 / 269 / 270 us, 7
+// of 17 to 300 tokens 26.4 / 19.4 / 18.6 / 18.0, 40 requests with chunks to 300 and tokens over e5m2 pages 129 / 111 / 113 / 118
 constexpr int PR_EXTRA = 2;
 // A unit of up to so many key tiles is never split: it is the block's in whose share it begins.  A part costs a store and a load of its 32-bit
-// sums (128 KB a unit) and its merge, more than such a unit is worth: 7 prompts of 17 to 300 tokens 21.5 us with 0, 19.4 with 2 and with 4
+// sums (128 KB a unit) and its merge, more than such a unit is worth.  0 / 2 / 4 / 8: 7 prompts of 17 to 300 tokens 22.1 / 18.6 / 18.6 / 18.7 us, 8
+// of 400 60 / 61 / 54 / 54, 20 of 500 143 / 144 / 131 / 131, one of 2000 with 4 heads on one 29.7 / 29.8 / 32.0 / 40.8, the 40 requests 113 / 113 / 113 / 121
 constexpr int PR_WHOLE = 4;
 struct Units {
     int n, units, tpu, causal, off, len;                      // new tokens, units, tokens of a unit; keys before the first new token
@@ -197,7 +189,8 @@ struct PromptAt {
         return keys <= 0 ? 0 : (keys - 1) / PR_KEYS + 1;
     }
 };
-// places that a block takes at least.  1 / 3 / 6: a prompt of 2000 tokens, 4 heads on one 31.0 / 28.8 / - us, seven of 17 to 300 tokens 17.6 / 17.5 / 24
+// places that a block takes at least.  1 / 3 / 6: a prompt of 2000 tokens, 4 heads on one 33.2 / 32.0 / 34.3 us, seven of 17 to 300 tokens 18.7 / 18.6 / 26.6, one of
+// 100, 8 heads, 13.3 / 12.6 / 18.3
 constexpr int PR_LEAST = 3;
 
 // the whole block: where place `pick` of all lies (`place` of its unit); `all` = places of all units
@@ -378,7 +371,7 @@ __global__ void __launch_bounds__((Prompt<DP, E5M2>::kWarps * 32), 1) paged_prom
                     if (!mbar_wait_lim(s_full(t), steps & 1, A.waits)) goto done;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     // 64 scores in registers at a time, by loops that are not unrolled: the roles share an instruction cache, and this one in a
-                    // row, three loads instead of four, took 640 us where this takes 553 (8000 tokens, 32 heads)
+                    // row, three loads instead of four, took 640 us where they took 553 (8000 tokens, 32 heads, P of one part)
                     const bool plain = j < plain_end / PR_KEYS;
                     const int left = n_vis - j * PR_KEYS;
                     float x[64], m0, m1, m2, m3;

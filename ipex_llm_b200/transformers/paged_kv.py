@@ -123,7 +123,8 @@ def paged_step(query_lens, context_lens, block_table, free_pages, free_count, pa
 def paged_release(done, block_table, free_pages, free_count, held=None, page_size=None):
     """Requests that are done give their pages back: rows of ``block_table`` with ``done`` (bool or uint8 [R]) set go onto the stack
     ``free_pages`` / ``free_count`` and become -1, in place.  With ``held`` (int32 [R]: tokens that they keep) and the ``page_size`` they give back
-    only what lies behind those: a step that found too few pages is taken back so, and tokens that a request drops."""
+    only what lies behind those: a step that found too few pages is taken back so, and tokens that a request drops.  A page that several rows name
+    would go back once for each."""
     dev = _device(done, block_table, free_pages, free_count)
     invalidInputError(done.dtype in (torch.bool, torch.uint8) and done.dim() == 1 and done.is_contiguous() and done.shape[0] > 0, "done must be a contiguous bool [R]")
     _table(block_table)
@@ -144,7 +145,7 @@ def paged_release(done, block_table, free_pages, free_count, held=None, page_siz
 
 def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache):
     """Rotary embedding of the query and key heads of the merged projection's output ``qkv`` [T, (n_heads + 2 n_kv_heads) * head_dim], in
-    place, and the write of keys and values into their ``slots`` (int64 [T]; -1: not written).  ``cos`` / ``sin`` [positions, rotary width]
+    place, and the write of keys and values into their ``slots`` (int64 [T], none twice; -1: not written).  ``cos`` / ``sin`` [positions, rotary width]
     in the rotate_half layout, indexed by ``positions`` (int64 [T]; beyond the tables: their last row); a rotary width below head_dim
     leaves the other elements; None: no rotation.  e5m2 caches keep the rounded activations' nearest value, saturating."""
     if _native("paged_append", qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache) is not None:
