@@ -15,7 +15,7 @@
 // prompts below 223 / 268 us, the long one 545 / 690, the chunk 155 / 181.
 // What bounds it: a tile's chain in a step of 256 rows and 128 keys, 5200 clocks: its softmax 3400 (maximum 570, exponentials and both parts of P 2800, while the
 // other tile's warps are in theirs), P V of the last 64 keys 790, Q K of the next ones 790; 32768 exponentials need 2048 clocks of a step, the MMAs of both
-// tiles 3072 (tensor pipe 48 %, issue slots 46 %).  8 prompts of 200 to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one
+// tiles 6 x 512 (tensor pipe 48 %, issue slots 46 %).  8 prompts of 200 to 4000 tokens, 32 heads on 8, bf16: 268 us, 564 TFLOP/s, each product counted once; one
 // of 8000, 32 heads, fp16: 690 us, 760 TFLOP/s (820 us in a long loop, under the power cap); 512 tokens behind 16000 keys, 32 on 8, bf16: 181 us, 752 TFLOP/s,
 // over e5m2 pages 272 us.  With TMA / without: 269 / 291, 698 / 746, 181 / 261 us.
 #include <string.h>
