@@ -325,6 +325,58 @@ int lowbit_sdp_packed_cuda(const void* d_q, int dtype, const int64_t* q_strides,
                            int causal, int64_t max_seqlen, void* d_out, const int64_t* out_strides, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* The same in front of the rotation of layers that normalise their query and key heads: x w / sqrt(mean x^2 + eps), w [D] of w_dtype, in 32 bits up to
+ * the rotated result, one rounding.  Caches of NULL: only d_qkv is written. */
+int lowbit_paged_norm_rope_append_cuda(void* d_qkv, int dtype, int64_t token_stride, int64_t T, int Hq, int Hkv, int D, int rotary_dim,
+                                       const void* d_q_weight, const void* d_k_weight, int w_dtype, float eps, const void* d_cos, const void* d_sin,
+                                       int cs_dtype, int64_t cs_row_stride, int64_t n_positions, const int64_t* d_positions, const int64_t* d_slots,
+                                       void* d_k_cache, const int64_t* k_strides, void* d_v_cache, const int64_t* v_strides, int cache_dtype,
+                                       int n_pages, int page_size, void* stream);
+
+/* Pages that several rows of the block table name.  d_shared [n_pages]: the rows beyond the first that name a page.
+ * fork: row children[i] becomes a fork of row parents[i], which holds lens[parents[i]] tokens: it names the parent's full pages, and a page off the stack
+ * (dst[i]; -1: none needed or none there) stands for those behind them, to be filled from src[i].  lens of the child is written.  A child is no parent.
+ * release: as lowbit_paged_release_cuda (d_held NULL) or lowbit_paged_release_behind_cuda, a page going back where no row is left that names it.
+ * compact: the highest page that the table names to the lowest one on the stack, as long as that lies in front; *_out: table [R][width] without padding,
+ * stack (lowest page last, -1 behind the count), count, shared (NULL with d_shared NULL), and the moves, -1 behind them, [n_pages] each.
+ * copy: page src[i] to page dst[i] of every cache, whose pages are page_bytes in one run, page_stride_bytes apart; numbers outside the cache: left out.
+ * `caches` is read by the call.  workspace: 4-byte aligned. */
+int lowbit_paged_fork_cuda(const int32_t* d_parents, const int32_t* d_children, int F, int32_t* d_lens, int32_t* d_table, int64_t table_stride,
+                           int R, int width, const int32_t* d_free_pages, int n_pages, const int32_t* d_free_count, int32_t* d_free_left,
+                           int32_t* d_shared, int page_size, int32_t* d_src, int32_t* d_dst, int32_t* d_missing, void* stream);
+size_t lowbit_paged_share_release_workspace_size(int n_pages, int R);
+int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int32_t* d_held, int page_size, int R, int32_t* d_table, int64_t table_stride,
+                                    int width, int32_t* d_free_pages, int n_pages, int32_t* d_free_count, int32_t* d_shared, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+size_t lowbit_paged_compact_workspace_size(int n_pages);
+int lowbit_paged_compact_cuda(const int32_t* d_table, int64_t table_stride, int R, int width, const int32_t* d_free_pages, int n_pages,
+                              const int32_t* d_free_count, const int32_t* d_shared, int32_t* d_table_out, int32_t* d_free_pages_out,
+                              int32_t* d_free_count_out, int32_t* d_shared_out, int32_t* d_src, int32_t* d_dst, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int lowbit_paged_copy_cuda(const int32_t* d_src, const int32_t* d_dst, int n, void* const* caches, int n_caches, int n_pages,
+                           int64_t page_stride_bytes, int64_t page_bytes, void* stream);
+
+/* Low-rank adapters of many requests beside a projection: out[t] += scales[l] (x[t] A_l^T) B_l^T with l = ids[r] of the request r that row t belongs to
+ * (rows cu[r] .. cu[r + 1]); an id outside [0, adapters), and rows of nobody: left as they are.  x [T][K], out [T][N] with N the sum of `splits`;
+ * A [adapters][n_splits][rank][K], B [adapters][N][rank], each adapter's in one run, strides in elements between adapters; columns of split s take the
+ * product with A's part s.  dtype fp16 or bf16; rank a multiple of 8 up to 256, K and the splits multiples of 8; pointers and strides on 16 bytes.
+ * `splits` is read by the call.  The product with A is kept in 32 bits, only out is rounded.  Two launches.  workspace: 16-byte aligned. */
+size_t lowbit_lora_workspace_size(int64_t T, int K, int rows, int R, int adapters);      /* rows = n_splits x rank */
+int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b,
+                         int64_t b_stride, int rank, const float* d_scales, int adapters, const int32_t* d_ids, const int32_t* d_cu_seqlens, int R,
+                         const int* splits, int n_splits, void* d_out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of tokens [rows] under softmax(logits / temperature), logits [rows][V] of dtype; the rows' entropy; the top_k (at most 32) largest
+ * logits in order, of equal ones the lower index first, with their log probabilities [rows][top_k].  A token outside the vocabulary: 0.  d_stats
+ * [rows][4] fp32, 16-byte aligned, or NULL: what the gradient needs.
+ * grad: the logits' gradient from those of the outputs (NULL: zero), rounded once to their type; d_grad is not d_logits. */
+int lowbit_token_logprobs_cuda(const void* d_logits, int dtype, int64_t row_stride, int64_t rows, int64_t V, const int64_t* d_tokens,
+                               float temperature, int top_k, float* d_logprobs, float* d_entropy, int64_t* d_top_ids, float* d_top_logprobs,
+                               float* d_stats, void* stream);
+int lowbit_token_logprobs_grad_cuda(const void* d_logits, int dtype, int64_t row_stride, int64_t rows, int64_t V, const int64_t* d_tokens,
+                                    float temperature, int top_k, const int64_t* d_top_ids, const float* d_g_logprobs, const float* d_g_entropy,
+                                    const float* d_g_top, const float* d_stats, void* d_grad, int64_t grad_row_stride, void* stream);
+
 /* canonical <-> device layout on device buffers (same byte size, src != dst).
  * to_device != 0: canonical -> tiled ; 0: tiled -> canonical. */
 int lowbit_relayout_cuda(const void* d_src, void* d_dst, int64_t rows, int64_t k, int qtype,

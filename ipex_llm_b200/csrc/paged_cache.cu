@@ -293,6 +293,160 @@ template <typename T, bool E5M2> void append_vec(const AppendArgs& A, unsigned g
     else launch_behind(paged_append_vec_kernel<T, E5M2, __nv_bfloat16>, dim3(grid), 256, 0, st, on, A);
 }
 
+// ------------------------------------------------------------------ the same with a norm of every query and key head in front of the rotation
+//   y = x w / sqrt(mean x^2 + eps), then y cos + rot(y) sin: one rounding, of the result
+struct NormArgs { AppendArgs a; const void *qw, *kw; int w_dtype; float eps; };
+
+// a head by a warp: whatever lies on no 16 bytes
+template <typename T, bool E5M2>
+__global__ void __launch_bounds__(256) paged_norm_append_kernel(const NormArgs N) {
+    const AppendArgs& A = N.a;
+    const int half = A.R / 2, per = half + (A.D - A.R), heads = A.Hq + 2 * A.Hkv, lane = threadIdx.x & 31;
+    const int64_t total = A.T * heads;
+    for (int64_t idx = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; idx < total; idx += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+        const int h = (int)(idx % heads);
+        const int64_t t = idx / heads;
+        T* const row = (T*)A.qkv + t * A.st + (int64_t)h * A.D;
+        const bool keeps = h < A.Hq + A.Hkv;                   // queries and keys
+        float inv = 1.0f;
+        if (keeps) {
+            float sum = 0.0f;
+            for (int e = lane; e < A.D; e += 32) { const float x = Act<T>::get(row[e]); sum = fmaf(x, x, sum); }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            inv = rsqrtf(sum / A.D + N.eps);
+        }
+        const void* const w = h < A.Hq ? N.qw : N.kw;
+        int64_t p = A.R > 0 ? A.positions[t] : 0;
+        p = p < 0 ? 0 : p < A.n_pos ? p : A.n_pos - 1;
+        const int64_t slot = A.kc && h >= A.Hq ? A.slots[t] : -1;
+        const bool kept = slot >= 0 && slot < A.n_slots;
+        const int hk = h - A.Hq - (keeps ? 0 : A.Hkv);
+        const int64_t pg = kept ? slot / A.page_size : 0, in = kept ? slot % A.page_size : 0;
+        const int64_t at = keeps ? pg * A.k_sp + in * A.k_ss + hk * A.k_sh : pg * A.v_sp + in * A.v_ss + hk * A.v_sh;
+        for (int i = lane; i < per; i += 32) {
+            const int e0 = i < half ? i : A.R + i - half, e1 = i < half ? i + half : e0;
+            T x0 = row[e0], x1 = row[e1];
+            if (keeps) {
+                const float a = Act<T>::get(x0) * inv * table_at(w, N.w_dtype, e0), b = Act<T>::get(x1) * inv * table_at(w, N.w_dtype, e1);
+                const float c = i < half ? table_at(A.cos, A.cs_dtype, p * A.cs_row + i) : 1.0f, s = i < half ? table_at(A.sin, A.cs_dtype, p * A.cs_row + i) : 0.0f;
+                x0 = Act<T>::put(i < half ? fmaf(a, c, -b * s) : a);
+                x1 = Act<T>::put(i < half ? fmaf(b, c, a * s) : a);
+                row[e0] = x0;
+                row[e1] = x1;
+            }
+            if (!kept) continue;
+            if (E5M2) {
+                uint8_t* const d = (keeps ? A.kc : A.vc) + at;
+                d[e0] = to_e5m2(Act<T>::get(x0));
+                d[e1] = to_e5m2(Act<T>::get(x1));
+            } else {
+                T* const d = (T*)(keeps ? A.kc : A.vc) + at;
+                d[e0] = x0;
+                d[e1] = x1;
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// Rows on 16 bytes: 16 elements a thread as in paged_append_vec_kernel, LANES (a power of two from D / 16 on) threads a head, whose squares meet by
+// shuffles.
+template <typename T, bool E5M2, typename C, int LANES>
+__global__ void __launch_bounds__(256) paged_norm_append_vec_kernel(const NormArgs N) {
+    const AppendArgs& A = N.a;
+    extern __shared__ __align__(16) float norm_w[];            // [2][D]
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (int i = threadIdx.x; i < 2 * A.D; i += 256) norm_w[i] = table_at(i < A.D ? N.qw : N.kw, N.w_dtype, i < A.D ? i : i - A.D);
+    __syncthreads();
+    const uint32_t heads = (uint32_t)(A.Hq + 2 * A.Hkv), per = heads * LANES, total = (uint32_t)A.T * per;
+    const int half = A.R / 2;
+    const float over = 1.0f / A.D;
+    for (uint32_t base = blockIdx.x * 256u; base < total; base += gridDim.x * 256u) {
+        const uint32_t idx = base + threadIdx.x, t = idx / per, in = idx - t * per;
+        const int h = (int)(in / LANES), i = (int)(in % LANES) * 8;                            // 8 elements from i and, rotated, from i + half
+        const bool live = idx < total && 2 * i < A.D, turn = i < half, keeps = h < A.Hq + A.Hkv;
+        const int e0 = turn ? i : A.R + 2 * (i - half), e1 = turn ? i + half : e0 + 8;
+        T* const row = (T*)A.qkv + t * A.st + (int64_t)h * A.D;
+        T x0[8], x1[8];
+        if (live) {
+            *reinterpret_cast<uint4*>(x0) = *reinterpret_cast<const uint4*>(row + e0);
+            *reinterpret_cast<uint4*>(x1) = *reinterpret_cast<const uint4*>(row + e1);
+        }
+        float sum = 0.0f;
+        if (live && keeps) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float a = Act<T>::get(x0[e]), b = Act<T>::get(x1[e]);
+                sum = fmaf(a, a, sum);
+                sum = fmaf(b, b, sum);
+            }
+        }
+#pragma unroll
+        for (int d = LANES / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (!live) continue;
+        if (keeps) {
+            const float inv = rsqrtf(fmaf(sum, over, N.eps));
+            const float* const w = norm_w + (h < A.Hq ? 0 : A.D);
+            float a[8], b[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) { a[e] = Act<T>::get(x0[e]) * inv * w[e0 + e]; b[e] = Act<T>::get(x1[e]) * inv * w[e1 + e]; }
+            if (turn) {
+                int64_t p = A.positions[t];
+                p = p < 0 ? 0 : p < A.n_pos ? p : A.n_pos - 1;
+                C c[8], s[8];
+#pragma unroll
+                for (int z = 0; z < (int)sizeof(C) / 2; z++) {
+                    reinterpret_cast<uint4*>(c)[z] = reinterpret_cast<const uint4*>((const C*)A.cos + p * A.cs_row + i)[z];
+                    reinterpret_cast<uint4*>(s)[z] = reinterpret_cast<const uint4*>((const C*)A.sin + p * A.cs_row + i)[z];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float cf = (float)c[e], sf = (float)s[e];
+                    x0[e] = Act<T>::put(fmaf(a[e], cf, -b[e] * sf));
+                    x1[e] = Act<T>::put(fmaf(b[e], cf, a[e] * sf));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) { x0[e] = Act<T>::put(a[e]); x1[e] = Act<T>::put(b[e]); }
+            }
+            *reinterpret_cast<uint4*>(row + e0) = *reinterpret_cast<const uint4*>(x0);
+            *reinterpret_cast<uint4*>(row + e1) = *reinterpret_cast<const uint4*>(x1);
+        }
+        if (h < A.Hq || !A.kc) continue;
+        const int64_t slot = A.slots[t];
+        if (slot < 0 || slot >= A.n_slots) continue;
+        const int hk = h - A.Hq - (keeps ? 0 : A.Hkv);
+        const int64_t pg = slot < 1ll << 31 ? (int64_t)((uint32_t)slot / (uint32_t)A.page_size) : slot / A.page_size, rw = slot - pg * A.page_size;
+        const int64_t at = keeps ? pg * A.k_sp + rw * A.k_ss + hk * A.k_sh : pg * A.v_sp + rw * A.v_ss + hk * A.v_sh;
+        if (E5M2) {
+            uint8_t* const d = (keeps ? A.kc : A.vc) + at;
+            uint8_t q0[8], q1[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) { q0[e] = to_e5m2(Act<T>::get(x0[e])); q1[e] = to_e5m2(Act<T>::get(x1[e])); }
+            *reinterpret_cast<uint2*>(d + e0) = *reinterpret_cast<const uint2*>(q0);
+            *reinterpret_cast<uint2*>(d + e1) = *reinterpret_cast<const uint2*>(q1);
+        } else {
+            T* const d = (T*)(keeps ? A.kc : A.vc) + at;
+            *reinterpret_cast<uint4*>(d + e0) = *reinterpret_cast<const uint4*>(x0);
+            *reinterpret_cast<uint4*>(d + e1) = *reinterpret_cast<const uint4*>(x1);
+        }
+    }
+}
+template <typename T, bool E5M2, typename C> void norm_append_lanes(const NormArgs& N, int lanes, unsigned grid, cudaStream_t st) {
+    const bool on = launch_overlaps(st);
+    const size_t smem = 2 * N.a.D * sizeof(float);
+    if (lanes <= 4) launch_behind(paged_norm_append_vec_kernel<T, E5M2, C, 4>, dim3(grid), 256, smem, st, on, N);
+    else if (lanes == 8) launch_behind(paged_norm_append_vec_kernel<T, E5M2, C, 8>, dim3(grid), 256, smem, st, on, N);
+    else launch_behind(paged_norm_append_vec_kernel<T, E5M2, C, 16>, dim3(grid), 256, smem, st, on, N);
+}
+template <typename T, bool E5M2> void norm_append_vec(const NormArgs& N, int lanes, unsigned grid, cudaStream_t st) {
+    if (N.a.R == 0 || N.a.cs_dtype == DT_F32) norm_append_lanes<T, E5M2, float>(N, lanes, grid, st);
+    else if (N.a.cs_dtype == DT_F16) norm_append_lanes<T, E5M2, __half>(N, lanes, grid, st);
+    else norm_append_lanes<T, E5M2, __nv_bfloat16>(N, lanes, grid, st);
+}
+
 }  // namespace
 }  // namespace lowbit
 
@@ -395,6 +549,57 @@ extern "C" int lowbit_paged_rope_append_cuda(void* d_qkv, int dtype, int64_t tok
     } else {
         if (cache_dtype == CACHE_E5M2) paged_append_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(A);
         else paged_append_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(A);
+    }
+    note_launch();
+    return check_launch();
+}
+
+extern "C" int lowbit_paged_norm_rope_append_cuda(void* d_qkv, int dtype, int64_t token_stride, int64_t T, int Hq, int Hkv, int D, int rotary_dim,
+                                                  const void* d_q_weight, const void* d_k_weight, int w_dtype, float eps, const void* d_cos, const void* d_sin, int cs_dtype,
+                                                  int64_t cs_row_stride, int64_t n_positions, const int64_t* d_positions, const int64_t* d_slots, void* d_k_cache,
+                                                  const int64_t* k_strides, void* d_v_cache, const int64_t* v_strides, int cache_dtype, int n_pages, int page_size,
+                                                  void* stream) {
+    reset_launch_count();
+    const bool cached = d_k_cache != nullptr;
+    if (!d_qkv || !d_q_weight || !d_k_weight || w_dtype < 0 || w_dtype > 2 || !(eps >= 0.0f) || (dtype != DT_F16 && dtype != DT_BF16) || T < 0 || Hq < 0 || Hkv < 0 || Hq + Hkv <= 0 || D <= 0 ||
+        rotary_dim < 0 || rotary_dim > D || (rotary_dim & 1) ||
+        (rotary_dim > 0 && (!d_cos || !d_sin || !d_positions || cs_dtype < 0 || cs_dtype > 2 || cs_row_stride < rotary_dim / 2 || n_positions <= 0)) ||
+        token_stride < (int64_t)(Hq + 2 * Hkv) * D || cached != (d_v_cache != nullptr) ||
+        (cached && (!d_slots || !k_strides || !v_strides || (cache_dtype != dtype && cache_dtype != CACHE_E5M2) || Hkv <= 0 || n_pages <= 0 || page_size <= 0))) {
+        set_error(LB_ERR_ARG, "lowbit_paged_norm_rope_append_cuda: bad argument (T %lld, Hq %d, Hkv %d, D %d, rotary %d, dtype %d, cache dtype %d)", (long long)T, Hq,
+                  Hkv, D, rotary_dim, dtype, cache_dtype);
+        return LB_ERR_ARG;
+    }
+    if (T == 0) return LB_OK;
+    const int64_t none[3] = {0, 0, 0};
+    if (!cached) { k_strides = v_strides = none; n_pages = page_size = 1; cache_dtype = dtype; }
+    const NormArgs N = {{d_qkv, token_stride, T, Hq, Hkv, D, rotary_dim, d_cos, d_sin, cs_dtype, cs_row_stride, n_positions, d_positions, d_slots,
+                         (uint8_t*)d_k_cache, (uint8_t*)d_v_cache, k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2],
+                         (int64_t)n_pages * page_size, page_size}, d_q_weight, d_k_weight, w_dtype, eps};
+    cudaStream_t st = (cudaStream_t)stream;
+    int lanes = 4;
+    while (lanes * 16 < D) lanes *= 2;
+    const int64_t threads = T * (Hq + 2 * Hkv) * lanes, table = rotary_dim == 0 ? 0 : cs_dtype == DT_F32 ? 3 : 7;
+    const bool e5m2 = cache_dtype == CACHE_E5M2;
+    if (D % 16 == 0 && D <= 256 && rotary_dim % 16 == 0 && threads < 1ll << 31 && !((uintptr_t)d_qkv & 15) && !(token_stride & 7) &&
+        !(((uintptr_t)d_k_cache | (uintptr_t)d_v_cache) & (e5m2 ? 7 : 15)) &&
+        !((k_strides[0] | k_strides[1] | k_strides[2] | v_strides[0] | v_strides[1] | v_strides[2]) & 7) &&
+        (rotary_dim == 0 || (!(((uintptr_t)d_cos | (uintptr_t)d_sin) & 15) && !(cs_row_stride & table)))) {
+        const int64_t want = (threads + 255) / 256, most = (int64_t)sm_count() * 5;
+        const unsigned grid = (unsigned)(want < most ? want : most);
+        if (dtype == DT_F16) e5m2 ? norm_append_vec<__half, true>(N, lanes, grid, st) : norm_append_vec<__half, false>(N, lanes, grid, st);
+        else e5m2 ? norm_append_vec<__nv_bfloat16, true>(N, lanes, grid, st) : norm_append_vec<__nv_bfloat16, false>(N, lanes, grid, st);
+        note_launch();
+        return check_launch();
+    }
+    const int64_t want = (T * (Hq + 2 * Hkv) + 7) / 8, most = (int64_t)sm_count() * 8;
+    const dim3 grid((unsigned)(want < most ? want : most));
+    if (dtype == DT_F16) {
+        if (e5m2) paged_norm_append_kernel<__half, true><<<grid, 256, 0, st>>>(N);
+        else paged_norm_append_kernel<__half, false><<<grid, 256, 0, st>>>(N);
+    } else {
+        if (e5m2) paged_norm_append_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(N);
+        else paged_norm_append_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(N);
     }
     note_launch();
     return check_launch();

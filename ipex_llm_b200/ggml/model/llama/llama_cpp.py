@@ -746,3 +746,122 @@ def lowbit_sdp_packed(q, k, v, cu_seqlens, scale, causal, max_seqlen, out, works
     _check(_lib.lowbit_sdp_packed_cuda(q.data_ptr(), _DT_OF[q.dtype], _strides(q, 2), T, k.data_ptr(), _strides(k, 2), v.data_ptr(), _strides(v, 2),
                                        cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, float(scale), int(bool(causal)), int(max_seqlen),
                                        out.data_ptr(), _strides(out, 2), workspace.data_ptr(), workspace.numel(), stream), "lowbit_sdp_packed_cuda")
+
+
+_lib.lowbit_paged_norm_rope_append_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4 + \
+    [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _I64P, ctypes.c_void_p, _I64P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+_lib.lowbit_paged_norm_rope_append_cuda.restype = ctypes.c_int
+
+
+def lowbit_paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary_dim, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache, stream):
+    """as lowbit_paged_rope_append with the norms' weights [D] in front; without caches (None) only qkv is written"""
+    cached = k_cache is not None
+    _check(_lib.lowbit_paged_norm_rope_append_cuda(
+        qkv.data_ptr(), _DT_OF[qkv.dtype], qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1], qkv.shape[0], n_heads, n_kv_heads, head_dim, rotary_dim,
+        q_weight.data_ptr(), k_weight.data_ptr(), _DT_OF[q_weight.dtype], float(eps), cos.data_ptr() if rotary_dim else None, sin.data_ptr() if rotary_dim else None,
+        _DT_OF[cos.dtype] if rotary_dim else 0, cos.stride(0) if rotary_dim else 0, cos.shape[0] if rotary_dim else 0, positions.data_ptr() if rotary_dim else None,
+        slots.data_ptr() if cached else None, k_cache.data_ptr() if cached else None, _strides(k_cache, 3) if cached else None,
+        v_cache.data_ptr() if cached else None, _strides(v_cache, 3) if cached else None, _cache_dtype(k_cache) if cached else 0,
+        k_cache.shape[0] if cached else 0, k_cache.shape[1] if cached else 0, stream), "lowbit_paged_norm_rope_append_cuda")
+
+
+# ---------------------------------------------------------------- pages that several rows share
+_lib.lowbit_paged_fork_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+                                        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 4
+_lib.lowbit_paged_fork_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_share_release_workspace_size.argtypes = [ctypes.c_int, ctypes.c_int]
+_lib.lowbit_paged_share_release_workspace_size.restype = ctypes.c_size_t
+_lib.lowbit_paged_share_release_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                                 ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+_lib.lowbit_paged_share_release_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_compact_workspace_size.argtypes = [ctypes.c_int]
+_lib.lowbit_paged_compact_workspace_size.restype = ctypes.c_size_t
+_lib.lowbit_paged_compact_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 9 + \
+    [ctypes.c_size_t, ctypes.c_void_p]
+_lib.lowbit_paged_compact_cuda.restype = ctypes.c_int
+_lib.lowbit_paged_copy_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
+                                        ctypes.c_void_p]
+_lib.lowbit_paged_copy_cuda.restype = ctypes.c_int
+
+
+def lowbit_paged_fork(parents, children, lens, table, free_pages, free_count, free_left, shared, page_size, src, dst, missing, stream):
+    _check(_lib.lowbit_paged_fork_cuda(parents.data_ptr(), children.data_ptr(), parents.shape[0], lens.data_ptr(), table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+                                       free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), free_left.data_ptr(), shared.data_ptr(), int(page_size), src.data_ptr(),
+                                       dst.data_ptr(), missing.data_ptr(), stream), "lowbit_paged_fork_cuda")
+
+
+def lowbit_paged_share_release_workspace_size(n_pages, rows):
+    return _lib.lowbit_paged_share_release_workspace_size(n_pages, rows)
+
+
+def lowbit_paged_share_release(done, held, page_size, table, free_pages, free_count, shared, workspace, stream):
+    _check(_lib.lowbit_paged_share_release_cuda(done.data_ptr(), held.data_ptr() if held is not None else None, int(page_size or 1), table.shape[0], table.data_ptr(),
+                                                table.stride(0), table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), shared.data_ptr(),
+                                                workspace.data_ptr(), workspace.numel(), stream), "lowbit_paged_share_release_cuda")
+
+
+def lowbit_paged_compact_workspace_size(n_pages):
+    return _lib.lowbit_paged_compact_workspace_size(n_pages)
+
+
+def lowbit_paged_compact(table, free_pages, free_count, shared, table_out, free_pages_out, free_count_out, shared_out, src, dst, workspace, stream):
+    _check(_lib.lowbit_paged_compact_cuda(table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
+                                          shared.data_ptr() if shared is not None else None, table_out.data_ptr(), free_pages_out.data_ptr(), free_count_out.data_ptr(),
+                                          shared_out.data_ptr() if shared is not None else None, src.data_ptr(), dst.data_ptr(), workspace.data_ptr(), workspace.numel(), stream),
+           "lowbit_paged_compact_cuda")
+
+
+def lowbit_paged_copy(src, dst, caches, n_pages, page_stride_bytes, page_bytes, stream):
+    """caches: addresses, of one layout"""
+    _check(_lib.lowbit_paged_copy_cuda(src.data_ptr(), dst.data_ptr(), src.shape[0], (ctypes.c_void_p * len(caches))(*caches), len(caches), n_pages, page_stride_bytes, page_bytes,
+                                       stream), "lowbit_paged_copy_cuda")
+
+
+# ---------------------------------------------------------------- low-rank adapters of many requests
+_lib.lowbit_lora_workspace_size.argtypes = [ctypes.c_int64] + [ctypes.c_int] * 4
+_lib.lowbit_lora_workspace_size.restype = ctypes.c_size_t
+_lib.lowbit_lora_add_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                      ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+                                      ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+_lib.lowbit_lora_add_cuda.restype = ctypes.c_int
+
+
+def lowbit_lora_workspace_size(tokens, k, rows, requests, adapters):
+    return _lib.lowbit_lora_workspace_size(tokens, k, rows, requests, adapters)
+
+
+def lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, workspace, stream):
+    """x [T, K], out [T, N], a [L, S, R, K], b [L, N, R], scales fp32 [L], adapter_ids [requests], cu_seqlens [requests + 1]"""
+    T, K = x.shape
+    _check(_lib.lowbit_lora_add_cuda(x.data_ptr(), x.stride(0) if T > 1 else K, _DT_OF[x.dtype], T, K, a.data_ptr(), a.stride(0) if a.shape[0] > 1 else a[0].numel(), b.data_ptr(),
+                                     b.stride(0) if b.shape[0] > 1 else b[0].numel(), b.shape[2], scales.data_ptr(), b.shape[0], adapter_ids.data_ptr(), cu_seqlens.data_ptr(),
+                                     adapter_ids.shape[0], (ctypes.c_int * len(splits))(*splits), len(splits), out.data_ptr(), out.stride(0) if T > 1 else out.shape[1],
+                                     workspace.data_ptr(), workspace.numel(), stream), "lowbit_lora_add_cuda")
+
+
+# ---------------------------------------------------------------- log probabilities of tokens
+_lib.lowbit_token_logprobs_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_int] + \
+    [ctypes.c_void_p] * 6
+_lib.lowbit_token_logprobs_cuda.restype = ctypes.c_int
+_lib.lowbit_token_logprobs_grad_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_int] + \
+    [ctypes.c_void_p] * 6 + [ctypes.c_int64, ctypes.c_void_p]
+_lib.lowbit_token_logprobs_grad_cuda.restype = ctypes.c_int
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def lowbit_token_logprobs(logits, tokens, temperature, top_k, logprobs, entropy, top_ids, top_logprobs, stats, stream):
+    """logits [rows, V]; tokens int64 [rows]; stats fp32 [rows, 4] or None"""
+    rows, V = logits.shape
+    _check(_lib.lowbit_token_logprobs_cuda(logits.data_ptr(), _DT_OF[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, tokens.data_ptr(), float(temperature), int(top_k),
+                                           logprobs.data_ptr(), entropy.data_ptr(), _ptr(top_ids), _ptr(top_logprobs), _ptr(stats), stream), "lowbit_token_logprobs_cuda")
+
+
+def lowbit_token_logprobs_grad(logits, tokens, temperature, top_k, top_ids, g_logprobs, g_entropy, g_top, stats, grad, stream):
+    rows, V = logits.shape
+    _check(_lib.lowbit_token_logprobs_grad_cuda(logits.data_ptr(), _DT_OF[logits.dtype], logits.stride(0) if rows > 1 else V, rows, V, tokens.data_ptr(), float(temperature),
+                                                int(top_k), _ptr(top_ids), _ptr(g_logprobs), _ptr(g_entropy), _ptr(g_top), stats.data_ptr(),
+                                                grad.data_ptr(), grad.stride(0) if rows > 1 else V, stream), "lowbit_token_logprobs_grad_cuda")

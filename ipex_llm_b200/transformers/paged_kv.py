@@ -12,7 +12,7 @@ whole prompt -- and ``paged_release`` for requests that are done.  None of them 
 gradient, or carry a tangent of forward mode, are refused.
 """
 import math
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -120,11 +120,12 @@ def paged_step(query_lens, context_lens, block_table, free_pages, free_count, pa
     return out
 
 
-def paged_release(done, block_table, free_pages, free_count, held=None, page_size=None):
+def paged_release(done, block_table, free_pages, free_count, held=None, page_size=None, shared=None):
     """Requests that are done give their pages back: rows of ``block_table`` with ``done`` (bool or uint8 [R]) set go onto the stack
     ``free_pages`` / ``free_count`` and become -1, in place.  With ``held`` (int32 [R]: tokens that they keep) and the ``page_size`` they give back
     only what lies behind those: a step that found too few pages is taken back so, and tokens that a request drops.  A page that several rows name
-    would go back once for each."""
+    would go back once for each, but for ``shared`` (``paged_fork``): a page that rows beside these name stays theirs, with its count in ``shared``
+    lowered, and one that is given up by all goes back once, in the order of the entries that name it first."""
     dev = _device(done, block_table, free_pages, free_count)
     invalidInputError(done.dtype in (torch.bool, torch.uint8) and done.dim() == 1 and done.is_contiguous() and done.shape[0] > 0, "done must be a contiguous bool [R]")
     _table(block_table)
@@ -136,11 +137,130 @@ def paged_release(done, block_table, free_pages, free_count, held=None, page_siz
         _device(done, held)
         _ints(held, done.shape[0], "held")
         invalidInputError(int(page_size) > 0, "page_size must be positive")
+    if shared is not None:
+        _device(done, shared)
+        _ints(shared, free_pages.shape[0], "shared")
+        with torch.cuda.device(dev):
+            ws = torch.empty(ggml.lowbit_paged_share_release_workspace_size(shared.shape[0], done.shape[0]), dtype=torch.uint8, device=dev)
+            ggml.lowbit_paged_share_release(done, held, page_size, block_table, free_pages, free_count, shared, ws, _stream(dev))
+        return
     with torch.cuda.device(dev):
         if held is None:
             ggml.lowbit_paged_release(done, block_table, free_pages, free_count, _stream(dev))
         else:
             ggml.lowbit_paged_release_behind(done, held, block_table, page_size, free_pages, free_count, _stream(dev))
+
+
+class PagedFork(NamedTuple):
+    """what ``paged_fork`` has handed out, all on the device"""
+    src: torch.Tensor                 # int32 [forks]: the parent's last page where it is not full, else -1
+    dst: torch.Tensor                 # int32 [forks]: the child's own page for those tokens, -1 where it needs none or none was to be had
+    free_count: torch.Tensor          # int32 [1]: free pages left
+    missing: torch.Tensor             # int32 [1]: pages that were not to be had
+
+
+class PagedCompact(NamedTuple):
+    """the bookkeeping of a cache whose pages in use lie in front, and the copies that make it true"""
+    block_table: torch.Tensor         # int32 [R, width]
+    free_pages: torch.Tensor          # int32 [pages]: the stack, its lowest page last (it comes off first), -1 behind the count
+    free_count: torch.Tensor          # int32 [1]
+    shared: Optional[torch.Tensor]    # int32 [pages]
+    src: torch.Tensor                 # int32 [pages]: page src[i] moves to dst[i]; -1 behind the last move
+    dst: torch.Tensor
+
+
+def paged_fork(parents, children, context_lens, block_table, free_pages, free_count, shared, page_size, free_left=None):
+    """Requests that go on from where others are: row ``children[i]`` of the table becomes a fork of row ``parents[i]`` (int32 [forks]; samples of a
+    prompt, the beams of a search), in one launch.
+
+    A child names its parent's full pages, each counted once more in ``shared`` (int32 [pages]: the rows beyond the first that name a page; zeros at first),
+    and gets a page of its own off the stack for the tokens behind them: ``paged_copy(src, dst, caches)`` of what comes back fills it, in all layers at
+    once.  So nobody writes to a page that others read.  ``context_lens`` (int32 [R]: tokens that every row holds) gets the children's, in place.  A parent may
+    have many children; a child's row must hold nothing (what it names is written over), come up once, and be no parent in the same call.
+    Pairs with a row outside the table, or of a row with itself, are left alone.
+
+    ``free_pages`` / ``free_count`` / ``free_left`` as in ``paged_step``.  Where ``missing`` is not 0 the last children lack that page: they are given back, with
+    ``shared``, before somebody forks again.  From now on rows go back by ``paged_release(..., shared=shared)``; a row that keeps part of its tokens (``held``)
+    must not be written to behind them while others name that page."""
+    F, R = parents.shape[0], block_table.shape[0]
+    dev = _device(parents, children, context_lens, block_table, free_pages, free_count, shared)
+    _ints(parents, F, "parents")
+    _ints(children, F, "children")
+    _table(block_table)
+    _ints(context_lens, R, "context_lens")
+    _ints(free_pages, free_pages.shape[0], "free_pages")
+    _ints(free_count, 1, "free_count")
+    _ints(shared, free_pages.shape[0], "shared")
+    page_size = int(page_size)
+    invalidInputError(page_size > 0 and free_pages.shape[0] > 0, "page_size and the number of pages must be positive")
+    if free_left is not None:
+        _device(free_count, free_left)
+        _ints(free_left, 1, "free_left")
+    out = torch.empty(2 * F + 2, dtype=torch.int32, device=dev)
+    got = PagedFork(out[:F], out[F:2 * F], out[2 * F:2 * F + 1] if free_left is None else free_left, out[2 * F + 1:])
+    with torch.cuda.device(dev):
+        if F == 0:
+            got.missing.zero_()
+            if got.free_count is not free_count:
+                got.free_count.copy_(free_count)
+            return got
+        ggml.lowbit_paged_fork(parents, children, context_lens, block_table, free_pages, free_count, got.free_count, shared, page_size, got.src, got.dst, got.missing, _stream(dev))
+    return got
+
+
+def _page_layout(cache):
+    """(pages, bytes from one page to the next, bytes of a page) of a cache whose pages are each one run of memory, whatever the order in it"""
+    invalidInputError(cache.dim() >= 2 and cache.numel() > 0 and cache.device.type == "cuda", "caches must be CUDA tensors [pages, ...]")
+    size = cache.element_size()
+    page = cache.numel() // cache.shape[0]
+    expect = 1
+    for n, st in sorted(((n, st) for n, st in zip(cache.shape[1:], cache.stride()[1:]) if n > 1), key=lambda d: d[1]):
+        invalidInputError(st == expect, "a page of a cache must be one run of memory")
+        expect *= n
+    invalidInputError(cache.shape[0] == 1 or cache.stride(0) >= page, "the pages of a cache overlap")
+    return cache.shape[0], max(cache.stride(0), page) * size, page * size
+
+
+def paged_copy(src, dst, caches):
+    """Page ``src[i]`` to page ``dst[i]`` (int32 [n]) of every cache in the list -- keys and values of all layers -- in one launch for up to 256 caches of one
+    layout.  Pairs with a number outside the cache (-1) are left out; no page may be a source and a target, or a target twice."""
+    caches = list(caches)
+    dev = _device(src, dst)
+    _ints(src, src.shape[0], "src")
+    _ints(dst, src.shape[0], "dst")
+    groups = {}
+    for c in caches:
+        _device(src, c)
+        groups.setdefault(_page_layout(c), []).append(c.data_ptr())
+    _no_grad(*caches)
+    if src.shape[0] == 0:
+        return
+    with torch.cuda.device(dev):
+        for layout, at in groups.items():
+            ggml.lowbit_paged_copy(src, dst, at, *layout, _stream(dev))
+
+
+def paged_compact(block_table, free_pages, free_count, shared=None):
+    """The pages in use moved to the front, as far as the pages on the stack allow: the table, the stack and ``shared`` as they are afterwards, and the list of
+    copies.  New tensors: what is passed in stays, so that ``paged_copy(src, dst, caches)`` can move the contents before anybody reads by the new
+    table.  The highest page in use moves to the lowest free one until no free page lies in front of a used one; pages that are neither in the table nor on the
+    stack stay where they are.  A page that several rows name moves once."""
+    dev = _device(block_table, free_pages, free_count)
+    _table(block_table)
+    _ints(free_pages, free_pages.shape[0], "free_pages")
+    _ints(free_count, 1, "free_count")
+    n = free_pages.shape[0]
+    invalidInputError(n > 0, "the number of pages must be positive")
+    if shared is not None:
+        _device(block_table, shared)
+        _ints(shared, n, "shared")
+    table = torch.empty(block_table.shape, dtype=torch.int32, device=dev)
+    out = torch.empty(4 * n + 1, dtype=torch.int32, device=dev)
+    got = PagedCompact(table, out[:n], out[4 * n:], None if shared is None else out[n:2 * n], out[2 * n:3 * n], out[3 * n:4 * n])
+    with torch.cuda.device(dev):
+        ws = torch.empty(ggml.lowbit_paged_compact_workspace_size(n), dtype=torch.uint8, device=dev)
+        ggml.lowbit_paged_compact(block_table, free_pages, free_count, shared, got.block_table, got.free_pages, got.free_count, got.shared, got.src, got.dst, ws, _stream(dev))
+    return got
 
 
 def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, slots, k_cache, v_cache):
@@ -171,6 +291,42 @@ def paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, cos, sin, positions, s
         return
     with torch.cuda.device(dev):
         ggml.lowbit_paged_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary, cos, sin, positions, slots, k_cache, v_cache, _stream(dev))
+
+
+def paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache):
+    """``paged_rope_append`` for layers that normalise their query and key heads: every head of ``qkv`` [T, (n_heads + 2 n_kv_heads) * head_dim] becomes
+    x w / sqrt(mean x^2 + eps), w = ``q_weight`` or ``k_weight`` [head_dim] (fp16, bf16 or fp32, both of one type), and is then rotated, in place; keys and
+    values go into their slots.  The norm and the rotation are in 32 bits with one rounding behind both.  ``cos`` / ``sin`` / ``positions`` / ``slots`` and the
+    caches as there; caches of None (another kind of cache): only ``qkv`` is written."""
+    _no_grad(qkv, q_weight, k_weight, cos, sin, k_cache, v_cache)
+    invalidInputError(qkv.dim() == 2 and qkv.dtype in _HALF and n_heads >= 0 and n_kv_heads >= 0 and n_heads + n_kv_heads > 0 and head_dim > 0
+                      and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and (qkv.stride(1) == 1 or qkv.numel() == 0),
+                      f"qkv must be a half-precision [T, {(n_heads + 2 * n_kv_heads) * head_dim}] with contiguous rows")
+    invalidInputError(qkv.shape[0] <= 1 or qkv.stride(0) >= qkv.shape[1], "the rows of qkv overlap")
+    T, rotary = qkv.shape[0], 0
+    dev = _device(qkv, q_weight, k_weight)
+    invalidInputError(q_weight.shape == (head_dim,) and k_weight.shape == (head_dim,) and q_weight.dtype == k_weight.dtype and q_weight.dtype in _HALF + (torch.float32,)
+                      and q_weight.is_contiguous() and k_weight.is_contiguous(), f"the norms' weights must be two contiguous [{head_dim}] of one type")
+    eps = float(eps)
+    invalidInputError(0 <= eps < math.inf, "eps must not be negative")
+    invalidInputError((k_cache is None) == (v_cache is None), "both caches or none")
+    if k_cache is not None:
+        _device(qkv, slots, k_cache, v_cache)
+        _ints(slots, T, "slots", torch.int64)
+        _caches(k_cache, v_cache, qkv.dtype, head_dim)
+        invalidInputError(k_cache.shape[2] == n_kv_heads, f"the cache has {k_cache.shape[2]} kv heads, the activations {n_kv_heads}")
+    invalidInputError((cos is None) == (sin is None), "cos and sin come together")
+    if cos is not None:
+        _device(qkv, cos, sin, positions)
+        _ints(positions, T, "positions", torch.int64)
+        invalidInputError(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype and cos.dtype in _HALF + (torch.float32,)
+                          and cos.stride(1) == 1 and cos.stride() == sin.stride() and cos.shape[0] > 0, "cos / sin must be two [positions, rotary width] of one type")
+        rotary = cos.shape[1]
+        invalidInputError(0 < rotary <= head_dim and rotary % 2 == 0, f"rotary width {rotary} with heads of {head_dim} elements")
+    if T == 0:
+        return
+    with torch.cuda.device(dev):
+        ggml.lowbit_paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache, _stream(dev))
 
 
 def _attention_args(query, n_kv_heads, cu_seqlens, scale, out):

@@ -1,0 +1,266 @@
+"""Adapters of many requests (transformers/lora.py) against 64-bit statements.
+
+Bounds.  x A^T: the K products of an element drop up to 2^-23 of their absolute sum in each of K / 16 steps of two MMAs, and some 20 times where warps and
+parts meet.  Its two 16-bit values leave 2^-16 of it (bf16) or 2^-21 (fp16, with 2^-38 of its row's largest).  The product with B drops up to 2^-23 of
+its absolute sum in each of its rank / 4 steps.  `out` is rounded once, finfo(t).eps / 2, behind an addition in 32 bits."""
+import math
+
+import pytest
+import torch
+
+HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+LEFT = {torch.float16: 2.0 ** -21, torch.bfloat16: 2.0 ** -16}
+
+
+@pytest.fixture(scope="module")
+def lora(native_lib):
+    from ipex_llm_b200.transformers import lora
+    return lora
+
+
+def rows_of(lens, ids, T):
+    """the adapter of every row"""
+    flat = [i for n, i in zip(lens, ids) for _ in range(n)]
+    return torch.tensor(flat + [-1] * (T - len(flat)))
+
+
+def make(lens, ids, K, splits, rank, adapters, dtype, dev, pad=0, seed=0):
+    g = torch.Generator(device=dev).manual_seed(seed + sum(lens) + K + rank)
+    T, N = sum(lens) + pad, sum(splits)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev)                                       # noqa: E731
+    return {"out": r(T, N).to(dtype), "x": r(T, K).to(dtype), "a": (r(adapters, len(splits), rank, K) * K ** -0.5).to(dtype), "b": (r(adapters, N, rank) * 0.3).to(dtype),
+            "scales": 0.25 + 2 * torch.rand(adapters, generator=g, device=dev), "ids": torch.tensor(ids, dtype=torch.int32, device=dev),
+            "cu": torch.tensor([0] + lens, dtype=torch.int32, device=dev).cumsum(0, dtype=torch.int32), "splits": splits}
+
+
+def statement(s, lens, ids):
+    """the result, and what it may be off by"""
+    dtype, dev = s["x"].dtype, s["x"].device
+    T, K = s["x"].shape
+    rank = s["b"].shape[2]
+    rows = rows_of(lens, ids, T).to(dev)
+    want, bound = s["out"].double(), torch.zeros(s["out"].shape, dtype=torch.float64, device=dev)
+    for i in range(s["b"].shape[0]):
+        at = (rows == i).nonzero()[:, 0]
+        first = 0
+        for j, n in enumerate(s["splits"]):
+            x, a, b, c = s["x"][at].double(), s["a"][i, j].double(), s["b"][i, first:first + n].double(), float(s["scales"][i])
+            h, size = x @ a.T, x.abs() @ a.abs().T
+            want[at, first:first + n] += c * (h @ b.T)
+            off = 2.0 ** -23 * (K / 16 + 20) * size + LEFT[dtype] * h.abs() + (2.0 ** -38 * h.abs().amax(-1, keepdim=True) if h.numel() else 0)
+            bound[at, first:first + n] += c * (off @ b.abs().T + 2.0 ** -23 * (rank / 4 + 4) * (h.abs() @ b.abs().T))
+            first += n
+    return want, HALF[dtype] * want.abs() + bound + 2.0 ** -23 * s["out"].double().abs() * (bound > 0) + (2.0 ** -25 if dtype == torch.float16 else 0)
+
+
+def run(lora, s, **more):
+    args = {"splits": s["splits"]} | more
+    out = s["out"].clone()
+    got = lora.lora_add_(out, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], **args)
+    assert got is out
+    return out
+
+
+def check(lora, s, lens, ids):
+    want, bound = statement(s, lens, ids)
+    got = run(lora, s)
+    assert bool(((got.double() - want).abs() <= bound).all())
+    nobody = rows_of(lens, [i if 0 <= i < s["b"].shape[0] else -1 for i in ids], s["x"].shape[0]).to(got.device) < 0
+    assert torch.equal(got[nobody], s["out"][nobody])
+    return got
+
+
+CASES = [([1], [0], 1), ([1], [-1], 1), ([1, 1, 1, 1, 1], [2, 0, 2, -1, 1], 3), ([0, 3, 0, 17], [1, 0, 5, 1], 2), ([16, 1, 15, 33], [0, 1, 2, 0], 4), ([64, 1, 63, 200], [3, -1, 0, 3], 4),
+         ([300], [0], 1), ([1] * 40 + [250] + [1] * 30, [i % 7 for i in range(71)], 7), ([1] * 300, [i * 5 % 67 for i in range(300)], 67), ([2, 1, 3] * 230, [i % 3 - 1 for i in range(690)], 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,ids,adapters", CASES)
+@pytest.mark.parametrize("K,splits,rank", [(8, [8], 8), (256, [256], 16), (1000, [136, 40, 40], 24), (4096, [520], 64), (96, [128, 128], 128)])
+def test_rows_take_their_adapters(lora, cuda_device, dtype, lens, ids, adapters, K, splits, rank):
+    check(lora, make(lens, ids, K, splits, rank, adapters, dtype, cuda_device, pad=5), lens, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K,splits,rank", [(14336, [4096], 16), (4096, [4096, 1024, 1024], 32), (4096, [11008, 11008], 8), (2048, [2040], 256), (512, [64] * 8, 256), (8, [8, 8], 256)])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [100, 1, 300]])
+def test_layer_sizes(lora, cuda_device, dtype, K, splits, rank, lens):
+    ids = [1, -1, 0]
+    check(lora, make(lens, ids, K, splits, rank, 2, dtype, cuda_device), lens, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[3, 1], [200, 130]])
+def test_only_the_result_is_rounded(lora, cuda_device, dtype, lens):
+    """`out` takes the product away again: what is left is far below what one 16-bit value of x A^T leaves"""
+    s = make(lens, [0, 1], 512, [256], 32, 2, dtype, cuda_device)
+    s["out"].zero_()
+    s["out"] = (-statement(s, lens, [0, 1])[0]).to(dtype)
+    want, bound = statement(s, lens, [0, 1])
+    check(lora, s, lens, [0, 1])
+    # with one value
+    first = s["x"].double() @ s["a"][0, 0].double().T
+    once = s["out"][:lens[0]].double() + float(s["scales"][0]) * (first[:lens[0]].to(dtype).double() @ s["b"][0].double().T)
+    assert bool(((once - want[:lens[0]]).abs() > bound[:lens[0]]).any())
+
+
+@pytest.mark.gpu
+def test_products_beyond_fp16(lora, cuda_device):
+    """x A^T of 10^6 and of 10^-6, which fp16 cannot hold, and a B that brings them back"""
+    for up in (2.0 ** 7, 2.0 ** -9):
+        s = make([5, 90], [0, 1], 256, [64], 16, 2, torch.float16, cuda_device)
+        s["x"] *= up
+        s["a"] *= up * 64 if up > 1 else up
+        s["b"] *= 2.0 ** -12 if up > 1 else 2.0 ** 8
+        want, bound = statement(s, [5, 90], [0, 1])
+        assert bool(torch.isfinite(want).all())
+        check(lora, s, [5, 90], [0, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[1, 1, 1, 1], [40, 300, 7, 90]])
+def test_what_is_not_finite_stays_in_its_row(lora, cuda_device, dtype, lens):
+    ids = [0, 1, 0, -1]
+    s = make(lens, ids, 256, [64, 64], 16, 3, dtype, cuda_device, pad=3)
+    clean = run(lora, s)
+    s["x"][lens[0]:sum(lens[:2])] = math.nan                           # a request's activations
+    s["x"][sum(lens):] = math.inf                                      # padding
+    s["a"][2], s["b"][2] = math.nan, math.inf                          # an adapter that nobody has
+    got = run(lora, s)
+    rows = torch.ones(len(got), dtype=torch.bool, device=cuda_device)
+    rows[lens[0]:sum(lens[:2])] = False
+    assert torch.equal(got[rows], clean[rows]) and bool(torch.isnan(got[~rows]).all())
+
+
+@pytest.mark.gpu
+def test_layouts(lora, cuda_device):
+    lens, ids = [30, 1, 60], [1, 0, 1]
+    s = make(lens, ids, 128, [96], 16, 2, torch.bfloat16, cuda_device)
+    want = run(lora, s)
+    T = sum(lens)
+    wide_x, wide_out = torch.zeros(T, 160, dtype=torch.bfloat16, device=cuda_device), torch.full((T, 128), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    wide_x[:, 16:144], wide_out[:, 24:120] = s["x"], s["out"]
+    wide_a, wide_b = torch.zeros(4, 1, 16, 128, dtype=torch.bfloat16, device=cuda_device), torch.zeros(2, 16, 96, dtype=torch.bfloat16, device=cuda_device)
+    wide_a[::2] = s["a"]
+    wide_b.copy_(s["b"].transpose(1, 2))
+    lora.lora_add_(wide_out[:, 24:120], wide_x[:, 16:144], wide_a[::2], wide_b.transpose(1, 2), s["scales"], s["ids"], s["cu"])
+    assert torch.equal(wide_out[:, 24:120], want) and bool((wide_out[:, :24] == 7).all()) and bool((wide_out[:, 120:] == 7).all())
+    odd = torch.zeros(T, 131, dtype=torch.bfloat16, device=cuda_device)
+    odd[:, 3:] = s["x"]                                                # rows off 16 bytes
+    out = s["out"].clone()
+    lora.lora_add_(out, odd[:, 3:], s["a"][:, 0], s["b"], s["scales"], s["ids"], s["cu"])        # one projection: a without the splits
+    assert torch.equal(out, want)
+    none = lora.lora_add_(out[:0], s["x"][:0], s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+    assert none.shape == (0, 96)
+
+
+@pytest.mark.gpu
+def test_lists_that_do_not_fit_the_rows(lora, cuda_device):
+    """more tokens than rows, requests in a padded batch, an adapter that is not there"""
+    s = make([20, 30, 4], [0, 9, 1], 64, [64], 8, 2, torch.float16, cuda_device)
+    want = run(lora, s)
+    assert torch.equal(want[20:50], s["out"][20:50])
+    cut = {**s, "x": s["x"][:52], "out": s["out"][:52]}
+    assert torch.equal(run(lora, cut), want[:52])
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(lora, cuda_device):
+    """a tensor of more than 2^32 bytes, in which the last rows have an adapter"""
+    T, K, N = 150000, 16384, 16
+    x = torch.empty(T, K, dtype=torch.float16, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    x[-40:] = torch.randn(40, K, generator=g, device=cuda_device).half()
+    s = make([40], [0], K, [N], 8, 1, torch.float16, cuda_device)
+    s["x"] = x[-40:].clone()
+    want = run(lora, s)
+    out = torch.zeros(T, N, dtype=torch.float16, device=cuda_device)
+    out[-40:] = s["out"]
+    ids, cu = torch.tensor([-1, 0], dtype=torch.int32, device=cuda_device), torch.tensor([0, T - 40, T], dtype=torch.int32, device=cuda_device)
+    lora.lora_add_(out, x, s["a"], s["b"], s["scales"], ids, cu)
+    # other tiles than above: other sums of the same products
+    assert bool(((out[-40:] - want).double().abs() <= 2 * statement(s, [40], [0])[1]).all()) and not bool(out[:-40].any())
+
+
+@pytest.mark.gpu
+def test_the_same_every_time_and_on_other_streams(lora, cuda_device):
+    lens = [1] * 30 + [200, 100]
+    s = make(lens, [i % 5 for i in range(32)], 1024, [512], 32, 5, torch.bfloat16, cuda_device)
+    want = run(lora, s)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for st in streams * 2:
+        with torch.cuda.stream(st):
+            got.append(run(lora, s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.gpu
+def test_a_recorded_call_serves_other_requests(lora, cuda_device):
+    lens = [1] * 8 + [50]
+    s = make(lens, [0] * 9, 256, [128, 64], 16, 3, torch.float16, cuda_device)
+    base, out = s["out"].clone(), s["out"].clone()
+    lora.lora_add_(out, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], splits=s["splits"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lora.lora_add_(out, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], splits=s["splits"])
+    for lens, ids in (([3, 0, 20, 1, 1, 1, 1, 1, 10], [2, 0, -1, 1, 1, 0, 0, 2, 2]), ([58] + [0] * 8, [1] * 9)):
+        s["cu"].copy_(torch.tensor([0] + lens, dtype=torch.int32, device=cuda_device).cumsum(0))
+        s["ids"].copy_(torch.tensor(ids, dtype=torch.int32))
+        out.copy_(base)
+        graph.replay()
+        assert torch.equal(out, run(lora, s))
+        check(lora, s, lens, ids)
+
+
+@pytest.mark.gpu
+def test_refusals(lora, cuda_device):
+    s = make([3, 2], [0, 1], 64, [32, 32], 16, 2, torch.float16, cuda_device)
+    names = ("out", "x", "a", "b", "scales", "ids", "cu")
+
+    def call(splits=(32, 32), **changed):
+        lora.lora_add_(*({**s, **changed}[n] for n in names), splits=splits)
+    call()
+    bad = [{"x": s["x"].float()}, {"out": s["out"].bfloat16()}, {"a": s["a"].bfloat16()}, {"x": s["x"][:4]}, {"x": s["x"][:, :56]}, {"b": s["b"][:, :56]}, {"b": s["b"][:, :, :8]}, {"a": s["a"][:1]},
+           {"scales": s["scales"].half()}, {"scales": s["scales"][:1]}, {"ids": s["ids"].long()}, {"ids": s["ids"][:1]}, {"cu": s["cu"].long()}, {"cu": s["cu"][:2]},
+           {"splits": (32, 24)}, {"splits": (36, 28)}, {"splits": (64,)}, {"splits": None}, {"splits": (64, 0)}, {"ids": s["ids"].cpu()}, {"scales": s["scales"].cpu()}, {"a": s["a"][0]},
+           {"a": s["a"][:, :, :12], "b": s["b"][:, :, :12]}, {"x": s["x"][:, :60], "a": s["a"][..., :60]}, {"out": torch.zeros(5, 67, dtype=torch.float16, device=cuda_device)[:, 3:]},
+           {"out": s["out"].t().contiguous().t()}, {"out": s["out"][0].expand(5, 64)}]
+    for i, more in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call(**more)
+            pytest.fail(f"call {i} was taken")
+    for n in ("out", "x", "a", "b", "scales"):
+        with pytest.raises(RuntimeError, match="backward"):
+            call(**{n: s[n].clone().requires_grad_()})
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(**{n: torch.autograd.forward_ad.make_dual(s[n], torch.ones_like(s[n]))})
+        with torch.no_grad():
+            call(**{n: s[n].clone().requires_grad_()})
+
+
+def test_refusals_on_the_cpu(lora, native_lib):
+    s = make([3, 2], [0, 1], 64, [32], 16, 2, torch.float16, torch.device("cpu"))
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        lora.lora_add_(s["out"], s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+    import ctypes
+    lib, some = native_lib._lib, 4096                                  # never read: every call is refused before anything is launched
+    splits = (ctypes.c_int * 2)(32, 32)
+    good = [some, 64, 1, 5, 64, some, 2 * 16 * 64, some, 64 * 16, 16, some, 2, some, some, 2, splits, 2, some, 64, some, 1 << 20, None]
+    for i, bad in ((0, None), (0, 4100), (1, 56), (1, 68), (2, 0), (3, -1), (3, 1 << 40), (4, 60), (4, 0), (5, None), (6, 100), (7, None), (8, 100), (9, 12), (9, 264), (9, 0), (10, None), (11, 0),
+                   (12, None), (13, None), (14, 0), (15, None), (15, (ctypes.c_int * 2)(32, 12)), (15, (ctypes.c_int * 2)(64, 0)), (16, 0), (16, 9), (17, None), (17, 4104), (18, 56)):
+        args = list(good)
+        args[i] = bad
+        assert lib.lowbit_lora_add_cuda(*args) == 1, (i, bad)
+    for i, bad in ((19, None), (19, 4100), (20, 15)):
+        args = list(good)
+        args[i] = bad
+        assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
+    assert lib.lowbit_lora_workspace_size(0, 64, 16, 1, 1) == 0 and lib.lowbit_lora_workspace_size(5, 64, 32, 2, 2) >= 5 * 32 * 4
