@@ -135,7 +135,7 @@ def build(force=False, verbose=False, ptxas_info=False):
 
 
 HOST_SRC = os.path.join(CSRC, "host", "linear_host.cpp")
-HOST_SRCS = [HOST_SRC, os.path.join(CSRC, "host", "paged_host.cpp")]
+HOST_SRCS = [HOST_SRC] + [os.path.join(CSRC, "host", f) for f in ("paged_host.cpp", "step_host.cpp")]
 
 
 def host_lib():
@@ -149,7 +149,7 @@ def build_host(force=False, verbose=False):
     """the CPython module behind LowBitLinear.forward (csrc/host).  Safe to call from several processes at once."""
     import sysconfig
     path = host_lib()
-    deps = HOST_SRCS + [os.path.join(CSRC, "host", "paged_host.h")]
+    deps = HOST_SRCS + [os.path.join(CSRC, "host", f) for f in ("paged_host.h", "host_common.h")]
     if not force and os.path.exists(path) and os.path.getmtime(path) >= max(map(os.path.getmtime, deps)):
         return path
     import torch

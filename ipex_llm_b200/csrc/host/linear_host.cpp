@@ -3,7 +3,7 @@
 // same took 20 us around a 4 us kernel.  A CPython module (b200_host); the kernels are reached through the addresses of
 // libb200lowbit.so's entry points, which the package hands over once.  Beside it, attention over the 8-bit cache (attention: the Python
 // statements took 24 us around kernels of 5 to 17 us) and the look at a mixture's experts that every call of theirs begins with
-// (expert_addresses).  The paged cache's operators: paged_host.cpp.
+// (expert_addresses).  The paged cache's operators: paged_host.cpp, what a server's step has beside its attention: step_host.cpp.
 #include <vector>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -244,6 +244,14 @@ PyMethodDef methods[] = {{"attach", attach, METH_VARARGS, nullptr},
                          {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_append)), METH_FASTCALL, nullptr},
                          {"sdp_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sdp_paged)), METH_FASTCALL, nullptr},
                          {"sdp_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sdp_packed)), METH_FASTCALL, nullptr},
+                         {"attach_step", attach_step, METH_VARARGS, nullptr},
+                         {"paged_norm_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_norm_append)), METH_FASTCALL, nullptr},
+                         {"paged_fork", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_fork)), METH_FASTCALL, nullptr},
+                         {"paged_share_release", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_share_release)), METH_FASTCALL, nullptr},
+                         {"paged_compact", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_compact)), METH_FASTCALL, nullptr},
+                         {"paged_copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_copy)), METH_FASTCALL, nullptr},
+                         {"lora_add", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lora_add)), METH_FASTCALL, nullptr},
+                         {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(token_logprobs)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

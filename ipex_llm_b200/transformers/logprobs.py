@@ -9,6 +9,7 @@ import torch
 from ipex_llm_b200.utils.common import invalidInputError, LazyModule
 
 ggml = LazyModule("ipex_llm_b200.ggml.model.llama.llama_cpp")      # loaded by the first call of one of its kernels
+paged_kv = LazyModule("ipex_llm_b200.transformers.paged_kv")        # its native host side has this operator's too
 
 _TYPES = (torch.float16, torch.bfloat16, torch.float32)
 TOP_MOST = 32                                                       # alternatives of a row
@@ -71,6 +72,9 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
 
     Where the logits want a gradient, ``logprobs``, ``entropy`` and ``top_logprobs`` have one: another launch, which reads the logits again and writes their
     gradient, rounded once to their type.  The logits must not be overwritten before it.  It has no derivative of its own."""
+    out = paged_kv._native("token_logprobs", logits, tokens, top_k, temperature)
+    if out is not None:
+        return TokenLogprobs._make(out)
     invalidInputError(logits.dim() >= 1 and logits.dtype in _TYPES and logits.shape[-1] > 0, "logits must be fp16, bf16 or fp32 [..., vocabulary]")
     invalidInputError(logits.device.type == "cuda", "token_logprobs runs on a CUDA device (there is no CPU path)")
     invalidInputError(tokens.dtype == torch.int64 and tokens.device == logits.device and tokens.shape == logits.shape[:-1],

@@ -8,6 +8,7 @@ import torch
 from ipex_llm_b200.utils.common import invalidInputError, LazyModule
 
 ggml = LazyModule("ipex_llm_b200.ggml.model.llama.llama_cpp")      # loaded by the first call of one of its kernels
+paged_kv = LazyModule("ipex_llm_b200.transformers.paged_kv")        # its native host side has this operator's too
 
 _HALF = (torch.float16, torch.bfloat16)
 RANK_MOST, SPLITS_MOST = 256, 8
@@ -30,6 +31,10 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     x A^T is kept in 32 bits and enters the second product as two 16-bit values, so that only ``out`` is rounded, once.  Two launches, nothing
     comes back to the host, and the lists are read on the device: a recorded step serves other requests.  There is no backward pass: tensors that want a
     gradient or carry a tangent are refused."""
+    if splits is not None:
+        splits = [int(n) for n in splits]
+    if paged_kv._native("lora_add", out, x, a, b, scales, adapter_ids, cu_seqlens, splits) is not None:
+        return out
     tensors = (out, x, a, b, scales)
     dev = x.device
     invalidInputError(dev.type == "cuda", "adapters run on a CUDA device (there is no CPU path)")
@@ -41,7 +46,7 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
                       "x [T, K], out [T, N] and the adapters must be fp16 or bf16, all of one type")
     T, K = x.shape
     N = out.shape[1]
-    splits = [N] if splits is None else [int(n) for n in splits]
+    splits = [N] if splits is None else splits
     if a.dim() == 3:
         a = a.unsqueeze(1)
     invalidInputError(a.dim() == 4 and b.dim() == 3, "a must be [adapters, (splits,) rank, K] and b [adapters, N, rank]")

@@ -63,6 +63,10 @@ def _load_host():
                 module.attach_paged(*(ctypes.cast(getattr(ggml._lib, f), ctypes.c_void_p).value
                                       for f in ("lowbit_paged_step_cuda", "lowbit_paged_rope_append_cuda", "lowbit_sdp_paged_workspace_size", "lowbit_sdp_paged_cuda",
                                                 "lowbit_sdp_packed_workspace_size", "lowbit_sdp_packed_cuda")))
+                module.attach_step(*(ctypes.cast(getattr(ggml._lib, f), ctypes.c_void_p).value
+                                     for f in ("lowbit_paged_norm_rope_append_cuda", "lowbit_paged_fork_cuda", "lowbit_paged_share_release_workspace_size",
+                                               "lowbit_paged_share_release_cuda", "lowbit_paged_compact_workspace_size", "lowbit_paged_compact_cuda", "lowbit_paged_copy_cuda",
+                                               "lowbit_lora_workspace_size", "lowbit_lora_add_cuda", "lowbit_token_logprobs_cuda")))
                 _host = module
             except Exception as e:
                 warnings.warn(f"the native host side of LowBitLinear and attention is not available, its Python statements run instead: {e}")

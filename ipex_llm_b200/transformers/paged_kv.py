@@ -126,6 +126,8 @@ def paged_release(done, block_table, free_pages, free_count, held=None, page_siz
     only what lies behind those: a step that found too few pages is taken back so, and tokens that a request drops.  A page that several rows name
     would go back once for each, but for ``shared`` (``paged_fork``): a page that rows beside these name stays theirs, with its count in ``shared``
     lowered, and one that is given up by all goes back once, in the order of the entries that name it first."""
+    if shared is not None and _native("paged_share_release", done, block_table, free_pages, free_count, held, page_size, shared) is not None:
+        return
     dev = _device(done, block_table, free_pages, free_count)
     invalidInputError(done.dtype in (torch.bool, torch.uint8) and done.dim() == 1 and done.is_contiguous() and done.shape[0] > 0, "done must be a contiguous bool [R]")
     _table(block_table)
@@ -182,6 +184,9 @@ def paged_fork(parents, children, context_lens, block_table, free_pages, free_co
     ``free_pages`` / ``free_count`` / ``free_left`` as in ``paged_step``.  Where ``missing`` is not 0 the last children lack that page: they are given back, with
     ``shared``, before somebody forks again.  From now on rows go back by ``paged_release(..., shared=shared)``; a row that keeps part of its tokens (``held``)
     must not be written to behind them while others name that page."""
+    out = _native("paged_fork", parents, children, context_lens, block_table, free_pages, free_count, shared, page_size, free_left)
+    if out is not None:
+        return PagedFork._make(out)
     F, R = parents.shape[0], block_table.shape[0]
     dev = _device(parents, children, context_lens, block_table, free_pages, free_count, shared)
     _ints(parents, F, "parents")
@@ -225,6 +230,8 @@ def paged_copy(src, dst, caches):
     """Page ``src[i]`` to page ``dst[i]`` (int32 [n]) of every cache in the list -- keys and values of all layers -- in one launch for up to 256 caches of one
     layout.  Pairs with a number outside the cache (-1) are left out; no page may be a source and a target, or a target twice."""
     caches = list(caches)
+    if _native("paged_copy", src, dst, caches) is not None:
+        return
     dev = _device(src, dst)
     _ints(src, src.shape[0], "src")
     _ints(dst, src.shape[0], "dst")
@@ -245,6 +252,9 @@ def paged_compact(block_table, free_pages, free_count, shared=None):
     copies.  New tensors: what is passed in stays, so that ``paged_copy(src, dst, caches)`` can move the contents before anybody reads by the new
     table.  The highest page in use moves to the lowest free one until no free page lies in front of a used one; pages that are neither in the table nor on the
     stack stay where they are.  A page that several rows name moves once."""
+    out = _native("paged_compact", block_table, free_pages, free_count, shared)
+    if out is not None:
+        return PagedCompact._make(out)
     dev = _device(block_table, free_pages, free_count)
     _table(block_table)
     _ints(free_pages, free_pages.shape[0], "free_pages")
@@ -298,6 +308,8 @@ def paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, q_weight, k_weigh
     x w / sqrt(mean x^2 + eps), w = ``q_weight`` or ``k_weight`` [head_dim] (fp16, bf16 or fp32, both of one type), and is then rotated, in place; keys and
     values go into their slots.  The norm and the rotation are in 32 bits with one rounding behind both.  ``cos`` / ``sin`` / ``positions`` / ``slots`` and the
     caches as there; caches of None (another kind of cache): only ``qkv`` is written."""
+    if _native("paged_norm_append", qkv, n_heads, n_kv_heads, head_dim, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache) is not None:
+        return
     _no_grad(qkv, q_weight, k_weight, cos, sin, k_cache, v_cache)
     invalidInputError(qkv.dim() == 2 and qkv.dtype in _HALF and n_heads >= 0 and n_kv_heads >= 0 and n_heads + n_kv_heads > 0 and head_dim > 0
                       and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and (qkv.stride(1) == 1 or qkv.numel() == 0),
