@@ -34,6 +34,13 @@ template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a
     else asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same from zero
+template <bool BF> __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF) asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 template <bool BF> __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if (BF) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t*>(&h); }
     const __half2 h = __floats2half2_rn(x, y);
@@ -42,6 +49,14 @@ template <bool BF> __device__ __forceinline__ uint32_t pack2(float x, float y) {
 template <bool BF> __device__ __forceinline__ float2 unpack2(uint32_t w) {
     if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// two 16-bit values plus two of 32 bits, rounded once, by the addition that takes a 16-bit term
+template <bool BF> __device__ __forceinline__ uint32_t add2(uint32_t v, float x, float y) {
+    float a, b;
+    if (BF) asm("{\n\t.reg .b16 p, q;\n\tmov.b32 {p, q}, %2;\n\tadd.rn.f32.bf16 %0, p, %3;\n\tadd.rn.f32.bf16 %1, q, %4;\n\t}" : "=f"(a), "=f"(b) : "r"(v), "f"(x), "f"(y));
+    else asm("{\n\t.reg .b16 p, q;\n\tmov.b32 {p, q}, %2;\n\tadd.rn.f32.f16 %0, p, %3;\n\tadd.rn.f32.f16 %1, q, %4;\n\t}" : "=f"(a), "=f"(b) : "r"(v), "f"(x), "f"(y));
+    return pack2<BF>(a, b);
 }
 
 // the blocks of a cluster meet; what they wrote, to one another too, is seen by all
@@ -57,151 +72,234 @@ __device__ __forceinline__ uint32_t shared_of(uint32_t at, uint32_t block) {
     return p;
 }
 
-// the different adapters among a tile's rows, and the rows of each
-template <int TM> struct Tile {
-    int id[TM];
-    int n, adapter[TM];
-    uint64_t rows[TM];
+constexpr int TM = 64;                                         // rows of a tile
+
+// the different adapters among a tile's rows, and the rows of each, one behind the other
+struct Tile {
+    int id[TM];                                                // of the request that begins in a row; -2: none does
+    int n, adapter[TM], first[TM + 1];
+    uint8_t row[TM];
 };
 // the whole block; ends behind a barrier
-template <int TM> __device__ __forceinline__ void find_adapters(const LoraArgs& A, int64_t t0, Tile<TM>& tile) {
+__device__ __forceinline__ void find_adapters(const LoraArgs& A, int64_t t0, Tile& tile) {
     const int lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < TM; i += LORA_THREADS) tile.id[i] = -1;
+    if (threadIdx.x < TM) tile.id[threadIdx.x] = -2;
     __syncthreads();
+    const int64_t end = min((int64_t)A.cu[A.R], A.T);          // rows behind it are nobody's
     for (int r = threadIdx.x; r < A.R; r += LORA_THREADS) {
-        const int64_t a = max((int64_t)A.cu[r], t0), b = min(min((int64_t)A.cu[r + 1], A.T), t0 + TM);
+        const int64_t a = A.cu[r], b = A.cu[r + 1];
         const int id = A.ids[r];
-        if (a < b && id >= 0 && id < A.adapters)
-            for (int64_t t = a; t < b; t++) tile.id[t - t0] = id;
+        if (a < b && b > t0 && a < t0 + TM) tile.id[max(a - t0, (int64_t)0)] = id >= 0 && id < A.adapters ? id : -1;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        // rows `lane` and, of tiles with more, `lane` + 32
-        int v[2] = {lane < TM ? tile.id[lane] : -1, TM > 32 ? tile.id[lane + 32 < TM ? lane + 32 : 0] : -1};
-        int n = 0;
-#pragma unroll
-        for (int h = 0; h < (TM > 32 ? 2 : 1); h++)
-            for (uint32_t left = __ballot_sync(0xffffffffu, v[h] >= 0); left; left = __ballot_sync(0xffffffffu, v[h] >= 0)) {
-                const int id = __shfl_sync(0xffffffffu, v[h], __ffs(left) - 1);
-                const uint32_t low = __ballot_sync(0xffffffffu, v[0] == id), high = __ballot_sync(0xffffffffu, v[1] == id);
-                if (lane == 0) { tile.adapter[n] = id; tile.rows[n] = (uint64_t)high << 32 | low; }
-                if (v[0] == id) v[0] = -1;
-                if (v[1] == id) v[1] = -1;
-                n++;
-            }
-        if (lane == 0) tile.n = n;
+        // of rows `lane` and `lane` + 32: what began last
+        int v[2] = {tile.id[lane], tile.id[lane + 32]};
+        const uint32_t under = (1u << lane) - 1u, upto = under | 1u << lane;
+        const uint32_t low = __ballot_sync(0xffffffffu, v[0] != -2), high = __ballot_sync(0xffffffffu, v[1] != -2);
+        const int last = __shfl_sync(0xffffffffu, v[0], low ? 31 - __clz(low) : 0);
+        const int v0 = __shfl_sync(0xffffffffu, v[0], low & upto ? 31 - __clz(low & upto) : lane), v1 = __shfl_sync(0xffffffffu, v[1], high & upto ? 31 - __clz(high & upto) : lane);
+        v[0] = t0 + lane < end ? v0 : -1;
+        v[1] = t0 + lane + 32 < end ? (high & upto ? v1 : last) : -1;
+        int n = 0, at = 0;
+        for (;;) {
+            const uint32_t left = __ballot_sync(0xffffffffu, v[0] >= 0), more = __ballot_sync(0xffffffffu, v[1] >= 0);
+            if (!(left | more)) break;
+            const int id = left ? __shfl_sync(0xffffffffu, v[0], __ffs(left) - 1) : __shfl_sync(0xffffffffu, v[1], __ffs(more) - 1);
+            const uint32_t here = __ballot_sync(0xffffffffu, v[0] == id), there = __ballot_sync(0xffffffffu, v[1] == id);
+            if (v[0] == id) { tile.row[at + __popc(here & under)] = (uint8_t)lane; v[0] = -1; }
+            if (v[1] == id) { tile.row[at + __popc(here) + __popc(there & under)] = (uint8_t)(lane + 32); v[1] = -1; }
+            if (lane == 0) { tile.adapter[n] = id; tile.first[n] = at; }
+            at += __popc(here) + __popc(there);
+            n++;
+        }
+        if (lane == 0) { tile.n = n; tile.first[n] = at; }
     }
     __syncthreads();
 }
 
-// Sizes of a tile of TM rows: warps in KG groups of the inner dimension and TG of the rows, 16 MT rows of A at a time
-template <int TM> struct Lora {
-    static constexpr int TG = TM > 16 ? 2 : 1, KG = LORA_WARPS / TG, NT = TM / 8 / TG, MT = TM > 16 ? 2 : 4, ROWS = 16 * MT;
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+    return r;
+}
+
+// Shared memory: two stages of 4 KB a warp, in which every lane finds what it asked for itself (so nobody waits for a neighbour), and in their place the
+// sums of the warps on their way together; h as two 16-bit values; the block's part of h.
+struct Lora {
+    static constexpr int NT = 4, MT = 2, TOKS = 8 * NT, ROWS = 16 * MT;      // tiles of 8 tokens and of 16 rows of A in the first product
     static constexpr int PITCH = ROWS + 4;                     // a warp's stores of sums meet every bank once
-    static constexpr int kSums = KG * TM * PITCH * 4;
+    static constexpr int kStage = 8 * 512, kRing = LORA_WARPS * 2 * kStage;
+    static_assert(kRing >= LORA_WARPS * TOKS * PITCH * 4, "the sums fit");
     static __host__ __device__ int steps(int rank) { return (rank + 15) / 16; }
-    // bytes of a row of h: 16 a step and split, 4 rows on different banks
-    static __host__ __device__ int pitch(int rank, int together) { const int n = steps(rank) * together; return 32 * n + (n & 1 ? 0 : 32); }
-    static __host__ __device__ int parts(int rank, int together) { const int h = 2 * TM * pitch(rank, together); return h > kSums ? h : kSums; }
-    static __host__ __device__ int smem(int rank, int together) { return parts(rank, together) + TM * together * rank * 4; }
+    // h as the second product's A operand: for each split, step of 16 and tile of 16 tokens 16 bytes a lane of high parts, then of low parts
+    static constexpr int kFrag = 1024, kStep = TM / 16 * kFrag;
+    static __host__ __device__ int smem(int rank, int together) { return kRing + together * steps(rank) * kStep + TM * together * rank * 4; }
 };
 
-// First product: A operand 16 MT rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two
-// steps' k = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.
+// First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
+// = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K.
 // Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
-// holds 16 bytes of a row of `out`.
-template <bool BF, int TM>
+// holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.
+template <bool BF, int STEPS>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
-    using L = Lora<TM>;
-    constexpr int NT = L::NT, MT = L::MT, ROWS = L::ROWS;
-    __shared__ Tile<TM> tile;
+    using L = Lora;
+    constexpr int NT = L::NT, MT = L::MT, ROWS = L::ROWS, TOKS = L::TOKS;
+    __shared__ Tile tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
-    extern __shared__ __align__(16) uint8_t lora_smem[];
+    extern __shared__ __align__(128) uint8_t lora_smem[];
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int kg = warp / L::TG, n0 = warp % L::TG * NT;       // this warp's part of the first product
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = (int64_t)(blockIdx.x / blocks) * TM;
-    const int steps = L::steps(A.rank), pitch = L::pitch(A.rank, A.together);
-    float* const sums = reinterpret_cast<float*>(lora_smem);  // [KG][TM][PITCH], and h behind it in the same place
-    float* const part = reinterpret_cast<float*>(lora_smem + L::parts(A.rank, A.together));
+    const int steps = STEPS ? STEPS : L::steps(A.rank);
+    float* const sums = reinterpret_cast<float*>(lora_smem);
+    float* const part = reinterpret_cast<float*>(lora_smem + L::kRing + A.together * steps * L::kStep);
+    const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, hs = smem + L::kRing;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    find_adapters<TM>(A, t0, tile);
+    find_adapters(A, t0, tile);
     const int chunks = (A.K + 31) / 32, each = (chunks + (int)blocks - 1) / (int)blocks, from = min((int)rank * each, chunks), to = min(from + each, chunks);
     for (int j = blockIdx.y; j < tile.n; j += gridDim.y) {
-        const uint64_t mask = tile.rows[j];
-        const int id = tile.adapter[j];
+        const int id = tile.adapter[j], count = tile.first[j + 1] - tile.first[j];
+        const uint8_t* const row_of = tile.row + tile.first[j];
         const float scale = A.scales[id];
         for (int s0 = 0; s0 < A.n_splits; s0 += A.together) {
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
-            const uint16_t* const w = (const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K;
-            // ---- h of this block's share of K
-            for (int row0 = 0; row0 < rows; row0 += ROWS) {
+            const uint4* const w = (const uint4*)((const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K);
+            // ---- h of this block's share of K.  Rows behind the last, of A and of x, are read as the last ones: nobody looks at what they give
+            for (int row0 = 0, i0 = 0; row0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, row0 += i0 ? 0 : ROWS) {
+                const int m_end = min(MT, (rows - row0 + 15) / 16), n_end = min(NT, (count - i0 + 7) / 8);
                 float acc[MT][NT][4] = {};
-#pragma unroll 2
-                for (int c = from + kg; c < to; c += L::KG) {
-                    const int k = 32 * c + 8 * t;
-                    const bool in = k < A.K;
-                    uint4 wr[MT][2], xr[NT];
+                uint32_t xs[NT], ws[MT][2];                    // in 16 bytes, of this lane's rows
+                const uint4* const x = (const uint4*)((const uint16_t*)A.x + t0 * A.x_st);
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
+                for (int n = 0; n < NT; n++) xs[n] = (uint32_t)(row_of[min(i0 + 8 * n + g, count - 1)] * (A.x_st / 8));
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int row = row0 + 16 * m + 8 * h + g;
-                            wr[m][h] = in && row < rows ? *reinterpret_cast<const uint4*>(w + (int64_t)row * A.K + k) : make_uint4(0, 0, 0, 0);
-                        }
+                for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const int64_t tok = t0 + 8 * (n0 + n) + g;
-                        xr[n] = in && tok < A.T && (mask >> (8 * (n0 + n)) & 0xff) ? *reinterpret_cast<const uint4*>((const uint16_t*)A.x + tok * A.x_st + k) : make_uint4(0, 0, 0, 0);
-                    }
+                    for (int h = 0; h < 2; h++) ws[m][h] = (uint32_t)min(row0 + 16 * m + 8 * h + g, rows - 1) * (uint32_t)(A.K / 8);
+                auto ask = [&](int c, int stage) {
+                    const bool in = c < to && 32 * c + 8 * t < A.K;
+                    const uint32_t k = in ? 4 * c + t : 0, at = ring + stage * L::kStage;
 #pragma unroll
                     for (int n = 0; n < NT; n++)
-                        if (mask >> (8 * (n0 + n)) & 0xff) {
-#pragma unroll
-                            for (int m = 0; m < MT; m++)
-                                if (row0 + 16 * m < rows) {
-                                    mma<BF>(acc[m][n], wr[m][0].x, wr[m][1].x, wr[m][0].y, wr[m][1].y, xr[n].x, xr[n].y);
-                                    mma<BF>(acc[m][n], wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w, xr[n].z, xr[n].w);
-                                }
-                        }
-                }
-                __syncthreads();                               // what was in the sums' place is read
-#pragma unroll
-                for (int n = 0; n < NT; n++)
+                        if (n < n_end) cp16(at + n * 512, x + (xs[n] + k), in);
 #pragma unroll
                     for (int m = 0; m < MT; m++)
+                        if (m < m_end) {
+                            cp16(at + (NT + 2 * m) * 512, w + (ws[m][0] + k), in);
+                            cp16(at + (NT + 2 * m + 1) * 512, w + (ws[m][1] + k), in);
+                        }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
+                __syncthreads();                               // what was in the ring's place is read
+                ask(from + warp, 0);
+                ask(from + warp + LORA_WARPS, 1);
+                int stage = 0;
+#pragma unroll 1
+                for (int c = from + warp; c < to; c += LORA_WARPS, stage ^= 1) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    const uint32_t at = ring + stage * L::kStage;
+                    uint4 wr[MT][2];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sums[(kg * TM + 8 * (n0 + n) + 2 * t + (e & 1)) * L::PITCH + 16 * m + g + 8 * (e >> 1)] = acc[m][n][e];
+                    for (int m = 0; m < MT; m++)
+                        if (m < m_end) { wr[m][0] = lds16(at + (NT + 2 * m) * 512); wr[m][1] = lds16(at + (NT + 2 * m + 1) * 512); }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        if (n < n_end) {
+                            const uint4 xr = lds16(at + n * 512);
+#pragma unroll
+                            for (int m = 0; m < MT; m++)
+                                if (m < m_end) {
+                                    mma<BF>(acc[m][n], wr[m][0].x, wr[m][1].x, wr[m][0].y, wr[m][1].y, xr.x, xr.y);
+                                    mma<BF>(acc[m][n], wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w, xr.z, xr.w);
+                                }
+                        }
+                    ask(c + 2 * LORA_WARPS, stage);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncthreads();                               // everybody is through with the ring
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    if (n < n_end) {
+#pragma unroll
+                        for (int m = 0; m < MT; m++)
+                            if (m < m_end) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) sums[(warp * TOKS + 8 * n + 2 * t + (e & 1)) * L::PITCH + 16 * m + g + 8 * (e >> 1)] = acc[m][n][e];
+                            }
+                    }
                 __syncthreads();
-                for (int i = threadIdx.x; i < TM * ROWS; i += LORA_THREADS) {
-                    const int tok = i / ROWS, row = i % ROWS;
-                    if ((mask >> tok & 1) && row0 + row < rows) {
-                        float s = 0.0f;
+                {
+                    const int i = threadIdx.x, tok = i / (ROWS / 4), row = i % (ROWS / 4) * 4;
+                    static_assert(TOKS * ROWS / 4 == LORA_THREADS, "four sums a thread");
+                    if (i0 + tok < count && row0 + row < rows) {
+                        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                        for (int v = 0; v < L::KG; v++) s += sums[(v * TM + tok) * L::PITCH + row];
-                        part[tok * rows + row0 + row] = s;
+                        for (int v = 0; v < LORA_WARPS; v++) {
+                            const float4 p = *reinterpret_cast<const float4*>(sums + (v * TOKS + tok) * L::PITCH + row);
+                            s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+                        }
+                        *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
                     }
                 }
             }
             meet(blocks);
+            // ---- this block's share of the columns, 32 a warp: where its groups lie, and what it asks for ahead.  Rows and columns behind the last are read
+            // as the last ones, and not written
+            const uint16_t* const wb = (const uint16_t*)A.b + id * A.b_st;
+            struct Group {
+                int s, before, groups, grp, c0, c_end;
+                __device__ __forceinline__ bool settle(const LoraArgs& A, int s0, int n_here) {
+                    while (grp - before >= groups) {
+                        before += groups;
+                        if (++s >= n_here) return false;
+                        groups = (A.first[s0 + s + 1] - A.first[s0 + s] + 31) / 32;
+                    }
+                    c0 = A.first[s0 + s] + 32 * (grp - before);
+                    c_end = A.first[s0 + s + 1];
+                    return true;
+                }
+            };
+            const int m_tiles = (count + 15) / 16;
+            uint32_t row_at[TM / 8];                           // rows 8 i + g of the adapter's, in 16 bytes from the tile's first on
+#pragma unroll
+            for (int i = 0; i < TM / 8; i++) row_at[i] = (uint32_t)(row_of[min(8 * i + g, count - 1)] * A.o_st / 8);
+            uint4* const out = reinterpret_cast<uint4*>((uint16_t*)A.out + t0 * A.o_st);
+            Group ahead = {0, 0, (A.first[s0 + 1] - A.first[s0] + 31) / 32, (int)rank * LORA_WARPS + warp, 0, 0};
+            bool more = ahead.settle(A, s0, n_here);
+            auto ask_out = [&](int stage) {
+                if (more) {
+                    const uint4* const from = out + min(ahead.c0 + 8 * t, ahead.c_end - 8) / 8;
+#pragma unroll
+                    for (int m = 0; m < TM / 16; m++)
+                        if (m < m_tiles) {
+                            cp16(ring + stage * L::kStage + 2 * m * 512, from + row_at[2 * m], true);
+                            cp16(ring + stage * L::kStage + (2 * m + 1) * 512, from + row_at[2 * m + 1], true);
+                        }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            ask_out(0);
             // ---- the blocks' parts together: a warp takes a row of the tile in one split
-            const uint32_t at_part = (uint32_t)__cvta_generic_to_shared(part), at_h = (uint32_t)__cvta_generic_to_shared(lora_smem), at_back = (uint32_t)__cvta_generic_to_shared(&back[0][0]);
-            for (int i = (int)rank + warp * (int)blocks; i < TM * n_here; i += LORA_WARPS * (int)blocks) {
-                const int tok = i % TM, s = i / TM;
-                if (!(mask >> (tok & ~15) & 0xffff)) continue;
-                const bool live = mask >> tok & 1;
+            const uint32_t at_part = (uint32_t)__cvta_generic_to_shared(part), at_back = (uint32_t)__cvta_generic_to_shared(&back[0][0]);
+            for (int i = (int)rank + warp * (int)blocks; i < count * n_here; i += LORA_WARPS * (int)blocks) {
+                const int tok = i % count, s = i / count;
                 float2 h[4];                                   // pairs `lane`, `lane` + 32, ...
                 float big = 0.0f;
 #pragma unroll
                 for (int z = 0; z < 4; z++) {
                     h[z] = make_float2(0.0f, 0.0f);
                     const int r = 2 * lane + 64 * z;
-                    if (live && r < A.rank) {
+                    if (r < A.rank) {
                         const uint32_t at = at_part + (tok * rows + s * A.rank + r) * 4;
+#pragma unroll 8
                         for (uint32_t b = 0; b < blocks; b++) {
                             float2 p;
                             asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(p.x), "=f"(p.y) : "r"(shared_of(at, b)) : "memory");
@@ -230,112 +328,134 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const uint32_t hi = pack2<BF>(x, y);
                     const float2 f = unpack2<BF>(hi);
                     const uint32_t lo = pack2<BF>(fabsf(f.x) < INFINITY ? x - f.x : 0.0f, fabsf(f.y) < INFINITY ? y - f.y : 0.0f);
-                    const uint32_t at = at_h + tok * pitch + s * steps * 32 + 2 * r;
+                    const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + ((tok & 7) * 4 + (r & 15) / 4) * 16 + (tok & 8) + (r & 2) * 2;
+#pragma unroll 8
                     for (uint32_t b = 0; b < blocks; b++) {
                         const uint32_t p = shared_of(at, b);
                         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p), "r"(hi) : "memory");
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p + TM * pitch), "r"(lo) : "memory");
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p + L::kFrag / 2), "r"(lo) : "memory");
                     }
                 }
+            }
+            const int off = (8 * (g >> 1) + (g & 1)) * A.rank + 4 * t;                         // this lane's rows of B are 2 n further on
+            auto fetch = [&](const Group& of, int st, uint2 (&br)[4]) {
+                const uint16_t* const p = wb + (int64_t)of.c0 * A.rank + 16 * st;
+                if (of.c0 + 32 <= of.c_end && 16 * st + 16 <= A.rank) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++) br[n] = *reinterpret_cast<const uint2*>(p + (off + 2 * n * A.rank));
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const bool there = of.c0 + 8 * (g >> 1) + 2 * n + (g & 1) < of.c_end && 16 * st + 4 * t < A.rank;
+                        br[n] = there ? *reinterpret_cast<const uint2*>(p + (off + 2 * n * A.rank)) : make_uint2(0, 0);
+                    }
+                }
+            };
+            uint2 br[STEPS ? STEPS : 1][4];
+            if (STEPS && more) {
+#pragma unroll
+                for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
             }
             meet(blocks);
-            // ---- this block's share of the columns, 32 a warp
-            const uint16_t* const wb = (const uint16_t*)A.b + id * A.b_st;
-            int s = 0, before = 0, groups = (A.first[s0 + 1] - A.first[s0] + 31) / 32;         // of the splits in front, and of this one
-            for (int grp = (int)rank * LORA_WARPS + warp;; grp += (int)blocks * LORA_WARPS) {
-                while (s < n_here && grp - before >= groups) {
-                    before += groups;
-                    s++;
-                    if (s < n_here) groups = (A.first[s0 + s + 1] - A.first[s0 + s] + 31) / 32;
-                }
-                if (s >= n_here) break;
-                const int c0 = A.first[s0 + s] + 32 * (grp - before), c_end = A.first[s0 + s + 1], col = c0 + 8 * t;
-                constexpr int MP = TM > 16 ? 2 : 1;            // tiles of 16 rows at a time
 #pragma unroll 1
-                for (int m0 = 0; m0 < TM / 16; m0 += MP) {
-                    const uint32_t some = (uint32_t)(mask >> (16 * m0)) & (MP == 2 ? 0xffffffffu : 0xffffu);
-                    if (!some) continue;
-                    uint4 o[MP][2];
+            for (int stage = 0; more; stage ^= 1) {
+                const Group now = ahead;
+                ahead.grp += (int)blocks * LORA_WARPS;
+                more = ahead.settle(A, s0, n_here);
+                ask_out(stage ^ 1);
+                const int col = now.c0 + 8 * t;
+                uint4* const to = out + col / 8;
+                const uint32_t h0 = hs + now.s * steps * L::kStep + lane * 16, o0 = ring + stage * L::kStage;
+                const int rows_here = col < now.c_end ? count - g : 0;
+                // 32 tokens at a time
 #pragma unroll
-                    for (int m = 0; m < MP; m++)
+                for (int m0 = 0; m0 < TM / 16; m0 += 2) {
+                    if (m0 >= m_tiles) break;
+                    float acc[2][4][4];
+                    auto products = [&](int st, bool first) {
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int tok = 16 * m + 8 * h + g;
-                            if ((some >> tok & 1) && col < c_end) o[m][h] = *reinterpret_cast<const uint4*>((const uint16_t*)A.out + (t0 + 16 * m0 + tok) * A.o_st + col);
-                        }
-                    float acc[MP][4][4] = {};
-                    for (int st = 0; st < steps; st++) {
-                        uint2 br[4];
-                        const int r = 16 * st + 4 * t;
-#pragma unroll
-                        for (int n = 0; n < 4; n++) {
-                            const int cc = c0 + 8 * (g >> 1) + 2 * n + (g & 1);
-                            br[n] = cc < c_end && r < A.rank ? *reinterpret_cast<const uint2*>(wb + (int64_t)cc * A.rank + r) : make_uint2(0, 0);
-                        }
-#pragma unroll
-                        for (int m = 0; m < MP; m++)
-                            if (some >> (16 * m) & 0xffff) {
-                                const uint8_t* const h = lora_smem + (16 * (m0 + m) + g) * pitch + s * steps * 32 + 32 * st + 8 * t;
-                                const uint2 a = *reinterpret_cast<const uint2*>(h), b = *reinterpret_cast<const uint2*>(h + 8 * pitch);
-                                const uint2 c = *reinterpret_cast<const uint2*>(h + TM * pitch), d = *reinterpret_cast<const uint2*>(h + (TM + 8) * pitch);
+                        for (int m = 0; m < 2; m++)
+                            if (m0 + m < m_tiles) {
+                                const uint32_t h = h0 + st * L::kStep + (m0 + m) * L::kFrag;
+                                const uint4 hi = lds16(h), lo = lds16(h + L::kFrag / 2);
 #pragma unroll
                                 for (int n = 0; n < 4; n++) {
-                                    mma<BF>(acc[m][n], c.x, d.x, c.y, d.y, br[n].x, br[n].y);
-                                    mma<BF>(acc[m][n], a.x, b.x, a.y, b.y, br[n].x, br[n].y);
+                                    const uint2 b = br[STEPS ? st : 0][n];
+                                    if (first) mma0<BF>(acc[m][n], lo.x, lo.z, lo.y, lo.w, b.x, b.y);
+                                    else mma<BF>(acc[m][n], lo.x, lo.z, lo.y, lo.w, b.x, b.y);
+                                    mma<BF>(acc[m][n], hi.x, hi.z, hi.y, hi.w, b.x, b.y);
                                 }
                             }
-                    }
+                    };
+                    if constexpr (STEPS > 0) {
 #pragma unroll
-                    for (int m = 0; m < MP; m++)
+                        for (int st = 0; st < STEPS; st++) products(st, st == 0);
+                        if (more && m0 + 2 >= m_tiles) {       // the products have B: the next group's
+#pragma unroll
+                            for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
+                        }
+                    } else {
+                        fetch(now, 0, br[0]);
+                        products(0, true);
+#pragma unroll 1
+                        for (int st = 1; st < steps; st++) {
+                            fetch(now, st, br[0]);
+                            products(st, false);
+                        }
+                    }
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int tok = 16 * m + 8 * h + g;
-                            if (!(some >> tok & 1) || col >= c_end) continue;
-                            uint32_t v[4] = {o[m][h].x, o[m][h].y, o[m][h].z, o[m][h].w};
-                            const float up = BF ? 1.0f : back[16 * m0 + tok][s];
+                            const int i = 16 * (m0 + m) + 8 * h;
+                            if (i >= rows_here) continue;
+                            const uint4 o = lds16(o0 + (2 * (m0 + m) + h) * 512);
+                            uint32_t v[4] = {o.x, o.y, o.z, o.w};
+                            const float up = BF ? 1.0f : back[i + g][now.s];
 #pragma unroll
-                            for (int n = 0; n < 4; n++) {
-                                const float2 f = unpack2<BF>(v[n]);
-                                v[n] = pack2<BF>(fmaf(acc[m][n][2 * h], up, f.x), fmaf(acc[m][n][2 * h + 1], up, f.y));
-                            }
-                            *reinterpret_cast<uint4*>((uint16_t*)A.out + (t0 + 16 * m0 + tok) * A.o_st + col) = make_uint4(v[0], v[1], v[2], v[3]);
+                            for (int n = 0; n < 4; n++) v[n] = add2<BF>(v[n], BF ? acc[m][n][2 * h] : acc[m][n][2 * h] * up, BF ? acc[m][n][2 * h + 1] : acc[m][n][2 * h + 1] * up);
+                            to[row_at[2 * (m0 + m) + h]] = make_uint4(v[0], v[1], v[2], v[3]);
                         }
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     }
 }
 
-template <bool BF, int TM> int lora_launch(LoraArgs A, cudaStream_t st) {
-    using L = Lora<TM>;
+template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     // splits that share a reading of x: 128 rows of A at most, or one split
     A.together = A.n_splits * A.rank <= 128 ? A.n_splits : A.rank >= 128 ? 1 : 128 / A.rank;
     static bool configured[64] = {};                           // the attribute is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        cudaFuncSetAttribute(lora_kernel<BF, TM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
     }
     const int64_t tiles = (A.T + TM - 1) / TM;
-    // clusters that share a tile's adapters: as many as a tile has on average
-    int64_t some = 1 + (int64_t)A.R * TM / A.T, most = TM < A.R ? TM : A.R;
+    // clusters that share a tile's adapters: twice as many as a tile has on average
+    int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
     if (most > A.adapters) most = A.adapters;
-    if (most > 16) most = 16;
     const int blocks = 8;                                      // of a cluster: the most that any device takes
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)(some < most ? some : most));
     cfg.blockDim = dim3(LORA_THREADS);
-    cfg.dynamicSmemBytes = (size_t)L::smem(A.rank, A.together);
+    cfg.dynamicSmemBytes = (size_t)Lora::smem(A.rank, A.together);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
-    cudaLaunchKernelEx(&cfg, lora_kernel<BF, TM>, A);
+    cudaLaunchKernelEx(&cfg, lora_kernel<BF, STEPS>, A);
     note_launch();
     return check_launch();
+}
+
+template <bool BF> int lora_steps(const LoraArgs& A, cudaStream_t st) {
+    return A.rank <= 16 ? lora_launch<BF, 1>(A, st) : A.rank <= 32 ? lora_launch<BF, 2>(A, st) : A.rank <= 64 && A.rank > 48 ? lora_launch<BF, 4>(A, st) : lora_launch<BF, 0>(A, st);
 }
 
 }  // namespace
@@ -347,10 +467,10 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
     reset_launch_count();
     const char* const name = "lowbit_lora_add_cuda";
     bool bad = !d_x || !d_a || !d_b || !d_scales || !d_ids || !d_cu_seqlens || !d_out || !splits || (dtype != DT_F16 && dtype != DT_BF16) || T < 0 || T > 0x7fffffffll || K <= 0 ||
-               K % 8 || K > 0x7fffff00 || rank <= 0 || rank % 8 || rank > 256 || adapters <= 0 || R <= 0 || n_splits <= 0 || n_splits > LORA_SPLITS || x_stride < K;
+               K % 8 || K > 1 << 20 || rank <= 0 || rank % 8 || rank > 256 || adapters <= 0 || R <= 0 || n_splits <= 0 || n_splits > LORA_SPLITS || x_stride < K;
     int64_t N = 0;
     for (int i = 0; !bad && i < n_splits; i++) { bad = splits[i] <= 0 || splits[i] % 8; N += splits[i]; }
-    bad = bad || N > 0x7fffff00ll || out_stride < N || a_stride < (int64_t)n_splits * rank * K || b_stride < N * rank;
+    bad = bad || N > 0x7fffff00ll || out_stride < N || a_stride < (int64_t)n_splits * rank * K || b_stride < N * rank || out_stride > 1 << 29 || x_stride > 1 << 29;
     if (bad) {
         set_error(LB_ERR_ARG, "%s: bad argument (T %lld, K %d, N %lld, rank %d, adapters %d, requests %d, splits %d, dtype %d)", name, (long long)T, K, (long long)N, rank, adapters, R,
                   n_splits, dtype);
@@ -364,6 +484,5 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
     LoraArgs A = {d_x, x_stride, T, K, d_a, a_stride, d_b, b_stride, d_scales, adapters, d_ids, d_cu_seqlens, R, d_out, out_stride, rank, n_splits, 0, {}};
     for (int i = 0; i < n_splits; i++) A.first[i + 1] = A.first[i] + splits[i];
     cudaStream_t st = (cudaStream_t)stream;
-    if (T <= 256) return dtype == DT_BF16 ? lora_launch<true, 16>(A, st) : lora_launch<false, 16>(A, st);
-    return dtype == DT_BF16 ? lora_launch<true, 64>(A, st) : lora_launch<false, 64>(A, st);
+    return dtype == DT_BF16 ? lora_steps<true>(A, st) : lora_steps<false>(A, st);
 }
