@@ -52,6 +52,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // a reference for exponents, the sum of powers, and of powers x exponents, relative to it; the largest logit
 struct Sums {
     float m, s, d, big;
@@ -154,6 +160,7 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
     __shared__ float level;
     __shared__ int n_found;
     __shared__ uint32_t owners[LP_WARPS];
+    __shared__ uint8_t owner[LP_THREADS];
     uint32_t rank, blocks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
@@ -168,9 +175,8 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
     // ---- the pass
     Sums x = {-INFINITY, 0.0f, 0.0f, -INFINITY};
     auto take = [&](const float (&v)[N]) {
-        float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
-        if (N == 8) { m0 = fmaxf(m0, fmaxf(v[N - 4], v[N - 3])); m1 = fmaxf(m1, fmaxf(v[N - 2], v[N - 1])); }
-        x.big = fmaxf(x.big, fmaxf(m0, m1));
+#pragma unroll
+        for (int i = 0; i < N; i += 2) x.big = max3(x.big, v[i], v[i + 1]);
         // the reference follows where an exponent would pass 2^20 of it: sums of powers up to that are as exact as those up to 1
         const float top = x.big * c;
         if (top > x.m + 20.0f) {
@@ -192,15 +198,15 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
         x.d += d0 + d1;
     };
     constexpr int AHEAD = 4;
-    int i = strip.first + t;
-    for (; i + (AHEAD - 1) * LP_THREADS < strip.last; i += AHEAD * LP_THREADS) {
+    for (int i = strip.first + t; i < strip.last; i += AHEAD * LP_THREADS) {
         uint4 w[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++) w[a] = strip.piece(i + a * LP_THREADS);
+        for (int a = 0; a < AHEAD; a++)
+            if (i + a * LP_THREADS < strip.last) w[a] = strip.piece(i + a * LP_THREADS);
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++) { float v[N]; Vec<T>::get(w[a], v); take(v); }
+        for (int a = 0; a < AHEAD; a++)
+            if (i + a * LP_THREADS < strip.last) { float v[N]; Vec<T>::get(w[a], v); take(v); }
     }
-    for (; i < strip.last; i += LP_THREADS) { float v[N]; Vec<T>::get(strip.piece(i), v); take(v); }
     const int end = strip.end_of(t);
     if (end >= 0) {
         float v[N];
@@ -230,24 +236,36 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
         const uint32_t own = __ballot_sync(0xffffffffu, own_big >= floor_);
         if (lane == 0) owners[warp] = own;
         __syncthreads();
+        int strips = 0, before = 0;
+#pragma unroll
+        for (int w = 0; w < LP_WARPS; w++) { const int c_ = __popc(owners[w]); strips += c_; before += w < warp ? c_ : 0; }
+        if (own >> lane & 1) owner[before + __popc(own & ((1u << lane) - 1u))] = (uint8_t)t;
+        __syncthreads();
         auto note = [&](float v, int at) {
             if (v >= floor_) {
                 const int slot = atomicAdd(&n_found, 1);       // their order does not matter: they are sorted
                 if (slot < LP_ROOM) found[slot] = key_of(v, (uint32_t)at);
             }
         };
-        int turn = 0;
-        for (int w = 0; w < LP_WARPS; w++)
-            for (uint32_t left = owners[w]; left; left &= left - 1, turn++) {
-                if ((turn & (LP_WARPS - 1)) != warp) continue; // a warp takes every eighth strip
-                const int first = strip.first + 32 * w + __ffs(left) - 1;
-                for (int p = first + lane * LP_THREADS; p < strip.last; p += 32 * LP_THREADS) {
-                    float v[N];
-                    Vec<T>::get(strip.piece(p), v);
+        const int deep = (strip.last - strip.first + LP_THREADS - 1) / LP_THREADS;             // pieces of a strip
+        for (int i = t; i < strips * deep; i += AHEAD * LP_THREADS) {
+            uint4 w[AHEAD];
+            int p[AHEAD];
 #pragma unroll
-                    for (int e = 0; e < N; e++) note(v[e], strip.base() + p * N + e);
-                }
+            for (int a = 0; a < AHEAD; a++) {
+                const int u = i + a * LP_THREADS, s = u / deep;
+                p[a] = s < strips ? strip.first + owner[s] + (u - s * deep) * LP_THREADS : strip.last;
+                if (p[a] < strip.last) w[a] = strip.piece(p[a]);
             }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (p[a] < strip.last) {
+                    float v[N];
+                    Vec<T>::get(w[a], v);
+#pragma unroll
+                    for (int e = 0; e < N; e++) note(v[e], strip.base() + p[a] * N + e);
+                }
+        }
         if (end >= 0) note(one(row + end), end);
         __syncthreads();
         const int n = n_found;
@@ -283,13 +301,15 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
                 keep(at >= 0 ? one(row + at) : 0.0f, at, at >= 0);
             }
         }
-        lists[warp][lane] = key;
+        if (n > 32) {                                          // else the first warp has them all
+            lists[warp][lane] = key;
 #pragma unroll
-        for (int h = LP_WARPS / 2; h; h >>= 1) {
-            __syncthreads();
-            if (warp < h) {
-                key = merge32(key, lists[warp + h][lane]);
-                lists[warp][lane] = key;
+            for (int h = LP_WARPS / 2; h; h >>= 1) {
+                __syncthreads();
+                if (warp < h) {
+                    key = merge32(key, lists[warp + h][lane]);
+                    lists[warp][lane] = key;
+                }
             }
         }
         if (warp == 0) best[lane] = key;
@@ -473,9 +493,11 @@ bool bad_logits(const char* name, const void* logits, int dtype, int64_t row_str
 }
 
 template <typename T> int logprobs_launch(const LogprobArgs& A, cudaStream_t st) {
-    // blocks of a row: enough for four blocks an SM, none with fewer than four pieces a thread
-    int blocks = 1;
-    while (blocks < 8 && A.rows * blocks < 4ll * sm_count() && A.V / (2 * blocks) >= LP_THREADS * Vec<T>::N) blocks *= 2;
+    // blocks of a row: as many as are resident at once, five an SM, each with a piece a thread at least
+    int64_t blocks = A.rows < 5ll * sm_count() ? 5ll * sm_count() / A.rows : 1;
+    if (blocks > 8) blocks = 8;
+    if (blocks > A.V / (LP_THREADS * Vec<T>::N)) blocks = A.V / (LP_THREADS * Vec<T>::N);
+    if (blocks < 1) blocks = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(A.rows * blocks));
     cfg.blockDim = dim3(LP_THREADS);

@@ -370,9 +370,12 @@ __global__ void __launch_bounds__(256) paged_norm_append_vec_kernel(const NormAr
         const int e0 = turn ? i : A.R + 2 * (i - half), e1 = turn ? i + half : e0 + 8;
         T* const row = (T*)A.qkv + t * A.st + (int64_t)h * A.D;
         T x0[8], x1[8];
+        int64_t p = 0, slot = -1;                              // asked for with the row: they lead to other loads
         if (live) {
             *reinterpret_cast<uint4*>(x0) = *reinterpret_cast<const uint4*>(row + e0);
             *reinterpret_cast<uint4*>(x1) = *reinterpret_cast<const uint4*>(row + e1);
+            if (turn && keeps) p = A.positions[t];
+            if (h >= A.Hq && A.kc) slot = A.slots[t];
         }
         float sum = 0.0f;
         if (live && keeps) {
@@ -393,7 +396,6 @@ __global__ void __launch_bounds__(256) paged_norm_append_vec_kernel(const NormAr
 #pragma unroll
             for (int e = 0; e < 8; e++) { a[e] = Act<T>::get(x0[e]) * inv * w[e0 + e]; b[e] = Act<T>::get(x1[e]) * inv * w[e1 + e]; }
             if (turn) {
-                int64_t p = A.positions[t];
                 p = p < 0 ? 0 : p < A.n_pos ? p : A.n_pos - 1;
                 C c[8], s[8];
 #pragma unroll
@@ -414,8 +416,6 @@ __global__ void __launch_bounds__(256) paged_norm_append_vec_kernel(const NormAr
             *reinterpret_cast<uint4*>(row + e0) = *reinterpret_cast<const uint4*>(x0);
             *reinterpret_cast<uint4*>(row + e1) = *reinterpret_cast<const uint4*>(x1);
         }
-        if (h < A.Hq || !A.kc) continue;
-        const int64_t slot = A.slots[t];
         if (slot < 0 || slot >= A.n_slots) continue;
         const int hk = h - A.Hq - (keeps ? 0 : A.Hkv);
         const int64_t pg = slot < 1ll << 31 ? (int64_t)((uint32_t)slot / (uint32_t)A.page_size) : slot / A.page_size, rw = slot - pg * A.page_size;

@@ -4,6 +4,7 @@
 // shared[p] counts the rows beyond the first that name page p.  A fork names its parent's full pages (one more each) and gets a page of its own for
 // the tokens behind them, so a page that anybody writes to is named by one row.  A row that goes takes its counts with it, and the last one gives
 // the page back.  All results are whole numbers that do not depend on the order in which threads run.
+#include <limits.h>
 #include "paged.h"
 
 using namespace lowbit;
@@ -12,6 +13,7 @@ namespace lowbit {
 namespace {
 
 constexpr int SHARE_THREADS = 1024, SHARE_WARPS = SHARE_THREADS / 32;
+constexpr int SHARE_DEEP = 8;                                  // entries of a row that a lane reads at a time: what follows waits for memory once for all
 
 // the blocks of a cluster meet; what they wrote is seen by all
 __device__ __forceinline__ void meet(uint32_t blocks) {
@@ -90,11 +92,18 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const Fork
             const int held = max(A.lens[par], 0), full = min(held / A.page_size, A.width);
             const int32_t* const from = A.table + par * A.table_stride;
             int32_t* const to = A.table + ch * A.table_stride;
-            for (int c = lane; c < A.width; c += 32) {
-                const int p = c <= full ? from[c] : -1;
-                if (c < full && p >= 0 && p < A.n_pages) atomicAdd(A.shared + p, 1);
-                to[c] = c < full ? p : c == full && page != -2 ? page : -1;
-                if (c == full) A.src[f0 + i] = page != -2 ? p : -1;
+            for (int c0 = lane; c0 < A.width; c0 += 32 * SHARE_DEEP) {
+                int p[SHARE_DEEP];
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) p[u] = c0 + 32 * u <= full && c0 + 32 * u < A.width ? from[c0 + 32 * u] : -1;
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) {
+                    const int c = c0 + 32 * u;
+                    if (c >= A.width) continue;
+                    if (c < full && p[u] >= 0 && p[u] < A.n_pages) atomicAdd(A.shared + p[u], 1);
+                    to[c] = c < full ? p[u] : c == full && page != -2 ? page : -1;
+                    if (c == full) A.src[f0 + i] = page != -2 ? p[u] : -1;
+                }
             }
             if (lane == 0) {
                 if (full == A.width) A.src[f0 + i] = -1;
@@ -130,24 +139,53 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = max(0, min(*A.count, A.n_pages));
     auto from = [&](int r) { return A.held ? (int)min((int64_t)A.width, ((int64_t)max(A.held[r], 0) + A.page_size - 1) / A.page_size) : 0; };
-    // every page of row r that is one, and its entry's number; whole warps
+    // the pages of row r, SHARE_DEEP a lane at a time: f(first column of this lane, pages, -1 what is none); whole warps
     auto each = [&](int r, auto&& f) {
         const int32_t* const row = A.table + r * A.table_stride;
-        for (int c0 = from(r); c0 < A.width; c0 += 32) {
-            const int c = c0 + lane, p = c < A.width ? row[c] : -1;
-            f(p >= 0 && p < A.n_pages, p, r * A.width + c, c);
+        for (int c0 = from(r); c0 < A.width; c0 += 32 * SHARE_DEEP) {
+            int p[SHARE_DEEP];
+#pragma unroll
+            for (int u = 0; u < SHARE_DEEP; u++) {
+                const int c = c0 + lane + 32 * u;
+                p[u] = c < A.width ? row[c] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < SHARE_DEEP; u++) p[u] = p[u] < A.n_pages ? p[u] : -1;
+            f(c0 + lane, p);
         }
     };
-    auto goes = [&](bool there, int p, int e) { return there && A.first[p] == e && A.times[p] > A.shared[p]; };
+    using Pages = const int (&)[SHARE_DEEP];
+    // whether entry e names its page first, and with how many others beyond what shared says (NEVER: not)
+    constexpr int NEVER = INT_MIN;
+    auto look = [&](int r, int c, Pages p, int (&more)[SHARE_DEEP], int (&times)[SHARE_DEEP]) {
+        bool mine[SHARE_DEEP];
+#pragma unroll
+        for (int u = 0; u < SHARE_DEEP; u++) mine[u] = p[u] >= 0 && A.first[p[u]] == r * A.width + c + 32 * u;
+#pragma unroll
+        for (int u = 0; u < SHARE_DEEP; u++) { times[u] = mine[u] ? A.times[p[u]] : 0; more[u] = mine[u] ? times[u] - A.shared[p[u]] : NEVER; }
+    };
     for (int r = me; r < A.R; r += all)
-        if (A.done[r]) each(r, [&](bool there, int p, int, int) { if (there) { A.times[p] = 0; A.first[p] = 0x7fffffff; } });
+        if (A.done[r]) each(r, [&](int, Pages p) {
+#pragma unroll
+            for (int u = 0; u < SHARE_DEEP; u++)
+                if (p[u] >= 0) { A.times[p[u]] = 0; A.first[p[u]] = 0x7fffffff; }
+        });
     meet(blocks);
     for (int r = me; r < A.R; r += all)
-        if (A.done[r]) each(r, [&](bool there, int p, int e, int) { if (there) { atomicAdd(A.times + p, 1); atomicMin(A.first + p, e); } });
+        if (A.done[r]) each(r, [&](int c, Pages p) {
+#pragma unroll
+            for (int u = 0; u < SHARE_DEEP; u++)
+                if (p[u] >= 0) { atomicAdd(A.times + p[u], 1); atomicMin(A.first + p[u], r * A.width + c + 32 * u); }
+        });
     meet(blocks);
     for (int r = me; r < A.R; r += all) {
         int n = 0;
-        if (A.done[r]) each(r, [&](bool there, int p, int e, int) { n += __popc(__ballot_sync(0xffffffffu, goes(there, p, e))); });
+        if (A.done[r]) each(r, [&](int c, Pages p) {
+            int more[SHARE_DEEP], times[SHARE_DEEP];
+            look(r, c, p, more, times);
+#pragma unroll
+            for (int u = 0; u < SHARE_DEEP; u++) n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
+        });
         if (lane == 0) A.gives[r] = n;
     }
     meet(blocks);
@@ -164,14 +202,18 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
             if (!A.done[r]) continue;
             int at = before[r - r0];
             int32_t* const row = A.table + r * A.table_stride;
-            each(r, [&](bool there, int p, int e, int c) {
-                const bool mine = there && A.first[p] == e, go = mine && A.times[p] > A.shared[p];
-                const uint32_t yes = __ballot_sync(0xffffffffu, go);
-                const int slot = at + __popc(yes & ((1u << lane) - 1u));
-                if (go && slot < A.n_pages) A.pages[slot] = p;
-                if (mine) A.shared[p] = max(A.shared[p] - A.times[p], 0);
-                if (c < A.width) row[c] = -1;
-                at += __popc(yes);
+            each(r, [&](int c, Pages p) {
+                int more[SHARE_DEEP], times[SHARE_DEEP];
+                look(r, c, p, more, times);
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) {
+                    const uint32_t yes = __ballot_sync(0xffffffffu, more[u] > 0);
+                    const int slot = at + __popc(yes & ((1u << lane) - 1u));
+                    if (more[u] > 0 && slot < A.n_pages) A.pages[slot] = p[u];
+                    if (more[u] != NEVER) A.shared[p[u]] = max(-more[u], 0);
+                    if (c + 32 * u < A.width) row[c + 32 * u] = -1;
+                    at += __popc(yes);
+                }
             });
         }
         top += total;
@@ -292,14 +334,14 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const C
 }
 
 // ------------------------------------------------------------------ copies
-constexpr int COPY_CACHES = 256, COPY_THREADS = 256, COPY_DEEP = 4;
+constexpr int COPY_CACHES = 256, COPY_THREADS = 256, COPY_DEEP = 8;
 struct CopyArgs {
     const int32_t *src, *dst; int n; int n_caches, n_pages;
     int64_t page_stride, page_bytes;                           // bytes
     int pieces; int64_t piece_bytes;                           // of a page
     uint8_t* caches[COPY_CACHES];
 };
-// page src[i] to page dst[i] of every cache: a piece of a page a block at a time, 64 bytes a thread in flight
+// page src[i] to page dst[i] of every cache: a piece of a page a block at a time, 128 bytes a thread in flight
 template <typename U>
 __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(const __grid_constant__ CopyArgs A) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
