@@ -311,7 +311,7 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *x = plain(a[0]), *tokens = plain(a[1]);
     int64_t k;
     double temperature;
-    if (!x || x->dim() != 2 || float_code(*x) < 0 || wants_grad(*x) || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature > 0.0) || !(temperature < INFINITY))
+    if (!x || x->dim() != 2 || float_code(*x) < 0 || wants_grad(*x) || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature >= 1e-7) || !(temperature <= 1e7))
         Py_RETURN_NONE;
     const int64_t rows = x->size(0), V = x->size(1);
     if (rows <= 0 || V <= 0 || k < 0 || k > 32 || k > V || (V > 1 && x->stride(1) != 1) || (rows > 1 && x->stride(0) < V) || !ints(tokens, rows, at::kLong, *x)) Py_RETURN_NONE;

@@ -12,7 +12,7 @@ using namespace lowbit;
 namespace lowbit {
 namespace {
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_MOST = 32, LP_ROOM = 512;
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_MOST = 32, LP_ROOM = 512, LP_RESIDENT = 5;
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -24,27 +24,54 @@ struct LogprobArgs {
 // A row's stats, for the gradient: ref and m of an element's exponent u = (x - ref) c - m, base 2 (ref is 0 but in rows whose products pass 32 bits);
 // the sum of the powers; the mean of the exponents under them
 
-template <typename T> struct Vec;                              // 16 bytes of logits
+// 16 bytes of logits.  floored: none below kFloor, so that the product of a power of 0 with its exponent is 0; fp16 has no number that is low enough at
+// every temperature, and its exponents are bounded one by one (kBound)
+template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int N = 4;
+    static constexpr float kFloor = -1e30f;
+    static constexpr bool kBound = false;
     static __device__ __forceinline__ void get(const uint4& w, float (&x)[4]) { x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w); }
+    static __device__ __forceinline__ void floored(const uint4& w, float (&x)[4]) {
+        get(w, x);
+#pragma unroll
+        for (int i = 0; i < 4; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(x[i]) : "f"(kFloor));
+    }
 };
 template <> struct Vec<__half> {
     static constexpr int N = 8;
+    static constexpr float kFloor = -INFINITY;
+    static constexpr bool kBound = true;
     static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(v + i)); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
     }
+    static __device__ __forceinline__ void floored(const uint4& w, float (&x)[8]) { get(w, x); }
 };
 template <> struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr float kFloor = -0x1.92p99f;               // -1e30 in its 16 bits, 0xf149
+    static constexpr bool kBound = false;
     static __device__ __forceinline__ void get(const uint4& w, float (&x)[8]) {
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(v[i] << 16); x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
     }
+    static __device__ __forceinline__ void floored(uint4 w, float (&x)[8]) {
+        uint32_t* const v[4] = {&w.x, &w.y, &w.z, &w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(*v[i]) : "r"(0xf149f149u));
+        get(w, x);
+    }
 };
+
+// two 32-bit numbers by one instruction
+struct Two { uint64_t v; };
+__device__ __forceinline__ Two two(float a, float b) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void apart(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) { Two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ Two add(Two a, Two b) { Two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -58,26 +85,30 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// a reference for exponents, the sum of powers, and of powers x exponents, relative to it; the largest logit
-struct Sums {
-    float m, s, d, big;
-    __device__ __forceinline__ void add(const Sums& o) {
-        const float to = fmaxf(m, o.m);
-        const float a = m == to ? 0.0f : m - to, b = o.m == to ? 0.0f : o.m - to;
-        const float wa = ex2(a), wb = ex2(b);
-        // a side that holds nothing has m = -inf: weight 0
-        d = (s == 0.0f ? 0.0f : wa * fmaf(s, a, d)) + (o.s == 0.0f ? 0.0f : wb * fmaf(o.s, b, o.d));
-        s = (s == 0.0f ? 0.0f : wa * s) + (o.s == 0.0f ? 0.0f : wb * o.s);
-        m = to;
-        big = fmaxf(big, o.big);
+// a reference for exponents, the sum of powers, and of powers x exponents, relative to it
+struct __align__(16) Sums { float m, s, d; };
+// those of the first `lanes` (a power of two) lanes together, in every one of them the same
+__device__ __forceinline__ Sums together(Sums x, int lanes) {
+    float m = x.m;
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    // a lane that holds nothing has m = -inf, and one whose weight is 0 holds nothing that counts, but for NaN
+    const float a = x.m - m, w = x.m == -INFINITY ? 0.0f : ex2(a);
+    x.d = w == 0.0f ? 0.0f : w * fmaf(x.s, a, x.d);
+    x.s = w != 0.0f ? w * x.s : x.s == x.s ? 0.0f : x.s;
+    for (int d = lanes / 2; d; d >>= 1) {
+        x.s += __shfl_xor_sync(0xffffffffu, x.s, d);
+        x.d += __shfl_xor_sync(0xffffffffu, x.d, d);
     }
-};
+    x.m = m;
+    return x;
+}
 
 // order of the alternatives: larger value first, then lower index.  -0 equals 0; key 0 is nobody's
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
     const uint32_t b = __float_as_uint(x + 0.0f), o = (int)b < 0 ? ~b : b | 0x80000000u;
     return (uint64_t)o << 32 | (0xffffffffu - i);
 }
+__device__ __forceinline__ float key_value(uint64_t k) { const uint32_t o = (uint32_t)(k >> 32); return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
 
 // one value a lane, sorted over the warp, the largest in lane 0
@@ -128,36 +159,34 @@ template <typename T> struct Strip {
 };
 template <typename T> __device__ __forceinline__ float one(const T* p) { return to_float<T>(*p); }
 
-// the k-th largest of the threads' values: a lower bound of the k-th largest element
-__device__ __forceinline__ float kth_of_threads(float x, int k, uint32_t (*lists)[32], float* out) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// a value that k threads reach at least, and so k elements: the least of the k / full-th largest values (rounded up) of the first `full` warps
+__device__ __forceinline__ float reached_by(float x, int k, int full, uint32_t* warps) {
+    if (full == 0) return -INFINITY;
+    const int lane = threadIdx.x & 31;
     const uint32_t b = __float_as_uint(x + 0.0f);
-    uint32_t key = sort32((int)b < 0 ? ~b : b | 0x80000000u);
-    lists[warp][lane] = key;
-#pragma unroll
-    for (int n = LP_WARPS / 2; n; n >>= 1) {
-        __syncthreads();
-        if (warp < n) {
-            key = merge32(key, lists[warp + n][lane]);
-            lists[warp][lane] = key;
-        }
+    uint32_t key = (int)b < 0 ? ~b : b | 0x80000000u, top = 0;
+    for (int left = (k + full - 1) / full; left; left--) {
+        top = __reduce_max_sync(0xffffffffu, key);
+        const uint32_t has = __ballot_sync(0xffffffffu, key == top);
+        if (lane == __ffs(has) - 1) key = 0;
     }
-    if (warp == 0 && lane == k - 1) *out = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    if (lane == 0) warps[threadIdx.x >> 5] = top;
     __syncthreads();
-    return *out;
+    uint32_t least = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < LP_WARPS; w++) least = w < full ? min(least, warps[w]) : least;
+    return __uint_as_float(least & 0x80000000u ? least & 0x7fffffffu : ~least);
 }
 
 // blocks of a cluster share a row.  What bounds it: see the launch below
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const LogprobArgs A) {
+__global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel(const LogprobArgs A) {
     constexpr int N = Vec<T>::N;
     __shared__ Sums warps[LP_WARPS];
-    __shared__ __align__(16) Sums mine;                        // read by the cluster's first block
-    __shared__ Sums total;
+    __shared__ Sums mine;                                      // read by the cluster's first block
     __shared__ uint64_t found[TOP ? LP_ROOM : 1];
     __shared__ uint64_t lists[TOP ? LP_WARPS : 1][32];
     __shared__ uint64_t best[32];                              // as `mine`
-    __shared__ float level;
     __shared__ int n_found;
     __shared__ uint32_t owners[LP_WARPS];
     __shared__ uint8_t owner[LP_THREADS];
@@ -172,68 +201,111 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
+    int64_t token = -1;                                        // the first thread's, asked for ahead: it leads to another load
+    float token_logit = 0.0f;
+    if (rank == 0 && t == 0) {
+        token = A.tokens[r];
+        if (token >= 0 && token < A.V) token_logit = one(row + token);
+        else token = -1;
+    }
     // ---- the pass
-    Sums x = {-INFINITY, 0.0f, 0.0f, -INFINITY};
-    auto take = [&](const float (&v)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) x.big = max3(x.big, v[i], v[i + 1]);
+    float m = -INFINITY, big = -INFINITY;                      // the reference; this thread's largest logit
+    Two sum = two(0.0f, 0.0f), dot = sum;                      // of powers, and of powers x exponents
+    const Two c2 = two(c, c);
+    auto follow = [&]() {
         // the reference follows where an exponent would pass 2^20 of it: sums of powers up to that are as exact as those up to 1
-        const float top = x.big * c;
-        if (top > x.m + 20.0f) {
-            const float a = x.m - top, w = ex2(a);
-            x.d = x.s == 0.0f ? 0.0f : w * fmaf(x.s, a, x.d);
-            x.s = x.s == 0.0f ? 0.0f : w * x.s;
-            x.m = top;
+        const float top = big * c;
+        if (top > m + 20.0f && big > Vec<T>::kFloor) {
+            const float a = m - top, w = ex2(a);
+            if (w == 0.0f) {
+                // nothing that counts so far.  (The exponents of logits beyond 2^24 have lost their differences: whatever they gave goes, but for NaN)
+                float p, q;
+                apart(sum, p, q);
+                sum = two(p == p ? 0.0f : p, q == q ? 0.0f : q);
+                dot = two(0.0f, 0.0f);
+            } else {
+                const Two w2 = two(w, w);
+                dot = fma(w2, fma(sum, two(a, a), dot), two(0.0f, 0.0f));
+                sum = fma(w2, sum, two(0.0f, 0.0f));
+            }
+            m = top;
         }
-        const float ref = x.m == -INFINITY ? 0.0f : x.m;       // nothing but -inf so far
-        float s0 = 0.0f, s1 = 0.0f, d0 = 0.0f, d1 = 0.0f;
+        return m == -INFINITY ? 0.0f : -m;                     // nothing above the floor so far
+    };
+    auto take = [&](const float* v, int n) {                   // n: a constant
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float a = fmaf(v[i], c, -ref), b = fmaf(v[i + 1], c, -ref), ea = ex2(a), eb = ex2(b);
-            s0 += ea; s1 += eb;
-            d0 = fmaf(ea, fmaxf(a, -300.0f), d0);              // a power of 0 adds 0, not 0 x inf
-            d1 = fmaf(eb, fmaxf(b, -300.0f), d1);
+        for (int i = 0; i < n; i += 2) big = max3(big, v[i], v[i + 1]);
+        const float r0 = follow();
+        const Two ref = two(r0, r0);
+#pragma unroll
+        for (int i = 0; i < n; i += 2) {
+            Two u = fma(two(v[i], v[i + 1]), c2, ref);
+            float a, b;
+            apart(u, a, b);
+            const Two e = two(ex2(a), ex2(b));
+            if (Vec<T>::kBound) u = two(fmaxf(a, -300.0f), fmaxf(b, -300.0f));
+            sum = add(sum, e);
+            dot = fma(e, u, dot);
         }
-        x.s += s0 + s1;
-        x.d += d0 + d1;
     };
     constexpr int AHEAD = 4;
-    for (int i = strip.first + t; i < strip.last; i += AHEAD * LP_THREADS) {
+    int next = strip.first + t;
+#pragma unroll 1
+    for (; next + (AHEAD - 1) * LP_THREADS < strip.last; next += AHEAD * LP_THREADS) {
         uint4 w[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++)
-            if (i + a * LP_THREADS < strip.last) w[a] = strip.piece(i + a * LP_THREADS);
+        for (int a = 0; a < AHEAD; a++) w[a] = strip.piece(next + a * LP_THREADS);
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++)
-            if (i + a * LP_THREADS < strip.last) { float v[N]; Vec<T>::get(w[a], v); take(v); }
+        for (int a = 0; a < AHEAD; a += 2) {
+            float v[2 * N];
+            Vec<T>::floored(w[a], *reinterpret_cast<float(*)[N]>(v));
+            Vec<T>::floored(w[a + 1], *reinterpret_cast<float(*)[N]>(v + N));
+            take(v, 2 * N);
+        }
+    }
+    {
+        // what is left of the pieces, asked for at once
+        uint4 w[AHEAD - 1];
+#pragma unroll
+        for (int a = 0; a < AHEAD - 1; a++)
+            if (next + a * LP_THREADS < strip.last) w[a] = strip.piece(next + a * LP_THREADS);
+#pragma unroll 1
+        for (int a = 0; a < AHEAD - 1; a++) {
+            if (next + a * LP_THREADS >= strip.last) break;
+            float v[N];
+            Vec<T>::floored(a == 0 ? w[0] : a == 1 ? w[1] : w[2], v);
+            take(v, N);
+        }
     }
     const int end = strip.end_of(t);
     if (end >= 0) {
-        float v[N];
-        v[0] = one(row + end);
-#pragma unroll
-        for (int e = 1; e < N; e++) v[e] = -INFINITY;
-        take(v);
+        float v = one(row + end);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(Vec<T>::kFloor));
+        big = fmaxf(big, v);
+        const float u = fmaf(v, c, follow()), e = ex2(u);
+        sum = add(sum, two(e, 0.0f));
+        dot = add(dot, two(e * (Vec<T>::kBound ? fmaxf(u, -300.0f) : u), 0.0f));
     }
 
     // ---- the block's sums, and the cluster's
-    const float own_big = x.big;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        Sums o = {__shfl_xor_sync(0xffffffffu, x.m, d), __shfl_xor_sync(0xffffffffu, x.s, d), __shfl_xor_sync(0xffffffffu, x.d, d), __shfl_xor_sync(0xffffffffu, x.big, d)};
-        // in the order of the lanes on both sides, so that both hold the same
-        Sums lo = lane & d ? o : x, hi = lane & d ? x : o;
-        lo.add(hi);
-        x = lo;
+    Sums x = {m, 0.0f, 0.0f};
+    {
+        float a, b;
+        apart(sum, a, b);
+        x.s = a + b;
+        apart(dot, a, b);
+        x.d = a + b;
     }
+    x = together(x, 32);
     if (lane == 0) warps[warp] = x;
     if (t == 0) n_found = 0;
-    if (!TOP) __syncthreads();
 
     if (TOP) {
         // ---- the strips in which the k largest lie, read again
-        const float floor_ = kth_of_threads(own_big, A.k, reinterpret_cast<uint32_t(*)[32]>(&lists[0][0]), &level);
-        const uint32_t own = __ballot_sync(0xffffffffu, own_big >= floor_);
+        const float reached = reached_by(big, A.k, min(strip.last - strip.first, LP_THREADS) / 32, owners);
+        const float floor_ = reached > Vec<T>::kFloor ? reached : -INFINITY;                   // what is below the floor was read as that
+        __syncthreads();                                       // everybody has read the warps' values
+        const uint32_t own = __ballot_sync(0xffffffffu, big >= floor_);
         if (lane == 0) owners[warp] = own;
         __syncthreads();
         int strips = 0, before = 0;
@@ -241,32 +313,37 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
         for (int w = 0; w < LP_WARPS; w++) { const int c_ = __popc(owners[w]); strips += c_; before += w < warp ? c_ : 0; }
         if (own >> lane & 1) owner[before + __popc(own & ((1u << lane) - 1u))] = (uint8_t)t;
         __syncthreads();
-        auto note = [&](float v, int at) {
-            if (v >= floor_) {
-                const int slot = atomicAdd(&n_found, 1);       // their order does not matter: they are sorted
-                if (slot < LP_ROOM) found[slot] = key_of(v, (uint32_t)at);
-            }
+        auto note = [&](int at) {
+            const int slot = atomicAdd(&n_found, 1);           // their order does not matter: they are sorted
+            if (slot < LP_ROOM) found[slot] = key_of(one(row + at), (uint32_t)at);
         };
         const int deep = (strip.last - strip.first + LP_THREADS - 1) / LP_THREADS;             // pieces of a strip
-        for (int i = t; i < strips * deep; i += AHEAD * LP_THREADS) {
-            uint4 w[AHEAD];
-            int p[AHEAD];
+#pragma unroll 1
+        for (int i = t; i < strips * deep; i += 2 * LP_THREADS) {
+            uint4 w[2];
+            int p[2];
 #pragma unroll
-            for (int a = 0; a < AHEAD; a++) {
+            for (int a = 0; a < 2; a++) {
                 const int u = i + a * LP_THREADS, s = u / deep;
                 p[a] = s < strips ? strip.first + owner[s] + (u - s * deep) * LP_THREADS : strip.last;
                 if (p[a] < strip.last) w[a] = strip.piece(p[a]);
             }
+            uint32_t hits = 0;
 #pragma unroll
-            for (int a = 0; a < AHEAD; a++)
+            for (int a = 0; a < 2; a++)
                 if (p[a] < strip.last) {
                     float v[N];
                     Vec<T>::get(w[a], v);
 #pragma unroll
-                    for (int e = 0; e < N; e++) note(v[e], strip.base() + p[a] * N + e);
+                    for (int e = 0; e < N; e++) hits |= v[e] >= floor_ ? 1u << (8 * a + e) : 0u;
                 }
+#pragma unroll 1
+            for (; hits; hits &= hits - 1) {
+                const int e = __ffs(hits) - 1;
+                note(strip.base() + (e < 8 ? p[0] : p[1]) * N + (e & 7));
+            }
         }
-        if (end >= 0) note(one(row + end), end);
+        if (end >= 0 && one(row + end) >= floor_) note(end);
         __syncthreads();
         const int n = n_found;
         uint64_t key = 0;
@@ -301,22 +378,19 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
                 keep(at >= 0 ? one(row + at) : 0.0f, at, at >= 0);
             }
         }
-        if (n > 32) {                                          // else the first warp has them all
+        // the lists of as many warps as have one, to the first
+        const int n_lists = n <= LP_ROOM ? min((n + 31) / 32, LP_WARPS) : LP_WARPS;
+        if (n_lists > 1) {
             lists[warp][lane] = key;
-#pragma unroll
-            for (int h = LP_WARPS / 2; h; h >>= 1) {
-                __syncthreads();
-                if (warp < h) {
-                    key = merge32(key, lists[warp + h][lane]);
-                    lists[warp][lane] = key;
-                }
-            }
+            __syncthreads();
+            if (warp == 0)
+                for (int w = 1; w < n_lists; w++) key = merge32(key, lists[w][lane]);
         }
         if (warp == 0) best[lane] = key;
-    }
-    if (t == 0) {
-        for (int w = 1; w < LP_WARPS; w++) x.add(warps[w]);
-        mine = x;
+    } else __syncthreads();
+    if (warp == 0) {
+        x = together(lane < LP_WARPS ? warps[lane] : Sums{-INFINITY, 0.0f, 0.0f}, LP_WARPS);
+        if (lane == 0) mine = x;
     }
     __syncthreads();
     if (blocks > 1) {
@@ -324,34 +398,51 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     if (rank == 0) {
-        // the first block's first warp: the others' sums and lists, in their order
+        // the first block: the others' sums and lists, a warp each
         uint64_t key = 0;
-        if (warp == 0) {
-            const uint32_t at_mine = (uint32_t)__cvta_generic_to_shared(&mine), at_best = (uint32_t)__cvta_generic_to_shared(&best[lane]);
-            Sums all = mine;
-            if (TOP) key = best[lane];
-            for (uint32_t b = 1; b < blocks; b++) {
+        Sums all = mine;
+        if (blocks > 1) {
+            if (warp < (int)blocks) {
+                const uint32_t at_mine = (uint32_t)__cvta_generic_to_shared(&mine), at_best = (uint32_t)__cvta_generic_to_shared(&best[lane]);
                 uint32_t p;
-                Sums o;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at_mine), "r"(b));
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.m), "=f"(o.s), "=f"(o.d), "=f"(o.big) : "r"(p) : "memory");
-                all.add(o);
+                if (lane == 0) {
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at_mine), "r"(warp));
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(all.m), "=f"(all.s) : "r"(p) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1 + 8];" : "=f"(all.d) : "r"(p) : "memory");
+                    warps[warp] = all;
+                }
                 if (TOP) {
-                    uint64_t other;
-                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at_best), "r"(b));
-                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(other) : "r"(p) : "memory");
-                    key = merge32(key, other);
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(at_best), "r"(warp));
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(p) : "memory");
+                    lists[warp][lane] = key;
                 }
             }
-            if (lane == 0) total = all;
-        }
-        __syncthreads();
-        Sums all = total;
+            __syncthreads();
+            if (TOP) {
+#pragma unroll
+                for (int h = 4; h; h >>= 1) {
+                    if (warp < h && warp + h < (int)blocks) {
+                        key = merge32(key, lists[warp + h][lane]);
+                        lists[warp][lane] = key;
+                    }
+                    __syncthreads();
+                }
+            }
+            all = together(lane < (int)blocks ? warps[lane] : Sums{-INFINITY, 0.0f, 0.0f}, LP_WARPS);
+            all = {__shfl_sync(0xffffffffu, all.m, 0), __shfl_sync(0xffffffffu, all.s, 0), __shfl_sync(0xffffffffu, all.d, 0)};
+        } else if (TOP) key = best[lane];
         float ref = 0.0f;
         if (!(fabsf(all.m) < 16777216.0f)) {
-            // the products have lost the logits' differences, or passed 32 bits: the row once more, the largest logit taken off first.  A row of the
+            // the products have lost the logits' differences, or passed 32 bits: the row twice more, the largest logit taken off first.  A row of the
             // type's lowest value is even; one of -inf alone, or with inf in it, has no probabilities
-            ref = all.big;
+            for (int j = t; j < A.V; j += LP_THREADS) ref = j == t ? one(row + j) : fmaxf(ref, one(row + j));
+            if (t >= A.V) ref = -INFINITY;
+#pragma unroll
+            for (int h = 16; h; h >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, h));
+            __syncthreads();                                   // everybody has read the warps' sums
+            if (lane == 0) warps[warp].m = ref;
+            __syncthreads();
+            for (int w = 0; w < LP_WARPS; w++) ref = fmaxf(ref, warps[w].m);
             float s = fabsf(ref) < INFINITY ? 0.0f : NAN, d = 0.0f;
             for (int j = t; j < A.V; j += LP_THREADS) {
                 const float a = (one(row + j) - ref) * c, e = ex2(a);
@@ -360,9 +451,10 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
             }
 #pragma unroll
             for (int h = 16; h; h >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, h); d += __shfl_xor_sync(0xffffffffu, d, h); }
-            if (lane == 0) warps[warp] = {0.0f, s, d, ref};
+            __syncthreads();                                   // everybody has read the warps' sums
+            if (lane == 0) warps[warp] = {0.0f, s, d};
             __syncthreads();
-            all = {0.0f, 0.0f, 0.0f, ref};
+            all = {0.0f, 0.0f, 0.0f};
             for (int w = 0; w < LP_WARPS; w++) { all.s += warps[w].s; all.d += warps[w].d; }
         }
         const float log2s = log2f(all.s);
@@ -372,15 +464,13 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
             return u == -INFINITY ? fmaf(v - ref, A.by, -(all.m + log2s) * LP_LN2) : (u - log2s) * LP_LN2;
         };
         if (t == 0) {
-            const int64_t token = A.tokens[r];
-            A.logp[r] = token >= 0 && token < A.V ? logp(one(row + token)) : 0.0f;
+            A.logp[r] = token >= 0 ? logp(token_logit) : 0.0f;
             A.entropy[r] = (log2s - all.d / all.s) * LP_LN2;
             if (A.stats) A.stats[r] = make_float4(ref, all.m, all.s, all.d / all.s);
         }
         if (TOP && t < A.k) {
-            const uint32_t id = key_index(key);
-            A.ids[r * A.k + t] = key ? (int64_t)id : -1;       // a row with fewer numbers than that
-            A.top[r * A.k + t] = key ? logp(one(row + id)) : NAN;
+            A.ids[r * A.k + t] = key ? (int64_t)key_index(key) : -1;       // a row with fewer numbers than that
+            A.top[r * A.k + t] = key ? logp(key_value(key)) : NAN;
         }
     }
     __syncwarp();
@@ -486,22 +576,36 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_grad_kernel(const L
 }
 
 bool bad_logits(const char* name, const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t V, const void* tokens, float temperature, int k) {
-    const bool bad = !logits || dtype < 0 || dtype > 2 || rows < 0 || V <= 0 || V > 0x7fff0000ll || row_stride < V || !tokens || !(temperature > 0.0f) || !(temperature < INFINITY) ||
+    const bool bad = !logits || dtype < 0 || dtype > 2 || rows < 0 || V <= 0 || V > 0x7fff0000ll || row_stride < V || !tokens || !(temperature >= 0.99e-7f) || !(temperature <= 1.01e7f) ||
                      k < 0 || k > LP_MOST || k > V || rows > 0x3ffffffll || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1));
     if (bad) set_error(LB_ERR_ARG, "%s: bad argument (rows %lld, vocabulary %lld, dtype %d, top_k %d)", name, (long long)rows, (long long)V, dtype, k);
     return bad;
 }
 
 template <typename T> int logprobs_launch(const LogprobArgs& A, cudaStream_t st) {
-    // blocks of a row: as many as are resident at once, five an SM, each with a piece a thread at least
-    int64_t blocks = A.rows < 5ll * sm_count() ? 5ll * sm_count() / A.rows : 1;
-    if (blocks > 8) blocks = 8;
-    if (blocks > A.V / (LP_THREADS * Vec<T>::N)) blocks = A.V / (LP_THREADS * Vec<T>::N);
-    if (blocks < 1) blocks = 1;
+    // blocks of a row, each with a piece a thread at least: of the numbers with which all are resident at once the one that leaves the fewest places empty
+    int64_t blocks = 1, most = A.V / (LP_THREADS * Vec<T>::N);
+    double best = 0.0;
+    for (int64_t b = 1; b <= 8 && (b == 1 || b <= most) && (b == 1 || A.rows * b <= (int64_t)LP_RESIDENT * sm_count()); b++) {
+        const int64_t n = A.rows * b, deep = (n + sm_count() - 1) / sm_count();
+        const double used = (double)n / (double)(deep * sm_count());
+        if (used >= best) { best = used; blocks = b; }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(A.rows * blocks));
     cfg.blockDim = dim3(LP_THREADS);
     cfg.stream = st;
+    // shared memory that nobody uses keeps an SM from taking more of them than its share while others have none left
+    static bool configured[64] = {};                           // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        cudaFuncSetAttribute(token_logprobs_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        cudaFuncSetAttribute(token_logprobs_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        configured[dev & 63] = true;
+    }
+    const int64_t deep = (A.rows * blocks + sm_count() - 1) / sm_count();
+    if (deep > 1 && deep < LP_RESIDENT) cfg.dynamicSmemBytes = (size_t)(216 / (int)deep - 10) * 1024;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};

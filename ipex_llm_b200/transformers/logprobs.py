@@ -1,7 +1,6 @@
 """What a row of logits says about its tokens: the log probability of a given token, the entropy, the most likely alternatives -- what a server
 answers beside its tokens (the reference's serving engine returns them with each; the greedy pick of the recorded decode step reads the same logits)
 and what a loss on token probabilities is made of, with its gradient."""
-import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -81,7 +80,7 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
                       f"tokens must be int64 {list(logits.shape[:-1])} on the logits' device")
     top_k, temperature, V = int(top_k), float(temperature), logits.shape[-1]
     invalidInputError(0 <= top_k <= min(TOP_MOST, V), f"top_k must be between 0 and {min(TOP_MOST, V)}")
-    invalidInputError(temperature > 0 and math.isfinite(temperature), "the temperature must be positive")
+    invalidInputError(1e-7 <= temperature <= 1e7, "the temperature must be between 1e-7 and 1e7")
     shape = tokens.shape
     rows = logits.reshape(-1, V)
     if rows.shape[0] > 1 and (rows.stride(1) != 1 or rows.stride(0) < V) or V > 1 and rows.stride(1) != 1:

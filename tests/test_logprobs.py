@@ -95,6 +95,36 @@ def test_orders_and_ties(lp, cuda_device, dtype, V, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [300, 40001])
+@pytest.mark.parametrize("low", [-1e4, -1e9, -1e12, -1e25, -1e29, -3e30, -1e37])
+def test_masks_of_large_numbers(lp, cuda_device, dtype, V, low):
+    """what masks are written with: numbers whose exponents have lost their differences, in front of the others, behind them, and alone"""
+    logits, tokens = make(6, V, dtype, cuda_device)
+    logits[0, :V // 2] = low
+    logits[1, V // 2:] = low
+    logits[2, torch.arange(V, device=cuda_device) % 3 > 0] = low
+    logits[3] = low
+    logits[4] = low
+    logits[4, V // 3] = low / 2
+    logits[5, 1:] = low
+    tokens[:] = V // 3
+    check(lp.token_logprobs(logits, tokens, 9, 1.0), logits, tokens, 9, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1e-7, 1e-3, 30.0, 1e7])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_temperatures(lp, cuda_device, dtype, temperature):
+    logits, tokens = make(5, 3001, dtype, cuda_device, masked=0.3)
+    logits[3] = torch.finfo(dtype).min
+    logits[4, 7:] = torch.finfo(dtype).min
+    logits[4, :7] = torch.arange(7) / 8
+    tokens[3:] = 5
+    check(lp.token_logprobs(logits, tokens, 6, temperature), logits, tokens, 6, temperature)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [300, 40001])
 def test_masks_infinities_and_nan(lp, cuda_device, dtype, V):
@@ -304,7 +334,7 @@ def test_refusals(lp, cuda_device):
     x, t = torch.zeros(4, 50, device=cuda_device), torch.zeros(4, dtype=torch.int64, device=cuda_device)
     for call in (lambda: lp.token_logprobs(x.double(), t), lambda: lp.token_logprobs(x, t.int()), lambda: lp.token_logprobs(x, t[:3]), lambda: lp.token_logprobs(x, t.cpu()),
                  lambda: lp.token_logprobs(x, t, 33), lambda: lp.token_logprobs(x[:, :5], t, 6), lambda: lp.token_logprobs(x, t, -1), lambda: lp.token_logprobs(x, t, 0, 0.0),
-                 lambda: lp.token_logprobs(x, t, 0, -1.0), lambda: lp.token_logprobs(x, t, 0, math.inf), lambda: lp.token_logprobs(x, t, 0, math.nan), lambda: lp.token_logprobs(x[:, :0], t)):
+                 lambda: lp.token_logprobs(x, t, 0, -1.0), lambda: lp.token_logprobs(x, t, 0, math.inf), lambda: lp.token_logprobs(x, t, 0, 1e-9), lambda: lp.token_logprobs(x, t, 0, 1e9), lambda: lp.token_logprobs(x, t, 0, math.nan), lambda: lp.token_logprobs(x[:, :0], t)):
         with pytest.raises(RuntimeError):
             call()
     leaf = x.clone().requires_grad_()
