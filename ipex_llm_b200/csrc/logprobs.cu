@@ -595,17 +595,6 @@ template <typename T> int logprobs_launch(const LogprobArgs& A, cudaStream_t st)
     cfg.gridDim = dim3((unsigned)(A.rows * blocks));
     cfg.blockDim = dim3(LP_THREADS);
     cfg.stream = st;
-    // shared memory that nobody uses keeps an SM from taking more of them than its share while others have none left
-    static bool configured[64] = {};                           // the attribute is per device
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!configured[dev & 63]) {
-        cudaFuncSetAttribute(token_logprobs_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-        cudaFuncSetAttribute(token_logprobs_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
-        configured[dev & 63] = true;
-    }
-    const int64_t deep = (A.rows * blocks + sm_count() - 1) / sm_count();
-    if (deep > 1 && deep < LP_RESIDENT) cfg.dynamicSmemBytes = (size_t)(216 / (int)deep - 10) * 1024;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};
