@@ -56,12 +56,12 @@ struct ForkArgs {
     int32_t *src, *dst, *missing;
 };
 
-// One block or a cluster; every block finds for itself which forks need a page (a round of a thread each), then a warp takes a fork at a time.
-__global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const ForkArgs A) {
+// Every block finds for itself which forks need a page (a round of a thread each), then a warp takes a fork at a time.  The count is read by all, and may
+// be written in place: by the one block that there is, or (`last` false) by a launch behind.
+__global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const ForkArgs A, bool last) {
     __shared__ int warps[32];
     __shared__ int fresh[SHARE_THREADS];                       // the page of a fork of this round, -1: none to be had, -2: it needs none
-    const uint32_t rank = cluster_rank(), blocks = cluster_blocks();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rank = blockIdx.x, blocks = gridDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = max(0, min(*A.count, A.n_pages));
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const Fork
         taken += total;
         __syncthreads();
         // lens of parents are read above and below, and children's written below: no row is both
-        for (int i = (int)rank * SHARE_WARPS + warp; i < min(SHARE_THREADS, A.F - f0); i += (int)blocks * SHARE_WARPS) {
+        for (int i = warp * blocks + rank; i < min(SHARE_THREADS, A.F - f0); i += blocks * SHARE_WARPS) {
             const int par = A.parents[f0 + i], ch = A.children[f0 + i], page = fresh[i];
             if (par < 0 || par >= A.R || ch < 0 || ch >= A.R || par == ch) {
                 if (lane == 0) A.src[f0 + i] = A.dst[f0 + i] = -1;
@@ -113,11 +113,19 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const Fork
         }
         __syncthreads();
     }
-    meet(blocks);                                              // everybody has read the count
-    if (rank == 0 && threadIdx.x == 0) {
+    if (!last) {
+        if (rank == 0 && threadIdx.x == 0) *A.missing = taken; // for the launch behind
+    } else if (threadIdx.x == 0) {                             // behind the barrier: everybody has read the count
         *A.left = max(count - taken, 0);
         *A.missing = max(taken - count, 0);
     }
+}
+__global__ void paged_fork_count_kernel(const int32_t* count_at, int n_pages, int32_t* left, int32_t* missing) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int count = max(0, min(*count_at, n_pages)), taken = *missing;
+    *left = max(count - taken, 0);
+    *missing = max(taken - count, 0);
 }
 
 // ------------------------------------------------------------------ release
@@ -125,16 +133,17 @@ struct ShareReleaseArgs {
     const uint8_t* done; const int32_t* held; int page_size;
     int R; int32_t* table; int64_t table_stride; int width;
     int32_t* pages; int n_pages; int32_t* count; int32_t* shared;
-    int32_t* times; int32_t* first; int32_t* gives;            // scratch: [pages], [pages], [R]
+    int32_t* times; int32_t* first; int32_t* gives;            // scratch: [pages], [pages], [R + 1]
 };
 
 // Rows that are done give up what they name (behind `held` tokens): page p, named `times` in all, goes onto the stack where that is more than shared[p],
-// in the order of the entries that name it first.  A warp a row, four times: places cleared, names counted, pages of a row counted, pages written.
+// in the order of the entries that name it first.  A warp a row, four times: places cleared, names counted, pages of a row counted, pages written.  One block
+// does all four (PART -1); where there is more to do each is a launch over the whole device, and the count's place is the launch's behind that reads it.
+template <int PART>
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(const ShareReleaseArgs A) {
     __shared__ int warps[32];
     __shared__ int before[SHARE_THREADS];
-    const uint32_t rank = cluster_rank(), blocks = cluster_blocks();
-    const int lane = threadIdx.x & 31, me = (int)rank * SHARE_WARPS + (threadIdx.x >> 5), all = (int)blocks * SHARE_WARPS;
+    const int lane = threadIdx.x & 31, blocks = gridDim.x, me = (threadIdx.x >> 5) * blocks + blockIdx.x, all = blocks * SHARE_WARPS;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = max(0, min(*A.count, A.n_pages));
@@ -164,31 +173,38 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
 #pragma unroll
         for (int u = 0; u < SHARE_DEEP; u++) { times[u] = mine[u] ? A.times[p[u]] : 0; more[u] = mine[u] ? times[u] - A.shared[p[u]] : NEVER; }
     };
-    for (int r = me; r < A.R; r += all)
-        if (A.done[r]) each(r, [&](int, Pages p) {
+    if (PART < 0 || PART == 0) {
+        for (int r = me; r < A.R; r += all)
+            if (A.done[r]) each(r, [&](int, Pages p) {
 #pragma unroll
-            for (int u = 0; u < SHARE_DEEP; u++)
-                if (p[u] >= 0) { A.times[p[u]] = 0; A.first[p[u]] = 0x7fffffff; }
-        });
-    meet(blocks);
-    for (int r = me; r < A.R; r += all)
-        if (A.done[r]) each(r, [&](int c, Pages p) {
-#pragma unroll
-            for (int u = 0; u < SHARE_DEEP; u++)
-                if (p[u] >= 0) { atomicAdd(A.times + p[u], 1); atomicMin(A.first + p[u], r * A.width + c + 32 * u); }
-        });
-    meet(blocks);
-    for (int r = me; r < A.R; r += all) {
-        int n = 0;
-        if (A.done[r]) each(r, [&](int c, Pages p) {
-            int more[SHARE_DEEP], times[SHARE_DEEP];
-            look(r, c, p, more, times);
-#pragma unroll
-            for (int u = 0; u < SHARE_DEEP; u++) n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
-        });
-        if (lane == 0) A.gives[r] = n;
+                for (int u = 0; u < SHARE_DEEP; u++)
+                    if (p[u] >= 0) { A.times[p[u]] = 0; A.first[p[u]] = 0x7fffffff; }
+            });
     }
-    meet(blocks);
+    if (PART < 0) __syncthreads();
+    if (PART < 0 || PART == 1) {
+        for (int r = me; r < A.R; r += all)
+            if (A.done[r]) each(r, [&](int c, Pages p) {
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++)
+                    if (p[u] >= 0) { atomicAdd(A.times + p[u], 1); atomicMin(A.first + p[u], r * A.width + c + 32 * u); }
+            });
+    }
+    if (PART < 0) __syncthreads();
+    if (PART < 0 || PART == 2) {
+        for (int r = me; r < A.R; r += all) {
+            int n = 0;
+            if (A.done[r]) each(r, [&](int c, Pages p) {
+                int more[SHARE_DEEP], times[SHARE_DEEP];
+                look(r, c, p, more, times);
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
+            });
+            if (lane == 0) A.gives[r] = n;
+        }
+    }
+    if (PART < 0) __syncthreads();
+    if (PART >= 0 && PART != 3) return;
     int top = count;
     for (int r0 = 0; r0 < A.R; r0 += SHARE_THREADS) {
         const int n = r0 + (int)threadIdx.x < A.R ? A.gives[r0 + threadIdx.x] : 0;
@@ -219,7 +235,13 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
         top += total;
         __syncthreads();
     }
-    if (rank == 0 && threadIdx.x == 0) *A.count = min(top, A.n_pages);
+    // the count may be read by other blocks yet: the sum of what was given goes where the launch behind finds it
+    if (blockIdx.x == 0 && threadIdx.x == 0) *(PART < 0 ? A.count : A.gives + A.R) = min(top, A.n_pages);
+}
+__global__ void paged_share_count_kernel(const int32_t* top, int32_t* count) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    *count = *top;
 }
 
 // ------------------------------------------------------------------ compact
@@ -382,8 +404,10 @@ template <typename A> int cluster_launch(void (*kern)(A), bool many, const A& ar
     return check_launch();
 }
 
-// entries of the table from which a cluster takes less time than one block
+// entries of the table from which several blocks take less time than one
 constexpr int64_t SHARE_MANY = 8192;
+// blocks over the whole device, of rows by warps
+int wide_grid(int rows) { return rows < sm_count() ? rows : sm_count(); }
 
 bool bad_table(const void* table, int64_t stride, int R, int width) { return !table || R <= 0 || width <= 0 || stride < width || (int64_t)R * width > 0x7fffffffll; }
 
@@ -401,10 +425,18 @@ extern "C" int lowbit_paged_fork_cuda(const int32_t* d_parents, const int32_t* d
     }
     const ForkArgs A = {d_parents, d_children, F, d_lens, d_table, table_stride, R, width, d_free_pages, n_pages, d_free_count, d_free_left, d_shared, page_size, d_src, d_dst,
                         d_missing};
-    return cluster_launch(paged_fork_kernel, (int64_t)F * width > SHARE_MANY, A, (cudaStream_t)stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool many = (int64_t)F * width > SHARE_MANY;
+    launch_behind(paged_fork_kernel, dim3((unsigned)(many ? wide_grid(F) : 1)), SHARE_THREADS, 0, st, launch_overlaps(st), A, !many);
+    note_launch();
+    if (many) {
+        launch_behind(paged_fork_count_kernel, dim3(1), 1, 0, st, launch_overlaps(st), d_free_count, n_pages, d_free_left, d_missing);
+        note_launch();
+    }
+    return check_launch();
 }
 
-extern "C" size_t lowbit_paged_share_release_workspace_size(int n_pages, int R) { return n_pages > 0 && R > 0 ? ((size_t)n_pages * 2 + R) * sizeof(int32_t) : 0; }
+extern "C" size_t lowbit_paged_share_release_workspace_size(int n_pages, int R) { return n_pages > 0 && R > 0 ? ((size_t)n_pages * 2 + R + 1) * sizeof(int32_t) : 0; }
 
 extern "C" int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int32_t* d_held, int page_size, int R, int32_t* d_table, int64_t table_stride, int width,
                                                int32_t* d_free_pages, int n_pages, int32_t* d_free_count, int32_t* d_shared, void* workspace, size_t workspace_bytes,
@@ -420,7 +452,20 @@ extern "C" int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int3
     }
     int32_t* const w = (int32_t*)workspace;
     const ShareReleaseArgs A = {d_done, d_held, page_size, R, d_table, table_stride, width, d_free_pages, n_pages, d_free_count, d_shared, w, w + n_pages, w + 2 * (int64_t)n_pages};
-    return cluster_launch(paged_share_release_kernel, (int64_t)R * width > SHARE_MANY, A, (cudaStream_t)stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((int64_t)R * width <= SHARE_MANY) {
+        launch_behind(paged_share_release_kernel<-1>, dim3(1), SHARE_THREADS, 0, st, launch_overlaps(st), A);
+        note_launch();
+        return check_launch();
+    }
+    const dim3 grid((unsigned)wide_grid(R));
+    launch_behind(paged_share_release_kernel<0>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
+    launch_behind(paged_share_release_kernel<1>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
+    launch_behind(paged_share_release_kernel<2>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
+    launch_behind(paged_share_release_kernel<3>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
+    launch_behind(paged_share_count_kernel, dim3(1), 1, 0, st, launch_overlaps(st), A.gives + R, d_free_count);
+    for (int i = 0; i < 5; i++) note_launch();
+    return check_launch();
 }
 
 extern "C" size_t lowbit_paged_compact_workspace_size(int n_pages) { return n_pages > 0 ? (size_t)n_pages * 4 * sizeof(int32_t) : 0; }

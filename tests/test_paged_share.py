@@ -546,7 +546,7 @@ def test_refusals_on_the_cpu(paged, native_lib):
             [(a, None) for a in (0, 1, 3, 4, 8, 10, 11, 12, 14, 15, 16)] + [(2, 0), (5, 3), (6, 0), (7, 0), (9, 0), (13, 0)])
     refused("lowbit_paged_share_release_cuda", [some, some, 4, 3, some, 4, 4, some, 9, some, some, some, 1 << 20, None],
             [(a, None) for a in (0, 4, 7, 9, 10)] + [(2, 0), (3, 0), (5, 3), (6, 0), (8, 0)])
-    refused("lowbit_paged_share_release_cuda", [some, some, 4, 3, some, 4, 4, some, 9, some, some, some, 1 << 20, None], [(11, None), (11, 4098), (12, 83)], 4)
+    refused("lowbit_paged_share_release_cuda", [some, some, 4, 3, some, 4, 4, some, 9, some, some, some, 1 << 20, None], [(11, None), (11, 4098), (12, 87)], 4)
     refused("lowbit_paged_compact_cuda", [some, 4, 3, 4, some, 9, some, some, some, some, some, some, some, some, some, 1 << 20, None],
             [(a, None) for a in (0, 4, 6, 7, 8, 9, 10, 11, 12, 13)] + [(1, 3), (2, 0), (3, 0), (5, 0)])
     refused("lowbit_paged_compact_cuda", [some, 4, 3, 4, some, 9, some, some, some, some, some, some, some, some, some, 1 << 20, None], [(14, None), (15, 143)], 4)
