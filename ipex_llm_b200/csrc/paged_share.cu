@@ -4,7 +4,6 @@
 // shared[p] counts the rows beyond the first that name page p.  A fork names its parent's full pages (one more each) and gets a page of its own for
 // the tokens behind them, so a page that anybody writes to is named by one row.  A row that goes takes its counts with it, and the last one gives
 // the page back.  All results are whole numbers that do not depend on the order in which threads run.
-#include <limits.h>
 #include "paged.h"
 
 using namespace lowbit;
@@ -137,7 +136,7 @@ struct ShareReleaseArgs {
 };
 
 // Rows that are done give up what they name (behind `held` tokens): page p, named `times` in all, goes onto the stack where that is more than shared[p],
-// in the order of the entries that name it first.  A warp a row, four times: places cleared, names counted, pages of a row counted, pages written.  One block
+// in the order of the entries that name it first.  A warp a row, four times: places cleared, names counted, pages settled and those of a row counted, pages written.  One block
 // does all four (PART -1); where there is more to do each is a launch over the whole device, and the count's place is the launch's behind that reads it.
 template <int PART>
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(const ShareReleaseArgs A) {
@@ -164,15 +163,6 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
         }
     };
     using Pages = const int (&)[SHARE_DEEP];
-    // whether entry e names its page first, and with how many others beyond what shared says (NEVER: not)
-    constexpr int NEVER = INT_MIN;
-    auto look = [&](int r, int c, Pages p, int (&more)[SHARE_DEEP], int (&times)[SHARE_DEEP]) {
-        bool mine[SHARE_DEEP];
-#pragma unroll
-        for (int u = 0; u < SHARE_DEEP; u++) mine[u] = p[u] >= 0 && A.first[p[u]] == r * A.width + c + 32 * u;
-#pragma unroll
-        for (int u = 0; u < SHARE_DEEP; u++) { times[u] = mine[u] ? A.times[p[u]] : 0; more[u] = mine[u] ? times[u] - A.shared[p[u]] : NEVER; }
-    };
     if (PART < 0 || PART == 0) {
         for (int r = me; r < A.R; r += all)
             if (A.done[r]) each(r, [&](int, Pages p) {
@@ -195,10 +185,18 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
         for (int r = me; r < A.R; r += all) {
             int n = 0;
             if (A.done[r]) each(r, [&](int c, Pages p) {
-                int more[SHARE_DEEP], times[SHARE_DEEP];
-                look(r, c, p, more, times);
+                // the entry that names its page first settles the page: `times` is from now on by how many more that was given up than shared says
+                bool mine[SHARE_DEEP];
+                int more[SHARE_DEEP];
 #pragma unroll
-                for (int u = 0; u < SHARE_DEEP; u++) n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
+                for (int u = 0; u < SHARE_DEEP; u++) mine[u] = p[u] >= 0 && A.first[p[u]] == r * A.width + c + 32 * u;
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) more[u] = mine[u] ? A.times[p[u]] - A.shared[p[u]] : 0;
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) {
+                    if (mine[u]) { A.times[p[u]] = more[u]; A.shared[p[u]] = max(-more[u], 0); }
+                    n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
+                }
             });
             if (lane == 0) A.gives[r] = n;
         }
@@ -213,20 +211,20 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
         __syncthreads();
         before[threadIdx.x] = top + sum - n;
         __syncthreads();
-        // rows as they were dealt above: this warp's own reads of an entry, and of shared, lie in front of its writes
+        // rows as they were dealt above
         for (int r = r0 + (me - r0 % all + all) % all; r < min(r0 + SHARE_THREADS, A.R); r += all) {
             if (!A.done[r]) continue;
             int at = before[r - r0];
             int32_t* const row = A.table + r * A.table_stride;
             each(r, [&](int c, Pages p) {
-                int more[SHARE_DEEP], times[SHARE_DEEP];
-                look(r, c, p, more, times);
+                bool goes[SHARE_DEEP];
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) goes[u] = p[u] >= 0 && A.first[p[u]] == r * A.width + c + 32 * u && A.times[p[u]] > 0;
 #pragma unroll
                 for (int u = 0; u < SHARE_DEEP; u++) {
-                    const uint32_t yes = __ballot_sync(0xffffffffu, more[u] > 0);
+                    const uint32_t yes = __ballot_sync(0xffffffffu, goes[u]);
                     const int slot = at + __popc(yes & ((1u << lane) - 1u));
-                    if (more[u] > 0 && slot < A.n_pages) A.pages[slot] = p[u];
-                    if (more[u] != NEVER) A.shared[p[u]] = max(-more[u], 0);
+                    if (goes[u] && slot < A.n_pages) A.pages[slot] = p[u];
                     if (c + 32 * u < A.width) row[c + 32 * u] = -1;
                     at += __popc(yes);
                 }
