@@ -18,8 +18,9 @@ using CompactSizeFn = size_t (*)(int);
 using CompactFn = int (*)(const int32_t*, int64_t, int, int, const int32_t*, int, const int32_t*, const int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, void*,
                           size_t, void*);
 using CopyFn = int (*)(const int32_t*, const int32_t*, int, void* const*, int, int, int64_t, int64_t, void*);
+using LoraSizeFn = size_t (*)(int64_t, int, int);
 using LoraFn = int (*)(const void*, int64_t, int, int64_t, int, const void*, int64_t, const void*, int64_t, int, const float*, int, const int32_t*, const int32_t*, int, const int*, int,
-                       void*, int64_t, void*);
+                       void*, int64_t, void*, size_t, void*);
 using LogprobsFn = int (*)(const void*, int, int64_t, int64_t, int64_t, const int64_t*, float, int, float*, float*, int64_t*, float*, float*, void*);
 NormFn g_norm = nullptr;
 ForkFn g_fork = nullptr;
@@ -28,6 +29,7 @@ ReleaseFn g_release = nullptr;
 CompactSizeFn g_compact_size = nullptr;
 CompactFn g_compact = nullptr;
 CopyFn g_copy = nullptr;
+LoraSizeFn g_lora_size = nullptr;
 LoraFn g_lora = nullptr;
 LogprobsFn g_logprobs = nullptr;
 
@@ -54,8 +56,8 @@ bool adapters_ok(const at::Tensor& t, int64_t each) {
 }  // namespace
 
 PyObject* attach_step(PyObject*, PyObject* args) {
-    unsigned long long f[9];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5, f + 6, f + 7, f + 8)) return nullptr;
+    unsigned long long f[10];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5, f + 6, f + 7, f + 8, f + 9)) return nullptr;
     g_norm = reinterpret_cast<NormFn>(f[0]);
     g_fork = reinterpret_cast<ForkFn>(f[1]);
     g_release_size = reinterpret_cast<ReleaseSizeFn>(f[2]);
@@ -63,8 +65,9 @@ PyObject* attach_step(PyObject*, PyObject* args) {
     g_compact_size = reinterpret_cast<CompactSizeFn>(f[4]);
     g_compact = reinterpret_cast<CompactFn>(f[5]);
     g_copy = reinterpret_cast<CopyFn>(f[6]);
-    g_lora = reinterpret_cast<LoraFn>(f[7]);
-    g_logprobs = reinterpret_cast<LogprobsFn>(f[8]);
+    g_lora_size = reinterpret_cast<LoraSizeFn>(f[7]);
+    g_lora = reinterpret_cast<LoraFn>(f[8]);
+    g_logprobs = reinterpret_cast<LogprobsFn>(f[9]);
     Py_RETURN_NONE;
 }
 
@@ -295,9 +298,12 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     {
         const WithoutGil released;
         const c10::cuda::CUDAGuard guard(x->device());
+        const size_t need = g_lora_size(T, (int)R, (int)S);
+        at::Tensor scratch;
+        if (need) scratch = at::empty({(int64_t)need}, x->options().dtype(at::kByte).requires_grad(false));
         rc = g_lora(x->const_data_ptr(), T > 1 ? x->stride(0) : K, half_code(*x), T, (int)K, wa->const_data_ptr(), L > 1 ? wa->stride(0) : S * R * K, wb->const_data_ptr(),
                     L > 1 ? wb->stride(0) : N * R, (int)R, scales->const_data_ptr<float>(), (int)L, ids->const_data_ptr<int32_t>(), cu->const_data_ptr<int32_t>(), (int)ids->size(0), splits,
-                    (int)S, out->mutable_data_ptr(), T > 1 ? out->stride(0) : N, stream_of(*x));
+                    (int)S, out->mutable_data_ptr(), T > 1 ? out->stride(0) : N, need ? scratch.mutable_data_ptr() : nullptr, need, stream_of(*x));
     }
     if (rc) return PyLong_FromLong(rc);
     Py_RETURN_TRUE;

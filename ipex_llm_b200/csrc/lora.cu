@@ -1,11 +1,13 @@
 // lora.cu -- low-rank adapters of many requests beside a projection that all share:
 //   out[t] += scale_l (x[t] A_l^T) B_l^T,      l = the adapter of the token's request (none: the row stays as it is).
 //
-// One launch.  A cluster takes a tile of packed rows, whoever they belong to: it finds the tile's requests in the list, and the different adapters among
+// A cluster takes a tile of packed rows, whoever they belong to: it finds the tile's requests in the list, and the different adapters among
 // its rows are dealt to the clusters that share the tile.  So an adapter that neighbours have in common is read once for them, and nobody sorts.  For each:
 //   every block multiplies its share of the inner dimension, h = x A^T in 32 bits;
 //   the blocks add up their parts, a share of the rows each, and hand the sums to all through their shared memories;
 //   every block multiplies its share of the columns, h B^T, and adds that to `out`, rounded once.
+// Few tokens take one launch of that.  Many take two, the first product and the second: no block waits for others there, parts of h cost little beside `out`,
+// and a tile's columns are dealt as finely as fills the device.
 // mma.sync m16n8k16: rank and tokens are far below a tcgen05 tile, and what bounds the kernel is what it reads and writes (x; out, twice).
 #include "lowbit_common.cuh"
 #include "lowbit_internal.h"
@@ -25,6 +27,7 @@ struct LoraArgs {
     const int32_t *ids, *cu; int R;                            // requests
     void* out; int64_t o_st;
     int rank, n_splits, together;                              // splits whose products with A are computed at once
+    uint8_t* tiles; float* part; int KS, shares;               // of two launches: the tiles' lists and the parts of h between them, blocks of a tile in each
     int first[LORA_SPLITS + 1];                                // columns in front of a split
 };
 
@@ -75,7 +78,7 @@ __device__ __forceinline__ uint32_t shared_of(uint32_t at, uint32_t block) {
 constexpr int TM = 64;                                         // rows of a tile
 
 // the different adapters among a tile's rows, and the rows of each, one behind the other
-struct Tile {
+struct __align__(16) Tile {
     int id[TM];                                                // of the request that begins in a row; -2: none does
     int n, adapter[TM], first[TM + 1];
     uint8_t row[TM];
@@ -137,7 +140,7 @@ struct Lora {
     static __host__ __device__ int steps(int rank) { return (rank + 15) / 16; }
     // h as the second product's A operand: for each split, step of 16 and tile of 16 tokens 16 bytes a lane of high parts, then of low parts
     static constexpr int kFrag = 1024, kStep = TM / 16 * kFrag;
-    static __host__ __device__ int smem(int rank, int together) { return kRing + together * steps(rank) * kStep + TM * together * rank * 4; }
+    static int smem(int rank, int together, bool part) { return kRing + together * steps(rank) * kStep + (part ? TM * together * rank * 4 : 0); }
 };
 
 // First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
@@ -145,16 +148,19 @@ struct Lora {
 // Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
 // holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.
-template <bool BF, int STEPS>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
+enum { LORA_BOTH, LORA_FIRST, LORA_SECOND };
+template <bool BF, int STEPS, int DO>
+__global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
     constexpr int NT = L::NT, MT = L::MT, ROWS = L::ROWS, TOKS = L::TOKS;
     __shared__ Tile tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
     extern __shared__ __align__(128) uint8_t lora_smem[];
-    uint32_t rank, blocks;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
+    uint32_t rank = blockIdx.x, blocks = DO == LORA_FIRST ? A.KS : A.shares;
+    if (DO == LORA_BOTH) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
+    } else rank %= blocks;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = (int64_t)(blockIdx.x / blocks) * TM;
     const int steps = STEPS ? STEPS : L::steps(A.rank);
@@ -163,7 +169,15 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, hs = smem + L::kRing;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    find_adapters(A, t0, tile);
+    if (DO == LORA_SECOND) {
+        const int4* const from = reinterpret_cast<const int4*>(A.tiles + (int64_t)(blockIdx.x / blocks) * sizeof(Tile));
+        for (int i = threadIdx.x; i < (int)(sizeof(Tile) / 16); i += LORA_THREADS) reinterpret_cast<int4*>(&tile)[i] = from[i];
+        __syncthreads();
+    } else find_adapters(A, t0, tile);
+    if (DO == LORA_FIRST && rank == 0 && blockIdx.y == 0) {
+        int4* const to = reinterpret_cast<int4*>(A.tiles + (int64_t)(blockIdx.x / blocks) * sizeof(Tile));
+        for (int i = threadIdx.x; i < (int)(sizeof(Tile) / 16); i += LORA_THREADS) to[i] = reinterpret_cast<const int4*>(&tile)[i];
+    }
     const int chunks = (A.K + 31) / 32, each = (chunks + (int)blocks - 1) / (int)blocks, from = min((int)rank * each, chunks), to = min(from + each, chunks);
     for (int j = blockIdx.y; j < tile.n; j += gridDim.y) {
         const int id = tile.adapter[j], count = tile.first[j + 1] - tile.first[j];
@@ -173,7 +187,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
             const uint4* const w = (const uint4*)((const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K);
             // ---- h of this block's share of K.  Rows behind the last, of A and of x, are read as the last ones: nobody looks at what they give
-            for (int row0 = 0, i0 = 0; row0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, row0 += i0 ? 0 : ROWS) {
+            for (int row0 = 0, i0 = 0; DO != LORA_SECOND && row0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, row0 += i0 ? 0 : ROWS) {
                 const int m_end = min(MT, (rows - row0 + 15) / 16), n_end = min(NT, (count - i0 + 7) / 8);
                 float acc[MT][NT][4] = {};
                 uint32_t xs[NT], ws[MT][2];                    // in 16 bytes, of this lane's rows
@@ -246,11 +260,14 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                             const float4 p = *reinterpret_cast<const float4*>(sums + (v * TOKS + tok) * L::PITCH + row);
                             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
                         }
-                        *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
+                        if (DO == LORA_FIRST) *reinterpret_cast<float4*>(A.part + ((int64_t)rank * A.T + t0 + row_of[i0 + tok]) * (A.n_splits * A.rank) + s0 * A.rank + row0 + row) = s;
+                        else *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
                     }
                 }
             }
-            meet(blocks);
+            if (DO == LORA_FIRST) continue;
+            if (DO == LORA_BOTH) meet(blocks);
+            else __syncthreads();                              // what was in the ring's and h's place is read
             // ---- this block's share of the columns, 32 a warp: where its groups lie, and what it asks for ahead.  Rows and columns behind the last are read
             // as the last ones, and not written
             const uint16_t* const wb = (const uint16_t*)A.b + id * A.b_st;
@@ -289,39 +306,27 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             ask_out(0);
             // ---- the blocks' parts together: a warp takes a row of the tile in one split
             const uint32_t at_part = (uint32_t)__cvta_generic_to_shared(part), at_back = (uint32_t)__cvta_generic_to_shared(&back[0][0]);
-            for (int i = (int)rank + warp * (int)blocks; i < count * n_here; i += LORA_WARPS * (int)blocks) {
-                const int tok = i % count, s = i / count;
-                float2 h[4];                                   // pairs `lane`, `lane` + 32, ...
-                float big = 0.0f;
+            constexpr int Z = STEPS ? 1 : 4;                   // pairs `lane`, `lane` + 32, ...
+            auto place = [&](int tok, int s, float2 (&h)[Z]) {
+                float big = 0.0f, down = 1.0f;
 #pragma unroll
-                for (int z = 0; z < 4; z++) {
-                    h[z] = make_float2(0.0f, 0.0f);
-                    const int r = 2 * lane + 64 * z;
-                    if (r < A.rank) {
-                        const uint32_t at = at_part + (tok * rows + s * A.rank + r) * 4;
-#pragma unroll 8
-                        for (uint32_t b = 0; b < blocks; b++) {
-                            float2 p;
-                            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(p.x), "=f"(p.y) : "r"(shared_of(at, b)) : "memory");
-                            h[z].x += p.x;
-                            h[z].y += p.y;
-                        }
-                        h[z].x *= scale;
-                        h[z].y *= scale;
-                        big = fmaxf(big, fmaxf(fabsf(h[z].x), fabsf(h[z].y)));
-                    }
+                for (int z = 0; z < Z; z++) {
+                    h[z].x *= scale;
+                    h[z].y *= scale;
+                    big = fmaxf(big, fmaxf(fabsf(h[z].x), fabsf(h[z].y)));
                 }
-                float down = 1.0f;
+                const uint32_t others = DO == LORA_BOTH ? blocks : 1;
                 if (!BF) {
 #pragma unroll
                     for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
                     const int e = (int)(__float_as_uint(big) >> 23) - 127 - 14, use = big > 0.0f && big < INFINITY ? max(e, -100) : 0;
+                    const float up = __uint_as_float((uint32_t)(127 + use) << 23);
                     down = __uint_as_float((uint32_t)(127 - use) << 23);
-                    if (lane < (int)blocks)
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(__uint_as_float((uint32_t)(127 + use) << 23)) : "memory");
+                    if (DO == LORA_SECOND) back[tok][s] = up;
+                    else if (lane < (int)others) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(up) : "memory");
                 }
 #pragma unroll
-                for (int z = 0; z < 4; z++) {
+                for (int z = 0; z < Z; z++) {
                     const int r = 2 * lane + 64 * z;
                     if (r >= 16 * steps) continue;
                     const float x = h[z].x * down, y = h[z].y * down;
@@ -329,12 +334,65 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const float2 f = unpack2<BF>(hi);
                     const uint32_t lo = pack2<BF>(fabsf(f.x) < INFINITY ? x - f.x : 0.0f, fabsf(f.y) < INFINITY ? y - f.y : 0.0f);
                     const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + ((tok & 7) * 4 + (r & 15) / 4) * 16 + (tok & 8) + (r & 2) * 2;
+                    if (DO == LORA_SECOND) {
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + L::kFrag / 2), "r"(lo) : "memory");
+                    } else {
 #pragma unroll 8
-                    for (uint32_t b = 0; b < blocks; b++) {
-                        const uint32_t p = shared_of(at, b);
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p), "r"(hi) : "memory");
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p + L::kFrag / 2), "r"(lo) : "memory");
+                        for (uint32_t b = 0; b < blocks; b++) {
+                            const uint32_t p = shared_of(at, b);
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p), "r"(hi) : "memory");
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(p + L::kFrag / 2), "r"(lo) : "memory");
+                        }
                     }
+                }
+            };
+            if constexpr (DO == LORA_SECOND) {
+                // four rows at a time, so that they wait for memory together
+                const int64_t wide = A.n_splits * A.rank;
+                for (int i0 = warp; i0 < count * n_here; i0 += 4 * LORA_WARPS) {
+                    float2 h[4][Z] = {};
+#pragma unroll 2
+                    for (int ks = 0; ks < A.KS; ks++)
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int i = i0 + u * LORA_WARPS, tok = i % count, s = i / count;
+#pragma unroll
+                            for (int z = 0; z < Z; z++) {
+                                const int r = 2 * lane + 64 * z;
+                                if (i < count * n_here && r < A.rank) {
+                                    const float2 p = *reinterpret_cast<const float2*>(A.part + (ks * A.T + t0 + row_of[tok]) * wide + (s0 + s) * A.rank + r);
+                                    h[u][z].x += p.x;
+                                    h[u][z].y += p.y;
+                                }
+                            }
+                        }
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int i = i0 + u * LORA_WARPS;
+                        if (i < count * n_here) place(i % count, i / count, h[u]);
+                    }
+                }
+            } else {
+                for (int i = (int)rank + warp * (int)blocks; i < count * n_here; i += LORA_WARPS * (int)blocks) {
+                    const int tok = i % count, s = i / count;
+                    float2 h[Z];
+#pragma unroll
+                    for (int z = 0; z < Z; z++) {
+                        h[z] = make_float2(0.0f, 0.0f);
+                        const int r = 2 * lane + 64 * z;
+                        if (r < A.rank) {
+                            const uint32_t at = at_part + (tok * rows + s * A.rank + r) * 4;
+#pragma unroll 8
+                            for (uint32_t b = 0; b < blocks; b++) {
+                                float2 p;
+                                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(p.x), "=f"(p.y) : "r"(shared_of(at, b)) : "memory");
+                                h[z].x += p.x;
+                                h[z].y += p.y;
+                            }
+                        }
+                    }
+                    place(tok, s, h);
                 }
             }
             const int off = (8 * (g >> 1) + (g & 1)) * A.rank + 4 * t;                         // this lane's rows of B are 2 n further on
@@ -356,7 +414,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
 #pragma unroll
                 for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
             }
-            meet(blocks);
+            if (DO == LORA_BOTH) meet(blocks);
+            else __syncthreads();
 #pragma unroll 1
             for (int stage = 0; more; stage ^= 1) {
                 const Group now = ahead;
@@ -424,32 +483,50 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     }
 }
 
+// Many tokens take two launches.
+constexpr int64_t LORA_MANY = 256;
+// splits that share a reading of x: 128 rows of A at most, or one split
+int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
+constexpr int LORA_KS = 4;                                     // parts of h
+size_t lora_tiles_bytes(int64_t T) { return (size_t)((T + TM - 1) / TM) * sizeof(Tile); }
+
 template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
-    // splits that share a reading of x: 128 rows of A at most, or one split
-    A.together = A.n_splits * A.rank <= 128 ? A.n_splits : A.rank >= 128 ? 1 : 128 / A.rank;
+    A.together = lora_together(A.rank, A.n_splits);
     static bool configured[64] = {};                           // the attribute is per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        cudaFuncSetAttribute(lora_kernel<BF, STEPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1, true));
+        cudaFuncSetAttribute(lora_kernel<BF, 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRing);
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1, false));
         configured[dev & 63] = true;
     }
     const int64_t tiles = (A.T + TM - 1) / TM;
-    // clusters that share a tile's adapters: twice as many as a tile has on average
+    // blocks, or clusters, that share a tile's adapters: twice as many as a tile has on average
     int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
     if (most > A.adapters) most = A.adapters;
+    if (some > most) some = most;
+    if (A.T > LORA_MANY) {
+        A.shares = 8;
+        launch_behind(lora_kernel<BF, 0, LORA_FIRST>, dim3((unsigned)(tiles * A.KS), (unsigned)some), LORA_THREADS, Lora::kRing, st, launch_overlaps(st), A);
+        note_launch();
+        launch_behind(lora_kernel<BF, STEPS, LORA_SECOND>, dim3((unsigned)(tiles * A.shares), (unsigned)some), LORA_THREADS, (size_t)Lora::smem(A.rank, A.together, false), st,
+                      launch_overlaps(st), A);
+        note_launch();
+        return check_launch();
+    }
     const int blocks = 8;                                      // of a cluster: the most that any device takes
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)(some < most ? some : most));
+    cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)some);
     cfg.blockDim = dim3(LORA_THREADS);
-    cfg.dynamicSmemBytes = (size_t)Lora::smem(A.rank, A.together);
+    cfg.dynamicSmemBytes = (size_t)Lora::smem(A.rank, A.together, true);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
-    cudaLaunchKernelEx(&cfg, lora_kernel<BF, STEPS>, A);
+    cudaLaunchKernelEx(&cfg, lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     return check_launch();
 }
@@ -461,9 +538,14 @@ template <bool BF> int lora_steps(const LoraArgs& A, cudaStream_t st) {
 }  // namespace
 }  // namespace lowbit
 
+extern "C" size_t lowbit_lora_workspace_size(int64_t T, int rank, int n_splits) {
+    if (T <= LORA_MANY || rank <= 0 || n_splits <= 0) return 0;
+    return lora_tiles_bytes(T) + (size_t)T * rank * n_splits * LORA_KS * sizeof(float);
+}
+
 extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b, int64_t b_stride,
                                     int rank, const float* d_scales, int adapters, const int32_t* d_ids, const int32_t* d_cu_seqlens, int R, const int* splits, int n_splits,
-                                    void* d_out, int64_t out_stride, void* stream) {
+                                    void* d_out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     reset_launch_count();
     const char* const name = "lowbit_lora_add_cuda";
     bool bad = !d_x || !d_a || !d_b || !d_scales || !d_ids || !d_cu_seqlens || !d_out || !splits || (dtype != DT_F16 && dtype != DT_BF16) || T < 0 || T > 0x7fffffffll || K <= 0 ||
@@ -481,7 +563,12 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
         return LB_ERR_ARG;
     }
     if (T == 0) return LB_OK;
-    LoraArgs A = {d_x, x_stride, T, K, d_a, a_stride, d_b, b_stride, d_scales, adapters, d_ids, d_cu_seqlens, R, d_out, out_stride, rank, n_splits, 0, {}};
+    if (T > LORA_MANY && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_lora_workspace_size(T, rank, n_splits))) {
+        set_error(LB_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of lowbit_lora_workspace_size() bytes is needed", name);
+        return LB_ERR_WORKSPACE;
+    }
+    LoraArgs A = {d_x, x_stride, T, K, d_a, a_stride, d_b, b_stride, d_scales, adapters, d_ids, d_cu_seqlens, R, d_out, out_stride, rank, n_splits, 0,
+                  (uint8_t*)workspace, (float*)((uint8_t*)workspace + lora_tiles_bytes(T)), LORA_KS, 0, {}};
     for (int i = 0; i < n_splits; i++) A.first[i + 1] = A.first[i] + splits[i];
     cudaStream_t st = (cudaStream_t)stream;
     return dtype == DT_BF16 ? lora_steps<true>(A, st) : lora_steps<false>(A, st);

@@ -819,19 +819,25 @@ def lowbit_paged_copy(src, dst, caches, n_pages, page_stride_bytes, page_bytes, 
 
 
 # ---------------------------------------------------------------- low-rank adapters of many requests
+_lib.lowbit_lora_workspace_size.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_int]
+_lib.lowbit_lora_workspace_size.restype = ctypes.c_size_t
 _lib.lowbit_lora_add_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                       ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
-                                      ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
+                                      ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
 _lib.lowbit_lora_add_cuda.restype = ctypes.c_int
 
 
-def lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, stream):
+def lowbit_lora_workspace_size(tokens, rank, n_splits):
+    return _lib.lowbit_lora_workspace_size(tokens, rank, n_splits)
+
+
+def lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, workspace, stream):
     """x [T, K], out [T, N], a [L, S, R, K], b [L, N, R], scales fp32 [L], adapter_ids [requests], cu_seqlens [requests + 1]"""
     T, K = x.shape
     _check(_lib.lowbit_lora_add_cuda(x.data_ptr(), x.stride(0) if T > 1 else K, _DT_OF[x.dtype], T, K, a.data_ptr(), a.stride(0) if a.shape[0] > 1 else a[0].numel(), b.data_ptr(),
                                      b.stride(0) if b.shape[0] > 1 else b[0].numel(), b.shape[2], scales.data_ptr(), b.shape[0], adapter_ids.data_ptr(), cu_seqlens.data_ptr(),
                                      adapter_ids.shape[0], (ctypes.c_int * len(splits))(*splits), len(splits), out.data_ptr(), out.stride(0) if T > 1 else out.shape[1],
-                                     stream), "lowbit_lora_add_cuda")
+                                     workspace.data_ptr(), workspace.numel(), stream), "lowbit_lora_add_cuda")
 
 
 # ---------------------------------------------------------------- log probabilities of tokens

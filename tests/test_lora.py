@@ -253,9 +253,15 @@ def test_refusals_on_the_cpu(lora, native_lib):
     import ctypes
     lib, some = native_lib._lib, 4096                                  # never read: every call is refused before anything is launched
     splits = (ctypes.c_int * 2)(32, 32)
-    good = [some, 64, 1, 5, 64, some, 2 * 16 * 64, some, 64 * 16, 16, some, 2, some, some, 2, splits, 2, some, 64, None]
+    good = [some, 64, 1, 5, 64, some, 2 * 16 * 64, some, 64 * 16, 16, some, 2, some, some, 2, splits, 2, some, 64, None, 0, None]
     for i, bad in ((0, None), (0, 4100), (1, 56), (1, 68), (2, 0), (3, -1), (3, 1 << 40), (4, 60), (4, 0), (5, None), (6, 100), (7, None), (8, 100), (9, 12), (9, 264), (9, 0), (10, None), (11, 0),
                    (12, None), (13, None), (14, 0), (15, None), (15, (ctypes.c_int * 2)(32, 12)), (15, (ctypes.c_int * 2)(64, 0)), (16, 0), (16, 9), (17, None), (17, 4104), (18, 56)):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 1, (i, bad)
+    good[3], good[19], good[20] = 300, some, 1 << 30
+    for i, bad in ((19, None), (19, 4100), (20, 300 * 2 * 16 * 4)):
+        args = list(good)
+        args[i] = bad
+        assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
+    assert lib.lowbit_lora_workspace_size(256, 16, 2) == 0 and lib.lowbit_lora_workspace_size(257, 16, 2) >= 257 * 32 * 4
