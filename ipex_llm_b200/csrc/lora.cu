@@ -6,8 +6,8 @@
 //   every block multiplies its share of the inner dimension, h = x A^T in 32 bits;
 //   the blocks add up their parts, a share of the rows each, and hand the sums to all through their shared memories;
 //   every block multiplies its share of the columns, h B^T, and adds that to `out`, rounded once.
-// Few tokens take one launch of that.  Many take two, the first product and the second: no block waits for others there, parts of h cost little beside `out`,
-// and a tile's columns are dealt as finely as fills the device.
+// Few tokens take one launch of that.  Many take two, the first product and the second, with h as two 16-bit values in memory between them: it costs little
+// beside `out`, each kernel has the registers that its product wants, and a tile's columns are dealt as finely as fills the device.
 // mma.sync m16n8k16: rank and tokens are far below a tcgen05 tile, and what bounds the kernel is what it reads and writes (x; out, twice).
 #include "lowbit_common.cuh"
 #include "lowbit_internal.h"
@@ -27,7 +27,7 @@ struct LoraArgs {
     const int32_t *ids, *cu; int R;                            // requests
     void* out; int64_t o_st;
     int rank, n_splits, together;                              // splits whose products with A are computed at once
-    uint8_t* tiles; float* part; int KS, shares;               // of two launches: the tiles' lists and the parts of h between them, blocks of a tile in each
+    uint8_t* tiles; uint16_t* h; float* back; int shares;      // of two launches: the tiles' lists and h between them, blocks of a tile in the second
     int first[LORA_SPLITS + 1];                                // columns in front of a split
 };
 
@@ -131,16 +131,18 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 }
 
 // Shared memory: two stages of 4 KB a warp, in which every lane finds what it asked for itself (so nobody waits for a neighbour), and in their place the
-// sums of the warps on their way together; h as two 16-bit values; the block's part of h.
+// sums of the warps on their way together; h as two 16-bit values; the block's part of h.  The first product takes 32 tokens at a time, 64 in a launch of
+// its own, whose stages are of 6 KB: A is read half as often.
 struct Lora {
-    static constexpr int NT = 4, MT = 2, TOKS = 8 * NT, ROWS = 16 * MT;      // tiles of 8 tokens and of 16 rows of A in the first product
+    static constexpr int MT = 2, ROWS = 16 * MT;              // tiles of 16 rows of A in the first product
     static constexpr int PITCH = ROWS + 4;                     // a warp's stores of sums meet every bank once
-    static constexpr int kStage = 8 * 512, kRing = LORA_WARPS * 2 * kStage;
-    static_assert(kRing >= LORA_WARPS * TOKS * PITCH * 4, "the sums fit");
+    static constexpr int kStage = 8 * 512, kRing = LORA_WARPS * 2 * kStage, kRingFirst = LORA_WARPS * 2 * 12 * 512;
+    static_assert(kRing >= LORA_WARPS * 32 * PITCH * 4 && kRingFirst >= LORA_WARPS * TM * PITCH * 4, "the sums fit");
     static __host__ __device__ int steps(int rank) { return (rank + 15) / 16; }
     // h as the second product's A operand: for each split, step of 16 and tile of 16 tokens 16 bytes a lane of high parts, then of low parts
     static constexpr int kFrag = 1024, kStep = TM / 16 * kFrag;
-    static int smem(int rank, int together, bool part) { return kRing + together * steps(rank) * kStep + (part ? TM * together * rank * 4 : 0); }
+    static int parts(int rank, int together) { return TM * together * rank * 4; }
+    static int smem(int rank, int together) { return kRing + together * steps(rank) * kStep; }
 };
 
 // First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
@@ -150,23 +152,23 @@ struct Lora {
 // holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.
 enum { LORA_BOTH, LORA_FIRST, LORA_SECOND };
 template <bool BF, int STEPS, int DO>
-__global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_kernel(const LoraArgs A) {
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
-    constexpr int NT = L::NT, MT = L::MT, ROWS = L::ROWS, TOKS = L::TOKS;
+    constexpr int NT = DO == LORA_FIRST ? 8 : 4, TOKS = 8 * NT, MT = L::MT, ROWS = L::ROWS, STAGE = (NT + 2 * MT) * 512;      // of the first product
     __shared__ Tile tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
     extern __shared__ __align__(128) uint8_t lora_smem[];
-    uint32_t rank = blockIdx.x, blocks = DO == LORA_FIRST ? A.KS : A.shares;
-    if (DO == LORA_BOTH) {
+    uint32_t rank = blockIdx.x % A.shares, blocks = A.shares;
+    if (DO != LORA_SECOND) {
         asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
-    } else rank %= blocks;
+    }
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = (int64_t)(blockIdx.x / blocks) * TM;
     const int steps = STEPS ? STEPS : L::steps(A.rank);
     float* const sums = reinterpret_cast<float*>(lora_smem);
-    float* const part = reinterpret_cast<float*>(lora_smem + L::kRing + A.together * steps * L::kStep);
-    const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, hs = smem + L::kRing;
+    float* const part = reinterpret_cast<float*>(lora_smem + (DO == LORA_FIRST ? L::kRingFirst : L::kRing + A.together * steps * L::kStep));
+    const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, ring1 = smem + warp * 2 * STAGE + lane * 16, hs = smem + L::kRing;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (DO == LORA_SECOND) {
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                     for (int h = 0; h < 2; h++) ws[m][h] = (uint32_t)min(row0 + 16 * m + 8 * h + g, rows - 1) * (uint32_t)(A.K / 8);
                 auto ask = [&](int c, int stage) {
                     const bool in = c < to && 32 * c + 8 * t < A.K;
-                    const uint32_t k = in ? 4 * c + t : 0, at = ring + stage * L::kStage;
+                    const uint32_t k = in ? 4 * c + t : 0, at = ring1 + stage * STAGE;
 #pragma unroll
                     for (int n = 0; n < NT; n++)
                         if (n < n_end) cp16(at + n * 512, x + (xs[n] + k), in);
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
 #pragma unroll 1
                 for (int c = from + warp; c < to; c += LORA_WARPS, stage ^= 1) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    const uint32_t at = ring + stage * L::kStage;
+                    const uint32_t at = ring1 + stage * STAGE;
                     uint4 wr[MT][2];
 #pragma unroll
                     for (int m = 0; m < MT; m++)
@@ -250,9 +252,9 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                             }
                     }
                 __syncthreads();
-                {
-                    const int i = threadIdx.x, tok = i / (ROWS / 4), row = i % (ROWS / 4) * 4;
-                    static_assert(TOKS * ROWS / 4 == LORA_THREADS, "four sums a thread");
+#pragma unroll 1
+                for (int i = threadIdx.x; i < TOKS * ROWS / 4; i += LORA_THREADS) {
+                    const int tok = i / (ROWS / 4), row = i % (ROWS / 4) * 4;
                     if (i0 + tok < count && row0 + row < rows) {
                         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -260,13 +262,11 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                             const float4 p = *reinterpret_cast<const float4*>(sums + (v * TOKS + tok) * L::PITCH + row);
                             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
                         }
-                        if (DO == LORA_FIRST) *reinterpret_cast<float4*>(A.part + ((int64_t)rank * A.T + t0 + row_of[i0 + tok]) * (A.n_splits * A.rank) + s0 * A.rank + row0 + row) = s;
-                        else *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
+                        *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
                     }
                 }
             }
-            if (DO == LORA_FIRST) continue;
-            if (DO == LORA_BOTH) meet(blocks);
+            if (DO != LORA_SECOND) meet(blocks);
             else __syncthreads();                              // what was in the ring's and h's place is read
             // ---- this block's share of the columns, 32 a warp: where its groups lie, and what it asks for ahead.  Rows and columns behind the last are read
             // as the last ones, and not written
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
             for (int i = 0; i < TM / 8; i++) row_at[i] = (uint32_t)(row_of[min(8 * i + g, count - 1)] * A.o_st / 8);
             uint4* const out = reinterpret_cast<uint4*>((uint16_t*)A.out + t0 * A.o_st);
             Group ahead = {0, 0, (A.first[s0 + 1] - A.first[s0] + 31) / 32, (int)rank * LORA_WARPS + warp, 0, 0};
-            bool more = ahead.settle(A, s0, n_here);
+            bool more = DO != LORA_FIRST && ahead.settle(A, s0, n_here);
             auto ask_out = [&](int stage) {
                 if (more) {
                     const uint4* const from = out + min(ahead.c0 + 8 * t, ahead.c_end - 8) / 8;
@@ -322,8 +322,9 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                     const int e = (int)(__float_as_uint(big) >> 23) - 127 - 14, use = big > 0.0f && big < INFINITY ? max(e, -100) : 0;
                     const float up = __uint_as_float((uint32_t)(127 + use) << 23);
                     down = __uint_as_float((uint32_t)(127 - use) << 23);
-                    if (DO == LORA_SECOND) back[tok][s] = up;
-                    else if (lane < (int)others) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(up) : "memory");
+                    if (DO == LORA_FIRST) {
+                        if (lane == 0) A.back[(t0 + row_of[tok]) * A.n_splits + s0 + s] = up;
+                    } else if (lane < (int)others) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(up) : "memory");
                 }
 #pragma unroll
                 for (int z = 0; z < Z; z++) {
@@ -333,11 +334,12 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                     const uint32_t hi = pack2<BF>(x, y);
                     const float2 f = unpack2<BF>(hi);
                     const uint32_t lo = pack2<BF>(fabsf(f.x) < INFINITY ? x - f.x : 0.0f, fabsf(f.y) < INFINITY ? y - f.y : 0.0f);
-                    const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + ((tok & 7) * 4 + (r & 15) / 4) * 16 + (tok & 8) + (r & 2) * 2;
-                    if (DO == LORA_SECOND) {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + L::kFrag / 2), "r"(lo) : "memory");
+                    if (DO == LORA_FIRST) {
+                        uint16_t* const to = A.h + (t0 + row_of[tok]) * (A.n_splits * 32 * steps) + (s0 + s) * 32 * steps + r;
+                        *reinterpret_cast<uint32_t*>(to) = hi;
+                        *reinterpret_cast<uint32_t*>(to + 16 * steps) = lo;
                     } else {
+                        const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + ((tok & 7) * 4 + (r & 15) / 4) * 16 + (tok & 8) + (r & 2) * 2;
 #pragma unroll 8
                         for (uint32_t b = 0; b < blocks; b++) {
                             const uint32_t p = shared_of(at, b);
@@ -348,31 +350,17 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                 }
             };
             if constexpr (DO == LORA_SECOND) {
-                // four rows at a time, so that they wait for memory together
-                const int64_t wide = A.n_splits * A.rank;
-                for (int i0 = warp; i0 < count * n_here; i0 += 4 * LORA_WARPS) {
-                    float2 h[4][Z] = {};
-#pragma unroll 2
-                    for (int ks = 0; ks < A.KS; ks++)
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            const int i = i0 + u * LORA_WARPS, tok = i % count, s = i / count;
-#pragma unroll
-                            for (int z = 0; z < Z; z++) {
-                                const int r = 2 * lane + 64 * z;
-                                if (i < count * n_here && r < A.rank) {
-                                    const float2 p = *reinterpret_cast<const float2*>(A.part + (ks * A.T + t0 + row_of[tok]) * wide + (s0 + s) * A.rank + r);
-                                    h[u][z].x += p.x;
-                                    h[u][z].y += p.y;
-                                }
-                            }
-                        }
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const int i = i0 + u * LORA_WARPS;
-                        if (i < count * n_here) place(i % count, i / count, h[u]);
-                    }
+                // 16 bytes, a row's eight neighbours, a thread: two lanes' share of a fragment
+                const int pieces = n_here * steps * 4;         // of a row: two of high parts, two of low ones a step
+                for (int i = threadIdx.x; i < count * pieces; i += LORA_THREADS) {
+                    const int tok = i / pieces, in = i - tok * pieces, s = in / (4 * steps), half = in / (2 * steps) & 1, r = in % (2 * steps) * 8;
+                    const uint4 v = *reinterpret_cast<const uint4*>(A.h + (t0 + row_of[tok]) * (A.n_splits * 32 * steps) + s0 * 32 * steps + in * 8);
+                    const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + half * (L::kFrag / 2) + ((tok & 7) * 4 + (r & 8) / 4) * 16 + (tok & 8);
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + 16), "r"(v.z), "r"(v.w) : "memory");
                 }
+                if (!BF)
+                    for (int i = threadIdx.x; i < count * n_here; i += LORA_THREADS) back[i / n_here][i % n_here] = A.back[(t0 + row_of[i / n_here]) * A.n_splits + s0 + i % n_here];
             } else {
                 for (int i = (int)rank + warp * (int)blocks; i < count * n_here; i += LORA_WARPS * (int)blocks) {
                     const int tok = i % count, s = i / count;
@@ -394,6 +382,10 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
                     }
                     place(tok, s, h);
                 }
+            }
+            if (DO == LORA_FIRST) {
+                meet(blocks);                                  // the parts are read: they may be written again, and their block may leave
+                continue;
             }
             const int off = (8 * (g >> 1) + (g & 1)) * A.rank + 4 * t;                         // this lane's rows of B are 2 n further on
             auto fetch = [&](const Group& of, int st, uint2 (&br)[4]) {
@@ -487,7 +479,6 @@ __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_FIRST ? 3 : 2) lora_k
 constexpr int64_t LORA_MANY = 256;
 // splits that share a reading of x: 128 rows of A at most, or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
-constexpr int LORA_KS = 4;                                     // parts of h
 size_t lora_tiles_bytes(int64_t T) { return (size_t)((T + TM - 1) / TM) * sizeof(Tile); }
 
 template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
@@ -496,38 +487,43 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1, true));
-        cudaFuncSetAttribute(lora_kernel<BF, 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRing);
-        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1, false));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1) + Lora::parts(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
     }
+    const bool many = A.T > LORA_MANY;
     const int64_t tiles = (A.T + TM - 1) / TM;
     // blocks, or clusters, that share a tile's adapters: twice as many as a tile has on average
     int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
     if (most > A.adapters) most = A.adapters;
     if (some > most) some = most;
-    if (A.T > LORA_MANY) {
-        A.shares = 8;
-        launch_behind(lora_kernel<BF, 0, LORA_FIRST>, dim3((unsigned)(tiles * A.KS), (unsigned)some), LORA_THREADS, Lora::kRing, st, launch_overlaps(st), A);
-        note_launch();
-        launch_behind(lora_kernel<BF, STEPS, LORA_SECOND>, dim3((unsigned)(tiles * A.shares), (unsigned)some), LORA_THREADS, (size_t)Lora::smem(A.rank, A.together, false), st,
-                      launch_overlaps(st), A);
-        note_launch();
-        return check_launch();
-    }
-    const int blocks = 8;                                      // of a cluster: the most that any device takes
+    // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes, fewer where the tiles fill the device
+    int blocks = 8;
+    while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)some);
     cfg.blockDim = dim3(LORA_THREADS);
-    cfg.dynamicSmemBytes = (size_t)Lora::smem(A.rank, A.together, true);
+    cfg.dynamicSmemBytes = (size_t)(many ? Lora::kRingFirst : Lora::smem(A.rank, A.together)) + Lora::parts(A.rank, A.together);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
-    cudaLaunchKernelEx(&cfg, lora_kernel<BF, STEPS, LORA_BOTH>, A);
+    A.shares = 1;
+    cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
+    if (many) {
+        // blocks of a tile's columns: eight an SM's two places, none with fewer than three groups a warp
+        const int64_t want = 8ll * sm_count() / tiles, room = A.first[A.n_splits] / (32 * LORA_WARPS * 3);
+        A.shares = (int)(want < 8 ? 8 : want);
+        if (A.shares > room) A.shares = (int)room;
+        if (A.shares < 1) A.shares = 1;
+        launch_behind(lora_kernel<BF, STEPS, LORA_SECOND>, dim3((unsigned)(tiles * A.shares), (unsigned)some), LORA_THREADS, (size_t)Lora::smem(A.rank, A.together), st,
+                      launch_overlaps(st), A);
+        note_launch();
+    }
     return check_launch();
 }
 
@@ -540,7 +536,7 @@ template <bool BF> int lora_steps(const LoraArgs& A, cudaStream_t st) {
 
 extern "C" size_t lowbit_lora_workspace_size(int64_t T, int rank, int n_splits) {
     if (T <= LORA_MANY || rank <= 0 || n_splits <= 0) return 0;
-    return lora_tiles_bytes(T) + (size_t)T * rank * n_splits * LORA_KS * sizeof(float);
+    return lora_tiles_bytes(T) + (size_t)T * n_splits * (Lora::steps(rank) * 64 + sizeof(float));
 }
 
 extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b, int64_t b_stride,
@@ -568,7 +564,11 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
         return LB_ERR_WORKSPACE;
     }
     LoraArgs A = {d_x, x_stride, T, K, d_a, a_stride, d_b, b_stride, d_scales, adapters, d_ids, d_cu_seqlens, R, d_out, out_stride, rank, n_splits, 0,
-                  (uint8_t*)workspace, (float*)((uint8_t*)workspace + lora_tiles_bytes(T)), LORA_KS, 0, {}};
+                  (uint8_t*)workspace, nullptr, nullptr, 0, {}};
+    if (T > LORA_MANY) {
+        A.h = (uint16_t*)((uint8_t*)workspace + lora_tiles_bytes(T));
+        A.back = (float*)(A.h + T * n_splits * Lora::steps(rank) * 32);
+    }
     for (int i = 0; i < n_splits; i++) A.first[i + 1] = A.first[i] + splits[i];
     cudaStream_t st = (cudaStream_t)stream;
     return dtype == DT_BF16 ? lora_steps<true>(A, st) : lora_steps<false>(A, st);
