@@ -149,7 +149,7 @@ struct Lora {
 // = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K.
 // Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
-// holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.
+// holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  (The first product alone: 4 for up to 4.)
 enum { LORA_BOTH, LORA_FIRST, LORA_SECOND };
 template <bool BF, int STEPS, int DO>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     }
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = (int64_t)(blockIdx.x / blocks) * TM;
-    const int steps = STEPS ? STEPS : L::steps(A.rank);
+    const int steps = STEPS && DO != LORA_FIRST ? STEPS : L::steps(A.rank);
     float* const sums = reinterpret_cast<float*>(lora_smem);
     float* const part = reinterpret_cast<float*>(lora_smem + (DO == LORA_FIRST ? L::kRingFirst : L::kRing + A.together * steps * L::kStep));
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, ring1 = smem + warp * 2 * STAGE + lane * 16, hs = smem + L::kRing;
@@ -488,7 +488,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1) + Lora::parts(256, 1));
-        cudaFuncSetAttribute(lora_kernel<BF, 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(256, 1));
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
     }
@@ -512,7 +512,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
     A.shares = 1;
-    cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
+    cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
         // blocks of a tile's columns: eight an SM's two places, none with fewer than three groups a warp
