@@ -3,6 +3,10 @@
 // function returns None when a call is not the plain case: the Python statements then serve or refuse it; an int: the native error code.
 #include <cmath>
 #include <vector>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include "host_common.h"
 #include "paged_host.h"
 
@@ -22,6 +26,8 @@ using LoraSizeFn = size_t (*)(int64_t, int, int);
 using LoraFn = int (*)(const void*, int64_t, int, int64_t, int, const void*, int64_t, const void*, int64_t, int, const float*, int, const int32_t*, const int32_t*, int, const int*, int,
                        void*, int64_t, void*, size_t, void*);
 using LogprobsFn = int (*)(const void*, int, int64_t, int64_t, int64_t, const int64_t*, float, int, float*, float*, int64_t*, float*, float*, void*);
+using LogprobsGradFn = int (*)(const void*, int, int64_t, int64_t, int64_t, const int64_t*, float, int, const int64_t*, const float*, const float*, const float*, const float*, void*, int64_t,
+                               void*);
 NormFn g_norm = nullptr;
 ForkFn g_fork = nullptr;
 ReleaseSizeFn g_release_size = nullptr;
@@ -32,6 +38,7 @@ CopyFn g_copy = nullptr;
 LoraSizeFn g_lora_size = nullptr;
 LoraFn g_lora = nullptr;
 LogprobsFn g_logprobs = nullptr;
+LogprobsGradFn g_logprobs_grad = nullptr;
 
 int float_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : half_code(t); }
 bool number(PyObject* o, double* out) {
@@ -56,8 +63,8 @@ bool adapters_ok(const at::Tensor& t, int64_t each) {
 }  // namespace
 
 PyObject* attach_step(PyObject*, PyObject* args) {
-    unsigned long long f[10];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5, f + 6, f + 7, f + 8, f + 9)) return nullptr;
+    unsigned long long f[11];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5, f + 6, f + 7, f + 8, f + 9, f + 10)) return nullptr;
     g_norm = reinterpret_cast<NormFn>(f[0]);
     g_fork = reinterpret_cast<ForkFn>(f[1]);
     g_release_size = reinterpret_cast<ReleaseSizeFn>(f[2]);
@@ -68,6 +75,7 @@ PyObject* attach_step(PyObject*, PyObject* args) {
     g_lora_size = reinterpret_cast<LoraSizeFn>(f[7]);
     g_lora = reinterpret_cast<LoraFn>(f[8]);
     g_logprobs = reinterpret_cast<LogprobsFn>(f[9]);
+    g_logprobs_grad = reinterpret_cast<LogprobsGradFn>(f[10]);
     Py_RETURN_NONE;
 }
 
@@ -310,32 +318,91 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// token_logprobs(logits [rows, vocabulary], tokens, top_k, temperature) -> the four of a TokenLogprobs
+namespace {
+
+// the gradient of token_logprobs (in Python, the engine's thread and two statements of 20 us beside kernels of 5)
+struct TokenLogprobsBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable logits, tokens, ids, stats;
+    float temperature = 1.0f;
+    int64_t k = 0;
+    std::string name() const override { return "TokenLogprobsBackward"; }
+    void release_variables() override { logits.reset_data(); tokens.reset_data(); ids.reset_data(); stats.reset_data(); }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+        const at::Tensor x = logits.unpack(), t = tokens.unpack(), s = stats.unpack(), i = k ? ids.unpack() : at::Tensor();
+        at::Tensor given[3], grad;
+        const float* at[3] = {};
+        for (size_t n = 0; n < grads.size() && n < 3; n++)
+            if (grads[n].defined()) {
+                given[n] = grads[n].to(at::kFloat).contiguous();
+                at[n] = given[n].const_data_ptr<float>();
+            }
+        {
+            const at::NoGradGuard none;
+            const c10::cuda::CUDAGuard guard(x.device());
+            const int64_t rows = x.size(0), V = x.size(1);
+            grad = at::empty({rows, V}, x.options().requires_grad(false));
+            const int rc = g_logprobs_grad(x.const_data_ptr(), float_code(x), rows > 1 ? x.stride(0) : V, rows, V, t.const_data_ptr<int64_t>(), temperature, (int)k,
+                                           k ? i.const_data_ptr<int64_t>() : nullptr, at[0], at[1], at[2], s.const_data_ptr<float>(), grad.mutable_data_ptr(), V, stream_of(x));
+            TORCH_CHECK(rc == 0, "lowbit_token_logprobs_grad_cuda: native error ", rc);
+        }
+        if (at::GradMode::is_enabled()) {                      // create_graph: there is no derivative of this
+            auto error = std::make_shared<torch::autograd::DelayedError>("the gradient of token_logprobs has no derivative", 1);
+            return (*error)({grad.requires_grad_()});
+        }
+        return {grad};
+    }
+};
+
+}  // namespace
+
+// token_logprobs(logits [rows, vocabulary], tokens, top_k, temperature) -> the four of a TokenLogprobs, with a gradient where the logits want one
 PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     if (n_args != 4 || !g_logprobs) Py_RETURN_NONE;
     const at::Tensor *x = plain(a[0]), *tokens = plain(a[1]);
     int64_t k;
     double temperature;
-    if (!x || x->dim() != 2 || float_code(*x) < 0 || wants_grad(*x) || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature >= 1e-7) || !(temperature <= 1e7))
+    if (!x || x->dim() != 2 || float_code(*x) < 0 || x->_fw_grad(0).defined() || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature >= 1e-7) || !(temperature <= 1e7))
         Py_RETURN_NONE;
     const int64_t rows = x->size(0), V = x->size(1);
     if (rows <= 0 || V <= 0 || k < 0 || k > 32 || k > V || (V > 1 && x->stride(1) != 1) || (rows > 1 && x->stride(0) < V) || !ints(tokens, rows, at::kLong, *x)) Py_RETURN_NONE;
+    const bool grad = x->requires_grad() && at::GradMode::is_enabled();
     at::Tensor out[4];
     int rc;
     {
         const WithoutGil released;
         const c10::cuda::CUDAGuard guard(x->device());
         const auto options = x->options().dtype(at::kFloat).requires_grad(false);
-        out[0] = at::empty({rows}, options);
-        out[1] = at::empty({rows}, options);
-        if (k) {
-            out[2] = at::empty({rows, k}, options.dtype(at::kLong));
-            out[3] = at::empty({rows, k}, options);
+        at::Tensor stats;
+        if (k) out[2] = at::empty({rows, k}, options.dtype(at::kLong));
+        if (grad) {
+            // tensors of their own: each may be written to without the others noticing
+            out[0] = at::empty({rows}, options);
+            out[1] = at::empty({rows}, options);
+            if (k) out[3] = at::empty({rows, k}, options);
+            stats = at::empty({rows, 4}, options);
+        } else {
+            const at::Tensor all = at::empty({rows * (2 + k)}, options);
+            out[0] = piece(all, 0, rows);
+            out[1] = piece(all, rows, rows);
+            if (k) out[3] = piece(all, 2 * rows, rows * k).view({rows, k});
         }
         rc = g_logprobs(x->const_data_ptr(), float_code(*x), rows > 1 ? x->stride(0) : V, rows, V, tokens->const_data_ptr<int64_t>(), (float)temperature, (int)k,
                         out[0].mutable_data_ptr<float>(), out[1].mutable_data_ptr<float>(), k ? out[2].mutable_data_ptr<int64_t>() : nullptr,
-                        k ? out[3].mutable_data_ptr<float>() : nullptr, nullptr, stream_of(*x));
+                        k ? out[3].mutable_data_ptr<float>() : nullptr, grad ? stats.mutable_data_ptr<float>() : nullptr, stream_of(*x));
+        if (grad && rc == 0) {
+            const std::shared_ptr<TokenLogprobsBackward> node(new TokenLogprobsBackward(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(*x));
+            node->logits = torch::autograd::SavedVariable(*x, false);
+            node->tokens = torch::autograd::SavedVariable(*tokens, false);
+            node->stats = torch::autograd::SavedVariable(stats, false);
+            if (k) node->ids = torch::autograd::SavedVariable(out[2], false);
+            node->temperature = (float)temperature;
+            node->k = k;
+            torch::autograd::set_history(out[0], node);
+            torch::autograd::set_history(out[1], node);
+            if (k) torch::autograd::set_history(out[3], node);
+        }
     }
     if (rc) return PyLong_FromLong(rc);
     PyObject* const r = PyTuple_New(4);

@@ -213,9 +213,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
     Two sum = two(0.0f, 0.0f), dot = sum;                      // of powers, and of powers x exponents
     const Two c2 = two(c, c);
     auto follow = [&]() {
-        // the reference follows where an exponent would pass 2^20 of it: sums of powers up to that are as exact as those up to 1
+        // the reference follows where an exponent would pass 2^4 of it: rarely, and what the sums lose by it is four bits of their distance from 1
         const float top = big * c;
-        if (top > m + 20.0f && big > Vec<T>::kFloor) {
+        if (top > m + 4.0f && big > Vec<T>::kFloor) {
             const float a = m - top, w = ex2(a);
             if (w == 0.0f) {
                 // nothing that counts so far.  (The exponents of logits beyond 2^24 have lost their differences: whatever they gave goes, but for NaN)

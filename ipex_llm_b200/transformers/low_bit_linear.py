@@ -66,7 +66,7 @@ def _load_host():
                 module.attach_step(*(ctypes.cast(getattr(ggml._lib, f), ctypes.c_void_p).value
                                      for f in ("lowbit_paged_norm_rope_append_cuda", "lowbit_paged_fork_cuda", "lowbit_paged_share_release_workspace_size",
                                                "lowbit_paged_share_release_cuda", "lowbit_paged_compact_workspace_size", "lowbit_paged_compact_cuda", "lowbit_paged_copy_cuda",
-                                               "lowbit_lora_workspace_size", "lowbit_lora_add_cuda", "lowbit_token_logprobs_cuda")))
+                                               "lowbit_lora_workspace_size", "lowbit_lora_add_cuda", "lowbit_token_logprobs_cuda", "lowbit_token_logprobs_grad_cuda")))
                 _host = module
             except Exception as e:
                 warnings.warn(f"the native host side of LowBitLinear and attention is not available, its Python statements run instead: {e}")
