@@ -7,6 +7,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include "host_common.h"
 #include "paged_host.h"
 
@@ -52,6 +54,17 @@ bool stack_ok(const at::Tensor* pages, const at::Tensor* count, const at::Tensor
 }
 // rows of a matrix contiguous, apart and on 16 bytes
 bool rows_ok(const at::Tensor& t) { return aligned(t) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
+// whether matrices of as many rows share memory: columns of one buffer side by side do not
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    const int64_t rows = a.size(0), size = (int64_t)a.element_size(), wide_a = a.size(1) * size, wide_b = b.size(1) * size, step = rows > 1 ? a.stride(0) * size : 0;
+    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a.const_data_ptr()), pb = (int64_t)reinterpret_cast<uintptr_t>(b.const_data_ptr());
+    if (pa + (rows - 1) * step + wide_a <= pb || pb + (rows > 1 ? (rows - 1) * b.stride(0) * size : 0) + wide_b <= pa) return false;
+    if (rows <= 1 || a.stride(0) != b.stride(0)) return true;
+    const int64_t behind = ((pb - pa) % step + step) % step;
+    return behind < wide_a || behind + wide_b > step;
+}
+// autograd hears of what a kernel writes over (a tensor of inference mode keeps no count)
+void written(const at::Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 // a stack of adapters, each in one run on 16 bytes
 bool adapters_ok(const at::Tensor& t, int64_t each) {
     int64_t run = 1;
@@ -124,6 +137,7 @@ PyObject* paged_norm_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                     v ? v->mutable_data_ptr() : nullptr, vs, k && k->scalar_type() == at::kByte ? kE5m2 : dt, k ? (int)k->size(0) : 0, k ? (int)k->size(1) : 0, stream_of(*x));
     }
     if (rc) return PyLong_FromLong(rc);
+    written(*x);
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
@@ -288,7 +302,7 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (T <= 0 || out->size(0) != T || K <= 0 || K % 8 || K > most || N <= 0 || N > most || L <= 0 || L > most || R <= 0 || R % 8 || R > 256 || S <= 0 || S > 8 || wa->size(0) != L ||
         wa->size(wa->dim() - 2) != R || wa->size(wa->dim() - 1) != K || wb->size(1) != N || scales->scalar_type() != at::kFloat || scales->dim() != 1 || scales->size(0) != L ||
         !scales->is_contiguous() || scales->device() != x->device() || ids->dim() != 1 || ids->size(0) <= 0 || ids->size(0) > most || !ints(ids, ids->size(0), at::kInt, *x) ||
-        !ints(cu, ids->size(0) + 1, at::kInt, *x) || !rows_ok(*out) || !rows_ok(*x) || !adapters_ok(*wa, S * R * K) || !adapters_ok(*wb, N * R))
+        !ints(cu, ids->size(0) + 1, at::kInt, *x) || !rows_ok(*out) || !rows_ok(*x) || !adapters_ok(*wa, S * R * K) || !adapters_ok(*wb, N * R) || overlap(*out, *x))
         Py_RETURN_NONE;
     int splits[8] = {(int)N};
     if (a[7] != Py_None) {
@@ -314,6 +328,7 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                     (int)S, out->mutable_data_ptr(), T > 1 ? out->stride(0) : N, need ? scratch.mutable_data_ptr() : nullptr, need, stream_of(*x));
     }
     if (rc) return PyLong_FromLong(rc);
+    written(*out);
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
@@ -328,7 +343,14 @@ struct TokenLogprobsBackward : public torch::autograd::Node {
     std::string name() const override { return "TokenLogprobsBackward"; }
     void release_variables() override { logits.reset_data(); tokens.reset_data(); ids.reset_data(); stats.reset_data(); }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
-        const at::Tensor x = logits.unpack(), t = tokens.unpack(), s = stats.unpack(), i = k ? ids.unpack() : at::Tensor();
+        at::Tensor x = logits.unpack(), t = tokens.unpack(), s = stats.unpack(), i = k ? ids.unpack() : at::Tensor();
+        // a hook for saved tensors may have brought them back in another layout
+        if (x.stride(1) != 1 || (x.size(0) > 1 && x.stride(0) < x.size(1))) x = x.contiguous();
+        t = t.contiguous();
+        s = s.contiguous();
+        if (k) i = i.contiguous();
+        TORCH_CHECK(x.is_cuda() && t.device() == x.device() && s.device() == x.device() && float_code(x) >= 0 && s.scalar_type() == at::kFloat && t.scalar_type() == at::kLong &&
+                        (!k || (i.device() == x.device() && i.scalar_type() == at::kLong)), "what token_logprobs saved came back as something else");
         at::Tensor given[3], grad;
         const float* at[3] = {};
         for (size_t n = 0; n < grads.size() && n < 3; n++)
@@ -362,6 +384,12 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *x = plain(a[0]), *tokens = plain(a[1]);
     int64_t k;
     double temperature;
+    if (x && x->requires_grad() && x->is_leaf() && at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+        // the engine would make that node's stream wait for the recorded one, which ends the recording, and the process with it
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*x);
+        TORCH_CHECK(!node || node->stream() == c10::cuda::getCurrentCUDAStream(x->device().index()).unwrap(),
+                    "these logits have a gradient's node from outside the recording: let go of what was computed from them before");
+    }
     if (!x || x->dim() != 2 || float_code(*x) < 0 || x->_fw_grad(0).defined() || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature >= 1e-7) || !(temperature <= 1e7))
         Py_RETURN_NONE;
     const int64_t rows = x->size(0), V = x->size(1);

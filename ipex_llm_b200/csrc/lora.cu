@@ -8,7 +8,13 @@
 //   every block multiplies its share of the columns, h B^T, and adds that to `out`, rounded once.
 // Few tokens take one launch of that.  Many take two, the first product and the second, with h as two 16-bit values in memory between them: it costs little
 // beside `out`, each kernel has the registers that its product wants, and a tile's columns are dealt as finely as fills the device.
-// mma.sync m16n8k16: rank and tokens are far below a tcgen05 tile, and what bounds the kernel is what it reads and writes (x; out, twice).
+// mma.sync m16n8k16: a tcgen05 tile wants 128 rows of one adapter, which here have some 1 to 64, and x and B would have to pass through shared memory in its layout,
+// the adapters' rows gathered.  What the operator cannot do without is to read x and out, to write out, and the adapters' A and B once.
+//
+// Measured, times without the launch's share on the host.  One token of K 4096 and N 4096 at rank 16: 6.5 us, the latency of five dependent trips to memory and
+// the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 13.0 us (1.2 TB/s; a tile's clusters read their adapters by themselves).
+// 882 rows of 40 requests, K 4096 and N 11008 at rank 64: 24 + 32 us for 69 MB.  11849 rows, N 14336 at rank 32: 38 + 111 us for 628 MB, 4.3 TB/s.
+// The second launch there is a copy of `out` (88 us by itself) whose products (98 us by themselves) overlap it but for a fifth.
 #include "lowbit_common.cuh"
 #include "lowbit_internal.h"
 
@@ -475,9 +481,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     }
 }
 
-// Many tokens take two launches.
+// From here on two launches: 11849 rows 147 us, 171 by one launch; 882 of 40 requests 53 and 68.  64 tokens, as first built by two: 18, and 13
+// by one.
 constexpr int64_t LORA_MANY = 256;
-// splits that share a reading of x: 128 rows of A at most, or one split
+// splits that share a reading of x: 128 rows of A at most (their parts and h fill what shared memory two blocks of an SM have), or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
 size_t lora_tiles_bytes(int64_t T) { return (size_t)((T + TM - 1) / TM) * sizeof(Tile); }
 
@@ -494,11 +501,12 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     }
     const bool many = A.T > LORA_MANY;
     const int64_t tiles = (A.T + TM - 1) / TM;
-    // blocks, or clusters, that share a tile's adapters: twice as many as a tile has on average
+    // blocks, or clusters, that share a tile's adapters: twice as many as a tile has on average, since neighbours' differ; those that find none leave at once
     int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
     if (most > A.adapters) most = A.adapters;
     if (some > most) some = most;
-    // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes, fewer where the tiles fill the device
+    // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
+    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the tiles fill the device: 11849 rows by 2 blocks of a tile 152 us, by 4 159, by 8 178
     int blocks = 8;
     while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
     cudaLaunchConfig_t cfg = {};
@@ -515,7 +523,8 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
-        // blocks of a tile's columns: eight an SM's two places, none with fewer than three groups a warp
+        // blocks of a tile's columns: eight an SM's two places (11849 rows by 8 shares of a tile 147 us, by 4 150, by 16 173), none with fewer than three groups a
+        // warp, which would read h more often than it uses it
         const int64_t want = 8ll * sm_count() / tiles, room = A.first[A.n_splits] / (32 * LORA_WARPS * 3);
         A.shares = (int)(want < 8 ? 8 : want);
         if (A.shares > room) A.shares = (int)room;
@@ -527,6 +536,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     return check_launch();
 }
 
+// B in registers for the ranks that adapters mostly have; other steps would cost a kernel each for less
 template <bool BF> int lora_steps(const LoraArgs& A, cudaStream_t st) {
     return A.rank <= 16 ? lora_launch<BF, 1>(A, st) : A.rank <= 32 ? lora_launch<BF, 2>(A, st) : A.rank <= 64 && A.rank > 48 ? lora_launch<BF, 4>(A, st) : lora_launch<BF, 0>(A, st);
 }

@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(256) paged_norm_append_kernel(const NormArgs N
 }
 
 // Rows on 16 bytes: 16 elements a thread as in paged_append_vec_kernel, LANES (a power of two from D / 16 on) threads a head, whose squares meet by
-// shuffles.
+// shuffles.  Memory bounds it: 8001 tokens of 32 + 8 + 8 heads of 128, 217 MB, in 39.7 us (5.5 TB/s); 32 tokens 3.0 us.  Blocks an SM: 4, 5, 8, 16, one a piece:
+// 42.3, 39.7, 45.2, 44.6, 51.0 us (each fills its table of weights first).
 template <typename T, bool E5M2, typename C, int LANES>
 __global__ void __launch_bounds__(256) paged_norm_append_vec_kernel(const NormArgs N) {
     const AppendArgs& A = N.a;

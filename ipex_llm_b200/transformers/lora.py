@@ -18,18 +18,30 @@ def _rows_aligned(t):
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])
 
 
+def _overlap(a, b):
+    """whether matrices of as many rows share memory: columns of one buffer side by side do not"""
+    size, rows = a.element_size(), a.shape[0]
+    at = [(t.data_ptr(), t.data_ptr() + ((rows - 1) * t.stride(0) * (rows > 1) + t.shape[1]) * size) for t in (a, b)]
+    if at[0][1] <= at[1][0] or at[1][1] <= at[0][0]:
+        return False
+    if rows <= 1 or a.stride(0) != b.stride(0):
+        return True
+    behind = (at[1][0] - at[0][0]) % (a.stride(0) * size)
+    return behind < a.shape[1] * size or behind + b.shape[1] * size > a.stride(0) * size
+
+
 def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     """``out`` [T, N] += scale (x A^T) B^T for every row whose request has an adapter, in place; returns ``out``.
 
     ``x`` [T, K]; ``a`` [adapters, rank, K] and ``b`` [adapters, N, rank], all fp16 or all bf16; ``scales`` fp32 [adapters]; ``adapter_ids`` int32 [requests],
     outside [0, adapters): none, and such rows stay as they are; ``cu_seqlens`` int32 [requests + 1] (``PagedStep.cu_seqlens``): rows behind the last request
-    stay too.  The rank is a multiple of 8 up to 256 (adapters of a smaller one: rows of zeros), K and N multiples of 8.
+    stay too.  The rank is a multiple of 8 up to 256 (adapters of a smaller one: rows of zeros), K (at most 2^20) and N multiples of 8.
 
     ``splits``: the widths of the projections that ``out`` merges (queries, keys and values: 4096, 1024, 1024), each with an A of its own: ``a`` is then
     [adapters, len(splits), rank, K], and columns of a projection take the product with its A.
 
     x A^T is kept in 32 bits and enters the second product as two 16-bit values, so that only ``out`` is rounded, once.  One launch for up to 256 rows, two for more; nothing
-    comes back to the host, and the lists are read on the device: a recorded step serves other requests.  There is no backward pass: tensors that want a
+    comes back to the host, and the lists are read on the device: a recorded step serves other requests.  An ``x`` that shares memory with ``out`` is copied first.  There is no backward pass: tensors that want a
     gradient or carry a tangent are refused."""
     if splits is not None:
         splits = [int(n) for n in splits]
@@ -55,7 +67,8 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
                       f"x {list(x.shape)}, out {list(out.shape)}, a {list(a.shape)} and b {list(b.shape)} do not belong together")
     invalidInputError(0 < len(splits) <= SPLITS_MOST and len(splits) == S and sum(splits) == N and all(n > 0 and n % 8 == 0 for n in splits),
                       f"splits must be up to {SPLITS_MOST} multiples of 8, one for each A, that add up to {N}")
-    invalidInputError(0 < R <= RANK_MOST and R % 8 == 0 and K % 8 == 0 and K > 0, f"rank {R} and K {K} must be multiples of 8, the rank at most {RANK_MOST}")
+    invalidInputError(0 < R <= RANK_MOST and R % 8 == 0 and K % 8 == 0 and 0 < K <= 1 << 20,
+                      f"rank {R} and K {K} must be multiples of 8, the rank at most {RANK_MOST}, K at most 2^20")
     invalidInputError(scales.dtype == torch.float32 and scales.shape == (L,) and scales.is_contiguous(), f"scales must be a contiguous fp32 [{L}]")
     invalidInputError(adapter_ids.dtype == torch.int32 and adapter_ids.dim() == 1 and adapter_ids.is_contiguous() and adapter_ids.shape[0] > 0,
                       "adapter_ids must be a contiguous int32 [requests]")
@@ -64,11 +77,13 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     if T == 0:
         return out
     invalidInputError(_rows_aligned(out), "the rows of out must be contiguous and 16-byte aligned")
-    if not _rows_aligned(x):
+    if not _rows_aligned(x) or _overlap(out, x):
         x = x.clone(memory_format=torch.contiguous_format)
     a, b = (t if t[0].is_contiguous() and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and (t.shape[0] == 1 or t.stride(0) >= t[0].numel())
             else t.clone(memory_format=torch.contiguous_format) for t in (a, b))
     with torch.cuda.device(dev):
         ws = torch.empty(ggml.lowbit_lora_workspace_size(T, R, S), dtype=torch.uint8, device=dev)
         ggml.lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, ws, torch._C._cuda_getCurrentRawStream(dev.index))
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     return out

@@ -339,6 +339,8 @@ def paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, q_weight, k_weigh
         return
     with torch.cuda.device(dev):
         ggml.lowbit_paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache, _stream(dev))
+    if not qkv.is_inference():
+        torch.autograd.graph.increment_version(qkv)
 
 
 def _attention_args(query, n_kv_heads, cu_seqlens, scale, out):

@@ -3,7 +3,7 @@
 Bounds.  The exponent of an element is one multiply-add of the logit and the factor log2 e / temperature, which is itself rounded: off by 2^-22 of the
 largest |z| / temperature of its row in all; the power adds 2^-22 and the sum of a row's V powers one rounding, 2^-24, for each of the V / 256 / 4 pieces
 that a thread adds up and some 40 where threads and blocks meet.  A log probability is off by that sum; an entropy by the same, weighted with the mean distance
-of an exponent from the reference, below H + 40 (the reference follows the maximum within 2^20, and the sum is below 2^37); a gradient by that of its
+of an exponent from the reference, below H + 40 (the reference follows the maximum within 2^4, and the sum is below 2^32); a gradient by that of its
 probabilities, and is rounded once, finfo(t).eps / 2."""
 import math
 
@@ -327,6 +327,97 @@ def test_recorded_with_its_gradient(lp, cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+@pytest.mark.gpu
+def test_no_recording_beside_a_living_graph(lp, cuda_device):
+    """the refusal of what the engine could not record, by the node alone: nothing of it is launched"""
+    for shape in ((20, 301), (4, 5, 301)):
+        leaf = torch.randn(shape, device=cuda_device).requires_grad_()
+        tokens = torch.zeros(shape[:-1], dtype=torch.int64, device=cuda_device)
+        alive = lp.token_logprobs(leaf, tokens)
+        with pytest.raises(RuntimeError, match="outside the recording"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                lp.token_logprobs(leaf, tokens)
+        alive.logprobs.sum().backward()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            grad, = torch.autograd.grad(lp.token_logprobs(leaf, tokens).logprobs.sum(), leaf)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, leaf.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_python_statements_say_the_same(lp, cuda_device, monkeypatch, dtype):
+    """what serves where the native host side is not to be had; three dimensions go through it"""
+    logits, tokens = make(24, 3001, dtype, cuda_device, 0.2)
+    w = torch.randn(24, 7, device=cuda_device)
+    results = []
+    for native, shape in ((True, (24,)), (True, (4, 6)), (False, (24,)), (False, (2, 3, 4))):
+        monkeypatch.setattr(lp.paged_kv, "_native", lp.paged_kv._native if native else lambda *args: None)
+        for k in (0, 5):
+            leaf = logits.clone().view(*shape, 3001).requires_grad_()
+            got = lp.token_logprobs(leaf, tokens.view(shape), k, 0.8)
+            loss = (got.logprobs.flatten() * w[:, 0]).sum() + (got.entropy.flatten() * w[:, 1]).sum()
+            if k:
+                loss = loss + (got.top_logprobs.view(24, 5) * w[:, 2:]).sum()
+            loss.backward()
+            with torch.no_grad():
+                again = lp.token_logprobs(leaf, tokens.view(shape), k, 0.8)
+            results.append([t.detach().reshape(24, -1) for t in (*got, *again, leaf.grad) if t is not None])
+    for i, r in enumerate(results):
+        assert len(r) == len(results[i % 2]) and all(torch.equal(a, b) for a, b in zip(r, results[i % 2]))
+
+
+@pytest.mark.gpu
+def test_outputs_by_themselves_and_saved_elsewhere(lp, cuda_device):
+    """a gradient of one output, none of the others; what was saved comes back from the host, or in another layout; a parameter; twice through one graph"""
+    logits, tokens = make(9, 2000, torch.float32, cuda_device)
+    def grad_of(what, hooks=None, parameter=False):                                               # noqa: E306
+        leaf = torch.nn.Parameter(logits.clone()) if parameter else logits.clone().requires_grad_()
+        with hooks or torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+            got = lp.token_logprobs(leaf, tokens, 4)
+        sum(getattr(got, n).sum() for n in what).backward(retain_graph=True)
+        first = leaf.grad.clone()
+        leaf.grad = None
+        sum(getattr(got, n).sum() for n in what).backward()
+        assert torch.equal(first, leaf.grad)
+        with pytest.raises(RuntimeError, match="second time"):
+            sum(getattr(got, n).sum() for n in what).backward()
+        return first
+    turned = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t)
+    for what in (["logprobs"], ["entropy"], ["top_logprobs"], ["entropy", "logprobs"]):
+        want = grad_of(what)
+        assert torch.equal(grad_of(what, torch.autograd.graph.save_on_cpu()), want)
+        assert torch.equal(grad_of(what, turned), want) and torch.equal(grad_of(what, parameter=True), want)
+
+
+@pytest.mark.gpu
+def test_calls_at_once_from_threads(lp, cuda_device):
+    import threading
+    jobs = [make(5 + i, 9000 + i, torch.bfloat16, cuda_device) for i in range(6)]
+    want = [lp.token_logprobs(x, t, 7) for x, t in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                leaf = jobs[i][0].clone().requires_grad_()
+                got = lp.token_logprobs(leaf, jobs[i][1], 7)
+                got.logprobs.sum().backward()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])) or not bool(torch.isfinite(leaf.grad).all()):
+                    wrong.append(i)
+    torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.gpu

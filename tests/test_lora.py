@@ -220,6 +220,81 @@ def test_a_recorded_call_serves_other_requests(lora, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [255, 256, 257, 321])
+@pytest.mark.parametrize("rank", [8, 48, 64, 136])
+def test_where_the_launches_change(lora, cuda_device, rows, rank):
+    lens, ids = [rows - 70, 1, 69], [2, 0, 1]
+    check(lora, make(lens, ids, 520, [264, 8], rank, 3, torch.float16, cuda_device), lens, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_the_python_statements_say_the_same(lora, cuda_device, monkeypatch, rows):
+    s = make([rows], [1], 256, [128, 64], 16, 2, torch.bfloat16, cuda_device)
+    native = run(lora, s)
+    monkeypatch.setattr(lora.paged_kv, "_native", lambda *args: None)
+    assert torch.equal(run(lora, s), native)
+    whole = {**s, "splits": [192], "a": s["a"][:, :1].contiguous()}
+    assert torch.equal(run(lora, {**whole, "a": whole["a"][:, 0], "splits": None}), check(lora, whole, [rows], [1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 7, 300])
+@pytest.mark.parametrize("native", [True, False])
+def test_rows_that_share_memory(lora, cuda_device, monkeypatch, rows, native):
+    """the output is the input, lies some way into it, or beside it in one buffer"""
+    if not native:
+        monkeypatch.setattr(lora.paged_kv, "_native", lambda *args: None)
+    s = make([rows], [0], 256, [256], 16, 1, torch.float16, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    buffer = torch.randn(rows + 3, 768, generator=g, device=cuda_device).half()
+    for x_at, out_at in (((0, 0), (0, 0)), ((0, 0), (0, 128)), ((0, 128), (0, 0)), ((0, 0), (1, 0)), ((0, 0), (0, 256)), ((0, 512), (0, 0)), ((0, 0), (2, 640))):
+        flat = buffer.clone().view(-1)
+        x, out = (flat.as_strided((rows, 256), (768, 1), 768 * r + c) for r, c in (x_at, out_at))
+        case = {**s, "x": x.clone(), "out": out.clone()}
+        want = run(lora, case)
+        lora.lora_add_(out, x, s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_autograd_hears_of_it(lora, cuda_device, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(lora.paged_kv, "_native", lambda *args: None)
+    s = make([3], [0], 64, [64], 8, 1, torch.float16, cuda_device)
+    w = torch.ones(64, device=cuda_device, dtype=torch.float16, requires_grad=True)
+    out = s["out"].clone()
+    y = out * w
+    lora.lora_add_(out, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], splits=[64])
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        fresh = s["out"].clone()
+    lora.lora_add_(fresh, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], splits=[64])
+    assert torch.equal(fresh, out)
+
+
+@pytest.mark.gpu
+def test_calls_at_once_from_threads(lora, cuda_device):
+    import threading
+    jobs = [make([50 * i + 1, 20], [0, 1], 512, [256], 16, 2, torch.bfloat16, cuda_device) for i in range(6)]
+    want = [run(lora, s) for s in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            wrong.extend(i for _ in range(20) if not torch.equal(run(lora, jobs[i]), want[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
 def test_refusals(lora, cuda_device):
     s = make([3, 2], [0, 1], 64, [32, 32], 16, 2, torch.float16, cuda_device)
     names = ("out", "x", "a", "b", "scales", "ids", "cu")
@@ -254,7 +329,7 @@ def test_refusals_on_the_cpu(lora, native_lib):
     lib, some = native_lib._lib, 4096                                  # never read: every call is refused before anything is launched
     splits = (ctypes.c_int * 2)(32, 32)
     good = [some, 64, 1, 5, 64, some, 2 * 16 * 64, some, 64 * 16, 16, some, 2, some, some, 2, splits, 2, some, 64, None, 0, None]
-    for i, bad in ((0, None), (0, 4100), (1, 56), (1, 68), (2, 0), (3, -1), (3, 1 << 40), (4, 60), (4, 0), (5, None), (6, 100), (7, None), (8, 100), (9, 12), (9, 264), (9, 0), (10, None), (11, 0),
+    for i, bad in ((0, None), (0, 4100), (1, 56), (1, 68), (2, 0), (3, -1), (3, 1 << 40), (4, 60), (4, 0), (4, (1 << 20) + 8), (5, None), (6, 100), (7, None), (8, 100), (9, 12), (9, 264), (9, 0), (10, None), (11, 0),
                    (12, None), (13, None), (14, 0), (15, None), (15, (ctypes.c_int * 2)(32, 12)), (15, (ctypes.c_int * 2)(64, 0)), (16, 0), (16, 9), (17, None), (17, 4104), (18, 56)):
         args = list(good)
         args[i] = bad

@@ -492,6 +492,49 @@ def test_on_other_streams_at_once(paged, cuda_device):
         assert table.tolist() == want[0] and stack[:len(want[1])].tolist() == want[1] and c.block_table.tolist() == moved[0] and c.src[:len(moved[3])].tolist() == [u for u, _ in moved[3]]
 
 
+@pytest.mark.gpu
+def test_the_python_statements_say_the_same(paged, cuda_device, monkeypatch):
+    """what serves where the native host side is not to be had"""
+    dev, page, width, R, pages = cuda_device, 4, 6, 8, 60
+    i = lambda x: dev_ints(x, dev)                                                                # noqa: E731
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(paged, "_native", lambda *args: None)
+        for in_place in (False, True):
+            table, stack, count = torch.full((R, width + 3), -1, dtype=torch.int32, device=dev)[:, :width], torch.arange(pages, dtype=torch.int32, device=dev), i([pages])
+            shared, held = torch.zeros(pages, dtype=torch.int32, device=dev), i([9, 4, 23, 0, 0, 0, 0, 0])
+            st = paged.paged_step(held, torch.zeros_like(held), table, stack, count, page, 36, free_left=count)
+            g = torch.Generator(device=dev).manual_seed(5)
+            caches = [torch.zeros(pages, page, 2, 64, dtype=torch.float16, device=dev) for _ in range(2)]
+            qkv, w, cos = torch.randn(36, 8 * 64, generator=g, device=dev).half(), torch.rand(64, generator=g, device=dev), torch.rand(50, 32, generator=g, device=dev)
+            paged.paged_norm_rope_append(qkv, 4, 2, 64, w, w, 1e-6, cos, cos, st.positions, st.slots, *caches)
+            bare = qkv.clone()
+            paged.paged_norm_rope_append(bare, 4, 2, 64, w, w, 1e-6, None, None, None, None, None, None)
+            f = paged.paged_fork(i([0, 0, 2]), i([4, 5, 6]), held, table, stack, count, shared, page, free_left=count if in_place else None)
+            count = f.free_count
+            paged.paged_copy(f.src, f.dst, caches)
+            paged.paged_release(torch.tensor([0, 0, 1, 0, 1, 0, 0, 0], dtype=torch.uint8, device=dev), table, stack, count, held=i([0, 0, 5, 0, 0, 0, 0, 0]), page_size=page, shared=shared)
+            paged.paged_release(torch.tensor([1, 0, 0, 0, 0, 0, 0, 0], dtype=torch.bool, device=dev), table, stack, count, shared=shared)
+            c = paged.paged_compact(table, stack, count, shared)
+            results.append((*f, *c, *paged.paged_compact(table, stack, count)[:3], table.clone(), shared, held, qkv, bare, *caches))
+    for r in results[1:]:
+        assert len(r) == len(results[0]) and all(torch.equal(a, b) for a, b in zip(r, results[0]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_autograd_hears_of_the_norms(paged, cuda_device, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(paged, "_native", lambda *args: None)
+    qkv = torch.randn(3, 256, device=cuda_device).half()
+    w, scale = torch.ones(64, device=cuda_device), torch.ones(256, device=cuda_device, dtype=torch.float16, requires_grad=True)
+    y = qkv * scale
+    paged.paged_norm_rope_append(qkv, 2, 1, 64, w, w, 1e-6, None, None, None, None, None, None)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
 # ------------------------------------------------------------------ refusals
 @pytest.mark.gpu
 def test_refusals(paged, cuda_device):
@@ -543,12 +586,12 @@ def test_refusals_on_the_cpu(paged, native_lib):
             args[at] = value
             assert getattr(lib, name)(*args) == code, (name, at, value)
     refused("lowbit_paged_fork_cuda", [some, some, 2, some, some, 4, 3, 4, some, 9, some, some, some, 16, some, some, some, None],
-            [(a, None) for a in (0, 1, 3, 4, 8, 10, 11, 12, 14, 15, 16)] + [(2, 0), (5, 3), (6, 0), (7, 0), (9, 0), (13, 0)])
+            [(a, None) for a in (0, 1, 3, 4, 8, 10, 11, 12, 14, 15, 16)] + [(2, 0), (2, (1 << 30) + 1), (5, 3), (6, 0), (6, (1 << 28) + 1), (7, 0), (9, 0), (9, (1 << 30) + 1), (13, 0)])
     refused("lowbit_paged_share_release_cuda", [some, some, 4, 3, some, 4, 4, some, 9, some, some, some, 1 << 20, None],
-            [(a, None) for a in (0, 4, 7, 9, 10)] + [(2, 0), (3, 0), (5, 3), (6, 0), (8, 0)])
+            [(a, None) for a in (0, 4, 7, 9, 10)] + [(2, 0), (3, 0), (5, 3), (6, 0), (8, 0), (8, (1 << 30) + 1)])
     refused("lowbit_paged_share_release_cuda", [some, some, 4, 3, some, 4, 4, some, 9, some, some, some, 1 << 20, None], [(11, None), (11, 4098), (12, 87)], 4)
     refused("lowbit_paged_compact_cuda", [some, 4, 3, 4, some, 9, some, some, some, some, some, some, some, some, some, 1 << 20, None],
-            [(a, None) for a in (0, 4, 6, 7, 8, 9, 10, 11, 12, 13)] + [(1, 3), (2, 0), (3, 0), (5, 0)])
+            [(a, None) for a in (0, 4, 6, 7, 8, 9, 10, 11, 12, 13)] + [(1, 3), (2, 0), (3, 0), (5, 0), (5, (1 << 30) + 1)])
     refused("lowbit_paged_compact_cuda", [some, 4, 3, 4, some, 9, some, some, some, some, some, some, some, some, some, 1 << 20, None], [(14, None), (15, 143)], 4)
     at = (ctypes.c_void_p * 1)(some)
     refused("lowbit_paged_copy_cuda", [some, some, 2, at, 1, 9, 64, 64, None], [(0, None), (1, None), (2, -1), (3, None), (4, -1), (5, 0), (6, 63), (7, 0), (3, (ctypes.c_void_p * 1)(None))])
