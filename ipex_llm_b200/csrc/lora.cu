@@ -238,10 +238,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                             const uint4 xr = lds16(at + n * 512);
 #pragma unroll
                             for (int m = 0; m < MT; m++)
-                                if (m < m_end) {
-                                    mma<BF>(acc[m][n], wr[m][0].x, wr[m][1].x, wr[m][0].y, wr[m][1].y, xr.x, xr.y);
-                                    mma<BF>(acc[m][n], wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w, xr.z, xr.w);
-                                }
+                                if (m < m_end) mma<BF>(acc[m][n], wr[m][0].x, wr[m][1].x, wr[m][0].y, wr[m][1].y, xr.x, xr.y);
+#pragma unroll
+                            for (int m = 0; m < MT; m++)
+                                if (m < m_end) mma<BF>(acc[m][n], wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w, xr.z, xr.w);
                         }
                     ask(c + 2 * LORA_WARPS, stage);
                 }
@@ -424,55 +424,85 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                 uint4* const to = out + col / 8;
                 const uint32_t h0 = hs + now.s * steps * L::kStep + lane * 16, o0 = ring + stage * L::kStage;
                 const int rows_here = col < now.c_end ? count - g : 0;
-                // 32 tokens at a time
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                // 16 tokens at a time; what the next ones need of h is asked for behind the products, ahead of what is done with them.  With B as it comes 32
+                constexpr int P = STEPS ? 1 : 2;
+                constexpr bool EARLY = STEPS == 1 || STEPS == 2;                                    // four steps of h and of B are more than the registers hold
+                constexpr int S = EARLY ? STEPS : 1;
+                uint4 hi[S][P], lo[S][P];
+                auto ask_h = [&](int m, int st, uint4 (&hi_)[P], uint4 (&lo_)[P]) {
 #pragma unroll
-                for (int m0 = 0; m0 < TM / 16; m0 += 2) {
-                    if (m0 >= m_tiles) break;
-                    float acc[2][4][4];
-                    auto products = [&](int st, bool first) {
+                    for (int q = 0; q < P; q++)
+                        if (m + q < m_tiles) {
+                            const uint32_t h = h0 + st * L::kStep + (m + q) * L::kFrag;
+                            hi_[q] = lds16(h);
+                            lo_[q] = lds16(h + L::kFrag / 2);
+                        }
+                };
+                if constexpr (EARLY) {
 #pragma unroll
-                        for (int m = 0; m < 2; m++)
-                            if (m0 + m < m_tiles) {
-                                const uint32_t h = h0 + st * L::kStep + (m0 + m) * L::kFrag;
-                                const uint4 hi = lds16(h), lo = lds16(h + L::kFrag / 2);
+                    for (int st = 0; st < STEPS; st++) ask_h(0, st, hi[st], lo[st]);
+                }
+#pragma unroll
+                for (int m = 0; m < TM / 16; m += P) {
+                    if (m >= m_tiles) break;
+                    uint4 o[P][2];
+#pragma unroll
+                    for (int q = 0; q < P; q++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) o[q][h] = lds16(o0 + (2 * (m + q) + h) * 512);
+                    float acc[P][4][4];
+                    auto products = [&](const uint4 (&hi_)[P], const uint4 (&lo_)[P], const uint2 (&b)[4], bool first) {
+#pragma unroll
+                        for (int q = 0; q < P; q++)
+                            if (m + q < m_tiles) {
 #pragma unroll
                                 for (int n = 0; n < 4; n++) {
-                                    const uint2 b = br[STEPS ? st : 0][n];
-                                    if (first) mma0<BF>(acc[m][n], lo.x, lo.z, lo.y, lo.w, b.x, b.y);
-                                    else mma<BF>(acc[m][n], lo.x, lo.z, lo.y, lo.w, b.x, b.y);
-                                    mma<BF>(acc[m][n], hi.x, hi.z, hi.y, hi.w, b.x, b.y);
+                                    if (first) mma0<BF>(acc[q][n], lo_[q].x, lo_[q].z, lo_[q].y, lo_[q].w, b[n].x, b[n].y);
+                                    else mma<BF>(acc[q][n], lo_[q].x, lo_[q].z, lo_[q].y, lo_[q].w, b[n].x, b[n].y);
                                 }
+#pragma unroll
+                                for (int n = 0; n < 4; n++) mma<BF>(acc[q][n], hi_[q].x, hi_[q].z, hi_[q].y, hi_[q].w, b[n].x, b[n].y);
                             }
                     };
                     if constexpr (STEPS > 0) {
 #pragma unroll
-                        for (int st = 0; st < STEPS; st++) products(st, st == 0);
-                        if (more && m0 + 2 >= m_tiles) {       // the products have B: the next group's
+                        for (int st = 0; st < STEPS; st++) {
+                            if (!EARLY) ask_h(m, st, hi[0], lo[0]);
+                            products(hi[EARLY ? st : 0], lo[EARLY ? st : 0], br[st], st == 0);
+                        }
+                        if (m + 1 < m_tiles && m + 1 < TM / 16) {
+                            if constexpr (EARLY) {
+#pragma unroll
+                                for (int st = 0; st < STEPS; st++) ask_h(m + 1, st, hi[st], lo[st]);
+                            }
+                        } else if (more) {                     // the products have B: the next group's
 #pragma unroll
                             for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
                         }
                     } else {
                         fetch(now, 0, br[0]);
-                        products(0, true);
+                        ask_h(m, 0, hi[0], lo[0]);
+                        products(hi[0], lo[0], br[0], true);
 #pragma unroll 1
                         for (int st = 1; st < steps; st++) {
                             fetch(now, st, br[0]);
-                            products(st, false);
+                            ask_h(m, st, hi[0], lo[0]);
+                            products(hi[0], lo[0], br[0], false);
                         }
                     }
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
-                    for (int m = 0; m < 2; m++)
+                    for (int q = 0; q < P; q++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int i = 16 * (m0 + m) + 8 * h;
+                            const int i = 16 * (m + q) + 8 * h;
                             if (i >= rows_here) continue;
-                            const uint4 o = lds16(o0 + (2 * (m0 + m) + h) * 512);
-                            uint32_t v[4] = {o.x, o.y, o.z, o.w};
+                            uint32_t v[4] = {o[q][h].x, o[q][h].y, o[q][h].z, o[q][h].w};
                             const float up = BF ? 1.0f : back[i + g][now.s];
 #pragma unroll
-                            for (int n = 0; n < 4; n++) v[n] = add2<BF>(v[n], BF ? acc[m][n][2 * h] : acc[m][n][2 * h] * up, BF ? acc[m][n][2 * h + 1] : acc[m][n][2 * h + 1] * up);
-                            to[row_at[2 * (m0 + m) + h]] = make_uint4(v[0], v[1], v[2], v[3]);
+                            for (int n = 0; n < 4; n++)
+                                v[n] = add2<BF>(v[n], BF ? acc[q][n][2 * h] : acc[q][n][2 * h] * up, BF ? acc[q][n][2 * h + 1] : acc[q][n][2 * h + 1] * up);
+                            to[row_at[2 * (m + q) + h]] = make_uint4(v[0], v[1], v[2], v[3]);
                         }
                 }
             }
