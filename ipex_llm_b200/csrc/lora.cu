@@ -1,12 +1,13 @@
 // lora.cu -- low-rank adapters of many requests beside a projection that all share:
 //   out[t] += scale_l (x[t] A_l^T) B_l^T,      l = the adapter of the token's request (none: the row stays as it is).
 //
-// A cluster takes a tile of packed rows, whoever they belong to: it finds the tile's requests in the list, and the different adapters among
-// its rows are dealt to the clusters that share the tile.  So an adapter that neighbours have in common is read once for them, and nobody sorts.  For each:
+// A cluster takes up to 64 rows of one adapter, wherever they lie.  Few tokens: it takes a tile of packed rows, finds the tile's requests in the list, and the different
+// adapters among its rows are dealt to the clusters that share the tile.  Many: a launch in front orders all rows by their adapters.  So an adapter that requests
+// have in common is read once for 64 rows of theirs.  For each:
 //   every block multiplies its share of the inner dimension, h = x A^T in 32 bits;
 //   the blocks add up their parts, a share of the rows each, and hand the sums to all through their shared memories;
 //   every block multiplies its share of the columns, h B^T, and adds that to `out`, rounded once.
-// Few tokens take one launch of that.  Many take two, the first product and the second, with h as two 16-bit values in memory between them: it costs little
+// Few tokens take one launch of that.  Many take one for each product, with h as two 16-bit values in memory between them: it costs little
 // beside `out`, each kernel has the registers that its product wants, and a tile's columns are dealt as finely as fills the device.
 // mma.sync m16n8k16: a tcgen05 tile wants 128 rows of one adapter, which here have some 1 to 64, and x and B would have to pass through shared memory in its layout,
 // the adapters' rows gathered.  What the operator cannot do without is to read x and out, to write out, and the adapters' A and B once.
@@ -15,6 +16,7 @@
 // the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 13.0 us (1.2 TB/s; a tile's clusters read their adapters by themselves).
 // 882 rows of 40 requests, K 4096 and N 11008 at rank 64: 24 + 32 us for 69 MB.  11849 rows, N 14336 at rank 32: 38 + 111 us for 628 MB, 4.3 TB/s.
 // The second launch there is a copy of `out` (88 us by itself) whose products (98 us by themselves) overlap it but for a fifth.
+#include <type_traits>
 #include "lowbit_common.cuh"
 #include "lowbit_internal.h"
 
@@ -33,7 +35,9 @@ struct LoraArgs {
     const int32_t *ids, *cu; int R;                            // requests
     void* out; int64_t o_st;
     int rank, n_splits, together;                              // splits whose products with A are computed at once
-    uint8_t* tiles; uint16_t* h; float* back; int shares;      // of two launches: the tiles' lists and h between them, blocks of a tile in the second
+    // of more launches: the pieces (adapter, first of its rows in the order of adapters, how many, 0), the rows in that order, h and what undoes its powers of
+    // two between the products, blocks of a piece in the second product
+    int4* pieces; int32_t* order; int32_t* lists; uint16_t* h; float* back; int shares;
     int first[LORA_SPLITS + 1];                                // columns in front of a split
 };
 
@@ -87,8 +91,9 @@ constexpr int TM = 64;                                         // rows of a tile
 struct __align__(16) Tile {
     int id[TM];                                                // of the request that begins in a row; -2: none does
     int n, adapter[TM], first[TM + 1];
-    uint8_t row[TM];
+    int row[TM];
 };
+struct Rows { int row[TM]; };                                  // of a piece
 // the whole block; ends behind a barrier
 __device__ __forceinline__ void find_adapters(const LoraArgs& A, int64_t t0, Tile& tile) {
     const int lane = threadIdx.x & 31;
@@ -116,8 +121,8 @@ __device__ __forceinline__ void find_adapters(const LoraArgs& A, int64_t t0, Til
             if (!(left | more)) break;
             const int id = left ? __shfl_sync(0xffffffffu, v[0], __ffs(left) - 1) : __shfl_sync(0xffffffffu, v[1], __ffs(more) - 1);
             const uint32_t here = __ballot_sync(0xffffffffu, v[0] == id), there = __ballot_sync(0xffffffffu, v[1] == id);
-            if (v[0] == id) { tile.row[at + __popc(here & under)] = (uint8_t)lane; v[0] = -1; }
-            if (v[1] == id) { tile.row[at + __popc(here) + __popc(there & under)] = (uint8_t)(lane + 32); v[1] = -1; }
+            if (v[0] == id) { tile.row[at + __popc(here & under)] = lane; v[0] = -1; }
+            if (v[1] == id) { tile.row[at + __popc(here) + __popc(there & under)] = lane + 32; v[1] = -1; }
             if (lane == 0) { tile.adapter[n] = id; tile.first[n] = at; }
             at += __popc(here) + __popc(there);
             n++;
@@ -161,7 +166,7 @@ template <bool BF, int STEPS, int DO>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
     constexpr int NT = DO == LORA_FIRST ? 8 : 4, TOKS = 8 * NT, MT = L::MT, ROWS = L::ROWS, STAGE = (NT + 2 * MT) * 512;      // of the first product
-    __shared__ Tile tile;
+    __shared__ std::conditional_t<DO == LORA_BOTH, Tile, Rows> tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
     extern __shared__ __align__(128) uint8_t lora_smem[];
     uint32_t rank = blockIdx.x % A.shares, blocks = A.shares;
@@ -170,26 +175,33 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
         asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
     }
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t t0 = (int64_t)(blockIdx.x / blocks) * TM;
+    const int64_t t0 = DO == LORA_BOTH ? (int64_t)(blockIdx.x / blocks) * TM : 0;
     const int steps = STEPS && DO != LORA_FIRST ? STEPS : L::steps(A.rank);
     float* const sums = reinterpret_cast<float*>(lora_smem);
     float* const part = reinterpret_cast<float*>(lora_smem + (DO == LORA_FIRST ? L::kRingFirst : L::kRing + A.together * steps * L::kStep));
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, ring1 = smem + warp * 2 * STAGE + lane * 16, hs = smem + L::kRing;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    if (DO == LORA_SECOND) {
-        const int4* const from = reinterpret_cast<const int4*>(A.tiles + (int64_t)(blockIdx.x / blocks) * sizeof(Tile));
-        for (int i = threadIdx.x; i < (int)(sizeof(Tile) / 16); i += LORA_THREADS) reinterpret_cast<int4*>(&tile)[i] = from[i];
+    int4 piece = {};
+    int n_adapters = 1;
+    if constexpr (DO == LORA_BOTH) {
+        find_adapters(A, t0, tile);
+        n_adapters = tile.n;
+    } else {
+        piece = A.pieces[blockIdx.x / blocks];
+        if (piece.z == 0) return;                              // the whole cluster
+        if (threadIdx.x < TM) tile.row[threadIdx.x] = A.order[piece.y + min((int)threadIdx.x, piece.z - 1)];
         __syncthreads();
-    } else find_adapters(A, t0, tile);
-    if (DO == LORA_FIRST && rank == 0 && blockIdx.y == 0) {
-        int4* const to = reinterpret_cast<int4*>(A.tiles + (int64_t)(blockIdx.x / blocks) * sizeof(Tile));
-        for (int i = threadIdx.x; i < (int)(sizeof(Tile) / 16); i += LORA_THREADS) to[i] = reinterpret_cast<const int4*>(&tile)[i];
     }
     const int chunks = (A.K + 31) / 32, each = (chunks + (int)blocks - 1) / (int)blocks, from = min((int)rank * each, chunks), to = min(from + each, chunks);
-    for (int j = blockIdx.y; j < tile.n; j += gridDim.y) {
-        const int id = tile.adapter[j], count = tile.first[j + 1] - tile.first[j];
-        const uint8_t* const row_of = tile.row + tile.first[j];
+    for (int j = blockIdx.y; j < n_adapters; j += gridDim.y) {
+        int id = piece.x, count = piece.z;
+        const int* row_of = tile.row;
+        if constexpr (DO == LORA_BOTH) {
+            id = tile.adapter[j];
+            count = tile.first[j + 1] - tile.first[j];
+            row_of += tile.first[j];
+        }
         const float scale = A.scales[id];
         for (int s0 = 0; s0 < A.n_splits; s0 += A.together) {
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
@@ -291,7 +303,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                 }
             };
             const int m_tiles = (count + 15) / 16;
-            uint32_t row_at[TM / 8];                           // rows 8 i + g of the adapter's, in 16 bytes from the tile's first on
+            uint32_t row_at[TM / 8];                           // rows 8 i + g of the adapter's, in 16 bytes from t0 on
 #pragma unroll
             for (int i = 0; i < TM / 8; i++) row_at[i] = (uint32_t)(row_of[min(8 * i + g, count - 1)] * A.o_st / 8);
             uint4* const out = reinterpret_cast<uint4*>((uint16_t*)A.out + t0 * A.o_st);
@@ -329,7 +341,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const float up = __uint_as_float((uint32_t)(127 + use) << 23);
                     down = __uint_as_float((uint32_t)(127 - use) << 23);
                     if (DO == LORA_FIRST) {
-                        if (lane == 0) A.back[(t0 + row_of[tok]) * A.n_splits + s0 + s] = up;
+                        if (lane == 0) A.back[(int64_t)(piece.y + tok) * A.n_splits + s0 + s] = up;
                     } else if (lane < (int)others) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(up) : "memory");
                 }
 #pragma unroll
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const float2 f = unpack2<BF>(hi);
                     const uint32_t lo = pack2<BF>(fabsf(f.x) < INFINITY ? x - f.x : 0.0f, fabsf(f.y) < INFINITY ? y - f.y : 0.0f);
                     if (DO == LORA_FIRST) {
-                        uint16_t* const to = A.h + (t0 + row_of[tok]) * (A.n_splits * 32 * steps) + (s0 + s) * 32 * steps + r;
+                        uint16_t* const to = A.h + (int64_t)(piece.y + tok) * (A.n_splits * 32 * steps) + (s0 + s) * 32 * steps + r;
                         *reinterpret_cast<uint32_t*>(to) = hi;
                         *reinterpret_cast<uint32_t*>(to + 16 * steps) = lo;
                     } else {
@@ -360,13 +372,13 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                 const int pieces = n_here * steps * 4;         // of a row: two of high parts, two of low ones a step
                 for (int i = threadIdx.x; i < count * pieces; i += LORA_THREADS) {
                     const int tok = i / pieces, in = i - tok * pieces, s = in / (4 * steps), half = in / (2 * steps) & 1, r = in % (2 * steps) * 8;
-                    const uint4 v = *reinterpret_cast<const uint4*>(A.h + (t0 + row_of[tok]) * (A.n_splits * 32 * steps) + s0 * 32 * steps + in * 8);
+                    const uint4 v = *reinterpret_cast<const uint4*>(A.h + (int64_t)(piece.y + tok) * (A.n_splits * 32 * steps) + s0 * 32 * steps + in * 8);
                     const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + half * (L::kFrag / 2) + ((tok & 7) * 4 + (r & 8) / 4) * 16 + (tok & 8);
                     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
                     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + 16), "r"(v.z), "r"(v.w) : "memory");
                 }
                 if (!BF)
-                    for (int i = threadIdx.x; i < count * n_here; i += LORA_THREADS) back[i / n_here][i % n_here] = A.back[(t0 + row_of[i / n_here]) * A.n_splits + s0 + i % n_here];
+                    for (int i = threadIdx.x; i < count * n_here; i += LORA_THREADS) back[i / n_here][i % n_here] = A.back[(int64_t)(piece.y + i / n_here) * A.n_splits + s0 + i % n_here];
             } else {
                 for (int i = (int)rank + warp * (int)blocks; i < count * n_here; i += LORA_WARPS * (int)blocks) {
                     const int tok = i % count, s = i / count;
@@ -511,14 +523,133 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     }
 }
 
-// From here on two launches: 11849 rows 147 us, 171 by one launch; 882 of 40 requests 53 and 68.  64 tokens, as first built by two: 18, and 13
-// by one.
+// ------------------------------------------------------------------ many tokens: the rows ordered by their adapters
+constexpr int SORT_THREADS = 1024, SORT_HERE = 4096;           // adapters whose lists lie in shared memory
+template <bool MOST> __device__ __forceinline__ int scan(int x, int* warps, int& all) {        // inclusive sums, or maxima, over the block; all: of the whole block
+    auto both = [](int a, int b) { return MOST ? max(a, b) : a + b; };
+    constexpr int none = MOST ? (int)0x80000000 : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x = both(x, y);
+    }
+    __syncthreads();
+    if (lane == 31) warps[warp] = x;
+    __syncthreads();
+    int w = warps[lane];                                       // 32 warps
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, d);
+        if (lane >= d) w = both(w, y);
+    }
+    all = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    return both(x, warp ? before : none);
+}
+// One block: rows counted by adapter, a place for each adapter's, the pieces of 64, the rows written to their places.  In which order the rows of an adapter lie is
+// chance, and nothing depends on it: a row's sums are its own.  Rows [row0, row0 + rows) count from 0; n_pieces: room for pieces.
+__global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraArgs A, int64_t row0, int rows, int n_pieces) {
+    __shared__ int warps[32];
+    __shared__ int here[2][SORT_HERE];
+    __shared__ int few[SORT_THREADS], few_n[SORT_THREADS], few_at[SORT_THREADS];               // stretches of rows: for a warp each from the front, for the block from the back
+    __shared__ int n_few, n_more;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int* const place = A.adapters <= SORT_HERE ? here[0] : A.lists;                           // rows of an adapter, then where they begin
+    int* const before = A.adapters <= SORT_HERE ? here[1] : A.lists + A.adapters;              // pieces of the adapters in front
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (int a = t; a < A.adapters; a += SORT_THREADS) place[a] = 0;
+    const int64_t end = min((int64_t)A.cu[A.R], row0 + rows);
+    // of request r0 + t: adapter, first row and number of rows; `seen`: where the requests in front end.  A list that goes back names no row twice
+    int id = -1, lo = 0, n = 0;
+    auto look = [&](int r0, int& seen) {
+        const int r = r0 + t;
+        const int c = r < A.R ? A.cu[r] : (int)0x80000000;
+        const int64_t to = r < A.R ? min((int64_t)A.cu[r + 1], end) : 0;
+        id = r < A.R ? A.ids[r] : -1;
+        int all;
+        const int most = scan<true>(c, warps, all);
+        const int64_t from = max((int64_t)max(most, seen), row0);
+        seen = max(seen, all);
+        if (id < 0 || id >= A.adapters || from >= to) { id = -1; n = 0; }
+        else { lo = (int)(from - row0); n = (int)(to - from); }
+    };
+    int seen = (int)0x80000000;
+    __syncthreads();
+    for (int r0 = 0; r0 < A.R; r0 += SORT_THREADS) {
+        look(r0, seen);
+        // one addition for the requests of an adapter in a warp
+        const uint32_t same = __match_any_sync(0xffffffffu, id);
+        const int sum = __reduce_add_sync(same, n);
+        if (id >= 0 && lane == __ffs(same) - 1) atomicAdd(place + id, sum);
+    }
+    __syncthreads();
+    int row_at = 0, piece_at = 0;
+    for (int a0 = 0; a0 < A.adapters; a0 += SORT_THREADS) {
+        const int a = a0 + t, c = a < A.adapters ? place[a] : 0, p = (c + TM - 1) / TM;
+        int all_rows, all_pieces;
+        const int r = scan<false>(c, warps, all_rows), q = scan<false>(p, warps, all_pieces);
+        if (a < A.adapters) { place[a] = row_at + r - c; before[a] = piece_at + q - p; }
+        row_at += all_rows;
+        piece_at += all_pieces;
+    }
+    __syncthreads();
+    for (int i = t; i < n_pieces; i += SORT_THREADS) {
+        int4 piece = make_int4(0, 0, 0, 0);
+        if (i < piece_at) {
+            int a = 0, last = A.adapters - 1;                  // the last adapter with no more pieces in front
+            while (a < last) {
+                const int mid = (a + last + 1) >> 1;
+                if (before[mid] <= i) a = mid;
+                else last = mid - 1;
+            }
+            const int first = place[a] + TM * (i - before[a]), stop = a + 1 < A.adapters ? place[a + 1] : row_at;
+            piece = make_int4(a, first, min(TM, stop - first), 0);
+        }
+        A.pieces[i] = piece;
+    }
+    seen = (int)0x80000000;
+    for (int r0 = 0; r0 < A.R; r0 += SORT_THREADS) {
+        __syncthreads();
+        if (t == 0) n_few = n_more = 0;
+        if (A.R > SORT_THREADS) look(r0, seen);
+        const uint32_t same = __match_any_sync(0xffffffffu, id);
+        const int sum = __reduce_add_sync(same, n), leader = __ffs(same) - 1;
+        int at = 0;
+#pragma unroll
+        for (int l = 0; l < 31; l++) {
+            const int v = __shfl_sync(0xffffffffu, n, l);
+            if (l < lane && same >> l & 1) at += v;
+        }
+        __syncthreads();
+        int base = id >= 0 && lane == leader ? atomicAdd(place + id, sum) : 0;
+        at += __shfl_sync(0xffffffffu, base, leader);
+        if (n <= 4) {
+            for (int k = 0; k < n; k++) A.order[at + k] = lo + k;
+        } else {
+            const int e = n <= 1024 ? atomicAdd(&n_few, 1) : SORT_THREADS - 1 - atomicAdd(&n_more, 1);
+            few[e] = lo; few_n[e] = n; few_at[e] = at;
+        }
+        __syncthreads();
+        for (int e = warp; e < n_few; e += 32)
+            for (int k = lane; k < few_n[e]; k += 32) A.order[few_at[e] + k] = few[e] + k;
+        for (int e = SORT_THREADS - n_more; e < SORT_THREADS; e++)
+            for (int k = t; k < few_n[e]; k += SORT_THREADS) A.order[few_at[e] + k] = few[e] + k;
+    }
+}
+
+// From here on three launches.
 constexpr int64_t LORA_MANY = 256;
 // splits that share a reading of x: 128 rows of A at most (their parts and h fill what shared memory two blocks of an SM have), or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
-size_t lora_tiles_bytes(int64_t T) { return (size_t)((T + TM - 1) / TM) * sizeof(Tile); }
+// pieces that T rows of R requests may have: of whole 64, and one of every adapter
+int64_t lora_pieces(int64_t T, int adapters, int R) { int64_t most = adapters < R ? adapters : R; if (most > T) most = T; return T / TM + most; }
+size_t lora_lists_bytes(int64_t T, int adapters, int R) {
+    return (size_t)lora_pieces(T, adapters, R) * sizeof(int4) + ((size_t)T + (adapters > SORT_HERE ? 2 * (size_t)adapters : 0) + 3) / 4 * 16;
+}
 
-template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
+template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStream_t st) {
     A.together = lora_together(A.rank, A.n_splits);
     static bool configured[64] = {};                           // the attribute is per device
     int dev = 0;
@@ -529,16 +660,23 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
     }
-    const bool many = A.T > LORA_MANY;
-    const int64_t tiles = (A.T + TM - 1) / TM;
-    // blocks, or clusters, that share a tile's adapters: twice as many as a tile has on average, since neighbours' differ; those that find none leave at once
+    const bool many = A.pieces != nullptr;
+    const bool on = launch_overlaps(st);
+    // clusters of tiles, and those that share a tile's adapters: twice as many as a tile has on average, since neighbours' differ; those that find none leave at
+    // once.  Or of pieces
+    const int64_t tiles = many ? lora_pieces(A.T, A.adapters, A.R) : (A.T + TM - 1) / TM;
     int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
     if (most > A.adapters) most = A.adapters;
     if (some > most) some = most;
+    if (many) some = 1;
     // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
     // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the tiles fill the device: 11849 rows by 2 blocks of a tile 152 us, by 4 159, by 8 178
     int blocks = 8;
     while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
+    if (many) {
+        launch_behind(lora_order_kernel, dim3(1), SORT_THREADS, 0, st, on, A, row0, (int)A.T, (int)tiles);
+        note_launch();
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)some);
     cfg.blockDim = dim3(LORA_THREADS);
@@ -548,35 +686,35 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, cudaStream_t st) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim = {(unsigned)blocks, 1u, 1u};
     cfg.attrs = at;
-    cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
+    cfg.numAttrs = add_overlap(at, 1, on);
     A.shares = 1;
     cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
-        // blocks of a tile's columns: eight an SM's two places (11849 rows by 8 shares of a tile 147 us, by 4 150, by 16 173), none with fewer than three groups a
+        // blocks of a piece's columns: eight an SM's two places (11849 rows by 8 shares of a tile 147 us, by 4 150, by 16 173), none with fewer than three groups a
         // warp, which would read h more often than it uses it
         const int64_t want = 8ll * sm_count() / tiles, room = A.first[A.n_splits] / (32 * LORA_WARPS * 3);
         A.shares = (int)(want < 8 ? 8 : want);
         if (A.shares > room) A.shares = (int)room;
         if (A.shares < 1) A.shares = 1;
-        launch_behind(lora_kernel<BF, STEPS, LORA_SECOND>, dim3((unsigned)(tiles * A.shares), (unsigned)some), LORA_THREADS, (size_t)Lora::smem(A.rank, A.together), st,
-                      launch_overlaps(st), A);
+        launch_behind(lora_kernel<BF, STEPS, LORA_SECOND>, dim3((unsigned)(tiles * A.shares)), LORA_THREADS, (size_t)Lora::smem(A.rank, A.together), st, on, A);
         note_launch();
     }
     return check_launch();
 }
 
 // B in registers for the ranks that adapters mostly have; other steps would cost a kernel each for less
-template <bool BF> int lora_steps(const LoraArgs& A, cudaStream_t st) {
-    return A.rank <= 16 ? lora_launch<BF, 1>(A, st) : A.rank <= 32 ? lora_launch<BF, 2>(A, st) : A.rank <= 64 && A.rank > 48 ? lora_launch<BF, 4>(A, st) : lora_launch<BF, 0>(A, st);
+template <bool BF> int lora_steps(const LoraArgs& A, int64_t row0, cudaStream_t st) {
+    return A.rank <= 16 ? lora_launch<BF, 1>(A, row0, st) : A.rank <= 32 ? lora_launch<BF, 2>(A, row0, st) : A.rank <= 64 && A.rank > 48 ? lora_launch<BF, 4>(A, row0, st)
+                                                                                                                  : lora_launch<BF, 0>(A, row0, st);
 }
 
 }  // namespace
 }  // namespace lowbit
 
-extern "C" size_t lowbit_lora_workspace_size(int64_t T, int rank, int n_splits) {
-    if (T <= LORA_MANY || rank <= 0 || n_splits <= 0) return 0;
-    return lora_tiles_bytes(T) + (size_t)T * n_splits * (Lora::steps(rank) * 64 + sizeof(float));
+extern "C" size_t lowbit_lora_workspace_size(int64_t T, int rank, int n_splits, int adapters, int R) {
+    if (T <= LORA_MANY || rank <= 0 || n_splits <= 0 || adapters <= 0 || R <= 0) return 0;
+    return lora_lists_bytes(T, adapters, R) + (size_t)T * n_splits * (Lora::steps(rank) * 64 + sizeof(float));
 }
 
 extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b, int64_t b_stride,
@@ -599,17 +737,30 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
         return LB_ERR_ARG;
     }
     if (T == 0) return LB_OK;
-    if (T > LORA_MANY && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_lora_workspace_size(T, rank, n_splits))) {
+    if (T > LORA_MANY && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_lora_workspace_size(T, rank, n_splits, adapters, R))) {
         set_error(LB_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of lowbit_lora_workspace_size() bytes is needed", name);
         return LB_ERR_WORKSPACE;
     }
     LoraArgs A = {d_x, x_stride, T, K, d_a, a_stride, d_b, b_stride, d_scales, adapters, d_ids, d_cu_seqlens, R, d_out, out_stride, rank, n_splits, 0,
-                  (uint8_t*)workspace, nullptr, nullptr, 0, {}};
-    if (T > LORA_MANY) {
-        A.h = (uint16_t*)((uint8_t*)workspace + lora_tiles_bytes(T));
-        A.back = (float*)(A.h + T * n_splits * Lora::steps(rank) * 32);
-    }
+                  nullptr, nullptr, nullptr, nullptr, nullptr, 0, {}};
     for (int i = 0; i < n_splits; i++) A.first[i + 1] = A.first[i] + splits[i];
     cudaStream_t st = (cudaStream_t)stream;
-    return dtype == DT_BF16 ? lora_steps<true>(A, st) : lora_steps<false>(A, st);
+    if (T <= LORA_MANY) return dtype == DT_BF16 ? lora_steps<true>(A, 0, st) : lora_steps<false>(A, 0, st);
+    uint8_t* const w = (uint8_t*)workspace;
+    A.pieces = (int4*)w;
+    A.order = (int32_t*)(w + lora_pieces(T, adapters, R) * sizeof(int4));
+    A.lists = A.order + T;
+    A.h = (uint16_t*)(w + lora_lists_bytes(T, adapters, R));
+    A.back = (float*)(A.h + T * n_splits * Lora::steps(rank) * 32);
+    // a row's offset has 32 bits, in 16 bytes: as many rows at a time as that reaches
+    const int64_t stride = x_stride > out_stride ? x_stride : out_stride;
+    int64_t rows = (1ll << 35) / stride / TM * TM;             // 64 at least
+    for (int64_t row0 = 0; row0 < T; row0 += rows) {
+        LoraArgs part = A;
+        part.T = T - row0 < rows ? T - row0 : rows;
+        part.x = (const uint16_t*)d_x + row0 * x_stride;
+        part.out = (uint16_t*)d_out + row0 * out_stride;
+        if (const int rc = dtype == DT_BF16 ? lora_steps<true>(part, row0, st) : lora_steps<false>(part, row0, st)) return rc;
+    }
+    return LB_OK;
 }

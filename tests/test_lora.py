@@ -339,4 +339,4 @@ def test_refusals_on_the_cpu(lora, native_lib):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
-    assert lib.lowbit_lora_workspace_size(256, 16, 2) == 0 and lib.lowbit_lora_workspace_size(257, 16, 2) >= 257 * 32 * 4
+    assert lib.lowbit_lora_workspace_size(256, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(257, 16, 2, 3, 4) >= 257 * (32 * 4 + 4)
