@@ -13,9 +13,10 @@
 // the adapters' rows gathered.  What the operator cannot do without is to read x and out, to write out, and the adapters' A and B once.
 //
 // Measured, times without the launch's share on the host.  One token of K 4096 and N 4096 at rank 16: 6.5 us, the latency of five dependent trips to memory and
-// the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 13.0 us (1.2 TB/s; a tile's clusters read their adapters by themselves).
-// 882 rows of 40 requests, K 4096 and N 11008 at rank 64: 24 + 32 us for 69 MB.  11849 rows, N 14336 at rank 32: 38 + 111 us for 628 MB, 4.3 TB/s.
-// The second launch there is a copy of `out` (88 us by itself) whose products (98 us by themselves) overlap it but for a fifth.
+// the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 12.3 us, the same.
+// 882 rows of 40 requests, K 4096 and N 11008 at rank 64, 69 MB: 40.4 us, 7 + 16 + 22.  11849 rows, N 14336 at rank 32, 628 MB: 140 us, 7 + 36 + 101.
+// The second product's launch there copies `out`, which alone takes 88 us; 57 % of what a SM's shared memory and L1 can move in that time is h, read
+// for 32 columns at a time, and `out` on its way through.
 #include <type_traits>
 #include "lowbit_common.cuh"
 #include "lowbit_internal.h"
@@ -157,14 +158,17 @@ struct Lora {
 };
 
 // First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
-// = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K.
+// = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K; with more than 32 rows groups
+// of them take 32 rows each, and their warps share K.
 // Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
-// holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  (The first product alone: 4 for up to 4.)
+// holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  With an even number a lane reads 16 bytes of B, in the first product's order
+// of two steps' k.  (The first product alone: 4 for up to 4.)
 enum { LORA_BOTH, LORA_FIRST, LORA_SECOND };
 template <bool BF, int STEPS, int DO>
 __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
+    constexpr bool WIDE = STEPS == 2 || STEPS == 4;
     constexpr int NT = DO == LORA_FIRST ? 8 : 4, TOKS = 8 * NT, MT = L::MT, ROWS = L::ROWS, STAGE = (NT + 2 * MT) * 512;      // of the first product
     __shared__ std::conditional_t<DO == LORA_BOTH, Tile, Rows> tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
@@ -207,8 +211,10 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
             const uint4* const w = (const uint4*)((const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K);
             // ---- h of this block's share of K.  Rows behind the last, of A and of x, are read as the last ones: nobody looks at what they give
-            for (int row0 = 0, i0 = 0; DO != LORA_SECOND && row0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, row0 += i0 ? 0 : ROWS) {
-                const int m_end = min(MT, (rows - row0 + 15) / 16), n_end = min(NT, (count - i0 + 7) / 8);
+            const int groups = DO == LORA_FIRST ? 1 : rows > 2 * ROWS ? 4 : rows > ROWS ? 2 : 1, of_group = LORA_WARPS / groups, nth = warp & (of_group - 1);
+            for (int rows0 = 0, i0 = 0; DO != LORA_SECOND && rows0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, rows0 += i0 ? 0 : ROWS * groups) {
+                const int row0 = rows0 + warp / of_group * ROWS, m_end = min(MT, (rows - row0 + 15) / 16), n_end = min(NT, (count - i0 + 7) / 8);
+                const int last = m_end > 0 ? to : from;        // nothing for a group behind the last row
                 float acc[MT][NT][4] = {};
                 uint32_t xs[NT], ws[MT][2];                    // in 16 bytes, of this lane's rows
                 const uint4* const x = (const uint4*)((const uint16_t*)A.x + t0 * A.x_st);
@@ -219,7 +225,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
 #pragma unroll
                     for (int h = 0; h < 2; h++) ws[m][h] = (uint32_t)min(row0 + 16 * m + 8 * h + g, rows - 1) * (uint32_t)(A.K / 8);
                 auto ask = [&](int c, int stage) {
-                    const bool in = c < to && 32 * c + 8 * t < A.K;
+                    const bool in = c < last && 32 * c + 8 * t < A.K;
                     const uint32_t k = in ? 4 * c + t : 0, at = ring1 + stage * STAGE;
 #pragma unroll
                     for (int n = 0; n < NT; n++)
@@ -233,11 +239,11 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     asm volatile("cp.async.commit_group;" ::: "memory");
                 };
                 __syncthreads();                               // what was in the ring's place is read
-                ask(from + warp, 0);
-                ask(from + warp + LORA_WARPS, 1);
+                ask(from + nth, 0);
+                ask(from + nth + of_group, 1);
                 int stage = 0;
 #pragma unroll 1
-                for (int c = from + warp; c < to; c += LORA_WARPS, stage ^= 1) {
+                for (int c = from + nth; c < last; c += of_group, stage ^= 1) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
                     const uint32_t at = ring1 + stage * STAGE;
                     uint4 wr[MT][2];
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                             for (int m = 0; m < MT; m++)
                                 if (m < m_end) mma<BF>(acc[m][n], wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w, xr.z, xr.w);
                         }
-                    ask(c + 2 * LORA_WARPS, stage);
+                    ask(c + 2 * of_group, stage);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncthreads();                               // everybody is through with the ring
@@ -271,16 +277,17 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     }
                 __syncthreads();
 #pragma unroll 1
-                for (int i = threadIdx.x; i < TOKS * ROWS / 4; i += LORA_THREADS) {
-                    const int tok = i / (ROWS / 4), row = i % (ROWS / 4) * 4;
-                    if (i0 + tok < count && row0 + row < rows) {
+                for (int i = threadIdx.x; i < TOKS * ROWS / 4 * groups; i += LORA_THREADS) {
+                    const int tok = i / (ROWS / 4) & (TOKS - 1), group = i / (TOKS * ROWS / 4), in = i % (ROWS / 4) * 4, row = rows0 + group * ROWS + in;
+                    if (i0 + tok < count && row < rows) {
                         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                         for (int v = 0; v < LORA_WARPS; v++) {
-                            const float4 p = *reinterpret_cast<const float4*>(sums + (v * TOKS + tok) * L::PITCH + row);
+                            if (v >= of_group) break;
+                            const float4 p = *reinterpret_cast<const float4*>(sums + ((group * of_group + v) * TOKS + tok) * L::PITCH + in);
                             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
                         }
-                        *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row0 + row) = s;
+                        *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row) = s;
                     }
                 }
             }
@@ -357,7 +364,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                         *reinterpret_cast<uint32_t*>(to) = hi;
                         *reinterpret_cast<uint32_t*>(to + 16 * steps) = lo;
                     } else {
-                        const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + ((tok & 7) * 4 + (r & 15) / 4) * 16 + (tok & 8) + (r & 2) * 2;
+                        const uint32_t at = hs + (s * steps + (WIDE ? r / 32 * 2 + (r >> 2 & 1) : r / 16)) * L::kStep + tok / 16 * L::kFrag +
+                                            ((tok & 7) * 4 + (WIDE ? r / 8 & 3 : r / 4 & 3)) * 16 + (tok & 8) + (r & 2) * 2;
 #pragma unroll 8
                         for (uint32_t b = 0; b < blocks; b++) {
                             const uint32_t p = shared_of(at, b);
@@ -368,14 +376,15 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                 }
             };
             if constexpr (DO == LORA_SECOND) {
-                // 16 bytes, a row's eight neighbours, a thread: two lanes' share of a fragment
+                // 16 bytes, a row's eight neighbours, a thread: two lanes' share of a fragment, or a lane's of two
                 const int pieces = n_here * steps * 4;         // of a row: two of high parts, two of low ones a step
                 for (int i = threadIdx.x; i < count * pieces; i += LORA_THREADS) {
                     const int tok = i / pieces, in = i - tok * pieces, s = in / (4 * steps), half = in / (2 * steps) & 1, r = in % (2 * steps) * 8;
                     const uint4 v = *reinterpret_cast<const uint4*>(A.h + (int64_t)(piece.y + tok) * (A.n_splits * 32 * steps) + s0 * 32 * steps + in * 8);
-                    const uint32_t at = hs + (s * steps + r / 16) * L::kStep + tok / 16 * L::kFrag + half * (L::kFrag / 2) + ((tok & 7) * 4 + (r & 8) / 4) * 16 + (tok & 8);
+                    const uint32_t at = hs + (s * steps + (WIDE ? r / 32 * 2 : r / 16)) * L::kStep + tok / 16 * L::kFrag + half * (L::kFrag / 2) +
+                                        ((tok & 7) * 4 + (WIDE ? r / 8 & 3 : r / 4 & 2)) * 16 + (tok & 8);
                     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + 16), "r"(v.z), "r"(v.w) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (WIDE ? L::kStep : 16)), "r"(v.z), "r"(v.w) : "memory");
                 }
                 if (!BF)
                     for (int i = threadIdx.x; i < count * n_here; i += LORA_THREADS) back[i / n_here][i % n_here] = A.back[(int64_t)(piece.y + i / n_here) * A.n_splits + s0 + i % n_here];
@@ -405,24 +414,29 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                 meet(blocks);                                  // the parts are read: they may be written again, and their block may leave
                 continue;
             }
-            const int off = (8 * (g >> 1) + (g & 1)) * A.rank + 4 * t;                         // this lane's rows of B are 2 n further on
-            auto fetch = [&](const Group& of, int st, uint2 (&br)[4]) {
+            const int off = (8 * (g >> 1) + (g & 1)) * A.rank + (WIDE ? 8 : 4) * t;            // this lane's rows of B are 2 n further on
+            // step `st`, or, WIDE, that and the next
+            auto fetch = [&](const Group& of, int st, uint2 (*br)[4]) {
                 const uint16_t* const p = wb + (int64_t)of.c0 * A.rank + 16 * st;
-                if (of.c0 + 32 <= of.c_end && 16 * st + 16 <= A.rank) {
+                auto take = [&](int n, bool there) {
+                    if constexpr (WIDE) {
+                        const uint4 v = there ? *reinterpret_cast<const uint4*>(p + (off + 2 * n * A.rank)) : make_uint4(0, 0, 0, 0);
+                        br[0][n] = make_uint2(v.x, v.y);
+                        br[1][n] = make_uint2(v.z, v.w);
+                    } else br[0][n] = there ? *reinterpret_cast<const uint2*>(p + (off + 2 * n * A.rank)) : make_uint2(0, 0);
+                };
+                if (of.c0 + 32 <= of.c_end && 16 * st + (WIDE ? 32 : 16) <= A.rank) {
 #pragma unroll
-                    for (int n = 0; n < 4; n++) br[n] = *reinterpret_cast<const uint2*>(p + (off + 2 * n * A.rank));
+                    for (int n = 0; n < 4; n++) take(n, true);
                 } else {
 #pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        const bool there = of.c0 + 8 * (g >> 1) + 2 * n + (g & 1) < of.c_end && 16 * st + 4 * t < A.rank;
-                        br[n] = there ? *reinterpret_cast<const uint2*>(p + (off + 2 * n * A.rank)) : make_uint2(0, 0);
-                    }
+                    for (int n = 0; n < 4; n++) take(n, of.c0 + 8 * (g >> 1) + 2 * n + (g & 1) < of.c_end && 16 * st + (WIDE ? 8 : 4) * t < A.rank);
                 }
             };
             uint2 br[STEPS ? STEPS : 1][4];
             if (STEPS && more) {
 #pragma unroll
-                for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
+                for (int st = 0; st < STEPS; st += WIDE ? 2 : 1) fetch(ahead, st, br + st);
             }
             if (DO == LORA_BOTH) meet(blocks);
             else __syncthreads();
@@ -490,15 +504,15 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                             }
                         } else if (more) {                     // the products have B: the next group's
 #pragma unroll
-                            for (int st = 0; st < STEPS; st++) fetch(ahead, st, br[st]);
+                            for (int st = 0; st < STEPS; st += WIDE ? 2 : 1) fetch(ahead, st, br + st);
                         }
                     } else {
-                        fetch(now, 0, br[0]);
+                        fetch(now, 0, br);
                         ask_h(m, 0, hi[0], lo[0]);
                         products(hi[0], lo[0], br[0], true);
 #pragma unroll 1
                         for (int st = 1; st < steps; st++) {
-                            fetch(now, st, br[0]);
+                            fetch(now, st, br);
                             ask_h(m, st, hi[0], lo[0]);
                             products(hi[0], lo[0], br[0], false);
                         }
@@ -524,7 +538,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
 }
 
 // ------------------------------------------------------------------ many tokens: the rows ordered by their adapters
-constexpr int SORT_THREADS = 1024, SORT_HERE = 4096;           // adapters whose lists lie in shared memory
+constexpr int SORT_THREADS = 512, SORT_HERE = 4096;            // adapters whose lists lie in shared memory
 template <bool MOST> __device__ __forceinline__ int scan(int x, int* warps, int& all) {        // inclusive sums, or maxima, over the block; all: of the whole block
     auto both = [](int a, int b) { return MOST ? max(a, b) : a + b; };
     constexpr int none = MOST ? (int)0x80000000 : 0;
@@ -537,7 +551,7 @@ template <bool MOST> __device__ __forceinline__ int scan(int x, int* warps, int&
     __syncthreads();
     if (lane == 31) warps[warp] = x;
     __syncthreads();
-    int w = warps[lane];                                       // 32 warps
+    int w = lane < SORT_THREADS / 32 ? warps[lane] : none;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, w, d);
@@ -548,7 +562,8 @@ template <bool MOST> __device__ __forceinline__ int scan(int x, int* warps, int&
     return both(x, warp ? before : none);
 }
 // One block: rows counted by adapter, a place for each adapter's, the pieces of 64, the rows written to their places.  In which order the rows of an adapter lie is
-// chance, and nothing depends on it: a row's sums are its own.  Rows [row0, row0 + rows) count from 0; n_pieces: room for pieces.
+// chance, and nothing depends on it: a row's sums are its own.  Rows [row0, row0 + rows) count from 0; n_pieces: room for pieces.  It waits for barriers and for
+// memory, some 6 us (1024 threads one more); 882 rows of 40 requests and 12 adapters become 20 pieces, of which tiles of neighbours' rows had some 50.
 __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraArgs A, int64_t row0, int rows, int n_pieces) {
     __shared__ int warps[32];
     __shared__ int here[2][SORT_HERE];
@@ -580,6 +595,7 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraA
     for (int r0 = 0; r0 < A.R; r0 += SORT_THREADS) {
         look(r0, seen);
         // one addition for the requests of an adapter in a warp
+        if (r0 + 32 * warp >= A.R) continue;
         const uint32_t same = __match_any_sync(0xffffffffu, id);
         const int sum = __reduce_add_sync(same, n);
         if (id >= 0 && lane == __ffs(same) - 1) atomicAdd(place + id, sum);
@@ -614,32 +630,34 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraA
         __syncthreads();
         if (t == 0) n_few = n_more = 0;
         if (A.R > SORT_THREADS) look(r0, seen);
-        const uint32_t same = __match_any_sync(0xffffffffu, id);
-        const int sum = __reduce_add_sync(same, n), leader = __ffs(same) - 1;
-        int at = 0;
+        __syncthreads();
+        if (r0 + 32 * warp < A.R) {
+            const uint32_t same = __match_any_sync(0xffffffffu, id);
+            const int sum = __reduce_add_sync(same, n), leader = __ffs(same) - 1;
+            int at = id >= 0 && lane == leader ? atomicAdd(place + id, sum) : 0;
+            at = __shfl_sync(0xffffffffu, at, leader);
 #pragma unroll
-        for (int l = 0; l < 31; l++) {
-            const int v = __shfl_sync(0xffffffffu, n, l);
-            if (l < lane && same >> l & 1) at += v;
+            for (int l = 0; l < 31; l++) {
+                const int v = __shfl_sync(0xffffffffu, n, l);
+                if (l < lane && same >> l & 1) at += v;
+            }
+            if (n <= 4) {
+                for (int k = 0; k < n; k++) A.order[at + k] = lo + k;
+            } else {
+                const int e = n <= 1024 ? atomicAdd(&n_few, 1) : SORT_THREADS - 1 - atomicAdd(&n_more, 1);
+                few[e] = lo; few_n[e] = n; few_at[e] = at;
+            }
         }
         __syncthreads();
-        int base = id >= 0 && lane == leader ? atomicAdd(place + id, sum) : 0;
-        at += __shfl_sync(0xffffffffu, base, leader);
-        if (n <= 4) {
-            for (int k = 0; k < n; k++) A.order[at + k] = lo + k;
-        } else {
-            const int e = n <= 1024 ? atomicAdd(&n_few, 1) : SORT_THREADS - 1 - atomicAdd(&n_more, 1);
-            few[e] = lo; few_n[e] = n; few_at[e] = at;
-        }
-        __syncthreads();
-        for (int e = warp; e < n_few; e += 32)
+        for (int e = warp; e < n_few; e += SORT_THREADS / 32)
             for (int k = lane; k < few_n[e]; k += 32) A.order[few_at[e] + k] = few[e] + k;
         for (int e = SORT_THREADS - n_more; e < SORT_THREADS; e++)
             for (int k = t; k < few_n[e]; k += SORT_THREADS) A.order[few_at[e] + k] = few[e] + k;
     }
 }
 
-// From here on three launches.
+// From here on three launches: 882 rows of 40 requests 40 us, by one 68; 11849 rows 140 and 171.  64 tokens are the other way round: 12.3 us by one launch, and no less
+// than 18 by two of the kind.
 constexpr int64_t LORA_MANY = 256;
 // splits that share a reading of x: 128 rows of A at most (their parts and h fill what shared memory two blocks of an SM have), or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
@@ -670,7 +688,8 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     if (some > most) some = most;
     if (many) some = 1;
     // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
-    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the tiles fill the device: 11849 rows by 2 blocks of a tile 152 us, by 4 159, by 8 178
+    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the tiles fill the device: 11849 rows by 2 blocks of a piece 141 us, by
+    // 4 143, by 8 152; 882 rows by 8 41, by 4 44, by 2 52
     int blocks = 8;
     while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
     if (many) {
@@ -691,7 +710,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
-        // blocks of a piece's columns: eight an SM's two places (11849 rows by 8 shares of a tile 147 us, by 4 150, by 16 173), none with fewer than three groups a
+        // blocks of a piece's columns: eight an SM's two places (11849 rows by 8 shares of a piece 147 us, by 4 150, by 16 173, in an earlier form), none with fewer than three groups a
         // warp, which would read h more often than it uses it
         const int64_t want = 8ll * sm_count() / tiles, room = A.first[A.n_splits] / (32 * LORA_WARPS * 3);
         A.shares = (int)(want < 8 ? 8 : want);

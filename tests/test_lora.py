@@ -228,6 +228,42 @@ def test_where_the_launches_change(lora, cuda_device, rows, rank):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,ids,adapters", [
+    ([1] * 2000, [0] * 2000, 1), ([1] * 600, [i % 600 for i in range(600)], 600), ([3, 0, 5, 1] * 300, [i * 7 % 9 - 1 for i in range(1200)], 8), ([1500, 1, 1023, 1024, 1025, 6], [1, 0, 1, 2, 1, -1], 3),
+    ([2] * 700 + [1100], [i * 31 % 5003 for i in range(701)], 5000), ([64] * 6, [4999, 0, 4096, 4095, 4999, 5000], 5000)])
+def test_orders_of_many_rows(lora, cuda_device, lens, ids, adapters):
+    """more requests and more adapters than a block looks at at a time, stretches of every kind, an adapter for each, one for all"""
+    check(lora, make(lens, ids, 16, [8, 16], 8, adapters, torch.float16, cuda_device, pad=9), lens, ids)
+
+
+@pytest.mark.gpu
+def test_a_list_that_goes_back(lora, cuda_device):
+    """of many rows none is taken twice: a request has what lies behind all in front of it"""
+    s = make([400, 200], [0, 1], 64, [64], 8, 3, torch.bfloat16, cuda_device)
+    want = run(lora, s)
+    for cu, ids in (([0, 400, 100, 400, 350, 600], [0, 2, 2, 2, 1]), ([-50, 400, 600, 0, 600], [0, 1, 2, 2])):
+        odd = {**s, "cu": torch.tensor(cu, dtype=torch.int32, device=cuda_device), "ids": torch.tensor(ids, dtype=torch.int32, device=cuda_device)}
+        assert torch.equal(run(lora, odd), want)
+
+
+@pytest.mark.gpu
+def test_rows_far_apart(lora, cuda_device):
+    """rows of 2^27 elements: as many at a time as a 32-bit offset in 16 bytes reaches"""
+    T, step = 270, 1 << 27
+    if torch.cuda.mem_get_info()[0] < T * step * 2 + (4 << 30):
+        pytest.skip("needs 73 GB")
+    lens, ids = [200, 30, 40], [0, -1, 1]
+    s = make(lens, ids, 64, [64], 16, 2, torch.float16, cuda_device)
+    want = run(lora, s)
+    far = torch.empty(T * step, dtype=torch.float16, device=cuda_device).as_strided((T, 64), (step, 1))
+    far.copy_(s["out"])
+    lora.lora_add_(far, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+    assert torch.equal(far, want)
+    far.copy_(s["x"])
+    assert torch.equal(run(lora, {**s, "x": far}), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 5, 300])
 def test_the_python_statements_say_the_same(lora, cuda_device, monkeypatch, rows):
     s = make([rows], [1], 256, [128, 64], 16, 2, torch.bfloat16, cuda_device)
