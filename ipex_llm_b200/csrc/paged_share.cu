@@ -217,9 +217,12 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
             int at = before[r - r0];
             int32_t* const row = A.table + r * A.table_stride;
             each(r, [&](int c, Pages p) {
+                int first[SHARE_DEEP], times[SHARE_DEEP];
                 bool goes[SHARE_DEEP];
 #pragma unroll
-                for (int u = 0; u < SHARE_DEEP; u++) goes[u] = p[u] >= 0 && A.first[p[u]] == r * A.width + c + 32 * u && A.times[p[u]] > 0;
+                for (int u = 0; u < SHARE_DEEP; u++) { first[u] = p[u] >= 0 ? A.first[p[u]] : -1; times[u] = p[u] >= 0 ? A.times[p[u]] : 0; }
+#pragma unroll
+                for (int u = 0; u < SHARE_DEEP; u++) goes[u] = first[u] == r * A.width + c + 32 * u && times[u] > 0;
 #pragma unroll
                 for (int u = 0; u < SHARE_DEEP; u++) {
                     const uint32_t yes = __ballot_sync(0xffffffffu, goes[u]);
@@ -261,29 +264,36 @@ __device__ __forceinline__ int below(const int32_t* list, int n, int x) {
 }
 
 // Free pages in ascending order against used ones in descending order, as long as the free one lies in front: move i goes from the i-th of these to the
-// i-th of those.  Pages that are neither in the table nor on the stack stay.  The stack's lowest page comes off first.
+// i-th of those.  Pages that are neither in the table nor on the stack stay.  The stack's lowest page comes off first.  HERE: one block, the scratch in
+// shared memory, where searching the lists costs a fifth; else a cluster's blocks share it in memory.
+template <bool HERE>
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const CompactArgs A) {
+    extern __shared__ int32_t compact_here[];
+    int32_t* const state = HERE ? compact_here : A.state;
+    int32_t* const goes_to = HERE ? compact_here + A.n_pages : A.to;
+    int32_t* const free_up = HERE ? compact_here + 2 * A.n_pages : A.free_up;
+    int32_t* const used_up = HERE ? compact_here + 3 * A.n_pages : A.used_up;
     __shared__ int warps[32];
     __shared__ int totals[2];                                  // of this block's pages: free, used
     __shared__ int moves;
     const uint32_t rank = cluster_rank(), blocks = cluster_blocks();
     const int me = (int)rank * SHARE_THREADS + threadIdx.x, all = (int)blocks * SHARE_THREADS;
-    const int64_t entries = (int64_t)A.R * A.width;
+    const int entries = A.R * A.width;                         // up to 2^30
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = max(0, min(*A.count, A.n_pages));
-    auto entry = [&](int64_t e) { const int r = (int)(e / A.width); return A.table[r * A.table_stride + (e - (int64_t)r * A.width)]; };
+    auto entry = [&](int e) { const int r = e / A.width; return A.table[r * A.table_stride + (e - r * A.width)]; };
     auto is_page = [&](int p) { return p >= 0 && p < A.n_pages; };
-    for (int p = me; p < A.n_pages; p += all) { A.state[p] = 0; A.to[p] = p; }
+    for (int p = me; p < A.n_pages; p += all) { state[p] = 0; goes_to[p] = p; }
     meet(blocks);
-    for (int i = me; i < count; i += all) { const int p = A.pages[i]; if (is_page(p)) atomicOr(A.state + p, 1); }
-    for (int64_t e = me; e < entries; e += all) { const int p = entry(e); if (is_page(p)) atomicOr(A.state + p, 2); }
+    for (int i = me; i < A.n_pages; i += all) { const int p = A.pages[i]; if (i < count && is_page(p)) atomicOr(state + p, 1); }
+    for (int e = me; e < entries; e += all) { const int p = entry(e); if (is_page(p)) atomicOr(state + p, 2); }
     meet(blocks);
     // both lists: this block's pages lie behind those of the blocks in front
     const int each = (A.n_pages + (int)blocks - 1) / (int)blocks, begin = min((int)rank * each, A.n_pages), end = min(begin + each, A.n_pages);
     int n_free = 0, n_used = 0;
     for (int p0 = begin; p0 < end; p0 += SHARE_THREADS) {
-        const int p = p0 + threadIdx.x, s = p < end ? A.state[p] : 0;
+        const int p = p0 + threadIdx.x, s = p < end ? state[p] : 0;
         n_free += __syncthreads_count(s == 1);
         n_used += __syncthreads_count(s & 2);
     }
@@ -300,13 +310,13 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const C
         F += f; U += u;
     }
     for (int p0 = begin; p0 < end; p0 += SHARE_THREADS) {
-        const int p = p0 + threadIdx.x, s = p < end ? A.state[p] : 0;
+        const int p = p0 + threadIdx.x, s = p < end ? state[p] : 0;
         int total;
         const int i = block_sum(s == 1, warps, total);
-        if (s == 1) A.free_up[free_at + i - 1] = p;
+        if (s == 1) free_up[free_at + i - 1] = p;
         free_at += total;
         const int j = block_sum((s & 2) != 0, warps, total);
-        if (s & 2) A.used_up[used_at + j - 1] = p;
+        if (s & 2) used_up[used_at + j - 1] = p;
         used_at += total;
     }
     meet(blocks);
@@ -314,7 +324,7 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const C
         int lo = 0, hi = min(F, U);                            // the first pair that does not move
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (A.free_up[mid] < A.used_up[U - 1 - mid]) lo = mid + 1;
+            if (free_up[mid] < used_up[U - 1 - mid]) lo = mid + 1;
             else hi = mid;
         }
         moves = lo;
@@ -322,34 +332,34 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const C
     __syncthreads();
     const int m = moves;
     for (int i = me; i < A.n_pages; i += all) {
-        const int a = i < m ? A.free_up[i] : -1, b = i < m ? A.used_up[U - 1 - i] : -1;
+        const int a = i < m ? free_up[i] : -1, b = i < m ? used_up[U - 1 - i] : -1;
         A.src[i] = b;
         A.dst[i] = a;
-        if (i < m) A.to[b] = a;
+        if (i < m) goes_to[b] = a;
         // the stack, from its highest page down: free pages that stay free, and the vacated ones
         if (i >= m && i < F) {
-            const int p = A.free_up[i];
-            A.pages_out[F - 1 - (i - m) - below(A.used_up + U - m, m, p)] = p;
+            const int p = free_up[i];
+            A.pages_out[F - 1 - (i - m) - below(used_up + U - m, m, p)] = p;
         }
         if (i < m) {
-            const int p = A.used_up[U - m + i];
-            A.pages_out[F - 1 - i - below(A.free_up + m, F - m, p)] = p;
+            const int p = used_up[U - m + i];
+            A.pages_out[F - 1 - i - below(free_up + m, F - m, p)] = p;
         }
         if (i >= F) A.pages_out[i] = -1;
         if (A.shared_out) {
-            const int s = A.state[i];                          // a page of nobody keeps its count
+            const int s = state[i];                          // a page of nobody keeps its count
             int x = A.shared[i];
             // where page i's contents come from: nothing new, the page that moved here, or it has moved away
-            if (s == 1) { const int k = below(A.free_up, F, i); if (k < m) x = A.shared[A.used_up[U - 1 - k]]; }
-            else if (s & 2) { const int k = U - 1 - below(A.used_up, U, i); if (k < m) x = 0; }
+            if (s == 1) { const int k = below(free_up, F, i); if (k < m) x = A.shared[used_up[U - 1 - k]]; }
+            else if (s & 2) { const int k = U - 1 - below(used_up, U, i); if (k < m) x = 0; }
             A.shared_out[i] = x;
         }
     }
     if (me == 0) *A.count_out = F;
     meet(blocks);
-    for (int64_t e = me; e < entries; e += all) {
+    for (int e = me; e < entries; e += all) {
         const int p = entry(e);
-        A.table_out[e] = is_page(p) ? A.to[p] : p;
+        A.table_out[e] = is_page(p) ? goes_to[p] : p;
     }
 }
 
@@ -385,21 +395,6 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(const __grid_c
                 if (e + k * COPY_THREADS < n) to[e + k * COPY_THREADS] = x[k];
         }
     }
-}
-
-template <typename A> int cluster_launch(void (*kern)(A), bool many, const A& args, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(many ? 8 : 1);                          // a cluster of eight is the most that any device takes
-    cfg.blockDim = dim3(SHARE_THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {many ? 8u : 1u, 1u, 1u};
-    cfg.attrs = at;
-    cfg.numAttrs = add_overlap(at, 1, launch_overlaps(st));
-    cudaLaunchKernelEx(&cfg, kern, args);
-    note_launch();
-    return check_launch();
 }
 
 // Entries of the table beyond which a launch over the device, or a cluster, takes less time than one block.  Latency bounds all of it: every trip to memory waits for
@@ -488,7 +483,27 @@ extern "C" int lowbit_paged_compact_cuda(const int32_t* d_table, int64_t table_s
     int32_t* const w = (int32_t*)workspace;
     const CompactArgs A = {d_table, table_stride, R, width, d_free_pages, n_pages, d_free_count, d_shared, d_table_out, d_free_pages_out, d_free_count_out, d_shared_out, d_src, d_dst,
                            w, w + n_pages, w + 2 * (int64_t)n_pages, w + 3 * (int64_t)n_pages};
-    return cluster_launch(paged_compact_kernel, (int64_t)R * width + n_pages > SHARE_MANY, A, (cudaStream_t)stream);
+    const bool many = (int64_t)R * width + n_pages > SHARE_MANY;
+    static bool configured[64] = {};                           // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        cudaFuncSetAttribute(paged_compact_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SHARE_MANY * 4 * sizeof(int32_t)));
+        configured[dev & 63] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(many ? 8 : 1);                          // a cluster of eight is the most that any device takes
+    cfg.blockDim = dim3(SHARE_THREADS);
+    cfg.dynamicSmemBytes = many ? 0 : lowbit_paged_compact_workspace_size(n_pages);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {many ? 8u : 1u, 1u, 1u};
+    cfg.attrs = at;
+    cfg.numAttrs = add_overlap(at, 1, launch_overlaps((cudaStream_t)stream));
+    cudaLaunchKernelEx(&cfg, many ? paged_compact_kernel<false> : paged_compact_kernel<true>, A);
+    note_launch();
+    return check_launch();
 }
 
 extern "C" int lowbit_paged_copy_cuda(const int32_t* d_src, const int32_t* d_dst, int n, void* const* caches, int n_caches, int n_pages, int64_t page_stride_bytes,
