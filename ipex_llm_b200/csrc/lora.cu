@@ -101,12 +101,26 @@ __device__ __forceinline__ void find_adapters(const LoraArgs& A, int64_t t0, Til
     if (threadIdx.x < TM) tile.id[threadIdx.x] = -2;
     __syncthreads();
     const int64_t end = min((int64_t)A.cu[A.R], A.T);          // rows behind it are nobody's
-    for (int r = threadIdx.x; r < A.R; r += LORA_THREADS) {
-        const int64_t a = A.cu[r], b = A.cu[r + 1];
+    auto begin = [&](int r, int64_t a, int64_t b) {
         const int id = A.ids[r];
         if (a < b && b > t0 && a < t0 + TM) tile.id[max(a - t0, (int64_t)0)] = id >= 0 && id < A.adapters ? id : -1;
+    };
+    bool rises = true;
+    for (int r = threadIdx.x; r < A.R; r += LORA_THREADS) {
+        const int a = A.cu[r], b = A.cu[r + 1];
+        rises &= a <= b;
+        begin(r, a, b);
     }
-    __syncthreads();
+    if (!__syncthreads_and(rises)) {                           // a list that goes back names no row twice: a request has what lies behind all in front of it
+        if (threadIdx.x < TM) tile.id[threadIdx.x] = -2;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int r = 0, most = A.cu[0]; r < A.R; r++) {
+                most = max(most, A.cu[r]);
+                begin(r, most, A.cu[r + 1]);
+            }
+        __syncthreads();
+    }
     if (threadIdx.x < 32) {
         // of rows `lane` and `lane` + 32: what began last
         int v[2] = {tile.id[lane], tile.id[lane + 32]};
@@ -198,7 +212,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
         __syncthreads();
     }
     const int chunks = (A.K + 31) / 32, each = (chunks + (int)blocks - 1) / (int)blocks, from = min((int)rank * each, chunks), to = min(from + each, chunks);
-    for (int j = blockIdx.y; j < n_adapters; j += gridDim.y) {
+    for (int j = DO == LORA_BOTH ? blockIdx.y : 0; j < n_adapters; j += gridDim.y) {
         int id = piece.x, count = piece.z;
         const int* row_of = tile.row;
         if constexpr (DO == LORA_BOTH) {
@@ -207,7 +221,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             row_of += tile.first[j];
         }
         const float scale = A.scales[id];
-        for (int s0 = 0; s0 < A.n_splits; s0 += A.together) {
+        const int s_from = DO == LORA_FIRST ? blockIdx.y * A.together : 0, s_step = DO == LORA_FIRST ? gridDim.y * A.together : A.together;
+        for (int s0 = s_from; s0 < A.n_splits; s0 += s_step) {
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
             const uint4* const w = (const uint4*)((const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K);
             // ---- h of this block's share of K.  Rows behind the last, of A and of x, are read as the last ones: nobody looks at what they give
@@ -433,7 +448,8 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     for (int n = 0; n < 4; n++) take(n, of.c0 + 8 * (g >> 1) + 2 * n + (g & 1) < of.c_end && 16 * st + (WIDE ? 8 : 4) * t < A.rank);
                 }
             };
-            uint2 br[STEPS ? STEPS : 1][4];
+            uint2 br[STEPS ? STEPS : 2][4];
+            if (!STEPS && more) fetch(ahead, 0, br);
             if (STEPS && more) {
 #pragma unroll
                 for (int st = 0; st < STEPS; st += WIDE ? 2 : 1) fetch(ahead, st, br + st);
@@ -507,15 +523,19 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                             for (int st = 0; st < STEPS; st += WIDE ? 2 : 1) fetch(ahead, st, br + st);
                         }
                     } else {
-                        fetch(now, 0, br);
-                        ask_h(m, 0, hi[0], lo[0]);
-                        products(hi[0], lo[0], br[0], true);
-#pragma unroll 1
-                        for (int st = 1; st < steps; st++) {
-                            fetch(now, st, br);
+                        if (m > 0) fetch(now, 0, br);
+                        auto step = [&](int st, int at, bool first) {
+                            if (st + 1 < steps) fetch(now, st + 1, br + (at ^ 1));
                             ask_h(m, st, hi[0], lo[0]);
-                            products(hi[0], lo[0], br[0], false);
+                            products(hi[0], lo[0], br[at], first);
+                        };
+                        step(0, 0, true);
+#pragma unroll 1
+                        for (int st = 1; st < steps; st += 2) {
+                            step(st, 1, false);
+                            if (st + 1 < steps) step(st + 1, 0, false);
                         }
+                        if (m + P >= m_tiles && more) fetch(ahead, 0, br);
                     }
 #pragma unroll
                     for (int q = 0; q < P; q++)
@@ -656,11 +676,21 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraA
     }
 }
 
-// From here on three launches: 882 rows of 40 requests 40 us, by one 68; 11849 rows 140 and 171.  64 tokens are the other way round: 12.3 us by one launch, and no less
-// than 18 by two of the kind.
-constexpr int64_t LORA_MANY = 256;
+// One launch or three.  One has a cluster for each adapter of a tile: where these are more than the device takes at once three take less time, and where they are few and
+// a cluster's columns many.  K 4096, N 4096, rank 16: 64 tokens of 32 adapters 12 us by one, 17 by three; 256 of 8 9 and 16; 150 of 30 31 and 17; 256 of 64 111 and 25.
+// N 22016: 16 tokens of one adapter 12 and 13, 64 24 and 18; at rank 64 22 and 23, 51 and 36; at rank 128 4 tokens 49 and 41, 64 124 and 74.
+constexpr int LORA_BLOCKS = 8;                                 // of a cluster: the most that any device takes
+int64_t lora_tile_adapters(int adapters, int R) { const int64_t most = adapters < R ? adapters : R; return most < TM ? most : TM; }
 // splits that share a reading of x: 128 rows of A at most (their parts and h fill what shared memory two blocks of an SM have), or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
+bool lora_many(int64_t T, int64_t N, int rank, int n_splits, int adapters, int R) {
+    const bool alone = lora_together(rank, n_splits) * rank > 64;                              // a block fills its SM's shared memory
+    const int64_t blocks = (T + TM - 1) / TM * lora_tile_adapters(adapters, R) * LORA_BLOCKS, places = (alone ? 1ll : 2ll) * sm_count();
+    if (blocks > places) return true;
+    // groups of columns a warp, by what one costs: itself, its tokens, its steps.  With half the device busy only large ranks are worth the launches
+    const int64_t each = T / (adapters < R ? adapters : R), work = N / 32 * ((each < TM ? each : TM) + 16 + 4 * Lora::steps(rank)), much = 400ll * LORA_BLOCKS * LORA_WARPS;
+    return 2 * blocks <= places ? work >= much : Lora::steps(rank) >= 4 && work >= (alone ? much : much * 3 / 2);
+}
 // pieces that T rows of R requests may have: of whole 64, and one of every adapter
 int64_t lora_pieces(int64_t T, int adapters, int R) { int64_t most = adapters < R ? adapters : R; if (most > T) most = T; return T / TM + most; }
 size_t lora_lists_bytes(int64_t T, int adapters, int R) {
@@ -683,16 +713,17 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     // clusters of tiles, and those that share a tile's adapters: twice as many as a tile has on average, since neighbours' differ; those that find none leave at
     // once.  Or of pieces
     const int64_t tiles = many ? lora_pieces(A.T, A.adapters, A.R) : (A.T + TM - 1) / TM;
-    int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T, most = TM < A.R ? TM : A.R;
-    if (most > A.adapters) most = A.adapters;
-    if (some > most) some = most;
-    if (many) some = 1;
-    // blocks of a cluster, which share the inner dimension (and the columns): 8, the most that any device takes (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
-    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the tiles fill the device: 11849 rows by 2 blocks of a piece 141 us, by
+    int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T;
+    if (some > lora_tile_adapters(A.adapters, A.R)) some = lora_tile_adapters(A.adapters, A.R);
+    // blocks of a cluster, which share the inner dimension (and the columns): 8 (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
+    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the pieces fill the device: 11849 rows by 2 blocks of a piece 141 us, by
     // 4 143, by 8 152; 882 rows by 8 41, by 4 44, by 2 52
-    int blocks = 8;
+    int blocks = LORA_BLOCKS;
     while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
     if (many) {
+        // splits one after the other share a reading of x, or, where there is room for their clusters, each has its own
+        some = 1;
+        if (tiles * blocks * A.n_splits <= 2ll * sm_count()) { A.together = 1; some = A.n_splits; }
         launch_behind(lora_order_kernel, dim3(1), SORT_THREADS, 0, st, on, A, row0, (int)A.T, (int)tiles);
         note_launch();
     }
@@ -710,6 +741,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
+        A.together = lora_together(A.rank, A.n_splits);
         // blocks of a piece's columns: eight an SM's two places (11849 rows by 8 shares of a piece 147 us, by 4 150, by 16 173, in an earlier form), none with fewer than three groups a
         // warp, which would read h more often than it uses it
         const int64_t want = 8ll * sm_count() / tiles, room = A.first[A.n_splits] / (32 * LORA_WARPS * 3);
@@ -731,8 +763,8 @@ template <bool BF> int lora_steps(const LoraArgs& A, int64_t row0, cudaStream_t 
 }  // namespace
 }  // namespace lowbit
 
-extern "C" size_t lowbit_lora_workspace_size(int64_t T, int rank, int n_splits, int adapters, int R) {
-    if (T <= LORA_MANY || rank <= 0 || n_splits <= 0 || adapters <= 0 || R <= 0) return 0;
+extern "C" size_t lowbit_lora_workspace_size(int64_t T, int64_t N, int rank, int n_splits, int adapters, int R) {
+    if (T <= 0 || N <= 0 || rank <= 0 || n_splits <= 0 || adapters <= 0 || R <= 0 || !lora_many(T, N, rank, n_splits, adapters, R)) return 0;
     return lora_lists_bytes(T, adapters, R) + (size_t)T * n_splits * (Lora::steps(rank) * 64 + sizeof(float));
 }
 
@@ -756,7 +788,8 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
         return LB_ERR_ARG;
     }
     if (T == 0) return LB_OK;
-    if (T > LORA_MANY && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < lowbit_lora_workspace_size(T, rank, n_splits, adapters, R))) {
+    const size_t need = lowbit_lora_workspace_size(T, N, rank, n_splits, adapters, R);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) {
         set_error(LB_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of lowbit_lora_workspace_size() bytes is needed", name);
         return LB_ERR_WORKSPACE;
     }
@@ -764,7 +797,7 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
                   nullptr, nullptr, nullptr, nullptr, nullptr, 0, {}};
     for (int i = 0; i < n_splits; i++) A.first[i + 1] = A.first[i] + splits[i];
     cudaStream_t st = (cudaStream_t)stream;
-    if (T <= LORA_MANY) return dtype == DT_BF16 ? lora_steps<true>(A, 0, st) : lora_steps<false>(A, 0, st);
+    if (!need) return dtype == DT_BF16 ? lora_steps<true>(A, 0, st) : lora_steps<false>(A, 0, st);
     uint8_t* const w = (uint8_t*)workspace;
     A.pieces = (int4*)w;
     A.order = (int32_t*)(w + lora_pieces(T, adapters, R) * sizeof(int4));

@@ -40,7 +40,7 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     ``splits``: the widths of the projections that ``out`` merges (queries, keys and values: 4096, 1024, 1024), each with an A of its own: ``a`` is then
     [adapters, len(splits), rank, K], and columns of a projection take the product with its A.
 
-    x A^T is kept in 32 bits and enters the second product as two 16-bit values, so that only ``out`` is rounded, once.  One launch for up to 256 rows, three for more; nothing
+    x A^T is kept in 32 bits and enters the second product as two 16-bit values, so that only ``out`` is rounded, once.  One launch, or three for more rows or larger products; nothing
     comes back to the host, and the lists are read on the device: a recorded step serves other requests.  An ``x`` that shares memory with ``out`` is copied first.  There is no backward pass: tensors that want a
     gradient or carry a tangent are refused."""
     if splits is not None:
@@ -82,7 +82,7 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     a, b = (t if t[0].is_contiguous() and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and (t.shape[0] == 1 or t.stride(0) >= t[0].numel())
             else t.clone(memory_format=torch.contiguous_format) for t in (a, b))
     with torch.cuda.device(dev):
-        ws = torch.empty(ggml.lowbit_lora_workspace_size(T, R, S, L, adapter_ids.shape[0]), dtype=torch.uint8, device=dev)
+        ws = torch.empty(ggml.lowbit_lora_workspace_size(T, N, R, S, L, adapter_ids.shape[0]), dtype=torch.uint8, device=dev)
         ggml.lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, ws, torch._C._cuda_getCurrentRawStream(dev.index))
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)

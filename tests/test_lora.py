@@ -370,9 +370,9 @@ def test_refusals_on_the_cpu(lora, native_lib):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 1, (i, bad)
-    good[3], good[19], good[20] = 300, some, 1 << 30
-    for i, bad in ((19, None), (19, 4100), (20, 300 * 2 * 16 * 4)):
+    good[3], good[19], good[20] = 3000, some, 1 << 30
+    for i, bad in ((19, None), (19, 4100), (20, 3000 * 2 * 16 * 4)):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
-    assert lib.lowbit_lora_workspace_size(256, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(257, 16, 2, 3, 4) >= 257 * (32 * 4 + 4)
+    assert lib.lowbit_lora_workspace_size(64, 64, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(3000, 64, 16, 2, 3, 4) >= 3000 * (32 * 4 + 4)
