@@ -160,10 +160,8 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 // sums of the warps on their way together; h as two 16-bit values; the block's part of h.  The first product takes 32 tokens at a time, 64 in a launch of
 // its own, whose stages are of 6 KB: A is read half as often.
 struct Lora {
-    static constexpr int MT = 2, ROWS = 16 * MT;              // tiles of 16 rows of A in the first product
-    static constexpr int PITCH = ROWS + 4;                     // a warp's stores of sums meet every bank once
     static constexpr int kStage = 8 * 512, kRing = LORA_WARPS * 2 * kStage, kRingFirst = LORA_WARPS * 2 * 12 * 512;
-    static_assert(kRing >= LORA_WARPS * 32 * PITCH * 4 && kRingFirst >= LORA_WARPS * TM * PITCH * 4, "the sums fit");
+    static constexpr int kRingWide = LORA_WARPS * TM * (64 + 4) * 4;                           // 64 rows of A at a time: the sums are larger than the stages
     static __host__ __device__ int steps(int rank) { return (rank + 15) / 16; }
     // h as the second product's A operand: for each split, step of 16 and tile of 16 tokens 16 bytes a lane of high parts, then of low parts
     static constexpr int kFrag = 1024, kStep = TM / 16 * kFrag;
@@ -178,12 +176,16 @@ struct Lora {
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
 // holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  With an even number a lane reads 16 bytes of B, in the first product's order
 // of two steps' k.  (The first product alone: 4 for up to 4.)
-enum { LORA_BOTH, LORA_FIRST, LORA_SECOND };
+enum { LORA_BOTH, LORA_FIRST, LORA_WIDE, LORA_SECOND };                                      // WIDE: the first with 64 rows of A at a time
 template <bool BF, int STEPS, int DO>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A) {
+__global__ void __launch_bounds__(LORA_THREADS, DO == LORA_WIDE ? 1 : 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
     constexpr bool WIDE = STEPS == 2 || STEPS == 4;
-    constexpr int NT = DO == LORA_FIRST ? 8 : 4, TOKS = 8 * NT, MT = L::MT, ROWS = L::ROWS, STAGE = (NT + 2 * MT) * 512;      // of the first product
+    constexpr bool FIRST = DO == LORA_FIRST || DO == LORA_WIDE;
+    // of the first product: tiles of 8 tokens and of 16 rows of A; a warp's stores of sums meet every bank once
+    constexpr int NT = FIRST ? 8 : 4, TOKS = 8 * NT, MT = DO == LORA_WIDE ? 4 : 2, ROWS = 16 * MT, PITCH = ROWS + 4, STAGE = (NT + 2 * MT) * 512;
+    constexpr int RING = DO == LORA_WIDE ? L::kRingWide : FIRST ? L::kRingFirst : L::kRing;
+    static_assert(RING >= LORA_WARPS * 2 * STAGE && RING >= LORA_WARPS * TOKS * PITCH * 4, "the stages fit, and the sums");
     __shared__ std::conditional_t<DO == LORA_BOTH, Tile, Rows> tile;
     __shared__ float back[TM][LORA_SPLITS];                    // what undoes a row's power of two
     extern __shared__ __align__(128) uint8_t lora_smem[];
@@ -194,9 +196,9 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
     }
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = DO == LORA_BOTH ? (int64_t)(blockIdx.x / blocks) * TM : 0;
-    const int steps = STEPS && DO != LORA_FIRST ? STEPS : L::steps(A.rank);
+    const int steps = STEPS && !FIRST ? STEPS : L::steps(A.rank);
     float* const sums = reinterpret_cast<float*>(lora_smem);
-    float* const part = reinterpret_cast<float*>(lora_smem + (DO == LORA_FIRST ? L::kRingFirst : L::kRing + A.together * steps * L::kStep));
+    float* const part = reinterpret_cast<float*>(lora_smem + RING + (FIRST ? 0 : A.together * steps * L::kStep));
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(lora_smem), ring = smem + warp * 2 * L::kStage + lane * 16, ring1 = smem + warp * 2 * STAGE + lane * 16, hs = smem + L::kRing;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -221,12 +223,12 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             row_of += tile.first[j];
         }
         const float scale = A.scales[id];
-        const int s_from = DO == LORA_FIRST ? blockIdx.y * A.together : 0, s_step = DO == LORA_FIRST ? gridDim.y * A.together : A.together;
+        const int s_from = FIRST ? blockIdx.y * A.together : 0, s_step = FIRST ? gridDim.y * A.together : A.together;
         for (int s0 = s_from; s0 < A.n_splits; s0 += s_step) {
             const int n_here = min(A.together, A.n_splits - s0), rows = n_here * A.rank;
             const uint4* const w = (const uint4*)((const uint16_t*)A.a + id * A.a_st + (int64_t)s0 * A.rank * A.K);
             // ---- h of this block's share of K.  Rows behind the last, of A and of x, are read as the last ones: nobody looks at what they give
-            const int groups = DO == LORA_FIRST ? 1 : rows > 2 * ROWS ? 4 : rows > ROWS ? 2 : 1, of_group = LORA_WARPS / groups, nth = warp & (of_group - 1);
+            const int groups = FIRST ? 1 : rows > 2 * ROWS ? 4 : rows > ROWS ? 2 : 1, of_group = LORA_WARPS / groups, nth = warp & (of_group - 1);
             for (int rows0 = 0, i0 = 0; DO != LORA_SECOND && rows0 < rows; i0 = i0 + TOKS < count ? i0 + TOKS : 0, rows0 += i0 ? 0 : ROWS * groups) {
                 const int row0 = rows0 + warp / of_group * ROWS, m_end = min(MT, (rows - row0 + 15) / 16), n_end = min(NT, (count - i0 + 7) / 8);
                 const int last = m_end > 0 ? to : from;        // nothing for a group behind the last row
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                         for (int m = 0; m < MT; m++)
                             if (m < m_end) {
 #pragma unroll
-                                for (int e = 0; e < 4; e++) sums[(warp * TOKS + 8 * n + 2 * t + (e & 1)) * L::PITCH + 16 * m + g + 8 * (e >> 1)] = acc[m][n][e];
+                                for (int e = 0; e < 4; e++) sums[(warp * TOKS + 8 * n + 2 * t + (e & 1)) * PITCH + 16 * m + g + 8 * (e >> 1)] = acc[m][n][e];
                             }
                     }
                 __syncthreads();
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
 #pragma unroll
                         for (int v = 0; v < LORA_WARPS; v++) {
                             if (v >= of_group) break;
-                            const float4 p = *reinterpret_cast<const float4*>(sums + ((group * of_group + v) * TOKS + tok) * L::PITCH + in);
+                            const float4 p = *reinterpret_cast<const float4*>(sums + ((group * of_group + v) * TOKS + tok) * PITCH + in);
                             s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
                         }
                         *reinterpret_cast<float4*>(part + (i0 + tok) * rows + row) = s;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
             for (int i = 0; i < TM / 8; i++) row_at[i] = (uint32_t)(row_of[min(8 * i + g, count - 1)] * A.o_st / 8);
             uint4* const out = reinterpret_cast<uint4*>((uint16_t*)A.out + t0 * A.o_st);
             Group ahead = {0, 0, (A.first[s0 + 1] - A.first[s0] + 31) / 32, (int)rank * LORA_WARPS + warp, 0, 0};
-            bool more = DO != LORA_FIRST && ahead.settle(A, s0, n_here);
+            bool more = !FIRST && ahead.settle(A, s0, n_here);
             auto ask_out = [&](int stage) {
                 if (more) {
                     const uint4* const from = out + min(ahead.c0 + 8 * t, ahead.c_end - 8) / 8;
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const int e = (int)(__float_as_uint(big) >> 23) - 127 - 14, use = big > 0.0f && big < INFINITY ? max(e, -100) : 0;
                     const float up = __uint_as_float((uint32_t)(127 + use) << 23);
                     down = __uint_as_float((uint32_t)(127 - use) << 23);
-                    if (DO == LORA_FIRST) {
+                    if (FIRST) {
                         if (lane == 0) A.back[(int64_t)(piece.y + tok) * A.n_splits + s0 + s] = up;
                     } else if (lane < (int)others) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(shared_of(at_back + (tok * LORA_SPLITS + s) * 4, lane)), "f"(up) : "memory");
                 }
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     const uint32_t hi = pack2<BF>(x, y);
                     const float2 f = unpack2<BF>(hi);
                     const uint32_t lo = pack2<BF>(fabsf(f.x) < INFINITY ? x - f.x : 0.0f, fabsf(f.y) < INFINITY ? y - f.y : 0.0f);
-                    if (DO == LORA_FIRST) {
+                    if (FIRST) {
                         uint16_t* const to = A.h + (int64_t)(piece.y + tok) * (A.n_splits * 32 * steps) + (s0 + s) * 32 * steps + r;
                         *reinterpret_cast<uint32_t*>(to) = hi;
                         *reinterpret_cast<uint32_t*>(to + 16 * steps) = lo;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_kernel(const LoraArgs A)
                     place(tok, s, h);
                 }
             }
-            if (DO == LORA_FIRST) {
+            if (FIRST) {
                 meet(blocks);                                  // the parts are read: they may be written again, and their block may leave
                 continue;
             }
@@ -705,6 +707,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     if (!configured[dev & 63]) {
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1) + Lora::parts(256, 1));
         cudaFuncSetAttribute(lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, STEPS ? 4 : 0, LORA_WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingWide + Lora::parts(256, 1));
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
     }
@@ -730,7 +733,10 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)some);
     cfg.blockDim = dim3(LORA_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(many ? Lora::kRingFirst : Lora::smem(A.rank, A.together)) + Lora::parts(A.rank, A.together);
+    // 64 rows of A at a time by a block that has its SM to itself: more work for what it reads, fewer to read.  Rank 128, K 4096, N 896: 12000 tokens 148 us and 192 by 32
+    // rows at a time, 600 50 and 54; rank 64, K 11008, N 4096: 12000 176 and 215, but 3000 80 and 79, and 882 of 40 requests 45 and 41
+    const bool wide = many && A.together * A.rank > 32 && (A.together * A.rank > 64 || tiles >= sm_count());
+    cfg.dynamicSmemBytes = (size_t)(wide ? Lora::kRingWide : many ? Lora::kRingFirst : Lora::smem(A.rank, A.together)) + Lora::parts(A.rank, A.together);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -738,7 +744,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, on);
     A.shares = 1;
-    cudaLaunchKernelEx(&cfg, many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
+    cudaLaunchKernelEx(&cfg, wide ? lora_kernel<BF, STEPS ? 4 : 0, LORA_WIDE> : many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
         A.together = lora_together(A.rank, A.n_splits);
