@@ -344,7 +344,7 @@ int lowbit_paged_norm_rope_append_cuda(void* d_qkv, int dtype, int64_t token_str
 int lowbit_paged_fork_cuda(const int32_t* d_parents, const int32_t* d_children, int F, int32_t* d_lens, int32_t* d_table, int64_t table_stride,
                            int R, int width, const int32_t* d_free_pages, int n_pages, const int32_t* d_free_count, int32_t* d_free_left,
                            int32_t* d_shared, int page_size, int32_t* d_src, int32_t* d_dst, int32_t* d_missing, void* stream);
-size_t lowbit_paged_share_release_workspace_size(int n_pages, int R);
+size_t lowbit_paged_share_release_workspace_size(int n_pages, int R, int width);
 int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int32_t* d_held, int page_size, int R, int32_t* d_table, int64_t table_stride,
                                     int width, int32_t* d_free_pages, int n_pages, int32_t* d_free_count, int32_t* d_shared, void* workspace,
                                     size_t workspace_bytes, void* stream);

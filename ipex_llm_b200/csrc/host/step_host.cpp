@@ -18,7 +18,7 @@ using NormFn = int (*)(void*, int, int64_t, int64_t, int, int, int, int, const v
                        const int64_t*, void*, const int64_t*, void*, const int64_t*, int, int, int, void*);
 using ForkFn = int (*)(const int32_t*, const int32_t*, int, int32_t*, int32_t*, int64_t, int, int, const int32_t*, int, const int32_t*, int32_t*, int32_t*, int, int32_t*, int32_t*,
                        int32_t*, void*);
-using ReleaseSizeFn = size_t (*)(int, int);
+using ReleaseSizeFn = size_t (*)(int, int, int);
 using ReleaseFn = int (*)(const uint8_t*, const int32_t*, int, int, int32_t*, int64_t, int, int32_t*, int, int32_t*, int32_t*, void*, size_t, void*);
 using CompactSizeFn = size_t (*)(int);
 using CompactFn = int (*)(const int32_t*, int64_t, int, int, const int32_t*, int, const int32_t*, const int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, void*,
@@ -191,7 +191,7 @@ PyObject* paged_share_release(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
     {
         const WithoutGil released;
         const c10::cuda::CUDAGuard guard(done->device());
-        const size_t need = g_release_size((int)pages->size(0), (int)done->size(0));
+        const size_t need = g_release_size((int)pages->size(0), (int)done->size(0), (int)table->size(1));
         const at::Tensor scratch = at::empty({(int64_t)need}, done->options().dtype(at::kByte));
         rc = g_release(static_cast<const uint8_t*>(done->const_data_ptr()), held ? held->const_data_ptr<int32_t>() : nullptr, (int)page, (int)done->size(0),
                        table->mutable_data_ptr<int32_t>(), table->stride(0), (int)table->size(1), pages->mutable_data_ptr<int32_t>(), (int)pages->size(0),

@@ -132,40 +132,44 @@ struct ShareReleaseArgs {
     const uint8_t* done; const int32_t* held; int page_size;
     int R; int32_t* table; int64_t table_stride; int width;
     int32_t* pages; int n_pages; int32_t* count; int32_t* shared;
-    int32_t* times; int32_t* first; int32_t* gives;            // scratch: [pages], [pages], [R + 1]
+    int32_t* times; int32_t* first; int32_t* gives;            // scratch: [pages], [pages], [stretches + 1]
 };
+constexpr int SHARE_STRETCH = 32 * SHARE_DEEP;                 // columns of a row that a warp takes at a time
+inline int64_t share_stretches(int R, int width) { return (int64_t)R * ((width + SHARE_STRETCH - 1) / SHARE_STRETCH); }
 
 // Rows that are done give up what they name (behind `held` tokens): page p, named `times` in all, goes onto the stack where that is more than shared[p],
-// in the order of the entries that name it first.  A warp a row, four times: places cleared, names counted, pages settled and those of a row counted, pages written.  One block
-// does all four (PART -1); where there is more to do each is a launch over the whole device, and the count's place is the launch's behind that reads it.
+// in the order of the entries that name it first.  A warp a stretch of a row, four times: places cleared, names counted, pages settled and those of a stretch counted, pages
+// written.  One block does all four (PART -1); where there is more to do each is a launch over the whole device, and the count's place is the launch's behind that reads it.
 template <int PART>
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(const ShareReleaseArgs A) {
     __shared__ int warps[32];
     __shared__ int before[SHARE_THREADS];
     const int lane = threadIdx.x & 31, blocks = gridDim.x, me = (threadIdx.x >> 5) * blocks + blockIdx.x, all = blocks * SHARE_WARPS;
+    const int of_row = (A.width + SHARE_STRETCH - 1) / SHARE_STRETCH, stretches = A.R * of_row;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = max(0, min(*A.count, A.n_pages));
-    auto from = [&](int r) { return A.held ? (int)min((int64_t)A.width, ((int64_t)max(A.held[r], 0) + A.page_size - 1) / A.page_size) : 0; };
-    // the pages of row r, SHARE_DEEP a lane at a time: f(first column of this lane, pages, -1 what is none); whole warps
-    auto each = [&](int r, auto&& f) {
+    // what stretch s gives up: f(its row, this lane's first column, its pages, SHARE_DEEP a lane, -1 what is none, the first column that goes); whole warps
+    auto each = [&](int s, auto&& f) {
+        const int r = s / of_row, c = (s - r * of_row) * SHARE_STRETCH + lane;
+        if (!A.done[r]) return;
+        const int from = A.held ? (int)min((int64_t)A.width, ((int64_t)max(A.held[r], 0) + A.page_size - 1) / A.page_size) : 0;
         const int32_t* const row = A.table + r * A.table_stride;
-        for (int c0 = from(r); c0 < A.width; c0 += 32 * SHARE_DEEP) {
-            int p[SHARE_DEEP];
+        int p[SHARE_DEEP];
 #pragma unroll
-            for (int u = 0; u < SHARE_DEEP; u++) {
-                const int c = c0 + lane + 32 * u;
-                p[u] = c < A.width ? row[c] : -1;
-            }
+        for (int u = 0; u < SHARE_DEEP; u++) p[u] = c + 32 * u >= from && c + 32 * u < A.width ? row[c + 32 * u] : -1;
 #pragma unroll
-            for (int u = 0; u < SHARE_DEEP; u++) p[u] = p[u] < A.n_pages ? p[u] : -1;
-            f(c0 + lane, p);
-        }
+        for (int u = 0; u < SHARE_DEEP; u++) p[u] = p[u] < A.n_pages ? p[u] : -1;
+        f(r, c, p, from);
     };
     using Pages = const int (&)[SHARE_DEEP];
+    if (PART == 0 && A.n_pages <= A.R * A.width) {             // all places: without a look at the table
+        for (int p = (int)(blockIdx.x * SHARE_THREADS + threadIdx.x); p < A.n_pages; p += blocks * SHARE_THREADS) { A.times[p] = 0; A.first[p] = 0x7fffffff; }
+        return;
+    }
     if (PART < 0 || PART == 0) {
-        for (int r = me; r < A.R; r += all)
-            if (A.done[r]) each(r, [&](int, Pages p) {
+        for (int s = me; s < stretches; s += all)
+            each(s, [&](int, int, Pages p, int) {
 #pragma unroll
                 for (int u = 0; u < SHARE_DEEP; u++)
                     if (p[u] >= 0) { A.times[p[u]] = 0; A.first[p[u]] = 0x7fffffff; }
@@ -173,8 +177,8 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
     }
     if (PART < 0) __syncthreads();
     if (PART < 0 || PART == 1) {
-        for (int r = me; r < A.R; r += all)
-            if (A.done[r]) each(r, [&](int c, Pages p) {
+        for (int s = me; s < stretches; s += all)
+            each(s, [&](int r, int c, Pages p, int) {
 #pragma unroll
                 for (int u = 0; u < SHARE_DEEP; u++)
                     if (p[u] >= 0) { atomicAdd(A.times + p[u], 1); atomicMin(A.first + p[u], r * A.width + c + 32 * u); }
@@ -182,9 +186,9 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
     }
     if (PART < 0) __syncthreads();
     if (PART < 0 || PART == 2) {
-        for (int r = me; r < A.R; r += all) {
+        for (int s = me; s < stretches; s += all) {
             int n = 0;
-            if (A.done[r]) each(r, [&](int c, Pages p) {
+            each(s, [&](int r, int c, Pages p, int) {
                 // the entry that names its page first settles the page: `times` is from now on by how many more that was given up than shared says
                 bool mine[SHARE_DEEP];
                 int more[SHARE_DEEP];
@@ -198,25 +202,24 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
                     n += __popc(__ballot_sync(0xffffffffu, more[u] > 0));
                 }
             });
-            if (lane == 0) A.gives[r] = n;
+            if (lane == 0) A.gives[s] = n;
         }
     }
     if (PART < 0) __syncthreads();
     if (PART >= 0 && PART != 3) return;
     int top = count;
-    for (int r0 = 0; r0 < A.R; r0 += SHARE_THREADS) {
-        const int n = r0 + (int)threadIdx.x < A.R ? A.gives[r0 + threadIdx.x] : 0;
+    for (int s0 = 0; s0 < stretches; s0 += SHARE_THREADS) {
+        const int n = s0 + (int)threadIdx.x < stretches ? A.gives[s0 + threadIdx.x] : 0;
         int total;
         const int sum = block_sum(n, warps, total);
         __syncthreads();
         before[threadIdx.x] = top + sum - n;
         __syncthreads();
-        // rows as they were dealt above
-        for (int r = r0 + (me - r0 % all + all) % all; r < min(r0 + SHARE_THREADS, A.R); r += all) {
-            if (!A.done[r]) continue;
-            int at = before[r - r0];
-            int32_t* const row = A.table + r * A.table_stride;
-            each(r, [&](int c, Pages p) {
+        // stretches as they were dealt above
+        for (int s = s0 + (me - s0 % all + all) % all; s < min(s0 + SHARE_THREADS, stretches); s += all) {
+            int at = before[s - s0];
+            each(s, [&](int r, int c, Pages p, int from) {
+                int32_t* const row = A.table + r * A.table_stride;
                 int first[SHARE_DEEP], times[SHARE_DEEP];
                 bool goes[SHARE_DEEP];
 #pragma unroll
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
                     const uint32_t yes = __ballot_sync(0xffffffffu, goes[u]);
                     const int slot = at + __popc(yes & ((1u << lane) - 1u));
                     if (goes[u] && slot < A.n_pages) A.pages[slot] = p[u];
-                    if (c + 32 * u < A.width) row[c + 32 * u] = -1;
+                    if (c + 32 * u >= from && c + 32 * u < A.width) row[c + 32 * u] = -1;
                     at += __popc(yes);
                 }
             });
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_share_release_kernel(c
         __syncthreads();
     }
     // the count may be read by other blocks yet: the sum of what was given goes where the launch behind finds it
-    if (blockIdx.x == 0 && threadIdx.x == 0) *(PART < 0 ? A.count : A.gives + A.R) = min(top, A.n_pages);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *(PART < 0 ? A.count : A.gives + stretches) = min(top, A.n_pages);
 }
 __global__ void paged_share_count_kernel(const int32_t* top, int32_t* count) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(const __grid_c
 // a block, 6.3 by a cluster.  Releases by a block with eight entries a lane at a time 45 us, with one 70, with four 52, with sixteen no less.
 constexpr int64_t SHARE_MANY = 8192;
 // blocks over the whole device, of rows by warps
-int wide_grid(int rows) { return rows < sm_count() ? rows : sm_count(); }
+int wide_grid(int64_t rows) { return rows < sm_count() ? (int)rows : sm_count(); }
 
 // of a list: a step beyond its end stays in 32 bits
 constexpr int SHARE_MOST = 1 << 30;
@@ -433,7 +436,9 @@ extern "C" int lowbit_paged_fork_cuda(const int32_t* d_parents, const int32_t* d
     return check_launch();
 }
 
-extern "C" size_t lowbit_paged_share_release_workspace_size(int n_pages, int R) { return n_pages > 0 && R > 0 ? ((size_t)n_pages * 2 + R + 1) * sizeof(int32_t) : 0; }
+extern "C" size_t lowbit_paged_share_release_workspace_size(int n_pages, int R, int width) {
+    return n_pages > 0 && R > 0 && width > 0 ? ((size_t)n_pages * 2 + share_stretches(R, width) + 1) * sizeof(int32_t) : 0;
+}
 
 extern "C" int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int32_t* d_held, int page_size, int R, int32_t* d_table, int64_t table_stride, int width,
                                                int32_t* d_free_pages, int n_pages, int32_t* d_free_count, int32_t* d_shared, void* workspace, size_t workspace_bytes,
@@ -443,7 +448,7 @@ extern "C" int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int3
         set_error(LB_ERR_ARG, "lowbit_paged_share_release_cuda: bad argument (R %d, width %d, pages %d, page_size %d)", R, width, n_pages, page_size);
         return LB_ERR_ARG;
     }
-    if (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < lowbit_paged_share_release_workspace_size(n_pages, R)) {
+    if (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < lowbit_paged_share_release_workspace_size(n_pages, R, width)) {
         set_error(LB_ERR_WORKSPACE, "lowbit_paged_share_release_cuda: a workspace of lowbit_paged_share_release_workspace_size() bytes is needed");
         return LB_ERR_WORKSPACE;
     }
@@ -455,12 +460,12 @@ extern "C" int lowbit_paged_share_release_cuda(const uint8_t* d_done, const int3
         note_launch();
         return check_launch();
     }
-    const dim3 grid((unsigned)wide_grid(R));
+    const dim3 grid((unsigned)wide_grid(share_stretches(R, width)));
     launch_behind(paged_share_release_kernel<0>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
     launch_behind(paged_share_release_kernel<1>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
     launch_behind(paged_share_release_kernel<2>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
     launch_behind(paged_share_release_kernel<3>, grid, SHARE_THREADS, 0, st, launch_overlaps(st), A);
-    launch_behind(paged_share_count_kernel, dim3(1), 1, 0, st, launch_overlaps(st), A.gives + R, d_free_count);
+    launch_behind(paged_share_count_kernel, dim3(1), 1, 0, st, launch_overlaps(st), A.gives + share_stretches(R, width), d_free_count);
     for (int i = 0; i < 5; i++) note_launch();
     return check_launch();
 }

@@ -770,7 +770,7 @@ def lowbit_paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary_dim
 _lib.lowbit_paged_fork_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
                                         ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 4
 _lib.lowbit_paged_fork_cuda.restype = ctypes.c_int
-_lib.lowbit_paged_share_release_workspace_size.argtypes = [ctypes.c_int, ctypes.c_int]
+_lib.lowbit_paged_share_release_workspace_size.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int]
 _lib.lowbit_paged_share_release_workspace_size.restype = ctypes.c_size_t
 _lib.lowbit_paged_share_release_cuda.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
                                                  ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
@@ -791,8 +791,8 @@ def lowbit_paged_fork(parents, children, lens, table, free_pages, free_count, fr
                                        dst.data_ptr(), missing.data_ptr(), stream), "lowbit_paged_fork_cuda")
 
 
-def lowbit_paged_share_release_workspace_size(n_pages, rows):
-    return _lib.lowbit_paged_share_release_workspace_size(n_pages, rows)
+def lowbit_paged_share_release_workspace_size(n_pages, rows, width):
+    return _lib.lowbit_paged_share_release_workspace_size(n_pages, rows, width)
 
 
 def lowbit_paged_share_release(done, held, page_size, table, free_pages, free_count, shared, workspace, stream):

@@ -143,7 +143,7 @@ def paged_release(done, block_table, free_pages, free_count, held=None, page_siz
         _device(done, shared)
         _ints(shared, free_pages.shape[0], "shared")
         with torch.cuda.device(dev):
-            ws = torch.empty(ggml.lowbit_paged_share_release_workspace_size(shared.shape[0], done.shape[0]), dtype=torch.uint8, device=dev)
+            ws = torch.empty(ggml.lowbit_paged_share_release_workspace_size(shared.shape[0], *block_table.shape), dtype=torch.uint8, device=dev)
             ggml.lowbit_paged_share_release(done, held, page_size, block_table, free_pages, free_count, shared, ws, _stream(dev))
         return
     with torch.cuda.device(dev):
