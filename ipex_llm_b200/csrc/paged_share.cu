@@ -268,7 +268,7 @@ __device__ __forceinline__ int below(const int32_t* list, int n, int x) {
 
 // Free pages in ascending order against used ones in descending order, as long as the free one lies in front: move i goes from the i-th of these to the
 // i-th of those.  Pages that are neither in the table nor on the stack stay.  The stack's lowest page comes off first.  HERE: one block, the scratch in
-// shared memory (a table of 2240 entries and 1365 pages 13 us, 16 with it in memory); else a cluster's blocks share it in memory.
+// shared memory (a table of 2240 entries and 1365 pages 12 us, 16 with it in memory); else a cluster's blocks share it in memory.
 template <bool HERE>
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const CompactArgs A) {
     extern __shared__ int32_t compact_here[];
@@ -294,34 +294,36 @@ __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_compact_kernel(const C
     meet(blocks);
     // both lists: this block's pages lie behind those of the blocks in front
     const int each = (A.n_pages + (int)blocks - 1) / (int)blocks, begin = min((int)rank * each, A.n_pages), end = min(begin + each, A.n_pages);
-    int n_free = 0, n_used = 0;
-    for (int p0 = begin; p0 < end; p0 += SHARE_THREADS) {
-        const int p = p0 + threadIdx.x, s = p < end ? state[p] : 0;
-        n_free += __syncthreads_count(s == 1);
-        n_used += __syncthreads_count(s & 2);
-    }
-    if (threadIdx.x == 0) { totals[0] = n_free; totals[1] = n_used; }
-    meet(blocks);
     int free_at = 0, used_at = 0, F = 0, U = 0;
-    for (uint32_t b = 0; b < blocks; b++) {
-        uint32_t at;
-        int f, u;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(totals)), "r"(b));
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(f) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.s32 %0, [%1 + 4];" : "=r"(u) : "r"(at) : "memory");
-        if (b < rank) { free_at += f; used_at += u; }
-        F += f; U += u;
+    if (!HERE) {
+        int n_free = 0, n_used = 0;
+        for (int p0 = begin; p0 < end; p0 += SHARE_THREADS) {
+            const int p = p0 + threadIdx.x, s = p < end ? state[p] : 0;
+            n_free += __syncthreads_count(s == 1);
+            n_used += __syncthreads_count(s & 2);
+        }
+        if (threadIdx.x == 0) { totals[0] = n_free; totals[1] = n_used; }
+        meet(blocks);
+        for (uint32_t b = 0; b < blocks; b++) {
+            uint32_t at;
+            int f, u;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(totals)), "r"(b));
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(f) : "r"(at) : "memory");
+            asm volatile("ld.shared::cluster.s32 %0, [%1 + 4];" : "=r"(u) : "r"(at) : "memory");
+            if (b < rank) { free_at += f; used_at += u; }
+            F += f; U += u;
+        }
     }
     for (int p0 = begin; p0 < end; p0 += SHARE_THREADS) {
         const int p = p0 + threadIdx.x, s = p < end ? state[p] : 0;
         int total;
-        const int i = block_sum(s == 1, warps, total);
-        if (s == 1) free_up[free_at + i - 1] = p;
-        free_at += total;
-        const int j = block_sum((s & 2) != 0, warps, total);
-        if (s & 2) used_up[used_at + j - 1] = p;
-        used_at += total;
+        const int both = block_sum((s == 1 ? 1 : 0) + (s & 2 ? 1 << 16 : 0), warps, total);     // up to 1024 each
+        if (s == 1) free_up[free_at + (both & 0xffff) - 1] = p;
+        if (s & 2) used_up[used_at + (both >> 16) - 1] = p;
+        free_at += total & 0xffff;
+        used_at += total >> 16;
     }
+    if (HERE) { F = free_at; U = used_at; }
     meet(blocks);
     if (threadIdx.x == 0) {
         int lo = 0, hi = min(F, U);                            // the first pair that does not move
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(const __grid_c
 }
 
 // Entries of the table beyond which a launch over the device, or a cluster, takes less time than one block.  Latency bounds all of it: every trip to memory waits for
-// the last.  300 forks of rows of up to 486 pages and the release of them: 200 us by a block, 55 by a cluster of eight, 24 over the device (seven launches); 4 forks of rows of 114: 6.0 by
+// the last.  300 forks of rows of up to 486 pages and the release of them: 200 us by a block, 55 by a cluster of eight, 20 over the device (seven launches); 4 forks of rows of 114: 6.0 by
 // a block, 6.3 by a cluster.  Releases by a block with eight entries a lane at a time 45 us, with one 70, with four 52, with sixteen no less.
 constexpr int64_t SHARE_MANY = 8192;
 // blocks over the whole device, of rows by warps

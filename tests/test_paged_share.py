@@ -143,7 +143,7 @@ def check_release(paged, dev, done, table, stack, shared, pages, held=None, page
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,width,pages", [(1, 1, 1), (2, 3, 9), (7, 40, 60), (64, 33, 400), (40, 300, 2000), (1100, 9, 3000), (5, 5000, 9000)])
+@pytest.mark.parametrize("rows,width,pages", [(1, 1, 1), (2, 3, 9), (7, 40, 60), (64, 33, 400), (40, 300, 2000), (1100, 9, 3000), (5, 5000, 9000), (9, 1000, 20000)])
 @pytest.mark.parametrize("what", ["all", "some", "none", "behind"])
 def test_release_of_shared_pages(paged, cuda_device, rows, width, pages, what):
     """rows that share beginnings, entries that are no page, rows that name a page twice"""
