@@ -385,10 +385,10 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     int64_t k;
     double temperature;
     if (x && x->requires_grad() && x->is_leaf() && at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-        // the engine would make that node's stream wait for the recorded one, which ends the recording, and the process with it
+        // the engine would make that node's stream wait for the recorded one, which the default stream cannot: that ends the recording, and the process with it
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*x);
-        TORCH_CHECK(!node || node->stream() == c10::cuda::getCurrentCUDAStream(x->device().index()).unwrap(),
-                    "these logits have a gradient's node from outside the recording: let go of what was computed from them before");
+        TORCH_CHECK(!node || node->stream() != c10::cuda::getDefaultCUDAStream(x->device().index()).unwrap(),
+                    "these logits have a gradient's node of the default stream from outside the recording: let go of what was computed from them before");
     }
     if (!x || x->dim() != 2 || float_code(*x) < 0 || x->_fw_grad(0).defined() || !integer(a[2], &k) || !number(a[3], &temperature) || !(temperature >= 1e-7) || !(temperature <= 1e7))
         Py_RETURN_NONE;

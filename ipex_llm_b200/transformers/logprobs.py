@@ -71,7 +71,7 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
 
     Where the logits want a gradient, ``logprobs``, ``entropy`` and ``top_logprobs`` have one: another launch, which reads the logits again and writes their
     gradient, rounded once to their type.  The logits must not be overwritten before it.  It has no derivative of its own.
-    The temperature lies between 1e-7 and 1e7.  A recording refuses logits that are a leaf with another stream's gradient node alive (something eager that was computed from them):
+    The temperature lies between 1e-7 and 1e7.  A recording refuses logits that are a leaf of which something lives that was computed on the default stream:
     their gradient cannot be recorded."""
     out = paged_kv._native("token_logprobs", logits, tokens, top_k, temperature)
     if out is not None:

@@ -347,6 +347,20 @@ def test_no_recording_beside_a_living_graph(lp, cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, leaf.grad)
+        # what lives of another stream joins the recording
+        want, leaf.grad = leaf.grad, None
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            kept = lp.token_logprobs(leaf, tokens)
+            kept.logprobs.sum().backward()
+        torch.cuda.synchronize()
+        leaf.grad = None
+        recorded = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(recorded):
+            lp.token_logprobs(leaf, tokens).logprobs.sum().backward()
+        recorded.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad, want)
 
 
 @pytest.mark.gpu
