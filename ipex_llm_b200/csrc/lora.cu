@@ -14,7 +14,7 @@
 //
 // Measured, times without the launch's share on the host.  One token of K 4096 and N 4096 at rank 16: 6.5 us, the latency of five dependent trips to memory and
 // the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 12.3 us, the same.
-// 882 rows of 40 requests, K 4096 and N 11008 at rank 64, 69 MB: 40.4 us, 7 + 16 + 22.  11849 rows, N 14336 at rank 32, 628 MB: 140 us, 7 + 36 + 101.
+// 882 rows of 40 requests, K 4096 and N 11008 at rank 64, 69 MB: 40.3 us, 7 + 15 + 22.  11849 rows, N 14336 at rank 32, 628 MB: 140 us, 7 + 36 + 101.
 // The second product's launch there copies `out`, which alone takes 88 us; 57 % of what a SM's shared memory and L1 can move in that time is h, read
 // for 32 columns at a time, and `out` on its way through.
 #include <type_traits>
@@ -170,13 +170,13 @@ struct Lora {
 };
 
 // First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
-// = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K; with more than 32 rows groups
-// of them take 32 rows each, and their warps share K.
+// = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K; with more than 32 rows of A groups
+// of them take 32 rows each in the one launch, and their warps share K.
 // Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
 // of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
 // holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  With an even number a lane reads 16 bytes of B, in the first product's order
 // of two steps' k.  (The first product alone: 4 for up to 4.)
-enum { LORA_BOTH, LORA_FIRST, LORA_WIDE, LORA_SECOND };                                      // WIDE: the first with 64 rows of A at a time
+enum { LORA_BOTH, LORA_FIRST, LORA_WIDE, LORA_SECOND };                                      // WIDE: the first where A has more than 32 rows, 64 of them at a time
 template <bool BF, int STEPS, int DO>
 __global__ void __launch_bounds__(LORA_THREADS, DO == LORA_WIDE ? 1 : 2) lora_kernel(const LoraArgs A) {
     using L = Lora;
@@ -706,7 +706,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1) + Lora::parts(256, 1));
-        cudaFuncSetAttribute(lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(256, 1));
+        cudaFuncSetAttribute(lora_kernel<BF, 4, LORA_FIRST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingFirst + Lora::parts(32, 1));
         cudaFuncSetAttribute(lora_kernel<BF, STEPS ? 4 : 0, LORA_WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::kRingWide + Lora::parts(256, 1));
         cudaFuncSetAttribute(lora_kernel<BF, STEPS, LORA_SECOND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lora::smem(256, 1));
         configured[dev & 63] = true;
@@ -718,24 +718,27 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     const int64_t tiles = many ? lora_pieces(A.T, A.adapters, A.R) : (A.T + TM - 1) / TM;
     int64_t some = 1 + (int64_t)A.R * TM * 2 / A.T;
     if (some > lora_tile_adapters(A.adapters, A.R)) some = lora_tile_adapters(A.adapters, A.R);
+    // splits one after the other share a reading of x, or, where there is room for their clusters, each has its own
+    if (many) some = 1;
+    if (many && tiles * LORA_BLOCKS * A.n_splits <= (A.rank > 32 ? 1ll : 2ll) * sm_count()) { A.together = 1; some = A.n_splits; }
+    // 64 rows of A at a time by a block that has its SM to itself: more work for what it reads, one pass for ranks up to 64.  Rank 128, K 4096, N 896: 12000 tokens 148 us
+    // and 192 by 32 rows at a time, 3000 83 and 108, 600 50 and 54; rank 64, K 11008, N 4096: 175 and 215, 74 and 79, 39 and 39
+    const bool wide = many && A.together * A.rank > 32;
     // blocks of a cluster, which share the inner dimension (and the columns): 8 (one token 7.1 us, by 4, 2 and 1 8.8, 11.8 and
-    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the pieces fill the device: 11849 rows by 2 blocks of a piece 141 us, by
-    // 4 143, by 8 152; 882 rows by 8 41, by 4 44, by 2 52
+    // 17.1; 64 tokens 13.2, and 14.3, 19.2, 28.1), fewer where the pieces fill the device: at 32 rows of A 11849 tokens by 2 blocks of a piece 141 us, by
+    // 4 143, by 8 152.  At 64 as many as the device takes at once (882 tokens of 40 requests by 5 blocks 41 us, by 7 49), two at least (12000 by one 154, 148)
     int blocks = LORA_BLOCKS;
-    while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
+    if (wide) {
+        while (blocks > 2 && tiles * some * blocks > sm_count()) blocks--;
+    } else
+        while (many && blocks > 1 && tiles * blocks >= 4ll * sm_count()) blocks /= 2;
     if (many) {
-        // splits one after the other share a reading of x, or, where there is room for their clusters, each has its own
-        some = 1;
-        if (tiles * blocks * A.n_splits <= 2ll * sm_count()) { A.together = 1; some = A.n_splits; }
         launch_behind(lora_order_kernel, dim3(1), SORT_THREADS, 0, st, on, A, row0, (int)A.T, (int)tiles);
         note_launch();
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * blocks), (unsigned)some);
     cfg.blockDim = dim3(LORA_THREADS);
-    // 64 rows of A at a time by a block that has its SM to itself: more work for what it reads, fewer to read.  Rank 128, K 4096, N 896: 12000 tokens 148 us and 192 by 32
-    // rows at a time, 600 50 and 54; rank 64, K 11008, N 4096: 12000 176 and 215, but 3000 80 and 79, and 882 of 40 requests 45 and 41
-    const bool wide = many && A.together * A.rank > 32 && (A.together * A.rank > 64 || tiles >= sm_count());
     cfg.dynamicSmemBytes = (size_t)(wide ? Lora::kRingWide : many ? Lora::kRingFirst : Lora::smem(A.rank, A.together)) + Lora::parts(A.rank, A.together);
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -744,7 +747,7 @@ template <bool BF, int STEPS> int lora_launch(LoraArgs A, int64_t row0, cudaStre
     cfg.attrs = at;
     cfg.numAttrs = add_overlap(at, 1, on);
     A.shares = 1;
-    cudaLaunchKernelEx(&cfg, wide ? lora_kernel<BF, STEPS ? 4 : 0, LORA_WIDE> : many ? lora_kernel<BF, STEPS ? 4 : 0, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
+    cudaLaunchKernelEx(&cfg, wide ? lora_kernel<BF, STEPS ? 4 : 0, LORA_WIDE> : many ? lora_kernel<BF, 4, LORA_FIRST> : lora_kernel<BF, STEPS, LORA_BOTH>, A);
     note_launch();
     if (many) {
         A.together = lora_together(A.rank, A.n_splits);
