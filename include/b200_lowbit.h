@@ -363,7 +363,7 @@ int lowbit_paged_copy_cuda(const int32_t* d_src, const int32_t* d_dst, int n, vo
  * `splits` is read by the call.  The product with A is kept in 32 bits, only out is rounded.  One launch, or three for more rows or larger products.  x and out
  * do not overlap; K up to 2^20, strides of rows up to 2^29.  workspace:
  * lowbit_lora_workspace_size() bytes (0: none), 16-byte aligned, one per call in flight, not initialised. */
-size_t lowbit_lora_workspace_size(int64_t T, int64_t N, int rank, int n_splits, int adapters, int R);
+size_t lowbit_lora_workspace_size(int64_t T, int K, int64_t N, int rank, int n_splits, int adapters, int R);
 int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b,
                          int64_t b_stride, int rank, const float* d_scales, int adapters, const int32_t* d_ids, const int32_t* d_cu_seqlens, int R,
                          const int* splits, int n_splits, void* d_out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);

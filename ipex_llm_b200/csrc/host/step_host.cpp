@@ -24,7 +24,7 @@ using CompactSizeFn = size_t (*)(int);
 using CompactFn = int (*)(const int32_t*, int64_t, int, int, const int32_t*, int, const int32_t*, const int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, int32_t*, void*,
                           size_t, void*);
 using CopyFn = int (*)(const int32_t*, const int32_t*, int, void* const*, int, int, int64_t, int64_t, void*);
-using LoraSizeFn = size_t (*)(int64_t, int64_t, int, int, int, int);
+using LoraSizeFn = size_t (*)(int64_t, int, int64_t, int, int, int, int);
 using LoraFn = int (*)(const void*, int64_t, int, int64_t, int, const void*, int64_t, const void*, int64_t, int, const float*, int, const int32_t*, const int32_t*, int, const int*, int,
                        void*, int64_t, void*, size_t, void*);
 using LogprobsFn = int (*)(const void*, int, int64_t, int64_t, int64_t, const int64_t*, float, int, float*, float*, int64_t*, float*, float*, void*);
@@ -320,7 +320,7 @@ PyObject* lora_add(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     {
         const WithoutGil released;
         const c10::cuda::CUDAGuard guard(x->device());
-        const size_t need = g_lora_size(T, N, (int)R, (int)S, (int)L, (int)ids->size(0));
+        const size_t need = g_lora_size(T, (int)K, N, (int)R, (int)S, (int)L, (int)ids->size(0));
         at::Tensor scratch;
         if (need) scratch = at::empty({(int64_t)need}, x->options().dtype(at::kByte).requires_grad(false));
         rc = g_lora(x->const_data_ptr(), T > 1 ? x->stride(0) : K, half_code(*x), T, (int)K, wa->const_data_ptr(), L > 1 ? wa->stride(0) : S * R * K, wb->const_data_ptr(),

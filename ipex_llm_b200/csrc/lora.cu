@@ -680,17 +680,21 @@ __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraA
 
 // One launch or three.  One has a cluster for each adapter of a tile: where these are more than the device takes at once three take less time, and where they are few and
 // a cluster's columns many.  K 4096, N 4096, rank 16: 64 tokens of 32 adapters 12 us by one, 17 by three; 256 of 8 9 and 16; 150 of 30 31 and 17; 256 of 64 111 and 25.
-// N 22016: 16 tokens of one adapter 12 and 13, 64 24 and 18; at rank 64 22 and 23, 51 and 36; at rank 128 4 tokens 49 and 41, 64 124 and 74.
+// N 22016: 16 tokens of one adapter 12 and 13, 64 24 and 18; at rank 64 22 and 16, 51 and 27; at rank 128 4 tokens 49 and 27, 64 124 and 53.
+// K 14336, N 4096, 64 tokens at rank 64: 39 and 32, at rank 16 16 and 22.
 constexpr int LORA_BLOCKS = 8;                                 // of a cluster: the most that any device takes
 int64_t lora_tile_adapters(int adapters, int R) { const int64_t most = adapters < R ? adapters : R; return most < TM ? most : TM; }
 // splits that share a reading of x: 128 rows of A at most (their parts and h fill what shared memory two blocks of an SM have), or one split
 int lora_together(int rank, int n_splits) { return n_splits * rank <= 128 ? n_splits : rank >= 128 ? 1 : 128 / rank; }
-bool lora_many(int64_t T, int64_t N, int rank, int n_splits, int adapters, int R) {
-    const bool alone = lora_together(rank, n_splits) * rank > 64;                              // a block fills its SM's shared memory
+bool lora_many(int64_t T, int64_t K, int64_t N, int rank, int n_splits, int adapters, int R) {
+    const int together = lora_together(rank, n_splits);
+    const bool alone = together * rank > 64;                                                   // a block fills its SM's shared memory
     const int64_t blocks = (T + TM - 1) / TM * lora_tile_adapters(adapters, R) * LORA_BLOCKS, places = (alone ? 1ll : 2ll) * sm_count();
     if (blocks > places) return true;
-    // groups of columns a warp, by what one costs: itself, its tokens, its steps.  With half the device busy only large ranks are worth the launches
-    const int64_t each = T / (adapters < R ? adapters : R), work = N / 32 * ((each < TM ? each : TM) + 16 + 4 * Lora::steps(rank)), much = 400ll * LORA_BLOCKS * LORA_WARPS;
+    // groups of columns a warp, by what one costs: itself, its tokens, its steps; and 32 k's of 32 rows of A and 32 tokens by what they cost beside those.  With half the
+    // device busy only large ranks are worth the launches
+    const int64_t tokens = T / (adapters < R ? adapters : R), each = tokens < 1 ? 1 : tokens < TM ? tokens : TM, much = 400ll * LORA_BLOCKS * LORA_WARPS;
+    const int64_t work = N / 32 * (each + 16 + 4 * Lora::steps(rank)) + K / 32 * ((n_splits * rank + 31) / 32) * ((each + 31) / 32) * 8;
     return 2 * blocks <= places ? work >= much : Lora::steps(rank) >= 4 && work >= (alone ? much : much * 3 / 2);
 }
 // pieces that T rows of R requests may have: of whole 64, and one of every adapter
@@ -772,8 +776,8 @@ template <bool BF> int lora_steps(const LoraArgs& A, int64_t row0, cudaStream_t 
 }  // namespace
 }  // namespace lowbit
 
-extern "C" size_t lowbit_lora_workspace_size(int64_t T, int64_t N, int rank, int n_splits, int adapters, int R) {
-    if (T <= 0 || N <= 0 || rank <= 0 || n_splits <= 0 || adapters <= 0 || R <= 0 || !lora_many(T, N, rank, n_splits, adapters, R)) return 0;
+extern "C" size_t lowbit_lora_workspace_size(int64_t T, int K, int64_t N, int rank, int n_splits, int adapters, int R) {
+    if (T <= 0 || K <= 0 || N <= 0 || rank <= 0 || n_splits <= 0 || adapters <= 0 || R <= 0 || !lora_many(T, K, N, rank, n_splits, adapters, R)) return 0;
     return lora_lists_bytes(T, adapters, R) + (size_t)T * n_splits * (Lora::steps(rank) * 64 + sizeof(float));
 }
 
@@ -797,7 +801,7 @@ extern "C" int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype
         return LB_ERR_ARG;
     }
     if (T == 0) return LB_OK;
-    const size_t need = lowbit_lora_workspace_size(T, N, rank, n_splits, adapters, R);
+    const size_t need = lowbit_lora_workspace_size(T, K, N, rank, n_splits, adapters, R);
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) {
         set_error(LB_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of lowbit_lora_workspace_size() bytes is needed", name);
         return LB_ERR_WORKSPACE;

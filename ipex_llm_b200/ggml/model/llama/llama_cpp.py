@@ -819,7 +819,7 @@ def lowbit_paged_copy(src, dst, caches, n_pages, page_stride_bytes, page_bytes, 
 
 
 # ---------------------------------------------------------------- low-rank adapters of many requests
-_lib.lowbit_lora_workspace_size.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+_lib.lowbit_lora_workspace_size.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]
 _lib.lowbit_lora_workspace_size.restype = ctypes.c_size_t
 _lib.lowbit_lora_add_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                       ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
@@ -827,8 +827,8 @@ _lib.lowbit_lora_add_cuda.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_
 _lib.lowbit_lora_add_cuda.restype = ctypes.c_int
 
 
-def lowbit_lora_workspace_size(tokens, columns, rank, n_splits, adapters, requests):
-    return _lib.lowbit_lora_workspace_size(tokens, columns, rank, n_splits, adapters, requests)
+def lowbit_lora_workspace_size(tokens, k, columns, rank, n_splits, adapters, requests):
+    return _lib.lowbit_lora_workspace_size(tokens, k, columns, rank, n_splits, adapters, requests)
 
 
 def lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, workspace, stream):

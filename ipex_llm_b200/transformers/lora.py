@@ -82,7 +82,7 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     a, b = (t if t[0].is_contiguous() and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and (t.shape[0] == 1 or t.stride(0) >= t[0].numel())
             else t.clone(memory_format=torch.contiguous_format) for t in (a, b))
     with torch.cuda.device(dev):
-        ws = torch.empty(ggml.lowbit_lora_workspace_size(T, N, R, S, L, adapter_ids.shape[0]), dtype=torch.uint8, device=dev)
+        ws = torch.empty(ggml.lowbit_lora_workspace_size(T, K, N, R, S, L, adapter_ids.shape[0]), dtype=torch.uint8, device=dev)
         ggml.lowbit_lora_add(x, a, b, scales, adapter_ids, cu_seqlens, splits, out, ws, torch._C._cuda_getCurrentRawStream(dev.index))
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)

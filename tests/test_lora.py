@@ -375,4 +375,4 @@ def test_refusals_on_the_cpu(lora, native_lib):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
-    assert lib.lowbit_lora_workspace_size(64, 64, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(3000, 64, 16, 2, 3, 4) >= 3000 * (32 * 4 + 4)
+    assert lib.lowbit_lora_workspace_size(64, 64, 64, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(3000, 64, 64, 16, 2, 3, 4) >= 3000 * (32 * 4 + 4)
