@@ -59,7 +59,7 @@ struct ForkArgs {
 // be written in place: by the one block that there is, or (`last` false) by a launch behind.
 __global__ void __launch_bounds__(SHARE_THREADS, 1) paged_fork_kernel(const ForkArgs A, bool last) {
     __shared__ int warps[32];
-    __shared__ int fresh[SHARE_THREADS];                       // the page of a fork of this round, -1: none to be had, -2: it needs none
+    __shared__ int fresh[SHARE_THREADS];                       // the page of each of these forks, -1: none to be had, -2: it needs none
     const int rank = blockIdx.x, blocks = gridDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
