@@ -54,6 +54,12 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logprobs, g_entropy, _=None, g_top=None):
         logits, tokens, ids, stats = ctx.saved_tensors
         temperature, top_k = ctx.more
+        # a hook for saved tensors may have brought them back in another layout, or as something else, which the kernel could not see
+        if logits.stride(1) != 1 or logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
+            logits = logits.contiguous()
+        tokens, stats, ids = (t if t is None else t.contiguous() for t in (tokens, stats, ids))
+        invalidInputError(logits.is_cuda and logits.dtype in _TYPES and stats.dtype == torch.float32 and tokens.dtype == torch.int64 and (ids is None or ids.dtype == torch.int64)
+                          and all(t is None or t.device == logits.device for t in (tokens, stats, ids)), "what token_logprobs saved came back as something else")
         given = [None if g is None else g.contiguous() for g in (g_logprobs, g_entropy, g_top)]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with torch.cuda.device(logits.device):

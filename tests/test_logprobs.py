@@ -473,3 +473,31 @@ def test_refusals_on_the_cpu(lp, native_lib):
         args = list(good)
         args[i] = bad
         assert lib.lowbit_token_logprobs_grad_cuda(*args) == 1, (i, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("shape", [(12,), (3, 4)])
+def test_what_was_saved_in_another_layout(lp, cuda_device, monkeypatch, native, shape):
+    """the gradient's node in Python, which serves three dimensions too, looks at what a hook brings back as the native one does"""
+    if not native:
+        monkeypatch.setattr(lp.paged_kv, "_native", lambda *args: None)
+    logits, tokens = make(12, 700, torch.float32, cuda_device)
+    logits, tokens = logits.view(*shape, 700), tokens.view(shape)
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    gs = [torch.randn(*shape, *more, generator=g, device=cuda_device) for more in ((), (), (4,))]
+
+    def grad_of(unpack):
+        leaf = logits.clone().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            got = lp.token_logprobs(leaf, tokens, 4, 0.8)
+            return torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], leaf, gs)[0]
+    want = grad_of(lambda t: t)
+    turned = lambda t: t.t().contiguous().t() if t.dim() == 2 else t                              # noqa: E731
+    apart = lambda t: torch.stack([t, t], -1).flatten(-2)[..., ::2]                               # noqa: E731  every other element of a wider one
+    alone = lambda width: lambda t: turned(t) if t.dim() == 2 and t.shape[1] == width else t      # noqa: E731
+    for unpack in (turned, apart, alone(4), alone(700)):
+        assert torch.equal(grad_of(unpack), want)
+    for unpack in (lambda t: t.int() if t.dtype == torch.int64 else t, lambda t: t.half() if t.shape[-1] == 4 and t.dtype == torch.float32 else t, lambda t: t.cpu()):
+        with pytest.raises(RuntimeError, match="came back as something else"):
+            grad_of(unpack)
