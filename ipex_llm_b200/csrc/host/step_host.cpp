@@ -138,6 +138,10 @@ PyObject* paged_norm_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     if (rc) return PyLong_FromLong(rc);
     written(*x);
+    if (k) {
+        written(*k);
+        written(*v);
+    }
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
@@ -170,6 +174,8 @@ PyObject* paged_fork(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                     out[2].mutable_data_ptr<int32_t>(), shared->mutable_data_ptr<int32_t>(), (int)page, o, o + F, o + 2 * F + 1, stream_of(*par));
     }
     if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor* t : {lens, table, shared, left})
+        if (t) written(*t);
     PyObject* const r = PyTuple_New(4);
     if (!r) return nullptr;
     for (int i = 0; i < 4; i++) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(out[i])));
@@ -198,6 +204,7 @@ PyObject* paged_share_release(PyObject*, PyObject* const* a, Py_ssize_t n_args) 
                        count->mutable_data_ptr<int32_t>(), shared->mutable_data_ptr<int32_t>(), scratch.mutable_data_ptr(), need, stream_of(*done));
     }
     if (rc) return PyLong_FromLong(rc);
+    for (const at::Tensor* t : {table, pages, count, shared}) written(*t);
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
@@ -282,6 +289,7 @@ PyObject* paged_copy(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             if (rc) break;
         }
     }
+    for (Py_ssize_t i = 0; i < n; i++) written(*plain(PyList_GET_ITEM(a[2], i)));
     if (rc) return PyLong_FromLong(rc);
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS

@@ -47,6 +47,13 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _written(*tensors):
+    """autograd hears of what a kernel writes over (a tensor of inference mode keeps no count)"""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _device(*tensors):
     """the one CUDA device that all of them are on"""
     dev = tensors[0].device
@@ -145,6 +152,7 @@ def paged_release(done, block_table, free_pages, free_count, held=None, page_siz
         with torch.cuda.device(dev):
             ws = torch.empty(ggml.lowbit_paged_share_release_workspace_size(shared.shape[0], *block_table.shape), dtype=torch.uint8, device=dev)
             ggml.lowbit_paged_share_release(done, held, page_size, block_table, free_pages, free_count, shared, ws, _stream(dev))
+        _written(block_table, free_pages, free_count, shared)
         return
     with torch.cuda.device(dev):
         if held is None:
@@ -210,6 +218,7 @@ def paged_fork(parents, children, context_lens, block_table, free_pages, free_co
                 got.free_count.copy_(free_count)
             return got
         ggml.lowbit_paged_fork(parents, children, context_lens, block_table, free_pages, free_count, got.free_count, shared, page_size, got.src, got.dst, got.missing, _stream(dev))
+    _written(context_lens, block_table, shared, free_left)
     return got
 
 
@@ -245,6 +254,7 @@ def paged_copy(src, dst, caches):
     with torch.cuda.device(dev):
         for layout, at in groups.items():
             ggml.lowbit_paged_copy(src, dst, at, *layout, _stream(dev))
+    _written(*caches)
 
 
 def paged_compact(block_table, free_pages, free_count, shared=None):
@@ -339,8 +349,7 @@ def paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, q_weight, k_weigh
         return
     with torch.cuda.device(dev):
         ggml.lowbit_paged_norm_rope_append(qkv, n_heads, n_kv_heads, head_dim, rotary, q_weight, k_weight, eps, cos, sin, positions, slots, k_cache, v_cache, _stream(dev))
-    if not qkv.is_inference():
-        torch.autograd.graph.increment_version(qkv)
+    _written(qkv, k_cache, v_cache)
 
 
 def _attention_args(query, n_kv_heads, cu_seqlens, scale, out):

@@ -599,3 +599,50 @@ def test_refusals_on_the_cpu(paged, native_lib):
     refused("lowbit_paged_norm_rope_append_cuda", [some, 1, 512, 6, 4, 2, 64, 64, some, some, 1, 1e-6, some, some, 1, 64, 9, some, some, some, strides, some, strides, 1, 3, 16, None],
             [(a, None) for a in (0, 8, 9, 12, 13, 17, 18, 19, 20, 21, 22)] + [(1, 0), (2, 511), (3, -1), (4, -1), (5, 0), (6, 0), (7, 66), (7, 63), (10, 3), (11, -1.0), (11, math.nan), (14, 3), (15, 31),
                                                                         (16, 0), (23, 2), (24, 0), (25, 0)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_autograd_hears_of_caches_and_lists(paged, cuda_device, monkeypatch, native):
+    """whatever the operators write over: caches, and whole numbers that a graph has kept as indices"""
+    if not native:
+        monkeypatch.setattr(paged, "_native", lambda *args: None)
+    dev = cuda_device
+    i = lambda x: dev_ints(x, dev)                                                                # noqa: E731
+    w, scale, rows = torch.ones(64, device=dev), torch.ones(64, device=dev, dtype=torch.float16, requires_grad=True), torch.ones(12, 2, device=dev, requires_grad=True)
+    slots = torch.arange(3, device=dev)
+    with torch.inference_mode():
+        keeps_no_count = torch.zeros(4, 8, 1, 64, dtype=torch.float16, device=dev)
+
+    def state():
+        return {"qkv": torch.randn(3, 256, device=dev).half(), "k_cache": torch.zeros(4, 8, 1, 64, dtype=torch.float16, device=dev), "v_cache": torch.zeros(4, 8, 1, 64, dtype=torch.float16, device=dev),
+                "lens": i([9, 0, 0]), "table": i([[3, 2], [0, 0], [0, 0]]), "stack": i([0, 1, 0, 0]), "count": i([2]), "shared": i([0, 0, 0, 0])}
+
+    def norms(s):
+        paged.paged_norm_rope_append(s["qkv"], 2, 1, 64, w, w, 1e-6, None, None, None, slots, s["k_cache"], s["v_cache"])
+
+    def fork(s):
+        paged.paged_fork(i([0]), i([1]), s["lens"], s["table"], s["stack"], s["count"], s["shared"], 8, free_left=s["count"])
+
+    def release(s):
+        paged.paged_release(torch.tensor([True, False, False], device=dev), s["table"], s["stack"], s["count"], shared=s["shared"])
+    for call, names in ((norms, ("qkv", "k_cache", "v_cache")), (lambda s: paged.paged_copy(i([0]), i([2]), [s["k_cache"], s["v_cache"]]), ("k_cache", "v_cache")),
+                        (lambda s: paged.paged_copy(i([-1, 3]), i([1, 0]), [s["k_cache"], keeps_no_count, s["v_cache"].view(torch.uint8)]), ("k_cache", "v_cache")),
+                        (fork, ("lens", "table", "count", "shared")), (release, ("table", "stack", "count", "shared"))):
+        for name in names:
+            s = state()
+            kept = s[name]
+            y = torch.nn.functional.embedding(kept, rows) if kept.dtype == torch.int32 else kept.view(-1, 64) * scale
+            call(s)
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                y.sum().backward()
+        s = state()
+        y = sum(t.float().sum() for t in s.values()) * scale.sum()     # what is read alone stays
+        call(s)
+        y.backward()
+    s = state() | {"k_cache": keeps_no_count, "v_cache": keeps_no_count.clone()}
+    norms(s)
+    table = i([[1, 2]])
+    y = torch.nn.functional.embedding(table, rows)
+    paged.paged_compact(table, i([0, 3, 0, 0]), i([2]))                # writes over nothing
+    y.sum().backward()
