@@ -392,9 +392,10 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *x = plain(a[0]), *tokens = plain(a[1]);
     int64_t k;
     double temperature;
-    if (x && x->requires_grad() && x->is_leaf() && at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-        // the engine would make that node's stream wait for the recorded one, which the default stream cannot: that ends the recording, and the process with it
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*x);
+    if (x && x->requires_grad() && at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+        // the engine would make a leaf's node's stream wait for the recorded one, which the default stream cannot: that ends the recording, and the process with it
+        const at::TensorBase& leaf = x->is_view() ? x->_base() : *x;
+        const auto node = leaf.is_leaf() && leaf.requires_grad() ? torch::autograd::impl::try_get_grad_accumulator(leaf) : nullptr;
         TORCH_CHECK(!node || node->stream() != c10::cuda::getDefaultCUDAStream(x->device().index()).unwrap(),
                     "these logits have a gradient's node of the default stream from outside the recording: let go of what was computed from them before");
     }

@@ -77,8 +77,8 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
 
     Where the logits want a gradient, ``logprobs``, ``entropy`` and ``top_logprobs`` have one: another launch, which reads the logits again and writes their
     gradient, rounded once to their type.  The logits must not be overwritten before it.  It has no derivative of its own.
-    The temperature lies between 1e-7 and 1e7.  A recording refuses logits that are a leaf of which something lives that was computed on the default stream:
-    their gradient cannot be recorded."""
+    The temperature lies between 1e-7 and 1e7.  A recording refuses logits that are a leaf, or a view of one, of which something lives that was computed on
+    the default stream: their gradient cannot be recorded.  Without the native host side, which alone can see that, it refuses every leaf that wants a gradient."""
     out = paged_kv._native("token_logprobs", logits, tokens, top_k, temperature)
     if out is not None:
         return TokenLogprobs._make(out)
@@ -89,6 +89,9 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
     top_k, temperature, V = int(top_k), float(temperature), logits.shape[-1]
     invalidInputError(0 <= top_k <= min(TOP_MOST, V), f"top_k must be between 0 and {min(TOP_MOST, V)}")
     invalidInputError(1e-7 <= temperature <= 1e7, "the temperature must be between 1e-7 and 1e7")
+    if not paged_kv.linears._host and torch.is_grad_enabled() and logits.requires_grad and torch.cuda.is_current_stream_capturing():
+        invalidInputError(not (logits._base if logits._is_view() else logits).is_leaf,
+                          "logits that are a leaf with a gradient take no part in a recording without the native host side: what lives of them may end the process")
     shape = tokens.shape
     rows = logits.reshape(-1, V)
     if rows.shape[0] > 1 and (rows.stride(1) != 1 or rows.stride(0) < V) or V > 1 and rows.stride(1) != 1:

@@ -501,3 +501,45 @@ def test_what_was_saved_in_another_layout(lp, cuda_device, monkeypatch, native, 
     for unpack in (lambda t: t.int() if t.dtype == torch.int64 else t, lambda t: t.half() if t.shape[-1] == 4 and t.dtype == torch.float32 else t, lambda t: t.cpu()):
         with pytest.raises(RuntimeError, match="came back as something else"):
             grad_of(unpack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_no_recording_of_a_leaf_s_view_nor_without_the_native_side(lp, cuda_device, monkeypatch, native):
+    """the refusals alone: no backward pass is recorded here beside a graph that lives.  Without the native host side nobody can look at a leaf's node, so that
+    a recording takes no leaf that wants a gradient"""
+    leaf = torch.randn(4, 6, 301, device=cuda_device).requires_grad_()
+    tokens = torch.zeros(4, 6, dtype=torch.int64, device=cuda_device)
+    forms = [(leaf, tokens), (leaf[:, :-1], tokens[:, 1:]), (leaf[0], tokens[0]), (leaf[1, :, :9], tokens[1])]
+    wants = [lp.token_logprobs(x.detach(), t) for x, t in forms]
+    if not native:
+        monkeypatch.setattr(lp.paged_kv.linears, "_host", False)
+    alive = lp.token_logprobs(leaf, tokens)
+    for x, t in forms:
+        with pytest.raises(RuntimeError, match="recording"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                lp.token_logprobs(x, t)
+    alive.logprobs.sum().backward()
+    del alive, x, forms
+    for take, want in zip((lambda x: (x, tokens), lambda x: (x[:, :-1], tokens[:, 1:]), lambda x: (x[0], tokens[0]), lambda x: (x[1, :, :9], tokens[1])), wants):
+        if native:                                                     # nothing lives any more
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = lp.token_logprobs(*take(leaf))
+                grad, = torch.autograd.grad(got.logprobs.sum(), leaf)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got.logprobs, want.logprobs) and bool(torch.isfinite(grad).all())
+            del got, grad
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():                 # no gradient is asked for
+            got = lp.token_logprobs(*take(leaf))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got.logprobs, want.logprobs) and torch.equal(got.entropy, want.entropy)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = lp.token_logprobs(*take(leaf.detach()))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got.logprobs, want.logprobs)
