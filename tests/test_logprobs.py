@@ -543,3 +543,116 @@ def test_no_recording_of_a_leaf_s_view_nor_without_the_native_side(lp, cuda_devi
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got.logprobs, want.logprobs)
+
+
+# ------------------------------------------------------------------ bounds that masked entries do not widen
+def tight(logits, tokens, k, temperature):
+    """what the results may be off by: (log probability of the token, entropy, of the alternatives; of every entry's probability, relative; of the entropy and an entry's log
+    probability together).
+
+    An exponent is taken relative to a reference within 2^4 above its row's largest: one multiply-add or a difference and a product, and a factor with
+    three roundings, so it is off by 2^-21 of its own distance from the largest (and of those 4); entries of probability 0 add nothing to any sum.  A power adds 2^-22; sums add
+    2^-24 for each of the V / 512 additions of a thread and some 40 where threads and blocks meet; a base-2 logarithm below 32 adds 2^-23 of that.  The entropy
+    is the logarithm of the sum less the mean exponent, whose absolute mean is below that of the distances and 4."""
+    q, w, h, token, ids, top = statement(logits, tokens, k, temperature)
+    z = logits.detach().double() / temperature
+    dist = z.amax(-1, keepdim=True) - z
+    U = torch.where(w > 0, dist, 0.0) + 4
+    R = 2.0 ** -22 + 2.0 ** -24 * (z.shape[-1] / 512 + 40)
+    off = 2.0 ** -21 * U
+    mean = (w * U).sum(-1)
+    of_sum = (w * off).sum(-1) + R + 2.0 ** -18
+    of_h = (w * (U * R + off * (1 + U))).sum(-1) + of_sum + 2.0 ** -23 * (mean + 32)
+    here = (tokens >= 0) & (tokens < z.shape[-1])
+    at = tokens.clamp(0, z.shape[-1] - 1)[:, None]
+    own = lambda i: 2.0 ** -21 * (dist.gather(1, i) + 4) + of_sum[:, None] + 2.0 ** -23 * q.gather(1, i).abs()       # noqa: E731  the entry's own distance, masked or not
+    return torch.where(here, own(at)[:, 0], 0.0), of_h, own(ids), off + of_sum[:, None], 2 * (off + of_sum[:, None] + of_h[:, None])
+
+
+def held(got, logits, tokens, k, temperature):
+    """whether results lie within the tight bounds; numbers that 32 bits cannot hold are their infinity"""
+    _, _, h, token, ids, top = statement(logits, tokens, k, temperature)
+    a, b, c, *_ = tight(logits, tokens, k, temperature)
+    near = lambda x, y, t: bool(((x.double() == y.float().double()) | ((x.double() - y).abs() <= t)).all())          # noqa: E731
+    return near(got.logprobs, token, a) and near(got.entropy, h, b) and (not k or torch.equal(got.top_ids, ids) and near(got.top_logprobs, top, c))
+
+
+MASKS = ["front", "behind", "between", "everything", "all but one", "all but the first", "half as low", "in every thread", "a few left"]
+
+
+def masked_rows(V, dtype, dev, low):
+    logits, tokens = make(len(MASKS), V, dtype, dev, seed=3)
+    i = torch.arange(V, device=dev)
+    for row, out in enumerate((i < V // 2, i >= V // 2, i % 3 > 0, i >= 0, i != V // 3, i > 0, i >= 0, i // 8 % 2 == 0, i * 7919 % V >= 9)):
+        logits[row, out] = low
+    logits[6, V // 3] = low / 2
+    tokens[:] = V // 3
+    return logits, tokens
+
+
+def lows(dtype):
+    return [-1e4, torch.finfo(dtype).min] + ([-1e9, -1e12, -1e25, -1e29, -3e30, -1e37] if dtype != torch.float16 else []) + [-math.inf]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [300, 40001, 128256])
+def test_masks_do_not_blur_what_is_left(lp, cuda_device, dtype, V):
+    """as test_masks_of_large_numbers, with the bounds of what the masks leave"""
+    for low in lows(dtype):
+        logits, tokens = masked_rows(V, dtype, cuda_device, low)
+        if low == -math.inf:
+            logits[3], logits[6] = 0.0, 1.0                            # rows of nothing else have no probabilities
+        for k, temperature in ((9, 1.0), (0, 0.7), (20, 3.0), (1, 1e-3), (5, 1e4)):
+            got = lp.token_logprobs(logits, tokens, k, temperature)
+            assert held(got, logits, tokens, k, temperature), (low, k, temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,k,temperature,masked", [(3, 999, 5, 1.0, 0.0), (33, 4099, 20, 0.7, 0.9), (2, 128256, 20, 1.5, 0.3), (800, 2056, 0, 0.3, 0.0), (5, 3001, 6, 1e-7, 0.3), (5, 3001, 6, 1e7, 0.3)])
+def test_values_within_the_bounds_of_what_counts(lp, cuda_device, dtype, rows, V, k, temperature, masked):
+    logits, tokens = make(rows, V, dtype, cuda_device, masked)
+    assert held(lp.token_logprobs(logits, tokens, k, temperature), logits, tokens, k, temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [300, 40001])
+def test_gradients_of_what_masks_leave(lp, cuda_device, dtype, V):
+    for low in lows(dtype):
+        logits, tokens = masked_rows(V, dtype, cuda_device, low)
+        if low == -math.inf:
+            logits[3], logits[6] = 0.0, 1.0
+        g = torch.Generator(device=cuda_device).manual_seed(V)
+        gs = [torch.randn(len(MASKS), *more, generator=g, device=cuda_device) for more in ((), (), (5,))]
+        for temperature in (1.0, 0.7):
+            leaf = logits.clone().requires_grad_()
+            got = lp.token_logprobs(leaf, tokens, 5, temperature)
+            grad, = torch.autograd.grad(list(got[:2]) + [got.top_logprobs], leaf, gs)
+            q, w, h, *_ = statement(logits, tokens, 5, temperature)
+            want, size, single = gradient(logits, tokens, got.top_ids, 5, temperature, gs)
+            *_, of_p, of_both = tight(logits, tokens, 5, temperature)
+            weight = gs[1].double().abs()[:, None] * w / temperature
+            bound = HALF[dtype] * want.abs() + 2 * of_p * size + weight * (of_both + 2.0 ** -22 * 8) + 2.0 ** -22 * (single + size) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126)
+            assert bool(((grad.double() - want).abs() <= bound).all()), (low, temperature)
+
+
+def test_the_bounds_refuse_planted_mistakes(lp):
+    """on the CPU: results of 64 bits are taken, and those with a mistake in what the masks leave are not"""
+    for dtype in TYPES:
+        for low in lows(dtype):
+            logits, tokens = masked_rows(300, dtype, torch.device("cpu"), low)
+            if low == -math.inf:
+                logits[3], logits[6] = 0.0, 1.0
+            _, w, h, token, ids, top = statement(logits, tokens, 5, 1.0)
+            right = lp.TokenLogprobs(token.float(), h.float(), ids, top.float())
+            assert held(right, logits, tokens, 5, 1.0)
+            for row in (0, 1, 2, 7, 8):                                # sums that are lost, counted twice, or off in the fourth digit
+                for name, value in (("logprobs", 0.0), ("logprobs", token[row] - math.log(2)), ("logprobs", token[row] + 1e-3), ("entropy", 0.0), ("entropy", h[row] + 1e-3),
+                                    ("top_logprobs", top[row] - 1e-3), ("top_ids", ids[row].flip(0))):
+                    if name == "logprobs" and token[row] < -1e3:       # this token is ruled out: its own distance
+                        continue
+                    wrong = right._replace(**{name: getattr(right, name).clone()})
+                    getattr(wrong, name)[row] = value
+                    assert not held(wrong, logits, tokens, 5, 1.0), (dtype, low, row, name)
