@@ -376,3 +376,180 @@ def test_refusals_on_the_cpu(lora, native_lib):
         args[i] = bad
         assert lib.lowbit_lora_add_cuda(*args) == 4, (i, bad)
     assert lib.lowbit_lora_workspace_size(64, 64, 64, 16, 2, 3, 4) == 0 and lib.lowbit_lora_workspace_size(3000, 64, 64, 16, 2, 3, 4) >= 3000 * (32 * 4 + 4)
+
+
+# ------------------------------------------------------------------ three launches: which calls take them is a rule of cost, so every test here asks for it
+def launches(lora, s):
+    """1, or 3 where the call needs a workspace"""
+    L, S, R, K = s["a"].shape
+    return 3 if lora.ggml.lowbit_lora_workspace_size(s["x"].shape[0], K, s["out"].shape[1], R, S, L, s["ids"].shape[0]) else 1
+
+
+def many(dtype, dev, K=256, splits=(128, 64), rank=16, pad=3, adapters=12, requests=40, seed=0):
+    """requests of one token and chunks, of more adapters than one launch takes"""
+    lens = [1 if i % 3 else 2 + i % 37 for i in range(requests)]
+    ids = [i * 5 % (adapters + 1) - 1 for i in range(requests)]
+    return make(lens, ids, K, list(splits), rank, adapters, dtype, dev, pad=pad, seed=seed), lens, ids
+
+
+def by_rows(cu, ids, adapters, T):
+    """the adapter of every row: a request has what lies behind all in front of it and before its own end, none behind the list's end"""
+    rows = [-1] * T
+    for r, i in enumerate(ids):
+        for t in range(max(max(cu[:r + 1]), 0), min(cu[r + 1], cu[-1], T)):
+            rows[t] = i if 0 <= i < adapters else -1
+    return rows
+
+
+SPREADS = [(256, (128, 64), 16), (1000, (136, 40, 40), 24), (512, (520,), 64), (96, (128, 128), 128), (64, (72,), 256), (2048, (2040,), 48)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("K,splits,rank", SPREADS)
+def test_three_launches_on_streams_recorded_and_from_threads(lora, cuda_device, dtype, K, splits, rank):
+    import threading
+    s, lens, ids = many(dtype, cuda_device, K, splits, rank)
+    assert launches(lora, s) == 3
+    want = check(lora, s, lens, ids)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.extend(run(lora, s) for _ in range(4))
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 12 and all(torch.equal(g, want) for g in got)
+    # recorded, and repeated for other requests
+    out = s["out"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lora.lora_add_(out, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"], splits=s["splits"])
+    T = s["x"].shape[0]
+    for lens, ids in ((lens, ids), ([0] * 39 + [T], [3] * 40), ([T // 40] * 40, [i % 14 - 1 for i in range(40)]), ([T - 60] + [1] * 39, [0] + list(range(39)))):
+        s["cu"].copy_(torch.tensor([0] + lens, dtype=torch.int32, device=cuda_device).cumsum(0))
+        s["ids"].copy_(torch.tensor(ids, dtype=torch.int32))
+        out.copy_(s["out"])
+        graph.replay()
+        assert torch.equal(out, check(lora, s, lens, ids))
+
+
+@pytest.mark.gpu
+def test_three_launches_of_rows_far_apart(lora, cuda_device):
+    """rows of 2^27 elements: 256 of them at a time, a request on both sides of the border and others behind it"""
+    T, step = 270, 1 << 27
+    if torch.cuda.mem_get_info()[0] < T * step * 2 + (4 << 30):
+        pytest.skip("needs 73 GB")
+    lens, ids = [20] * 12 + [10, 9, 8], [0, 1, 2, 3, -1, 5, 6, 7, 8, 9, 1, 2, 3, 4, 5]
+    s = make(lens, ids, 64, [64], 16, 10, torch.float16, cuda_device, pad=3)
+    assert launches(lora, s) == 3
+    want = run(lora, s)
+    far = torch.empty(T * step, dtype=torch.float16, device=cuda_device).as_strided((T, 64), (step, 1))
+    far.copy_(s["out"])
+    lora.lora_add_(far, s["x"], s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+    value, bound = statement(s, lens, ids)
+    assert bool(((far.double() - value).abs() <= bound).all()) and torch.equal(far[-3:], s["out"][-3:]) and torch.equal(far[80:100], s["out"][80:100])
+    far.copy_(s["x"])
+    got = run(lora, {**s, "x": far})
+    assert bool(((got.double() - value).abs() <= bound).all()) and torch.equal(got[-3:], want[-3:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [40, 1100])
+def test_three_launches_of_a_list_that_goes_back(lora, cuda_device, R):
+    """the running maximum within a block's look at the requests, and from one look to the next"""
+    T, adapters = 400, 9
+    g = torch.Generator().manual_seed(R)
+    cu = [-30] + (torch.arange(R) * T // R + torch.randint(-60, 30, (R,), generator=g)).tolist()
+    ids = torch.randint(-1, adapters + 1, (R,), generator=g).tolist()
+    for end in (T + 5, T - 11):
+        s = make([T], [0], 64, [64], 8, adapters, torch.bfloat16, cuda_device)
+        cu[-1] = end
+        s["cu"], s["ids"] = (torch.tensor(v, dtype=torch.int32, device=cuda_device) for v in (cu, ids))
+        assert launches(lora, s) == 3
+        check(lora, s, [1] * T, by_rows(cu, ids, adapters, T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("up", [2.0 ** 7, 2.0 ** -9])
+def test_three_launches_of_products_beyond_fp16(lora, cuda_device, up):
+    """as above: rows of very different size, and what brings them back through memory"""
+    s, lens, ids = many(torch.float16, cuda_device, splits=(64, 24))
+    s["x"] *= up
+    s["x"][::3] *= 2.0 ** -6
+    s["a"] *= up * 64 if up > 1 else up
+    s["b"] *= 2.0 ** -12 if up > 1 else 2.0 ** 8
+    assert launches(lora, s) == 3 and bool(torch.isfinite(statement(s, lens, ids)[0]).all())
+    check(lora, s, lens, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_three_launches_round_the_result_alone(lora, cuda_device, dtype):
+    s, lens, ids = many(dtype, cuda_device, 512, (256,), 32)
+    assert launches(lora, s) == 3
+    s["out"].zero_()
+    s["out"] = (-statement(s, lens, ids)[0]).to(dtype)
+    check(lora, s, lens, ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_three_launches_keep_what_is_not_finite_in_its_row(lora, cuda_device, dtype):
+    s, lens, ids = many(dtype, cuda_device)
+    ids = [2 if i == 11 else i for i in ids]                           # nobody has the last adapter
+    s["ids"].copy_(torch.tensor(ids, dtype=torch.int32))
+    assert launches(lora, s) == 3
+    clean = run(lora, s)
+    nan = torch.zeros(len(clean), dtype=torch.bool, device=cuda_device)
+    for r in (3, 9, 21):                                               # chunks, and one of their rows alone
+        assert ids[r] >= 0 and lens[r] > 1
+        nan[sum(lens[:r]):sum(lens[:r + 1]) if r != 9 else sum(lens[:r]) + 1] = True
+    s["x"][nan] = math.nan
+    s["x"][sum(lens):] = math.inf
+    s["a"][11], s["b"][11] = math.nan, math.inf
+    got = run(lora, s)
+    assert torch.equal(got[~nan], clean[~nan]) and bool(torch.isnan(got[nan]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_three_launches_of_views_and_shared_memory(lora, cuda_device, monkeypatch, native):
+    """rows of wider tensors, rows off 16 bytes, the output in the input's place; with the native host side and without"""
+    s, lens, ids = many(torch.bfloat16, cuda_device, 256, (256,), 16, pad=0)
+    assert launches(lora, s) == 3
+    want = check(lora, s, lens, ids)
+    if not native:
+        monkeypatch.setattr(lora.paged_kv, "_native", lambda *args: None)
+    assert torch.equal(run(lora, s), want)
+    T = sum(lens)
+    wide_x, wide_out, odd = (torch.full((T, n), 7.0, dtype=torch.bfloat16, device=cuda_device) for n in (304, 288, 259))
+    wide_x[:, 16:272], wide_out[:, 24:280], odd[:, 3:] = s["x"], s["out"], s["x"]
+    lora.lora_add_(wide_out[:, 24:280], wide_x[:, 16:272], s["a"], s["b"], s["scales"], s["ids"], s["cu"])
+    assert torch.equal(wide_out[:, 24:280], want) and bool((wide_out[:, :24] == 7).all()) and bool((wide_out[:, 280:] == 7).all())
+    assert torch.equal(run(lora, {**s, "x": odd[:, 3:]}), want)
+    both = s["x"].clone()                                              # x += adapters of x
+    case = {**s, "out": s["x"]}
+    assert torch.equal(lora.lora_add_(both, both, s["a"], s["b"], s["scales"], s["ids"], s["cu"]), run(lora, case))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("adapters,K,splits,rank", [(1, 520, (264, 8), 64), (3, 520, (264, 8), 136), (8, 520, (264, 8), 8), (8, 4096, (4096,), 16), (8, 96, (64,), 48)])
+def test_both_sides_of_where_the_launches_change(lora, cuda_device, adapters, K, splits, rank):
+    """the last number of rows that takes one launch, and the first that takes three"""
+    for T in range(max(adapters, 2), 5000):
+        args = (K, sum(splits), rank, len(splits), adapters, adapters)
+        if lora.ggml.lowbit_lora_workspace_size(T, *args):
+            break
+    assert lora.ggml.lowbit_lora_workspace_size(T, *args) > 0 == lora.ggml.lowbit_lora_workspace_size(T - 1, *args)
+    for rows, expect in ((T - 1, 1), (T, 3)):
+        lens = [rows // adapters] * (adapters - 1)
+        lens.append(rows - sum(lens))
+        s = make(lens, list(range(adapters)), K, list(splits), rank, adapters, torch.float16, cuda_device)
+        assert launches(lora, s) == expect
+        check(lora, s, lens, list(range(adapters)))
