@@ -463,9 +463,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
         }
         const float log2s = log2f(all.s);
         auto logp = [&](float v) {
-            const float u = fmaf(v - ref, c, -all.m);
-            // the type's lowest value: base e has room for what base 2 has not
-            return u == -INFINITY ? fmaf(v - ref, A.by, -(all.m + log2s) * LP_LN2) : (u - log2s) * LP_LN2;
+            const float d = v - ref, u = fmaf(d, c, -all.m);
+            if (u > -INFINITY || u != u) return (u - log2s) * LP_LN2;
+            // the type's lowest value: base e has room for what base 2 has not, and the quotients by the temperature for what their difference has not
+            return (d > -INFINITY ? d * A.by : fmaf(v, A.by, -(ref * A.by))) - (all.m + log2s) * LP_LN2;
         };
         if (t == 0) {
             A.logp[r] = token >= 0 ? logp(token_logit) : 0.0f;

@@ -656,3 +656,29 @@ def test_the_bounds_refuse_planted_mistakes(lp):
                     wrong = right._replace(**{name: getattr(right, name).clone()})
                     getattr(wrong, name)[row] = value
                     assert not held(wrong, logits, tokens, 5, 1.0), (dtype, low, row, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 2.0, 1e3, 1e7])
+def test_logits_of_the_type_s_whole_range(lp, cuda_device, dtype, temperature):
+    """the difference from the row's largest may pass 32 bits where its quotient by the temperature does not, and the other way round"""
+    big = torch.finfo(dtype).max
+    logits = torch.zeros(6, 3000, dtype=dtype, device=cuda_device)
+    for row, (a, b) in enumerate(((big / 2, -big), (big, -big), (big, big / 4), (0.0, -big), (-big / 4, -big), (1e30, -big))):
+        logits[row, ::2], logits[row, 1::2] = a, b
+        logits[row, 5] = 0.0 if row < 3 else -big / 2
+    for token in (0, 1, 5):
+        tokens = torch.full((6,), token, device=cuda_device)
+        for k in (0, 32):
+            assert held(lp.token_logprobs(logits, tokens, k, temperature), logits, tokens, k, temperature)
+    tokens[::2] = 1
+    leaf = logits.clone().requires_grad_()
+    got = lp.token_logprobs(leaf, tokens, 4, temperature)
+    gs = [torch.ones(6, device=cuda_device), torch.full((6,), 0.5, device=cuda_device), torch.ones(6, 4, device=cuda_device)]
+    grad, = torch.autograd.grad([got.logprobs, got.entropy, got.top_logprobs], leaf, gs)
+    want, size, single = gradient(logits, tokens, got.top_ids, 4, temperature, gs)
+    *_, of_p, of_both = tight(logits, tokens, 4, temperature)
+    w = statement(logits, tokens, 4, temperature)[1]
+    bound = HALF[dtype] * want.abs() + 2 * of_p * size + 0.5 * w / temperature * (of_both + 2.0 ** -19) + 2.0 ** -22 * (single + size) + 2.0 ** -126
+    assert bool(((grad.double() - want).abs() <= bound).all())
