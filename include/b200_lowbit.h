@@ -360,8 +360,8 @@ int lowbit_paged_copy_cuda(const int32_t* d_src, const int32_t* d_dst, int n, vo
  * (rows cu[r] .. cu[r + 1]); an id outside [0, adapters), and rows of nobody: left as they are.  x [T][K], out [T][N] with N the sum of `splits`;
  * A [adapters][n_splits][rank][K], B [adapters][N][rank], each adapter's in one run, strides in elements between adapters; columns of split s take the
  * product with A's part s.  dtype fp16 or bf16; rank a multiple of 8 up to 256, K and the splits multiples of 8; pointers and strides on 16 bytes.
- * `splits` is read by the call.  The product with A is kept in 32 bits, only out is rounded.  One launch, or three for more rows or larger products.  x and out
- * do not overlap; K up to 2^20, strides of rows up to 2^29.  workspace:
+ * `splits` is read by the call.  The product with A is summed in 32 bits and enters that with B as two values of dtype, which leave out 2^-16 (bf16) or 2^-22
+ * (fp16) of it; out is rounded once.  One launch, or three for more rows or larger products.  x and out do not overlap; K up to 2^20, strides of rows up to 2^29.  workspace:
  * lowbit_lora_workspace_size() bytes (0: none), 16-byte aligned, one per call in flight, not initialised. */
 size_t lowbit_lora_workspace_size(int64_t T, int K, int64_t N, int rank, int n_splits, int adapters, int R);
 int lowbit_lora_add_cuda(const void* d_x, int64_t x_stride, int dtype, int64_t T, int K, const void* d_a, int64_t a_stride, const void* d_b,

@@ -9,8 +9,11 @@
 //   every block multiplies its share of the columns, h B^T, and adds that to `out`, rounded once.
 // Few tokens take one launch of that.  Many take one for each product, with h as two 16-bit values in memory between them: it costs little
 // beside `out`, each kernel has the registers that its product wants, and a tile's columns are dealt as finely as fills the device.
-// mma.sync m16n8k16: a tcgen05 tile wants 128 rows of one adapter, which here have some 1 to 64, and x and B would have to pass through shared memory in its layout,
-// the adapters' rows gathered.  What the operator cannot do without is to read x and out, to write out, and the adapters' A and B once.
+// mma.sync m16n8k16: a tcgen05 tile wants 128 rows of one adapter, and x and B would have to pass through shared memory in its layout, the adapters' rows gathered.  In decode
+// steps and mixed ones an adapter has some 1 to 64 rows.  In prompts it has thousands: at rank 32 the second product is little more than the copy of `out`; at rank
+// 128 the first product, whose warps each read operands of their own, bounds the call (12000 tokens of K 4096 and N 896 148 us, 21 for their bytes), and a
+// form for pieces of 128 rows that all warps share is not built.
+// What the operator cannot do without is to read x and out, to write out, and the adapters' A and B once.
 //
 // Measured, times without the launch's share on the host.  One token of K 4096 and N 4096 at rank 16: 6.5 us, the latency of five dependent trips to memory and
 // the cluster's two meetings.  64 tokens of 32 adapters at rank 16, 15.4 MB: 12.3 us, the same.
@@ -172,8 +175,8 @@ struct Lora {
 // First product: A operand 32 rows of the adapter, B operand 8 tokens, both from global memory, 16 bytes a lane: eight neighbours of a row are two steps' k
 // = 2t, 2t + 1, 2t + 8, 2t + 9 of lane t, in the same order on both sides.  The eight warps share K; with more than 32 rows of A groups
 // of them take 32 rows each in the one launch, and their warps share K.
-// Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left, so that only `out` is rounded; fp16's lie a power
-// of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
+// Second: A operand h of 16 tokens as two 16-bit values each, the second with what rounding the first left: 2^-16 of h stays out in bf16, 2^-22 in fp16, beside `out`'s
+// rounding of 2^-8 and 2^-11.  fp16's lie a power of two off, which brings the row's largest to 2^14.  B operand 8 columns; column 2t + e of n-tile j is column 8t + 2j + e of the warp's 32, so that a lane
 // holds 16 bytes of a row of `out`.  STEPS: of 16 in the rank, B in registers; 0: any number, B as it comes.  With an even number a lane reads 16 bytes of B, in the first product's order
 // of two steps' k.  (The first product alone: 4 for up to 4.)
 enum { LORA_BOTH, LORA_FIRST, LORA_WIDE, LORA_SECOND };                                      // WIDE: the first where A has more than 32 rows, 64 of them at a time
@@ -585,7 +588,7 @@ template <bool MOST> __device__ __forceinline__ int scan(int x, int* warps, int&
 }
 // One block: rows counted by adapter, a place for each adapter's, the pieces of 64, the rows written to their places.  In which order the rows of an adapter lie is
 // chance, and nothing depends on it: a row's sums are its own.  Rows [row0, row0 + rows) count from 0; n_pieces: room for pieces.  It waits for barriers and for
-// memory, some 6 us (1024 threads one more); 882 rows of 40 requests and 12 adapters become 20 pieces, of which tiles of neighbours' rows had some 50.
+// memory, some 6 us (1024 threads one more); 882 rows of 40 requests and 12 adapters become 23 pieces, of which tiles of neighbours' rows had some 50.
 __global__ void __launch_bounds__(SORT_THREADS, 1) lora_order_kernel(const LoraArgs A, int64_t row0, int rows, int n_pieces) {
     __shared__ int warps[32];
     __shared__ int here[2][SORT_HERE];

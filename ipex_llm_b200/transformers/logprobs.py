@@ -69,7 +69,9 @@ class _TokenLogprobs(torch.autograd.Function):
 
 def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
     """Log probabilities of ``tokens`` (int64 [...]) under softmax(``logits`` / ``temperature``) with ``logits`` [..., vocabulary] (fp16, bf16 or fp32), the
-    entropy of every row in nats, and its ``top_k`` (at most 32) most likely tokens: one launch, one pass over the logits.
+    entropy of every row in nats, and its ``top_k`` (at most 32) most likely tokens: one launch, one pass over logits [rows, vocabulary].  More dimensions are brought to that
+    first, by a copy where rows do not follow one another (``logits[:, :-1]``), and their gradient's node is one in Python.  ``temperature`` and ``top_k`` are the
+    call's, for all rows: a recorded call keeps them.
 
     A token outside the vocabulary (-100) has log probability 0 and no gradient of it.  Logits of -inf are tokens that cannot come: probability 0, nothing to
     the entropy, and among the alternatives last.  A row that has no probabilities -- a NaN, +inf, or nothing but -inf in it -- gives NaN, and -1 among the

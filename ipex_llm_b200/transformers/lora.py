@@ -40,7 +40,8 @@ def lora_add_(out, x, a, b, scales, adapter_ids, cu_seqlens, splits=None):
     ``splits``: the widths of the projections that ``out`` merges (queries, keys and values: 4096, 1024, 1024), each with an A of its own: ``a`` is then
     [adapters, len(splits), rank, K], and columns of a projection take the product with its A.
 
-    x A^T is kept in 32 bits and enters the second product as two 16-bit values, so that only ``out`` is rounded, once.  One launch, or three for more rows or larger products; nothing
+    x A^T is summed in 32 bits and enters the second product as two 16-bit values, which leave out 2^-16 of it (bf16) or 2^-22 (fp16); ``out`` is rounded once, by
+    2^-8 or 2^-11.  So the former shows only where ``out`` all but cancels what is added.  One launch, or three for more rows or larger products; nothing
     comes back to the host, and the lists are read on the device: a recorded step serves other requests.  An ``x`` that shares memory with ``out`` is copied first.  There is no backward pass: tensors that want a
     gradient or carry a tangent are refused."""
     if splits is not None:
